@@ -360,6 +360,195 @@ salt_status salt_float_fc_layer_trace(const salt_float_fc_desc *layer, const flo
                                       const salt_stream_in *in, const float *in_gain,
                                       float *v_final, const salt_float_trace *trace, void *stream);
 
+/* ---------------------------------------------------------------- sequence operators
+ * No reference counterpart: the dense, trained counterpart of the event-driven affine scan.  A
+ * token mixer for sequences of feature vectors (binned spike counts, tokens) is a root-mean-square
+ * norm, a short causal convolution and a selective state space scan, an affine recurrence
+ * h = a h + b whose a and b depend on the token.  Each runs over whole rows of tokens, for single
+ * tokens on a pool of states, and backward.
+ *
+ * Conventions of this section
+ *   - Activations are (batch, len, dim); channels are contiguous, batch and token strides are
+ *     given in elements, so that slices of one projection need no copy.  They hold SALT_F32,
+ *     SALT_F16 or SALT_BF16 (`type`); all arithmetic, sums and states are 32-bit floats.
+ *   - n_real (batch, may be NULL = len) gives each row's tokens, clamped to [0, len].  Inputs past
+ *     them are never read; outputs past them are written as zero.  A row without tokens returns its
+ *     initial state (zero where none is given).
+ *   - Arrays without a stride here are contiguous.  batch, len or rows may be 0: a call then does
+ *     what is left (weight gradients become zero).
+ *   - Gradients of weights are sums over rows in an order fixed by the sizes: no atomics, the same
+ *     inputs give the same bits.  `workspace` needs the bytes the matching *_workspace_size
+ *     returns (256-byte aligned; may be NULL when that is 0) and no initialisation.
+ *   - Outputs may not overlap inputs unless a comment says so. */
+enum { SALT_F32 = 0, SALT_F16 = 1, SALT_BF16 = 2 };
+
+/* Root-mean-square norm with the residual's addition, over rows of `dim` <= 16384 elements:
+ *   r = x + residual (r = x without one);  residual_out = r;  rstd = 1 / sqrt(mean(r^2) + eps);
+ *   out = r * rstd * weight.
+ * `type` holds x and out, `residual_type` (`type` or SALT_F32) residual and residual_out,
+ * `weight_type` (`type` or SALT_F32) the weight (dim).  r is rounded only where it is stored.
+ * residual_out and rstd (rows) may be NULL; residual_out may be residual itself, out may be x.
+ * With `scale` given, out is 8 bits (e4m3) instead: each group of `group` (32, 64, 128, 256, or
+ * 0 = the whole row) neighbouring elements has scale = max|out| / 448 (1 where the group is zero)
+ * and out = the nearest e4m3 of value / scale; scale is (rows, ceil(dim / group)) float32. */
+typedef struct {
+  int32_t rows, dim;
+  int32_t type, residual_type, weight_type;
+  int32_t group;
+  float eps;
+  int64_t x_stride, residual_stride, out_stride, residual_out_stride;
+  const void *x, *residual, *weight;
+  void *out, *residual_out;
+  float *rstd, *scale;
+} salt_rms_norm_args;
+
+salt_status salt_rms_norm(const salt_rms_norm_args *args, void *stream);
+
+/* Its gradient.  x (`residual_type`) is what was normalised (residual_out), rstd (rows) from the
+ * forward; dresidual (may be NULL) is the gradient that reaches residual_out from elsewhere.
+ *   h = x * rstd;  dx = rstd * (w dy - h * mean(w dy h)) + dresidual;  dweight = sum_rows dy h.
+ * dx (`residual_type`) is the gradient of x and of residual alike, and may be dresidual itself;
+ * dweight (dim) float32, may be NULL. */
+typedef struct {
+  int32_t rows, dim;
+  int32_t type, residual_type, weight_type;
+  int32_t pad;
+  int64_t dy_stride, x_stride, dresidual_stride, dx_stride;
+  const void *dy, *x, *weight;
+  const float *rstd;
+  const void *dresidual;
+  void *dx;
+  float *dweight;
+} salt_rms_norm_backward_args;
+
+salt_status salt_rms_norm_backward_workspace_size(const salt_rms_norm_backward_args *args,
+                                                  size_t *bytes);
+salt_status salt_rms_norm_backward(const salt_rms_norm_backward_args *args, void *workspace,
+                                   size_t workspace_bytes, void *stream);
+
+/* Causal convolution of each channel with `width` (1 to 8) taps:
+ *   p[t] = bias + sum_k weight[k] x[t - width + 1 + k];  out = p, or p * sigmoid(p) with silu.
+ * Tokens before the row come from initial_state (batch, dim, width - 1), oldest first, zero when
+ * NULL; final_state (same shape, may be NULL or initial_state itself) receives the last
+ * width - 1 inputs.  weight (dim, width) and bias (dim, may be NULL) hold `weight_type` (`type` or
+ * SALT_F32); states hold `type`. */
+typedef struct {
+  int32_t batch, len, dim, width;
+  int32_t type, weight_type;
+  int32_t silu, pad;
+  int64_t x_batch_stride, x_stride, out_batch_stride, out_stride;
+  const void *x, *weight, *bias;
+  const int32_t *n_real;
+  const void *initial_state;
+  void *out, *final_state;
+} salt_causal_conv_args;
+
+salt_status salt_causal_conv(const salt_causal_conv_args *args, void *stream);
+
+/* One token for each of `batch` rows: row b uses and shifts state[slots[b]] of a pool
+ * (n_slots, dim, width - 1); slots NULL = row b is slot b.  A slot outside [0, n_slots) is an
+ * empty row: its out is zero and no state changes.  No slot may appear twice. */
+typedef struct {
+  int32_t batch, dim, width, n_slots;
+  int32_t type, weight_type;
+  int32_t silu, pad;
+  int64_t x_stride, out_stride;
+  const void *x, *weight, *bias;
+  const int32_t *slots;
+  void *state, *out;
+} salt_causal_conv_step_args;
+
+salt_status salt_causal_conv_step(const salt_causal_conv_step_args *args, void *stream);
+
+/* Gradient of salt_causal_conv for the gradient dy of out.  dweight (dim, width) and dbias (dim)
+ * are float32; dx and dinitial (batch, dim, width - 1) hold `type`; dinitial and dbias may be
+ * NULL. */
+typedef struct {
+  int32_t batch, len, dim, width;
+  int32_t type, weight_type;
+  int32_t silu, pad;
+  int64_t dy_batch_stride, dy_stride, x_batch_stride, x_stride, dx_batch_stride, dx_stride;
+  const void *dy, *x, *weight, *bias;
+  const int32_t *n_real;
+  const void *initial_state;
+  void *dx, *dinitial;
+  float *dweight, *dbias;
+} salt_causal_conv_backward_args;
+
+salt_status salt_causal_conv_backward_workspace_size(const salt_causal_conv_backward_args *args,
+                                                     size_t *bytes);
+salt_status salt_causal_conv_backward(const salt_causal_conv_backward_args *args, void *workspace,
+                                      size_t workspace_bytes, void *stream);
+
+/* Selective state space scan.  With s[t] = delta[t] + delta_bias, put through
+ * softplus(s) = log(1 + exp(s)) with softplus set:
+ *   h[t] = exp(s[t] A) h[t-1] + s[t] x[t] B[t];  y = sum_n C[t] h[t] + D x[t];
+ *   out = y, or y * z * sigmoid(z) where z is given.
+ * h is (dim, state) per row, `state` 1 to 64; A (dim, state), D (dim, may be NULL) and delta_bias
+ * (dim, may be NULL) are float32; B and C are (batch, len, groups, state) with contiguous
+ * (groups, state), and channel d reads group d / (dim / groups).  initial_state and final_state
+ * (batch, dim, state) float32 may be NULL, or be the same array.
+ * checkpoints (may be NULL) receives what the backward pass restarts from, the state in front of
+ * every SALT_SCAN_CHECKPOINT-th token: (batch, ceil(len / SALT_SCAN_CHECKPOINT), dim, state)
+ * float32. */
+#define SALT_SCAN_CHECKPOINT 16
+typedef struct {
+  int32_t batch, len, dim, state, groups;
+  int32_t type, softplus, pad;
+  int64_t x_batch_stride, x_stride, delta_batch_stride, delta_stride, z_batch_stride, z_stride,
+      B_batch_stride, B_stride, C_batch_stride, C_stride, out_batch_stride, out_stride;
+  const void *x, *delta, *z, *B, *C;
+  const float *A, *D, *delta_bias;
+  const int32_t *n_real;
+  const float *initial_state;
+  void *out;
+  float *final_state, *checkpoints;
+} salt_selective_scan_args;
+
+salt_status salt_selective_scan_workspace_size(const salt_selective_scan_args *args,
+                                               size_t *bytes);
+salt_status salt_selective_scan(const salt_selective_scan_args *args, void *workspace,
+                                size_t workspace_bytes, void *stream);
+
+/* One token for each of `batch` rows on a pool (n_slots, dim, state) of float32 states; slots as
+ * in salt_causal_conv_step. */
+typedef struct {
+  int32_t batch, dim, state, groups, n_slots;
+  int32_t type, softplus, pad;
+  int64_t x_stride, delta_stride, z_stride, B_stride, C_stride, out_stride;
+  const void *x, *delta, *z, *B, *C;
+  const float *A, *D, *delta_bias;
+  const int32_t *slots;
+  float *pool;
+  void *out;
+} salt_selective_scan_step_args;
+
+salt_status salt_selective_scan_step(const salt_selective_scan_step_args *args, void *stream);
+
+/* Gradient of salt_selective_scan for the gradient dy of out and dfinal (batch, dim, state;
+ * may be NULL) of final_state, from the forward's inputs and checkpoints.  dx, ddelta, dz hold
+ * `type` and share one batch and token stride per array; dB and dC are contiguous
+ * (batch, len, groups, state) of `type`; dA, dD, ddelta_bias and dinitial are float32.  dz is
+ * needed exactly where z is; dD, ddelta_bias and dinitial may be NULL. */
+typedef struct {
+  int32_t batch, len, dim, state, groups;
+  int32_t type, softplus, pad;
+  int64_t x_batch_stride, x_stride, delta_batch_stride, delta_stride, z_batch_stride, z_stride,
+      B_batch_stride, B_stride, C_batch_stride, C_stride, dy_batch_stride, dy_stride,
+      dx_batch_stride, dx_stride, ddelta_batch_stride, ddelta_stride, dz_batch_stride, dz_stride;
+  const void *x, *delta, *z, *B, *C, *dy;
+  const float *A, *D, *delta_bias;
+  const int32_t *n_real;
+  const float *checkpoints, *dfinal;
+  void *dx, *ddelta, *dz, *dB, *dC;
+  float *dA, *dD, *ddelta_bias, *dinitial;
+} salt_selective_scan_backward_args;
+
+salt_status salt_selective_scan_backward_workspace_size(
+    const salt_selective_scan_backward_args *args, size_t *bytes);
+salt_status salt_selective_scan_backward(const salt_selective_scan_backward_args *args,
+                                         void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---------------------------------------------------------------- stream transfer
  * No reference counterpart (the reference's input lives in XLA buffers): copies a batch of event
  * streams from PINNED host memory to the device, moving each sample's row only up to

@@ -18,6 +18,11 @@ from .io import (QuantizedModel, load_quantized, load_weights, network_from_dict
 from .quant_run import (REFERENCE_FIELDS, QuantSplitOutput, check_quantized, quant_forward_split,
                         reference_arrays, run_until_fits)
 
+# the sequence operators (sequence.py)
+_SEQUENCE = ("rms_norm", "rms_norm_q8", "rms_norm_backward", "causal_conv", "causal_conv_step",
+             "causal_conv_backward", "selective_scan", "selective_scan_step",
+             "selective_scan_backward")
+
 
 def __getattr__(name):  # the CUDA-backed objects load the library lazily
     if name in ("QuantB200Backend", "QuantLayerResult", "NetworkOutput", "default_backend"):
@@ -29,6 +34,9 @@ def __getattr__(name):  # the CUDA-backed objects load the library lazily
     if name == "NetworkPlan":
         from .plan import NetworkPlan
         return NetworkPlan
+    if name in _SEQUENCE:
+        from . import sequence
+        return getattr(sequence, name)
     raise AttributeError(name)
 
 
@@ -40,4 +48,5 @@ __all__ = ["REFERENCE_FIELDS", "QuantSplitOutput", "QuantizedModel", "check_quan
            "Network", "NetworkPlan", "OverflowMode", "PAD_TIME", "QuantB200Backend",
            "QuantizedLayerParams", "RoundMode", "build_decay_table_int", "check_layer_connections",
            "conv", "delta_t_max", "fc", "grown_to_fit", "input_stream", "quantize_to_int",
-           "reduce_over_batch", "round_half_away_from_zero", "run_network", "v_th_to_int"]
+           "reduce_over_batch", "round_half_away_from_zero", "run_network", "v_th_to_int",
+           *_SEQUENCE]

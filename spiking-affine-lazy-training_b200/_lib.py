@@ -79,6 +79,69 @@ class LayerSpec(ctypes.Structure):
                 ("q_host", _vp), ("lut_host", _vp), ("vth_host", _vp)]
 
 
+def _fields(ints: str, longs: str, pointers: str, before: tuple = ()):
+    """int32 fields, fields given as they are, int64 fields, pointers: the order of every argument
+    struct of the sequence operators."""
+    return ([(n, _i32) for n in ints.split()] + list(before)
+            + [(n, ctypes.c_int64) for n in longs.split()] + [(n, _vp) for n in pointers.split()])
+
+
+class RmsNormArgs(ctypes.Structure):
+    _fields_ = _fields("rows dim type residual_type weight_type group",
+                       "x_stride residual_stride out_stride residual_out_stride",
+                       "x residual weight out residual_out rstd scale",
+                       (("eps", ctypes.c_float),))
+
+
+class RmsNormBackwardArgs(ctypes.Structure):
+    _fields_ = _fields("rows dim type residual_type weight_type pad",
+                       "dy_stride x_stride dresidual_stride dx_stride",
+                       "dy x weight rstd dresidual dx dweight")
+
+
+class CausalConvArgs(ctypes.Structure):
+    _fields_ = _fields("batch len dim width type weight_type silu pad",
+                       "x_batch_stride x_stride out_batch_stride out_stride",
+                       "x weight bias n_real initial_state out final_state")
+
+
+class CausalConvStepArgs(ctypes.Structure):
+    _fields_ = _fields("batch dim width n_slots type weight_type silu pad",
+                       "x_stride out_stride", "x weight bias slots state out")
+
+
+class CausalConvBackwardArgs(ctypes.Structure):
+    _fields_ = _fields("batch len dim width type weight_type silu pad",
+                       "dy_batch_stride dy_stride x_batch_stride x_stride dx_batch_stride "
+                       "dx_stride",
+                       "dy x weight bias n_real initial_state dx dinitial dweight dbias")
+
+
+class SelectiveScanArgs(ctypes.Structure):
+    _fields_ = _fields("batch len dim state groups type softplus pad",
+                       "x_batch_stride x_stride delta_batch_stride delta_stride z_batch_stride "
+                       "z_stride B_batch_stride B_stride C_batch_stride C_stride out_batch_stride "
+                       "out_stride",
+                       "x delta z B C A D delta_bias n_real initial_state out final_state "
+                       "checkpoints")
+
+
+class SelectiveScanStepArgs(ctypes.Structure):
+    _fields_ = _fields("batch dim state groups n_slots type softplus pad",
+                       "x_stride delta_stride z_stride B_stride C_stride out_stride",
+                       "x delta z B C A D delta_bias slots pool out")
+
+
+class SelectiveScanBackwardArgs(ctypes.Structure):
+    _fields_ = _fields("batch len dim state groups type softplus pad",
+                       "x_batch_stride x_stride delta_batch_stride delta_stride z_batch_stride "
+                       "z_stride B_batch_stride B_stride C_batch_stride C_stride dy_batch_stride "
+                       "dy_stride dx_batch_stride dx_stride ddelta_batch_stride ddelta_stride "
+                       "dz_batch_stride dz_stride",
+                       "x delta z B C dy A D delta_bias n_real checkpoints dfinal dx ddelta dz dB "
+                       "dC dA dD ddelta_bias dinitial")
+
+
 # every function of include/salt_b200.h: name -> (restype, argtypes)
 _SIGS = {
     "salt_conv_layer_workspace_size": (_i32, [_vp, _vp, _i32, _i32, _vp]),
@@ -116,6 +179,18 @@ _SIGS = {
     "salt_float_fc_profile_read": (_i32, [_vp, _vp, _vp, _i32]),
     "salt_float_fc_layer_forward": (_i32, [_vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp,
                                            ctypes.c_size_t, _vp]),
+    "salt_rms_norm": (_i32, [_vp, _vp]),
+    "salt_rms_norm_backward_workspace_size": (_i32, [_vp, _vp]),
+    "salt_rms_norm_backward": (_i32, [_vp, _vp, ctypes.c_size_t, _vp]),
+    "salt_causal_conv": (_i32, [_vp, _vp]),
+    "salt_causal_conv_step": (_i32, [_vp, _vp]),
+    "salt_causal_conv_backward_workspace_size": (_i32, [_vp, _vp]),
+    "salt_causal_conv_backward": (_i32, [_vp, _vp, ctypes.c_size_t, _vp]),
+    "salt_selective_scan_workspace_size": (_i32, [_vp, _vp]),
+    "salt_selective_scan": (_i32, [_vp, _vp, ctypes.c_size_t, _vp]),
+    "salt_selective_scan_step": (_i32, [_vp, _vp]),
+    "salt_selective_scan_backward_workspace_size": (_i32, [_vp, _vp]),
+    "salt_selective_scan_backward": (_i32, [_vp, _vp, ctypes.c_size_t, _vp]),
     "salt_malloc": (_i32, [ctypes.c_size_t, _vp, _vp]),
     "salt_free": (_i32, [_vp, _vp]),
     "salt_host_alloc": (_i32, [ctypes.c_size_t, _vp]),

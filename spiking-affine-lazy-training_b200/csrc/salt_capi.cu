@@ -7,6 +7,7 @@
 #include <string>
 #include <vector>
 
+#include "salt_host.h"
 #include "salt_layers.cuh"
 
 namespace salt {
@@ -19,6 +20,9 @@ static salt_status fail(salt_status s, const std::string& msg) {
   g_err = msg;
   return s;
 }
+
+salt_status host_fail(salt_status s, const std::string& msg) { return fail(s, msg); }
+void host_launched(int n) { g_launches += n; }
 
 #define SALT_CUDA(call)                                                                \
   do {                                                                                 \

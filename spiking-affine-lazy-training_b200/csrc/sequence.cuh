@@ -1,0 +1,165 @@
+// Shared device helpers and launch declarations of the sequence operators (root-mean-square norm,
+// short causal convolution, selective state space scan).
+#pragma once
+#include <cstddef>
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "../../include/salt_b200.h"
+
+namespace salt {
+
+constexpr int kVec = 8;  // elements a thread moves at once: 16 bytes of a 16-bit type
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+
+// N neighbouring elements as they lie in memory; loads and stores are 16 (or 8, 4) bytes wide.
+template <typename T, int N>
+struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Pack {
+  T v[N];
+};
+
+// p[0 .. n) of N elements, zero behind; n outside [0, N] is clipped.  Without `vec` (the pointer
+// may be unaligned) or with n < N every element is loaded by itself.
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> load_pack(const T* p, int n, bool vec) {
+  Pack<T, N> r;
+  if (vec && n >= N) {
+    r = *reinterpret_cast<const Pack<T, N>*>(p);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) r.v[i] = i < n ? p[i] : from_f32<T>(0.f);
+  }
+  return r;
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_pack(T* p, const float* f, int n, bool vec) {
+  Pack<T, N> r;
+#pragma unroll
+  for (int i = 0; i < N; ++i) r.v[i] = from_f32<T>(f[i]);
+  if (vec && n >= N) {
+    *reinterpret_cast<Pack<T, N>*>(p) = r;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < n) p[i] = r.v[i];
+  }
+}
+
+// A weight that holds T or float32.
+template <typename T>
+__device__ __forceinline__ float weight_at(const void* w, int64_t i, bool is_f32) {
+  return is_f32 ? static_cast<const float*>(w)[i] : to_f32(static_cast<const T*>(w)[i]);
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// 2^x to about 2 ulp in one instruction; results below the normal range become 0.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float exp_fast(float x) { return exp2_fast(x * kLog2e); }
+
+// 1 / (1 + e^-x).  e^-x overflows to infinity for x < -88; the quotient is then 0.
+__device__ __forceinline__ float sigmoid(float x) {
+  return __fdividef(1.f, 1.f + exp_fast(-x));
+}
+
+// log(1 + e^x) = max(x, 0) + log1p(u) with u = e^-|x| in (0, 1].  log1p keeps its relative
+// precision at small u (a step of 1e-3 is an ordinary value, and 1 + u would drop 4 of its
+// digits) through log1p(u) = 2 atanh(q), q = u / (2 + u) <= 1/3, and the series of atanh:
+// q^17 / 17 is the first term left out, under 1e-9 of q.
+__device__ __forceinline__ float softplus_f(float x) {
+  const float u = exp_fast(-fabsf(x));
+  const float q = __fdividef(u, 2.f + u), s = q * q;
+  float p = 2.f / 15.f;
+  p = fmaf(p, s, 2.f / 13.f);
+  p = fmaf(p, s, 2.f / 11.f);
+  p = fmaf(p, s, 2.f / 9.f);
+  p = fmaf(p, s, 2.f / 7.f);
+  p = fmaf(p, s, 2.f / 5.f);
+  p = fmaf(p, s, 2.f / 3.f);
+  p = fmaf(p, s, 2.f);
+  // fmaxf drops a NaN; u keeps it
+  return fmaf(p, q, fmaxf(x, 0.f));
+}
+
+// d/dx of x * sigmoid(x).
+__device__ __forceinline__ float silu_slope(float x, float p) { return p * fmaf(x, 1.f - p, 1.f); }
+
+__device__ __forceinline__ int32_t row_tokens(const int32_t* n_real, int b, int32_t len) {
+  if (!n_real) return len;
+  const int32_t n = n_real[b];
+  return n < 0 ? 0 : (n < len ? n : len);
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Launches (argument checks are the caller's; each returns the launch's status).
+cudaError_t rms_norm_launch(const salt_rms_norm_args& a, cudaStream_t st, int* launches);
+size_t rms_norm_backward_bytes(const salt_rms_norm_backward_args& a);
+cudaError_t rms_norm_backward_launch(const salt_rms_norm_backward_args& a, void* ws,
+                                     cudaStream_t st, int* launches);
+cudaError_t causal_conv_launch(const salt_causal_conv_args& a, cudaStream_t st, int* launches);
+cudaError_t causal_conv_step_launch(const salt_causal_conv_step_args& a, cudaStream_t st,
+                                    int* launches);
+size_t causal_conv_backward_bytes(const salt_causal_conv_backward_args& a);
+cudaError_t causal_conv_backward_launch(const salt_causal_conv_backward_args& a, void* ws,
+                                        cudaStream_t st, int* launches);
+size_t selective_scan_bytes(const salt_selective_scan_args& a);
+cudaError_t selective_scan_launch(const salt_selective_scan_args& a, void* ws, cudaStream_t st,
+                                  int* launches);
+cudaError_t selective_scan_step_launch(const salt_selective_scan_step_args& a, cudaStream_t st,
+                                       int* launches);
+size_t selective_scan_backward_bytes(const salt_selective_scan_backward_args& a);
+cudaError_t selective_scan_backward_launch(const salt_selective_scan_backward_args& a, void* ws,
+                                           cudaStream_t st, int* launches);
+
+// Sums `parts` partial arrays of n float32 in order (part p at in + p * n): the second stage of
+// every weight gradient.
+cudaError_t sum_parts_launch(const float* in, int64_t parts, int64_t n, float* out,
+                             cudaStream_t st);
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// Whether rows at p with these strides (in elements) start on 16-byte boundaries.
+inline bool vec_rows(const void* p, size_t size, int64_t s0, int64_t s1 = 0) {
+  return !p || (aligned16(p) && (s0 * size) % 16 == 0 && (s1 * size) % 16 == 0);
+}
+inline size_t type_size(int32_t type) { return type == SALT_F32 ? 4 : 2; }
+
+// Calls F<T>(...) for the C type that `type` names.
+#define SALT_WITH_TYPE(type, T, ...)          \
+  do {                                        \
+    if ((type) == SALT_F32) {                 \
+      using T = float;                        \
+      __VA_ARGS__;                            \
+    } else if ((type) == SALT_F16) {          \
+      using T = __half;                       \
+      __VA_ARGS__;                            \
+    } else {                                  \
+      using T = __nv_bfloat16;                \
+      __VA_ARGS__;                            \
+    }                                         \
+  } while (0)
+
+}  // namespace salt

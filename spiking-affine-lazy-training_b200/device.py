@@ -25,6 +25,35 @@ from .stream import PAD_TIME, EventStream
 
 _tls = threading.local()
 
+# Types without a numpy counterpart, as one-field records of their bits: arrays of them move and
+# index like any other; the functions below convert their values.
+bfloat16 = np.dtype([("bfloat16", "<u2")])
+float8_e4m3 = np.dtype([("float8_e4m3", "u1")])
+
+
+def to_bfloat16(a) -> np.ndarray:
+    """float values as a `bfloat16` host array (to the nearest, ties to even; NaN stays NaN)."""
+    f = np.ascontiguousarray(a, dtype=np.float32)
+    bits = f.view(np.uint32).astype(np.uint64)
+    top = ((bits + 0x7FFF + ((bits >> 16) & 1)) >> 16).astype(np.uint16)
+    return np.where(np.isnan(f), np.uint16(0x7FC0), top).astype(np.uint16).view(bfloat16)
+
+
+def from_bfloat16(a) -> np.ndarray:
+    """A `bfloat16` host array's values as float32."""
+    bits = np.ascontiguousarray(a).view(np.uint16)
+    return (bits.astype(np.uint32) << 16).view(np.float32)
+
+
+def from_float8_e4m3(a) -> np.ndarray:
+    """A `float8_e4m3` host array's values as float32 (4 exponent bits, 3 of mantissa, no
+    infinities; 0x7f and 0xff are NaN)."""
+    bits = np.ascontiguousarray(a).view(np.uint8).astype(np.int32)
+    e, m = (bits >> 3) & 15, bits & 7
+    v = np.where(e == 0, np.ldexp(m / 8.0, -6), np.ldexp(1 + m / 8.0, e - 7))
+    v = np.where((e == 15) & (m == 7), np.nan, v)
+    return np.where(bits & 128, -v, v).astype(np.float32)
+
 
 def _vp(x) -> ctypes.c_void_p:
     return ctypes.c_void_p(x)
@@ -82,6 +111,11 @@ class Stream:
     @staticmethod
     def default() -> "Stream":
         return Stream(0, _owned=False)
+
+    @staticmethod
+    def external(handle: int) -> "Stream":
+        """A stream that another library owns, by its cudaStream_t."""
+        return Stream(int(handle), _owned=False)
 
     @property
     def ptr(self) -> ctypes.c_void_p:
@@ -254,6 +288,14 @@ class DeviceArray:
 
     def data_ptr(self) -> int:
         return self.ptr
+
+    def stride(self) -> tuple:
+        """Strides in elements (always those of a contiguous array)."""
+        out, at = [], 1
+        for n in reversed(self.shape):
+            out.append(at)
+            at *= n
+        return tuple(reversed(out))
 
     def __len__(self) -> int:
         return self.shape[0]

@@ -1,0 +1,491 @@
+"""Sequence operators: root-mean-square norm, short causal convolution, selective state space scan.
+
+The dense, trained counterpart of the float layers' affine scan, for sequences of feature vectors
+(binned spike counts, tokens): ``h = exp(s A) h + s x B`` with a step ``s``, an input map ``B`` and
+a readout ``C`` that depend on the token.  Each operator runs over whole rows, for single tokens on
+a pool of states, and backward, as one call of the C ABI (include/salt_b200.h, "sequence operators")
+on the current stream; no CPU fallback.  No reference counterpart.
+
+Arrays are `DeviceArray`s or any object of another library with ``data_ptr()``, ``shape``,
+``dtype`` and ``stride()`` (in elements) that lives on the current device.  Activations are float32,
+float16 or bfloat16 (`device.bfloat16`), (batch, len, dim) with contiguous channels and any token
+and batch strides; weights of the norm and the convolution hold that type or float32; the scan's
+``A``, ``D``, ``delta_bias`` and its states are float32.  Every output is written into the array
+given for it, or into a new `DeviceArray` where none is; an optional output takes ``None`` (not
+wanted), ``True`` (make one) or an array.
+
+Streams: a call enqueues on `device.current_stream()` and orders nothing else.  Arrays that another
+stream writes have to be waited for (`Stream.wait_event`, `Stream.external`), and must stay
+allocated until the call's work is done.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple
+
+import numpy as np
+
+from . import _lib
+from .device import (DeviceArray, bfloat16, current_device, empty, float8_e4m3, stream_handle,
+                     workspace)
+
+CHECKPOINT = 16       # tokens between the scan's checkpoints (SALT_SCAN_CHECKPOINT)
+GROUPS_8BIT = (0, 32, 64, 128, 256)
+_F32, _F16, _BF16, _I32, _E4M3 = range(5)
+_NUMPY = {_F32: np.dtype(np.float32), _F16: np.dtype(np.float16), _BF16: bfloat16,
+          _I32: np.dtype(np.int32), _E4M3: float8_e4m3}
+_NAMES = ("float32", "float16", "bfloat16", "int32", "float8_e4m3")
+_TYPE_IDS = {v: k for k, v in _NUMPY.items()}
+_ACTIVATIONS = (_F32, _F16, _BF16)
+_INT = ctypes.c_size_t
+
+
+class NormOutput(NamedTuple):
+    out: object
+    residual: object = None
+    rstd: object = None
+    scale: object = None
+
+
+class NormGradients(NamedTuple):
+    dx: object
+    dweight: object = None
+
+
+class ConvOutput(NamedTuple):
+    out: object
+    final_state: object = None
+
+
+class ConvGradients(NamedTuple):
+    dx: object
+    dweight: object
+    dbias: object = None
+    dinitial: object = None
+
+
+class ScanOutput(NamedTuple):
+    out: object
+    final_state: object = None
+    checkpoints: object = None
+
+
+class ScanGradients(NamedTuple):
+    dx: object
+    ddelta: object
+    dA: object
+    dB: object
+    dC: object
+    dD: object = None
+    dz: object = None
+    ddelta_bias: object = None
+    dinitial: object = None
+
+
+# ---------------------------------------------------------------- arguments
+
+def _type_of(a, name: str) -> int:
+    t = a.dtype
+    got = _TYPE_IDS.get(t)
+    if got is None:
+        text = str(t).rsplit(".", 1)[-1].replace("float8_e4m3fn", "float8_e4m3")
+        if text not in _NAMES:
+            raise TypeError(f"{name}: unsupported type {t}")
+        got = _TYPE_IDS[t] = _NAMES.index(text)
+    return got
+
+
+class _Call:
+    """One call's arrays: every pointer that is taken has been checked for shape, type, layout and
+    device."""
+    __slots__ = ("device",)
+
+    def __init__(self):
+        self.device = None
+
+    def type(self, a, name: str) -> int:
+        if not hasattr(a, "data_ptr"):
+            raise TypeError(f"{name}: needs a device array, got {type(a).__name__}")
+        t = _type_of(a, name)
+        if t not in _ACTIVATIONS:
+            raise TypeError(f"{name}: activations are float32, float16 or bfloat16")
+        return t
+
+    def _pointer(self, a, name: str) -> int:
+        where = getattr(a, "get_device", None)
+        if where is not None:
+            d = where()
+            if d != self.device:
+                if self.device is None:
+                    self.device = current_device()
+                if d != self.device:
+                    raise ValueError(f"{name}: not on the current device ({self.device})")
+        return a.data_ptr()
+
+    def _check(self, a, name: str, shape: tuple, type_id: int) -> None:
+        if not hasattr(a, "data_ptr"):
+            raise TypeError(f"{name}: needs a device array, got {type(a).__name__}")
+        if a.shape != shape:
+            raise ValueError(f"{name}: shape {tuple(a.shape)}, expected {shape}")
+        if _type_of(a, name) != type_id:
+            raise TypeError(f"{name}: {_NAMES[_type_of(a, name)]}, expected {_NAMES[type_id]}")
+
+    def whole(self, a, name: str, shape: tuple, type_id: int):
+        """Pointer of a contiguous array, None for None."""
+        if a is None:
+            return None
+        self._check(a, name, shape, type_id)
+        if not isinstance(a, DeviceArray):
+            at = 1
+            for n, s in zip(reversed(shape), reversed(a.stride())):
+                if n != 1 and s != at and 0 not in shape:
+                    raise ValueError(f"{name}: must be contiguous")
+                at *= n
+        return self._pointer(a, name)
+
+    def weight(self, a, name: str, shape: tuple, type_id: int):
+        """(pointer, type) of a contiguous weight of type_id or float32."""
+        if a is None:
+            return None, type_id
+        got = _type_of(a, name) if hasattr(a, "data_ptr") else type_id
+        return self.whole(a, name, shape, _F32 if got == _F32 else type_id), got
+
+    def rows(self, a, name: str, shape: tuple, type_id: int, inner: int = 1):
+        """(pointer, strides of the leading axes) of an array whose last `inner` axes are
+        contiguous; (None, zeros) for None."""
+        lead = len(shape) - inner
+        if a is None:
+            return None, (0,) * lead
+        self._check(a, name, shape, type_id)
+        strides = a.stride()
+        at = 1
+        for n, s in zip(reversed(shape[lead:]), reversed(strides[lead:])):
+            if n != 1 and s != at:
+                raise ValueError(f"{name}: its last {inner} axes must be contiguous"
+                                 if inner > 1 else f"{name}: channels must be contiguous")
+            at *= n
+        return self._pointer(a, name), strides[:lead]
+
+    def flat(self, a, name: str, shape: tuple, type_id: int):
+        """(pointer, row stride) of an array whose leading axes fold into one axis of rows."""
+        if a is None:
+            return None, 0
+        p, strides = self.rows(a, name, shape, type_id)
+        stride, span = shape[-1], None
+        for n, s in zip(reversed(shape[:-1]), reversed(strides)):
+            if n == 1:
+                continue
+            if span is None:
+                stride = s
+            elif s != span and 0 not in shape:
+                raise ValueError(f"{name}: its leading axes do not fold into rows of one stride")
+            span = s * n
+        return p, stride
+
+
+def _wanted(a, shape, type_id):
+    """The array for an optional output: None, a new one for True, or what was given."""
+    if a is None or a is False:
+        return None
+    return empty(shape, _NUMPY[type_id]) if a is True else a
+
+
+def _made(a, shape, type_id):
+    return empty(shape, _NUMPY[type_id]) if a is None else a
+
+
+def _axes(a, name: str, n: int) -> tuple:
+    shape = tuple(getattr(a, "shape", ()))
+    if len(shape) != n:
+        raise ValueError(f"{name}: needs {n} axes, got shape {shape}")
+    return shape
+
+
+def _work(query, args):
+    """(buffer, bytes) that the matching *_workspace_size asks for."""
+    n = _INT(0)
+    _lib.check(query(ctypes.byref(args), ctypes.byref(n)))
+    if n.value == 0:
+        return None, 0
+    return workspace(n.value), n.value
+
+
+# ---------------------------------------------------------------- root-mean-square norm
+
+def _norm(x, weight, residual, eps, out, residual_out, rstd, scale, group):
+    c = _Call()
+    t = c.type(x, "x")
+    shape = tuple(x.shape)
+    if not shape:
+        raise ValueError("x: needs at least one axis")
+    rows, dim = int(np.prod(shape[:-1], dtype=np.int64)), shape[-1]
+    wide = t if residual is None else _type_of(residual, "residual")
+    if residual is None and residual_out is not None and residual_out is not True \
+            and residual_out is not False:
+        wide = _type_of(residual_out, "residual_out")
+    if wide not in (t, _F32):
+        raise TypeError("residual: must hold x's type or float32")
+    out = _made(out, shape, _E4M3 if group is not None else t)
+    residual_out = _wanted(residual_out, shape, wide)
+    rstd = _wanted(rstd, shape[:-1], _F32)
+    ps = None
+    if group is not None:
+        parts = (-(-dim // group) if group else 1,)
+        scale = _made(scale, shape[:-1] + parts, _F32)
+        ps = c.whole(scale, "scale", shape[:-1] + parts, _F32)
+    pw, wt = c.weight(weight, "weight", (dim,), t)
+    px, sx = c.flat(x, "x", shape, t)
+    pr, sr = c.flat(residual, "residual", shape, wide)
+    po, so = c.flat(out, "out", shape, t if group is None else _E4M3)
+    pro, sro = c.flat(residual_out, "residual_out", shape, wide)
+    args = _lib.RmsNormArgs(rows, dim, t, wide, wt, group or 0, eps, sx, sr, so, sro, px, pr, pw,
+                            po, pro, c.whole(rstd, "rstd", shape[:-1], _F32), ps)
+    _lib.check(_lib.lib().salt_rms_norm(ctypes.byref(args), stream_handle()))
+    return NormOutput(out, residual_out, rstd, scale)
+
+
+def rms_norm(x, weight, *, residual=None, eps: float = 1e-5, out=None, residual_out=None,
+             rstd=None) -> NormOutput:
+    """``r = x + residual; out = r / sqrt(mean(r^2) + eps) * weight`` over the last axis (at most
+    16384 wide).  `residual` holds x's type or float32; `residual_out` takes r in that type (it may
+    be `residual`, and `out` may be `x`), `rstd` the factors that the gradient needs."""
+    return _norm(x, weight, residual, eps, out, residual_out, rstd, None, None)
+
+
+def rms_norm_q8(x, weight, *, residual=None, eps: float = 1e-5, group: int = 128, out=None,
+                scale=None, residual_out=None, rstd=None) -> NormOutput:
+    """`rms_norm` with an output in 8 bits (`device.float8_e4m3`): every `group` neighbouring
+    elements (32, 64, 128, 256, or 0 for the whole row) share a float32 scale, the largest
+    magnitude / 448 (1 for a group of zeros), and ``out * scale`` is the normed value."""
+    if group not in GROUPS_8BIT:
+        raise ValueError(f"group must be one of {GROUPS_8BIT}")
+    return _norm(x, weight, residual, eps, out, residual_out, rstd, scale, int(group))
+
+
+def rms_norm_backward(dy, x, weight, rstd, *, dresidual=None, dx=None, dweight=None
+                      ) -> NormGradients:
+    """Gradients of `rms_norm`: x is what was normed (`residual_out`, or the input where there was
+    no residual), rstd its factors, dresidual the gradient that reaches `residual_out` from
+    elsewhere.  dx, the gradient of the input and of the residual alike, holds x's type (it may be
+    `dresidual`); dweight (float32) is made unless given, and left out for False."""
+    c = _Call()
+    t, wide = c.type(dy, "dy"), c.type(x, "x")
+    if wide not in (t, _F32):
+        raise TypeError("x: must hold dy's type or float32")
+    shape = tuple(dy.shape)
+    if not shape:
+        raise ValueError("dy: needs at least one axis")
+    rows, dim = int(np.prod(shape[:-1], dtype=np.int64)), shape[-1]
+    dx = _made(dx, shape, wide)
+    dweight = _wanted(True if dweight is None else dweight, (dim,), _F32)
+    pdy, sdy = c.flat(dy, "dy", shape, t)
+    px, sx = c.flat(x, "x", shape, wide)
+    pr, sr = c.flat(dresidual, "dresidual", shape, wide)
+    pdx, sdx = c.flat(dx, "dx", shape, wide)
+    pw, wt = c.weight(weight, "weight", (dim,), t)
+    args = _lib.RmsNormBackwardArgs(rows, dim, t, wide, wt, 0, sdy, sx, sr, sdx, pdy, px, pw,
+                                    c.whole(rstd, "rstd", shape[:-1], _F32), pr, pdx,
+                                    c.whole(dweight, "dweight", (dim,), _F32))
+    lib = _lib.lib()
+    ws, n = _work(lib.salt_rms_norm_backward_workspace_size, args)
+    _lib.check(lib.salt_rms_norm_backward(ctypes.byref(args), ws and ws.ptr, n, stream_handle()))
+    return NormGradients(dx, dweight)
+
+
+# ---------------------------------------------------------------- causal convolution
+
+def causal_conv(x, weight, bias=None, *, n_real=None, initial_state=None, silu: bool = True,
+                out=None, final_state=None) -> ConvOutput:
+    """``p[t] = bias + sum_k weight[:, k] x[t - width + 1 + k]``, put through ``p * sigmoid(p)``
+    with silu, over rows x (batch, len, dim) with weight (dim, width), width 1 to 8.  n_real
+    (batch, int32) ends each row early: what lies past it is not read and comes back as zero.
+    initial_state (batch, dim, width - 1) holds the inputs in front of the row, oldest first;
+    final_state takes the last ones (and may be initial_state)."""
+    c = _Call()
+    t = c.type(x, "x")
+    batch, n, dim = shape = _axes(x, "x", 3)
+    width = _axes(weight, "weight", 2)[1]
+    edge = (batch, dim, width - 1)
+    out, final_state = _made(out, shape, t), _wanted(final_state, edge, t)
+    pw, wt = c.weight(weight, "weight", (dim, width), t)
+    px, sx = c.rows(x, "x", shape, t)
+    po, so = c.rows(out, "out", shape, t)
+    args = _lib.CausalConvArgs(batch, n, dim, width, t, wt, bool(silu), 0, *sx, *so, px, pw,
+                               c.whole(bias, "bias", (dim,), wt),
+                               c.whole(n_real, "n_real", (batch,), _I32),
+                               c.whole(initial_state, "initial_state", edge, t), po,
+                               c.whole(final_state, "final_state", edge, t))
+    _lib.check(_lib.lib().salt_causal_conv(ctypes.byref(args), stream_handle()))
+    return ConvOutput(out, final_state)
+
+
+def causal_conv_step(x, state, weight, bias=None, *, slots=None, silu: bool = True, out=None
+                     ) -> ConvOutput:
+    """One token x (batch, dim) for each row: row b shifts it into state[slots[b]] of a pool
+    (n_slots, dim, width - 1), in place.  Without slots row b is slot b.  A slot outside the pool
+    marks an empty row (its out is zero); no slot may appear twice."""
+    c = _Call()
+    t = c.type(x, "x")
+    batch, dim = shape = _axes(x, "x", 2)
+    width = _axes(weight, "weight", 2)[1]
+    n_slots = _axes(state, "state", 3)[0]
+    out = _made(out, shape, t)
+    pw, wt = c.weight(weight, "weight", (dim, width), t)
+    px, sx = c.rows(x, "x", shape, t)
+    po, so = c.rows(out, "out", shape, t)
+    args = _lib.CausalConvStepArgs(batch, dim, width, n_slots, t, wt, bool(silu), 0, *sx, *so, px,
+                                   pw, c.whole(bias, "bias", (dim,), wt),
+                                   c.whole(slots, "slots", (batch,), _I32),
+                                   c.whole(state, "state", (n_slots, dim, width - 1), t), po)
+    _lib.check(_lib.lib().salt_causal_conv_step(ctypes.byref(args), stream_handle()))
+    return ConvOutput(out, state)
+
+
+def causal_conv_backward(dy, x, weight, bias=None, *, n_real=None, initial_state=None,
+                         silu: bool = True, dx=None, dweight=None, dbias=None, dinitial=None
+                         ) -> ConvGradients:
+    """Gradients of `causal_conv` for dy, the gradient of its out.  dweight and dbias are float32
+    (dbias is made where there is a bias); dinitial (batch, dim, width - 1) holds x's type and is
+    optional."""
+    c = _Call()
+    t = c.type(x, "x")
+    batch, n, dim = shape = _axes(x, "x", 3)
+    width = _axes(weight, "weight", 2)[1]
+    edge = (batch, dim, width - 1)
+    dx, dweight = _made(dx, shape, t), _made(dweight, (dim, width), _F32)
+    dbias = _wanted(bias is not None if dbias is None else dbias, (dim,), _F32)
+    dinitial = _wanted(dinitial, edge, t)
+    pw, wt = c.weight(weight, "weight", (dim, width), t)
+    pdy, sdy = c.rows(dy, "dy", shape, t)
+    px, sx = c.rows(x, "x", shape, t)
+    pdx, sdx = c.rows(dx, "dx", shape, t)
+    args = _lib.CausalConvBackwardArgs(
+        batch, n, dim, width, t, wt, bool(silu), 0, *sdy, *sx, *sdx, pdy, px, pw,
+        c.whole(bias, "bias", (dim,), wt), c.whole(n_real, "n_real", (batch,), _I32),
+        c.whole(initial_state, "initial_state", edge, t), pdx,
+        c.whole(dinitial, "dinitial", edge, t), c.whole(dweight, "dweight", (dim, width), _F32),
+        c.whole(dbias, "dbias", (dim,), _F32))
+    lib = _lib.lib()
+    ws, size = _work(lib.salt_causal_conv_backward_workspace_size, args)
+    _lib.check(lib.salt_causal_conv_backward(ctypes.byref(args), ws and ws.ptr, size,
+                                             stream_handle()))
+    return ConvGradients(dx, dweight, dbias, dinitial)
+
+
+# ---------------------------------------------------------------- selective scan
+
+def _checkpoint_shape(batch, n, dim, state):
+    return batch, -(-n // CHECKPOINT), dim, state
+
+
+def selective_scan(x, delta, A, B, C, *, D=None, z=None, delta_bias=None, softplus: bool = True,
+                   n_real=None, initial_state=None, out=None, final_state=None, checkpoints=None
+                   ) -> ScanOutput:
+    """With ``s[t] = softplus(delta[t] + delta_bias)`` (or the sum itself without softplus):
+
+        h[t] = exp(s[t] A) h[t-1] + s[t] x[t] B[t];   y[t] = sum_n C[t] h[t] + D x[t]
+
+    and ``out = y``, or ``y * z * sigmoid(z)`` where z is given.  x, delta, z: (batch, len, dim); A:
+    (dim, state) float32, state 1 to 64; B, C: (batch, len, groups, state), channel d reading group
+    ``d // (dim / groups)``; D, delta_bias: (dim,) float32.  n_real (batch, int32) ends each row
+    early.  initial_state and final_state: (batch, dim, state) float32, may be one array.
+    checkpoints takes the states that `selective_scan_backward` starts from."""
+    c = _Call()
+    t = c.type(x, "x")
+    batch, n, dim = shape = _axes(x, "x", 3)
+    groups, state = _axes(B, "B", 4)[2:]
+    both, ends = (batch, n, groups, state), (batch, dim, state)
+    marks = _checkpoint_shape(batch, n, dim, state)
+    out, final_state = _made(out, shape, t), _wanted(final_state, ends, _F32)
+    checkpoints = _wanted(checkpoints, marks, _F32)
+    px, sx = c.rows(x, "x", shape, t)
+    pd, sd = c.rows(delta, "delta", shape, t)
+    pz, sz = c.rows(z, "z", shape, t)
+    pb, sb = c.rows(B, "B", both, t, 2)
+    pc, sc = c.rows(C, "C", both, t, 2)
+    po, so = c.rows(out, "out", shape, t)
+    args = _lib.SelectiveScanArgs(
+        batch, n, dim, state, groups, t, bool(softplus), 0, *sx, *sd, *sz, *sb, *sc, *so, px, pd,
+        pz, pb, pc, c.whole(A, "A", (dim, state), _F32), c.whole(D, "D", (dim,), _F32),
+        c.whole(delta_bias, "delta_bias", (dim,), _F32),
+        c.whole(n_real, "n_real", (batch,), _I32),
+        c.whole(initial_state, "initial_state", ends, _F32), po,
+        c.whole(final_state, "final_state", ends, _F32),
+        c.whole(checkpoints, "checkpoints", marks, _F32))
+    lib = _lib.lib()
+    ws, size = _work(lib.salt_selective_scan_workspace_size, args)
+    _lib.check(lib.salt_selective_scan(ctypes.byref(args), ws and ws.ptr, size, stream_handle()))
+    return ScanOutput(out, final_state, checkpoints)
+
+
+def selective_scan_step(pool, x, delta, A, B, C, *, D=None, z=None, delta_bias=None,
+                        softplus: bool = True, slots=None, out=None) -> ScanOutput:
+    """One token of `selective_scan` for each row, x, delta, z (batch, dim) and B, C (batch,
+    groups, state), on pool[slots[b]] of float32 states (n_slots, dim, state), in place; slots as in
+    `causal_conv_step`."""
+    c = _Call()
+    t = c.type(x, "x")
+    batch, dim = shape = _axes(x, "x", 2)
+    groups, state = _axes(B, "B", 3)[1:]
+    n_slots = _axes(pool, "pool", 3)[0]
+    both = (batch, groups, state)
+    out = _made(out, shape, t)
+    px, (sx,) = c.rows(x, "x", shape, t)
+    pd, (sd,) = c.rows(delta, "delta", shape, t)
+    pz, (sz,) = c.rows(z, "z", shape, t)
+    pb, (sb,) = c.rows(B, "B", both, t, 2)
+    pc, (sc,) = c.rows(C, "C", both, t, 2)
+    po, (so,) = c.rows(out, "out", shape, t)
+    args = _lib.SelectiveScanStepArgs(
+        batch, dim, state, groups, n_slots, t, bool(softplus), 0, sx, sd, sz, sb, sc, so, px, pd,
+        pz, pb, pc, c.whole(A, "A", (dim, state), _F32), c.whole(D, "D", (dim,), _F32),
+        c.whole(delta_bias, "delta_bias", (dim,), _F32), c.whole(slots, "slots", (batch,), _I32),
+        c.whole(pool, "pool", (n_slots, dim, state), _F32), po)
+    _lib.check(_lib.lib().salt_selective_scan_step(ctypes.byref(args), stream_handle()))
+    return ScanOutput(out, pool)
+
+
+def selective_scan_backward(dy, x, delta, A, B, C, *, checkpoints, D=None, z=None,
+                            delta_bias=None, softplus: bool = True, n_real=None, dfinal=None,
+                            dx=None, ddelta=None, dA=None, dB=None, dC=None, dD=None, dz=None,
+                            ddelta_bias=None, dinitial=None) -> ScanGradients:
+    """Gradients of `selective_scan` for dy, the gradient of its out, and dfinal, that of its final
+    state, from the forward's arguments and checkpoints.  dA, dD, ddelta_bias and dinitial are
+    float32, the others hold x's type; dD, dz and ddelta_bias are made where their input is given,
+    dinitial is optional."""
+    c = _Call()
+    t = c.type(x, "x")
+    batch, n, dim = shape = _axes(x, "x", 3)
+    groups, state = _axes(B, "B", 4)[2:]
+    both, ends = (batch, n, groups, state), (batch, dim, state)
+    dx, ddelta = _made(dx, shape, t), _made(ddelta, shape, t)
+    dA, dB, dC = _made(dA, (dim, state), _F32), _made(dB, both, t), _made(dC, both, t)
+    dD = None if D is None else _made(dD, (dim,), _F32)
+    dz = None if z is None else _made(dz, shape, t)
+    ddelta_bias = None if delta_bias is None else _made(ddelta_bias, (dim,), _F32)
+    dinitial = _wanted(dinitial, ends, _F32)
+    px, sx = c.rows(x, "x", shape, t)
+    pd, sd = c.rows(delta, "delta", shape, t)
+    pz, sz = c.rows(z, "z", shape, t)
+    pb, sb = c.rows(B, "B", both, t, 2)
+    pc, sc = c.rows(C, "C", both, t, 2)
+    pdy, sdy = c.rows(dy, "dy", shape, t)
+    pdx, sdx = c.rows(dx, "dx", shape, t)
+    pdd, sdd = c.rows(ddelta, "ddelta", shape, t)
+    pdz, sdz = c.rows(dz, "dz", shape, t)
+    marks = _checkpoint_shape(batch, n, dim, state)
+    args = _lib.SelectiveScanBackwardArgs(
+        batch, n, dim, state, groups, t, bool(softplus), 0, *sx, *sd, *sz, *sb, *sc, *sdy, *sdx,
+        *sdd, *sdz, px, pd, pz, pb, pc, pdy, c.whole(A, "A", (dim, state), _F32),
+        c.whole(D, "D", (dim,), _F32), c.whole(delta_bias, "delta_bias", (dim,), _F32),
+        c.whole(n_real, "n_real", (batch,), _I32),
+        c.whole(checkpoints, "checkpoints", marks, _F32),
+        c.whole(dfinal, "dfinal", ends, _F32), pdx, pdd, pdz, c.whole(dB, "dB", both, t),
+        c.whole(dC, "dC", both, t), c.whole(dA, "dA", (dim, state), _F32),
+        c.whole(dD, "dD", (dim,), _F32), c.whole(ddelta_bias, "ddelta_bias", (dim,), _F32),
+        c.whole(dinitial, "dinitial", ends, _F32))
+    lib = _lib.lib()
+    ws, size = _work(lib.salt_selective_scan_backward_workspace_size, args)
+    _lib.check(lib.salt_selective_scan_backward(ctypes.byref(args), ws and ws.ptr, size,
+                                                stream_handle()))
+    return ScanGradients(dx, ddelta, dA, dB, dC, dD, dz, ddelta_bias, dinitial)
