@@ -11,32 +11,42 @@ namespace salt {
 
 namespace {
 
-// LPC lanes hold a channel's states, NS each.
-template <int NS_, int LPC_>
+// LPC lanes hold a channel's states, NS each, and CPT channels each: what a lane reads of B and C
+// serves both.  A thread loads and stores 8 neighbouring channels of one token.
+template <int NS_, int LPC_, int CPT_>
 struct Shape {
-  static constexpr int NS = NS_, LPC = LPC_;
-  static constexpr int kThreads = kScanChannels * LPC;
-  static constexpr int kTile = kThreads / (kScanChannels / kVec);  // tokens: one pack a thread
+  static constexpr int NS = NS_, LPC = LPC_, CPT = CPT_;
+  static constexpr int kChannels = LPC == 1 ? 64 : 32;  // of a block
+  static constexpr int kThreads = kChannels * LPC / CPT;
+  static constexpr int kIo = kChannels / kVec;  // threads of one token
+  static constexpr int kTile = kThreads / kIo;  // tokens
   static constexpr int kStates = NS * LPC;
-  static constexpr int kYPitch = kScanChannels + 8;  // 4 tokens x 8 channels on 32 banks
+  static constexpr int kStepPitch = kChannels + 4;  // 4 tokens' stores on 32 banks
+  static constexpr int kYPitch = kChannels + 8;
 };
 
+// Where a channel of a block lies in shared memory: channel 8 v + k at place kIo k + v, so that the
+// threads of a token store next to each other.  This is the channel at a place.
 template <class S>
-struct ScanShared {
-  float2 step[S::kTile][kScanChannels];  // s and s * x
-  float y[S::kTile][S::kYPitch];
-  float B[S::kTile][S::kStates], C[S::kTile][S::kStates];
-};
-
-// B or C of a tile into shared memory as float32, zero past `real` and past the last state.
-template <typename T, class S>
-__device__ __forceinline__ void stage_states(float (*to)[S::kStates], const T* from,
-                                             int64_t stride, int state, int t0, int real) {
-  for (int i = threadIdx.x; i < S::kTile * S::kStates; i += S::kThreads) {
-    const int t = i / S::kStates, n = i % S::kStates;
-    to[t][n] = (t0 + t < real && n < state) ? to_f32(from[(t0 + t) * stride + n]) : 0.f;
-  }
+__device__ __forceinline__ int scan_channel(int place) {
+  return place % S::kIo * kVec + place / S::kIo;
 }
+
+constexpr int kStages = 2;  // tiles in shared memory as they were loaded: this one and the next
+
+template <typename T, class S, bool FULL>
+struct ScanShared {
+  struct Raw {
+    alignas(16) T x[S::kTile][S::kChannels], delta[S::kTile][S::kChannels];
+    alignas(16) T z[FULL ? S::kTile : 1][S::kChannels];
+    alignas(16) T bc[FULL ? 2 : 1][S::kTile][S::kStates];
+  } raw[kStages];
+  alignas(16) float2 step[S::kTile][S::kStepPitch];  // s and s * x
+  alignas(16) float B[S::kTile][S::kStates];
+  alignas(16) float C[FULL ? S::kTile : 1][S::kStates];
+  alignas(8) float y[FULL ? S::kTile : 1][S::kYPitch];
+  alignas(8) float bias[S::kChannels], skip[S::kChannels];
+};
 
 // The state in front of chunk c, from the first pass's results.
 template <int NS>
@@ -55,182 +65,250 @@ __device__ __forceinline__ void chunk_start(float (&h)[NS], const float (&A2)[NS
   }
 }
 
+// Warps of an SM that the registers are held down for.
 template <typename T, class S>
-__global__ void __launch_bounds__(S::kThreads)
-selective_scan_kernel(salt_selective_scan_args a, ScanSplit sp, int blocks, bool vec, bool svec) {
-  constexpr int NS = S::NS, LPC = S::LPC;
-  __shared__ ScanShared<S> sm;
-  const int tid = threadIdx.x;
-  const int64_t b = blockIdx.x / (blocks * sp.chunks);
-  const int rest = (int)(blockIdx.x - b * blocks * sp.chunks), c = rest / blocks;
-  const ScanBlock cb = scan_block(rest - c * blocks, a.dim, a.groups, kScanChannels);
+constexpr int resident() {
+  return (S::NS == 4 ? 20 : 16) * 32 / S::kThreads;
+}
+
+// FULL: the scan.  Otherwise the first pass over a split row: chunk c's state from zero (chunk 0's
+// from the initial state) into place c + 1, and the sum of its steps; the last chunk has no
+// successor and is not run.
+template <typename T, class S, bool FULL, int COPY>
+__global__ void __launch_bounds__(S::kThreads, resident<T, S>())
+selective_scan_kernel(salt_selective_scan_args a, ScanSplit sp, int blocks, bool svec) {
+  constexpr int NS = S::NS, LPC = S::LPC, CPT = S::CPT, H = NS / 2;
+  extern __shared__ __align__(16) unsigned char raw_shared[];
+  ScanShared<T, S, FULL>& sm = *reinterpret_cast<ScanShared<T, S, FULL>*>(raw_shared);
+  const int tid = threadIdx.x, chunks = FULL ? sp.chunks : sp.chunks - 1;
+  const int64_t b = blockIdx.x / (blocks * chunks);
+  const int rest = (int)(blockIdx.x - b * blocks * chunks), c = rest / blocks;
+  const ScanBlock cb = scan_block(rest - c * blocks, a.dim, a.groups, S::kChannels);
   const int real = row_tokens(a.n_real, (int)b, a.len);
   const int begin = c * sp.chunk_len, end = min(begin + sp.chunk_len, a.len);
+  const int stop = min(real, end);
   const int last = real > 0 ? (real - 1) / sp.chunk_len : 0;  // the chunk with the last token
 
-  // this thread's channel and states in the recurrence
-  const int ch = tid / LPC, n0 = tid % LPC * NS, ns = a.state - n0;
-  const bool mine = ch < cb.n;
-  const int64_t d = cb.d0 + (mine ? ch : 0);
-  float A2[NS], h[NS];
-  load_states<NS>(A2, a.A + d * a.state + n0, mine ? ns : 0, svec);
+  // this thread's channels and states in the recurrence
+  const int at = tid / LPC * CPT, n0 = tid % LPC * NS, ns = a.state - n0;
+  bool mine[CPT];
+  int64_t d[CPT];
+  f32x2 A2[CPT][H], h[CPT][H];
 #pragma unroll
-  for (int i = 0; i < NS; ++i) A2[i] *= kLog2e;
-  if (sp.chunks > 1) {
-    chunk_start<NS>(h, A2, sp, b, min(c, last), a.dim, d, a.state, n0, svec);
-  } else {
-    load_states<NS>(h, a.initial_state + (b * a.dim + d) * a.state + n0,
-                    mine && a.initial_state ? ns : 0, svec);
+  for (int j = 0; j < CPT; ++j) {
+    const int ch = scan_channel<S>(at + j);
+    mine[j] = ch < cb.n;
+    d[j] = cb.d0 + (mine[j] ? ch : 0);
+    float f[NS], s[NS];
+    load_states<NS>(f, a.A + d[j] * a.state + n0, mine[j] ? ns : 0, svec);
+#pragma unroll
+    for (int i = 0; i < NS; ++i) f[i] *= kLog2e;
+    if (FULL && sp.chunks > 1)
+      chunk_start<NS>(s, f, sp, b, min(c, last), a.dim, d[j], a.state, n0, svec);
+    else
+      load_states<NS>(s, a.initial_state + (b * a.dim + d[j]) * a.state + n0,
+                      mine[j] && a.initial_state && c == 0 ? ns : 0, svec);
+    if (!FULL && c == 0 && mine[j])
+      store_states<NS>(sp.state + (b * sp.chunks * a.dim + d[j]) * a.state + n0, s, ns, svec);
+#pragma unroll
+    for (int i = 0; i < H; ++i) {
+      A2[j][i] = pair(f[2 * i], f[2 * i + 1]);
+      h[j][i] = pair(s[2 * i], s[2 * i + 1]);
+    }
   }
+  auto store_h = [&](int j, float* to) {
+    float f[NS];
+#pragma unroll
+    for (int i = 0; i < H; ++i) {
+      const float2 v = halves(h[j][i]);
+      f[2 * i] = v.x, f[2 * i + 1] = v.y;
+    }
+    store_states<NS>(to + d[j] * a.state + n0, f, ns, svec);
+  };
 
   // and its 8 channels of one token in loads and stores
-  const int io_t = tid / (kScanChannels / kVec), io_c = tid % (kScanChannels / kVec) * kVec;
-  const int io_d = cb.d0 + io_c, io_n = cb.n - io_c;
+  const int io_t = tid / S::kIo, io_v = tid % S::kIo;
+  const int io_d = cb.d0 + io_v * kVec, io_n = cb.n - io_v * kVec;
   const T* x = static_cast<const T*>(a.x) + b * a.x_batch_stride + io_d;
   const T* delta = static_cast<const T*>(a.delta) + b * a.delta_batch_stride + io_d;
-  const T* z = a.z ? static_cast<const T*>(a.z) + b * a.z_batch_stride + io_d : nullptr;
+  const T* z = FULL && a.z ? static_cast<const T*>(a.z) + b * a.z_batch_stride + io_d : nullptr;
   T* out = static_cast<T*>(a.out) + b * a.out_batch_stride + io_d;
   const T* B = static_cast<const T*>(a.B) + b * a.B_batch_stride + (int64_t)cb.group * a.state;
   const T* C = static_cast<const T*>(a.C) + b * a.C_batch_stride + (int64_t)cb.group * a.state;
-  float bias[kVec], skip[kVec];
-#pragma unroll
-  for (int k = 0; k < kVec; ++k) {
-    bias[k] = a.delta_bias && k < io_n ? a.delta_bias[io_d + k] : 0.f;
-    skip[k] = a.D && k < io_n ? a.D[io_d + k] : 0.f;
+  for (int i = tid; i < S::kChannels; i += S::kThreads) {
+    sm.bias[i] = a.delta_bias && i < cb.n ? a.delta_bias[cb.d0 + i] : 0.f;
+    sm.skip[i] = a.D && i < cb.n ? a.D[cb.d0 + i] : 0.f;
   }
+  // Each thread copies what it converts itself: its 8 channels of one token, and packs of 4 states
+  // of B and C.  So a copy has arrived for its reader once that thread has waited for it.
+  constexpr int kPacks = S::kTile * S::kStates / 4;
+  auto load = [&](int t0) {
+    auto& raw = sm.raw[t0 / S::kTile % kStages];
+    const int t = t0 + io_t, n = t < stop ? io_n : 0;
+    copy_pack<COPY, kVec>(&raw.x[io_t][io_v * kVec], x + t * a.x_stride, n);
+    copy_pack<COPY, kVec>(&raw.delta[io_t][io_v * kVec], delta + t * a.delta_stride, n);
+    if (z) copy_pack<COPY, kVec>(&raw.z[FULL ? io_t : 0][io_v * kVec], z + t * a.z_stride, n);
+    for (int i = tid; i < kPacks; i += S::kThreads) {
+      const int q = i / (S::kStates / 4), n1 = i % (S::kStates / 4) * 4;
+      const int left = t0 + q < stop ? a.state - n1 : 0;
+      copy_pack<COPY, 4>(&raw.bc[0][q][n1], B + (t0 + q) * a.B_stride + n1, left);
+      if (FULL)
+        copy_pack<COPY, 4>(&raw.bc[FULL ? 1 : 0][q][n1], C + (t0 + q) * a.C_stride + n1, left);
+    }
+    copies_commit();
+  };
 
-  for (int t0 = begin; t0 < end; t0 += S::kTile) {
+  float sum[CPT] = {};
+  if (begin < stop) load(begin);
+  __syncthreads();  // bias and skip
+  for (int t0 = begin; t0 < (FULL ? end : stop); t0 += S::kTile) {
     const int t = t0 + io_t;
-    float xs[kVec], y[kVec];
-    Pack<T, kVec> pz;
-    if (t0 < real) {
-      const int n = t < real ? io_n : 0;
-      const Pack<T, kVec> px = load_pack<T, kVec>(x + t * a.x_stride, n, vec);
-      const Pack<T, kVec> pd = load_pack<T, kVec>(delta + t * a.delta_stride, n, vec);
-      if (z) pz = load_pack<T, kVec>(z + t * a.z_stride, n, vec);
-#pragma unroll
-      for (int k = 0; k < kVec; ++k) {
-        xs[k] = to_f32(px.v[k]);
-        // past the last token s = 0: the state stays as it is
-        const float s = t < real ? scan_step(to_f32(pd.v[k]) + bias[k], a.softplus) : 0.f;
-        sm.step[io_t][io_c + k] = make_float2(s, s * xs[k]);
+    const auto& raw = sm.raw[t0 / S::kTile % kStages];
+    if (t0 < stop) {
+      if (t0 + S::kTile < stop) {
+        load(t0 + S::kTile);
+        copies_wait<1>();
+      } else {
+        copies_wait<0>();
       }
-      stage_states<T, S>(sm.B, B, a.B_stride, a.state, t0, min(real, end));
-      stage_states<T, S>(sm.C, C, a.C_stride, a.state, t0, min(real, end));
-      __syncthreads();
-#pragma unroll 1
-      for (int g = 0; g < S::kTile; g += 4) {
-        if (a.checkpoints && mine && (t0 + g) % SALT_SCAN_CHECKPOINT == 0 && t0 + g < real) {
-          const int64_t per = (a.len + SALT_SCAN_CHECKPOINT - 1) / SALT_SCAN_CHECKPOINT;
-          store_states<NS>(a.checkpoints +
-                               ((b * per + (t0 + g) / SALT_SCAN_CHECKPOINT) * a.dim + d) * a.state +
-                               n0,
-                           h, ns, svec);
+      const T *rx = &raw.x[io_t][io_v * kVec], *rd = &raw.delta[io_t][io_v * kVec];
+#pragma unroll
+      for (int k = 0; k < kVec; k += 2) {
+        const f32x2 in = add2(pair(to_f32(rd[k]), to_f32(rd[k + 1])),
+                              *reinterpret_cast<const f32x2*>(&sm.bias[io_v * kVec + k]));
+        // past the last token s = 0: the state stays as it is
+        const f32x2 s2 = t < stop ? scan_step2(in, a.softplus) : 0;
+        const float2 s = halves(s2), sx = halves(mul2(s2, pair(to_f32(rx[k]), to_f32(rx[k + 1]))));
+        sm.step[io_t][k * S::kIo + io_v] = make_float2(s.x, sx.x);
+        sm.step[io_t][(k + 1) * S::kIo + io_v] = make_float2(s.y, sx.y);
+      }
+      for (int i = tid; i < kPacks; i += S::kThreads) {
+        const int q = i / (S::kStates / 4), n1 = i % (S::kStates / 4) * 4;
+        const T* p = &raw.bc[0][q][n1];
+        *reinterpret_cast<float4*>(&sm.B[q][n1]) =
+            make_float4(to_f32(p[0]), to_f32(p[1]), to_f32(p[2]), to_f32(p[3]));
+        if (FULL) {
+          p = &raw.bc[FULL ? 1 : 0][q][n1];
+          *reinterpret_cast<float4*>(&sm.C[FULL ? q : 0][n1]) =
+              make_float4(to_f32(p[0]), to_f32(p[1]), to_f32(p[2]), to_f32(p[3]));
         }
-        float yq[4];
+      }
+    }
+    __syncthreads();
+    if (t0 < stop) {
+      constexpr int kUnroll = 4;
+#pragma unroll kUnroll
+      for (int g = 0; g < S::kTile; g += 4) {
+        if (FULL && a.checkpoints && (t0 + g) % SALT_SCAN_CHECKPOINT == 0 && t0 + g < stop) {
+          const int64_t per = (a.len + SALT_SCAN_CHECKPOINT - 1) / SALT_SCAN_CHECKPOINT;
+          float* to = a.checkpoints + (b * per + (t0 + g) / SALT_SCAN_CHECKPOINT) * a.dim * a.state;
+#pragma unroll
+          for (int j = 0; j < CPT; ++j)
+            if (mine[j]) store_h(j, to);
+        }
+        float yq[4 * CPT];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const float2 st = sm.step[g + q][ch];
-          yq[q] = 0.f;
+          f32x2 s[CPT], sx[CPT], y2[CPT];
+          float2 st[CPT];
+          if constexpr (CPT == 2) {
+            const float4 v = *reinterpret_cast<const float4*>(&sm.step[g + q][at]);
+            st[0] = make_float2(v.x, v.y), st[1] = make_float2(v.z, v.w);
+          } else {
+            st[0] = sm.step[g + q][at];
+          }
 #pragma unroll
-          for (int i = 0; i < NS; ++i) {
-            h[i] = fmaf(exp2_fast(A2[i] * st.x), h[i], st.y * sm.B[g + q][n0 + i]);
-            yq[q] = fmaf(h[i], sm.C[g + q][n0 + i], yq[q]);
+          for (int j = 0; j < CPT; ++j) {
+            s[j] = pair(st[j].x, st[j].x), sx[j] = pair(st[j].y, st[j].y);
+            if (!FULL) sum[j] += st[j].x;
+          }
+#pragma unroll
+          for (int i = 0; i < NS; i += 4) {
+            const ulonglong2 bn = *reinterpret_cast<const ulonglong2*>(&sm.B[g + q][n0 + i]);
+#pragma unroll
+            for (int j = 0; j < CPT; ++j) {
+              f32x2 &h0 = h[j][i / 2], &h1 = h[j][i / 2 + 1];
+              h0 = fma2(exp2_fast2(mul2(A2[j][i / 2], s[j])), h0, mul2(sx[j], bn.x));
+              h1 = fma2(exp2_fast2(mul2(A2[j][i / 2 + 1], s[j])), h1, mul2(sx[j], bn.y));
+            }
+            if (FULL) {
+              const ulonglong2 cn = *reinterpret_cast<const ulonglong2*>(&sm.C[g + q][n0 + i]);
+#pragma unroll
+              for (int j = 0; j < CPT; ++j) {
+                y2[j] = i ? fma2(h[j][i / 2], cn.x, y2[j]) : mul2(h[j][0], cn.x);
+                y2[j] = fma2(h[j][i / 2 + 1], cn.y, y2[j]);
+              }
+            }
+          }
+          if (FULL) {
+#pragma unroll
+            for (int j = 0; j < CPT; ++j) {
+              const float2 v = halves(y2[j]);
+              yq[q * CPT + j] = v.x + v.y;
+            }
           }
         }
-        int first = 0;
-        lane_sums<4, 1, LPC>(yq, tid, first);
+        if (FULL) {
+          int first = 0;
+          lane_sums<4 * CPT, 1, LPC>(yq, tid, first);
+          constexpr int kept = 4 * CPT / LPC;
 #pragma unroll
-        for (int q = 0; q < 4 / LPC; ++q) sm.y[g + first + q][ch] = yq[q];
+          for (int i = 0; i < kept; ++i)
+            sm.y[g + (first + i) / CPT][at + (first + i) % CPT] = yq[i];
+        }
       }
-      __syncthreads();
     }
-    if (t < end) {
+    __syncthreads();
+    if (FULL && t < end) {
+      const T *rx = &raw.x[io_t][io_v * kVec], *rz = &raw.z[FULL ? io_t : 0][io_v * kVec];
+      float y[kVec];
 #pragma unroll
-      for (int k = 0; k < kVec; ++k) {
-        y[k] = 0.f;
-        if (t < real) {
-          y[k] = fmaf(skip[k], xs[k], sm.y[io_t][io_c + k]);
+      for (int k = 0; k < kVec; k += 2) {
+        f32x2 v = 0;
+        if (t < stop) {
+          v = fma2(*reinterpret_cast<const f32x2*>(&sm.skip[io_v * kVec + k]),
+                   pair(to_f32(rx[k]), to_f32(rx[k + 1])),
+                   pair(sm.y[FULL ? io_t : 0][k * S::kIo + io_v],
+                        sm.y[FULL ? io_t : 0][(k + 1) * S::kIo + io_v]));
           if (z) {
-            const float v = to_f32(pz.v[k]);
-            y[k] *= v * sigmoid(v);
+            const f32x2 g = pair(to_f32(rz[k]), to_f32(rz[k + 1]));
+            v = mul2(v, mul2(g, sigmoid2(g)));
           }
         }
+        const float2 f = halves(v);
+        y[k] = f.x, y[k + 1] = f.y;
       }
-      store_pack<T, kVec>(out + t * a.out_stride, y, io_n, vec);
+      scan_store<T, kVec, COPY == kCopy16>(out + t * a.out_stride, y, io_n);
     }
   }
-  if (c == last && mine && a.final_state)
-    store_states<NS>(a.final_state + (b * a.dim + d) * a.state + n0, h, ns, svec);
-}
-
-// The first pass over a split row: chunk c's state from zero (chunk 0's from the initial state)
-// into place c + 1, and the sum of its steps.  The last chunk has no successor and is not run.
-template <typename T, class S>
-__global__ void __launch_bounds__(S::kThreads)
-scan_state_kernel(salt_selective_scan_args a, ScanSplit sp, int blocks, bool vec, bool svec) {
-  constexpr int NS = S::NS, LPC = S::LPC;
-  __shared__ float2 step[S::kTile][kScanChannels];
-  __shared__ float sB[S::kTile][S::kStates];
-  const int tid = threadIdx.x, run = sp.chunks - 1;
-  const int64_t b = blockIdx.x / (blocks * run);
-  const int rest = (int)(blockIdx.x - b * blocks * run), c = rest / blocks;
-  const ScanBlock cb = scan_block(rest - c * blocks, a.dim, a.groups, kScanChannels);
-  const int begin = c * sp.chunk_len;
-  const int real = min(row_tokens(a.n_real, (int)b, a.len), begin + sp.chunk_len);
-  const int ch = tid / LPC, n0 = tid % LPC * NS, ns = a.state - n0;
-  const bool mine = ch < cb.n;
-  const int64_t d = cb.d0 + (mine ? ch : 0);
-  float A2[NS], h[NS], sum = 0.f;
-  load_states<NS>(A2, a.A + d * a.state + n0, mine ? ns : 0, svec);
 #pragma unroll
-  for (int i = 0; i < NS; ++i) A2[i] *= kLog2e;
-  const int64_t at = ((b * sp.chunks + c) * a.dim + d) * a.state + n0;
-  load_states<NS>(h, a.initial_state + (b * a.dim + d) * a.state + n0,
-                  c == 0 && mine && a.initial_state ? ns : 0, svec);
-  if (c == 0 && mine) store_states<NS>(sp.state + at, h, ns, svec);
-  const int io_t = tid / (kScanChannels / kVec), io_c = tid % (kScanChannels / kVec) * kVec;
-  const int io_d = cb.d0 + io_c, io_n = cb.n - io_c;
-  const T* x = static_cast<const T*>(a.x) + b * a.x_batch_stride + io_d;
-  const T* delta = static_cast<const T*>(a.delta) + b * a.delta_batch_stride + io_d;
-  const T* B = static_cast<const T*>(a.B) + b * a.B_batch_stride + (int64_t)cb.group * a.state;
-  float bias[kVec];
-#pragma unroll
-  for (int k = 0; k < kVec; ++k)
-    bias[k] = a.delta_bias && k < io_n ? a.delta_bias[io_d + k] : 0.f;
-  for (int t0 = begin; t0 < real; t0 += S::kTile) {
-    const int t = t0 + io_t, n = t < real ? io_n : 0;
-    const Pack<T, kVec> px = load_pack<T, kVec>(x + t * a.x_stride, n, vec);
-    const Pack<T, kVec> pd = load_pack<T, kVec>(delta + t * a.delta_stride, n, vec);
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kVec; ++k) {
-      const float s = t < real ? scan_step(to_f32(pd.v[k]) + bias[k], a.softplus) : 0.f;
-      step[io_t][io_c + k] = make_float2(s, s * to_f32(px.v[k]));
-    }
-    stage_states<T, S>(sB, B, a.B_stride, a.state, t0, real);
-    __syncthreads();
-#pragma unroll 4
-    for (int q = 0; q < S::kTile; ++q) {
-      const float2 st = step[q][ch];
-      sum += st.x;
-#pragma unroll
-      for (int i = 0; i < NS; ++i) h[i] = fmaf(exp2_fast(A2[i] * st.x), h[i], st.y * sB[q][n0 + i]);
+  for (int j = 0; j < CPT; ++j) {
+    if (!mine[j]) continue;
+    if (!FULL) {
+      store_h(j, sp.state + (b * sp.chunks + c + 1) * a.dim * a.state);
+      if (n0 == 0) sp.steps[(b * sp.chunks + c) * a.dim + d[j]] = sum[j];
+    } else if (c == last && a.final_state) {
+      store_h(j, a.final_state + b * a.dim * a.state);
     }
   }
-  if (!mine) return;
-  store_states<NS>(sp.state + at + (int64_t)a.dim * a.state, h, ns, svec);
-  if (n0 == 0) sp.steps[(b * sp.chunks + c) * a.dim + d] = sum;
 }
 
 // ---------------------------------------------------------------- single tokens
+
+constexpr int kStepChannels = 32;  // of a block
+
+template <int NS_, int LPC_>
+struct StepShape {
+  static constexpr int NS = NS_, LPC = LPC_;
+  static constexpr int kThreads = kStepChannels * LPC;
+};
 
 template <typename T, class S>
 __global__ void __launch_bounds__(S::kThreads)
 selective_scan_step_kernel(salt_selective_scan_step_args a, int blocks, int rows, bool svec) {
   constexpr int NS = S::NS, LPC = S::LPC;
   const int tid = threadIdx.x, part = blockIdx.x / blocks;
-  const ScanBlock cb = scan_block(blockIdx.x - part * blocks, a.dim, a.groups, kScanChannels);
+  const ScanBlock cb = scan_block(blockIdx.x - part * blocks, a.dim, a.groups, kStepChannels);
   const int ch = tid / LPC, n0 = tid % LPC * NS, ns = a.state - n0;
   const bool mine = ch < cb.n;
   const int64_t d = cb.d0 + (mine ? ch : 0);
@@ -278,33 +356,48 @@ selective_scan_step_kernel(salt_selective_scan_step_args a, int blocks, int rows
 
 // ---------------------------------------------------------------- host side
 
-#define SALT_SCAN_SHAPE(state, S, ...)  \
-  do {                                  \
-    if ((state) <= 4) {                 \
-      using S = Shape<4, 1>;            \
-      __VA_ARGS__;                      \
-    } else if ((state) <= 8) {          \
-      using S = Shape<4, 2>;            \
-      __VA_ARGS__;                      \
-    } else if ((state) <= 16) {         \
-      using S = Shape<4, 4>;            \
-      __VA_ARGS__;                      \
-    } else if ((state) <= 32) {         \
-      using S = Shape<8, 4>;            \
-      __VA_ARGS__;                      \
-    } else {                            \
-      using S = Shape<16, 4>;           \
-      __VA_ARGS__;                      \
-    }                                   \
-  } while (0)
+using Scan4 = Shape<4, 1, 2>;
+using Scan8 = Shape<4, 2, 2>;
+using Scan16 = Shape<4, 4, 1>;
+using Scan32 = Shape<8, 4, 2>;
+using Scan64 = Shape<8, 8, 2>;
+#define SALT_SCAN_SHAPE(state, S, ...) \
+  SALT_BY_STATE(state, S, Scan4, Scan8, Scan16, Scan32, Scan64, __VA_ARGS__)
+int scan_channels(int32_t state) { return state <= 4 ? Scan4::kChannels : Scan16::kChannels; }
 
-constexpr int kFillBlocks = 148 * 2;
+using Step4 = StepShape<4, 1>;
+using Step8 = StepShape<4, 2>;
+using Step16 = StepShape<4, 4>;
+using Step32 = StepShape<8, 4>;
+using Step64 = StepShape<16, 4>;
+#define SALT_STEP_SHAPE(state, S, ...) \
+  SALT_BY_STATE(state, S, Step4, Step8, Step16, Step32, Step64, __VA_ARGS__)
+
+constexpr int kEnoughBlocks = 148 * 2;  // rows are not split
+constexpr int kFillBlocks = 148 * 12;   // and otherwise into about so many
+
+template <typename T, class S, bool FULL>
+cudaError_t scan_launch(const salt_selective_scan_args& a, const ScanSplit& sp, int blocks,
+                        int chunks, int copy, bool svec, cudaStream_t st) {
+  constexpr size_t shared = sizeof(ScanShared<T, S, FULL>);
+  const auto kernel = copy == kCopy16  ? selective_scan_kernel<T, S, FULL, kCopy16>
+                      : copy == kCopy4 ? selective_scan_kernel<T, S, FULL, kCopy4>
+                                       : selective_scan_kernel<T, S, FULL, kCopyPlain>;
+  if (shared > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(
+        kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
+    if (e != cudaSuccess) return e;
+  }
+  kernel<<<(unsigned)((int64_t)a.batch * blocks * chunks), S::kThreads, shared, st>>>(a, sp, blocks,
+                                                                                    svec);
+  return cudaGetLastError();
+}
 
 ScanSplit scan_split(const salt_selective_scan_args& a) {
   ScanSplit s{1, std::max(a.len, 1), nullptr, nullptr};
-  const int64_t blocks = (int64_t)a.batch * scan_blocks(a.dim, a.groups, kScanChannels);
-  if (blocks >= kFillBlocks || blocks == 0) return s;
-  const int want = (int)((2 * kFillBlocks + blocks - 1) / blocks);
+  const int64_t blocks = (int64_t)a.batch * scan_blocks(a.dim, a.groups, scan_channels(a.state));
+  if (blocks == 0 || blocks >= kEnoughBlocks) return s;
+  const int want = (int)(kFillBlocks / blocks);
   const int each = std::max(128, (a.len + want - 1) / want);
   s.chunk_len = (each + 31) / 32 * 32;  // whole tiles and checkpoints of every shape
   s.chunks = std::max(1, (a.len + s.chunk_len - 1) / s.chunk_len);
@@ -328,28 +421,31 @@ cudaError_t selective_scan_launch(const salt_selective_scan_args& a, void* ws, c
     sp.state = static_cast<float*>(ws);
     sp.steps = sp.state + (size_t)a.batch * sp.chunks * a.dim * a.state;
   }
-  const int blocks = scan_blocks(a.dim, a.groups, kScanChannels);
+  const int blocks = scan_blocks(a.dim, a.groups, scan_channels(a.state));
   const size_t ts = type_size(a.type);
-  const bool vec = (a.groups == 1 || (a.dim / a.groups * ts) % 16 == 0) &&
-                   vec_rows(a.x, ts, a.x_batch_stride, a.x_stride) &&
-                   vec_rows(a.delta, ts, a.delta_batch_stride, a.delta_stride) &&
-                   vec_rows(a.z, ts, a.z_batch_stride, a.z_stride) &&
-                   vec_rows(a.out, ts, a.out_batch_stride, a.out_stride);
+  // the widest copies that no row's start and end stand against
+  auto fits = [&](int64_t bytes) {
+    const int64_t whole = bytes / ts, few = std::min<int64_t>(bytes, 4 * ts);
+    return (a.dim / a.groups) % (bytes == 16 ? (int)kVec : (int)whole) == 0 &&
+           a.state % (few / ts) == 0 && packed_rows(a.x, bytes, ts, a.x_batch_stride, a.x_stride) &&
+           packed_rows(a.delta, bytes, ts, a.delta_batch_stride, a.delta_stride) &&
+           (!a.z || packed_rows(a.z, bytes, ts, a.z_batch_stride, a.z_stride)) &&
+           packed_rows(a.out, bytes, ts, a.out_batch_stride, a.out_stride) &&
+           packed_rows(a.B, few, ts, a.B_batch_stride, a.B_stride) &&
+           packed_rows(a.C, few, ts, a.C_batch_stride, a.C_stride);
+  };
+  const int copy = fits(16) ? kCopy16 : fits(4) ? kCopy4 : kCopyPlain;
   const bool svec = a.state % 4 == 0 && aligned16(a.A) && aligned16(a.initial_state) &&
                     aligned16(a.final_state) && aligned16(a.checkpoints);
   cudaError_t e = cudaSuccess;
   SALT_WITH_TYPE(a.type, T, SALT_SCAN_SHAPE(a.state, S, {
     if (sp.chunks > 1) {
-      scan_state_kernel<T, S><<<(unsigned)((int64_t)a.batch * blocks * (sp.chunks - 1)),
-                                S::kThreads, 0, st>>>(a, sp, blocks, vec, svec);
+      e = scan_launch<T, S, false>(a, sp, blocks, sp.chunks - 1, copy, svec, st);
       ++*launches;
-      e = cudaGetLastError();
     }
     if (e == cudaSuccess) {
-      selective_scan_kernel<T, S><<<(unsigned)((int64_t)a.batch * blocks * sp.chunks),
-                                    S::kThreads, 0, st>>>(a, sp, blocks, vec, svec);
+      e = scan_launch<T, S, true>(a, sp, blocks, sp.chunks, copy, svec, st);
       ++*launches;
-      e = cudaGetLastError();
     }
   }));
   return e;
@@ -358,13 +454,13 @@ cudaError_t selective_scan_launch(const salt_selective_scan_args& a, void* ws, c
 cudaError_t selective_scan_step_launch(const salt_selective_scan_step_args& a, cudaStream_t st,
                                        int* launches) {
   if (a.batch == 0) return cudaSuccess;
-  const int blocks = scan_blocks(a.dim, a.groups, kScanChannels);
+  const int blocks = scan_blocks(a.dim, a.groups, kStepChannels);
   // A's rows are loaded once for the token rows that a block walks over
   int rows = 1;
   while (rows < 8 && (int64_t)blocks * ((a.batch + 2 * rows - 1) / (2 * rows)) >= 148 * 8) rows *= 2;
   const int parts = (a.batch + rows - 1) / rows;
   const bool svec = a.state % 4 == 0 && aligned16(a.A) && aligned16(a.pool);
-  SALT_WITH_TYPE(a.type, T, SALT_SCAN_SHAPE(a.state, S, {
+  SALT_WITH_TYPE(a.type, T, SALT_STEP_SHAPE(a.state, S, {
     selective_scan_step_kernel<T, S>
         <<<(unsigned)((int64_t)blocks * parts), S::kThreads, 0, st>>>(a, blocks, rows, svec);
   }));

@@ -5,7 +5,6 @@
 
 namespace salt {
 
-constexpr int kScanChannels = 64;  // channels of a block (fewer backward where state > 16)
 
 // A row's tokens are cut into `chunks` pieces of `chunk_len` tokens where channels and rows alone
 // leave the GPU empty.  A first pass then runs the recurrence of each chunk from zero; the second
@@ -37,6 +36,84 @@ inline int scan_blocks(int dim, int groups, int channels) {
 // s of one token and channel: softplus(delta + bias), or their sum.
 __device__ __forceinline__ float scan_step(float raw, int softplus) {
   return softplus ? softplus_f(raw) : raw;
+}
+__device__ __forceinline__ f32x2 scan_step2(f32x2 raw, int softplus) {
+  return softplus ? softplus2(raw) : raw;
+}
+
+// Calls ... with S the shape for `state` states.
+#define SALT_BY_STATE(state, S, S4, S8, S16, S32, S64, ...) \
+  do {                                                      \
+    if ((state) <= 4) {                                     \
+      using S = S4;                                         \
+      __VA_ARGS__;                                          \
+    } else if ((state) <= 8) {                              \
+      using S = S8;                                         \
+      __VA_ARGS__;                                          \
+    } else if ((state) <= 16) {                             \
+      using S = S16;                                        \
+      __VA_ARGS__;                                          \
+    } else if ((state) <= 32) {                             \
+      using S = S32;                                        \
+      __VA_ARGS__;                                          \
+    } else {                                                \
+      using S = S64;                                        \
+      __VA_ARGS__;                                          \
+    }                                                       \
+  } while (0)
+
+// How a tile's rows reach shared memory: in asynchronous copies of 16 bytes where every row starts
+// on such a boundary and no pack is cut, of 4 where it does on those, else by plain loads.
+constexpr int kCopy16 = 16, kCopy4 = 4, kCopyPlain = 0;
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* to, const void* from, bool valid) {
+  const uint32_t dst = (uint32_t)__cvta_generic_to_shared(to);
+  const int bytes = valid ? BYTES : 0;  // the rest of the BYTES is filled with zeros
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(from), "r"(bytes)
+                 : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(from), "n"(BYTES),
+                 "r"(bytes)
+                 : "memory");
+}
+__device__ __forceinline__ void copies_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int LEFT>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+
+// N neighbouring elements at `from`, of which `n` are there (none if n <= 0), into shared memory;
+// zeros behind them.
+template <int COPY, int N, typename T>
+__device__ __forceinline__ void copy_pack(T* to, const T* from, int n) {
+  if constexpr (COPY == kCopyPlain) {
+    const Pack<T, N> p = load_pack<T, N>(from, n, false);
+#pragma unroll
+    for (int i = 0; i < N; ++i) to[i] = p.v[i];
+  } else {
+    constexpr int bytes = COPY < (int)(N * sizeof(T)) ? COPY : N * sizeof(T);
+    constexpr int each = bytes / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < N; i += each) copy_async<bytes>(to + i, from + (i < n ? i : 0), i < n);
+  }
+}
+
+// Stores N values of which `n` are wanted.  WIDE: n is a multiple of N or not positive, and the
+// place is aligned.
+template <typename T, int N, bool WIDE>
+__device__ __forceinline__ void scan_store(T* p, const float* f, int n) {
+  if (!WIDE) {
+    store_pack<T, N>(p, f, n, false);
+  } else if (n > 0) {
+    Pack<T, N> r;
+#pragma unroll
+    for (int i = 0; i < N; ++i) r.v[i] = from_f32<T>(f[i]);
+    *reinterpret_cast<Pack<T, N>*>(p) = r;
+  }
 }
 
 // NS neighbouring states of `p`, those at or past `n` as zero.

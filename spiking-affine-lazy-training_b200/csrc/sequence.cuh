@@ -81,25 +81,6 @@ __device__ __forceinline__ float sigmoid(float x) {
   return __fdividef(1.f, 1.f + exp_fast(-x));
 }
 
-// log(1 + e^x) = max(x, 0) + log1p(u) with u = e^-|x| in (0, 1].  log1p keeps its relative
-// precision at small u (a step of 1e-3 is an ordinary value, and 1 + u would drop 4 of its
-// digits) through log1p(u) = 2 atanh(q), q = u / (2 + u) <= 1/3, and the series of atanh:
-// q^17 / 17 is the first term left out, under 1e-9 of q.
-__device__ __forceinline__ float softplus_f(float x) {
-  const float u = exp_fast(-fabsf(x));
-  const float q = __fdividef(u, 2.f + u), s = q * q;
-  float p = 2.f / 15.f;
-  p = fmaf(p, s, 2.f / 13.f);
-  p = fmaf(p, s, 2.f / 11.f);
-  p = fmaf(p, s, 2.f / 9.f);
-  p = fmaf(p, s, 2.f / 7.f);
-  p = fmaf(p, s, 2.f / 5.f);
-  p = fmaf(p, s, 2.f / 3.f);
-  p = fmaf(p, s, 2.f);
-  // fmaxf drops a NaN; u keeps it
-  return fmaf(p, q, fmaxf(x, 0.f));
-}
-
 // d/dx of x * sigmoid(x).
 __device__ __forceinline__ float silu_slope(float x, float p) { return p * fmaf(x, 1.f - p, 1.f); }
 
@@ -113,6 +94,70 @@ __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
+}
+
+// Two float32 side by side: one instruction does both.
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pair(float lo, float hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 halves(f32x2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 exp2_fast2(f32x2 v) {
+  const float2 h = halves(v);
+  return pair(exp2_fast(h.x), exp2_fast(h.y));
+}
+
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// log(1 + e^x) = max(x, 0) + log1p(u) with u = e^-|x| in (0, 1].  log1p keeps its relative
+// precision at small u (a step of 1e-3 is an ordinary value, and 1 + u would drop 4 of its
+// digits) through log1p(u) = 2 atanh(q), q = u / (2 + u) <= 1/3: 2 atanh(q) / q is interpolated at
+// the Chebyshev nodes of q^2 in [0, 1/9] by a polynomial of degree 4, within 8e-9 of itself.  A NaN
+// stays one: fmaxf drops it, u keeps it.
+__device__ __forceinline__ f32x2 softplus2(f32x2 x) {
+  const float2 v = halves(x);
+  const f32x2 u = pair(exp2_fast(fabsf(v.x) * -kLog2e), exp2_fast(fabsf(v.y) * -kLog2e));
+  const float2 w = halves(add2(u, pair(2.f, 2.f)));
+  const f32x2 q = mul2(u, pair(rcp_fast(w.x), rcp_fast(w.y))), s = mul2(q, q);
+  f32x2 p = pair(0.2815778f, 0.2815778f);
+  p = fma2(p, s, pair(0.27965158f, 0.27965158f));
+  p = fma2(p, s, pair(0.40024596f, 0.40024596f));
+  p = fma2(p, s, pair(0.6666632f, 0.6666632f));
+  p = fma2(p, s, pair(2.f, 2.f));
+  return fma2(p, q, pair(fmaxf(v.x, 0.f), fmaxf(v.y, 0.f)));
+}
+__device__ __forceinline__ float softplus_f(float x) { return halves(softplus2(pair(x, x))).x; }
+
+// 1 / (1 + e^-x) of both.
+__device__ __forceinline__ f32x2 sigmoid2(f32x2 x) {
+  const f32x2 e = exp2_fast2(mul2(x, pair(-kLog2e, -kLog2e)));
+  const float2 d = halves(add2(e, pair(1.f, 1.f)));
+  return pair(rcp_fast(d.x), rcp_fast(d.y));
 }
 
 // Launches (argument checks are the caller's; each returns the launch's status).
@@ -144,6 +189,11 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 // Whether rows at p with these strides (in elements) start on 16-byte boundaries.
 inline bool vec_rows(const void* p, size_t size, int64_t s0, int64_t s1 = 0) {
   return !p || (aligned16(p) && (s0 * size) % 16 == 0 && (s1 * size) % 16 == 0);
+}
+// The same for boundaries of `bytes`.
+inline bool packed_rows(const void* p, int64_t bytes, size_t size, int64_t s0, int64_t s1) {
+  return reinterpret_cast<uintptr_t>(p) % bytes == 0 && (int64_t)(s0 * size) % bytes == 0 &&
+         (int64_t)(s1 * size) % bytes == 0;
 }
 inline size_t type_size(int32_t type) { return type == SALT_F32 ? 4 : 2; }
 

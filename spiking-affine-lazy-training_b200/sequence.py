@@ -21,6 +21,9 @@ allocated until the call's work is done.
 from __future__ import annotations
 
 import ctypes
+import functools
+import math
+import struct
 from typing import NamedTuple
 
 import numpy as np
@@ -37,7 +40,6 @@ _NUMPY = {_F32: np.dtype(np.float32), _F16: np.dtype(np.float16), _BF16: bfloat1
 _NAMES = ("float32", "float16", "bfloat16", "int32", "float8_e4m3")
 _TYPE_IDS = {v: k for k, v in _NUMPY.items()}
 _ACTIVATIONS = (_F32, _F16, _BF16)
-_INT = ctypes.c_size_t
 
 
 class NormOutput(NamedTuple):
@@ -95,92 +97,107 @@ def _type_of(a, name: str) -> int:
     return got
 
 
-class _Call:
-    """One call's arrays: every pointer that is taken has been checked for shape, type, layout and
-    device."""
-    __slots__ = ("device",)
+# The checks of an array come in two forms.  A call on small inputs costs the host more time than
+# the GPU, so each array first goes through one chain of comparisons that ends in its pointer;
+# whatever fails there (an unusual layout, or a mistake) goes through `_look`, which decides and
+# words the error.
 
-    def __init__(self):
-        self.device = None
+def _activation(a, name: str) -> int:
+    if not hasattr(a, "data_ptr"):
+        raise TypeError(f"{name}: needs a device array, got {type(a).__name__}")
+    t = _type_of(a, name)
+    if t not in _ACTIVATIONS:
+        raise TypeError(f"{name}: activations are float32, float16 or bfloat16")
+    return t
 
-    def type(self, a, name: str) -> int:
-        if not hasattr(a, "data_ptr"):
-            raise TypeError(f"{name}: needs a device array, got {type(a).__name__}")
-        t = _type_of(a, name)
-        if t not in _ACTIVATIONS:
-            raise TypeError(f"{name}: activations are float32, float16 or bfloat16")
-        return t
 
-    def _pointer(self, a, name: str) -> int:
-        where = getattr(a, "get_device", None)
-        if where is not None:
-            d = where()
-            if d != self.device:
-                if self.device is None:
-                    self.device = current_device()
-                if d != self.device:
-                    raise ValueError(f"{name}: not on the current device ({self.device})")
+def _look(a, name: str, shape: tuple, type_id: int, inner: int) -> None:
+    """Raises unless `a` is an array of that shape and type on the current device whose last
+    `inner` axes are contiguous (an axis of length 1 has any stride)."""
+    if not hasattr(a, "data_ptr"):
+        raise TypeError(f"{name}: needs a device array, got {type(a).__name__}")
+    if tuple(a.shape) != shape:
+        raise ValueError(f"{name}: shape {tuple(a.shape)}, expected {shape}")
+    got = _type_of(a, name)
+    if got != type_id:
+        raise TypeError(f"{name}: {_NAMES[got]}, expected {_NAMES[type_id]}")
+    at = 1
+    for n, s in list(zip(reversed(shape), reversed(a.stride())))[:inner]:
+        if n != 1 and s != at and 0 not in shape:
+            raise ValueError(f"{name}: must be contiguous" if inner == len(shape) else
+                             f"{name}: its last {inner} axes must be contiguous")
+        at *= n
+    where = getattr(a, "get_device", None)
+    if where is not None and where() != current_device():
+        raise ValueError(f"{name}: not on the current device ({current_device()})")
+
+
+def _here() -> int:
+    """The current device, -1 where there is none (the library then says so)."""
+    d = ctypes.c_int32(-1)
+    return d.value if _lib.lib().salt_get_device(ctypes.byref(d)) == _lib.SALT_OK else -1
+
+
+@functools.lru_cache(maxsize=4096)
+def _dense(shape: tuple) -> tuple:
+    return DeviceArray(0, shape, np.uint8, None).stride()
+
+
+def _whole(here: int, a, name: str, shape: tuple, type_id: int) -> int:
+    """Pointer of a contiguous array on device `here`; 0 for None."""
+    if a is None:
+        return 0
+    if type(a) is DeviceArray:
+        if a.shape == shape and _TYPE_IDS.get(a.dtype) == type_id:
+            return a.ptr
+    elif hasattr(a, "get_device") and a.shape == shape and _TYPE_IDS.get(a.dtype) == type_id \
+            and a.stride() == _dense(shape) and a.get_device() == here:
         return a.data_ptr()
+    _look(a, name, shape, type_id, len(shape))
+    return a.data_ptr()
 
-    def _check(self, a, name: str, shape: tuple, type_id: int) -> None:
-        if not hasattr(a, "data_ptr"):
-            raise TypeError(f"{name}: needs a device array, got {type(a).__name__}")
-        if a.shape != shape:
-            raise ValueError(f"{name}: shape {tuple(a.shape)}, expected {shape}")
-        if _type_of(a, name) != type_id:
-            raise TypeError(f"{name}: {_NAMES[_type_of(a, name)]}, expected {_NAMES[type_id]}")
 
-    def whole(self, a, name: str, shape: tuple, type_id: int):
-        """Pointer of a contiguous array, None for None."""
-        if a is None:
-            return None
-        self._check(a, name, shape, type_id)
-        if not isinstance(a, DeviceArray):
-            at = 1
-            for n, s in zip(reversed(shape), reversed(a.stride())):
-                if n != 1 and s != at and 0 not in shape:
-                    raise ValueError(f"{name}: must be contiguous")
-                at *= n
-        return self._pointer(a, name)
+def _rows(here: int, a, name: str, shape: tuple, type_id: int, inner: int = 1):
+    """(pointer, strides of the leading axes) of an array whose last `inner` axes are contiguous;
+    (0, zeros) for None."""
+    if a is None:
+        return 0, (0,) * (len(shape) - inner)
+    if type(a) is DeviceArray:
+        if a.shape == shape and _TYPE_IDS.get(a.dtype) == type_id:
+            return a.ptr, _dense(shape)[:-inner]
+    elif hasattr(a, "get_device") and a.shape == shape and _TYPE_IDS.get(a.dtype) == type_id:
+        s = a.stride()
+        if s[-1] == 1 and (inner == 1 or s[-2] == shape[-1]) and a.get_device() == here:
+            return a.data_ptr(), s[:-inner]
+    _look(a, name, shape, type_id, inner)
+    return a.data_ptr(), tuple(a.stride())[:-inner]
 
-    def weight(self, a, name: str, shape: tuple, type_id: int):
-        """(pointer, type) of a contiguous weight of type_id or float32."""
-        if a is None:
-            return None, type_id
-        got = _type_of(a, name) if hasattr(a, "data_ptr") else type_id
-        return self.whole(a, name, shape, _F32 if got == _F32 else type_id), got
 
-    def rows(self, a, name: str, shape: tuple, type_id: int, inner: int = 1):
-        """(pointer, strides of the leading axes) of an array whose last `inner` axes are
-        contiguous; (None, zeros) for None."""
-        lead = len(shape) - inner
-        if a is None:
-            return None, (0,) * lead
-        self._check(a, name, shape, type_id)
-        strides = a.stride()
-        at = 1
-        for n, s in zip(reversed(shape[lead:]), reversed(strides[lead:])):
-            if n != 1 and s != at:
-                raise ValueError(f"{name}: its last {inner} axes must be contiguous"
-                                 if inner > 1 else f"{name}: channels must be contiguous")
-            at *= n
-        return self._pointer(a, name), strides[:lead]
+def _weight(here: int, a, name: str, shape: tuple, type_id: int):
+    """(pointer, type) of a contiguous weight of type_id or float32."""
+    if a is None:
+        return 0, type_id
+    got = _F32 if hasattr(a, "data_ptr") and _type_of(a, name) == _F32 else type_id
+    return _whole(here, a, name, shape, got), got
 
-    def flat(self, a, name: str, shape: tuple, type_id: int):
-        """(pointer, row stride) of an array whose leading axes fold into one axis of rows."""
-        if a is None:
-            return None, 0
-        p, strides = self.rows(a, name, shape, type_id)
-        stride, span = shape[-1], None
-        for n, s in zip(reversed(shape[:-1]), reversed(strides)):
-            if n == 1:
-                continue
-            if span is None:
-                stride = s
-            elif s != span and 0 not in shape:
-                raise ValueError(f"{name}: its leading axes do not fold into rows of one stride")
-            span = s * n
-        return p, stride
+
+def _flat(here: int, a, name: str, shape: tuple, type_id: int):
+    """(pointer, row stride) of an array whose leading axes fold into one axis of rows."""
+    if a is None:
+        return 0, 0
+    p, strides = _rows(here, a, name, shape, type_id)
+    if len(shape) == 2:
+        return p, strides[0]
+    stride, span = shape[-1], None
+    for n, s in zip(reversed(shape[:-1]), reversed(strides)):
+        if n == 1:
+            continue
+        if span is None:
+            stride = s
+        elif s != span and 0 not in shape:
+            raise ValueError(f"{name}: its leading axes do not fold into rows of one stride")
+        span = s * n
+    return p, stride
 
 
 def _wanted(a, shape, type_id):
@@ -201,24 +218,48 @@ def _axes(a, name: str, n: int) -> tuple:
     return shape
 
 
-def _work(query, args):
-    """(buffer, bytes) that the matching *_workspace_size asks for."""
-    n = _INT(0)
-    _lib.check(query(ctypes.byref(args), ctypes.byref(n)))
+def _row_count(shape: tuple, name: str) -> int:
+    if not shape:
+        raise ValueError(f"{name}: needs at least one axis")
+    return math.prod(shape[:-1])
+
+
+def _packer(struct_type) -> struct.Struct:
+    """Packs the fields of an argument struct, in order, into its bytes (integers, floats and
+    pointers as integers): a third of the time of filling the ctypes structure."""
+    codes = {ctypes.c_int32: "i", ctypes.c_int64: "q", ctypes.c_float: "f", ctypes.c_void_p: "P"}
+    pack = struct.Struct("@" + "".join(codes[t] for _, t in struct_type._fields_))
+    assert pack.size == ctypes.sizeof(struct_type)
+    return pack.pack
+
+
+_pack_norm = _packer(_lib.RmsNormArgs)
+_pack_norm_backward = _packer(_lib.RmsNormBackwardArgs)
+_pack_conv = _packer(_lib.CausalConvArgs)
+_pack_conv_step = _packer(_lib.CausalConvStepArgs)
+_pack_conv_backward = _packer(_lib.CausalConvBackwardArgs)
+_pack_scan = _packer(_lib.SelectiveScanArgs)
+_pack_scan_step = _packer(_lib.SelectiveScanStepArgs)
+_pack_scan_backward = _packer(_lib.SelectiveScanBackwardArgs)
+
+
+def _work(query, args: bytes):
+    """(buffer or None, its pointer, bytes) that the matching *_workspace_size asks for."""
+    n = ctypes.c_size_t(0)
+    _lib.check(query(args, ctypes.byref(n)))
     if n.value == 0:
-        return None, 0
-    return workspace(n.value), n.value
+        return None, None, 0
+    ws = workspace(n.value)
+    return ws, ws.ptr, n.value
 
 
 # ---------------------------------------------------------------- root-mean-square norm
 
 def _norm(x, weight, residual, eps, out, residual_out, rstd, scale, group):
-    c = _Call()
-    t = c.type(x, "x")
+    here = _here()
+    t = _activation(x, "x")
     shape = tuple(x.shape)
-    if not shape:
-        raise ValueError("x: needs at least one axis")
-    rows, dim = int(np.prod(shape[:-1], dtype=np.int64)), shape[-1]
+    rows, dim = _row_count(shape, "x"), shape[-1]
     wide = t if residual is None else _type_of(residual, "residual")
     if residual is None and residual_out is not None and residual_out is not True \
             and residual_out is not False:
@@ -228,19 +269,20 @@ def _norm(x, weight, residual, eps, out, residual_out, rstd, scale, group):
     out = _made(out, shape, _E4M3 if group is not None else t)
     residual_out = _wanted(residual_out, shape, wide)
     rstd = _wanted(rstd, shape[:-1], _F32)
-    ps = None
+    ps = 0
     if group is not None:
         parts = (-(-dim // group) if group else 1,)
         scale = _made(scale, shape[:-1] + parts, _F32)
-        ps = c.whole(scale, "scale", shape[:-1] + parts, _F32)
-    pw, wt = c.weight(weight, "weight", (dim,), t)
-    px, sx = c.flat(x, "x", shape, t)
-    pr, sr = c.flat(residual, "residual", shape, wide)
-    po, so = c.flat(out, "out", shape, t if group is None else _E4M3)
-    pro, sro = c.flat(residual_out, "residual_out", shape, wide)
-    args = _lib.RmsNormArgs(rows, dim, t, wide, wt, group or 0, eps, sx, sr, so, sro, px, pr, pw,
-                            po, pro, c.whole(rstd, "rstd", shape[:-1], _F32), ps)
-    _lib.check(_lib.lib().salt_rms_norm(ctypes.byref(args), stream_handle()))
+        ps = _whole(here, scale, "scale", shape[:-1] + parts, _F32)
+    pw, wt = _weight(here, weight, "weight", (dim,), t)
+    px, sx = _flat(here, x, "x", shape, t)
+    pr, sr = _flat(here, residual, "residual", shape, wide)
+    po, so = _flat(here, out, "out", shape, t if group is None else _E4M3)
+    pro, sro = _flat(here, residual_out, "residual_out", shape, wide)
+    args = _pack_norm(
+        rows, dim, t, wide, wt, group or 0, eps, sx, sr, so, sro, px, pr, pw, po, pro,
+        _whole(here, rstd, "rstd", shape[:-1], _F32), ps)
+    _lib.check(_lib.lib().salt_rms_norm(args, stream_handle()))
     return NormOutput(out, residual_out, rstd, scale)
 
 
@@ -268,27 +310,26 @@ def rms_norm_backward(dy, x, weight, rstd, *, dresidual=None, dx=None, dweight=N
     no residual), rstd its factors, dresidual the gradient that reaches `residual_out` from
     elsewhere.  dx, the gradient of the input and of the residual alike, holds x's type (it may be
     `dresidual`); dweight (float32) is made unless given, and left out for False."""
-    c = _Call()
-    t, wide = c.type(dy, "dy"), c.type(x, "x")
+    here = _here()
+    t, wide = _activation(dy, "dy"), _activation(x, "x")
     if wide not in (t, _F32):
         raise TypeError("x: must hold dy's type or float32")
     shape = tuple(dy.shape)
-    if not shape:
-        raise ValueError("dy: needs at least one axis")
-    rows, dim = int(np.prod(shape[:-1], dtype=np.int64)), shape[-1]
+    rows, dim = _row_count(shape, "dy"), shape[-1]
     dx = _made(dx, shape, wide)
     dweight = _wanted(True if dweight is None else dweight, (dim,), _F32)
-    pdy, sdy = c.flat(dy, "dy", shape, t)
-    px, sx = c.flat(x, "x", shape, wide)
-    pr, sr = c.flat(dresidual, "dresidual", shape, wide)
-    pdx, sdx = c.flat(dx, "dx", shape, wide)
-    pw, wt = c.weight(weight, "weight", (dim,), t)
-    args = _lib.RmsNormBackwardArgs(rows, dim, t, wide, wt, 0, sdy, sx, sr, sdx, pdy, px, pw,
-                                    c.whole(rstd, "rstd", shape[:-1], _F32), pr, pdx,
-                                    c.whole(dweight, "dweight", (dim,), _F32))
+    pdy, sdy = _flat(here, dy, "dy", shape, t)
+    px, sx = _flat(here, x, "x", shape, wide)
+    pr, sr = _flat(here, dresidual, "dresidual", shape, wide)
+    pdx, sdx = _flat(here, dx, "dx", shape, wide)
+    pw, wt = _weight(here, weight, "weight", (dim,), t)
+    args = _pack_norm_backward(
+        rows, dim, t, wide, wt, 0, sdy, sx, sr, sdx, pdy, px, pw,
+        _whole(here, rstd, "rstd", shape[:-1], _F32), pr, pdx,
+        _whole(here, dweight, "dweight", (dim,), _F32))
     lib = _lib.lib()
-    ws, n = _work(lib.salt_rms_norm_backward_workspace_size, args)
-    _lib.check(lib.salt_rms_norm_backward(ctypes.byref(args), ws and ws.ptr, n, stream_handle()))
+    ws, at, n = _work(lib.salt_rms_norm_backward_workspace_size, args)
+    _lib.check(lib.salt_rms_norm_backward(args, at, n, stream_handle()))
     return NormGradients(dx, dweight)
 
 
@@ -301,21 +342,21 @@ def causal_conv(x, weight, bias=None, *, n_real=None, initial_state=None, silu: 
     (batch, int32) ends each row early: what lies past it is not read and comes back as zero.
     initial_state (batch, dim, width - 1) holds the inputs in front of the row, oldest first;
     final_state takes the last ones (and may be initial_state)."""
-    c = _Call()
-    t = c.type(x, "x")
+    here = _here()
+    t = _activation(x, "x")
     batch, n, dim = shape = _axes(x, "x", 3)
     width = _axes(weight, "weight", 2)[1]
     edge = (batch, dim, width - 1)
     out, final_state = _made(out, shape, t), _wanted(final_state, edge, t)
-    pw, wt = c.weight(weight, "weight", (dim, width), t)
-    px, sx = c.rows(x, "x", shape, t)
-    po, so = c.rows(out, "out", shape, t)
-    args = _lib.CausalConvArgs(batch, n, dim, width, t, wt, bool(silu), 0, *sx, *so, px, pw,
-                               c.whole(bias, "bias", (dim,), wt),
-                               c.whole(n_real, "n_real", (batch,), _I32),
-                               c.whole(initial_state, "initial_state", edge, t), po,
-                               c.whole(final_state, "final_state", edge, t))
-    _lib.check(_lib.lib().salt_causal_conv(ctypes.byref(args), stream_handle()))
+    pw, wt = _weight(here, weight, "weight", (dim, width), t)
+    px, sx = _rows(here, x, "x", shape, t)
+    po, so = _rows(here, out, "out", shape, t)
+    args = _pack_conv(
+        batch, n, dim, width, t, wt, bool(silu), 0, *sx, *so, px, pw,
+        _whole(here, bias, "bias", (dim,), wt), _whole(here, n_real, "n_real", (batch,), _I32),
+        _whole(here, initial_state, "initial_state", edge, t), po,
+        _whole(here, final_state, "final_state", edge, t))
+    _lib.check(_lib.lib().salt_causal_conv(args, stream_handle()))
     return ConvOutput(out, final_state)
 
 
@@ -324,20 +365,20 @@ def causal_conv_step(x, state, weight, bias=None, *, slots=None, silu: bool = Tr
     """One token x (batch, dim) for each row: row b shifts it into state[slots[b]] of a pool
     (n_slots, dim, width - 1), in place.  Without slots row b is slot b.  A slot outside the pool
     marks an empty row (its out is zero); no slot may appear twice."""
-    c = _Call()
-    t = c.type(x, "x")
+    here = _here()
+    t = _activation(x, "x")
     batch, dim = shape = _axes(x, "x", 2)
     width = _axes(weight, "weight", 2)[1]
     n_slots = _axes(state, "state", 3)[0]
     out = _made(out, shape, t)
-    pw, wt = c.weight(weight, "weight", (dim, width), t)
-    px, sx = c.rows(x, "x", shape, t)
-    po, so = c.rows(out, "out", shape, t)
-    args = _lib.CausalConvStepArgs(batch, dim, width, n_slots, t, wt, bool(silu), 0, *sx, *so, px,
-                                   pw, c.whole(bias, "bias", (dim,), wt),
-                                   c.whole(slots, "slots", (batch,), _I32),
-                                   c.whole(state, "state", (n_slots, dim, width - 1), t), po)
-    _lib.check(_lib.lib().salt_causal_conv_step(ctypes.byref(args), stream_handle()))
+    pw, wt = _weight(here, weight, "weight", (dim, width), t)
+    px, sx = _rows(here, x, "x", shape, t)
+    po, so = _rows(here, out, "out", shape, t)
+    args = _pack_conv_step(
+        batch, dim, width, n_slots, t, wt, bool(silu), 0, *sx, *so, px, pw,
+        _whole(here, bias, "bias", (dim,), wt), _whole(here, slots, "slots", (batch,), _I32),
+        _whole(here, state, "state", (n_slots, dim, width - 1), t), po)
+    _lib.check(_lib.lib().salt_causal_conv_step(args, stream_handle()))
     return ConvOutput(out, state)
 
 
@@ -347,28 +388,28 @@ def causal_conv_backward(dy, x, weight, bias=None, *, n_real=None, initial_state
     """Gradients of `causal_conv` for dy, the gradient of its out.  dweight and dbias are float32
     (dbias is made where there is a bias); dinitial (batch, dim, width - 1) holds x's type and is
     optional."""
-    c = _Call()
-    t = c.type(x, "x")
+    here = _here()
+    t = _activation(x, "x")
     batch, n, dim = shape = _axes(x, "x", 3)
     width = _axes(weight, "weight", 2)[1]
     edge = (batch, dim, width - 1)
     dx, dweight = _made(dx, shape, t), _made(dweight, (dim, width), _F32)
     dbias = _wanted(bias is not None if dbias is None else dbias, (dim,), _F32)
     dinitial = _wanted(dinitial, edge, t)
-    pw, wt = c.weight(weight, "weight", (dim, width), t)
-    pdy, sdy = c.rows(dy, "dy", shape, t)
-    px, sx = c.rows(x, "x", shape, t)
-    pdx, sdx = c.rows(dx, "dx", shape, t)
-    args = _lib.CausalConvBackwardArgs(
+    pw, wt = _weight(here, weight, "weight", (dim, width), t)
+    pdy, sdy = _rows(here, dy, "dy", shape, t)
+    px, sx = _rows(here, x, "x", shape, t)
+    pdx, sdx = _rows(here, dx, "dx", shape, t)
+    args = _pack_conv_backward(
         batch, n, dim, width, t, wt, bool(silu), 0, *sdy, *sx, *sdx, pdy, px, pw,
-        c.whole(bias, "bias", (dim,), wt), c.whole(n_real, "n_real", (batch,), _I32),
-        c.whole(initial_state, "initial_state", edge, t), pdx,
-        c.whole(dinitial, "dinitial", edge, t), c.whole(dweight, "dweight", (dim, width), _F32),
-        c.whole(dbias, "dbias", (dim,), _F32))
+        _whole(here, bias, "bias", (dim,), wt), _whole(here, n_real, "n_real", (batch,), _I32),
+        _whole(here, initial_state, "initial_state", edge, t), pdx,
+        _whole(here, dinitial, "dinitial", edge, t),
+        _whole(here, dweight, "dweight", (dim, width), _F32),
+        _whole(here, dbias, "dbias", (dim,), _F32))
     lib = _lib.lib()
-    ws, size = _work(lib.salt_causal_conv_backward_workspace_size, args)
-    _lib.check(lib.salt_causal_conv_backward(ctypes.byref(args), ws and ws.ptr, size,
-                                             stream_handle()))
+    ws, at, size = _work(lib.salt_causal_conv_backward_workspace_size, args)
+    _lib.check(lib.salt_causal_conv_backward(args, at, size, stream_handle()))
     return ConvGradients(dx, dweight, dbias, dinitial)
 
 
@@ -390,31 +431,31 @@ def selective_scan(x, delta, A, B, C, *, D=None, z=None, delta_bias=None, softpl
     ``d // (dim / groups)``; D, delta_bias: (dim,) float32.  n_real (batch, int32) ends each row
     early.  initial_state and final_state: (batch, dim, state) float32, may be one array.
     checkpoints takes the states that `selective_scan_backward` starts from."""
-    c = _Call()
-    t = c.type(x, "x")
+    here = _here()
+    t = _activation(x, "x")
     batch, n, dim = shape = _axes(x, "x", 3)
     groups, state = _axes(B, "B", 4)[2:]
     both, ends = (batch, n, groups, state), (batch, dim, state)
     marks = _checkpoint_shape(batch, n, dim, state)
     out, final_state = _made(out, shape, t), _wanted(final_state, ends, _F32)
     checkpoints = _wanted(checkpoints, marks, _F32)
-    px, sx = c.rows(x, "x", shape, t)
-    pd, sd = c.rows(delta, "delta", shape, t)
-    pz, sz = c.rows(z, "z", shape, t)
-    pb, sb = c.rows(B, "B", both, t, 2)
-    pc, sc = c.rows(C, "C", both, t, 2)
-    po, so = c.rows(out, "out", shape, t)
-    args = _lib.SelectiveScanArgs(
+    px, sx = _rows(here, x, "x", shape, t)
+    pd, sd = _rows(here, delta, "delta", shape, t)
+    pz, sz = _rows(here, z, "z", shape, t)
+    pb, sb = _rows(here, B, "B", both, t, 2)
+    pc, sc = _rows(here, C, "C", both, t, 2)
+    po, so = _rows(here, out, "out", shape, t)
+    args = _pack_scan(
         batch, n, dim, state, groups, t, bool(softplus), 0, *sx, *sd, *sz, *sb, *sc, *so, px, pd,
-        pz, pb, pc, c.whole(A, "A", (dim, state), _F32), c.whole(D, "D", (dim,), _F32),
-        c.whole(delta_bias, "delta_bias", (dim,), _F32),
-        c.whole(n_real, "n_real", (batch,), _I32),
-        c.whole(initial_state, "initial_state", ends, _F32), po,
-        c.whole(final_state, "final_state", ends, _F32),
-        c.whole(checkpoints, "checkpoints", marks, _F32))
+        pz, pb, pc, _whole(here, A, "A", (dim, state), _F32), _whole(here, D, "D", (dim,), _F32),
+        _whole(here, delta_bias, "delta_bias", (dim,), _F32),
+        _whole(here, n_real, "n_real", (batch,), _I32),
+        _whole(here, initial_state, "initial_state", ends, _F32), po,
+        _whole(here, final_state, "final_state", ends, _F32),
+        _whole(here, checkpoints, "checkpoints", marks, _F32))
     lib = _lib.lib()
-    ws, size = _work(lib.salt_selective_scan_workspace_size, args)
-    _lib.check(lib.salt_selective_scan(ctypes.byref(args), ws and ws.ptr, size, stream_handle()))
+    ws, at, size = _work(lib.salt_selective_scan_workspace_size, args)
+    _lib.check(lib.salt_selective_scan(args, at, size, stream_handle()))
     return ScanOutput(out, final_state, checkpoints)
 
 
@@ -423,25 +464,26 @@ def selective_scan_step(pool, x, delta, A, B, C, *, D=None, z=None, delta_bias=N
     """One token of `selective_scan` for each row, x, delta, z (batch, dim) and B, C (batch,
     groups, state), on pool[slots[b]] of float32 states (n_slots, dim, state), in place; slots as in
     `causal_conv_step`."""
-    c = _Call()
-    t = c.type(x, "x")
+    here = _here()
+    t = _activation(x, "x")
     batch, dim = shape = _axes(x, "x", 2)
     groups, state = _axes(B, "B", 3)[1:]
     n_slots = _axes(pool, "pool", 3)[0]
     both = (batch, groups, state)
     out = _made(out, shape, t)
-    px, (sx,) = c.rows(x, "x", shape, t)
-    pd, (sd,) = c.rows(delta, "delta", shape, t)
-    pz, (sz,) = c.rows(z, "z", shape, t)
-    pb, (sb,) = c.rows(B, "B", both, t, 2)
-    pc, (sc,) = c.rows(C, "C", both, t, 2)
-    po, (so,) = c.rows(out, "out", shape, t)
-    args = _lib.SelectiveScanStepArgs(
+    px, (sx,) = _rows(here, x, "x", shape, t)
+    pd, (sd,) = _rows(here, delta, "delta", shape, t)
+    pz, (sz,) = _rows(here, z, "z", shape, t)
+    pb, (sb,) = _rows(here, B, "B", both, t, 2)
+    pc, (sc,) = _rows(here, C, "C", both, t, 2)
+    po, (so,) = _rows(here, out, "out", shape, t)
+    args = _pack_scan_step(
         batch, dim, state, groups, n_slots, t, bool(softplus), 0, sx, sd, sz, sb, sc, so, px, pd,
-        pz, pb, pc, c.whole(A, "A", (dim, state), _F32), c.whole(D, "D", (dim,), _F32),
-        c.whole(delta_bias, "delta_bias", (dim,), _F32), c.whole(slots, "slots", (batch,), _I32),
-        c.whole(pool, "pool", (n_slots, dim, state), _F32), po)
-    _lib.check(_lib.lib().salt_selective_scan_step(ctypes.byref(args), stream_handle()))
+        pz, pb, pc, _whole(here, A, "A", (dim, state), _F32), _whole(here, D, "D", (dim,), _F32),
+        _whole(here, delta_bias, "delta_bias", (dim,), _F32),
+        _whole(here, slots, "slots", (batch,), _I32),
+        _whole(here, pool, "pool", (n_slots, dim, state), _F32), po)
+    _lib.check(_lib.lib().salt_selective_scan_step(args, stream_handle()))
     return ScanOutput(out, pool)
 
 
@@ -453,8 +495,8 @@ def selective_scan_backward(dy, x, delta, A, B, C, *, checkpoints, D=None, z=Non
     state, from the forward's arguments and checkpoints.  dA, dD, ddelta_bias and dinitial are
     float32, the others hold x's type; dD, dz and ddelta_bias are made where their input is given,
     dinitial is optional."""
-    c = _Call()
-    t = c.type(x, "x")
+    here = _here()
+    t = _activation(x, "x")
     batch, n, dim = shape = _axes(x, "x", 3)
     groups, state = _axes(B, "B", 4)[2:]
     both, ends = (batch, n, groups, state), (batch, dim, state)
@@ -464,28 +506,28 @@ def selective_scan_backward(dy, x, delta, A, B, C, *, checkpoints, D=None, z=Non
     dz = None if z is None else _made(dz, shape, t)
     ddelta_bias = None if delta_bias is None else _made(ddelta_bias, (dim,), _F32)
     dinitial = _wanted(dinitial, ends, _F32)
-    px, sx = c.rows(x, "x", shape, t)
-    pd, sd = c.rows(delta, "delta", shape, t)
-    pz, sz = c.rows(z, "z", shape, t)
-    pb, sb = c.rows(B, "B", both, t, 2)
-    pc, sc = c.rows(C, "C", both, t, 2)
-    pdy, sdy = c.rows(dy, "dy", shape, t)
-    pdx, sdx = c.rows(dx, "dx", shape, t)
-    pdd, sdd = c.rows(ddelta, "ddelta", shape, t)
-    pdz, sdz = c.rows(dz, "dz", shape, t)
+    px, sx = _rows(here, x, "x", shape, t)
+    pd, sd = _rows(here, delta, "delta", shape, t)
+    pz, sz = _rows(here, z, "z", shape, t)
+    pb, sb = _rows(here, B, "B", both, t, 2)
+    pc, sc = _rows(here, C, "C", both, t, 2)
+    pdy, sdy = _rows(here, dy, "dy", shape, t)
+    pdx, sdx = _rows(here, dx, "dx", shape, t)
+    pdd, sdd = _rows(here, ddelta, "ddelta", shape, t)
+    pdz, sdz = _rows(here, dz, "dz", shape, t)
     marks = _checkpoint_shape(batch, n, dim, state)
-    args = _lib.SelectiveScanBackwardArgs(
+    args = _pack_scan_backward(
         batch, n, dim, state, groups, t, bool(softplus), 0, *sx, *sd, *sz, *sb, *sc, *sdy, *sdx,
-        *sdd, *sdz, px, pd, pz, pb, pc, pdy, c.whole(A, "A", (dim, state), _F32),
-        c.whole(D, "D", (dim,), _F32), c.whole(delta_bias, "delta_bias", (dim,), _F32),
-        c.whole(n_real, "n_real", (batch,), _I32),
-        c.whole(checkpoints, "checkpoints", marks, _F32),
-        c.whole(dfinal, "dfinal", ends, _F32), pdx, pdd, pdz, c.whole(dB, "dB", both, t),
-        c.whole(dC, "dC", both, t), c.whole(dA, "dA", (dim, state), _F32),
-        c.whole(dD, "dD", (dim,), _F32), c.whole(ddelta_bias, "ddelta_bias", (dim,), _F32),
-        c.whole(dinitial, "dinitial", ends, _F32))
+        *sdd, *sdz, px, pd, pz, pb, pc, pdy, _whole(here, A, "A", (dim, state), _F32),
+        _whole(here, D, "D", (dim,), _F32), _whole(here, delta_bias, "delta_bias", (dim,), _F32),
+        _whole(here, n_real, "n_real", (batch,), _I32),
+        _whole(here, checkpoints, "checkpoints", marks, _F32),
+        _whole(here, dfinal, "dfinal", ends, _F32), pdx, pdd, pdz, _whole(here, dB, "dB", both, t),
+        _whole(here, dC, "dC", both, t), _whole(here, dA, "dA", (dim, state), _F32),
+        _whole(here, dD, "dD", (dim,), _F32),
+        _whole(here, ddelta_bias, "ddelta_bias", (dim,), _F32),
+        _whole(here, dinitial, "dinitial", ends, _F32))
     lib = _lib.lib()
-    ws, size = _work(lib.salt_selective_scan_backward_workspace_size, args)
-    _lib.check(lib.salt_selective_scan_backward(ctypes.byref(args), ws and ws.ptr, size,
-                                                stream_handle()))
+    ws, at, size = _work(lib.salt_selective_scan_backward_workspace_size, args)
+    _lib.check(lib.salt_selective_scan_backward(args, at, size, stream_handle()))
     return ScanGradients(dx, ddelta, dA, dB, dC, dD, dz, ddelta_bias, dinitial)
