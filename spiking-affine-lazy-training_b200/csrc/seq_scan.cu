@@ -45,7 +45,6 @@ struct ScanShared {
   alignas(16) float B[S::kTile][S::kStates];
   alignas(16) float C[FULL ? S::kTile : 1][S::kStates];
   alignas(8) float y[FULL ? S::kTile : 1][S::kYPitch];
-  alignas(8) float bias[S::kChannels], skip[S::kChannels];
 };
 
 // The state in front of chunk c, from the first pass's results.
@@ -135,9 +134,15 @@ selective_scan_kernel(salt_selective_scan_args a, ScanSplit sp, int blocks, bool
   T* out = static_cast<T*>(a.out) + b * a.out_batch_stride + io_d;
   const T* B = static_cast<const T*>(a.B) + b * a.B_batch_stride + (int64_t)cb.group * a.state;
   const T* C = static_cast<const T*>(a.C) + b * a.C_batch_stride + (int64_t)cb.group * a.state;
-  for (int i = tid; i < S::kChannels; i += S::kThreads) {
-    sm.bias[i] = a.delta_bias && i < cb.n ? a.delta_bias[cb.d0 + i] : 0.f;
-    sm.skip[i] = a.D && i < cb.n ? a.D[cb.d0 + i] : 0.f;
+  f32x2 bias[kVec / 2], skip[kVec / 2];
+#pragma unroll
+  for (int k = 0; k < kVec; k += 2) {
+    const bool one = k < io_n, two = k + 1 < io_n;
+    bias[k / 2] = a.delta_bias ? pair(one ? a.delta_bias[io_d + k] : 0.f,
+                                      two ? a.delta_bias[io_d + k + 1] : 0.f)
+                               : 0;
+    skip[k / 2] =
+        a.D ? pair(one ? a.D[io_d + k] : 0.f, two ? a.D[io_d + k + 1] : 0.f) : 0;
   }
   // Each thread copies what it converts itself: its 8 channels of one token, and packs of 4 states
   // of B and C.  So a copy has arrived for its reader once that thread has waited for it.
@@ -160,7 +165,6 @@ selective_scan_kernel(salt_selective_scan_args a, ScanSplit sp, int blocks, bool
 
   float sum[CPT] = {};
   if (begin < stop) load(begin);
-  __syncthreads();  // bias and skip
   for (int t0 = begin; t0 < (FULL ? end : stop); t0 += S::kTile) {
     const int t = t0 + io_t;
     const auto& raw = sm.raw[t0 / S::kTile % kStages];
@@ -171,27 +175,21 @@ selective_scan_kernel(salt_selective_scan_args a, ScanSplit sp, int blocks, bool
       } else {
         copies_wait<0>();
       }
-      const T *rx = &raw.x[io_t][io_v * kVec], *rd = &raw.delta[io_t][io_v * kVec];
+      const auto px = pack_at<kVec>(&raw.x[io_t][io_v * kVec]);
+      const auto pd = pack_at<kVec>(&raw.delta[io_t][io_v * kVec]);
 #pragma unroll
       for (int k = 0; k < kVec; k += 2) {
-        const f32x2 in = add2(pair(to_f32(rd[k]), to_f32(rd[k + 1])),
-                              *reinterpret_cast<const f32x2*>(&sm.bias[io_v * kVec + k]));
+        const f32x2 in = add2(pair_of(pd, k), bias[k / 2]);
         // past the last token s = 0: the state stays as it is
         const f32x2 s2 = t < stop ? scan_step2(in, a.softplus) : 0;
-        const float2 s = halves(s2), sx = halves(mul2(s2, pair(to_f32(rx[k]), to_f32(rx[k + 1]))));
+        const float2 s = halves(s2), sx = halves(mul2(s2, pair_of(px, k)));
         sm.step[io_t][k * S::kIo + io_v] = make_float2(s.x, sx.x);
         sm.step[io_t][(k + 1) * S::kIo + io_v] = make_float2(s.y, sx.y);
       }
       for (int i = tid; i < kPacks; i += S::kThreads) {
         const int q = i / (S::kStates / 4), n1 = i % (S::kStates / 4) * 4;
-        const T* p = &raw.bc[0][q][n1];
-        *reinterpret_cast<float4*>(&sm.B[q][n1]) =
-            make_float4(to_f32(p[0]), to_f32(p[1]), to_f32(p[2]), to_f32(p[3]));
-        if (FULL) {
-          p = &raw.bc[FULL ? 1 : 0][q][n1];
-          *reinterpret_cast<float4*>(&sm.C[FULL ? q : 0][n1]) =
-              make_float4(to_f32(p[0]), to_f32(p[1]), to_f32(p[2]), to_f32(p[3]));
-        }
+        widen4(&sm.B[q][n1], &raw.bc[0][q][n1]);
+        if (FULL) widen4(&sm.C[FULL ? q : 0][n1], &raw.bc[FULL ? 1 : 0][q][n1]);
       }
     }
     __syncthreads();
@@ -260,18 +258,18 @@ selective_scan_kernel(salt_selective_scan_args a, ScanSplit sp, int blocks, bool
     }
     __syncthreads();
     if (FULL && t < end) {
-      const T *rx = &raw.x[io_t][io_v * kVec], *rz = &raw.z[FULL ? io_t : 0][io_v * kVec];
+      const auto px = pack_at<kVec>(&raw.x[io_t][io_v * kVec]);
+      const auto pz = pack_at<kVec>(&raw.z[FULL ? io_t : 0][io_v * kVec]);
       float y[kVec];
 #pragma unroll
       for (int k = 0; k < kVec; k += 2) {
         f32x2 v = 0;
         if (t < stop) {
-          v = fma2(*reinterpret_cast<const f32x2*>(&sm.skip[io_v * kVec + k]),
-                   pair(to_f32(rx[k]), to_f32(rx[k + 1])),
+          v = fma2(skip[k / 2], pair_of(px, k),
                    pair(sm.y[FULL ? io_t : 0][k * S::kIo + io_v],
                         sm.y[FULL ? io_t : 0][(k + 1) * S::kIo + io_v]));
           if (z) {
-            const f32x2 g = pair(to_f32(rz[k]), to_f32(rz[k + 1]));
+            const f32x2 g = pair_of(pz, k);
             v = mul2(v, mul2(g, sigmoid2(g)));
           }
         }
@@ -373,8 +371,8 @@ using Step64 = StepShape<16, 4>;
 #define SALT_STEP_SHAPE(state, S, ...) \
   SALT_BY_STATE(state, S, Step4, Step8, Step16, Step32, Step64, __VA_ARGS__)
 
-constexpr int kEnoughBlocks = 148 * 2;  // rows are not split
-constexpr int kFillBlocks = 148 * 12;   // and otherwise into about so many
+constexpr int kSlots = 148 * 5;      // blocks of 128 threads at 96 registers
+constexpr float kFirstPass = 0.55f;  // its time, of the second pass's
 
 template <typename T, class S, bool FULL>
 cudaError_t scan_launch(const salt_selective_scan_args& a, const ScanSplit& sp, int blocks,
@@ -393,22 +391,15 @@ cudaError_t scan_launch(const salt_selective_scan_args& a, const ScanSplit& sp, 
   return cudaGetLastError();
 }
 
-ScanSplit scan_split(const salt_selective_scan_args& a) {
-  ScanSplit s{1, std::max(a.len, 1), nullptr, nullptr};
+ScanSplit split_of(const salt_selective_scan_args& a) {
   const int64_t blocks = (int64_t)a.batch * scan_blocks(a.dim, a.groups, scan_channels(a.state));
-  if (blocks == 0 || blocks >= kEnoughBlocks) return s;
-  const int want = (int)(kFillBlocks / blocks);
-  const int each = std::max(128, (a.len + want - 1) / want);
-  s.chunk_len = (each + 31) / 32 * 32;  // whole tiles and checkpoints of every shape
-  s.chunks = std::max(1, (a.len + s.chunk_len - 1) / s.chunk_len);
-  if (s.chunks == 1) s.chunk_len = std::max(a.len, 1);
-  return s;
+  return scan_split(blocks, kSlots, a.len, kFirstPass);
 }
 
 }  // namespace
 
 size_t selective_scan_bytes(const salt_selective_scan_args& a) {
-  const ScanSplit s = scan_split(a);
+  const ScanSplit s = split_of(a);
   if (s.chunks == 1) return 0;
   return (size_t)a.batch * s.chunks * a.dim * (a.state + 1) * sizeof(float);
 }
@@ -416,7 +407,7 @@ size_t selective_scan_bytes(const salt_selective_scan_args& a) {
 cudaError_t selective_scan_launch(const salt_selective_scan_args& a, void* ws, cudaStream_t st,
                                   int* launches) {
   if (a.batch == 0) return cudaSuccess;
-  ScanSplit sp = scan_split(a);
+  ScanSplit sp = split_of(a);
   if (sp.chunks > 1) {
     sp.state = static_cast<float*>(ws);
     sp.steps = sp.state + (size_t)a.batch * sp.chunks * a.dim * a.state;

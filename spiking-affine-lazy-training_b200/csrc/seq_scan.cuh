@@ -15,6 +15,25 @@ struct ScanSplit {
   float* steps;  // (batch, chunks, dim): the sum of s over the chunk
 };
 
+// Into how many chunks of equal length rows are cut: those that need the least time, counted in
+// rounds of the `slots` blocks that the GPU runs at once.  A split row pays for its first pass,
+// `first` of the time of the second.
+inline ScanSplit scan_split(int64_t blocks, int64_t slots, int32_t len, float first) {
+  ScanSplit s{1, len > 0 ? len : 1, nullptr, nullptr};
+  float least = 0.f;
+  for (int c = 1; c <= 64 && (c == 1 || c * 128 <= len); ++c) {
+    const int64_t rounds = (blocks * c + slots - 1) / slots;
+    const float time = (float)rounds / c * (c > 1 ? 1.f + first : 1.f);
+    if (c > 1 && time > 0.97f * least) continue;  // not for a trifle
+    least = time;
+    s.chunks = c;
+  }
+  if (s.chunks == 1) return s;
+  s.chunk_len = ((len + s.chunks - 1) / s.chunks + 31) / 32 * 32;  // whole tiles and checkpoints
+  s.chunks = (len + s.chunk_len - 1) / s.chunk_len;
+  return s;
+}
+
 // Which 64 (or fewer) channels a block has: they lie in one group, so that B and C are shared.
 struct ScanBlock {
   int d0, n, group;
@@ -100,6 +119,18 @@ __device__ __forceinline__ void copy_pack(T* to, const T* from, int n) {
 #pragma unroll
     for (int i = 0; i < N; i += each) copy_async<bytes>(to + i, from + (i < n ? i : 0), i < n);
   }
+}
+
+// A pack of shared memory that copy_pack filled.
+template <int N, typename T>
+__device__ __forceinline__ Pack<T, N> pack_at(const T* p) {
+  return *reinterpret_cast<const Pack<T, N>*>(p);
+}
+template <typename T>
+__device__ __forceinline__ void widen4(float* to, const T* from) {
+  const Pack<T, 4> p = pack_at<4>(from);
+  const float2 lo = halves(pair_of(p, 0)), hi = halves(pair_of(p, 2));
+  *reinterpret_cast<float4*>(to) = make_float4(lo.x, lo.y, hi.x, hi.y);
 }
 
 // Stores N values of which `n` are wanted.  WIDE: n is a multiple of N or not positive, and the

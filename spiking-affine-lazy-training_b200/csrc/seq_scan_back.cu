@@ -45,15 +45,40 @@ struct BackShared {
         dy[kTile][S::kChannels];
     alignas(16) T bc[2][kTile][S::kStates];
   } raw[2];  // this tile and the next, as they were loaded
-  alignas(16) float2 step[kTile][S::kStepPitch];  // s and s * x
-  alignas(16) float g[kTile][S::kPitch];
-  alignas(16) float y[kTile][S::kPitch], to[kTile][S::kPitch], As[kTile][S::kPitch];
-  alignas(16) float B[kTile][S::kStates], C[kTile][S::kStates];
+  alignas(16) float2 step[kTile][S::kStepPitch];  // s and s * x; at last s and y
+  alignas(16) float g[kTile][S::kPitch], to[kTile][S::kPitch], As[kTile][S::kPitch];
+  alignas(16) float B[4][kTile][S::kStates], C[4][kTile][S::kStates];  // in every lane order
   alignas(16) float part[S::kWarps][kTile][2 * S::kStates];    // each warp's dB and dC
   float4 start[kGroups - 1][S::CPT][S::kThreads];  // the states in front of groups 1, 2, 3
   float4 dA[S::CPT][S::kThreads];                  // the sum over the tiles so far
   alignas(8) float bias[S::kChannels], skip[S::kChannels];
 };
+
+// The sums over channels, of dB and dC, halve what a lane holds at each step across lanes: it keeps
+// one half and sends the other.  So that no lane has to choose between registers, the lanes hold
+// their 4 states in different orders, always keep what lies first and send what lies second: lane
+// bit LPC swaps the pairs of states, bit 2 LPC the two of a pair (where the warp has such bits).
+// Likewise bit 1 swaps a lane's two channels for the sums over states.
+template <class S>
+struct LaneOrder {
+  int pairs, halves, channels;  // 0 or 1 each
+  __device__ __forceinline__ explicit LaneOrder(int lane)
+      : pairs(S::LPC < 32 ? lane / S::LPC % 2 : 0),
+        halves(2 * S::LPC < 32 ? lane / (2 * S::LPC) % 2 : 0),
+        channels(S::CPT == 2 && S::LPC > 1 ? lane % 2 : 0) {}
+  // memory order to lane order, or back (either is its own inverse)
+  __device__ __forceinline__ void turn(float (&f)[4]) const {
+    const float p0 = pairs ? f[2] : f[0], p1 = pairs ? f[3] : f[1];
+    const float q0 = pairs ? f[0] : f[2], q1 = pairs ? f[1] : f[3];
+    f[0] = halves ? p1 : p0, f[1] = halves ? p0 : p1;
+    f[2] = halves ? q1 : q0, f[3] = halves ? q0 : q1;
+  }
+};
+
+__device__ __forceinline__ f32x2 shuffle2(f32x2 v, int mask) {
+  const float2 h = salt::halves(v);
+  return pair(__shfl_xor_sync(0xffffffffu, h.x, mask), __shfl_xor_sync(0xffffffffu, h.y, mask));
+}
 
 struct BackParts {
   float* BC;            // (blocks, batch, len, 2 state): a block's dB and dC of its channels
@@ -78,13 +103,16 @@ selective_scan_backward_kernel(salt_selective_scan_backward_args a, ScanSplit sp
   const int stop = min(real, end);
   const int last = real > 0 ? (real - 1) / sp.chunk_len : 0;
 
-  const int at = tid / LPC * CPT, n0 = tid % LPC * NS, ns = a.state - n0;
+  const LaneOrder<S> order(lane);
+  const int n0 = tid % LPC * NS, ns = a.state - n0;
+  int at[CPT];  // places of the lane's channels
   bool mine[CPT];
   int64_t d[CPT];
   f32x2 A[CPT][H], carry[CPT][H];
 #pragma unroll
   for (int j = 0; j < CPT; ++j) {
-    const int ch = back_channel<S>(at + j);
+    at[j] = tid / LPC * CPT + (j ^ order.channels);
+    const int ch = back_channel<S>(at[j]);
     mine[j] = ch < cb.n;
     d[j] = cb.d0 + (mine[j] ? ch : 0);
     float f[NS], r[NS];
@@ -106,6 +134,8 @@ selective_scan_backward_kernel(salt_selective_scan_backward_args a, ScanSplit sp
         for (int i = 0; i < NS; ++i) r[i] = fmaf(exp_fast(f[i] * s), r[i], l[i]);
       }
     }
+    order.turn(f);
+    order.turn(r);
 #pragma unroll
     for (int i = 0; i < H; ++i) {
       A[j][i] = pair(f[2 * i] * kLog2e, f[2 * i + 1] * kLog2e);
@@ -131,9 +161,7 @@ selective_scan_backward_kernel(salt_selective_scan_backward_args a, ScanSplit sp
     sm.bias[i] = a.delta_bias && i < cb.n ? a.delta_bias[cb.d0 + i] : 0.f;
     sm.skip[i] = a.D && i < cb.n ? a.D[cb.d0 + i] : 0.f;
   }
-  float dbias[P], dskip[P];
-#pragma unroll
-  for (int k = 0; k < P; ++k) dbias[k] = dskip[k] = 0.f;
+  f32x2 dbias[P / 2] = {}, dskip[P / 2] = {};
 
   // tokens past the row's end
   for (int t = max(stop, begin) / kTile * kTile + io_t; t < end; t += kTile) {
@@ -170,14 +198,13 @@ selective_scan_backward_kernel(salt_selective_scan_backward_args a, ScanSplit sp
     const int t = t0 + io_t;
     const bool live = t < stop;
     const auto& raw = sm.raw[t0 / kTile % 2];
-    const T *rx = &raw.x[io_t][io_v * P], *rd = &raw.delta[io_t][io_v * P];
-    const T *rz = &raw.z[io_t][io_v * P], *ry = &raw.dy[io_t][io_v * P];
     f32x2 h[CPT][H];  // the state in front of the tile
 #pragma unroll
     for (int j = 0; j < CPT; ++j) {
       float f[NS];
       load_states<NS>(f, a.checkpoints + ((b * per + t0 / kTile) * a.dim + d[j]) * a.state + n0,
                       mine[j] ? ns : 0, svec);
+      order.turn(f);
       h[j][0] = pair(f[0], f[1]), h[j][1] = pair(f[2], f[3]);
     }
     if (t0 - kTile >= begin) {
@@ -186,46 +213,52 @@ selective_scan_backward_kernel(salt_selective_scan_backward_args a, ScanSplit sp
     } else {
       copies_wait<0>();
     }
+    {
+      const auto px = pack_at<P>(&raw.x[io_t][io_v * P]), pd = pack_at<P>(&raw.delta[io_t][io_v * P]);
+      const auto pz = pack_at<P>(&raw.z[io_t][io_v * P]), py = pack_at<P>(&raw.dy[io_t][io_v * P]);
 #pragma unroll
-    for (int k = 0; k < P; ++k) {
-      float g = to_f32(ry[k]), s = 0.f;
-      if (z) {
-        const float v = to_f32(rz[k]);
-        g *= v * sigmoid(v);
+      for (int k = 0; k < P; k += 2) {
+        f32x2 g2 = pair_of(py, k);
+        if (z) {
+          const f32x2 v = pair_of(pz, k);
+          g2 = mul2(g2, mul2(v, sigmoid2(v)));
+        }
+        const f32x2 in = add2(pair_of(pd, k), pair(sm.bias[io_v * P + k], sm.bias[io_v * P + k + 1]));
+        const f32x2 s2 = live ? scan_step2(in, a.softplus) : 0;
+        const float2 s = halves(s2), sx = halves(mul2(s2, pair_of(px, k))), g = halves(g2);
+        sm.step[io_t][k * S::kIo + io_v] = make_float2(s.x, sx.x);
+        sm.step[io_t][(k + 1) * S::kIo + io_v] = make_float2(s.y, sx.y);
+        sm.g[io_t][k * S::kIo + io_v] = g.x;  // 0 past the end, as dy there
+        sm.g[io_t][(k + 1) * S::kIo + io_v] = g.y;
       }
-      if (live) s = scan_step(to_f32(rd[k]) + sm.bias[io_v * P + k], a.softplus);
-      sm.step[io_t][k * S::kIo + io_v] = make_float2(s, s * to_f32(rx[k]));
-      sm.g[io_t][k * S::kIo + io_v] = g;  // 0 past the end, as dy there
     }
     for (int i = tid; i < kPacks; i += S::kThreads) {
       const int q = i / (S::kStates / 4), n1 = i % (S::kStates / 4) * 4;
-      const T *p = &raw.bc[0][q][n1], *r = &raw.bc[1][q][n1];
-      *reinterpret_cast<float4*>(&sm.B[q][n1]) =
-          make_float4(to_f32(p[0]), to_f32(p[1]), to_f32(p[2]), to_f32(p[3]));
-      *reinterpret_cast<float4*>(&sm.C[q][n1]) =
-          make_float4(to_f32(r[0]), to_f32(r[1]), to_f32(r[2]), to_f32(r[3]));
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const auto p = pack_at<4>(&raw.bc[k][q][n1]);
+        const float2 lo = halves(pair_of(p, 0)), hi = halves(pair_of(p, 2));
+        auto to = k ? sm.C : sm.B;
+        *reinterpret_cast<float4*>(&to[0][q][n1]) = make_float4(lo.x, lo.y, hi.x, hi.y);
+        *reinterpret_cast<float4*>(&to[1][q][n1]) = make_float4(hi.x, hi.y, lo.x, lo.y);
+        *reinterpret_cast<float4*>(&to[2][q][n1]) = make_float4(lo.y, lo.x, hi.y, hi.x);
+        *reinterpret_cast<float4*>(&to[3][q][n1]) = make_float4(hi.y, hi.x, lo.y, lo.x);
+      }
     }
     __syncthreads();
 
-    auto step_of = [&](int q, float2 (&st)[CPT]) {
-      if constexpr (CPT == 2) {
-        const float4 v = *reinterpret_cast<const float4*>(&sm.step[q][at]);
-        st[0] = make_float2(v.x, v.y), st[1] = make_float2(v.z, v.w);
-      } else {
-        st[0] = sm.step[q][at];
-      }
-    };
+    const float(*Bo)[S::kStates] = sm.B[order.pairs + 2 * order.halves];
+    const float(*Co)[S::kStates] = sm.C[order.pairs + 2 * order.halves];
     // the states in front of each group but the first
 #pragma unroll 1
     for (int u = 0; u < kGroups - 1; ++u) {
 #pragma unroll
       for (int q = 0; q < kGroup; ++q) {
-        float2 st[CPT];
-        step_of(u * kGroup + q, st);
-        const ulonglong2 bn = *reinterpret_cast<const ulonglong2*>(&sm.B[u * kGroup + q][n0]);
+        const ulonglong2 bn = *reinterpret_cast<const ulonglong2*>(&Bo[u * kGroup + q][n0]);
 #pragma unroll
         for (int j = 0; j < CPT; ++j) {
-          const f32x2 s = pair(st[j].x, st[j].x), sx = pair(st[j].y, st[j].y);
+          const float2 st = sm.step[u * kGroup + q][at[j]];
+          const f32x2 s = both(st.x), sx = both(st.y);
           h[j][0] = fma2(exp2_fast2(mul2(A[j][0], s)), h[j][0], mul2(sx, bn.x));
           h[j][1] = fma2(exp2_fast2(mul2(A[j][1], s)), h[j][1], mul2(sx, bn.y));
         }
@@ -247,17 +280,17 @@ selective_scan_backward_kernel(salt_selective_scan_backward_args a, ScanSplit sp
           float f[NS];  // the checkpoint once more: from L1
           load_states<NS>(f, a.checkpoints + ((b * per + t0 / kTile) * a.dim + d[j]) * a.state + n0,
                           mine[j] ? ns : 0, svec);
+          order.turn(f);
           h0[j][0] = pair(f[0], f[1]), h0[j][1] = pair(f[2], f[3]);
         }
       }
 #pragma unroll
       for (int q = 0; q < kGroup; ++q) {
-        float2 st[CPT];
-        step_of(u * kGroup + q, st);
-        const ulonglong2 bn = *reinterpret_cast<const ulonglong2*>(&sm.B[u * kGroup + q][n0]);
+        const ulonglong2 bn = *reinterpret_cast<const ulonglong2*>(&Bo[u * kGroup + q][n0]);
 #pragma unroll
         for (int j = 0; j < CPT; ++j) {
-          const f32x2 s = pair(st[j].x, st[j].x), sx = pair(st[j].y, st[j].y);
+          const float2 st = sm.step[u * kGroup + q][at[j]];
+          const f32x2 s = both(st.x), sx = both(st.y);
           const f32x2* before = q ? hs[q ? q - 1 : 0][j] : h0[j];
           ea[q][j][0] = exp2_fast2(mul2(A[j][0], s));
           ea[q][j][1] = exp2_fast2(mul2(A[j][1], s));
@@ -265,25 +298,17 @@ selective_scan_backward_kernel(salt_selective_scan_backward_args a, ScanSplit sp
           hs[q][j][1] = fma2(ea[q][j][1], before[1], mul2(sx, bn.y));
         }
       }
-      float sums[3][kGroup * CPT];  // y, sum of dh B, sum of m A: over this lane's states
+      float sums[3][CPT][kGroup];  // y, sum of dh B, sum of m A: over this lane's states
 #pragma unroll
       for (int q = kGroup - 1; q >= 0; --q) {
         const int row = u * kGroup + q;
-        float2 st[CPT];
-        float g[CPT];
-        step_of(row, st);
-        if constexpr (CPT == 2) {
-          const float2 v = *reinterpret_cast<const float2*>(&sm.g[row][at]);
-          g[0] = v.x, g[1] = v.y;
-        } else {
-          g[0] = sm.g[row][at];
-        }
-        const ulonglong2 bn = *reinterpret_cast<const ulonglong2*>(&sm.B[row][n0]);
-        const ulonglong2 cn = *reinterpret_cast<const ulonglong2*>(&sm.C[row][n0]);
+        const ulonglong2 bn = *reinterpret_cast<const ulonglong2*>(&Bo[row][n0]);
+        const ulonglong2 cn = *reinterpret_cast<const ulonglong2*>(&Co[row][n0]);
         f32x2 dB[H] = {}, dC[H] = {};
 #pragma unroll
         for (int j = 0; j < CPT; ++j) {
-          const f32x2 s = pair(st[j].x, st[j].x), sx = pair(st[j].y, st[j].y), gg = pair(g[j], g[j]);
+          const float2 st = sm.step[row][at[j]];
+          const f32x2 s = both(st.x), sx = both(st.y), gg = both(sm.g[row][at[j]]);
           const f32x2* before = q ? hs[q ? q - 1 : 0][j] : h0[j];
           f32x2 y2 = 0, to2 = 0, As2 = 0;
 #pragma unroll
@@ -303,38 +328,57 @@ selective_scan_backward_kernel(salt_selective_scan_backward_args a, ScanSplit sp
 #pragma unroll
           for (int k = 0; k < 3; ++k) {
             const float2 v = halves(all[k]);
-            sums[k][q * CPT + j] = v.x + v.y;
+            sums[k][j][q] = v.x + v.y;
           }
         }
-        float bc[2 * NS];
+        // what is left of dB and dC on this lane after the halvings: of pair order.pairs, its
+        // half order.halves, and one of the two
+        float* to = &sm.part[warp][row][n0 + 2 * order.pairs];
+        dB[0] = add2(dB[0], shuffle2(dB[1], LPC));
+        dC[0] = add2(dC[0], shuffle2(dC[1], LPC));
+        const float2 vb = halves(dB[0]), vc = halves(dC[0]);
+        if constexpr (2 * LPC >= 32) {
+          *reinterpret_cast<float2*>(to) = vb;
+          *reinterpret_cast<float2*>(to + S::kStates) = vc;
+        } else {
+          const float kb = vb.x + __shfl_xor_sync(0xffffffffu, vb.y, 2 * LPC);
+          const float kc = vc.x + __shfl_xor_sync(0xffffffffu, vc.y, 2 * LPC);
+          to += order.halves;
+          if constexpr (4 * LPC >= 32) {
+            to[0] = kb;
+            to[S::kStates] = kc;
+          } else {
+            const bool up = lane & (4 * LPC);
+            float v = (up ? kc : kb) + __shfl_xor_sync(0xffffffffu, up ? kb : kc, 4 * LPC);
 #pragma unroll
-        for (int i = 0; i < H; ++i) {
-          const float2 v = halves(dB[i]), w = halves(dC[i]);
-          bc[2 * i] = v.x, bc[2 * i + 1] = v.y;
-          bc[NS + 2 * i] = w.x, bc[NS + 2 * i + 1] = w.y;
-        }
-        int first = 0;
-        lane_sums<2 * NS, LPC, 32>(bc, lane, first);
-        constexpr int DL = 32 / LPC, kept = DL >= 2 * NS ? 1 : 2 * NS / DL;
-        // with more lanes than sums the first lanes of each group write
-        if (DL <= 2 * NS || lane / (LPC * 2 * NS) == 0)
-#pragma unroll
-          for (int i = 0; i < kept; ++i) {
-            const int v = first + i;
-            sm.part[warp][row][(v < NS ? 0 : S::kStates) + n0 + v % NS] = bc[i];
+            for (int o = 8 * LPC; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+            if (lane < 8 * LPC) to[up ? S::kStates : 0] = v;
           }
+        }
       }
-      constexpr int values = kGroup * CPT;
-      constexpr int left = LPC <= values ? values / LPC : 1;
+      __syncwarp();  // the group's s x has been read
 #pragma unroll
       for (int k = 0; k < 3; ++k) {
-        int first = 0;
-        lane_sums<values, 1, LPC>(sums[k], lane, first);
-        float(*out)[S::kPitch] = k == 0 ? sm.y : k == 1 ? sm.to : sm.As;
-        if (LPC <= values || (lane & (LPC - 1)) < values)
+        float* v = sums[k][0];
+        if constexpr (CPT == 2 && LPC > 1) {
 #pragma unroll
-          for (int i = 0; i < left; ++i)
-            out[u * kGroup + (first + i) / CPT][at + (first + i) % CPT] = sums[k][i];
+          for (int q = 0; q < kGroup; ++q)
+            v[q] += __shfl_xor_sync(0xffffffffu, sums[k][CPT - 1][q], 1);
+        }
+        // the rest of the channel's lanes, over the group's tokens
+        int first = 0;
+        constexpr int from = CPT == 2 ? 2 : 1, lanes = LPC / from;
+        constexpr int left = lanes >= kGroup ? 1 : lanes > 1 ? kGroup / lanes : kGroup;
+        lane_sums<kGroup, from, LPC>(v, lane, first);
+        if (lanes <= kGroup || (lane & (LPC - 1)) / from < kGroup)
+#pragma unroll
+          for (int i = 0; i < left; ++i) {
+            const int row = u * kGroup + first + i;
+            if (k == 0)
+              sm.step[row][at[0]].y = v[i];
+            else
+              (k == 1 ? sm.to : sm.As)[row][at[0]] = v[i];
+          }
       }
     }
 #pragma unroll
@@ -347,21 +391,32 @@ selective_scan_backward_kernel(salt_selective_scan_backward_args a, ScanSplit sp
     }
     __syncthreads();
     if (live) {
+      const auto px = pack_at<P>(&raw.x[io_t][io_v * P]), pd = pack_at<P>(&raw.delta[io_t][io_v * P]);
+      const auto pz = pack_at<P>(&raw.z[io_t][io_v * P]), py = pack_at<P>(&raw.dy[io_t][io_v * P]);
       float ox[P], od[P], oz[P];
 #pragma unroll
-      for (int k = 0; k < P; ++k) {
-        const int place = k * S::kIo + io_v;
-        const float xs = to_f32(rx[k]), g = sm.g[io_t][place], s = sm.step[io_t][place].x;
-        const float to = sm.to[io_t][place], skip = sm.skip[io_v * P + k];
-        ox[k] = fmaf(s, to, g * skip);
+      for (int k = 0; k < P; k += 2) {
+        const int p0 = k * S::kIo + io_v, p1 = p0 + S::kIo;
+        const f32x2 xs = pair_of(px, k), g = pair(sm.g[io_t][p0], sm.g[io_t][p1]);
+        const f32x2 s = pair(sm.step[io_t][p0].x, sm.step[io_t][p1].x);
+        const f32x2 to = pair(sm.to[io_t][p0], sm.to[io_t][p1]);
+        const f32x2 skip = pair(sm.skip[io_v * P + k], sm.skip[io_v * P + k + 1]);
+        float2 f = halves(fma2(s, to, mul2(g, skip)));
+        ox[k] = f.x, ox[k + 1] = f.y;
         // A held log2(e) times A
-        od[k] = fmaf(xs, to, sm.As[io_t][place] * (1.f / kLog2e));
-        if (a.softplus) od[k] *= sigmoid(to_f32(rd[k]) + sm.bias[io_v * P + k]);
-        dbias[k] += od[k];
-        dskip[k] = fmaf(g, xs, dskip[k]);
+        f32x2 dd = fma2(xs, to, mul2(pair(sm.As[io_t][p0], sm.As[io_t][p1]), both(1.f / kLog2e)));
+        if (a.softplus)
+          dd = mul2(dd, sigmoid2(add2(pair_of(pd, k), pair(sm.bias[io_v * P + k],
+                                                           sm.bias[io_v * P + k + 1]))));
+        f = halves(dd);
+        od[k] = f.x, od[k + 1] = f.y;
+        dbias[k / 2] = add2(dbias[k / 2], dd);
+        dskip[k / 2] = fma2(g, xs, dskip[k / 2]);
         if (z) {
-          const float v = to_f32(rz[k]), y = fmaf(skip, xs, sm.y[io_t][place]);
-          oz[k] = to_f32(ry[k]) * y * silu_slope(v, sigmoid(v));
+          const f32x2 v = pair_of(pz, k);
+          const f32x2 y = fma2(skip, xs, pair(sm.step[io_t][p0].y, sm.step[io_t][p1].y));
+          f = halves(mul2(mul2(pair_of(py, k), y), silu_slope2(v, sigmoid2(v))));
+          oz[k] = f.x, oz[k + 1] = f.y;
         }
       }
       scan_store<T, P, WIDE>(dx + t * a.dx_stride, ox, io_n);
@@ -386,26 +441,28 @@ selective_scan_backward_kernel(salt_selective_scan_backward_args a, ScanSplit sp
   for (int j = 0; j < CPT; ++j) {
     if (!mine[j]) continue;
     const float4 v = sm.dA[j][tid];
-    const float f[NS] = {v.x, v.y, v.z, v.w};
+    float f[NS] = {v.x, v.y, v.z, v.w};
+    order.turn(f);
     store_states<NS>(parts.A + ((b * sp.chunks + c) * a.dim + d[j]) * a.state + n0, f, ns, svec);
     if (c == 0 && a.dinitial) {
       const float2 lo = halves(carry[j][0]), hi = halves(carry[j][1]);
-      const float r[NS] = {lo.x, lo.y, hi.x, hi.y};
+      float r[NS] = {lo.x, lo.y, hi.x, hi.y};
+      order.turn(r);
       store_states<NS>(a.dinitial + (b * a.dim + d[j]) * a.state + n0, r, ns, svec);
     }
   }
   // the 16 tokens' threads of a channel pack add up what they saw, in order
 #pragma unroll
-  for (int k = 0; k < P; ++k) {
-    sm.y[io_t][io_v * P + k] = dbias[k];
-    sm.g[io_t][io_v * P + k] = dskip[k];
+  for (int k = 0; k < P; k += 2) {
+    *reinterpret_cast<f32x2*>(&sm.to[io_t][io_v * P + k]) = dbias[k / 2];
+    *reinterpret_cast<f32x2*>(&sm.g[io_t][io_v * P + k]) = dskip[k / 2];
   }
   __syncthreads();
   for (int i = tid; i < cb.n; i += S::kThreads) {
     float sb = 0.f, ss = 0.f;
 #pragma unroll
     for (int q = 0; q < kTile; ++q) {
-      sb += sm.y[q][i];
+      sb += sm.to[q][i];
       ss += sm.g[q][i];
     }
     const int64_t to = (b * sp.chunks + c) * a.dim + cb.d0 + i;
@@ -493,22 +550,25 @@ scan_back_state_kernel(salt_selective_scan_backward_args a, ScanSplit sp, int bl
       copies_wait<0>();
     }
     __syncthreads();  // the last tile's readers; the first time, bias
+    {
+      const auto pd = pack_at<P>(&raw.delta[io_t][io_v * P]);
+      const auto pz = pack_at<P>(&raw.z[io_t][io_v * P]), py = pack_at<P>(&raw.dy[io_t][io_v * P]);
 #pragma unroll
-    for (int k = 0; k < P; ++k) {
-      float g = to_f32(raw.dy[io_t][io_v * P + k]), s = 0.f;
-      if (z) {
-        const float v = to_f32(raw.z[io_t][io_v * P + k]);
-        g *= v * sigmoid(v);
+      for (int k = 0; k < P; k += 2) {
+        f32x2 g2 = pair_of(py, k);
+        if (z) {
+          const f32x2 v = pair_of(pz, k);
+          g2 = mul2(g2, mul2(v, sigmoid2(v)));
+        }
+        const f32x2 in = add2(pair_of(pd, k), pair(sm.bias[io_v * P + k], sm.bias[io_v * P + k + 1]));
+        const float2 s = halves(t < stop ? scan_step2(in, a.softplus) : 0), g = halves(g2);
+        sm.step[io_t][k * S::kIo + io_v] = make_float2(s.x, g.x);
+        sm.step[io_t][(k + 1) * S::kIo + io_v] = make_float2(s.y, g.y);
       }
-      if (t < stop)
-        s = scan_step(to_f32(raw.delta[io_t][io_v * P + k]) + sm.bias[io_v * P + k], a.softplus);
-      sm.step[io_t][k * S::kIo + io_v] = make_float2(s, g);
     }
     for (int i = tid; i < kPacks; i += S::kThreads) {
       const int q = i / (S::kStates / 4), n1 = i % (S::kStates / 4) * 4;
-      const T* p = &raw.c[q][n1];
-      *reinterpret_cast<float4*>(&sm.C[q][n1]) =
-          make_float4(to_f32(p[0]), to_f32(p[1]), to_f32(p[2]), to_f32(p[3]));
+      widen4(&sm.C[q][n1], &raw.c[q][n1]);
     }
     __syncthreads();
 #pragma unroll 4
@@ -554,25 +614,21 @@ __global__ void scan_BC_gradient(salt_selective_scan_backward_args a, const floa
 }
 
 using Back4 = BackShape<1, 1, 64>;
-using Back8 = BackShape<2, 1, 64>;
-#ifndef BCPT
-#define BCPT 2
-#endif
-using Back16 = BackShape<4, BCPT, 64>;
+using Back8 = BackShape<2, 2, 64>;
+using Back16 = BackShape<4, 2, 64>;
 using Back32 = BackShape<8, 2, 64>;
 using Back64 = BackShape<16, 2, 32>;
 #define SALT_BACK_SHAPE(state, S, ...) \
   SALT_BY_STATE(state, S, Back4, Back8, Back16, Back32, Back64, __VA_ARGS__)
 int back_channels(int32_t state) {
-  return state <= 32 ? Back16::kChannels : Back64::kChannels;
+  return state <= 8    ? Back8::kChannels
+         : state <= 16 ? Back16::kChannels
+         : state <= 32 ? Back32::kChannels
+                       : Back64::kChannels;
 }
 
-#ifndef BENOUGH
-#define BENOUGH 3
-#define BFILL 9
-#endif
-constexpr int kEnoughBlocks = 148 * BENOUGH;  // rows are not split
-constexpr int kFillBlocks = 148 * BFILL;    // and otherwise into about so many
+constexpr int kSlots = 148 * 3;      // blocks of 128 threads at 168 registers
+constexpr float kFirstPass = 0.22f;  // its time, of the second pass's
 
 template <typename T, class S, int COPY>
 cudaError_t back_launch(const salt_selective_scan_backward_args& a, const ScanSplit& sp,
@@ -609,14 +665,8 @@ struct BackPlan {
 BackPlan back_plan(const salt_selective_scan_backward_args& a) {
   BackPlan p;
   p.blocks = scan_blocks(a.dim, a.groups, back_channels(a.state));
-  p.chunks = 1, p.chunk_len = std::max(a.len, 1);
-  const int64_t blocks = (int64_t)a.batch * p.blocks;
-  if (blocks > 0 && blocks < kEnoughBlocks) {
-    const int want = (int)(kFillBlocks / blocks);
-    const int each = std::max(128, (a.len + want - 1) / want);
-    p.chunk_len = (each + kTile - 1) / kTile * kTile;
-    p.chunks = std::max(1, (a.len + p.chunk_len - 1) / p.chunk_len);
-  }
+  const ScanSplit split = scan_split((int64_t)a.batch * p.blocks, kSlots, a.len, kFirstPass);
+  p.chunks = split.chunks, p.chunk_len = split.chunk_len;
   size_t at = 0;
   auto take = [&](size_t n) {
     const size_t o = at;
@@ -650,7 +700,7 @@ cudaError_t selective_scan_backward_launch(const salt_selective_scan_backward_ar
   // the widest copies that no row's start and end stand against
   auto fits = [&](int64_t bytes) {
     const int64_t few = std::min<int64_t>(bytes, 4 * ts);
-    const int pack = a.state <= 4 ? Back4::P : kVec;  // channels of the largest pack
+    const int pack = a.state <= 8 ? Back4::P : kVec;  // channels of the largest pack
     return (a.dim / a.groups) % (bytes == 16 ? pack : (int)(bytes / ts)) == 0 &&
            a.state % (few / ts) == 0 && packed_rows(a.x, bytes, ts, a.x_batch_stride, a.x_stride) &&
            packed_rows(a.delta, bytes, ts, a.delta_batch_stride, a.delta_stride) &&

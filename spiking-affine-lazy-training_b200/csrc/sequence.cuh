@@ -160,6 +160,22 @@ __device__ __forceinline__ f32x2 sigmoid2(f32x2 x) {
   return pair(rcp_fast(d.x), rcp_fast(d.y));
 }
 
+// Elements k and k + 1 of a pack.
+template <typename T, int N>
+__device__ __forceinline__ f32x2 pair_of(const Pack<T, N>& p, int k) {
+  return pair(to_f32(p.v[k]), to_f32(p.v[k + 1]));
+}
+template <int N>
+__device__ __forceinline__ f32x2 pair_of(const Pack<__nv_bfloat16, N>& p, int k) {
+  const uint32_t u = *reinterpret_cast<const uint32_t*>(&p.v[k]);  // k is even
+  return pair(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+__device__ __forceinline__ f32x2 both(float v) { return pair(v, v); }
+// d/dx of x * sigmoid(x), of both.
+__device__ __forceinline__ f32x2 silu_slope2(f32x2 x, f32x2 p) {
+  return mul2(p, fma2(x, fma2(p, both(-1.f), both(1.f)), both(1.f)));
+}
+
 // Launches (argument checks are the caller's; each returns the launch's status).
 cudaError_t rms_norm_launch(const salt_rms_norm_args& a, cudaStream_t st, int* launches);
 size_t rms_norm_backward_bytes(const salt_rms_norm_backward_args& a);
