@@ -12,87 +12,99 @@ namespace salt {
 
 namespace {
 
-// weight[d][k] of channels d0 .. d0 + N; tap W - 1 is the newest input's.
+// weight[d][k] of channels d0 .. d0 + N, of which n are there; tap W - 1 is the newest input's.
+// The N W values lie together: W packs.
 template <typename T, int N, int W>
 __device__ __forceinline__ void load_taps(float (&w)[N][W], const void* weight, int d0, int n,
-                                          bool w_f32) {
+                                          bool w_f32, bool vec) {
 #pragma unroll
-  for (int i = 0; i < N; ++i)
+  for (int i = 0; i < W; ++i) {
+    float f[N];
+    load_weights<T, N>(f, weight, (int64_t)d0 * W + i * N, n * W - i * N, w_f32, vec);
 #pragma unroll
-    for (int k = 0; k < W; ++k)
-      w[i][k] = i < n ? weight_at<T>(weight, (int64_t)(d0 + i) * W + k, w_f32) : 0.f;
+    for (int k = 0; k < N; ++k) w[(i * N + k) / W][(i * N + k) % W] = f[k];
+  }
 }
 
-// Token s of a channel, for s < 0 from the initial state (token s is its entry W - 1 + s), zero
-// where there is none.
-template <typename T, int W>
-__device__ __forceinline__ float token_at(const T* x, int64_t stride, const T* init, int d, int s) {
-  if (s >= 0) return to_f32(x[s * stride + d]);
-  return init ? to_f32(init[(int64_t)d * (W - 1) + W - 1 + s]) : 0.f;
+// Token s of N neighbouring channels of a row, the first at x + s * stride and init: for s < 0 from
+// the initial state (token s is its entry W - 1 + s), zero where there is none and past `real`.
+template <typename T, int N, int W>
+__device__ __forceinline__ void load_token(float (&f)[N], const T* x, int64_t stride, const T* init,
+                                           int s, int real, int n, bool vec) {
+  if (s >= 0 || !init) {
+    const Pack<T, N> p = load_pack<T, N>(x + s * stride, s >= 0 && s < real ? n : 0, vec);
+#pragma unroll
+    for (int k = 0; k < N; ++k) f[k] = to_f32(p.v[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) f[k] = k < n ? to_f32(init[k * (W - 1) + W - 1 + s]) : 0.f;
+  }
 }
 
 // ---------------------------------------------------------------- whole rows
 
-// Thread = 8 channels x `run` tokens; threads count channel packs fastest, then runs, then rows.
-template <typename T, int W>
+// Thread = V channels x `run` tokens; threads count channel packs fastest, then runs, then rows.
+template <typename T, int V, int W>
 __global__ void __launch_bounds__(128)
-causal_conv_kernel(salt_causal_conv_args a, int packs, int runs, int run, bool vec, bool w_f32) {
+causal_conv_kernel(salt_causal_conv_args a, int packs, int runs, int run, bool w_f32, bool w_vec) {
   const int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   const int64_t per_row = (int64_t)packs * runs;
   if (id >= per_row * a.batch) return;
   const int b = (int)(id / per_row);
   const int rest = (int)(id - b * per_row);
-  const int c = rest / packs, d0 = (rest - c * packs) * kVec;
-  const int n = a.dim - d0;
+  const int c = rest / packs, d0 = (rest - c * packs) * V;
+  const int n = a.dim - d0;  // at least V: V divides dim
   const int real = row_tokens(a.n_real, b, a.len);
-  const T* x = static_cast<const T*>(a.x) + b * a.x_batch_stride;
-  const int64_t state0 = (int64_t)b * a.dim * (W - 1);
+  const T* x = static_cast<const T*>(a.x) + b * a.x_batch_stride + d0;
+  const int64_t state0 = ((int64_t)b * a.dim + d0) * (W - 1);
   const T* init = a.initial_state ? static_cast<const T*>(a.initial_state) + state0 : nullptr;
-  T* out = static_cast<T*>(a.out) + b * a.out_batch_stride;
-  const int t0 = c * run, t1 = min(t0 + run, a.len);
-  float w[kVec][W], bias[kVec], win[W][kVec];  // win[W - 1] is the newest input
-  load_taps<T, kVec, W>(w, a.weight, d0, n, w_f32);
+  T* out = static_cast<T*>(a.out) + b * a.out_batch_stride + d0;
+  const int t0 = c * run, t1 = min(t0 + run, a.len), stop = min(t1, real);
+  float win[W][V];  // win[W - 1] is the newest input
+  if (t0 < stop || c == 0) {
 #pragma unroll
-  for (int k = 0; k < kVec; ++k)
-    bias[k] = a.bias && k < n ? weight_at<T>(a.bias, d0 + k, w_f32) : 0.f;
-#pragma unroll
-  for (int j = 1; j < W; ++j) {
-    const int s = t0 + j - W;
-#pragma unroll
-    for (int k = 0; k < kVec; ++k)
-      win[j][k] = k < n && s < real ? token_at<T, W>(x, a.x_stride, init, d0 + k, s) : 0.f;
+    for (int j = 1; j < W; ++j)
+      load_token<T, V, W>(win[j], x, a.x_stride, init, t0 + j - W, real, n, true);
   }
   // Reads its own channels of initial_state, here and above, before it writes: they may be one.
-  if (c == 0 && a.final_state) {
+  if (c == 0 && a.final_state && W > 1) {
     T* fin = static_cast<T*>(a.final_state) + state0;
+    float f[W][V];
 #pragma unroll
-    for (int k = 0; k < kVec; ++k) {
-      if (k >= n) break;
-      float f[W];
+    for (int j = 0; j < W - 1; ++j)
+      load_token<T, V, W>(f[j], x, a.x_stride, init, real - (W - 1) + j, real, n, true);
 #pragma unroll
-      for (int j = 0; j < W - 1; ++j)
-        f[j] = token_at<T, W>(x, a.x_stride, init, d0 + k, real - (W - 1) + j);
+    for (int k = 0; k < V; ++k)
 #pragma unroll
-      for (int j = 0; j < W - 1; ++j) fin[(int64_t)(d0 + k) * (W - 1) + j] = from_f32<T>(f[j]);
-    }
+      for (int j = 0; j < W - 1; ++j) fin[k * (W - 1) + j] = from_f32<T>(f[j][k]);
   }
+  int t = t0;
+  if (t0 < stop) {
+    float w[V][W], bias[V];
+    load_taps<T, V, W>(w, a.weight, d0, n, w_f32, w_vec);
+#pragma unroll
+    for (int k = 0; k < V; ++k) bias[k] = a.bias ? weight_at<T>(a.bias, d0 + k, w_f32) : 0.f;
 #pragma unroll 4
-  for (int t = t0; t < t1; ++t) {
-    const Pack<T, kVec> p = load_pack<T, kVec>(x + t * a.x_stride + d0, t < real ? n : 0, vec);
-    float y[kVec];
+    for (; t < stop; ++t) {
+      const Pack<T, V> p = load_pack<T, V>(x + t * a.x_stride, V, true);
+      float y[V];
 #pragma unroll
-    for (int k = 0; k < kVec; ++k) {
+      for (int k = 0; k < V; ++k) {
 #pragma unroll
-      for (int j = 0; j < W - 1; ++j) win[j][k] = win[j + 1][k];
-      win[W - 1][k] = to_f32(p.v[k]);
-      float s = bias[k];
+        for (int j = 0; j < W - 1; ++j) win[j][k] = win[j + 1][k];
+        win[W - 1][k] = to_f32(p.v[k]);
+        float s = bias[k];
 #pragma unroll
-      for (int j = 0; j < W; ++j) s = fmaf(w[k][j], win[j][k], s);
-      if (a.silu) s *= sigmoid(s);
-      y[k] = t < real ? s : 0.f;
+        for (int j = 0; j < W; ++j) s = fmaf(w[k][j], win[j][k], s);
+        if (a.silu) s *= sigmoid(s);
+        y[k] = s;
+      }
+      store_pack<T, V>(out + t * a.out_stride, y, V, true);
     }
-    store_pack<T, kVec>(out + t * a.out_stride + d0, y, n, vec);
   }
+  const float zero[V] = {};
+#pragma unroll 4
+  for (; t < t1; ++t) store_pack<T, V>(out + t * a.out_stride, zero, V, true);
 }
 
 // ---------------------------------------------------------------- single tokens
@@ -126,51 +138,46 @@ causal_conv_step_kernel(salt_causal_conv_step_args a, int64_t total, bool w_f32)
 
 // ---------------------------------------------------------------- gradient
 
-constexpr int kBackVec = 4;   // channels of a thread: 8 would need 150 registers
 constexpr int kBackRuns = 8;  // runs of tokens in a block, one per warp
 constexpr int kBackLanes = 32;
 
-// A warp takes 128 channels through `run` tokens, a block 8 such runs one after the other in the
+// A warp takes 32 V channels through `run` tokens, a block 8 such runs one after the other in the
 // row.  g[t] = dy[t] * act'(p[t]) for the run and the width - 1 tokens behind it gives
 // dx[s] = sum_k w[k] g[s + width - 1 - k]; the weight's gradient takes the run's own tokens only.
-template <typename T, int W>
+template <typename T, int V, int W>
 __global__ void __launch_bounds__(kBackLanes * kBackRuns)
 causal_conv_backward_kernel(salt_causal_conv_backward_args a, int packs, int chunks, int run,
-                            bool vec, bool w_f32, float* parts) {
-  __shared__ float red[kBackRuns][kBackLanes * kBackVec];
-  constexpr int V = kBackVec;
+                            bool w_f32, bool w_vec, float* parts) {
+  __shared__ float red[kBackRuns][kBackLanes * V];
   const int pack = blockIdx.x % packs, part_id = blockIdx.x / packs;  // part_id = b * chunks + chunk
   const int b = part_id / chunks, chunk = part_id - b * chunks;
-  const int lane = threadIdx.x, d0 = (pack * kBackLanes + lane) * V, n = a.dim - d0;
+  const int lane = threadIdx.x, d0 = (pack * kBackLanes + lane) * V;
+  const int n = d0 < a.dim ? V : 0;  // V divides dim
   const int t0 = (chunk * kBackRuns + threadIdx.y) * run, t1 = min(t0 + run, a.len);
   const int real = row_tokens(a.n_real, b, a.len);
-  const T* x = static_cast<const T*>(a.x) + b * a.x_batch_stride;
-  const T* dy = static_cast<const T*>(a.dy) + b * a.dy_batch_stride;
-  T* dx = static_cast<T*>(a.dx) + b * a.dx_batch_stride;
-  const int64_t state0 = (int64_t)b * a.dim * (W - 1);
+  const T* x = static_cast<const T*>(a.x) + b * a.x_batch_stride + d0;
+  const T* dy = static_cast<const T*>(a.dy) + b * a.dy_batch_stride + d0;
+  T* dx = static_cast<T*>(a.dx) + b * a.dx_batch_stride + d0;
+  const int64_t state0 = ((int64_t)b * a.dim + d0) * (W - 1);
   const T* init = a.initial_state ? static_cast<const T*>(a.initial_state) + state0 : nullptr;
   float w[V][W], bias[V], win[W][V], g[W][V], dw[V][W], db[V];  // [W - 1] is the newest token
-  load_taps<T, V, W>(w, a.weight, d0, n, w_f32);
 #pragma unroll
   for (int k = 0; k < V; ++k) {
-    bias[k] = a.bias && k < n ? weight_at<T>(a.bias, d0 + k, w_f32) : 0.f;
     db[k] = 0.f;
 #pragma unroll
     for (int j = 0; j < W; ++j) dw[k][j] = win[j][k] = g[j][k] = 0.f;
   }
   if (n > 0 && (t0 < t1 || t0 == 0)) {  // a row without tokens has an initial state's gradient
+    load_taps<T, V, W>(w, a.weight, d0, n, w_f32, w_vec);
 #pragma unroll
-    for (int j = 1; j < W; ++j) {
-      const int s = t0 + j - W;
+    for (int k = 0; k < V; ++k) bias[k] = a.bias ? weight_at<T>(a.bias, d0 + k, w_f32) : 0.f;
 #pragma unroll
-      for (int k = 0; k < V; ++k)
-        if (k < n && s < real) win[j][k] = token_at<T, W>(x, a.x_stride, init, d0 + k, s);
-    }
+    for (int j = 1; j < W; ++j)
+      load_token<T, V, W>(win[j], x, a.x_stride, init, t0 + j - W, real, n, true);
 #pragma unroll 4
     for (int t = t0; t < t1 + W - 1; ++t) {
-      const int m = t < real ? n : 0;
-      const Pack<T, V> px = load_pack<T, V>(x + t * a.x_stride + d0, m, vec);
-      const Pack<T, V> pd = load_pack<T, V>(dy + t * a.dy_stride + d0, m, vec);
+      const Pack<T, V> px = load_pack<T, V>(x + t * a.x_stride, t < real ? V : 0, true);
+      const Pack<T, V> pd = load_pack<T, V>(dy + t * a.dy_stride, t < real ? V : 0, true);
       const int s = t - (W - 1);
       float out[V];
 #pragma unroll
@@ -201,12 +208,11 @@ causal_conv_backward_kernel(salt_causal_conv_backward_args a, int packs, int chu
         if (s >= real) out[k] = 0.f;
       }
       if (s >= t0) {
-        store_pack<T, V>(dx + s * a.dx_stride + d0, out, n, vec);
+        store_pack<T, V>(dx + s * a.dx_stride, out, V, true);
       } else if (t0 == 0 && a.dinitial) {
         T* di = static_cast<T*>(a.dinitial) + state0;
 #pragma unroll
-        for (int k = 0; k < V; ++k)
-          if (k < n) di[(int64_t)(d0 + k) * (W - 1) + t] = from_f32<T>(out[k]);
+        for (int k = 0; k < V; ++k) di[k * (W - 1) + t] = from_f32<T>(out[k]);
       }
     }
   }
@@ -227,20 +233,6 @@ causal_conv_backward_kernel(salt_causal_conv_backward_args a, int packs, int chu
       part[(int64_t)j * a.dim + d] = s;
     }
   }
-}
-
-// Adds the partial sums (parts, width + 1, dim) into dweight (dim, width) and dbias (dim).
-__global__ void conv_weight_gradient(const float* __restrict__ parts, int64_t n_parts, int dim,
-                                     int width, float* dweight, float* dbias) {
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, n = (int64_t)dim * (width + 1);
-  if (i >= n) return;
-  const int j = (int)(i / dim), d = (int)(i - (int64_t)j * dim);
-  float s = 0.f;
-  for (int64_t p = 0; p < n_parts; ++p) s += parts[p * n + i];
-  if (j < width)
-    dweight[(int64_t)d * width + j] = s;
-  else if (dbias)
-    dbias[d] = s;
 }
 
 #define SALT_WITH_WIDTH(width, ...)                  \
@@ -266,11 +258,19 @@ int conv_run(int64_t packs, int32_t batch, int32_t len) {
 }
 
 struct ConvBackPlan {
-  int run, chunks, packs;
+  int v, run, chunks, packs;
 };
+#ifndef CBV
+#define CBV 4
+#endif
 ConvBackPlan conv_back_plan(const salt_causal_conv_backward_args& a) {
   ConvBackPlan p;
-  p.packs = (a.dim + kBackLanes * kBackVec - 1) / (kBackLanes * kBackVec);
+  const size_t ts = type_size(a.type);
+  const bool fits = a.dim % CBV == 0 && pack_rows(a.x, CBV, ts, a.x_batch_stride, a.x_stride) &&
+                    pack_rows(a.dy, CBV, ts, a.dy_batch_stride, a.dy_stride) &&
+                    pack_rows(a.dx, CBV, ts, a.dx_batch_stride, a.dx_stride);
+  p.v = fits ? CBV : 1;
+  p.packs = (a.dim + kBackLanes * p.v - 1) / (kBackLanes * p.v);
   p.run = 64;
   while (p.run > 8 && (int64_t)p.packs * a.batch *
                               ((a.len + p.run * kBackRuns - 1) / (p.run * kBackRuns)) <
@@ -284,17 +284,25 @@ ConvBackPlan conv_back_plan(const salt_causal_conv_backward_args& a) {
 
 cudaError_t causal_conv_launch(const salt_causal_conv_args& a, cudaStream_t st, int* launches) {
   if (a.batch == 0) return cudaSuccess;
-  const int packs = (a.dim + kVec - 1) / kVec;
+  const size_t ts = type_size(a.type);
+  auto fits = [&](int v) {
+    return a.dim % v == 0 && pack_rows(a.x, v, ts, a.x_batch_stride, a.x_stride) &&
+           pack_rows(a.out, v, ts, a.out_batch_stride, a.out_stride);
+  };
+  const int v = fits(kVec) ? kVec : fits(4) ? 4 : 1, packs = a.dim / v;
   const int run = conv_run(packs, a.batch, a.len);
   const int runs = std::max(1, (a.len + run - 1) / run);  // a row without tokens has a final state
-  const size_t ts = type_size(a.type);
-  const bool vec = vec_rows(a.x, ts, a.x_batch_stride, a.x_stride) &&
-                   vec_rows(a.out, ts, a.out_batch_stride, a.out_stride);
   const int64_t threads = (int64_t)packs * runs * a.batch;
   const unsigned blocks = (unsigned)((threads + 127) / 128);
   const bool w_f32 = a.weight_type == SALT_F32;
+  const bool w_vec = pack_rows(a.weight, v, w_f32 ? 4 : ts, 0);
   SALT_WITH_TYPE(a.type, T, SALT_WITH_WIDTH(a.width, {
-    causal_conv_kernel<T, W><<<blocks, 128, 0, st>>>(a, packs, runs, run, vec, w_f32);
+    if (v == kVec)
+      causal_conv_kernel<T, kVec, W><<<blocks, 128, 0, st>>>(a, packs, runs, run, w_f32, w_vec);
+    else if (v == 4)
+      causal_conv_kernel<T, 4, W><<<blocks, 128, 0, st>>>(a, packs, runs, run, w_f32, w_vec);
+    else
+      causal_conv_kernel<T, 1, W><<<blocks, 128, 0, st>>>(a, packs, runs, run, w_f32, w_vec);
   }));
   ++*launches;
   return cudaGetLastError();
@@ -321,28 +329,29 @@ size_t causal_conv_backward_bytes(const salt_causal_conv_backward_args& a) {
 cudaError_t causal_conv_backward_launch(const salt_causal_conv_backward_args& a, void* ws,
                                         cudaStream_t st, int* launches) {
   const ConvBackPlan p = conv_back_plan(a);
-  const size_t ts = type_size(a.type);
-  const bool vec = vec_rows(a.x, ts, a.x_batch_stride, a.x_stride) &&
-                   vec_rows(a.dy, ts, a.dy_batch_stride, a.dy_stride) &&
-                   vec_rows(a.dx, ts, a.dx_batch_stride, a.dx_stride);
   const bool w_f32 = a.weight_type == SALT_F32;
+  const bool w_vec = pack_rows(a.weight, p.v, w_f32 ? 4 : type_size(a.type), 0);
   float* parts = static_cast<float*>(ws);
   if (a.batch > 0) {
     const unsigned blocks = (unsigned)((int64_t)p.packs * p.chunks * a.batch);
     const dim3 block(kBackLanes, kBackRuns);
     SALT_WITH_TYPE(a.type, T, SALT_WITH_WIDTH(a.width, {
-      causal_conv_backward_kernel<T, W><<<blocks, block, 0, st>>>(a, p.packs, p.chunks, p.run, vec,
-                                                               w_f32, parts);
+      if (p.v == 1)
+        causal_conv_backward_kernel<T, 1, W>
+            <<<blocks, block, 0, st>>>(a, p.packs, p.chunks, p.run, w_f32, w_vec, parts);
+      else
+        causal_conv_backward_kernel<T, CBV, W>
+            <<<blocks, block, 0, st>>>(a, p.packs, p.chunks, p.run, w_f32, w_vec, parts);
     }));
     ++*launches;
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
   }
-  const int64_t n = (int64_t)a.dim * (a.width + 1);
-  conv_weight_gradient<<<(unsigned)((n + 127) / 128), 128, 0, st>>>(
-      parts, (int64_t)p.chunks * a.batch, a.dim, a.width, a.dweight, a.dbias);
   ++*launches;
-  return cudaGetLastError();
+  const int64_t dim = a.dim;
+  return sum_parts_launch(
+      parts, (int64_t)p.chunks * a.batch,
+      PartSums{dim * a.width, dim, 0, a.dweight, a.dbias, nullptr, a.width}, st);
 }
 
 }  // namespace salt

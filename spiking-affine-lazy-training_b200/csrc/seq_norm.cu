@@ -43,10 +43,10 @@ __device__ __forceinline__ float row_max(float v, int threads, float* red) {
   return s;
 }
 
-// A thread holds PER packs of 8 neighbouring elements, pack i of the row's thread t at element
-// 8 * (i * threads + t).  Rows of up to 1024 elements take a warp each, 4 to a block; wider ones a
-// block.
-template <typename T, typename R, int PER>
+// A thread holds PER packs of V neighbouring elements, pack i of the row's thread t at element
+// V * (i * threads + t); V is the widest that all rows' starts allow.  Rows of up to 1024 elements
+// take a warp each, 4 to a block; wider ones a block.
+template <typename T, typename R, int V, int PER>
 __global__ void __launch_bounds__(kRowThreadsMost)
 rms_norm_kernel(salt_rms_norm_args a, int threads, bool vec, bool w_f32) {
   __shared__ float red[32];
@@ -56,83 +56,89 @@ rms_norm_kernel(salt_rms_norm_args a, int threads, bool vec, bool w_f32) {
   if (row >= a.rows) return;  // a whole warp, or no thread of the block
   const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
   const R* res = static_cast<const R*>(a.residual);
-  float r[PER][kVec];
+  float r[PER][V];
   float sq = 0.f;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int at = kVec * (i * threads + t), n = a.dim - at;
-    const Pack<T, kVec> px = load_pack<T, kVec>(x + at, n, vec);
+    const int at = V * (i * threads + t), n = a.dim - at;
+    const Pack<T, V> px = load_pack<T, V>(x + at, n, vec);
 #pragma unroll
-    for (int k = 0; k < kVec; ++k) r[i][k] = to_f32(px.v[k]);
+    for (int k = 0; k < V; ++k) r[i][k] = to_f32(px.v[k]);
     if (res) {
-      const Pack<R, kVec> pr = load_pack<R, kVec>(res + row * a.residual_stride + at, n, vec);
+      const Pack<R, V> pr = load_pack<R, V>(res + row * a.residual_stride + at, n, vec);
 #pragma unroll
-      for (int k = 0; k < kVec; ++k) r[i][k] += to_f32(pr.v[k]);
+      for (int k = 0; k < V; ++k) r[i][k] += to_f32(pr.v[k]);
     }
 #pragma unroll
-    for (int k = 0; k < kVec; ++k) sq = fmaf(r[i][k], r[i][k], sq);
+    for (int k = 0; k < V; ++k) sq = fmaf(r[i][k], r[i][k], sq);
   }
   const float rstd = rsqrtf(row_sum(sq, threads, red) / (float)a.dim + a.eps);
   if (a.rstd && t == 0) a.rstd[row] = rstd;
   float most = 0.f;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int at = kVec * (i * threads + t), n = a.dim - at;
+    const int at = V * (i * threads + t), n = a.dim - at;
     if (a.residual_out)
-      store_pack<R, kVec>(static_cast<R*>(a.residual_out) + row * a.residual_out_stride + at, r[i],
+      store_pack<R, V>(static_cast<R*>(a.residual_out) + row * a.residual_out_stride + at, r[i],
                           n, vec);
+    float w[V];
+    load_weights<T, V>(w, a.weight, at, n, w_f32, vec);
 #pragma unroll
-    for (int k = 0; k < kVec; ++k) {
-      const float w = k < n ? weight_at<T>(a.weight, at + k, w_f32) : 0.f;
-      r[i][k] *= rstd * w;
+    for (int k = 0; k < V; ++k) {
+      r[i][k] *= rstd * w[k];
       most = fmaxf(most, fabsf(r[i][k]));
     }
     if (!a.scale) {
-      store_pack<T, kVec>(static_cast<T*>(a.out) + row * a.out_stride + at, r[i], n, vec);
+      store_pack<T, V>(static_cast<T*>(a.out) + row * a.out_stride + at, r[i], n, vec);
     } else if (a.group) {
-      // group / 8 neighbouring lanes hold a group (4 to 32 of them, so never across warps)
+      // group / V neighbouring lanes hold a group (at V = 8, which 8 bits always take: 4 to 32, never across warps)
       float m = 0.f;
 #pragma unroll
-      for (int k = 0; k < kVec; ++k) m = fmaxf(m, fabsf(r[i][k]));
-      for (int o = a.group / kVec / 2; o; o >>= 1)
+      for (int k = 0; k < V; ++k) m = fmaxf(m, fabsf(r[i][k]));
+      for (int o = a.group / V / 2; o; o >>= 1)
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       const float scale = m > 0.f ? m / kE4m3Max : 1.f;
       if (n > 0 && at % a.group == 0)
         a.scale[row * ((a.dim + a.group - 1) / a.group) + at / a.group] = scale;
+      const float by = 1.f / scale;
 #pragma unroll
-      for (int k = 0; k < kVec; ++k) r[i][k] /= scale;
+      for (int k = 0; k < V; ++k) r[i][k] *= by;
     }
   }
   if (!a.scale) return;
   if (!a.group) {
     const float m = row_max(most, threads, red), scale = m > 0.f ? m / kE4m3Max : 1.f;
     if (t == 0) a.scale[row] = scale;
+    const float by = 1.f / scale;
 #pragma unroll
     for (int i = 0; i < PER; ++i)
 #pragma unroll
-      for (int k = 0; k < kVec; ++k) r[i][k] /= scale;
+      for (int k = 0; k < V; ++k) r[i][k] *= by;
   }
   uint8_t* out = static_cast<uint8_t*>(a.out) + row * a.out_stride;
-  const bool wide = (reinterpret_cast<uintptr_t>(out) & 7) == 0;
+  const bool wide = V == 8 && (reinterpret_cast<uintptr_t>(out) & 7) == 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int at = kVec * (i * threads + t), n = a.dim - at;
-    alignas(8) uint8_t q[kVec];
+    const int at = V * (i * threads + t), n = a.dim - at;
+    alignas(8) uint8_t q[V < 2 ? 2 : V];
 #pragma unroll
-    for (int k = 0; k < kVec; ++k)
-      q[k] = __nv_cvt_float_to_fp8(r[i][k], __NV_SATFINITE, __NV_E4M3);
-    if (wide && n >= kVec)
+    for (int k = 0; k + 1 < V; k += 2)
+      *reinterpret_cast<uint16_t*>(q + k) =
+          __nv_cvt_float2_to_fp8x2(make_float2(r[i][k], r[i][k + 1]), __NV_SATFINITE, __NV_E4M3);
+    if (wide && n >= V) {
       *reinterpret_cast<uint2*>(out + at) = *reinterpret_cast<const uint2*>(q);
-    else
-      for (int k = 0; k < kVec; ++k)
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; ++k)
         if (k < n) out[at + k] = q[k];
+    }
   }
 }
 
 // The gradient.  Blocks walk over rows with a fixed set of columns for each thread, so that the
 // weight's gradient stays in registers; each block (each warp, for narrow rows) writes one partial
 // row of it, which sum_parts adds up in order.
-template <typename T, typename R, int PER>
+template <typename T, typename R, int V, int PER>
 __global__ void __launch_bounds__(kRowThreadsMost)
 rms_norm_backward_kernel(salt_rms_norm_backward_args a, int threads, bool vec, bool w_f32,
                          float* parts) {
@@ -142,29 +148,28 @@ rms_norm_backward_kernel(salt_rms_norm_backward_args a, int threads, bool vec, b
   const int64_t worker = by_warp ? (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)
                                  : (int64_t)blockIdx.x;
   const int64_t workers = by_warp ? (int64_t)gridDim.x * (blockDim.x >> 5) : (int64_t)gridDim.x;
-  float w[PER][kVec], dw[PER][kVec];
+  float w[PER][V], dw[PER][V];
 #pragma unroll
-  for (int i = 0; i < PER; ++i)
+  for (int i = 0; i < PER; ++i) {
+    const int at = V * (i * threads + t);
+    load_weights<T, V>(w[i], a.weight, at, a.dim - at, w_f32, vec);
 #pragma unroll
-    for (int k = 0; k < kVec; ++k) {
-      const int at = kVec * (i * threads + t) + k;
-      w[i][k] = at < a.dim ? weight_at<T>(a.weight, at, w_f32) : 0.f;
-      dw[i][k] = 0.f;
-    }
+    for (int k = 0; k < V; ++k) dw[i][k] = 0.f;
+  }
   for (int64_t row = worker; row < a.rows; row += workers) {
     const T* dy = static_cast<const T*>(a.dy) + row * a.dy_stride;
     const R* x = static_cast<const R*>(a.x) + row * a.x_stride;
     const R* dres = static_cast<const R*>(a.dresidual);
     const float rstd = a.rstd[row];
-    float h[PER][kVec], g[PER][kVec];
+    float h[PER][V], g[PER][V];
     float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int at = kVec * (i * threads + t), n = a.dim - at;
-      const Pack<T, kVec> pdy = load_pack<T, kVec>(dy + at, n, vec);
-      const Pack<R, kVec> px = load_pack<R, kVec>(x + at, n, vec);
+      const int at = V * (i * threads + t), n = a.dim - at;
+      const Pack<T, V> pdy = load_pack<T, V>(dy + at, n, vec);
+      const Pack<R, V> px = load_pack<R, V>(x + at, n, vec);
 #pragma unroll
-      for (int k = 0; k < kVec; ++k) {
+      for (int k = 0; k < V; ++k) {
         h[i][k] = to_f32(px.v[k]) * rstd;
         const float d = to_f32(pdy.v[k]);
         dw[i][k] = fmaf(d, h[i][k], dw[i][k]);
@@ -175,53 +180,77 @@ rms_norm_backward_kernel(salt_rms_norm_backward_args a, int threads, bool vec, b
     const float mean = row_sum(dot, threads, red) / (float)a.dim;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int at = kVec * (i * threads + t), n = a.dim - at;
-      Pack<R, kVec> pr;
-      if (dres) pr = load_pack<R, kVec>(dres + row * a.dresidual_stride + at, n, vec);
-      float dx[kVec];
+      const int at = V * (i * threads + t), n = a.dim - at;
+      Pack<R, V> pr;
+      if (dres) pr = load_pack<R, V>(dres + row * a.dresidual_stride + at, n, vec);
+      float dx[V];
 #pragma unroll
-      for (int k = 0; k < kVec; ++k) {
+      for (int k = 0; k < V; ++k) {
         dx[k] = rstd * fmaf(-h[i][k], mean, g[i][k]);
         if (dres) dx[k] += to_f32(pr.v[k]);
       }
-      store_pack<R, kVec>(static_cast<R*>(a.dx) + row * a.dx_stride + at, dx, n, vec);
+      store_pack<R, V>(static_cast<R*>(a.dx) + row * a.dx_stride + at, dx, n, vec);
     }
   }
   if (!parts) return;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int at = kVec * (i * threads + t);
+    const int at = V * (i * threads + t);
 #pragma unroll
-    for (int k = 0; k < kVec; ++k)
+    for (int k = 0; k < V; ++k)
       if (at + k < a.dim) parts[worker * a.dim + at + k] = dw[i][k];
   }
 }
 
-__global__ void sum_parts_kernel(const float* __restrict__ in, int64_t parts, int64_t n,
-                                 float* __restrict__ out) {
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= n) return;
+// A block takes 32 elements; thread row y adds the parts y, y + rows, ... and the first row adds
+// the rows' sums in order.
+template <int ROWS>
+__global__ void __launch_bounds__(32 * ROWS)
+sum_parts_kernel(const float* __restrict__ in, int64_t parts, int64_t n, PartSums to) {
+  __shared__ float red[ROWS][32];
+  const int64_t i = (int64_t)blockIdx.x * 32 + threadIdx.x;
   float s = 0.f;
-  for (int64_t p = 0; p < parts; ++p) s += in[p * n + i];
-  out[i] = s;
+  if (i < n) {
+#pragma unroll 4
+    for (int64_t p = threadIdx.y; p < parts; p += ROWS) s += in[p * n + i];
+  }
+  red[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.y != 0 || i >= n) return;
+#pragma unroll
+  for (int r = 1; r < ROWS; ++r) s += red[r][threadIdx.x];
+  if (i < to.n0) {
+    const int64_t dim = to.width ? to.n0 / to.width : 1;
+    if (to.out0) to.out0[to.width ? i % dim * to.width + i / dim : i] = s;
+  } else if (i < to.n0 + to.n1) {
+    if (to.out1) to.out1[i - to.n0] = s;
+  } else if (to.out2) {
+    to.out2[i - to.n0 - to.n1] = s;
+  }
 }
 
 struct NormPlan {
-  int threads, per, block;
+  int v, threads, per, block;
   int64_t blocks;
 };
 
-NormPlan norm_plan(int32_t rows, int32_t dim) {
+NormPlan norm_plan(int32_t rows, int32_t dim, int v) {
   NormPlan p;
-  const int packs = (dim + kVec - 1) / kVec;
+  p.v = v;
+  const int packs = (dim + v - 1) / v, most = 32 / v;  // a thread holds up to 32 elements
   if (dim <= kWarpRowMost) {
     p.threads = 32;
     p.block = 128;
     p.blocks = ((int64_t)rows + 3) / 4;
-    p.per = packs <= 32 ? 1 : packs <= 64 ? 2 : 4;
+    p.per = (packs + 31) / 32;
   } else {
-    p.per = packs <= 512 ? 1 : packs <= 1024 ? 2 : 4;
-    p.threads = p.block = (((packs + p.per - 1) / p.per) + 31) / 32 * 32;
+    p.per = std::max((packs + kRowThreadsMost - 1) / kRowThreadsMost, 8 / v);
+  }
+  int per = std::max(1, most / 4);  // 8, 16 or 32 elements
+  while (per < p.per) per *= 2;
+  p.per = per;
+  if (dim > kWarpRowMost) {
+    p.threads = p.block = ((packs + per - 1) / per + 31) / 32 * 32;
     p.blocks = rows;
   }
   return p;
@@ -239,73 +268,112 @@ void norm_back_grid(const NormPlan& p, int32_t rows, int* blocks, int* workers) 
 
 }  // namespace
 
-cudaError_t sum_parts_launch(const float* in, int64_t parts, int64_t n, float* out,
-                             cudaStream_t st) {
-  if (n > 0) sum_parts_kernel<<<(unsigned)((n + 127) / 128), 128, 0, st>>>(in, parts, n, out);
+cudaError_t sum_parts_launch(const float* in, int64_t parts, const PartSums& to, cudaStream_t st) {
+  const int64_t n = to.n0 + to.n1 + to.n2;
+  if (n == 0) return cudaSuccess;
+  const unsigned blocks = (unsigned)((n + 31) / 32);
+  if (parts <= 16)
+    sum_parts_kernel<4><<<blocks, dim3(32, 4), 0, st>>>(in, parts, n, to);
+  else
+    sum_parts_kernel<32><<<blocks, dim3(32, 32), 0, st>>>(in, parts, n, to);
   return cudaGetLastError();
 }
 
-#define SALT_NORM_PER(kernel, per, T, R, ...)             \
-  do {                                                    \
-    if ((per) == 1)                                       \
-      kernel<T, R, 1> __VA_ARGS__;                        \
-    else if ((per) == 2)                                  \
-      kernel<T, R, 2> __VA_ARGS__;                        \
-    else                                                  \
-      kernel<T, R, 4> __VA_ARGS__;                        \
+// Elements per pack by V, packs of a thread by PER.
+#define SALT_NORM_SHAPE(p, kernel, T, R, ...)                      \
+  do {                                                             \
+    if ((p).v == 8) {                                              \
+      if ((p).per == 1)                                            \
+        kernel<T, R, 8, 1> __VA_ARGS__;                            \
+      else if ((p).per == 2)                                       \
+        kernel<T, R, 8, 2> __VA_ARGS__;                            \
+      else                                                         \
+        kernel<T, R, 8, 4> __VA_ARGS__;                            \
+    } else if ((p).v == 4) {                                       \
+      if ((p).per == 2)                                            \
+        kernel<T, R, 4, 2> __VA_ARGS__;                            \
+      else if ((p).per == 4)                                       \
+        kernel<T, R, 4, 4> __VA_ARGS__;                            \
+      else                                                         \
+        kernel<T, R, 4, 8> __VA_ARGS__;                            \
+    } else {                                                       \
+      if ((p).per == 8)                                            \
+        kernel<T, R, 1, 8> __VA_ARGS__;                            \
+      else if ((p).per == 16)                                      \
+        kernel<T, R, 1, 16> __VA_ARGS__;                           \
+      else                                                         \
+        kernel<T, R, 1, 32> __VA_ARGS__;                           \
+    }                                                              \
   } while (0)
 
 cudaError_t rms_norm_launch(const salt_rms_norm_args& a, cudaStream_t st, int* launches) {
   if (a.rows == 0) return cudaSuccess;
-  const NormPlan p = norm_plan(a.rows, a.dim);
   const size_t ts = type_size(a.type), rs = type_size(a.residual_type);
-  const bool vec = vec_rows(a.x, ts, a.x_stride) && vec_rows(a.residual, rs, a.residual_stride) &&
-                   vec_rows(a.residual_out, rs, a.residual_out_stride) &&
-                   (a.scale || vec_rows(a.out, ts, a.out_stride));
   const bool w_f32 = a.weight_type == SALT_F32;
+  auto fits = [&](int v) {
+    return a.dim % v == 0 && pack_rows(a.x, v, ts, a.x_stride) &&
+           pack_rows(a.residual, v, rs, a.residual_stride) &&
+           pack_rows(a.residual_out, v, rs, a.residual_out_stride) &&
+           pack_rows(a.weight, v, w_f32 ? 4 : ts, 0) &&
+           (a.scale || pack_rows(a.out, v, ts, a.out_stride));
+  };
+  // a group's lanes are counted in packs of 8, whether those can be moved at once or not
+  const bool vec = fits(8) || (!a.scale && fits(4));
+  const NormPlan p = norm_plan(a.rows, a.dim, a.scale || fits(8) ? 8 : vec ? 4 : 1);
   SALT_WITH_TYPE(a.type, T, {
     if (a.residual_type == SALT_F32)
-      SALT_NORM_PER(rms_norm_kernel, p.per, T, float,
-                    <<<(unsigned)p.blocks, p.block, 0, st>>>(a, p.threads, vec, w_f32));
+      SALT_NORM_SHAPE(p, rms_norm_kernel, T, float,
+                      <<<(unsigned)p.blocks, p.block, 0, st>>>(a, p.threads, vec, w_f32));
     else
-      SALT_NORM_PER(rms_norm_kernel, p.per, T, T,
-                    <<<(unsigned)p.blocks, p.block, 0, st>>>(a, p.threads, vec, w_f32));
+      SALT_NORM_SHAPE(p, rms_norm_kernel, T, T,
+                      <<<(unsigned)p.blocks, p.block, 0, st>>>(a, p.threads, vec, w_f32));
   });
   ++*launches;
   return cudaGetLastError();
 }
 
+namespace {
+NormPlan norm_back_plan(const salt_rms_norm_backward_args& a) {
+  const size_t ts = type_size(a.type), rs = type_size(a.residual_type);
+  auto fits = [&](int v) {
+    return a.dim % v == 0 && pack_rows(a.dy, v, ts, a.dy_stride) &&
+           pack_rows(a.x, v, rs, a.x_stride) &&
+           pack_rows(a.dresidual, v, rs, a.dresidual_stride) &&
+           pack_rows(a.dx, v, rs, a.dx_stride) &&
+           pack_rows(a.weight, v, a.weight_type == SALT_F32 ? 4 : ts, 0);
+  };
+  return norm_plan(a.rows, a.dim, fits(8) ? 8 : fits(4) ? 4 : 1);
+}
+}  // namespace
+
 size_t rms_norm_backward_bytes(const salt_rms_norm_backward_args& a) {
   if (!a.dweight) return 0;
   int blocks, workers;
-  norm_back_grid(norm_plan(a.rows, a.dim), a.rows, &blocks, &workers);
+  norm_back_grid(norm_back_plan(a), a.rows, &blocks, &workers);
   return (size_t)workers * a.dim * sizeof(float);
 }
 
 cudaError_t rms_norm_backward_launch(const salt_rms_norm_backward_args& a, void* ws,
                                      cudaStream_t st, int* launches) {
-  const NormPlan p = norm_plan(a.rows, a.dim);
+  const NormPlan p = norm_back_plan(a);
   int blocks, workers;
   norm_back_grid(p, a.rows, &blocks, &workers);
-  const size_t ts = type_size(a.type), rs = type_size(a.residual_type);
-  const bool vec = vec_rows(a.dy, ts, a.dy_stride) && vec_rows(a.x, rs, a.x_stride) &&
-                   vec_rows(a.dresidual, rs, a.dresidual_stride) &&
-                   vec_rows(a.dx, rs, a.dx_stride);
-  const bool w_f32 = a.weight_type == SALT_F32;
+  const bool vec = p.v > 1, w_f32 = a.weight_type == SALT_F32;
   float* parts = a.dweight ? static_cast<float*>(ws) : nullptr;
   SALT_WITH_TYPE(a.type, T, {
     if (a.residual_type == SALT_F32)
-      SALT_NORM_PER(rms_norm_backward_kernel, p.per, T, float,
-                    <<<blocks, p.block, 0, st>>>(a, p.threads, vec, w_f32, parts));
+      SALT_NORM_SHAPE(p, rms_norm_backward_kernel, T, float,
+                      <<<blocks, p.block, 0, st>>>(a, p.threads, vec, w_f32, parts));
     else
-      SALT_NORM_PER(rms_norm_backward_kernel, p.per, T, T,
-                    <<<blocks, p.block, 0, st>>>(a, p.threads, vec, w_f32, parts));
+      SALT_NORM_SHAPE(p, rms_norm_backward_kernel, T, T,
+                      <<<blocks, p.block, 0, st>>>(a, p.threads, vec, w_f32, parts));
   });
   ++*launches;
-  cudaError_t e = cudaGetLastError();
+  const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || !parts) return e;
   ++*launches;
-  return sum_parts_launch(parts, workers, a.dim, a.dweight, st);
+  return sum_parts_launch(parts, workers, PartSums{a.dim, 0, 0, a.dweight, nullptr, nullptr, 0},
+                          st);
 }
 
 }  // namespace salt

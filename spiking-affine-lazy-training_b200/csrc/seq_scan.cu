@@ -301,7 +301,19 @@ struct StepShape {
   static constexpr int kThreads = kStepChannels * LPC;
 };
 
-template <typename T, class S>
+// What one token's row needs before its arithmetic: all loads of a row are issued together, and
+// those of the next row in front of this row's arithmetic.
+template <typename T, int NS>
+struct StepRow {
+  float h[NS];
+  T x, delta, z;
+  Pack<T, 4> B[NS / 4], C[NS / 4];
+  float* pool;  // NULL: an empty row
+};
+
+// A block holds A of its 32 channels and walks over `rows` tokens' rows.  The states' bytes, read
+// and written once, are the bound: 8 a state and token, against 2 of x, z, delta and out.
+template <typename T, class S, bool VEC>
 __global__ void __launch_bounds__(S::kThreads)
 selective_scan_step_kernel(salt_selective_scan_step_args a, int blocks, int rows, bool svec) {
   constexpr int NS = S::NS, LPC = S::LPC;
@@ -310,45 +322,57 @@ selective_scan_step_kernel(salt_selective_scan_step_args a, int blocks, int rows
   const int ch = tid / LPC, n0 = tid % LPC * NS, ns = a.state - n0;
   const bool mine = ch < cb.n;
   const int64_t d = cb.d0 + (mine ? ch : 0);
+  const int64_t begin = (int64_t)part * rows, end = min((int64_t)a.batch, begin + rows);
+  auto load = [&](StepRow<T, NS>& r, int64_t b) {
+    const int64_t slot = a.slots ? a.slots[b] : b;
+    r.pool = slot >= 0 && slot < a.n_slots ? a.pool + (slot * a.dim + d) * a.state + n0 : nullptr;
+    if (!r.pool) return;
+    load_states<NS>(r.h, r.pool, ns, svec);
+    r.x = static_cast<const T*>(a.x)[b * a.x_stride + d];
+    r.delta = static_cast<const T*>(a.delta)[b * a.delta_stride + d];
+    if (a.z) r.z = static_cast<const T*>(a.z)[b * a.z_stride + d];
+    const int64_t at = (int64_t)cb.group * a.state + n0;
+#pragma unroll
+    for (int i = 0; i < NS; i += 4) {
+      r.B[i / 4] =
+          load_pack<T, 4>(static_cast<const T*>(a.B) + b * a.B_stride + at + i, ns - i, VEC);
+      r.C[i / 4] =
+          load_pack<T, 4>(static_cast<const T*>(a.C) + b * a.C_stride + at + i, ns - i, VEC);
+    }
+  };
+  StepRow<T, NS> now, next;
+  load(now, begin);
   float A2[NS];
   load_states<NS>(A2, a.A + d * a.state + n0, ns, svec);
 #pragma unroll
   for (int i = 0; i < NS; ++i) A2[i] *= kLog2e;
   const float bias = a.delta_bias ? a.delta_bias[d] : 0.f, skip = a.D ? a.D[d] : 0.f;
-  for (int64_t b = (int64_t)part * rows; b < min((int64_t)a.batch, (int64_t)(part + 1) * rows);
-       ++b) {
-    const int64_t slot = a.slots ? a.slots[b] : b;
+  for (int64_t b = begin; b < end; ++b) {
+    if (b + 1 < end) load(next, b + 1);
     T* out = static_cast<T*>(a.out) + b * a.out_stride + d;
-    if (slot < 0 || slot >= a.n_slots) {
-      if (mine && n0 == 0) *out = from_f32<T>(0.f);
-      continue;  // the whole block
-    }
-    float* pool = a.pool + (slot * a.dim + d) * a.state + n0;
-    float h[NS];
-    load_states<NS>(h, pool, ns, svec);
-    const float x = to_f32(static_cast<const T*>(a.x)[b * a.x_stride + d]);
-    const float s =
-        scan_step(to_f32(static_cast<const T*>(a.delta)[b * a.delta_stride + d]) + bias, a.softplus);
-    const T* B = static_cast<const T*>(a.B) + b * a.B_stride + (int64_t)cb.group * a.state + n0;
-    const T* C = static_cast<const T*>(a.C) + b * a.C_stride + (int64_t)cb.group * a.state + n0;
-    float y = 0.f;
+    if (now.pool) {
+      const float x = to_f32(now.x), s = scan_step(to_f32(now.delta) + bias, a.softplus);
+      float y = 0.f;
 #pragma unroll
-    for (int i = 0; i < NS; ++i) {
-      const float bn = i < ns ? to_f32(B[i]) : 0.f, cn = i < ns ? to_f32(C[i]) : 0.f;
-      h[i] = fmaf(exp2_fast(A2[i] * s), h[i], s * x * bn);
-      y = fmaf(h[i], cn, y);
-    }
-    if (mine) store_states<NS>(pool, h, ns, svec);
-#pragma unroll
-    for (int o = 1; o < LPC; o <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-    if (mine && n0 == 0) {
-      y = fmaf(skip, x, y);
-      if (a.z) {
-        const float z = to_f32(static_cast<const T*>(a.z)[b * a.z_stride + d]);
-        y *= z * sigmoid(z);
+      for (int i = 0; i < NS; ++i) {
+        now.h[i] = fmaf(exp2_fast(A2[i] * s), now.h[i], s * x * to_f32(now.B[i / 4].v[i % 4]));
+        y = fmaf(now.h[i], to_f32(now.C[i / 4].v[i % 4]), y);
       }
-      *out = from_f32<T>(y);
+      if (mine) store_states<NS>(now.pool, now.h, ns, svec);
+#pragma unroll
+      for (int o = 1; o < LPC; o <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+      if (mine && n0 == 0) {
+        y = fmaf(skip, x, y);
+        if (a.z) {
+          const float z = to_f32(now.z);
+          y *= z * sigmoid(z);
+        }
+        *out = from_f32<T>(y);
+      }
+    } else if (mine && n0 == 0) {
+      *out = from_f32<T>(0.f);  // the whole block skips an empty row
     }
+    now = next;
   }
 }
 
@@ -446,14 +470,26 @@ cudaError_t selective_scan_step_launch(const salt_selective_scan_step_args& a, c
                                        int* launches) {
   if (a.batch == 0) return cudaSuccess;
   const int blocks = scan_blocks(a.dim, a.groups, kStepChannels);
-  // A's rows are loaded once for the token rows that a block walks over
+  // A is loaded once for the rows that a block walks over
+#ifndef STEPB
+#define STEPB 8
+#endif
   int rows = 1;
-  while (rows < 8 && (int64_t)blocks * ((a.batch + 2 * rows - 1) / (2 * rows)) >= 148 * 8) rows *= 2;
+  while (rows < 8 && (int64_t)blocks * ((a.batch + 2 * rows - 1) / (2 * rows)) >= 148 * STEPB)
+    rows *= 2;
   const int parts = (a.batch + rows - 1) / rows;
+  const size_t ts = type_size(a.type);
   const bool svec = a.state % 4 == 0 && aligned16(a.A) && aligned16(a.pool);
+  const bool vec = a.state % 4 == 0 && pack_rows(a.B, 4, ts, a.B_stride) &&
+                   pack_rows(a.C, 4, ts, a.C_stride);
+  const unsigned grid = (unsigned)((int64_t)blocks * parts);
   SALT_WITH_TYPE(a.type, T, SALT_STEP_SHAPE(a.state, S, {
-    selective_scan_step_kernel<T, S>
-        <<<(unsigned)((int64_t)blocks * parts), S::kThreads, 0, st>>>(a, blocks, rows, svec);
+    if (vec)
+      selective_scan_step_kernel<T, S, true>
+          <<<grid, S::kThreads, 0, st>>>(a, blocks, rows, svec);
+    else
+      selective_scan_step_kernel<T, S, false>
+          <<<grid, S::kThreads, 0, st>>>(a, blocks, rows, svec);
   }));
   ++*launches;
   return cudaGetLastError();

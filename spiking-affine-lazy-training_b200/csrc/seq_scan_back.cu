@@ -82,7 +82,7 @@ __device__ __forceinline__ f32x2 shuffle2(f32x2 v, int mask) {
 
 struct BackParts {
   float* BC;            // (blocks, batch, len, 2 state): a block's dB and dC of its channels
-  float *A, *D, *bias;  // (batch * chunks, dim, state), (batch * chunks, dim) twice
+  float* sums;          // (batch * chunks, dim * (state + 2)): dA, dD and ddelta_bias
   int per_group;        // blocks of one group
 };
 
@@ -437,13 +437,15 @@ selective_scan_backward_kernel(salt_selective_scan_backward_args a, ScanSplit sp
     __syncthreads();
   }
 
+  float* sums = parts.sums + (b * sp.chunks + c) * a.dim * (a.state + 2);
 #pragma unroll
   for (int j = 0; j < CPT; ++j) {
     if (!mine[j]) continue;
     const float4 v = sm.dA[j][tid];
     float f[NS] = {v.x, v.y, v.z, v.w};
     order.turn(f);
-    store_states<NS>(parts.A + ((b * sp.chunks + c) * a.dim + d[j]) * a.state + n0, f, ns, svec);
+    // a row of sums has dim * (state + 2) values
+    store_states<NS>(sums + d[j] * a.state + n0, f, ns, svec && a.dim % 2 == 0);
     if (c == 0 && a.dinitial) {
       const float2 lo = halves(carry[j][0]), hi = halves(carry[j][1]);
       float r[NS] = {lo.x, lo.y, hi.x, hi.y};
@@ -465,9 +467,9 @@ selective_scan_backward_kernel(salt_selective_scan_backward_args a, ScanSplit sp
       sb += sm.to[q][i];
       ss += sm.g[q][i];
     }
-    const int64_t to = (b * sp.chunks + c) * a.dim + cb.d0 + i;
-    parts.bias[to] = sb;
-    parts.D[to] = ss;
+    float* to = sums + (int64_t)a.dim * a.state + cb.d0 + i;
+    to[0] = ss;
+    to[a.dim] = sb;
   }
 }
 
@@ -659,7 +661,7 @@ cudaError_t back_launch(const salt_selective_scan_backward_args& a, const ScanSp
 
 struct BackPlan {
   int blocks, chunks, chunk_len;
-  size_t state, steps, BC, A, D, bias, bytes;  // offsets in floats, and the whole in bytes
+  size_t state, steps, BC, sums, bytes;  // offsets in floats, and the whole in bytes
 };
 
 BackPlan back_plan(const salt_selective_scan_backward_args& a) {
@@ -677,9 +679,7 @@ BackPlan back_plan(const salt_selective_scan_backward_args& a) {
   p.state = take(p.chunks > 1 ? rows * a.state : 0);
   p.steps = take(p.chunks > 1 ? rows : 0);
   p.BC = take((size_t)p.blocks * a.batch * a.len * 2 * a.state);
-  p.A = take(rows * a.state);
-  p.D = take(rows);
-  p.bias = take(rows);
+  p.sums = take(rows * (a.state + 2));
   p.bytes = at * sizeof(float);
   return p;
 }
@@ -695,7 +695,7 @@ cudaError_t selective_scan_backward_launch(const salt_selective_scan_backward_ar
   const BackPlan p = back_plan(a);
   float* base = static_cast<float*>(ws);
   const ScanSplit sp{p.chunks, p.chunk_len, base + p.state, base + p.steps};
-  const BackParts parts{base + p.BC, base + p.A, base + p.D, base + p.bias, p.blocks / a.groups};
+  const BackParts parts{base + p.BC, base + p.sums, p.blocks / a.groups};
   const size_t ts = type_size(a.type);
   // the widest copies that no row's start and end stand against
   auto fits = [&](int64_t bytes) {
@@ -733,17 +733,10 @@ cudaError_t selective_scan_backward_launch(const salt_selective_scan_backward_ar
       e = cudaGetLastError();
     }
   }
-  const int64_t rows = (int64_t)a.batch * p.chunks;
   if (e == cudaSuccess) {
-    e = sum_parts_launch(parts.A, rows, (int64_t)a.dim * a.state, a.dA, st);
-    ++*launches;
-  }
-  if (e == cudaSuccess && a.dD) {
-    e = sum_parts_launch(parts.D, rows, a.dim, a.dD, st);
-    ++*launches;
-  }
-  if (e == cudaSuccess && a.ddelta_bias) {
-    e = sum_parts_launch(parts.bias, rows, a.dim, a.ddelta_bias, st);
+    const int64_t dim = a.dim;
+    e = sum_parts_launch(parts.sums, (int64_t)a.batch * p.chunks,
+                         PartSums{dim * a.state, dim, dim, a.dA, a.dD, a.ddelta_bias, 0}, st);
     ++*launches;
   }
   return e;

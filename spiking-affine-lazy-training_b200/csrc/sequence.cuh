@@ -1,6 +1,7 @@
 // Shared device helpers and launch declarations of the sequence operators (root-mean-square norm,
 // short causal convolution, selective state space scan).
 #pragma once
+#include <algorithm>
 #include <cstddef>
 #include <cstdint>
 #include <cuda_bf16.h>
@@ -57,6 +58,21 @@ __device__ __forceinline__ void store_pack(T* p, const float* f, int n, bool vec
 #pragma unroll
     for (int i = 0; i < N; ++i)
       if (i < n) p[i] = r.v[i];
+  }
+}
+
+// N neighbouring weights that hold T or float32; n as in load_pack.
+template <typename T, int N>
+__device__ __forceinline__ void load_weights(float (&f)[N], const void* w, int64_t at, int n,
+                                             bool is_f32, bool vec) {
+  if (is_f32) {
+    const Pack<float, N> p = load_pack<float, N>(static_cast<const float*>(w) + at, n, vec);
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = p.v[i];
+  } else {
+    const Pack<T, N> p = load_pack<T, N>(static_cast<const T*>(w) + at, n, vec);
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = to_f32(p.v[i]);
   }
 }
 
@@ -196,10 +212,16 @@ size_t selective_scan_backward_bytes(const salt_selective_scan_backward_args& a)
 cudaError_t selective_scan_backward_launch(const salt_selective_scan_backward_args& a, void* ws,
                                            cudaStream_t st, int* launches);
 
-// Sums `parts` partial arrays of n float32 in order (part p at in + p * n): the second stage of
-// every weight gradient.
-cudaError_t sum_parts_launch(const float* in, int64_t parts, int64_t n, float* out,
-                             cudaStream_t st);
+// The second stage of every weight gradient: sums `parts` partial arrays of float32, part p at
+// in + p * n, in an order that their number alone decides.  A part holds up to three gradients of
+// n0, n1 and n2 elements one after the other (n is their sum; an out that is NULL is left out).
+// With width set, the first is (width, n0 / width) there and comes out transposed.
+struct PartSums {
+  int64_t n0, n1, n2;
+  float *out0, *out1, *out2;
+  int width;
+};
+cudaError_t sum_parts_launch(const float* in, int64_t parts, const PartSums& to, cudaStream_t st);
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 // Whether rows at p with these strides (in elements) start on 16-byte boundaries.
@@ -212,6 +234,10 @@ inline bool packed_rows(const void* p, int64_t bytes, size_t size, int64_t s0, i
          (int64_t)(s1 * size) % bytes == 0;
 }
 inline size_t type_size(int32_t type) { return type == SALT_F32 ? 4 : 2; }
+// Whether rows at p can be moved in packs of `n` elements.
+inline bool pack_rows(const void* p, int n, size_t size, int64_t s0, int64_t s1 = 0) {
+  return !p || packed_rows(p, std::min<int64_t>(16, n * size), size, s0, s1);
+}
 
 // Calls F<T>(...) for the C type that `type` names.
 #define SALT_WITH_TYPE(type, T, ...)          \
