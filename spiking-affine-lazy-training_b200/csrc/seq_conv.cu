@@ -12,18 +12,33 @@ namespace salt {
 
 namespace {
 
-// weight[d][k] of channels d0 .. d0 + N, of which n are there; tap W - 1 is the newest input's.
-// The N W values lie together: W packs.
-template <typename T, int N, int W>
-__device__ __forceinline__ void load_taps(float (&w)[N][W], const void* weight, int d0, int n,
+// Values of V channels as pairs; one channel has a zero beside it.
+template <int V>
+__device__ __forceinline__ void to_pairs(f32x2 (&p)[(V + 1) / 2], const float* f) {
+#pragma unroll
+  for (int k = 0; k < (V + 1) / 2; ++k) p[k] = pair(f[2 * k], V == 1 ? 0.f : f[2 * k + (V > 1)]);
+}
+
+// weight[d][j] of channels d0 .. d0 + V, of which n (V or none) are there, as w[j]; tap W - 1 is the
+// newest input's.  The V W values lie together: W packs.
+template <typename T, int V, int W>
+__device__ __forceinline__ void load_taps(f32x2 (&w)[W][(V + 1) / 2], f32x2 (&bias)[(V + 1) / 2],
+                                          const void* weight, const void* from, int d0, int n,
                                           bool w_f32, bool vec) {
+  float f[W][V];
 #pragma unroll
   for (int i = 0; i < W; ++i) {
-    float f[N];
-    load_weights<T, N>(f, weight, (int64_t)d0 * W + i * N, n * W - i * N, w_f32, vec);
+    float g[V];
+    load_weights<T, V>(g, weight, (int64_t)d0 * W + i * V, n * W - i * V, w_f32, vec);
 #pragma unroll
-    for (int k = 0; k < N; ++k) w[(i * N + k) / W][(i * N + k) % W] = f[k];
+    for (int k = 0; k < V; ++k) f[(i * V + k) % W][(i * V + k) / W] = g[k];
   }
+#pragma unroll
+  for (int j = 0; j < W; ++j) to_pairs<V>(w[j], f[j]);
+  float g[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) g[k] = from && k < n ? weight_at<T>(from, d0 + k, w_f32) : 0.f;
+  to_pairs<V>(bias, g);
 }
 
 // Token s of N neighbouring channels of a row, the first at x + s * stride and init: for s < 0 from
@@ -43,6 +58,8 @@ __device__ __forceinline__ void load_token(float (&f)[N], const T* x, int64_t st
 
 // ---------------------------------------------------------------- whole rows
 
+constexpr int kAhead = 4;  // tokens
+
 // Thread = V channels x `run` tokens; threads count channel packs fastest, then runs, then rows.
 template <typename T, int V, int W>
 __global__ void __launch_bounds__(128)
@@ -60,11 +77,15 @@ causal_conv_kernel(salt_causal_conv_args a, int packs, int runs, int run, bool w
   const T* init = a.initial_state ? static_cast<const T*>(a.initial_state) + state0 : nullptr;
   T* out = static_cast<T*>(a.out) + b * a.out_batch_stride + d0;
   const int t0 = c * run, t1 = min(t0 + run, a.len), stop = min(t1, real);
-  float win[W][V];  // win[W - 1] is the newest input
-  if (t0 < stop || c == 0) {
+  constexpr int H = (V + 1) / 2;
+  f32x2 win[W][H];  // win[W - 1] is the newest input
+  if (t0 < stop) {
 #pragma unroll
-    for (int j = 1; j < W; ++j)
-      load_token<T, V, W>(win[j], x, a.x_stride, init, t0 + j - W, real, n, true);
+    for (int j = 1; j < W; ++j) {
+      float f[V];
+      load_token<T, V, W>(f, x, a.x_stride, init, t0 + j - W, real, n, true);
+      to_pairs<V>(win[j], f);
+    }
   }
   // Reads its own channels of initial_state, here and above, before it writes: they may be one.
   if (c == 0 && a.final_state && W > 1) {
@@ -80,27 +101,34 @@ causal_conv_kernel(salt_causal_conv_args a, int packs, int runs, int run, bool w
   }
   int t = t0;
   if (t0 < stop) {
-    float w[V][W], bias[V];
-    load_taps<T, V, W>(w, a.weight, d0, n, w_f32, w_vec);
+    f32x2 w[W][H], bias[H];
+    load_taps<T, V, W>(w, bias, a.weight, a.bias, d0, n, w_f32, w_vec);
+    // The loads of kAhead tokens go out together; behind the first store the compiler would have to
+    // keep them in order.
+    for (; t < stop; t += kAhead) {
+      Pack<T, V> p[kAhead];
 #pragma unroll
-    for (int k = 0; k < V; ++k) bias[k] = a.bias ? weight_at<T>(a.bias, d0 + k, w_f32) : 0.f;
-#pragma unroll 4
-    for (; t < stop; ++t) {
-      const Pack<T, V> p = load_pack<T, V>(x + t * a.x_stride, V, true);
-      float y[V];
+      for (int q = 0; q < kAhead; ++q)
+        p[q] = load_pack<T, V>(x + (t + q) * a.x_stride, t + q < stop ? V : 0, true);
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
+      for (int q = 0; q < kAhead; ++q) {
+        float y[V + 1];
 #pragma unroll
-        for (int j = 0; j < W - 1; ++j) win[j][k] = win[j + 1][k];
-        win[W - 1][k] = to_f32(p.v[k]);
-        float s = bias[k];
+        for (int k = 0; k < H; ++k) {
 #pragma unroll
-        for (int j = 0; j < W; ++j) s = fmaf(w[k][j], win[j][k], s);
-        if (a.silu) s *= sigmoid(s);
-        y[k] = s;
+          for (int j = 0; j < W - 1; ++j) win[j][k] = win[j + 1][k];
+          win[W - 1][k] = pair_in(p[q], k);
+          f32x2 s = bias[k];
+#pragma unroll
+          for (int j = 0; j < W; ++j) s = fma2(w[j][k], win[j][k], s);
+          if (a.silu) s = mul2(s, sigmoid2(s));
+          const float2 f = halves(s);
+          y[2 * k] = f.x, y[2 * k + 1] = f.y;
+        }
+        if (t + q < stop) store_pack<T, V>(out + (t + q) * a.out_stride, y, V, true);
       }
-      store_pack<T, V>(out + t * a.out_stride, y, V, true);
     }
+    t = stop;
   }
   const float zero[V] = {};
 #pragma unroll 4
@@ -138,6 +166,10 @@ causal_conv_step_kernel(salt_causal_conv_step_args a, int64_t total, bool w_f32)
 
 // ---------------------------------------------------------------- gradient
 
+#ifndef BAHEAD
+#define BAHEAD 4
+#endif
+constexpr int kBackAhead = BAHEAD;  // tokens
 constexpr int kBackRuns = 8;  // runs of tokens in a block, one per warp
 constexpr int kBackLanes = 32;
 
@@ -145,7 +177,10 @@ constexpr int kBackLanes = 32;
 // row.  g[t] = dy[t] * act'(p[t]) for the run and the width - 1 tokens behind it gives
 // dx[s] = sum_k w[k] g[s + width - 1 - k]; the weight's gradient takes the run's own tokens only.
 template <typename T, int V, int W>
-__global__ void __launch_bounds__(kBackLanes * kBackRuns)
+#ifndef CBB
+#define CBB 2
+#endif
+__global__ void __launch_bounds__(kBackLanes * kBackRuns, W <= 4 ? CBB : 1)
 causal_conv_backward_kernel(salt_causal_conv_backward_args a, int packs, int chunks, int run,
                             bool w_f32, bool w_vec, float* parts) {
   __shared__ float red[kBackRuns][kBackLanes * V];
@@ -160,59 +195,65 @@ causal_conv_backward_kernel(salt_causal_conv_backward_args a, int packs, int chu
   T* dx = static_cast<T*>(a.dx) + b * a.dx_batch_stride + d0;
   const int64_t state0 = ((int64_t)b * a.dim + d0) * (W - 1);
   const T* init = a.initial_state ? static_cast<const T*>(a.initial_state) + state0 : nullptr;
-  float w[V][W], bias[V], win[W][V], g[W][V], dw[V][W], db[V];  // [W - 1] is the newest token
-#pragma unroll
-  for (int k = 0; k < V; ++k) {
-    db[k] = 0.f;
-#pragma unroll
-    for (int j = 0; j < W; ++j) dw[k][j] = win[j][k] = g[j][k] = 0.f;
-  }
+  constexpr int H = (V + 1) / 2;
+  // [W - 1] is the newest token
+  f32x2 w[W][H], bias[H], win[W][H], g[W][H] = {}, dw[W][H] = {}, db[H] = {};
   if (n > 0 && (t0 < t1 || t0 == 0)) {  // a row without tokens has an initial state's gradient
-    load_taps<T, V, W>(w, a.weight, d0, n, w_f32, w_vec);
+    load_taps<T, V, W>(w, bias, a.weight, a.bias, d0, n, w_f32, w_vec);
 #pragma unroll
-    for (int k = 0; k < V; ++k) bias[k] = a.bias ? weight_at<T>(a.bias, d0 + k, w_f32) : 0.f;
+    for (int j = 1; j < W; ++j) {
+      float f[V];
+      load_token<T, V, W>(f, x, a.x_stride, init, t0 + j - W, real, n, true);
+      to_pairs<V>(win[j], f);
+    }
+    for (int tt = t0; tt < t1 + W - 1; tt += kBackAhead) {
+      Pack<T, V> ax[kBackAhead], ad[kBackAhead];
 #pragma unroll
-    for (int j = 1; j < W; ++j)
-      load_token<T, V, W>(win[j], x, a.x_stride, init, t0 + j - W, real, n, true);
-#pragma unroll 4
-    for (int t = t0; t < t1 + W - 1; ++t) {
-      const Pack<T, V> px = load_pack<T, V>(x + t * a.x_stride, t < real ? V : 0, true);
-      const Pack<T, V> pd = load_pack<T, V>(dy + t * a.dy_stride, t < real ? V : 0, true);
-      const int s = t - (W - 1);
-      float out[V];
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-#pragma unroll
-        for (int j = 0; j < W - 1; ++j) {
-          win[j][k] = win[j + 1][k];
-          g[j][k] = g[j + 1][k];
-        }
-        win[W - 1][k] = to_f32(px.v[k]);
-        float gt = to_f32(pd.v[k]);
-        if (a.silu) {
-          float p = bias[k];
-#pragma unroll
-          for (int j = 0; j < W; ++j) p = fmaf(w[k][j], win[j][k], p);
-          gt *= silu_slope(p, sigmoid(p));
-        }
-        g[W - 1][k] = t < real ? gt : 0.f;
-        if (t < t1) {
-          db[k] += g[W - 1][k];
-#pragma unroll
-          for (int j = 0; j < W; ++j) dw[k][j] = fmaf(g[W - 1][k], win[j][k], dw[k][j]);
-        }
-        // token s met tap j at token s + W - 1 - j = t - j
-        out[k] = 0.f;
-#pragma unroll
-        for (int j = 0; j < W; ++j) out[k] = fmaf(w[k][j], g[W - 1 - j][k], out[k]);
-        if (s >= real) out[k] = 0.f;
+      for (int q = 0; q < kBackAhead; ++q) {
+        const int m = tt + q < min(real, t1 + W - 1) ? V : 0;
+        ax[q] = load_pack<T, V>(x + (tt + q) * a.x_stride, m, true);
+        ad[q] = load_pack<T, V>(dy + (tt + q) * a.dy_stride, m, true);
       }
-      if (s >= t0) {
-        store_pack<T, V>(dx + s * a.dx_stride, out, V, true);
-      } else if (t0 == 0 && a.dinitial) {
-        T* di = static_cast<T*>(a.dinitial) + state0;
 #pragma unroll
-        for (int k = 0; k < V; ++k) di[k * (W - 1) + t] = from_f32<T>(out[k]);
+      for (int q = 0; q < kBackAhead; ++q) {
+        const int t = tt + q, s = t - (W - 1);
+        if (t >= t1 + W - 1) break;
+        float out[V + 1];
+#pragma unroll
+        for (int k = 0; k < H; ++k) {
+#pragma unroll
+          for (int j = 0; j < W - 1; ++j) {
+            win[j][k] = win[j + 1][k];
+            g[j][k] = g[j + 1][k];
+          }
+          win[W - 1][k] = pair_in(ax[q], k);
+          f32x2 gt = pair_in(ad[q], k);  // 0 past the row's end
+          if (a.silu) {
+            f32x2 p = bias[k];
+#pragma unroll
+            for (int j = 0; j < W; ++j) p = fma2(w[j][k], win[j][k], p);
+            gt = mul2(gt, silu_slope2(p, sigmoid2(p)));
+          }
+          g[W - 1][k] = gt;
+          if (t < t1) {
+            db[k] = add2(db[k], gt);
+#pragma unroll
+            for (int j = 0; j < W; ++j) dw[j][k] = fma2(gt, win[j][k], dw[j][k]);
+          }
+          // token s met tap j at token s + W - 1 - j = t - j
+          f32x2 v = mul2(w[0][k], g[W - 1][k]);
+#pragma unroll
+          for (int j = 1; j < W; ++j) v = fma2(w[j][k], g[W - 1 - j][k], v);
+          const float2 f = halves(s < real ? v : 0);
+          out[2 * k] = f.x, out[2 * k + 1] = f.y;
+        }
+        if (s >= t0) {
+          store_pack<T, V>(dx + s * a.dx_stride, out, V, true);
+        } else if (t0 == 0 && a.dinitial) {
+          T* di = static_cast<T*>(a.dinitial) + state0;
+#pragma unroll
+          for (int k = 0; k < V; ++k) di[k * (W - 1) + t] = from_f32<T>(out[k]);
+        }
       }
     }
   }
@@ -222,7 +263,10 @@ causal_conv_backward_kernel(salt_causal_conv_backward_args a, int packs, int chu
   for (int j = 0; j <= W; ++j) {
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < V; ++k) red[threadIdx.y][lane * V + k] = j < W ? dw[k][j % W] : db[k];
+    for (int k = 0; k < V; ++k) {
+      const float2 f = halves(j < W ? dw[j % W][k / 2] : db[k / 2]);
+      red[threadIdx.y][lane * V + k] = k % 2 ? f.y : f.x;
+    }
     __syncthreads();
     const int i = threadIdx.y * kBackLanes + lane;
     const int d = pack * kBackLanes * V + i;
@@ -289,7 +333,11 @@ cudaError_t causal_conv_launch(const salt_causal_conv_args& a, cudaStream_t st, 
     return a.dim % v == 0 && pack_rows(a.x, v, ts, a.x_batch_stride, a.x_stride) &&
            pack_rows(a.out, v, ts, a.out_batch_stride, a.out_stride);
   };
-  const int v = fits(kVec) ? kVec : fits(4) ? 4 : 1, packs = a.dim / v;
+  
+#ifndef CFV
+#define CFV kVec
+#endif
+  const int v = fits(CFV) ? CFV : fits(4) ? 4 : 1, packs = a.dim / v;
   const int run = conv_run(packs, a.batch, a.len);
   const int runs = std::max(1, (a.len + run - 1) / run);  // a row without tokens has a final state
   const int64_t threads = (int64_t)packs * runs * a.batch;

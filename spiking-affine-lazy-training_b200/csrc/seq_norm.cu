@@ -43,11 +43,45 @@ __device__ __forceinline__ float row_max(float v, int threads, float* red) {
   return s;
 }
 
+template <typename T, int V>
+__device__ __forceinline__ void store_pairs(T* p, const f32x2 (&r)[(V + 1) / 2], int n, bool vec) {
+  float f[V + 1];
+#pragma unroll
+  for (int k = 0; k < (V + 1) / 2; ++k) {
+    const float2 v = halves(r[k]);
+    f[2 * k] = v.x, f[2 * k + 1] = v.y;
+  }
+  store_pack<T, V>(p, f, n, vec);
+}
+template <typename T, int V>
+__device__ __forceinline__ void load_weight_pairs(f32x2 (&w)[(V + 1) / 2], const void* from,
+                                                  int64_t at, int n, bool is_f32, bool vec) {
+  float f[V];
+  load_weights<T, V>(f, from, at, n, is_f32, vec);
+  if constexpr (V == 1) {
+    w[0] = pair(f[0], 0.f);
+  } else {
+#pragma unroll
+    for (int k = 0; k < V / 2; ++k) w[k] = pair(f[2 * k], f[2 * k + 1]);
+  }
+}
+
+// The scale of a group whose largest magnitude is m, and its inverse.  A product with the inverse
+// instead of a quotient may round a value that lies halfway between two 8-bit ones the other way.
+// fmaxf leaves NaNs out of m: they become e4m3's own, beside the other elements' scale.
+__device__ __forceinline__ float e4m3_scale(float m) {
+  return m == 0.f ? 1.f : m * (1.f / kE4m3Max);
+}
+__device__ __forceinline__ float e4m3_inverse(float m) {
+  if (m < 1e-30f) return m == 0.f ? 1.f : kE4m3Max / m;  // where the fast quotient would overflow
+  return __fdividef(kE4m3Max, m);
+}
+
 // A thread holds PER packs of V neighbouring elements, pack i of the row's thread t at element
 // V * (i * threads + t); V is the widest that all rows' starts allow.  Rows of up to 1024 elements
 // take a warp each, 4 to a block; wider ones a block.
 template <typename T, typename R, int V, int PER>
-__global__ void __launch_bounds__(kRowThreadsMost)
+__global__ void __launch_bounds__(kRowThreadsMost, V * PER <= 8 ? 4 : V * PER <= 16 ? 3 : 1)
 rms_norm_kernel(salt_rms_norm_args a, int threads, bool vec, bool w_f32) {
   __shared__ float red[32];
   const int t = threads == 32 ? threadIdx.x & 31 : threadIdx.x;
@@ -56,75 +90,78 @@ rms_norm_kernel(salt_rms_norm_args a, int threads, bool vec, bool w_f32) {
   if (row >= a.rows) return;  // a whole warp, or no thread of the block
   const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
   const R* res = static_cast<const R*>(a.residual);
-  float r[PER][V];
-  float sq = 0.f;
+  constexpr int H = (V + 1) / 2;  // pairs of a pack; the one element of V = 1 has a zero beside it
+  f32x2 r[PER][H], sq = 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int at = V * (i * threads + t), n = a.dim - at;
     const Pack<T, V> px = load_pack<T, V>(x + at, n, vec);
+    Pack<R, V> pr;
+    if (res) pr = load_pack<R, V>(res + row * a.residual_stride + at, n, vec);
 #pragma unroll
-    for (int k = 0; k < V; ++k) r[i][k] = to_f32(px.v[k]);
-    if (res) {
-      const Pack<R, V> pr = load_pack<R, V>(res + row * a.residual_stride + at, n, vec);
-#pragma unroll
-      for (int k = 0; k < V; ++k) r[i][k] += to_f32(pr.v[k]);
+    for (int k = 0; k < H; ++k) {
+      r[i][k] = pair_in(px, k);
+      if (res) r[i][k] = add2(r[i][k], pair_in(pr, k));
+      sq = fma2(r[i][k], r[i][k], sq);
     }
-#pragma unroll
-    for (int k = 0; k < V; ++k) sq = fmaf(r[i][k], r[i][k], sq);
   }
-  const float rstd = rsqrtf(row_sum(sq, threads, red) / (float)a.dim + a.eps);
+  const float2 both_sq = halves(sq);
+  const float rstd =
+      rsqrtf(row_sum(both_sq.x + both_sq.y, threads, red) / (float)a.dim + a.eps);
   if (a.rstd && t == 0) a.rstd[row] = rstd;
   float most = 0.f;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int at = V * (i * threads + t), n = a.dim - at;
     if (a.residual_out)
-      store_pack<R, V>(static_cast<R*>(a.residual_out) + row * a.residual_out_stride + at, r[i],
-                          n, vec);
-    float w[V];
-    load_weights<T, V>(w, a.weight, at, n, w_f32, vec);
+      store_pairs<R, V>(static_cast<R*>(a.residual_out) + row * a.residual_out_stride + at, r[i], n,
+                        vec);
+    f32x2 w[H];
+    load_weight_pairs<T, V>(w, a.weight, at, n, w_f32, vec);
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      r[i][k] *= rstd * w[k];
-      most = fmaxf(most, fabsf(r[i][k]));
-    }
+    for (int k = 0; k < H; ++k) r[i][k] = mul2(mul2(r[i][k], both(rstd)), w[k]);
     if (!a.scale) {
-      store_pack<T, V>(static_cast<T*>(a.out) + row * a.out_stride + at, r[i], n, vec);
-    } else if (a.group) {
-      // group / V neighbouring lanes hold a group (at V = 8, which 8 bits always take: 4 to 32, never across warps)
-      float m = 0.f;
+      store_pairs<T, V>(static_cast<T*>(a.out) + row * a.out_stride + at, r[i], n, vec);
+      continue;
+    }
+    float m = 0.f;
 #pragma unroll
-      for (int k = 0; k < V; ++k) m = fmaxf(m, fabsf(r[i][k]));
-      for (int o = a.group / V / 2; o; o >>= 1)
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      const float scale = m > 0.f ? m / kE4m3Max : 1.f;
+    for (int k = 0; k < H; ++k) {
+      const float2 v = halves(r[i][k]);
+      m = fmaxf(m, fmaxf(fabsf(v.x), fabsf(v.y)));
+    }
+    most = fmaxf(most, m);
+    if (a.group) {
+      // group / V neighbouring lanes hold a group (at V = 8, which 8 bits always take: 4 to 32,
+      // never across warps)
+      for (int o = a.group / V / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       if (n > 0 && at % a.group == 0)
-        a.scale[row * ((a.dim + a.group - 1) / a.group) + at / a.group] = scale;
-      const float by = 1.f / scale;
+        a.scale[row * ((a.dim + a.group - 1) / a.group) + at / a.group] = e4m3_scale(m);
+      const f32x2 by = both(e4m3_inverse(m));
 #pragma unroll
-      for (int k = 0; k < V; ++k) r[i][k] *= by;
+      for (int k = 0; k < H; ++k) r[i][k] = mul2(r[i][k], by);
     }
   }
   if (!a.scale) return;
   if (!a.group) {
-    const float m = row_max(most, threads, red), scale = m > 0.f ? m / kE4m3Max : 1.f;
-    if (t == 0) a.scale[row] = scale;
-    const float by = 1.f / scale;
+    const float m = row_max(most, threads, red);
+    if (t == 0) a.scale[row] = e4m3_scale(m);
+    const f32x2 by = both(e4m3_inverse(m));
 #pragma unroll
     for (int i = 0; i < PER; ++i)
 #pragma unroll
-      for (int k = 0; k < V; ++k) r[i][k] *= by;
+      for (int k = 0; k < H; ++k) r[i][k] = mul2(r[i][k], by);
   }
   uint8_t* out = static_cast<uint8_t*>(a.out) + row * a.out_stride;
   const bool wide = V == 8 && (reinterpret_cast<uintptr_t>(out) & 7) == 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int at = V * (i * threads + t), n = a.dim - at;
-    alignas(8) uint8_t q[V < 2 ? 2 : V];
+    alignas(8) uint8_t q[2 * H];
 #pragma unroll
-    for (int k = 0; k + 1 < V; k += 2)
-      *reinterpret_cast<uint16_t*>(q + k) =
-          __nv_cvt_float2_to_fp8x2(make_float2(r[i][k], r[i][k + 1]), __NV_SATFINITE, __NV_E4M3);
+    for (int k = 0; k < H; ++k)
+      *reinterpret_cast<uint16_t*>(q + 2 * k) =
+          __nv_cvt_float2_to_fp8x2(halves(r[i][k]), __NV_SATFINITE, __NV_E4M3);
     if (wide && n >= V) {
       *reinterpret_cast<uint2*>(out + at) = *reinterpret_cast<const uint2*>(q);
     } else {
@@ -161,17 +198,24 @@ rms_norm_backward_kernel(salt_rms_norm_backward_args a, int threads, bool vec, b
     const R* x = static_cast<const R*>(a.x) + row * a.x_stride;
     const R* dres = static_cast<const R*>(a.dresidual);
     const float rstd = a.rstd[row];
+    // all of a row's loads before the barriers of its sum
+    Pack<T, V> pdy[PER];
+    Pack<R, V> px[PER], pr[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int at = V * (i * threads + t), n = a.dim - at;
+      pdy[i] = load_pack<T, V>(dy + at, n, vec);
+      px[i] = load_pack<R, V>(x + at, n, vec);
+      if (dres) pr[i] = load_pack<R, V>(dres + row * a.dresidual_stride + at, n, vec);
+    }
     float h[PER][V], g[PER][V];
     float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int at = V * (i * threads + t), n = a.dim - at;
-      const Pack<T, V> pdy = load_pack<T, V>(dy + at, n, vec);
-      const Pack<R, V> px = load_pack<R, V>(x + at, n, vec);
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        h[i][k] = to_f32(px.v[k]) * rstd;
-        const float d = to_f32(pdy.v[k]);
+        h[i][k] = to_f32(px[i].v[k]) * rstd;
+        const float d = to_f32(pdy[i].v[k]);
         dw[i][k] = fmaf(d, h[i][k], dw[i][k]);
         g[i][k] = d * w[i][k];
         dot = fmaf(g[i][k], h[i][k], dot);
@@ -181,13 +225,11 @@ rms_norm_backward_kernel(salt_rms_norm_backward_args a, int threads, bool vec, b
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int at = V * (i * threads + t), n = a.dim - at;
-      Pack<R, V> pr;
-      if (dres) pr = load_pack<R, V>(dres + row * a.dresidual_stride + at, n, vec);
       float dx[V];
 #pragma unroll
       for (int k = 0; k < V; ++k) {
         dx[k] = rstd * fmaf(-h[i][k], mean, g[i][k]);
-        if (dres) dx[k] += to_f32(pr.v[k]);
+        if (dres) dx[k] += to_f32(pr[i].v[k]);
       }
       store_pack<R, V>(static_cast<R*>(a.dx) + row * a.dx_stride + at, dx, n, vec);
     }
@@ -256,13 +298,11 @@ NormPlan norm_plan(int32_t rows, int32_t dim, int v) {
   return p;
 }
 
-constexpr int kNormBackBlocks = 148 * 4;
-
 // Workers (blocks, or warps of narrow rows) of the gradient: one partial weight gradient each.
 void norm_back_grid(const NormPlan& p, int32_t rows, int* blocks, int* workers) {
   const int each = p.threads == 32 ? p.block / 32 : 1;
-  *blocks = (int)std::max<int64_t>(
-      1, std::min<int64_t>(kNormBackBlocks, ((int64_t)rows + each - 1) / each));
+  const int64_t at_once = 148 * std::max(1, 1024 / p.block);
+  *blocks = (int)std::max<int64_t>(1, std::min(at_once, ((int64_t)rows + each - 1) / each));
   *workers = *blocks * each;
 }
 

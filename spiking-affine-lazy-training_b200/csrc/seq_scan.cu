@@ -293,7 +293,7 @@ selective_scan_kernel(salt_selective_scan_args a, ScanSplit sp, int blocks, bool
 
 // ---------------------------------------------------------------- single tokens
 
-constexpr int kStepChannels = 32;  // of a block
+constexpr int kStepChannels = 64;  // of a block
 
 template <int NS_, int LPC_>
 struct StepShape {
@@ -323,8 +323,12 @@ selective_scan_step_kernel(salt_selective_scan_step_args a, int blocks, int rows
   const bool mine = ch < cb.n;
   const int64_t d = cb.d0 + (mine ? ch : 0);
   const int64_t begin = (int64_t)part * rows, end = min((int64_t)a.batch, begin + rows);
+  // the rows' slots, one a lane: a state's load does not wait for its slot's
+  const int lane = tid & 31;
+  int mine_slot = (int)begin + lane;
+  if (a.slots && begin + lane < end) mine_slot = a.slots[begin + lane];
   auto load = [&](StepRow<T, NS>& r, int64_t b) {
-    const int64_t slot = a.slots ? a.slots[b] : b;
+    const int64_t slot = __shfl_sync(0xffffffffu, mine_slot, (int)(b - begin));
     r.pool = slot >= 0 && slot < a.n_slots ? a.pool + (slot * a.dim + d) * a.state + n0 : nullptr;
     if (!r.pool) return;
     load_states<NS>(r.h, r.pool, ns, svec);
@@ -342,22 +346,31 @@ selective_scan_step_kernel(salt_selective_scan_step_args a, int blocks, int rows
   };
   StepRow<T, NS> now, next;
   load(now, begin);
-  float A2[NS];
-  load_states<NS>(A2, a.A + d * a.state + n0, ns, svec);
+  f32x2 A2[NS / 2];
+  {
+    float f[NS];
+    load_states<NS>(f, a.A + d * a.state + n0, ns, svec);
 #pragma unroll
-  for (int i = 0; i < NS; ++i) A2[i] *= kLog2e;
+    for (int i = 0; i < NS / 2; ++i) A2[i] = pair(f[2 * i] * kLog2e, f[2 * i + 1] * kLog2e);
+  }
   const float bias = a.delta_bias ? a.delta_bias[d] : 0.f, skip = a.D ? a.D[d] : 0.f;
   for (int64_t b = begin; b < end; ++b) {
     if (b + 1 < end) load(next, b + 1);
     T* out = static_cast<T*>(a.out) + b * a.out_stride + d;
     if (now.pool) {
       const float x = to_f32(now.x), s = scan_step(to_f32(now.delta) + bias, a.softplus);
-      float y = 0.f;
+      const f32x2 s2 = both(s), sx2 = both(s * x);
+      f32x2 y2 = 0;
 #pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        now.h[i] = fmaf(exp2_fast(A2[i] * s), now.h[i], s * x * to_f32(now.B[i / 4].v[i % 4]));
-        y = fmaf(now.h[i], to_f32(now.C[i / 4].v[i % 4]), y);
+      for (int i = 0; i < NS; i += 2) {
+        const f32x2 h = fma2(exp2_fast2(mul2(A2[i / 2], s2)), pair(now.h[i], now.h[i + 1]),
+                             mul2(sx2, pair_of(now.B[i / 4], i % 4)));
+        y2 = fma2(h, pair_of(now.C[i / 4], i % 4), y2);
+        const float2 f = halves(h);
+        now.h[i] = f.x, now.h[i + 1] = f.y;
       }
+      const float2 yy = halves(y2);
+      float y = yy.x + yy.y;
       if (mine) store_states<NS>(now.pool, now.h, ns, svec);
 #pragma unroll
       for (int o = 1; o < LPC; o <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
@@ -388,9 +401,12 @@ using Scan64 = Shape<8, 8, 2>;
 int scan_channels(int32_t state) { return state <= 4 ? Scan4::kChannels : Scan16::kChannels; }
 
 using Step4 = StepShape<4, 1>;
-using Step8 = StepShape<4, 2>;
-using Step16 = StepShape<4, 4>;
-using Step32 = StepShape<8, 4>;
+using Step8 = StepShape<8, 1>;
+#ifndef SLPC
+#define SLPC 2
+#endif
+using Step16 = StepShape<16 / SLPC, SLPC>;
+using Step32 = StepShape<16, 2>;
 using Step64 = StepShape<16, 4>;
 #define SALT_STEP_SHAPE(state, S, ...) \
   SALT_BY_STATE(state, S, Step4, Step8, Step16, Step32, Step64, __VA_ARGS__)
@@ -470,7 +486,7 @@ cudaError_t selective_scan_step_launch(const salt_selective_scan_step_args& a, c
                                        int* launches) {
   if (a.batch == 0) return cudaSuccess;
   const int blocks = scan_blocks(a.dim, a.groups, kStepChannels);
-  // A is loaded once for the rows that a block walks over
+  // A is loaded once for the rows that a block walks over (at most 32: a lane holds each one's slot)
 #ifndef STEPB
 #define STEPB 8
 #endif

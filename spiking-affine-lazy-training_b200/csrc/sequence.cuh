@@ -186,6 +186,14 @@ __device__ __forceinline__ f32x2 pair_of(const Pack<__nv_bfloat16, N>& p, int k)
   const uint32_t u = *reinterpret_cast<const uint32_t*>(&p.v[k]);  // k is even
   return pair(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
 }
+// Elements 2 k and 2 k + 1 of a pack; a pack of one has a zero behind it.
+template <typename T, int V>
+__device__ __forceinline__ f32x2 pair_in(const Pack<T, V>& p, int k) {
+  if constexpr (V == 1)
+    return pair(to_f32(p.v[0]), 0.f);
+  else
+    return pair_of(p, 2 * k);
+}
 __device__ __forceinline__ f32x2 both(float v) { return pair(v, v); }
 // d/dx of x * sigmoid(x), of both.
 __device__ __forceinline__ f32x2 silu_slope2(f32x2 x, f32x2 p) {
