@@ -109,7 +109,7 @@ causal_conv_kernel(salt_causal_conv_args a, int packs, int runs, int run, bool w
       Pack<T, V> p[kAhead];
 #pragma unroll
       for (int q = 0; q < kAhead; ++q)
-        p[q] = load_pack<T, V>(x + (t + q) * a.x_stride, t + q < stop ? V : 0, true);
+        p[q] = load_whole<T, V>(x, min(t + q, stop - 1) * a.x_stride, INT64_MAX);
 #pragma unroll
       for (int q = 0; q < kAhead; ++q) {
         float y[V + 1];
@@ -166,10 +166,8 @@ causal_conv_step_kernel(salt_causal_conv_step_args a, int64_t total, bool w_f32)
 
 // ---------------------------------------------------------------- gradient
 
-#ifndef BAHEAD
-#define BAHEAD 4
-#endif
-constexpr int kBackAhead = BAHEAD;  // tokens
+constexpr int kBackVec = 4;    // channels of a thread: 2 leave too little to a load, 8 too few threads
+constexpr int kBackAhead = 4;  // tokens whose loads go out together
 constexpr int kBackRuns = 8;  // runs of tokens in a block, one per warp
 constexpr int kBackLanes = 32;
 
@@ -177,10 +175,7 @@ constexpr int kBackLanes = 32;
 // row.  g[t] = dy[t] * act'(p[t]) for the run and the width - 1 tokens behind it gives
 // dx[s] = sum_k w[k] g[s + width - 1 - k]; the weight's gradient takes the run's own tokens only.
 template <typename T, int V, int W>
-#ifndef CBB
-#define CBB 2
-#endif
-__global__ void __launch_bounds__(kBackLanes * kBackRuns, W <= 4 ? CBB : 1)
+__global__ void __launch_bounds__(kBackLanes * kBackRuns, W <= 4 ? 2 : 1)
 causal_conv_backward_kernel(salt_causal_conv_backward_args a, int packs, int chunks, int run,
                             bool w_f32, bool w_vec, float* parts) {
   __shared__ float red[kBackRuns][kBackLanes * V];
@@ -206,13 +201,16 @@ causal_conv_backward_kernel(salt_causal_conv_backward_args a, int packs, int chu
       load_token<T, V, W>(f, x, a.x_stride, init, t0 + j - W, real, n, true);
       to_pairs<V>(win[j], f);
     }
-    for (int tt = t0; tt < t1 + W - 1; tt += kBackAhead) {
+    // without tokens there is nothing to load, and dinitial is 0
+    for (int k = 0; a.len == 0 && a.dinitial && k < V * (W - 1); ++k)
+      static_cast<T*>(a.dinitial)[state0 + k] = from_f32<T>(0.f);
+    for (int tt = t0; a.len > 0 && tt < t1 + W - 1; tt += kBackAhead) {
       Pack<T, V> ax[kBackAhead], ad[kBackAhead];
 #pragma unroll
       for (int q = 0; q < kBackAhead; ++q) {
-        const int m = tt + q < min(real, t1 + W - 1) ? V : 0;
-        ax[q] = load_pack<T, V>(x + (tt + q) * a.x_stride, m, true);
-        ad[q] = load_pack<T, V>(dy + (tt + q) * a.dy_stride, m, true);
+        const int t = min(tt + q, max(real, 1) - 1);  // past the row's end its last token
+        ax[q] = load_whole<T, V>(x, t * a.x_stride, INT64_MAX);
+        ad[q] = load_whole<T, V>(dy, t * a.dy_stride, INT64_MAX);
       }
 #pragma unroll
       for (int q = 0; q < kBackAhead; ++q) {
@@ -226,8 +224,8 @@ causal_conv_backward_kernel(salt_causal_conv_backward_args a, int packs, int chu
             win[j][k] = win[j + 1][k];
             g[j][k] = g[j + 1][k];
           }
-          win[W - 1][k] = pair_in(ax[q], k);
-          f32x2 gt = pair_in(ad[q], k);  // 0 past the row's end
+          win[W - 1][k] = t < real ? pair_in(ax[q], k) : 0;
+          f32x2 gt = t < real ? pair_in(ad[q], k) : 0;
           if (a.silu) {
             f32x2 p = bias[k];
 #pragma unroll
@@ -304,16 +302,13 @@ int conv_run(int64_t packs, int32_t batch, int32_t len) {
 struct ConvBackPlan {
   int v, run, chunks, packs;
 };
-#ifndef CBV
-#define CBV 4
-#endif
 ConvBackPlan conv_back_plan(const salt_causal_conv_backward_args& a) {
   ConvBackPlan p;
   const size_t ts = type_size(a.type);
-  const bool fits = a.dim % CBV == 0 && pack_rows(a.x, CBV, ts, a.x_batch_stride, a.x_stride) &&
-                    pack_rows(a.dy, CBV, ts, a.dy_batch_stride, a.dy_stride) &&
-                    pack_rows(a.dx, CBV, ts, a.dx_batch_stride, a.dx_stride);
-  p.v = fits ? CBV : 1;
+  const bool fits = a.dim % kBackVec == 0 && pack_rows(a.x, kBackVec, ts, a.x_batch_stride, a.x_stride) &&
+                    pack_rows(a.dy, kBackVec, ts, a.dy_batch_stride, a.dy_stride) &&
+                    pack_rows(a.dx, kBackVec, ts, a.dx_batch_stride, a.dx_stride);
+  p.v = fits ? kBackVec : 1;
   p.packs = (a.dim + kBackLanes * p.v - 1) / (kBackLanes * p.v);
   p.run = 64;
   while (p.run > 8 && (int64_t)p.packs * a.batch *
@@ -333,11 +328,7 @@ cudaError_t causal_conv_launch(const salt_causal_conv_args& a, cudaStream_t st, 
     return a.dim % v == 0 && pack_rows(a.x, v, ts, a.x_batch_stride, a.x_stride) &&
            pack_rows(a.out, v, ts, a.out_batch_stride, a.out_stride);
   };
-  
-#ifndef CFV
-#define CFV kVec
-#endif
-  const int v = fits(CFV) ? CFV : fits(4) ? 4 : 1, packs = a.dim / v;
+    const int v = fits(kVec) ? kVec : fits(4) ? 4 : 1, packs = a.dim / v;
   const int run = conv_run(packs, a.batch, a.len);
   const int runs = std::max(1, (a.len + run - 1) / run);  // a row without tokens has a final state
   const int64_t threads = (int64_t)packs * runs * a.batch;
@@ -388,7 +379,7 @@ cudaError_t causal_conv_backward_launch(const salt_causal_conv_backward_args& a,
         causal_conv_backward_kernel<T, 1, W>
             <<<blocks, block, 0, st>>>(a, p.packs, p.chunks, p.run, w_f32, w_vec, parts);
       else
-        causal_conv_backward_kernel<T, CBV, W>
+        causal_conv_backward_kernel<T, kBackVec, W>
             <<<blocks, block, 0, st>>>(a, p.packs, p.chunks, p.run, w_f32, w_vec, parts);
     }));
     ++*launches;

@@ -9,6 +9,9 @@
 
 #include "sequence.cuh"
 
+#ifndef NBT
+#define NBT 1024
+#endif
 namespace salt {
 
 namespace {
@@ -80,31 +83,45 @@ __device__ __forceinline__ float e4m3_inverse(float m) {
 // A thread holds PER packs of V neighbouring elements, pack i of the row's thread t at element
 // V * (i * threads + t); V is the widest that all rows' starts allow.  Rows of up to 1024 elements
 // take a warp each, 4 to a block; wider ones a block.
-template <typename T, typename R, int V, int PER>
-__global__ void __launch_bounds__(kRowThreadsMost, V * PER <= 8 ? 4 : V * PER <= 16 ? 3 : 1)
-rms_norm_kernel(salt_rms_norm_args a, int threads, bool vec, bool w_f32) {
+template <typename T, typename R, int V, int PER, bool VEC>
+__global__ void __launch_bounds__(kRowThreadsMost, V * PER <= 8 ? 3 : V * PER <= 16 ? 2 : 1)
+rms_norm_kernel(salt_rms_norm_args a, int threads, bool w_f32) {
+  constexpr bool vec = VEC;
   __shared__ float red[32];
   const int t = threads == 32 ? threadIdx.x & 31 : threadIdx.x;
-  const int64_t row = threads == 32 ? (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)
-                                    : (int64_t)blockIdx.x;
-  if (row >= a.rows) return;  // a whole warp, or no thread of the block
-  const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+  const int each = threads == 32 ? blockDim.x >> 5 : 1;  // rows of the block at a time
+  const int64_t step = (int64_t)gridDim.x * each;
+  int64_t row = (int64_t)blockIdx.x * each + (threads == 32 ? threadIdx.x >> 5 : 0);
   const R* res = static_cast<const R*>(a.residual);
+  Pack<T, V> px[PER];
+  Pack<R, V> pr[PER];
+  auto load = [&](int64_t at_row) {
+    const T* x = static_cast<const T*>(a.x) + at_row * a.x_stride;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int at = V * (i * threads + t), n = a.dim - at;
+      px[i] = VEC ? load_whole<T, V>(x, at, a.dim) : load_pack<T, V>(x + at, n, false);
+      if (res) {
+        const R* from = res + at_row * a.residual_stride;
+        pr[i] = VEC ? load_whole<R, V>(from, at, a.dim) : load_pack<R, V>(from + at, n, false);
+      }
+    }
+  };
+  if (row < a.rows) load(row);
+  for (; row < a.rows; row += step) {  // the same for a whole warp, or a whole block
   constexpr int H = (V + 1) / 2;  // pairs of a pack; the one element of V = 1 has a zero beside it
   f32x2 r[PER][H], sq = 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int at = V * (i * threads + t), n = a.dim - at;
-    const Pack<T, V> px = load_pack<T, V>(x + at, n, vec);
-    Pack<R, V> pr;
-    if (res) pr = load_pack<R, V>(res + row * a.residual_stride + at, n, vec);
 #pragma unroll
     for (int k = 0; k < H; ++k) {
-      r[i][k] = pair_in(px, k);
-      if (res) r[i][k] = add2(r[i][k], pair_in(pr, k));
+      r[i][k] = pair_in(px[i], k);
+      if (res) r[i][k] = add2(r[i][k], pair_in(pr[i], k));
+      if (V * (i * threads + t) >= a.dim) r[i][k] = 0;
       sq = fma2(r[i][k], r[i][k], sq);
     }
   }
+  if (row + step < a.rows) load(row + step);  // on its way while this row is summed and stored
   const float2 both_sq = halves(sq);
   const float rstd =
       rsqrtf(row_sum(both_sq.x + both_sq.y, threads, red) / (float)a.dim + a.eps);
@@ -142,7 +159,7 @@ rms_norm_kernel(salt_rms_norm_args a, int threads, bool vec, bool w_f32) {
       for (int k = 0; k < H; ++k) r[i][k] = mul2(r[i][k], by);
     }
   }
-  if (!a.scale) return;
+  if (!a.scale) continue;
   if (!a.group) {
     const float m = row_max(most, threads, red);
     if (t == 0) a.scale[row] = e4m3_scale(m);
@@ -170,15 +187,16 @@ rms_norm_kernel(salt_rms_norm_args a, int threads, bool vec, bool w_f32) {
         if (k < n) out[at + k] = q[k];
     }
   }
+  }
 }
 
 // The gradient.  Blocks walk over rows with a fixed set of columns for each thread, so that the
 // weight's gradient stays in registers; each block (each warp, for narrow rows) writes one partial
 // row of it, which sum_parts adds up in order.
-template <typename T, typename R, int V, int PER>
+template <typename T, typename R, int V, int PER, bool VEC>
 __global__ void __launch_bounds__(kRowThreadsMost)
-rms_norm_backward_kernel(salt_rms_norm_backward_args a, int threads, bool vec, bool w_f32,
-                         float* parts) {
+rms_norm_backward_kernel(salt_rms_norm_backward_args a, int threads, bool w_f32, float* parts) {
+  constexpr bool vec = VEC;
   __shared__ float red[32];
   const bool by_warp = threads == 32;
   const int t = by_warp ? threadIdx.x & 31 : threadIdx.x;
@@ -204,9 +222,12 @@ rms_norm_backward_kernel(salt_rms_norm_backward_args a, int threads, bool vec, b
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int at = V * (i * threads + t), n = a.dim - at;
-      pdy[i] = load_pack<T, V>(dy + at, n, vec);
-      px[i] = load_pack<R, V>(x + at, n, vec);
-      if (dres) pr[i] = load_pack<R, V>(dres + row * a.dresidual_stride + at, n, vec);
+      pdy[i] = VEC ? load_whole<T, V>(dy, at, a.dim) : load_pack<T, V>(dy + at, n, false);
+      px[i] = VEC ? load_whole<R, V>(x, at, a.dim) : load_pack<R, V>(x + at, n, false);
+      if (dres) {
+        const R* from = dres + row * a.dresidual_stride;
+        pr[i] = VEC ? load_whole<R, V>(from, at, a.dim) : load_pack<R, V>(from + at, n, false);
+      }
     }
     float h[PER][V], g[PER][V];
     float dot = 0.f;
@@ -214,8 +235,9 @@ rms_norm_backward_kernel(salt_rms_norm_backward_args a, int threads, bool vec, b
     for (int i = 0; i < PER; ++i) {
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        h[i][k] = to_f32(px[i].v[k]) * rstd;
-        const float d = to_f32(pdy[i].v[k]);
+        const bool in = V * (i * threads + t) < a.dim;
+        h[i][k] = in ? to_f32(px[i].v[k]) * rstd : 0.f;
+        const float d = in ? to_f32(pdy[i].v[k]) : 0.f;
         dw[i][k] = fmaf(d, h[i][k], dw[i][k]);
         g[i][k] = d * w[i][k];
         dot = fmaf(g[i][k], h[i][k], dot);
@@ -319,31 +341,41 @@ cudaError_t sum_parts_launch(const float* in, int64_t parts, const PartSums& to,
   return cudaGetLastError();
 }
 
-// Elements per pack by V, packs of a thread by PER.
+// Elements per pack by V, packs of a thread by PER.  Packs of one element are whole always; packs of
+// 8 may be cut in the 8-bit form alone, whose groups are counted in them.
 #define SALT_NORM_SHAPE(p, kernel, T, R, ...)                      \
   do {                                                             \
     if ((p).v == 8) {                                              \
       if ((p).per == 1)                                            \
-        kernel<T, R, 8, 1> __VA_ARGS__;                            \
+        kernel<T, R, 8, 1, true> __VA_ARGS__;                      \
       else if ((p).per == 2)                                       \
-        kernel<T, R, 8, 2> __VA_ARGS__;                            \
+        kernel<T, R, 8, 2, true> __VA_ARGS__;                      \
       else                                                         \
-        kernel<T, R, 8, 4> __VA_ARGS__;                            \
+        kernel<T, R, 8, 4, true> __VA_ARGS__;                      \
     } else if ((p).v == 4) {                                       \
       if ((p).per == 2)                                            \
-        kernel<T, R, 4, 2> __VA_ARGS__;                            \
+        kernel<T, R, 4, 2, true> __VA_ARGS__;                      \
       else if ((p).per == 4)                                       \
-        kernel<T, R, 4, 4> __VA_ARGS__;                            \
+        kernel<T, R, 4, 4, true> __VA_ARGS__;                      \
       else                                                         \
-        kernel<T, R, 4, 8> __VA_ARGS__;                            \
+        kernel<T, R, 4, 8, true> __VA_ARGS__;                      \
     } else {                                                       \
       if ((p).per == 8)                                            \
-        kernel<T, R, 1, 8> __VA_ARGS__;                            \
+        kernel<T, R, 1, 8, true> __VA_ARGS__;                      \
       else if ((p).per == 16)                                      \
-        kernel<T, R, 1, 16> __VA_ARGS__;                           \
+        kernel<T, R, 1, 16, true> __VA_ARGS__;                     \
       else                                                         \
-        kernel<T, R, 1, 32> __VA_ARGS__;                           \
+        kernel<T, R, 1, 32, true> __VA_ARGS__;                     \
     }                                                              \
+  } while (0)
+#define SALT_NORM_CUT(p, kernel, T, R, ...)                        \
+  do {                                                             \
+    if ((p).per == 1)                                              \
+      kernel<T, R, 8, 1, false> __VA_ARGS__;                       \
+    else if ((p).per == 2)                                         \
+      kernel<T, R, 8, 2, false> __VA_ARGS__;                       \
+    else                                                           \
+      kernel<T, R, 8, 4, false> __VA_ARGS__;                       \
   } while (0)
 
 cudaError_t rms_norm_launch(const salt_rms_norm_args& a, cudaStream_t st, int* launches) {
@@ -357,16 +389,27 @@ cudaError_t rms_norm_launch(const salt_rms_norm_args& a, cudaStream_t st, int* l
            pack_rows(a.weight, v, w_f32 ? 4 : ts, 0) &&
            (a.scale || pack_rows(a.out, v, ts, a.out_stride));
   };
-  // a group's lanes are counted in packs of 8, whether those can be moved at once or not
-  const bool vec = fits(8) || (!a.scale && fits(4));
-  const NormPlan p = norm_plan(a.rows, a.dim, a.scale || fits(8) ? 8 : vec ? 4 : 1);
+  const bool cut = a.scale && !fits(8);
+  const NormPlan p = norm_plan(a.rows, a.dim, cut || fits(8) ? 8 : fits(4) ? 4 : 1);
+  // as many blocks as the GPU holds at once: each goes on to further rows
+  const int64_t at_once = 148 * std::max(1, NBT / p.block);
+  const unsigned blocks = (unsigned)std::min<int64_t>(p.blocks, at_once);
   SALT_WITH_TYPE(a.type, T, {
-    if (a.residual_type == SALT_F32)
-      SALT_NORM_SHAPE(p, rms_norm_kernel, T, float,
-                      <<<(unsigned)p.blocks, p.block, 0, st>>>(a, p.threads, vec, w_f32));
-    else
-      SALT_NORM_SHAPE(p, rms_norm_kernel, T, T,
-                      <<<(unsigned)p.blocks, p.block, 0, st>>>(a, p.threads, vec, w_f32));
+    using Wide = float;
+    if (a.residual_type == SALT_F32) {
+      if (cut)
+        SALT_NORM_CUT(p, rms_norm_kernel, T, Wide,
+                      <<<blocks, p.block, 0, st>>>(a, p.threads, w_f32));
+      else
+        SALT_NORM_SHAPE(p, rms_norm_kernel, T, Wide,
+                        <<<blocks, p.block, 0, st>>>(a, p.threads, w_f32));
+    } else {
+      if (cut)
+        SALT_NORM_CUT(p, rms_norm_kernel, T, T, <<<blocks, p.block, 0, st>>>(a, p.threads, w_f32));
+      else
+        SALT_NORM_SHAPE(p, rms_norm_kernel, T, T,
+                        <<<blocks, p.block, 0, st>>>(a, p.threads, w_f32));
+    }
   });
   ++*launches;
   return cudaGetLastError();
@@ -398,15 +441,15 @@ cudaError_t rms_norm_backward_launch(const salt_rms_norm_backward_args& a, void*
   const NormPlan p = norm_back_plan(a);
   int blocks, workers;
   norm_back_grid(p, a.rows, &blocks, &workers);
-  const bool vec = p.v > 1, w_f32 = a.weight_type == SALT_F32;
+  const bool w_f32 = a.weight_type == SALT_F32;
   float* parts = a.dweight ? static_cast<float*>(ws) : nullptr;
   SALT_WITH_TYPE(a.type, T, {
     if (a.residual_type == SALT_F32)
       SALT_NORM_SHAPE(p, rms_norm_backward_kernel, T, float,
-                      <<<blocks, p.block, 0, st>>>(a, p.threads, vec, w_f32, parts));
+                      <<<blocks, p.block, 0, st>>>(a, p.threads, w_f32, parts));
     else
       SALT_NORM_SHAPE(p, rms_norm_backward_kernel, T, T,
-                      <<<blocks, p.block, 0, st>>>(a, p.threads, vec, w_f32, parts));
+                      <<<blocks, p.block, 0, st>>>(a, p.threads, w_f32, parts));
   });
   ++*launches;
   const cudaError_t e = cudaGetLastError();

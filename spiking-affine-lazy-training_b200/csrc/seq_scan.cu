@@ -301,22 +301,35 @@ struct StepShape {
   static constexpr int kThreads = kStepChannels * LPC;
 };
 
-// What one token's row needs before its arithmetic: all loads of a row are issued together, and
-// those of the next row in front of this row's arithmetic.
+// What one token's row needs beside its states; loaded a row ahead.
 template <typename T, int NS>
 struct StepRow {
-  float h[NS];
   T x, delta, z;
   Pack<T, 4> B[NS / 4], C[NS / 4];
-  float* pool;  // NULL: an empty row
 };
 
-// A block holds A of its 32 channels and walks over `rows` tokens' rows.  The states' bytes, read
-// and written once, are the bound: 8 a state and token, against 2 of x, z, delta and out.
+#ifndef STEPD
+#define STEPD 4
+#endif
+#ifndef STEPR
+#define STEPR 8
+#endif
+// Rows whose states are on their way to shared memory, in 32 KB of it at most.
+template <class S>
+constexpr int step_depth() {
+  const int fit = 32 * 1024 / (S::kThreads * S::NS * 4);
+  return fit < STEPD ? fit : STEPD;
+}
+
+// A block holds A of its 64 channels and walks over `rows` tokens' rows.  The states' bytes, read
+// and written once, are the bound: 8 a state and token, against 2 of x, z, delta and out.  VEC:
+// states come by asynchronous copies, each thread its own, some rows ahead; registers
+// would hold one row ahead at most.
 template <typename T, class S, bool VEC>
 __global__ void __launch_bounds__(S::kThreads)
-selective_scan_step_kernel(salt_selective_scan_step_args a, int blocks, int rows, bool svec) {
-  constexpr int NS = S::NS, LPC = S::LPC;
+selective_scan_step_kernel(salt_selective_scan_step_args a, int blocks, int rows) {
+  constexpr int NS = S::NS, LPC = S::LPC, kStepDepth = step_depth<S>();
+  __shared__ float4 ring[VEC ? kStepDepth : 1][NS / 4][S::kThreads];
   const int tid = threadIdx.x, part = blockIdx.x / blocks;
   const ScanBlock cb = scan_block(blockIdx.x - part * blocks, a.dim, a.groups, kStepChannels);
   const int ch = tid / LPC, n0 = tid % LPC * NS, ns = a.state - n0;
@@ -327,29 +340,43 @@ selective_scan_step_kernel(salt_selective_scan_step_args a, int blocks, int rows
   const int lane = tid & 31;
   int mine_slot = (int)begin + lane;
   if (a.slots && begin + lane < end) mine_slot = a.slots[begin + lane];
+  auto pool_of = [&](int64_t b) -> float* {  // NULL: an empty row
+    const int64_t slot = __shfl_sync(0xffffffffu, mine_slot, (int)(b - begin) & 31);
+    return slot >= 0 && slot < a.n_slots ? a.pool + (slot * a.dim + d) * a.state + n0 : nullptr;
+  };
+  auto fetch = [&](int64_t b) {
+    if (b < end) {
+      const float* pool = pool_of(b);
+      if (pool)
+#pragma unroll
+        for (int i = 0; i < NS; i += 4)
+          copy_async<16>(&ring[(b - begin) % kStepDepth][i / 4][tid], pool + (i < ns ? i : 0),
+                         i < ns);
+    }
+    copies_commit();
+  };
   auto load = [&](StepRow<T, NS>& r, int64_t b) {
-    const int64_t slot = __shfl_sync(0xffffffffu, mine_slot, (int)(b - begin));
-    r.pool = slot >= 0 && slot < a.n_slots ? a.pool + (slot * a.dim + d) * a.state + n0 : nullptr;
-    if (!r.pool) return;
-    load_states<NS>(r.h, r.pool, ns, svec);
     r.x = static_cast<const T*>(a.x)[b * a.x_stride + d];
     r.delta = static_cast<const T*>(a.delta)[b * a.delta_stride + d];
     if (a.z) r.z = static_cast<const T*>(a.z)[b * a.z_stride + d];
-    const int64_t at = (int64_t)cb.group * a.state + n0;
+    const int64_t at = (int64_t)cb.group * a.state + (ns > 0 ? n0 : 0);
 #pragma unroll
     for (int i = 0; i < NS; i += 4) {
-      r.B[i / 4] =
-          load_pack<T, 4>(static_cast<const T*>(a.B) + b * a.B_stride + at + i, ns - i, VEC);
-      r.C[i / 4] =
-          load_pack<T, 4>(static_cast<const T*>(a.C) + b * a.C_stride + at + i, ns - i, VEC);
+      const T* B = static_cast<const T*>(a.B) + b * a.B_stride + at;
+      const T* C = static_cast<const T*>(a.C) + b * a.C_stride + at;
+      r.B[i / 4] = VEC ? load_whole<T, 4>(B, i, ns) : load_pack<T, 4>(B + i, ns - i, false);
+      r.C[i / 4] = VEC ? load_whole<T, 4>(C, i, ns) : load_pack<T, 4>(C + i, ns - i, false);
     }
   };
+  if (VEC)
+#pragma unroll
+    for (int i = 0; i < kStepDepth - 1; ++i) fetch(begin + i);
   StepRow<T, NS> now, next;
   load(now, begin);
   f32x2 A2[NS / 2];
   {
     float f[NS];
-    load_states<NS>(f, a.A + d * a.state + n0, ns, svec);
+    load_states<NS>(f, a.A + d * a.state + n0, ns, VEC);
 #pragma unroll
     for (int i = 0; i < NS / 2; ++i) A2[i] = pair(f[2 * i] * kLog2e, f[2 * i + 1] * kLog2e);
   }
@@ -357,21 +384,37 @@ selective_scan_step_kernel(salt_selective_scan_step_args a, int blocks, int rows
   for (int64_t b = begin; b < end; ++b) {
     if (b + 1 < end) load(next, b + 1);
     T* out = static_cast<T*>(a.out) + b * a.out_stride + d;
-    if (now.pool) {
+    float* pool = pool_of(b);
+    float h[NS];
+    if (VEC) {
+      fetch(b + kStepDepth - 1);
+      copies_wait<kStepDepth - 1>();
+#pragma unroll
+      for (int i = 0; i < NS; i += 4) {
+        const float4 v = ring[(b - begin) % kStepDepth][i / 4][tid];
+        h[i] = v.x, h[i + 1] = v.y, h[i + 2] = v.z, h[i + 3] = v.w;
+      }
+    } else if (pool) {
+      load_states<NS>(h, pool, ns, false);
+    }
+    if (pool) {
       const float x = to_f32(now.x), s = scan_step(to_f32(now.delta) + bias, a.softplus);
       const f32x2 s2 = both(s), sx2 = both(s * x);
       f32x2 y2 = 0;
 #pragma unroll
       for (int i = 0; i < NS; i += 2) {
-        const f32x2 h = fma2(exp2_fast2(mul2(A2[i / 2], s2)), pair(now.h[i], now.h[i + 1]),
-                             mul2(sx2, pair_of(now.B[i / 4], i % 4)));
-        y2 = fma2(h, pair_of(now.C[i / 4], i % 4), y2);
-        const float2 f = halves(h);
-        now.h[i] = f.x, now.h[i + 1] = f.y;
+        const bool in = !VEC || i < ns;  // load_whole leaves this to its user
+        const f32x2 bn = in ? pair_of(now.B[i / 4], i % 4) : 0;
+        const f32x2 cn = in ? pair_of(now.C[i / 4], i % 4) : 0;
+        const f32x2 v =
+            fma2(exp2_fast2(mul2(A2[i / 2], s2)), pair(h[i], h[i + 1]), mul2(sx2, bn));
+        y2 = fma2(v, cn, y2);
+        const float2 f = halves(v);
+        h[i] = f.x, h[i + 1] = f.y;
       }
       const float2 yy = halves(y2);
       float y = yy.x + yy.y;
-      if (mine) store_states<NS>(now.pool, now.h, ns, svec);
+      if (mine) store_states<NS>(pool, h, ns, VEC);
 #pragma unroll
       for (int o = 1; o < LPC; o <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
       if (mine && n0 == 0) {
@@ -402,10 +445,7 @@ int scan_channels(int32_t state) { return state <= 4 ? Scan4::kChannels : Scan16
 
 using Step4 = StepShape<4, 1>;
 using Step8 = StepShape<8, 1>;
-#ifndef SLPC
-#define SLPC 2
-#endif
-using Step16 = StepShape<16 / SLPC, SLPC>;
+using Step16 = StepShape<8, 2>;
 using Step32 = StepShape<16, 2>;
 using Step64 = StepShape<16, 4>;
 #define SALT_STEP_SHAPE(state, S, ...) \
@@ -487,25 +527,21 @@ cudaError_t selective_scan_step_launch(const salt_selective_scan_step_args& a, c
   if (a.batch == 0) return cudaSuccess;
   const int blocks = scan_blocks(a.dim, a.groups, kStepChannels);
   // A is loaded once for the rows that a block walks over (at most 32: a lane holds each one's slot)
-#ifndef STEPB
-#define STEPB 8
-#endif
   int rows = 1;
-  while (rows < 8 && (int64_t)blocks * ((a.batch + 2 * rows - 1) / (2 * rows)) >= 148 * STEPB)
+  while (rows < STEPR && (int64_t)blocks * ((a.batch + 2 * rows - 1) / (2 * rows)) >= 148 * 8)
     rows *= 2;
   const int parts = (a.batch + rows - 1) / rows;
   const size_t ts = type_size(a.type);
-  const bool svec = a.state % 4 == 0 && aligned16(a.A) && aligned16(a.pool);
-  const bool vec = a.state % 4 == 0 && pack_rows(a.B, 4, ts, a.B_stride) &&
-                   pack_rows(a.C, 4, ts, a.C_stride);
+  const bool vec = a.state % 4 == 0 && aligned16(a.A) && aligned16(a.pool) &&
+                   pack_rows(a.B, 4, ts, a.B_stride) && pack_rows(a.C, 4, ts, a.C_stride);
   const unsigned grid = (unsigned)((int64_t)blocks * parts);
   SALT_WITH_TYPE(a.type, T, SALT_STEP_SHAPE(a.state, S, {
     if (vec)
       selective_scan_step_kernel<T, S, true>
-          <<<grid, S::kThreads, 0, st>>>(a, blocks, rows, svec);
+          <<<grid, S::kThreads, 0, st>>>(a, blocks, rows);
     else
       selective_scan_step_kernel<T, S, false>
-          <<<grid, S::kThreads, 0, st>>>(a, blocks, rows, svec);
+          <<<grid, S::kThreads, 0, st>>>(a, blocks, rows);
   }));
   ++*launches;
   return cudaGetLastError();

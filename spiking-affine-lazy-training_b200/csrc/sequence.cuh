@@ -47,6 +47,14 @@ __device__ __forceinline__ Pack<T, N> load_pack(const T* p, int n, bool vec) {
   }
   return r;
 }
+// The same where packs are whole (the pointer is aligned, and `at` or the end lies on a pack): p[at ..
+// at + N), or p[0 .. N) if at is not under `end`, for the caller to leave out where it uses them.  A
+// branch around a load, or a choice behind it, would make the thread wait for the load there and
+// then, and not where its values are used.
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> load_whole(const T* p, int64_t at, int64_t end) {
+  return *reinterpret_cast<const Pack<T, N>*>(p + (at < end ? at : 0));
+}
 template <typename T, int N>
 __device__ __forceinline__ void store_pack(T* p, const float* f, int n, bool vec) {
   Pack<T, N> r;
