@@ -9,9 +9,6 @@
 
 #include "sequence.cuh"
 
-#ifndef NBT
-#define NBT 1024
-#endif
 namespace salt {
 
 namespace {
@@ -107,9 +104,15 @@ rms_norm_kernel(salt_rms_norm_args a, int threads, bool w_f32) {
       }
     }
   };
-  if (row < a.rows) load(row);
-  for (; row < a.rows; row += step) {  // the same for a whole warp, or a whole block
   constexpr int H = (V + 1) / 2;  // pairs of a pack; the one element of V = 1 has a zero beside it
+  if (row < a.rows) load(row);
+  f32x2 w[PER][H];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int at = V * (i * threads + t);
+    load_weight_pairs<T, V>(w[i], a.weight, at, a.dim - at, w_f32, vec);
+  }
+  for (; row < a.rows; row += step) {  // the same for a whole warp, or a whole block
   f32x2 r[PER][H], sq = 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
@@ -133,10 +136,8 @@ rms_norm_kernel(salt_rms_norm_args a, int threads, bool w_f32) {
     if (a.residual_out)
       store_pairs<R, V>(static_cast<R*>(a.residual_out) + row * a.residual_out_stride + at, r[i], n,
                         vec);
-    f32x2 w[H];
-    load_weight_pairs<T, V>(w, a.weight, at, n, w_f32, vec);
 #pragma unroll
-    for (int k = 0; k < H; ++k) r[i][k] = mul2(mul2(r[i][k], both(rstd)), w[k]);
+    for (int k = 0; k < H; ++k) r[i][k] = mul2(mul2(r[i][k], both(rstd)), w[i][k]);
     if (!a.scale) {
       store_pairs<T, V>(static_cast<T*>(a.out) + row * a.out_stride + at, r[i], n, vec);
       continue;
@@ -392,7 +393,7 @@ cudaError_t rms_norm_launch(const salt_rms_norm_args& a, cudaStream_t st, int* l
   const bool cut = a.scale && !fits(8);
   const NormPlan p = norm_plan(a.rows, a.dim, cut || fits(8) ? 8 : fits(4) ? 4 : 1);
   // as many blocks as the GPU holds at once: each goes on to further rows
-  const int64_t at_once = 148 * std::max(1, NBT / p.block);
+  const int64_t at_once = 148 * std::max(1, 1024 / p.block);
   const unsigned blocks = (unsigned)std::min<int64_t>(p.blocks, at_once);
   SALT_WITH_TYPE(a.type, T, {
     using Wide = float;

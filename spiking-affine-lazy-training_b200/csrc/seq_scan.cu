@@ -128,10 +128,11 @@ selective_scan_kernel(salt_selective_scan_args a, ScanSplit sp, int blocks, bool
   // and its 8 channels of one token in loads and stores
   const int io_t = tid / S::kIo, io_v = tid % S::kIo;
   const int io_d = cb.d0 + io_v * kVec, io_n = cb.n - io_v * kVec;
-  const T* x = static_cast<const T*>(a.x) + b * a.x_batch_stride + io_d;
-  const T* delta = static_cast<const T*>(a.delta) + b * a.delta_batch_stride + io_d;
-  const T* z = FULL && a.z ? static_cast<const T*>(a.z) + b * a.z_batch_stride + io_d : nullptr;
-  T* out = static_cast<T*>(a.out) + b * a.out_batch_stride + io_d;
+  const T* x = static_cast<const T*>(a.x) + b * a.x_batch_stride + cb.d0;
+  const T* delta = static_cast<const T*>(a.delta) + b * a.delta_batch_stride + cb.d0;
+  const T* z = FULL && a.z ? static_cast<const T*>(a.z) + b * a.z_batch_stride + cb.d0 : nullptr;
+  T* out = static_cast<T*>(a.out) + b * a.out_batch_stride + cb.d0;
+  constexpr bool WIDE = COPY == kCopy16;
   const T* B = static_cast<const T*>(a.B) + b * a.B_batch_stride + (int64_t)cb.group * a.state;
   const T* C = static_cast<const T*>(a.C) + b * a.C_batch_stride + (int64_t)cb.group * a.state;
   f32x2 bias[kVec / 2], skip[kVec / 2];
@@ -144,15 +145,18 @@ selective_scan_kernel(salt_selective_scan_args a, ScanSplit sp, int blocks, bool
     skip[k / 2] =
         a.D ? pair(one ? a.D[io_d + k] : 0.f, two ? a.D[io_d + k + 1] : 0.f) : 0;
   }
-  // Each thread copies what it converts itself: its 8 channels of one token, and packs of 4 states
-  // of B and C.  So a copy has arrived for its reader once that thread has waited for it.
+  // In copies of 16 bytes each thread copies what it converts itself: its 8 channels of one token,
+  // and packs of 4 states of B and C.  So a copy has arrived for its reader once that thread has
+  // waited for it.
   constexpr int kPacks = S::kTile * S::kStates / 4;
   auto load = [&](int t0) {
     auto& raw = sm.raw[t0 / S::kTile % kStages];
-    const int t = t0 + io_t, n = t < stop ? io_n : 0;
-    copy_pack<COPY, kVec>(&raw.x[io_t][io_v * kVec], x + t * a.x_stride, n);
-    copy_pack<COPY, kVec>(&raw.delta[io_t][io_v * kVec], delta + t * a.delta_stride, n);
-    if (z) copy_pack<COPY, kVec>(&raw.z[FULL ? io_t : 0][io_v * kVec], z + t * a.z_stride, n);
+    auto tile = [&](T(*to)[S::kChannels], const T* from, int64_t stride) {
+      copy_tile<COPY, kVec, S::kTile, S::kChannels, S::kThreads>(to, from, stride, t0, stop, cb.n);
+    };
+    tile(raw.x, x, a.x_stride);
+    tile(raw.delta, delta, a.delta_stride);
+    if (z) tile(raw.z, z, a.z_stride);
     for (int i = tid; i < kPacks; i += S::kThreads) {
       const int q = i / (S::kStates / 4), n1 = i % (S::kStates / 4) * 4;
       const int left = t0 + q < stop ? a.state - n1 : 0;
@@ -167,7 +171,7 @@ selective_scan_kernel(salt_selective_scan_args a, ScanSplit sp, int blocks, bool
   if (begin < stop) load(begin);
   for (int t0 = begin; t0 < (FULL ? end : stop); t0 += S::kTile) {
     const int t = t0 + io_t;
-    const auto& raw = sm.raw[t0 / S::kTile % kStages];
+    auto& raw = sm.raw[t0 / S::kTile % kStages];
     if (t0 < stop) {
       if (t0 + S::kTile < stop) {
         load(t0 + S::kTile);
@@ -175,6 +179,7 @@ selective_scan_kernel(salt_selective_scan_args a, ScanSplit sp, int blocks, bool
       } else {
         copies_wait<0>();
       }
+      if (!WIDE) __syncthreads();
       const auto px = pack_at<kVec>(&raw.x[io_t][io_v * kVec]);
       const auto pd = pack_at<kVec>(&raw.delta[io_t][io_v * kVec]);
 #pragma unroll
@@ -276,7 +281,13 @@ selective_scan_kernel(salt_selective_scan_args a, ScanSplit sp, int blocks, bool
         const float2 f = halves(v);
         y[k] = f.x, y[k + 1] = f.y;
       }
-      scan_store<T, kVec, COPY == kCopy16>(out + t * a.out_stride, y, io_n);
+      scan_store<T, kVec, WIDE>(out + t * a.out_stride + io_v * kVec, &raw.x[io_t][io_v * kVec], y,
+                                io_n);
+    }
+    if (FULL && !WIDE) {
+      __syncthreads();
+      store_tile<COPY, S::kTile, S::kChannels, S::kThreads>(out, raw.x, a.out_stride, t0, end, cb.n);
+      __syncthreads();
     }
   }
 #pragma unroll
@@ -308,17 +319,11 @@ struct StepRow {
   Pack<T, 4> B[NS / 4], C[NS / 4];
 };
 
-#ifndef STEPD
-#define STEPD 4
-#endif
-#ifndef STEPR
-#define STEPR 8
-#endif
 // Rows whose states are on their way to shared memory, in 32 KB of it at most.
 template <class S>
 constexpr int step_depth() {
   const int fit = 32 * 1024 / (S::kThreads * S::NS * 4);
-  return fit < STEPD ? fit : STEPD;
+  return fit < 4 ? fit : 4;
 }
 
 // A block holds A of its 64 channels and walks over `rows` tokens' rows.  The states' bytes, read
@@ -528,7 +533,7 @@ cudaError_t selective_scan_step_launch(const salt_selective_scan_step_args& a, c
   const int blocks = scan_blocks(a.dim, a.groups, kStepChannels);
   // A is loaded once for the rows that a block walks over (at most 32: a lane holds each one's slot)
   int rows = 1;
-  while (rows < STEPR && (int64_t)blocks * ((a.batch + 2 * rows - 1) / (2 * rows)) >= 148 * 8)
+  while (rows < 8 && (int64_t)blocks * ((a.batch + 2 * rows - 1) / (2 * rows)) >= 148 * 8)
     rows *= 2;
   const int parts = (a.batch + rows - 1) / rows;
   const size_t ts = type_size(a.type);

@@ -121,6 +121,35 @@ __device__ __forceinline__ void copy_pack(T* to, const T* from, int n) {
   }
 }
 
+// A tile of TILE tokens from t0 on and CH channels, of which n are there, into shared memory; zeros
+// where the row (at `stop`) or its channels end.  In copies of 16 bytes each thread moves the P
+// channels of one token that it converts itself; narrower ones go element by element through the
+// rows, so that a warp's lie together, and the block has to meet before it reads them.
+template <int COPY, int P, int TILE, int CH, int THREADS, typename T>
+__device__ __forceinline__ void copy_tile(T (*to)[CH], const T* from, int64_t stride, int t0,
+                                          int stop, int n) {
+  constexpr int E = COPY == kCopy16 ? P : COPY == kCopy4 ? 4 / sizeof(T) : 1;
+  constexpr int per = CH / E;
+#pragma unroll
+  for (int i = threadIdx.x; i < TILE * per; i += THREADS) {
+    const int q = i / per, c = i % per * E;
+    copy_pack<COPY, E>(&to[q][c], from + (int64_t)(t0 + q) * stride + c, t0 + q < stop ? n - c : 0);
+  }
+}
+// The way back for narrow rows, once the block has met: tokens [t0, end) of the tile.
+template <int COPY, int TILE, int CH, int THREADS, typename T>
+__device__ __forceinline__ void store_tile(T* to, T (*from)[CH], int64_t stride, int t0, int end,
+                                           int n) {
+  constexpr int E = COPY == kCopy4 ? 4 / sizeof(T) : 1, per = CH / E;
+#pragma unroll
+  for (int i = threadIdx.x; i < TILE * per; i += THREADS) {
+    const int q = i / per, c = i % per * E;
+    if (t0 + q < end && c < n)
+      *reinterpret_cast<Pack<T, E>*>(to + (int64_t)(t0 + q) * stride + c) =
+          *reinterpret_cast<const Pack<T, E>*>(&from[q][c]);
+  }
+}
+
 // A pack of shared memory that copy_pack filled.
 template <int N, typename T>
 __device__ __forceinline__ Pack<T, N> pack_at(const T* p) {
@@ -133,18 +162,15 @@ __device__ __forceinline__ void widen4(float* to, const T* from) {
   *reinterpret_cast<float4*>(to) = make_float4(lo.x, lo.y, hi.x, hi.y);
 }
 
-// Stores N values of which `n` are wanted.  WIDE: n is a multiple of N or not positive, and the
-// place is aligned.
+// N values to global memory where rows are wide (n is a multiple of N or not positive), else to the
+// same place of the tile that store_tile writes.
 template <typename T, int N, bool WIDE>
-__device__ __forceinline__ void scan_store(T* p, const float* f, int n) {
-  if (!WIDE) {
-    store_pack<T, N>(p, f, n, false);
-  } else if (n > 0) {
-    Pack<T, N> r;
+__device__ __forceinline__ void scan_store(T* global, T* tile, const float* f, int n) {
+  if (WIDE && n <= 0) return;
+  Pack<T, N> r;
 #pragma unroll
-    for (int i = 0; i < N; ++i) r.v[i] = from_f32<T>(f[i]);
-    *reinterpret_cast<Pack<T, N>*>(p) = r;
-  }
+  for (int i = 0; i < N; ++i) r.v[i] = from_f32<T>(f[i]);
+  *reinterpret_cast<Pack<T, N>*>(WIDE ? global : tile) = r;
 }
 
 // NS neighbouring states of `p`, those at or past `n` as zero.

@@ -145,14 +145,14 @@ selective_scan_backward_kernel(salt_selective_scan_backward_args a, ScanSplit sp
   }
 
   const int io_t = tid / S::kIo, io_v = tid % S::kIo;
-  const int io_d = cb.d0 + io_v * P, io_n = cb.n - io_v * P;
-  const T* x = static_cast<const T*>(a.x) + b * a.x_batch_stride + io_d;
-  const T* delta = static_cast<const T*>(a.delta) + b * a.delta_batch_stride + io_d;
-  const T* z = a.z ? static_cast<const T*>(a.z) + b * a.z_batch_stride + io_d : nullptr;
-  const T* dy = static_cast<const T*>(a.dy) + b * a.dy_batch_stride + io_d;
-  T* dx = static_cast<T*>(a.dx) + b * a.dx_batch_stride + io_d;
-  T* ddelta = static_cast<T*>(a.ddelta) + b * a.ddelta_batch_stride + io_d;
-  T* dz = z ? static_cast<T*>(a.dz) + b * a.dz_batch_stride + io_d : nullptr;
+  const int io_n = cb.n - io_v * P;
+  const T* x = static_cast<const T*>(a.x) + b * a.x_batch_stride + cb.d0;
+  const T* delta = static_cast<const T*>(a.delta) + b * a.delta_batch_stride + cb.d0;
+  const T* z = a.z ? static_cast<const T*>(a.z) + b * a.z_batch_stride + cb.d0 : nullptr;
+  const T* dy = static_cast<const T*>(a.dy) + b * a.dy_batch_stride + cb.d0;
+  T* dx = static_cast<T*>(a.dx) + b * a.dx_batch_stride + cb.d0;
+  T* ddelta = static_cast<T*>(a.ddelta) + b * a.ddelta_batch_stride + cb.d0;
+  T* dz = z ? static_cast<T*>(a.dz) + b * a.dz_batch_stride + cb.d0 : nullptr;
   const T* B = static_cast<const T*>(a.B) + b * a.B_batch_stride + (int64_t)cb.group * a.state;
   const T* C = static_cast<const T*>(a.C) + b * a.C_batch_stride + (int64_t)cb.group * a.state;
   const int64_t per = (a.len + kTile - 1) / kTile;
@@ -166,22 +166,22 @@ selective_scan_backward_kernel(salt_selective_scan_backward_args a, ScanSplit sp
   // tokens past the row's end
   for (int t = max(stop, begin) / kTile * kTile + io_t; t < end; t += kTile) {
     if (t < stop) continue;
-    float zero[P];
-#pragma unroll
-    for (int k = 0; k < P; ++k) zero[k] = 0.f;
-    scan_store<T, P, WIDE>(dx + t * a.dx_stride, zero, io_n);
-    scan_store<T, P, WIDE>(ddelta + t * a.ddelta_stride, zero, io_n);
-    if (dz) scan_store<T, P, WIDE>(dz + t * a.dz_stride, zero, io_n);
+    const float zero[P] = {};
+    store_pack<T, P>(dx + t * a.dx_stride + io_v * P, zero, io_n, WIDE);
+    store_pack<T, P>(ddelta + t * a.ddelta_stride + io_v * P, zero, io_n, WIDE);
+    if (dz) store_pack<T, P>(dz + t * a.dz_stride + io_v * P, zero, io_n, WIDE);
   }
 
   constexpr int kPacks = kTile * S::kStates / 4;
-  auto load = [&](int t0) {  // each thread copies what it converts itself
+  auto load = [&](int t0) {  // in copies of 16 bytes each thread copies what it converts itself
     auto& raw = sm.raw[t0 / kTile % 2];
-    const int t = t0 + io_t, n = t < stop ? io_n : 0;
-    copy_pack<COPY, P>(&raw.x[io_t][io_v * P], x + t * a.x_stride, n);
-    copy_pack<COPY, P>(&raw.delta[io_t][io_v * P], delta + t * a.delta_stride, n);
-    copy_pack<COPY, P>(&raw.dy[io_t][io_v * P], dy + t * a.dy_stride, n);
-    if (z) copy_pack<COPY, P>(&raw.z[io_t][io_v * P], z + t * a.z_stride, n);
+    auto tile = [&](T(*to)[S::kChannels], const T* from, int64_t stride) {
+      copy_tile<COPY, P, kTile, S::kChannels, S::kThreads>(to, from, stride, t0, stop, cb.n);
+    };
+    tile(raw.x, x, a.x_stride);
+    tile(raw.delta, delta, a.delta_stride);
+    tile(raw.dy, dy, a.dy_stride);
+    if (z) tile(raw.z, z, a.z_stride);
     for (int i = tid; i < kPacks; i += S::kThreads) {
       const int q = i / (S::kStates / 4), n1 = i % (S::kStates / 4) * 4;
       const int left = t0 + q < stop ? a.state - n1 : 0;
@@ -197,7 +197,7 @@ selective_scan_backward_kernel(salt_selective_scan_backward_args a, ScanSplit sp
   for (int t0 = first_tile; t0 >= begin; t0 -= kTile) {
     const int t = t0 + io_t;
     const bool live = t < stop;
-    const auto& raw = sm.raw[t0 / kTile % 2];
+    auto& raw = sm.raw[t0 / kTile % 2];
     f32x2 h[CPT][H];  // the state in front of the tile
 #pragma unroll
     for (int j = 0; j < CPT; ++j) {
@@ -213,6 +213,7 @@ selective_scan_backward_kernel(salt_selective_scan_backward_args a, ScanSplit sp
     } else {
       copies_wait<0>();
     }
+    if (!WIDE) __syncthreads();
     {
       const auto px = pack_at<P>(&raw.x[io_t][io_v * P]), pd = pack_at<P>(&raw.delta[io_t][io_v * P]);
       const auto pz = pack_at<P>(&raw.z[io_t][io_v * P]), py = pack_at<P>(&raw.dy[io_t][io_v * P]);
@@ -419,9 +420,19 @@ selective_scan_backward_kernel(salt_selective_scan_backward_args a, ScanSplit sp
           oz[k] = f.x, oz[k + 1] = f.y;
         }
       }
-      scan_store<T, P, WIDE>(dx + t * a.dx_stride, ox, io_n);
-      scan_store<T, P, WIDE>(ddelta + t * a.ddelta_stride, od, io_n);
-      if (dz) scan_store<T, P, WIDE>(dz + t * a.dz_stride, oz, io_n);
+      const int at = io_v * P;
+      scan_store<T, P, WIDE>(dx + t * a.dx_stride + at, &raw.x[io_t][at], ox, io_n);
+      scan_store<T, P, WIDE>(ddelta + t * a.ddelta_stride + at, &raw.delta[io_t][at], od, io_n);
+      if (dz) scan_store<T, P, WIDE>(dz + t * a.dz_stride + at, &raw.z[io_t][at], oz, io_n);
+    }
+    if (!WIDE) {
+      __syncthreads();
+      auto back = [&](T* to, T(*from)[S::kChannels], int64_t stride) {
+        store_tile<COPY, kTile, S::kChannels, S::kThreads>(to, from, stride, t0, stop, cb.n);
+      };
+      back(dx, raw.x, a.dx_stride);
+      back(ddelta, raw.delta, a.ddelta_stride);
+      if (dz) back(dz, raw.z, a.dz_stride);
     }
     // the block's sum of dB and dC over its warps, in order
     for (int i = tid; i < kTile * 2 * a.state; i += S::kThreads) {
@@ -519,20 +530,21 @@ scan_back_state_kernel(salt_selective_scan_backward_args a, ScanSplit sp, int bl
     }
   }
   const int io_t = tid / S::kIo, io_v = tid % S::kIo;
-  const int io_d = cb.d0 + io_v * P, io_n = cb.n - io_v * P;
-  const T* delta = static_cast<const T*>(a.delta) + b * a.delta_batch_stride + io_d;
-  const T* z = a.z ? static_cast<const T*>(a.z) + b * a.z_batch_stride + io_d : nullptr;
-  const T* dy = static_cast<const T*>(a.dy) + b * a.dy_batch_stride + io_d;
+  const T* delta = static_cast<const T*>(a.delta) + b * a.delta_batch_stride + cb.d0;
+  const T* z = a.z ? static_cast<const T*>(a.z) + b * a.z_batch_stride + cb.d0 : nullptr;
+  const T* dy = static_cast<const T*>(a.dy) + b * a.dy_batch_stride + cb.d0;
   const T* C = static_cast<const T*>(a.C) + b * a.C_batch_stride + (int64_t)cb.group * a.state;
   for (int i = tid; i < S::kChannels; i += S::kThreads)
     sm.bias[i] = a.delta_bias && i < cb.n ? a.delta_bias[cb.d0 + i] : 0.f;
   constexpr int kPacks = kTile * S::kStates / 4;
   auto load = [&](int t0) {
     auto& raw = sm.raw[t0 / kTile % 2];
-    const int t = t0 + io_t, n = t < stop ? io_n : 0;
-    copy_pack<COPY, P>(&raw.delta[io_t][io_v * P], delta + t * a.delta_stride, n);
-    copy_pack<COPY, P>(&raw.dy[io_t][io_v * P], dy + t * a.dy_stride, n);
-    if (z) copy_pack<COPY, P>(&raw.z[io_t][io_v * P], z + t * a.z_stride, n);
+    auto tile = [&](T(*to)[S::kChannels], const T* from, int64_t stride) {
+      copy_tile<COPY, P, kTile, S::kChannels, S::kThreads>(to, from, stride, t0, stop, cb.n);
+    };
+    tile(raw.delta, delta, a.delta_stride);
+    tile(raw.dy, dy, a.dy_stride);
+    if (z) tile(raw.z, z, a.z_stride);
     for (int i = tid; i < kPacks; i += S::kThreads) {
       const int q = i / (S::kStates / 4), n1 = i % (S::kStates / 4) * 4;
       copy_pack<COPY, 4>(&raw.c[q][n1], C + (t0 + q) * a.C_stride + n1,
