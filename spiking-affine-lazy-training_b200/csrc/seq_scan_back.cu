@@ -484,6 +484,17 @@ selective_scan_backward_kernel(salt_selective_scan_backward_args a, ScanSplit sp
   }
 }
 
+template <typename T, class S>
+struct BackStateShared {
+  struct Raw {
+    alignas(16) T delta[kTile][S::kChannels], z[kTile][S::kChannels], dy[kTile][S::kChannels];
+    alignas(16) T c[kTile][S::kStates];
+  } raw[2];
+  alignas(16) float2 step[kTile][S::kStepPitch];  // s and g
+  alignas(16) float C[kTile][S::kStates];
+  float bias[S::kChannels];
+};
+
 // The first pass over a split row, from its end: the carry in front of chunk c + 1 with nothing
 // behind it (the last live chunk: the final state's gradient) into place c, and the chunk's steps.
 template <typename T, class S, int COPY>
@@ -491,17 +502,7 @@ __global__ void __launch_bounds__(S::kThreads)
 scan_back_state_kernel(salt_selective_scan_backward_args a, ScanSplit sp, int blocks, bool svec) {
   constexpr int NS = S::NS, LPC = S::LPC, CPT = S::CPT, P = S::P, H = NS / 2;
   extern __shared__ __align__(16) unsigned char raw_shared[];
-  struct Shared {
-    struct Raw {
-      alignas(16) T delta[kTile][S::kChannels], z[kTile][S::kChannels], dy[kTile][S::kChannels];
-      alignas(16) T c[kTile][S::kStates];
-    } raw[2];
-    alignas(16) float2 step[kTile][S::kStepPitch];  // s and g
-    alignas(16) float C[kTile][S::kStates];
-    float bias[S::kChannels];
-  };
-  static_assert(sizeof(Shared) <= sizeof(BackShared<T, S>), "");
-  Shared& sm = *reinterpret_cast<Shared*>(raw_shared);
+  BackStateShared<T, S>& sm = *reinterpret_cast<BackStateShared<T, S>*>(raw_shared);
   const int tid = threadIdx.x, run = sp.chunks - 1;
   const int64_t b = blockIdx.x / (blocks * run);
   const int rest = (int)(blockIdx.x - b * blocks * run), c = rest / blocks + 1;
@@ -641,25 +642,25 @@ int back_channels(int32_t state) {
                        : Back64::kChannels;
 }
 
-constexpr int kSlots = 148 * 3;      // blocks of 128 threads at 168 registers
+// Blocks that the GPU holds at once: of 128 threads at 168 registers, and of the shared memory that
+// two tiles as loaded leave (75 KB, or 93 KB in 32 bits).
+int back_slots(int32_t type) { return 148 * (type == SALT_F32 ? 2 : 3); }
 constexpr float kFirstPass = 0.22f;  // its time, of the second pass's
 
 template <typename T, class S, int COPY>
 cudaError_t back_launch(const salt_selective_scan_backward_args& a, const ScanSplit& sp,
                         const BackParts& parts, int blocks, bool svec, cudaStream_t st,
                         int* launches) {
-  constexpr size_t shared = sizeof(BackShared<T, S>);
+  constexpr size_t shared = sizeof(BackShared<T, S>), few = sizeof(BackStateShared<T, S>);
   const auto first = scan_back_state_kernel<T, S, COPY>;
   const auto main = selective_scan_backward_kernel<T, S, COPY>;
+  const auto limit = cudaFuncAttributeMaxDynamicSharedMemorySize;
   cudaError_t e = cudaSuccess;
-  if (shared > 48 * 1024) {
-    const auto limit = cudaFuncAttributeMaxDynamicSharedMemorySize;
-    e = cudaFuncSetAttribute(main, limit, (int)shared);
-    if (e == cudaSuccess && sp.chunks > 1) e = cudaFuncSetAttribute(first, limit, (int)shared);
-  }
+  if (shared > 48 * 1024) e = cudaFuncSetAttribute(main, limit, (int)shared);
+  if (few > 48 * 1024 && e == cudaSuccess) e = cudaFuncSetAttribute(first, limit, (int)few);
   const int64_t rows = (int64_t)a.batch * blocks;
   if (e == cudaSuccess && sp.chunks > 1) {
-    first<<<(unsigned)(rows * (sp.chunks - 1)), S::kThreads, shared, st>>>(a, sp, blocks, svec);
+    first<<<(unsigned)(rows * (sp.chunks - 1)), S::kThreads, few, st>>>(a, sp, blocks, svec);
     ++*launches;
     e = cudaGetLastError();
   }
@@ -679,7 +680,7 @@ struct BackPlan {
 BackPlan back_plan(const salt_selective_scan_backward_args& a) {
   BackPlan p;
   p.blocks = scan_blocks(a.dim, a.groups, back_channels(a.state));
-  const ScanSplit split = scan_split((int64_t)a.batch * p.blocks, kSlots, a.len, kFirstPass);
+  const ScanSplit split = scan_split((int64_t)a.batch * p.blocks, back_slots(a.type), a.len, kFirstPass);
   p.chunks = split.chunks, p.chunk_len = split.chunk_len;
   size_t at = 0;
   auto take = [&](size_t n) {
