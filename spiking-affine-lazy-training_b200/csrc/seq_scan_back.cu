@@ -642,9 +642,7 @@ int back_channels(int32_t state) {
                        : Back64::kChannels;
 }
 
-// Blocks that the GPU holds at once: of 128 threads at 168 registers, and of the shared memory that
-// two tiles as loaded leave (75 KB, or 93 KB in 32 bits).
-int back_slots(int32_t type) { return 148 * (type == SALT_F32 ? 2 : 3); }
+constexpr int kSlots = 148 * 3;      // blocks of 128 threads at 168 registers
 constexpr float kFirstPass = 0.22f;  // its time, of the second pass's
 
 template <typename T, class S, int COPY>
@@ -680,7 +678,7 @@ struct BackPlan {
 BackPlan back_plan(const salt_selective_scan_backward_args& a) {
   BackPlan p;
   p.blocks = scan_blocks(a.dim, a.groups, back_channels(a.state));
-  const ScanSplit split = scan_split((int64_t)a.batch * p.blocks, back_slots(a.type), a.len, kFirstPass);
+  const ScanSplit split = scan_split((int64_t)a.batch * p.blocks, kSlots, a.len, kFirstPass);
   p.chunks = split.chunks, p.chunk_len = split.chunk_len;
   size_t at = 0;
   auto take = [&](size_t n) {
