@@ -29,8 +29,7 @@ from typing import NamedTuple
 import numpy as np
 
 from . import _lib
-from .device import (DeviceArray, bfloat16, current_device, empty, float8_e4m3, stream_handle,
-                     workspace)
+from .device import (DeviceArray, _tls, bfloat16, current_device, empty, float8_e4m3, workspace)
 
 CHECKPOINT = 16       # tokens between the scan's checkpoints (SALT_SCAN_CHECKPOINT)
 GROUPS_8BIT = (0, 32, 64, 128, 256)
@@ -97,6 +96,9 @@ def _type_of(a, name: str) -> int:
     return got
 
 
+# Types of other libraries' arrays that know their device and whether they are contiguous.
+_TORCH_LIKE: set = set()
+
 # The checks of an array come in two forms.  A call on small inputs costs the host more time than
 # the GPU, so each array first goes through one chain of comparisons that ends in its pointer;
 # whatever fails there (an unusual layout, or a mistake) goes through `_look`, which decides and
@@ -132,6 +134,12 @@ def _look(a, name: str, shape: tuple, type_id: int, inner: int) -> None:
         raise ValueError(f"{name}: not on the current device ({current_device()})")
 
 
+def _stream():
+    """The current stream's handle: `device.stream_handle` without an object for the default one."""
+    stack = getattr(_tls, "streams", None)
+    return stack[-1].handle if stack else None
+
+
 def _here() -> int:
     """The current device, -1 where there is none (the library then says so)."""
     d = ctypes.c_int32(-1)
@@ -150,9 +158,12 @@ def _whole(here: int, a, name: str, shape: tuple, type_id: int) -> int:
     if type(a) is DeviceArray:
         if a.shape == shape and _TYPE_IDS.get(a.dtype) == type_id:
             return a.ptr
-    elif hasattr(a, "get_device") and a.shape == shape and _TYPE_IDS.get(a.dtype) == type_id \
-            and a.stride() == _dense(shape) and a.get_device() == here:
-        return a.data_ptr()
+    elif type(a) in _TORCH_LIKE:
+        if a.shape == shape and _TYPE_IDS.get(a.dtype) == type_id and a.is_contiguous() \
+                and a.get_device() == here:
+            return a.data_ptr()
+    elif hasattr(a, "is_contiguous") and hasattr(a, "get_device"):
+        _TORCH_LIKE.add(type(a))
     _look(a, name, shape, type_id, len(shape))
     return a.data_ptr()
 
@@ -165,7 +176,7 @@ def _rows(here: int, a, name: str, shape: tuple, type_id: int, inner: int = 1):
     if type(a) is DeviceArray:
         if a.shape == shape and _TYPE_IDS.get(a.dtype) == type_id:
             return a.ptr, _dense(shape)[:-inner]
-    elif hasattr(a, "get_device") and a.shape == shape and _TYPE_IDS.get(a.dtype) == type_id:
+    elif type(a) in _TORCH_LIKE and a.shape == shape and _TYPE_IDS.get(a.dtype) == type_id:
         s = a.stride()
         if s[-1] == 1 and (inner == 1 or s[-2] == shape[-1]) and a.get_device() == here:
             return a.data_ptr(), s[:-inner]
@@ -282,7 +293,7 @@ def _norm(x, weight, residual, eps, out, residual_out, rstd, scale, group):
     args = _pack_norm(
         rows, dim, t, wide, wt, group or 0, eps, sx, sr, so, sro, px, pr, pw, po, pro,
         _whole(here, rstd, "rstd", shape[:-1], _F32), ps)
-    _lib.check(_lib.lib().salt_rms_norm(args, stream_handle()))
+    _lib.check(_lib.lib().salt_rms_norm(args, _stream()))
     return NormOutput(out, residual_out, rstd, scale)
 
 
@@ -329,7 +340,7 @@ def rms_norm_backward(dy, x, weight, rstd, *, dresidual=None, dx=None, dweight=N
         _whole(here, dweight, "dweight", (dim,), _F32))
     lib = _lib.lib()
     ws, at, n = _work(lib.salt_rms_norm_backward_workspace_size, args)
-    _lib.check(lib.salt_rms_norm_backward(args, at, n, stream_handle()))
+    _lib.check(lib.salt_rms_norm_backward(args, at, n, _stream()))
     return NormGradients(dx, dweight)
 
 
@@ -356,7 +367,7 @@ def causal_conv(x, weight, bias=None, *, n_real=None, initial_state=None, silu: 
         _whole(here, bias, "bias", (dim,), wt), _whole(here, n_real, "n_real", (batch,), _I32),
         _whole(here, initial_state, "initial_state", edge, t), po,
         _whole(here, final_state, "final_state", edge, t))
-    _lib.check(_lib.lib().salt_causal_conv(args, stream_handle()))
+    _lib.check(_lib.lib().salt_causal_conv(args, _stream()))
     return ConvOutput(out, final_state)
 
 
@@ -378,7 +389,7 @@ def causal_conv_step(x, state, weight, bias=None, *, slots=None, silu: bool = Tr
         batch, dim, width, n_slots, t, wt, bool(silu), 0, *sx, *so, px, pw,
         _whole(here, bias, "bias", (dim,), wt), _whole(here, slots, "slots", (batch,), _I32),
         _whole(here, state, "state", (n_slots, dim, width - 1), t), po)
-    _lib.check(_lib.lib().salt_causal_conv_step(args, stream_handle()))
+    _lib.check(_lib.lib().salt_causal_conv_step(args, _stream()))
     return ConvOutput(out, state)
 
 
@@ -409,7 +420,7 @@ def causal_conv_backward(dy, x, weight, bias=None, *, n_real=None, initial_state
         _whole(here, dbias, "dbias", (dim,), _F32))
     lib = _lib.lib()
     ws, at, size = _work(lib.salt_causal_conv_backward_workspace_size, args)
-    _lib.check(lib.salt_causal_conv_backward(args, at, size, stream_handle()))
+    _lib.check(lib.salt_causal_conv_backward(args, at, size, _stream()))
     return ConvGradients(dx, dweight, dbias, dinitial)
 
 
@@ -455,7 +466,7 @@ def selective_scan(x, delta, A, B, C, *, D=None, z=None, delta_bias=None, softpl
         _whole(here, checkpoints, "checkpoints", marks, _F32))
     lib = _lib.lib()
     ws, at, size = _work(lib.salt_selective_scan_workspace_size, args)
-    _lib.check(lib.salt_selective_scan(args, at, size, stream_handle()))
+    _lib.check(lib.salt_selective_scan(args, at, size, _stream()))
     return ScanOutput(out, final_state, checkpoints)
 
 
@@ -483,7 +494,7 @@ def selective_scan_step(pool, x, delta, A, B, C, *, D=None, z=None, delta_bias=N
         _whole(here, delta_bias, "delta_bias", (dim,), _F32),
         _whole(here, slots, "slots", (batch,), _I32),
         _whole(here, pool, "pool", (n_slots, dim, state), _F32), po)
-    _lib.check(_lib.lib().salt_selective_scan_step(args, stream_handle()))
+    _lib.check(_lib.lib().salt_selective_scan_step(args, _stream()))
     return ScanOutput(out, pool)
 
 
@@ -529,5 +540,5 @@ def selective_scan_backward(dy, x, delta, A, B, C, *, checkpoints, D=None, z=Non
         _whole(here, dinitial, "dinitial", ends, _F32))
     lib = _lib.lib()
     ws, at, size = _work(lib.salt_selective_scan_backward_workspace_size, args)
-    _lib.check(lib.salt_selective_scan_backward(args, at, size, stream_handle()))
+    _lib.check(lib.salt_selective_scan_backward(args, at, size, _stream()))
     return ScanGradients(dx, ddelta, dA, dB, dC, dD, dz, ddelta_bias, dinitial)
