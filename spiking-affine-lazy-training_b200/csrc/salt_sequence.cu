@@ -180,6 +180,9 @@ void scan_common(Checks& c, const A* a, int32_t len) {
   c.need(a->state >= 1 && a->state <= 64, "state must lie in [1, 64]");
   c.need(a->groups >= 1 && a->dim % (a->groups < 1 ? 1 : a->groups) == 0,
          "groups must divide dim");
+  // a group has blocks of its own, and dB and dC a value for each of its states
+  c.need((int64_t)a->batch * (len / 8 + 1) <= (int64_t)0x7fffffff / (a->groups < 1 ? 1 : a->groups),
+         "batch * len * groups is too large for one launch");
   const bool used = a->batch > 0 && len > 0;
   c.input(a->x, used, "x is NULL");
   c.input(a->delta, used, "delta is NULL");

@@ -47,10 +47,10 @@ __device__ __forceinline__ Pack<T, N> load_pack(const T* p, int n, bool vec) {
   }
   return r;
 }
-// The same where packs are whole (the pointer is aligned, and `at` or the end lies on a pack): p[at ..
-// at + N), or p[0 .. N) if at is not under `end`, for the caller to leave out where it uses them.  A
-// branch around a load, or a choice behind it, would make the thread wait for the load there and
-// then, and not where its values are used.
+// The same where packs are whole (the pointer is aligned, and `at` or the end lies on a pack): p[at
+// .. at + N), or p[0 .. N) if at is not under `end`, for the caller to leave out where it uses
+// them.  A branch around a load, or a choice behind it, would make the thread wait for the load
+// there and then, and not where its values are used.
 template <typename T, int N>
 __device__ __forceinline__ Pack<T, N> load_whole(const T* p, int64_t at, int64_t end) {
   return *reinterpret_cast<const Pack<T, N>*>(p + (at < end ? at : 0));
@@ -105,8 +105,6 @@ __device__ __forceinline__ float sigmoid(float x) {
   return __fdividef(1.f, 1.f + exp_fast(-x));
 }
 
-// d/dx of x * sigmoid(x).
-__device__ __forceinline__ float silu_slope(float x, float p) { return p * fmaf(x, 1.f - p, 1.f); }
 
 __device__ __forceinline__ int32_t row_tokens(const int32_t* n_real, int b, int32_t len) {
   if (!n_real) return len;
@@ -240,11 +238,7 @@ struct PartSums {
 cudaError_t sum_parts_launch(const float* in, int64_t parts, const PartSums& to, cudaStream_t st);
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-// Whether rows at p with these strides (in elements) start on 16-byte boundaries.
-inline bool vec_rows(const void* p, size_t size, int64_t s0, int64_t s1 = 0) {
-  return !p || (aligned16(p) && (s0 * size) % 16 == 0 && (s1 * size) % 16 == 0);
-}
-// The same for boundaries of `bytes`.
+// Whether rows at p with these strides (in elements) start on boundaries of `bytes`.
 inline bool packed_rows(const void* p, int64_t bytes, size_t size, int64_t s0, int64_t s1) {
   return reinterpret_cast<uintptr_t>(p) % bytes == 0 && (int64_t)(s0 * size) % bytes == 0 &&
          (int64_t)(s1 * size) % bytes == 0;
