@@ -170,11 +170,11 @@ causal_conv_step_kernel(salt_causal_conv_step_args a, int64_t total, bool w_f32)
 
 // ---------------------------------------------------------------- gradient
 
-// Forward and backward of 8 rows of 2048 tokens x 2048 channels in bf16 take 129 us, 2.6 TB/s or 40
-// % of the copy rate: 40 us forward, 80 us backward, 6 us the sum of the parts.  The backward
+// Forward and backward of 8 rows of 2048 tokens x 2048 channels in bf16 take 123 us, 2.7 TB/s or
+// 42 % of the copy rate: 37 us forward, 80 us backward, 6 us the sum of the parts.  The backward
 // kernel holds 16 warps on an SM (128 registers for weights, inputs, gradients and their sums) and
-// waits for its loads.  Channels of a thread: 2 154 us, 8 276 us (before the arithmetic in pairs);
-// loads of 2 tokens together 154 us, of 8 130 us.
+// issues in every second cycle.  Channels of a thread: 2 154 us, 8 276 us (before the arithmetic in
+// pairs); loads of 2 tokens together 154 us, of 8 130 us.
 constexpr int kBackVec = 4;    // channels of a thread
 constexpr int kBackAhead = 4;  // tokens whose loads go out together
 constexpr int kBackRuns = 8;  // runs of tokens in a block, one per warp
@@ -225,7 +225,6 @@ causal_conv_backward_kernel(salt_causal_conv_backward_args a, int packs, int chu
 #pragma unroll
       for (int q = 0; q < kBackAhead; ++q) {
         const int t = tt + q, s = t - (W - 1);
-        if (t >= t1 + W - 1) break;
         float out[V + 1];
 #pragma unroll
         for (int k = 0; k < H; ++k) {
@@ -243,11 +242,10 @@ causal_conv_backward_kernel(salt_causal_conv_backward_args a, int packs, int chu
             gt = mul2(gt, silu_slope2(p, sigmoid2(p)));
           }
           g[W - 1][k] = gt;
-          if (t < t1) {
-            db[k] = add2(db[k], gt);
+          const f32x2 own = t < t1 ? gt : 0;
+          db[k] = add2(db[k], own);
 #pragma unroll
-            for (int j = 0; j < W; ++j) dw[j][k] = fma2(gt, win[j][k], dw[j][k]);
-          }
+          for (int j = 0; j < W; ++j) dw[j][k] = fma2(own, win[j][k], dw[j][k]);
           // token s met tap j at token s + W - 1 - j = t - j
           f32x2 v = mul2(w[0][k], g[W - 1][k]);
 #pragma unroll
@@ -255,8 +253,9 @@ causal_conv_backward_kernel(salt_causal_conv_backward_args a, int packs, int chu
           const float2 f = halves(s < real ? v : 0);
           out[2 * k] = f.x, out[2 * k + 1] = f.y;
         }
+        // tokens behind the run (and, in the last round, behind its gradients) are another's
         if (s >= t0) {
-          store_pack<T, V>(dx + s * a.dx_stride, out, V, true);
+          if (s < t1) store_pack<T, V>(dx + s * a.dx_stride, out, V, true);
         } else if (t0 == 0 && a.dinitial) {
           T* di = static_cast<T*>(a.dinitial) + state0;
 #pragma unroll

@@ -82,13 +82,15 @@ __device__ __forceinline__ float e4m3_inverse(float m) {
 // A thread holds PER packs of V neighbouring elements, pack i of the row's thread t at element
 // V * (i * threads + t); V is the widest that all rows' starts allow.  Rows of up to 1024 elements
 // take a warp each, 4 to a block; wider ones a block.  Blocks go on to further rows, with the next
-// row's loads on their way while this one is summed and stored: 143 us against 167 us a block a
-// row, for 16384 rows of 5120 in bf16 with a residual to 8 bits by groups of 128.  That now takes
-// 141 us, 4.2 TB/s or 65 % of the measured copy rate; the two barriers of a row's sum and about 8
-// instructions an element share the rest.  Few rows cost the call alone: 10 us from the host.
+// row's loads on their way while this one is summed and stored (16384 rows of 5120 in bf16 with a
+// residual to 8 bits by groups of 128: 143 us against 150 us with a block for each row, 167 us with
+// branches around the loads, 123 us without divisions by the group's size).  Those 123 us are 4.8
+// TB/s or 74 % of the measured copy rate; an instruction issues in two of three cycles, so what is
+// left is shared by instructions and the two barriers of a row's sum.  Few rows cost the call alone:
+// 10 us from the host.
 template <typename T, typename R, int V, int PER, bool VEC>
 __global__ void __launch_bounds__(kRowThreadsMost, V * PER <= 8 ? 3 : V * PER <= 16 ? 2 : 1)
-rms_norm_kernel(salt_rms_norm_args a, int threads, bool w_f32) {
+rms_norm_kernel(salt_rms_norm_args a, int threads, bool w_f32, int group_bits, int groups) {
   constexpr bool vec = VEC;
   __shared__ float red[32];
   const int t = threads == 32 ? threadIdx.x & 31 : threadIdx.x;
@@ -159,8 +161,9 @@ rms_norm_kernel(salt_rms_norm_args a, int threads, bool w_f32) {
         // group / V neighbouring lanes hold a group (at V = 8, which 8 bits always take: 4 to 32,
         // never across warps)
         for (int o = a.group / V / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        if (n > 0 && at % a.group == 0)
-          a.scale[row * ((a.dim + a.group - 1) / a.group) + at / a.group] = e4m3_scale(m);
+        // a division by the group's size would cost as much as the rest of the pack
+        if (n > 0 && (at & (a.group - 1)) == 0)
+          a.scale[row * groups + (at >> group_bits)] = e4m3_scale(m);
         const f32x2 by = both(e4m3_inverse(m));
 #pragma unroll
         for (int k = 0; k < H; ++k) r[i][k] = mul2(r[i][k], by);
@@ -181,17 +184,17 @@ rms_norm_kernel(salt_rms_norm_args a, int threads, bool w_f32) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int at = V * (i * threads + t), n = a.dim - at;
-      alignas(8) uint8_t q[2 * H];
+      uint16_t q[H];
 #pragma unroll
       for (int k = 0; k < H; ++k)
-        *reinterpret_cast<uint16_t*>(q + 2 * k) =
-            __nv_cvt_float2_to_fp8x2(halves(r[i][k]), __NV_SATFINITE, __NV_E4M3);
-      if (wide && n >= V) {
-        *reinterpret_cast<uint2*>(out + at) = *reinterpret_cast<const uint2*>(q);
+        q[k] = __nv_cvt_float2_to_fp8x2(halves(r[i][k]), __NV_SATFINITE, __NV_E4M3);
+      if (V == 8 && wide && n >= V) {
+        *reinterpret_cast<uint2*>(out + at) =
+            make_uint2(q[0] | (uint32_t)q[1 % H] << 16, q[2 % H] | (uint32_t)q[3 % H] << 16);
       } else {
 #pragma unroll
         for (int k = 0; k < V; ++k)
-          if (k < n) out[at + k] = q[k];
+          if (k < n) out[at + k] = (uint8_t)(q[k / 2] >> (k % 2 * 8));
       }
     }
   }
@@ -286,7 +289,7 @@ sum_parts_kernel(const float* __restrict__ in, int64_t parts, int64_t n, PartSum
   const int64_t i = (int64_t)blockIdx.x * 32 + threadIdx.x;
   float s = 0.f;
   if (i < n) {
-#pragma unroll 4
+#pragma unroll 8
     for (int64_t p = threadIdx.y; p < parts; p += ROWS) s += in[p * n + i];
   }
   red[threadIdx.y][threadIdx.x] = s;
@@ -401,6 +404,9 @@ cudaError_t rms_norm_launch(const salt_rms_norm_args& a, cudaStream_t st, int* l
            (a.scale || pack_rows(a.out, v, ts, a.out_stride));
   };
   const bool cut = a.scale && !fits(8);
+  int bits = 0;
+  while (a.group > (1 << bits)) ++bits;
+  const int groups = a.group ? (a.dim + a.group - 1) / a.group : 1;
   const NormPlan p = norm_plan(a.rows, a.dim, cut || fits(8) ? 8 : fits(4) ? 4 : 1);
   // as many blocks as the GPU holds at once: each goes on to further rows
   const int64_t at_once = 148 * std::max(1, 1024 / p.block);
@@ -410,16 +416,17 @@ cudaError_t rms_norm_launch(const salt_rms_norm_args& a, cudaStream_t st, int* l
     if (a.residual_type == SALT_F32) {
       if (cut)
         SALT_NORM_CUT(p, rms_norm_kernel, T, Wide,
-                      <<<blocks, p.block, 0, st>>>(a, p.threads, w_f32));
+                      <<<blocks, p.block, 0, st>>>(a, p.threads, w_f32, bits, groups));
       else
         SALT_NORM_SHAPE(p, rms_norm_kernel, T, Wide,
-                        <<<blocks, p.block, 0, st>>>(a, p.threads, w_f32));
+                        <<<blocks, p.block, 0, st>>>(a, p.threads, w_f32, bits, groups));
     } else {
       if (cut)
-        SALT_NORM_CUT(p, rms_norm_kernel, T, T, <<<blocks, p.block, 0, st>>>(a, p.threads, w_f32));
+        SALT_NORM_CUT(p, rms_norm_kernel, T, T,
+                      <<<blocks, p.block, 0, st>>>(a, p.threads, w_f32, bits, groups));
       else
         SALT_NORM_SHAPE(p, rms_norm_kernel, T, T,
-                        <<<blocks, p.block, 0, st>>>(a, p.threads, w_f32));
+                        <<<blocks, p.block, 0, st>>>(a, p.threads, w_f32, bits, groups));
     }
   });
   ++*launches;
