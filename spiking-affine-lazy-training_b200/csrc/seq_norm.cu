@@ -86,8 +86,8 @@ __device__ __forceinline__ float e4m3_inverse(float m) {
 // residual to 8 bits by groups of 128: 143 us against 150 us with a block for each row, 167 us with
 // branches around the loads, 123 us without divisions by the group's size).  Those 123 us are 4.8
 // TB/s or 74 % of the measured copy rate; an instruction issues in two of three cycles, so what is
-// left is shared by instructions and the two barriers of a row's sum.  Few rows cost the call alone:
-// 10 us from the host.
+// left is shared by instructions and the two barriers of a row's sum.  Few rows cost the call
+// alone: 10 us from the host.
 template <typename T, typename R, int V, int PER, bool VEC>
 __global__ void __launch_bounds__(kRowThreadsMost, V * PER <= 8 ? 3 : V * PER <= 16 ? 2 : 1)
 rms_norm_kernel(salt_rms_norm_args a, int threads, bool w_f32, int group_bits, int groups) {

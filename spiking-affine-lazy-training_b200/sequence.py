@@ -29,7 +29,7 @@ from typing import NamedTuple
 import numpy as np
 
 from . import _lib
-from .device import (DeviceArray, _tls, bfloat16, current_device, empty, float8_e4m3, workspace)
+from .device import DeviceArray, _tls, bfloat16, current_device, empty, float8_e4m3
 
 CHECKPOINT = 16       # tokens between the scan's checkpoints (SALT_SCAN_CHECKPOINT)
 GROUPS_8BIT = (0, 32, 64, 128, 256)
@@ -254,14 +254,19 @@ _pack_scan_step = _packer(_lib.SelectiveScanStepArgs)
 _pack_scan_backward = _packer(_lib.SelectiveScanBackwardArgs)
 
 
-def _work(query, args: bytes):
-    """(buffer or None, its pointer, bytes) that the matching *_workspace_size asks for."""
-    n = ctypes.c_size_t(0)
+def _with_workspace(query, call, args: bytes) -> None:
+    """call(args, workspace, bytes, stream) with the workspace that query asks for: stream-ordered
+    memory, given back behind the call's work."""
+    lib, stream, n = _lib.lib(), _stream(), ctypes.c_size_t(0)
     _lib.check(query(args, ctypes.byref(n)))
-    if n.value == 0:
-        return None, None, 0
-    ws = workspace(n.value)
-    return ws, ws.ptr, n.value
+    ws = ctypes.c_void_p()
+    if n.value:
+        _lib.check(lib.salt_malloc(n.value, stream, ctypes.byref(ws)))
+    try:
+        _lib.check(call(args, ws, n.value, stream))
+    finally:
+        if ws:
+            lib.salt_free(ws, stream)
 
 
 # ---------------------------------------------------------------- root-mean-square norm
@@ -339,8 +344,7 @@ def rms_norm_backward(dy, x, weight, rstd, *, dresidual=None, dx=None, dweight=N
         _whole(here, rstd, "rstd", shape[:-1], _F32), pr, pdx,
         _whole(here, dweight, "dweight", (dim,), _F32))
     lib = _lib.lib()
-    ws, at, n = _work(lib.salt_rms_norm_backward_workspace_size, args)
-    _lib.check(lib.salt_rms_norm_backward(args, at, n, _stream()))
+    _with_workspace(lib.salt_rms_norm_backward_workspace_size, lib.salt_rms_norm_backward, args)
     return NormGradients(dx, dweight)
 
 
@@ -419,8 +423,8 @@ def causal_conv_backward(dy, x, weight, bias=None, *, n_real=None, initial_state
         _whole(here, dweight, "dweight", (dim, width), _F32),
         _whole(here, dbias, "dbias", (dim,), _F32))
     lib = _lib.lib()
-    ws, at, size = _work(lib.salt_causal_conv_backward_workspace_size, args)
-    _lib.check(lib.salt_causal_conv_backward(args, at, size, _stream()))
+    _with_workspace(lib.salt_causal_conv_backward_workspace_size, lib.salt_causal_conv_backward,
+                    args)
     return ConvGradients(dx, dweight, dbias, dinitial)
 
 
@@ -465,8 +469,7 @@ def selective_scan(x, delta, A, B, C, *, D=None, z=None, delta_bias=None, softpl
         _whole(here, final_state, "final_state", ends, _F32),
         _whole(here, checkpoints, "checkpoints", marks, _F32))
     lib = _lib.lib()
-    ws, at, size = _work(lib.salt_selective_scan_workspace_size, args)
-    _lib.check(lib.salt_selective_scan(args, at, size, _stream()))
+    _with_workspace(lib.salt_selective_scan_workspace_size, lib.salt_selective_scan, args)
     return ScanOutput(out, final_state, checkpoints)
 
 
@@ -539,6 +542,6 @@ def selective_scan_backward(dy, x, delta, A, B, C, *, checkpoints, D=None, z=Non
         _whole(here, ddelta_bias, "ddelta_bias", (dim,), _F32),
         _whole(here, dinitial, "dinitial", ends, _F32))
     lib = _lib.lib()
-    ws, at, size = _work(lib.salt_selective_scan_backward_workspace_size, args)
-    _lib.check(lib.salt_selective_scan_backward(args, at, size, _stream()))
+    _with_workspace(lib.salt_selective_scan_backward_workspace_size,
+                    lib.salt_selective_scan_backward, args)
     return ScanGradients(dx, ddelta, dA, dB, dC, dD, dz, ddelta_bias, dinitial)
