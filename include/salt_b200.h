@@ -390,7 +390,8 @@ enum { SALT_F32 = 0, SALT_F16 = 1, SALT_BF16 = 2 };
  * residual_out and rstd (rows) may be NULL; residual_out may be residual itself, out may be x.
  * With `scale` given, out is 8 bits (e4m3) instead: each group of `group` (32, 64, 128, 256, or
  * 0 = the whole row) neighbouring elements has scale = max|out| / 448 (1 where the group is zero)
- * and out = the nearest e4m3 of value / scale; scale is (rows, ceil(dim / group)) float32. */
+ * and out = the nearest e4m3 of value / scale, ties to even, both of them quotients rounded to
+ * float32; scale is (rows, ceil(dim / group)) float32. */
 typedef struct {
   int32_t rows, dim;
   int32_t type, residual_type, weight_type;

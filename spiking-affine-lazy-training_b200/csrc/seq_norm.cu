@@ -66,16 +66,48 @@ __device__ __forceinline__ void load_weight_pairs(f32x2 (&w)[(V + 1) / 2], const
   }
 }
 
-// The scale of a group whose largest magnitude is m, and its inverse.  A product with the inverse
-// instead of a quotient may round a value that lies halfway between two 8-bit ones the other way.
-// fmaxf leaves NaNs out of m: they become e4m3's own, beside the other elements' scale.
-__device__ __forceinline__ float e4m3_scale(float m) {
-  return m == 0.f ? 1.f : m * (1.f / kE4m3Max);
-}
-__device__ __forceinline__ float e4m3_inverse(float m) {
-  if (m < 1e-30f) return m == 0.f ? 1.f : kE4m3Max / m;  // where the fast quotient would overflow
-  return __fdividef(kE4m3Max, m);
-}
+// The scale of a group whose largest magnitude is m: the float32 quotient m / 448 (1 for a group of
+// zeros), and what divides the group's values by it.  fmaxf leaves NaNs out of m: they become e4m3's
+// own, beside the other elements' scale.
+//
+// A product with one rounded inverse may bring a value near the middle of two 8-bit ones to the other
+// side than the quotient.  So the scale is the product m (1/448) with its remainder added (P.
+// Markstein, "Computation of elementary functions on the IBM RISC System/6000 processor", 1990): m /
+// 448 rounded, for every m.  The inverse of the scale has two parts, y and y (1 - scale y); the sum of
+// a value's products with them is rounded once, and off by less than 2^-44 of itself before that.
+// Against the one product: 16384 rows of 5120 in bf16 with a residual, by groups of 128, take 128
+// us instead of 123.
+// Far from 1 the parts or products would underflow: `lift` moves both operands by a power of two.  An
+// infinity as the largest value leaves 0 for all finite ones.
+struct E4m3Scale {
+  float scale, lift;
+  f32x2 high, low;
+  __device__ __forceinline__ explicit E4m3Scale(float m) : lift(1.f) {
+    float divisor;
+    if (m >= 0x1p-60f && m < 0x1p60f) {
+      constexpr float by = 1.f / kE4m3Max;
+      const float q = m * by;
+      divisor = scale = fmaf(fmaf(-q, kE4m3Max, m), by, q);
+    } else {
+      scale = m == 0.f ? 1.f : m / kE4m3Max;
+      lift = m < 1.f ? 0x1p64f : 0x1p-64f;
+      divisor = scale * lift;
+    }
+    const float y = rcp_fast(divisor);
+    high = both(y);
+    low = both(divisor < INFINITY ? fmaf(-divisor, y, 1.f) * y : 0.f);
+  }
+  // the values' quotients by the scale
+  template <int H>
+  __device__ __forceinline__ void divide(f32x2 (&v)[H]) const {
+    if (lift != 1.f) {
+#pragma unroll
+      for (int k = 0; k < H; ++k) v[k] = mul2(v[k], both(lift));
+    }
+#pragma unroll
+    for (int k = 0; k < H; ++k) v[k] = fma2(v[k], high, mul2(v[k], low));
+  }
+};
 
 // r = x + residual; out = r * rsqrt(mean(r^2) + eps) * weight.
 //
@@ -84,9 +116,9 @@ __device__ __forceinline__ float e4m3_inverse(float m) {
 // take a warp each, 4 to a block; wider ones a block.  Blocks go on to further rows, with the next
 // row's loads on their way while this one is summed and stored (16384 rows of 5120 in bf16 with a
 // residual to 8 bits by groups of 128: 143 us against 150 us with a block for each row, 167 us with
-// branches around the loads, 123 us without divisions by the group's size).  Those 123 us are 4.8
-// TB/s or 74 % of the measured copy rate; an instruction issues in two of three cycles, so what is
-// left is shared by instructions and the two barriers of a row's sum.  Few rows cost the call
+// branches around the loads, 123 us without divisions by the group's size, 128 us with exact
+// quotients).  Those 128 us are 4.6 TB/s or 71 % of the measured copy rate; an instruction issues in
+// two of three cycles, so what is left is shared by instructions and the two barriers of a row's sum.  Few rows cost the call
 // alone: 10 us from the host.
 template <typename T, typename R, int V, int PER, bool VEC>
 __global__ void __launch_bounds__(kRowThreadsMost, V * PER <= 8 ? 3 : V * PER <= 16 ? 2 : 1)
@@ -161,23 +193,19 @@ rms_norm_kernel(salt_rms_norm_args a, int threads, bool w_f32, int group_bits, i
         // group / V neighbouring lanes hold a group (at V = 8, which 8 bits always take: 4 to 32,
         // never across warps)
         for (int o = a.group / V / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const E4m3Scale by(m);
         // a division by the group's size would cost as much as the rest of the pack
         if (n > 0 && (at & (a.group - 1)) == 0)
-          a.scale[row * groups + (at >> group_bits)] = e4m3_scale(m);
-        const f32x2 by = both(e4m3_inverse(m));
-#pragma unroll
-        for (int k = 0; k < H; ++k) r[i][k] = mul2(r[i][k], by);
+          a.scale[row * groups + (at >> group_bits)] = by.scale;
+        by.divide(r[i]);
       }
     }
     if (!a.scale) continue;
     if (!a.group) {
-      const float m = row_max(most, threads, red);
-      if (t == 0) a.scale[row] = e4m3_scale(m);
-      const f32x2 by = both(e4m3_inverse(m));
+      const E4m3Scale by(row_max(most, threads, red));
+      if (t == 0) a.scale[row] = by.scale;
 #pragma unroll
-      for (int i = 0; i < PER; ++i)
-#pragma unroll
-        for (int k = 0; k < H; ++k) r[i][k] = mul2(r[i][k], by);
+      for (int i = 0; i < PER; ++i) by.divide(r[i]);
     }
     uint8_t* out = static_cast<uint8_t*>(a.out) + row * a.out_stride;
     const bool wide = V == 8 && (reinterpret_cast<uintptr_t>(out) & 7) == 0;
