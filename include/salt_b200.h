@@ -389,9 +389,9 @@ enum { SALT_F32 = 0, SALT_F16 = 1, SALT_BF16 = 2 };
  * `weight_type` (`type` or SALT_F32) the weight (dim).  r is rounded only where it is stored.
  * residual_out and rstd (rows) may be NULL; residual_out may be residual itself, out may be x.
  * With `scale` given, out is 8 bits (e4m3) instead: each group of `group` (32, 64, 128, 256, or
- * 0 = the whole row) neighbouring elements has scale = max|out| / 448 (1 where the group is zero)
- * and out = the nearest e4m3 of value / scale, ties to even, both of them quotients rounded to
- * float32; scale is (rows, ceil(dim / group)) float32. */
+ * 0 = the whole row) neighbouring elements has scale = max|out| / 448 (at least 2^-149, float32's
+ * smallest value; 1 where the group is zero) and out = the nearest e4m3 of value / scale, ties to
+ * even, both of them quotients rounded to float32; scale is (rows, ceil(dim / group)) float32. */
 typedef struct {
   int32_t rows, dim;
   int32_t type, residual_type, weight_type;

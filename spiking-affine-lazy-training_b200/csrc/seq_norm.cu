@@ -66,8 +66,8 @@ __device__ __forceinline__ void load_weight_pairs(f32x2 (&w)[(V + 1) / 2], const
   }
 }
 
-// The scale of a group whose largest magnitude is m: the float32 quotient m / 448 (1 for a group of
-// zeros), and what divides the group's values by it.  fmaxf leaves NaNs out of m: they become e4m3's
+// The scale of a group whose largest magnitude is m: the float32 quotient m / 448 (at least float32's
+// smallest value; 1 for a group of zeros), and what divides the group's values by it.  fmaxf leaves NaNs out of m: they become e4m3's
 // own, beside the other elements' scale.
 //
 // A product with one rounded inverse may bring a value near the middle of two 8-bit ones to the other
@@ -89,7 +89,7 @@ struct E4m3Scale {
       const float q = m * by;
       divisor = scale = fmaf(fmaf(-q, kE4m3Max, m), by, q);
     } else {
-      scale = m == 0.f ? 1.f : m / kE4m3Max;
+      scale = m == 0.f ? 1.f : fmaxf(m / kE4m3Max, 0x1p-149f);  // a scale of 0 would divide by it
       lift = m < 1.f ? 0x1p64f : 0x1p-64f;
       divisor = scale * lift;
     }
@@ -118,8 +118,8 @@ struct E4m3Scale {
 // residual to 8 bits by groups of 128: 143 us against 150 us with a block for each row, 167 us with
 // branches around the loads, 123 us without divisions by the group's size, 128 us with exact
 // quotients).  Those 128 us are 4.6 TB/s or 71 % of the measured copy rate; an instruction issues in
-// two of three cycles, so what is left is shared by instructions and the two barriers of a row's sum.  Few rows cost the call
-// alone: 10 us from the host.
+// two of three cycles, so what is left is shared by instructions and the two barriers of a row's sum.
+// Few rows cost the call alone: 10 us from the host.
 template <typename T, typename R, int V, int PER, bool VEC>
 __global__ void __launch_bounds__(kRowThreadsMost, V * PER <= 8 ? 3 : V * PER <= 16 ? 2 : 1)
 rms_norm_kernel(salt_rms_norm_args a, int threads, bool w_f32, int group_bits, int groups) {

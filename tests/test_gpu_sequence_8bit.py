@@ -35,7 +35,7 @@ def check(x, w, group, eps=1e-5, kind="float32", residual=None):
     wide = wide.reshape(rows, -1, g)
     most = np.abs(wide).max(-1)
     with np.errstate(under="ignore"):
-        scale = np.where(most == 0, F(1), most / F(448))
+        scale = np.where(most == 0, F(1), np.maximum(most / F(448), F(2.0 ** -149)))
         want = e4m3(wide / scale[..., None]).reshape(rows, -1)[:, :dim]
     np.testing.assert_array_equal(got.scale.numpy(), scale)
     np.testing.assert_array_equal(R.values(got.out), want)
@@ -73,3 +73,18 @@ def test_8_bits_of_large_values(group):
     w = (rng.uniform(0.5, 1, 512) * 2.0 ** 126).astype(F)
     x[np.abs(x) > 2] = 2  # below 2^128 with the factor, which is about 1
     check(x, w, group)
+
+
+@pytest.mark.parametrize("kind", ("float32", "bfloat16"))
+@pytest.mark.parametrize("group", [0, 32])
+def test_8_bits_of_tiny_values(kind, group):
+    """Groups of tiny values and zeros, down to float32's smallest: zeros stay zeros, and values keep
+    their places between them."""
+    rng = np.random.default_rng(2)
+    sizes = np.array([1e-30, 1e-35, 1.2e-36, 1e-37, 1e-38, 1e-40, 1e-42, 1e-43, 3e-45, 0])
+    w = np.repeat(sizes, 32) * rng.uniform(0.01, 1, 320) * rng.choice([0, 1, 1, -1], 320)
+    w = R.rounded(w, kind)
+    x = R.rounded(rng.normal(size=(4, 320)), kind)
+    check(x, w, group, kind=kind)
+    for k in range(0, 320, 32):  # one size a row
+        check(x[:, k:k + 32], w[k:k + 32], group, kind=kind)
