@@ -91,7 +91,8 @@ causal_conv_kernel(salt_causal_conv_args a, int packs, int runs, int run, bool w
       to_pairs<V>(win[j], f);
     }
   }
-  // Reads its own channels of initial_state, here and above, before it writes: they may be one.
+  // initial_state and final_state may be one array: of a row's threads this one alone reads its
+  // channels of the first, here and above, before it writes the second.
   if (c == 0 && a.final_state && W > 1) {
     T* fin = static_cast<T*>(a.final_state) + state0;
     float f[W][V];
@@ -301,10 +302,12 @@ causal_conv_backward_kernel(salt_causal_conv_backward_args a, int packs, int chu
   } while (0)
 
 // Tokens of a thread's run: long enough that the tokens read twice are few, short enough that the
-// threads fill the GPU.
-int conv_run(int64_t packs, int32_t batch, int32_t len) {
+// threads fill the GPU.  No run is shorter than the width - 1 tokens in front of the next one, which
+// would then reach into the initial state: a row's first run may be writing the final state there.
+int conv_run(int64_t packs, int32_t batch, int32_t len, int32_t width) {
+  const int least = width <= 5 ? 4 : 8;
   int run = 32;
-  while (run > 4 && packs * batch * ((len + run - 1) / run) < 148 * 1024) run >>= 1;
+  while (run > least && packs * batch * ((len + run - 1) / run) < 148 * 1024) run >>= 1;
   return run;
 }
 
@@ -339,7 +342,7 @@ cudaError_t causal_conv_launch(const salt_causal_conv_args& a, cudaStream_t st, 
            pack_rows(a.out, v, ts, a.out_batch_stride, a.out_stride);
   };
     const int v = fits(kRowVec) ? kRowVec : 1, packs = a.dim / v;
-  const int run = conv_run(packs, a.batch, a.len);
+  const int run = conv_run(packs, a.batch, a.len, a.width);
   const int runs = std::max(1, (a.len + run - 1) / run);  // a row without tokens has a final state
   const int64_t threads = (int64_t)packs * runs * a.batch;
   const unsigned blocks = (unsigned)((threads + 127) / 128);
