@@ -104,7 +104,7 @@ Checks check(const salt_rms_norm_backward_args* a) {
   const bool used = a->rows > 0;
   c.input(a->dy, used, "dy is NULL");
   c.input(a->x, used, "x is NULL");
-  c.input(a->weight, used, "weight is NULL");
+  c.input(a->weight, true, "weight is NULL");  // without rows, too, a block loads it
   c.input(a->rstd, used, "rstd is NULL");
   c.input(a->dx, used, "dx is NULL");
   c.strides(a->dy_stride, a->x_stride, "a stride is negative");
