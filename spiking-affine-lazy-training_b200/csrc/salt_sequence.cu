@@ -163,7 +163,7 @@ Checks check(const salt_causal_conv_backward_args* a) {
   const bool used = a->batch > 0 && a->len > 0;
   c.input(a->dy, used, "dy is NULL");
   c.input(a->x, used, "x is NULL");
-  c.input(a->weight, used, "weight is NULL");
+  c.input(a->weight, a->batch > 0, "weight is NULL");  // rows without tokens load it, too
   c.input(a->dx, used, "dx is NULL");
   c.input(a->dweight, true, "dweight is NULL");
   c.strides(a->x_batch_stride, a->x_stride, "a stride is negative");

@@ -33,3 +33,8 @@ def test_norm_backward_of_no_rows_needs_its_weight():
     with pytest.raises(ValueError, match="weight is NULL"):
         sequence.rms_norm_backward(fake((0, 64)), fake((0, 64)), None, fake((0,)),
                                    dx=fake((0, 64)), dweight=fake((64,)))
+
+
+def test_conv_backward_of_no_tokens_needs_its_weight():
+    a = _lib.CausalConvBackwardArgs(batch=2, len=0, dim=16, width=4, dweight=AT)
+    refused("salt_causal_conv_backward", a, b"weight is NULL")
