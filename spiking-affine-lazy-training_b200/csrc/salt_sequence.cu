@@ -188,7 +188,7 @@ void scan_common(Checks& c, const A* a, int32_t len) {
   c.input(a->delta, used, "delta is NULL");
   c.input(a->B, used, "B is NULL");
   c.input(a->C, used, "C is NULL");
-  c.input(a->A, used, "A is NULL");
+  c.input(a->A, a->batch > 0, "A is NULL");  // rows without tokens load it, too
   c.strides(a->x_stride, a->delta_stride, "a stride is negative");
   c.strides(a->B_stride, a->C_stride, "a stride is negative");
   c.strides(a->z_stride, 0, "a stride is negative");

@@ -38,3 +38,16 @@ def test_norm_backward_of_no_rows_needs_its_weight():
 def test_conv_backward_of_no_tokens_needs_its_weight():
     a = _lib.CausalConvBackwardArgs(batch=2, len=0, dim=16, width=4, dweight=AT)
     refused("salt_causal_conv_backward", a, b"weight is NULL")
+
+
+def test_scan_of_no_tokens_needs_its_decay():
+    a = _lib.SelectiveScanArgs(batch=2, len=0, dim=16, state=8, groups=1)
+    refused("salt_selective_scan", a, b"A is NULL")
+    with pytest.raises(ValueError, match="A is NULL"):
+        sequence.selective_scan(fake((2, 0, 16)), fake((2, 0, 16)), None, fake((2, 0, 1, 8)),
+                                fake((2, 0, 1, 8)), out=fake((2, 0, 16)))
+
+
+def test_scan_backward_of_no_tokens_needs_its_decay():
+    a = _lib.SelectiveScanBackwardArgs(batch=2, len=0, dim=16, state=8, groups=1, dA=AT)
+    refused("salt_selective_scan_backward", a, b"A is NULL")
