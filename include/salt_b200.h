@@ -379,7 +379,8 @@ salt_status salt_float_fc_layer_trace(const salt_float_fc_desc *layer, const flo
  *   - Gradients of weights are sums over rows in an order fixed by the sizes: no atomics, the same
  *     inputs give the same bits.  `workspace` needs the bytes the matching *_workspace_size
  *     returns (256-byte aligned; may be NULL when that is 0) and no initialisation.
- *   - Outputs may not overlap inputs unless a comment says so. */
+ *   - Outputs may not overlap inputs unless a comment says so, nor may an output's rows overlap
+ *     each other (strides that let them are refused). */
 enum { SALT_F32 = 0, SALT_F16 = 1, SALT_BF16 = 2 };
 
 /* Root-mean-square norm with the residual's addition, over rows of `dim` <= 16384 elements:

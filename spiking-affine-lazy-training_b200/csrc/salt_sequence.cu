@@ -10,6 +10,26 @@ namespace {
 constexpr int32_t kMostLen = 1 << 30;
 constexpr int32_t kMostDim = 1 << 24;
 
+// Whether no two of rows * len runs of `dim` elements, at b * batch + t * token, share an element.
+bool apart(int64_t batch, int64_t token, int32_t rows, int32_t len, int32_t dim) {
+  if (rows < 1 || len < 1) return true;
+  if ((len > 1 && token < dim) || (rows > 1 && batch < dim)) return false;
+  if (len == 1 || rows == 1) return true;
+  using wide = __int128;
+  // one axis lies within a step of the other, either way around
+  if (batch >= (wide)(len - 1) * token + dim || token >= (wide)(rows - 1) * batch + dim) return true;
+  // else a step of one axis must not meet any of the other: only the two around it can
+  const bool few = rows < len;
+  const int64_t outer = few ? batch : token, inner = few ? token : batch;
+  const int32_t steps = few ? rows : len, most = few ? len : rows;
+  for (int32_t i = 1; i < steps; ++i) {
+    const wide at = (wide)i * outer, j = at / inner;
+    if ((j < most && at - j * inner < dim) || (j + 1 < most && (j + 1) * inner - at < dim))
+      return false;
+  }
+  return true;
+}
+
 // The first failed check of a call; `ok` stays true while all hold.
 struct Checks {
   const char* who;
@@ -33,9 +53,7 @@ struct Checks {
   }
   void written(int64_t batch, int64_t token, int32_t rows, int32_t len, int32_t dim,
                const char* text) {
-    need(batch >= 0 && token >= 0 && (len <= 1 || token >= dim) &&
-             (rows <= 1 || len == 0 || batch >= dim),
-         text);
+    need(batch >= 0 && token >= 0 && apart(batch, token, rows, len, dim), text);
   }
   salt_status status() const { return host_fail(SALT_BAD_ARG, why); }
 };
@@ -132,7 +150,7 @@ Checks check(const salt_causal_conv_args* a) {
   c.input(a->out, used, "out is NULL");
   c.strides(a->x_batch_stride, a->x_stride, "a stride is negative");
   c.written(a->out_batch_stride, a->out_stride, a->batch, a->len, a->dim,
-            "out's strides must be at least dim");
+            "out's strides let its rows overlap");
   return c;
 }
 
@@ -169,7 +187,7 @@ Checks check(const salt_causal_conv_backward_args* a) {
   c.strides(a->x_batch_stride, a->x_stride, "a stride is negative");
   c.strides(a->dy_batch_stride, a->dy_stride, "a stride is negative");
   c.written(a->dx_batch_stride, a->dx_stride, a->batch, a->len, a->dim,
-            "dx's strides must be at least dim");
+            "dx's strides let its rows overlap");
   return c;
 }
 
@@ -209,7 +227,7 @@ Checks check(const salt_selective_scan_args* a) {
   scan_batch_strides(c, a);
   c.input(a->out, a->batch > 0 && a->len > 0, "out is NULL");
   c.written(a->out_batch_stride, a->out_stride, a->batch, a->len, a->dim,
-            "out's strides must be at least dim");
+            "out's strides let its rows overlap");
   return c;
 }
 
@@ -242,7 +260,7 @@ Checks check(const salt_selective_scan_backward_args* a) {
   c.input(a->dA, true, "dA is NULL");
   c.need(!used || (a->z == nullptr) == (a->dz == nullptr), "dz is needed exactly where z is given");
   c.strides(a->dy_batch_stride, a->dy_stride, "a stride is negative");
-  const char* text = "a gradient's strides must be at least dim";
+  const char* text = "a gradient's strides let its rows overlap";
   c.written(a->dx_batch_stride, a->dx_stride, a->batch, a->len, a->dim, text);
   c.written(a->ddelta_batch_stride, a->ddelta_stride, a->batch, a->len, a->dim, text);
   if (a->dz) c.written(a->dz_batch_stride, a->dz_stride, a->batch, a->len, a->dim, text);
