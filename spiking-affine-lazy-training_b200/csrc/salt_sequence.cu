@@ -144,6 +144,9 @@ Checks check(const salt_causal_conv_args* a) {
   if (!c.ok()) return c;
   conv_common(c, a);
   shape(c, a->batch, a->len, a->dim);
+  // a thread takes one channel through 32 tokens at most there, and counts its row's in 32 bits
+  c.need((int64_t)a->dim * ((a->len + 31) / 32) <= (int64_t)UINT32_MAX,
+         "len * dim is too large for one launch");
   const bool used = a->batch > 0 && a->len > 0;
   c.input(a->x, used, "x is NULL");
   c.input(a->weight, used, "weight is NULL");

@@ -72,8 +72,8 @@ causal_conv_kernel(salt_causal_conv_args a, int packs, int runs, int run, bool w
   const int64_t per_row = (int64_t)packs * runs;
   if (id >= per_row * a.batch) return;
   const int b = (int)(id / per_row);
-  const int rest = (int)(id - b * per_row);
-  const int c = rest / packs, d0 = (rest - c * packs) * V;
+  const uint32_t rest = (uint32_t)(id - b * per_row);  // a row has under 2^32 threads
+  const int c = rest / (uint32_t)packs, d0 = (int)(rest - c * (uint32_t)packs) * V;
   const int n = a.dim - d0;  // at least V: V divides dim
   const int real = row_tokens(a.n_real, b, a.len);
   const T* x = static_cast<const T*>(a.x) + b * a.x_batch_stride + d0;
