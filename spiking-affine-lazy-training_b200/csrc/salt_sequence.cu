@@ -253,6 +253,8 @@ Checks check(const salt_selective_scan_backward_args* a) {
   if (!c.ok()) return c;
   scan_common(c, a, a->len);
   scan_batch_strides(c, a);
+  // the kernel that writes dB and dC counts a token's values of both in 32 bits
+  c.need((int64_t)2 * a->state * a->groups <= INT32_MAX, "groups * state is too large");
   const bool used = a->batch > 0 && a->len > 0;
   c.input(a->dy, used, "dy is NULL");
   c.input(a->checkpoints, used, "checkpoints is NULL");
