@@ -218,11 +218,12 @@ class Graph:
 
 class _Allocation:
     """One device allocation, freed (stream-ordered) on the stream that made it."""
-    __slots__ = ("ptr", "nbytes", "stream", "__weakref__")
+    __slots__ = ("ptr", "nbytes", "stream", "device", "__weakref__")
 
     def __init__(self, nbytes: int):
         self.nbytes = int(nbytes)
         self.stream = current_stream()
+        self.device = current_device()
         p = ctypes.c_void_p()
         _lib.check(_lib.lib().salt_malloc(ctypes.c_size_t(max(self.nbytes, 1)), self.stream.ptr,
                                           ctypes.byref(p)))
@@ -237,13 +238,15 @@ def _free_on(ptr: int, stream: "Stream") -> None:
 
 class DeviceArray:
     """A C-contiguous array in device memory: shape, numpy dtype and a device pointer.
-    Indexing the leading axis (an integer or a step-1 slice) gives a view sharing the memory."""
-    __slots__ = ("ptr", "shape", "dtype", "_owner")
+    Indexing the leading axis (an integer or a step-1 slice) gives a view sharing the memory.
+    `device` is the index of the GPU whose memory it is, None for a pointer from elsewhere."""
+    __slots__ = ("ptr", "shape", "dtype", "device", "_owner")
 
     def __init__(self, ptr: int, shape, dtype, owner):
         self.ptr = int(ptr)
         self.shape = tuple(int(v) for v in shape)
         self.dtype = np.dtype(dtype)
+        self.device = owner.device if isinstance(owner, (_Allocation, DeviceArray)) else None
         self._owner = owner
 
     # construction

@@ -29,7 +29,7 @@ from typing import NamedTuple
 import numpy as np
 
 from . import _lib
-from .device import DeviceArray, _tls, bfloat16, current_device, empty, float8_e4m3
+from .device import DeviceArray, _tls, bfloat16, empty, float8_e4m3
 
 CHECKPOINT = 16       # tokens between the scan's checkpoints (SALT_SCAN_CHECKPOINT)
 GROUPS_8BIT = (0, 32, 64, 128, 256)
@@ -113,9 +113,9 @@ def _activation(a, name: str) -> int:
     return t
 
 
-def _look(a, name: str, shape: tuple, type_id: int, inner: int) -> None:
-    """Raises unless `a` is an array of that shape and type on the current device whose last
-    `inner` axes are contiguous (an axis of length 1 has any stride)."""
+def _look(here: int, a, name: str, shape: tuple, type_id: int, inner: int) -> None:
+    """Raises unless `a` is an array of that shape and type on device `here` whose last `inner`
+    axes are contiguous (an axis of length 1 has any stride)."""
     if not hasattr(a, "data_ptr"):
         raise TypeError(f"{name}: needs a device array, got {type(a).__name__}")
     if tuple(a.shape) != shape:
@@ -129,9 +129,12 @@ def _look(a, name: str, shape: tuple, type_id: int, inner: int) -> None:
             raise ValueError(f"{name}: must be contiguous" if inner == len(shape) else
                              f"{name}: its last {inner} axes must be contiguous")
         at *= n
-    where = getattr(a, "get_device", None)
-    if where is not None and where() != current_device():
-        raise ValueError(f"{name}: not on the current device ({current_device()})")
+    if isinstance(a, DeviceArray):
+        where = here if a.device is None else a.device
+    else:
+        where = a.get_device() if hasattr(a, "get_device") else here
+    if where != here:
+        raise ValueError(f"{name}: not on the current device ({here})")
 
 
 def _stream():
@@ -156,7 +159,8 @@ def _whole(here: int, a, name: str, shape: tuple, type_id: int) -> int:
     if a is None:
         return 0
     if type(a) is DeviceArray:
-        if a.shape == shape and _TYPE_IDS.get(a.dtype) == type_id:
+        if a.shape == shape and _TYPE_IDS.get(a.dtype) == type_id \
+                and (a.device == here or a.device is None):
             return a.ptr
     elif type(a) in _TORCH_LIKE:
         if a.shape == shape and _TYPE_IDS.get(a.dtype) == type_id and a.is_contiguous() \
@@ -164,7 +168,7 @@ def _whole(here: int, a, name: str, shape: tuple, type_id: int) -> int:
             return a.data_ptr()
     elif hasattr(a, "is_contiguous") and hasattr(a, "get_device"):
         _TORCH_LIKE.add(type(a))
-    _look(a, name, shape, type_id, len(shape))
+    _look(here, a, name, shape, type_id, len(shape))
     return a.data_ptr()
 
 
@@ -174,13 +178,14 @@ def _rows(here: int, a, name: str, shape: tuple, type_id: int, inner: int = 1):
     if a is None:
         return 0, (0,) * (len(shape) - inner)
     if type(a) is DeviceArray:
-        if a.shape == shape and _TYPE_IDS.get(a.dtype) == type_id:
+        if a.shape == shape and _TYPE_IDS.get(a.dtype) == type_id \
+                and (a.device == here or a.device is None):
             return a.ptr, _dense(shape)[:-inner]
     elif type(a) in _TORCH_LIKE and a.shape == shape and _TYPE_IDS.get(a.dtype) == type_id:
         s = a.stride()
         if s[-1] == 1 and (inner == 1 or s[-2] == shape[-1]) and a.get_device() == here:
             return a.data_ptr(), s[:-inner]
-    _look(a, name, shape, type_id, inner)
+    _look(here, a, name, shape, type_id, inner)
     return a.data_ptr(), tuple(a.stride())[:-inner]
 
 
