@@ -370,7 +370,8 @@ salt_status salt_float_fc_layer_trace(const salt_float_fc_desc *layer, const flo
  * Conventions of this section
  *   - Activations are (batch, len, dim); channels are contiguous, batch and token strides are
  *     given in elements, so that slices of one projection need no copy.  They hold SALT_F32,
- *     SALT_F16 or SALT_BF16 (`type`); all arithmetic, sums and states are 32-bit floats.
+ *     SALT_F16 or SALT_BF16 (`type`); all arithmetic, sums and states are 32-bit floats, with
+ *     exponentials and reciprocals good to about 2 units in the last place.
  *   - n_real (batch, may be NULL = len) gives each row's tokens, clamped to [0, len].  Inputs past
  *     them are never read; outputs past them are written as zero.  A row without tokens returns its
  *     initial state (zero where none is given).

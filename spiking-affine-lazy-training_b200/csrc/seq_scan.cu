@@ -237,8 +237,8 @@ selective_scan_kernel(salt_selective_scan_args a, ScanSplit sp, int blocks, bool
 #pragma unroll
             for (int j = 0; j < CPT; ++j) {
               f32x2 &h0 = h[j][i / 2], &h1 = h[j][i / 2 + 1];
-              h0 = fma2(exp2_fast2(mul2(A2[j][i / 2], s[j])), h0, mul2(sx[j], bn.x));
-              h1 = fma2(exp2_fast2(mul2(A2[j][i / 2 + 1], s[j])), h1, mul2(sx[j], bn.y));
+              h0 = fma2(decay2(A2[j][i / 2], s[j]), h0, mul2(sx[j], bn.x));
+              h1 = fma2(decay2(A2[j][i / 2 + 1], s[j]), h1, mul2(sx[j], bn.y));
             }
             if (FULL) {
               const ulonglong2 cn = *reinterpret_cast<const ulonglong2*>(&sm.C[g + q][n0 + i]);
@@ -421,7 +421,7 @@ selective_scan_step_kernel(salt_selective_scan_step_args a, int blocks, int rows
         const f32x2 bn = in ? pair_of(now.B[i / 4], i % 4) : 0;
         const f32x2 cn = in ? pair_of(now.C[i / 4], i % 4) : 0;
         const f32x2 v =
-            fma2(exp2_fast2(mul2(A2[i / 2], s2)), pair(h[i], h[i + 1]), mul2(sx2, bn));
+            fma2(decay2(A2[i / 2], s2), pair(h[i], h[i + 1]), mul2(sx2, bn));
         y2 = fma2(v, cn, y2);
         const float2 f = halves(v);
         h[i] = f.x, h[i + 1] = f.y;

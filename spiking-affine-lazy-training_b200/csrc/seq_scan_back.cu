@@ -267,8 +267,8 @@ selective_scan_backward_kernel(salt_selective_scan_backward_args a, ScanSplit sp
         for (int j = 0; j < CPT; ++j) {
           const float2 st = sm.step[u * kGroup + q][at[j]];
           const f32x2 s = both(st.x), sx = both(st.y);
-          h[j][0] = fma2(exp2_fast2(mul2(A[j][0], s)), h[j][0], mul2(sx, bn.x));
-          h[j][1] = fma2(exp2_fast2(mul2(A[j][1], s)), h[j][1], mul2(sx, bn.y));
+          h[j][0] = fma2(decay2(A[j][0], s), h[j][0], mul2(sx, bn.x));
+          h[j][1] = fma2(decay2(A[j][1], s), h[j][1], mul2(sx, bn.y));
         }
       }
 #pragma unroll
@@ -300,8 +300,8 @@ selective_scan_backward_kernel(salt_selective_scan_backward_args a, ScanSplit sp
           const float2 st = sm.step[u * kGroup + q][at[j]];
           const f32x2 s = both(st.x), sx = both(st.y);
           const f32x2* before = q ? hs[q ? q - 1 : 0][j] : h0[j];
-          ea[q][j][0] = exp2_fast2(mul2(A[j][0], s));
-          ea[q][j][1] = exp2_fast2(mul2(A[j][1], s));
+          ea[q][j][0] = decay2(A[j][0], s);
+          ea[q][j][1] = decay2(A[j][1], s);
           hs[q][j][0] = fma2(ea[q][j][0], before[0], mul2(sx, bn.x));
           hs[q][j][1] = fma2(ea[q][j][1], before[1], mul2(sx, bn.y));
         }
@@ -603,8 +603,8 @@ scan_back_state_kernel(salt_selective_scan_backward_args a, ScanSplit sp, int bl
         const float2 st = sm.step[q][at + j];
         sum[j] += st.x;
         const f32x2 s = pair(st.x, st.x), g = pair(st.y, st.y);
-        carry[j][0] = mul2(exp2_fast2(mul2(A2[j][0], s)), fma2(g, cn.x, carry[j][0]));
-        carry[j][1] = mul2(exp2_fast2(mul2(A2[j][1], s)), fma2(g, cn.y, carry[j][1]));
+        carry[j][0] = mul2(decay2(A2[j][0], s), fma2(g, cn.x, carry[j][0]));
+        carry[j][1] = mul2(decay2(A2[j][1], s), fma2(g, cn.y, carry[j][1]));
       }
     }
   }
