@@ -465,7 +465,8 @@ salt_status salt_causal_conv_step(const salt_causal_conv_step_args *args, void *
 
 /* Gradient of salt_causal_conv for the gradient dy of out.  dweight (dim, width) and dbias (dim)
  * are float32; dx and dinitial (batch, dim, width - 1) hold `type`; dinitial and dbias may be
- * NULL. */
+ * NULL.  A gradient of final_state is the caller's to add: that state holds inputs as they are, the
+ * row's last width - 1 tokens (in front of them, in shorter rows, initial_state's entries). */
 typedef struct {
   int32_t batch, len, dim, width;
   int32_t type, weight_type;
@@ -487,8 +488,8 @@ salt_status salt_causal_conv_backward(const salt_causal_conv_backward_args *args
  * softplus(s) = log(1 + exp(s)) with softplus set:
  *   h[t] = exp(s[t] A) h[t-1] + s[t] x[t] B[t];  y = sum_n C[t] h[t] + D x[t];
  *   out = y, or y * z * sigmoid(z) where z is given.
- * h is (dim, state) per row, `state` 1 to 64; A (dim, state), D (dim, may be NULL) and delta_bias
- * (dim, may be NULL) are float32; B and C are (batch, len, groups, state) with contiguous
+ * h is (dim, state) per row, `state` 1 to 64; A (dim, state, finite), D (dim, may be NULL) and
+ * delta_bias (dim, may be NULL) are float32; B and C are (batch, len, groups, state) with contiguous
  * (groups, state), and channel d reads group d / (dim / groups).  initial_state and final_state
  * (batch, dim, state) float32 may be NULL, or be the same array.
  * checkpoints (may be NULL) receives what the backward pass restarts from, the state in front of

@@ -53,7 +53,7 @@ struct Checks {
   }
   void written(int64_t batch, int64_t token, int32_t rows, int32_t len, int32_t dim,
                const char* text) {
-    need(batch >= 0 && token >= 0 && apart(batch, token, rows, len, dim), text);
+    if (ok()) need(batch >= 0 && token >= 0 && apart(batch, token, rows, len, dim), text);
   }
   salt_status status() const { return host_fail(SALT_BAD_ARG, why); }
 };
@@ -145,7 +145,7 @@ Checks check(const salt_causal_conv_args* a) {
   conv_common(c, a);
   shape(c, a->batch, a->len, a->dim);
   // a thread takes one channel through 32 tokens at most there, and counts its row's in 32 bits
-  c.need((int64_t)a->dim * ((a->len + 31) / 32) <= (int64_t)UINT32_MAX,
+  c.need((int64_t)a->dim * (((int64_t)a->len + 31) / 32) <= (int64_t)UINT32_MAX,
          "len * dim is too large for one launch");
   const bool used = a->batch > 0 && a->len > 0;
   c.input(a->x, used, "x is NULL");

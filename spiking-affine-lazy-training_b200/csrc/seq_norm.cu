@@ -120,6 +120,9 @@ struct E4m3Scale {
 // quotients).  Those 128 us are 4.6 TB/s or 71 % of the measured copy rate; an instruction issues in
 // two of three cycles, so what is left is shared by instructions and the two barriers of a row's sum.
 // Few rows cost the call alone: 10 us from the host.
+// The registers are held down for more threads than the grid starts (1024 an SM), and the compiler
+// spills: 36 to 536 bytes a thread for packs of 8, 36 to 604 for packs of 4 and 532 to 824 for packs of
+// 1.  Those take 144 us for 8192 rows of 2501 in bf16, where rows of 4096 take 52 us.
 template <typename T, typename R, int V, int PER, bool VEC>
 __global__ void __launch_bounds__(kRowThreadsMost, V * PER <= 8 ? 3 : V * PER <= 16 ? 2 : 1)
 rms_norm_kernel(salt_rms_norm_args a, int threads, bool w_f32, int group_bits, int groups) {
@@ -235,6 +238,8 @@ rms_norm_kernel(salt_rms_norm_args a, int threads, bool w_f32, int group_bits, i
 // row of it, which sum_parts adds up in order.  All three arrays' loads of a row go out before the
 // barriers of its sum: 59 us against 77 us with branches between them, for 8190 rows of 2500 (packs
 // of 4) in bf16 with a 32-bit residual, sum_parts' 7 us included: 4.9 TB/s, 75 % of the copy rate.
+// Rows over 8192 wide spill 416 to 1956 bytes a thread (8192 rows of 12288 in bf16: 254 us, those of
+// 4096 80 us).
 template <typename T, typename R, int V, int PER, bool VEC>
 __global__ void __launch_bounds__(kRowThreadsMost)
 rms_norm_backward_kernel(salt_rms_norm_backward_args a, int threads, bool w_f32, float* parts) {

@@ -4,8 +4,9 @@
 // each state, against one read of x, delta and z and one write of out for all of them.  What bounds
 // the scan is the exponentials (16 a cycle and SM) and the shared memory that hands B, C and s to
 // every lane (128 bytes a cycle), not memory: 8 rows of 2048 tokens x 4096 channels x 16 states in
-// bf16 take 489 us, where the exponentials (the states' and four a token and channel) need 290 us
-// and the bytes 166 us.  The same rows ragged, from none to 2048 tokens: 309 us.
+// bf16 take 488 us, where the exponentials (the states' and four a token and channel) need 290 us
+// and the bytes 83 us.  The same rows ragged, from none to 2048 tokens: 304 to 319 us by the order of
+// their lengths.
 #include <algorithm>
 
 #include "seq_scan.cuh"
@@ -465,8 +466,11 @@ using Step64 = StepShape<16, 4>;
 #define SALT_STEP_SHAPE(state, S, ...) \
   SALT_BY_STATE(state, S, Step4, Step8, Step16, Step32, Step64, __VA_ARGS__)
 
-// One row of 16384 tokens x 2048 channels x 16 states: 406 us in 22 chunks, where 5 chunks take
-// 530 us, and the first pass 0.55 of the second's time.
+// One row of 16384 tokens x 2048 channels x 16 states: 406 us in 23 chunks, where 5 chunks take
+// 530 us, and the first pass 0.55 of the second's time.  Both constants are those of 9 to 16 states in
+// 16 bits; the rule takes them for all shapes, although the GPU holds about 20 of the blocks for up
+// to 8 states an SM, 8 of those for 32 and 3 for 64 (4 rows of 2048 tokens x 2048 channels in bf16:
+// 138, 146, 332 and 651 us at 4, 8, 32 and 64 states).
 constexpr int kSlots = 148 * 5;      // blocks of 128 threads at 96 registers
 constexpr float kFirstPass = 0.55f;  // its time, of the second pass's
 

@@ -12,7 +12,8 @@ float16 or bfloat16 (`device.bfloat16`), (batch, len, dim) with contiguous chann
 and batch strides; weights of the norm and the convolution hold that type or float32; the scan's
 ``A``, ``D``, ``delta_bias`` and its states are float32.  Every output is written into the array
 given for it, or into a new `DeviceArray` where none is; an optional output takes ``None`` (not
-wanted), ``True`` (make one) or an array.
+wanted), ``True`` (make one) or an array.  Calls work on the arrays' memory alone: another library's
+automatic differentiation does not see them, and gradients come from the `*_backward` calls.
 
 Streams: a call enqueues on `device.current_stream()` and orders nothing else.  Arrays that another
 stream writes have to be waited for (`Stream.wait_event`, `Stream.external`), and must stay
@@ -407,7 +408,9 @@ def causal_conv_backward(dy, x, weight, bias=None, *, n_real=None, initial_state
                          ) -> ConvGradients:
     """Gradients of `causal_conv` for dy, the gradient of its out.  dweight and dbias are float32
     (dbias is made where there is a bias); dinitial (batch, dim, width - 1) holds x's type and is
-    optional."""
+    optional.  A gradient of final_state is not taken: that state holds inputs as they are, so it is
+    the caller's to add to dx of the row's last width - 1 tokens (and to dinitial, in shorter
+    rows)."""
     here = _here()
     t = _activation(x, "x")
     batch, n, dim = shape = _axes(x, "x", 3)
@@ -447,7 +450,7 @@ def selective_scan(x, delta, A, B, C, *, D=None, z=None, delta_bias=None, softpl
         h[t] = exp(s[t] A) h[t-1] + s[t] x[t] B[t];   y[t] = sum_n C[t] h[t] + D x[t]
 
     and ``out = y``, or ``y * z * sigmoid(z)`` where z is given.  x, delta, z: (batch, len, dim); A:
-    (dim, state) float32, state 1 to 64; B, C: (batch, len, groups, state), channel d reading group
+    (dim, state) float32, finite, state 1 to 64; B, C: (batch, len, groups, state), channel d reading group
     ``d // (dim / groups)``; D, delta_bias: (dim,) float32.  n_real (batch, int32) ends each row
     early.  initial_state and final_state: (batch, dim, state) float32, may be one array.
     checkpoints takes the states that `selective_scan_backward` starts from."""
