@@ -553,6 +553,119 @@ salt_status salt_selective_scan_backward_workspace_size(
 salt_status salt_selective_scan_backward(const salt_selective_scan_backward_args *args,
                                          void *workspace, size_t workspace_bytes, void *stream);
 
+/* Linear attention with a decay for each head: an affine recurrence whose state is a matrix,
+ *   S[t] = exp(log_decay[h]) S[t-1] + k[t]^T v[t];  out[t] = scale * q[t] S[t],
+ * with S (dim_k, dim_v) for each row and head.  q is (batch, len, heads, dim_k), k and v are
+ * (batch, len, kv_heads, dim_k or dim_v), out (batch, len, heads, dim_v), all with contiguous
+ * (heads, dim); head h reads key head h / (heads / kv_heads).  dim_k and dim_v are 1 to 128.
+ * log_decay (heads) is float32 and at most 0: greater values count as 0, values under -200 as -200
+ * (a decay that float32 rounds to 0).  initial_state and final_state (batch, heads, dim_k, dim_v)
+ * float32 may be NULL, or be the same array. */
+typedef struct {
+  int32_t batch, len, heads, kv_heads, dim_k, dim_v;
+  int32_t type;
+  float scale;
+  int64_t q_batch_stride, q_stride, k_batch_stride, k_stride, v_batch_stride, v_stride,
+      out_batch_stride, out_stride;
+  const void *q, *k, *v;
+  const float *log_decay;
+  const int32_t *n_real;
+  const float *initial_state;
+  void *out;
+  float *final_state;
+} salt_linear_attention_args;
+
+salt_status salt_linear_attention_workspace_size(const salt_linear_attention_args *args,
+                                                 size_t *bytes);
+salt_status salt_linear_attention(const salt_linear_attention_args *args, void *workspace,
+                                  size_t workspace_bytes, void *stream);
+
+/* One token for each of `batch` rows on a pool (n_slots, heads, dim_k, dim_v) of float32 states;
+ * slots as in salt_causal_conv_step. */
+typedef struct {
+  int32_t batch, heads, kv_heads, dim_k, dim_v, n_slots;
+  int32_t type;
+  float scale;
+  int64_t q_stride, k_stride, v_stride, out_stride;
+  const void *q, *k, *v;
+  const float *log_decay;
+  const int32_t *slots;
+  float *pool;
+  void *out;
+} salt_linear_attention_step_args;
+
+salt_status salt_linear_attention_step(const salt_linear_attention_step_args *args, void *stream);
+
+/* Gradient of salt_linear_attention for the gradient dout of out and dfinal (batch, heads, dim_k,
+ * dim_v; may be NULL) of final_state, from the forward's inputs.  With D[t] the gradient of S[t],
+ *   dq[t] = scale * S[t] dout[t];  D[t] = scale * q[t]^T dout[t] + exp(log_decay) D[t+1];
+ *   dk[t] = D[t] v[t];  dv[t] = k[t] D[t];  dinitial = exp(log_decay) D[0],
+ * dk and dv summed over the heads that share a key head.  dq, dk and dv hold `type` with
+ * contiguous (heads, dim); dinitial (float32) may be NULL.  log_decay is a constant of the head:
+ * it has no gradient here. */
+typedef struct {
+  int32_t batch, len, heads, kv_heads, dim_k, dim_v;
+  int32_t type;
+  float scale;
+  int64_t q_batch_stride, q_stride, k_batch_stride, k_stride, v_batch_stride, v_stride,
+      dout_batch_stride, dout_stride, dq_batch_stride, dq_stride, dk_batch_stride, dk_stride,
+      dv_batch_stride, dv_stride;
+  const void *q, *k, *v, *dout;
+  const float *log_decay;
+  const int32_t *n_real;
+  const float *initial_state, *dfinal;
+  void *dq, *dk, *dv;
+  float *dinitial;
+} salt_linear_attention_backward_args;
+
+salt_status salt_linear_attention_backward_workspace_size(
+    const salt_linear_attention_backward_args *args, size_t *bytes);
+salt_status salt_linear_attention_backward(const salt_linear_attention_backward_args *args,
+                                           void *workspace, size_t workspace_bytes, void *stream);
+
+/* An array of rows (rows, dim) of `type`, or its transpose, in 8 bits (e4m3) with float32 scales.
+ * The output is (rows, dim), or (dim, rows) with `transposed`; each SALT_Q8_GROUP neighbours of an
+ * output row share a scale, or with `blocks` each SALT_Q8_GROUP x SALT_Q8_GROUP block of the output
+ * does.  Scale and values are those of salt_rms_norm's 8-bit form: max|x| / 448 and the nearest e4m3
+ * of x / scale.  scale is (output rows, or blocks of them; ceil(output dim / SALT_Q8_GROUP)),
+ * contiguous; out_stride is that of the output's rows. */
+#define SALT_Q8_GROUP 128
+typedef struct {
+  int32_t rows, dim;
+  int32_t type, blocks, transposed, pad;
+  int64_t x_stride, out_stride;
+  const void *x;
+  void *out;
+  float *scale;
+} salt_quantize_q8_args;
+
+salt_status salt_quantize_q8(const salt_quantize_q8_args *args, void *stream);
+
+/* Product of two matrices in 8 bits (e4m3) with a float32 scale for every SALT_Q8_GROUP of the
+ * depth k:
+ *   out[m][j] = bias[j] + sum_i (x[m][i] x_scale[m][i / G]) (weight[j][i] w[j][i / G]).
+ * x is (rows, k) with x_scale (rows, ceil(k / G)), as salt_rms_norm and salt_quantize_q8 write
+ * them; weight is (n, k), and w[j] row j / G of weight_scale (ceil(n / G), ceil(k / G)) (blocks),
+ * or with `weight_rows` row j of weight_scale (n, ceil(k / G)).  out (rows, n) holds `type`, bias
+ * (n, may be NULL) `bias_type` (`type` or SALT_F32).  Products of a group are added up by the
+ * tensor cores in 32 bits, groups in float32.  Rows of x and weight that do not start on 16-byte
+ * boundaries (address or stride) are first copied, into the workspace. */
+typedef struct {
+  int32_t rows, n, k;
+  int32_t type, bias_type, weight_rows;
+  int64_t x_stride, weight_stride, out_stride;
+  const void *x;
+  const float *x_scale;
+  const void *weight;
+  const float *weight_scale;
+  const void *bias;
+  void *out;
+} salt_matmul_q8_args;
+
+salt_status salt_matmul_q8_workspace_size(const salt_matmul_q8_args *args, size_t *bytes);
+salt_status salt_matmul_q8(const salt_matmul_q8_args *args, void *workspace,
+                           size_t workspace_bytes, void *stream);
+
 /* ---------------------------------------------------------------- stream transfer
  * No reference counterpart (the reference's input lives in XLA buffers): copies a batch of event
  * streams from PINNED host memory to the device, moving each sample's row only up to

@@ -21,7 +21,8 @@ from .quant_run import (REFERENCE_FIELDS, QuantSplitOutput, check_quantized, qua
 # the sequence operators (sequence.py)
 _SEQUENCE = ("rms_norm", "rms_norm_q8", "rms_norm_backward", "causal_conv", "causal_conv_step",
              "causal_conv_backward", "selective_scan", "selective_scan_step",
-             "selective_scan_backward")
+             "selective_scan_backward", "linear_attention", "linear_attention_step",
+             "linear_attention_backward", "quantize_q8", "matmul_q8")
 
 
 def __getattr__(name):  # the CUDA-backed objects load the library lazily

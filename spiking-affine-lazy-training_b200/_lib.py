@@ -142,6 +142,39 @@ class SelectiveScanBackwardArgs(ctypes.Structure):
                        "dC dA dD ddelta_bias dinitial")
 
 
+class LinearAttentionArgs(ctypes.Structure):
+    _fields_ = _fields("batch len heads kv_heads dim_k dim_v type",
+                       "q_batch_stride q_stride k_batch_stride k_stride v_batch_stride v_stride "
+                       "out_batch_stride out_stride",
+                       "q k v log_decay n_real initial_state out final_state",
+                       (("scale", ctypes.c_float),))
+
+
+class LinearAttentionStepArgs(ctypes.Structure):
+    _fields_ = _fields("batch heads kv_heads dim_k dim_v n_slots type",
+                       "q_stride k_stride v_stride out_stride",
+                       "q k v log_decay slots pool out", (("scale", ctypes.c_float),))
+
+
+class LinearAttentionBackwardArgs(ctypes.Structure):
+    _fields_ = _fields("batch len heads kv_heads dim_k dim_v type",
+                       "q_batch_stride q_stride k_batch_stride k_stride v_batch_stride v_stride "
+                       "dout_batch_stride dout_stride dq_batch_stride dq_stride dk_batch_stride "
+                       "dk_stride dv_batch_stride dv_stride",
+                       "q k v dout log_decay n_real initial_state dfinal dq dk dv dinitial",
+                       (("scale", ctypes.c_float),))
+
+
+class QuantizeQ8Args(ctypes.Structure):
+    _fields_ = _fields("rows dim type blocks transposed pad", "x_stride out_stride",
+                       "x out scale")
+
+
+class MatmulQ8Args(ctypes.Structure):
+    _fields_ = _fields("rows n k type bias_type weight_rows", "x_stride weight_stride out_stride",
+                       "x x_scale weight weight_scale bias out")
+
+
 # every function of include/salt_b200.h: name -> (restype, argtypes)
 _SIGS = {
     "salt_conv_layer_workspace_size": (_i32, [_vp, _vp, _i32, _i32, _vp]),
@@ -191,6 +224,14 @@ _SIGS = {
     "salt_selective_scan_step": (_i32, [_vp, _vp]),
     "salt_selective_scan_backward_workspace_size": (_i32, [_vp, _vp]),
     "salt_selective_scan_backward": (_i32, [_vp, _vp, ctypes.c_size_t, _vp]),
+    "salt_linear_attention_workspace_size": (_i32, [_vp, _vp]),
+    "salt_linear_attention": (_i32, [_vp, _vp, ctypes.c_size_t, _vp]),
+    "salt_linear_attention_step": (_i32, [_vp, _vp]),
+    "salt_linear_attention_backward_workspace_size": (_i32, [_vp, _vp]),
+    "salt_linear_attention_backward": (_i32, [_vp, _vp, ctypes.c_size_t, _vp]),
+    "salt_quantize_q8": (_i32, [_vp, _vp]),
+    "salt_matmul_q8_workspace_size": (_i32, [_vp, _vp]),
+    "salt_matmul_q8": (_i32, [_vp, _vp, ctypes.c_size_t, _vp]),
     "salt_malloc": (_i32, [ctypes.c_size_t, _vp, _vp]),
     "salt_free": (_i32, [_vp, _vp]),
     "salt_host_alloc": (_i32, [ctypes.c_size_t, _vp]),

@@ -9,6 +9,7 @@ namespace {
 
 constexpr int32_t kMostLen = 1 << 30;
 constexpr int32_t kMostDim = 1 << 24;
+constexpr int32_t kMostHeads = 1 << 16;
 
 // Whether no two of rows * len runs of `dim` elements, at b * batch + t * token, share an element.
 bool apart(int64_t batch, int64_t token, int32_t rows, int32_t len, int32_t dim) {
@@ -272,6 +273,124 @@ Checks check(const salt_selective_scan_backward_args* a) {
   return c;
 }
 
+template <class A>
+void attention_common(Checks& c, const A* a) {
+  c.type(a->type);
+  c.need(a->batch >= 0, "batch is negative");
+  c.need(a->heads >= 1 && a->heads <= kMostHeads, "heads must lie in [1, 65536]");
+  c.need(a->kv_heads >= 1 && a->heads % (a->kv_heads < 1 ? 1 : a->kv_heads) == 0,
+         "kv_heads must divide heads");
+  c.need(a->dim_k >= 1 && a->dim_k <= 128 && a->dim_v >= 1 && a->dim_v <= 128,
+         "dim_k and dim_v must lie in [1, 128]");
+  // a row's head has a few blocks of its own
+  c.need((int64_t)a->batch * a->heads <= kMostDim, "batch * heads must not exceed 2^24");
+  c.need(a->scale - a->scale == 0.f, "scale must be finite");
+}
+
+template <class A>
+void attention_rows(Checks& c, const A* a) {
+  c.need(a->len >= 0 && a->len <= kMostLen, "len must lie in [0, 2^30]");
+  const bool used = a->batch > 0 && a->len > 0;
+  c.input(a->q, used, "q is NULL");
+  c.input(a->k, used, "k is NULL");
+  c.input(a->v, used, "v is NULL");
+  c.input(a->log_decay, a->batch > 0, "log_decay is NULL");  // rows without tokens load it, too
+  c.strides(a->q_batch_stride, a->q_stride, "a stride is negative");
+  c.strides(a->k_batch_stride, a->k_stride, "a stride is negative");
+  c.strides(a->v_batch_stride, a->v_stride, "a stride is negative");
+}
+
+Checks check(const salt_linear_attention_args* a) {
+  Checks c("salt_linear_attention");
+  c.need(a, "args is NULL");
+  if (!c.ok()) return c;
+  attention_common(c, a);
+  attention_rows(c, a);
+  c.input(a->out, a->batch > 0 && a->len > 0, "out is NULL");
+  c.written(a->out_batch_stride, a->out_stride, a->batch, a->len, a->heads * a->dim_v,
+            "out's strides let its rows overlap");
+  return c;
+}
+
+Checks check(const salt_linear_attention_step_args* a) {
+  Checks c("salt_linear_attention_step");
+  c.need(a, "args is NULL");
+  if (!c.ok()) return c;
+  attention_common(c, a);
+  c.need(a->n_slots >= 0, "n_slots is negative");
+  c.need(a->slots || a->batch <= a->n_slots, "without slots, batch must not exceed n_slots");
+  const bool used = a->batch > 0;
+  c.input(a->q, used, "q is NULL");
+  c.input(a->k, used, "k is NULL");
+  c.input(a->v, used, "v is NULL");
+  c.input(a->log_decay, used, "log_decay is NULL");
+  c.input(a->pool, used && a->n_slots > 0, "pool is NULL");
+  c.input(a->out, used, "out is NULL");
+  c.strides(a->q_stride, a->k_stride, "a stride is negative");
+  c.strides(a->v_stride, 0, "a stride is negative");
+  c.written(0, a->out_stride, 1, a->batch, a->heads * a->dim_v,
+            "out_stride must be at least heads * dim_v");
+  return c;
+}
+
+Checks check(const salt_linear_attention_backward_args* a) {
+  Checks c("salt_linear_attention_backward");
+  c.need(a, "args is NULL");
+  if (!c.ok()) return c;
+  attention_common(c, a);
+  attention_rows(c, a);
+  const bool used = a->batch > 0 && a->len > 0;
+  c.input(a->dout, used, "dout is NULL");
+  c.input(a->dq, used, "dq is NULL");
+  c.input(a->dk, used, "dk is NULL");
+  c.input(a->dv, used, "dv is NULL");
+  c.strides(a->dout_batch_stride, a->dout_stride, "a stride is negative");
+  const char* text = "a gradient's strides let its rows overlap";
+  c.written(a->dq_batch_stride, a->dq_stride, a->batch, a->len, a->heads * a->dim_k, text);
+  c.written(a->dk_batch_stride, a->dk_stride, a->batch, a->len, a->kv_heads * a->dim_k, text);
+  c.written(a->dv_batch_stride, a->dv_stride, a->batch, a->len, a->kv_heads * a->dim_v, text);
+  return c;
+}
+
+Checks check(const salt_quantize_q8_args* a) {
+  Checks c("salt_quantize_q8");
+  c.need(a, "args is NULL");
+  if (!c.ok()) return c;
+  c.type(a->type);
+  c.need(a->rows >= 0, "rows is negative");
+  c.need(a->dim >= 1 && a->dim <= kMostDim, "dim must lie in [1, 2^24]");
+  const bool used = a->rows > 0;
+  c.input(a->x, used, "x is NULL");
+  c.input(a->out, used, "out is NULL");
+  c.input(a->scale, used, "scale is NULL");
+  c.strides(a->x_stride, 0, "a stride is negative");
+  if (a->transposed)
+    c.written(0, a->out_stride, 1, a->dim, a->rows, "out_stride must be at least rows");
+  else
+    c.written(0, a->out_stride, 1, a->rows, a->dim, "out_stride must be at least dim");
+  return c;
+}
+
+Checks check(const salt_matmul_q8_args* a) {
+  Checks c("salt_matmul_q8");
+  c.need(a, "args is NULL");
+  if (!c.ok()) return c;
+  c.type(a->type);
+  c.wide(a->bias_type, a->type, "bias_type must be type or SALT_F32");
+  c.need(a->rows >= 0, "rows is negative");
+  c.need(a->n >= 1 && a->n <= kMostDim, "n must lie in [1, 2^24]");
+  c.need(a->k >= 1 && a->k <= kMostDim, "k must lie in [1, 2^24]");
+  const bool used = a->rows > 0;
+  c.input(a->x, used, "x is NULL");
+  c.input(a->x_scale, used, "x_scale is NULL");
+  c.input(a->weight, used, "weight is NULL");
+  c.input(a->weight_scale, used, "weight_scale is NULL");
+  c.input(a->out, used, "out is NULL");
+  c.strides(a->x_stride, a->weight_stride, "a stride is negative");
+  c.written(0, a->out_stride, 1, a->rows, a->n, "out_stride must be at least n");
+  return c;
+}
+
 }  // namespace
 }  // namespace salt
 
@@ -389,6 +508,79 @@ salt_status salt_selective_scan_backward(const salt_selective_scan_backward_args
   if (s) return s;
   int n = 0;
   const cudaError_t e = selective_scan_backward_launch(*args, workspace, (cudaStream_t)stream, &n);
+  return launched(e, n, c.who);
+}
+
+salt_status salt_linear_attention_workspace_size(const salt_linear_attention_args* args, size_t* bytes) {
+  const Checks c = check(args);
+  if (!c.ok()) return c.status();
+  if (!bytes) return host_fail(SALT_BAD_ARG, "bytes is NULL");
+  *bytes = linear_attention_bytes(*args);
+  return SALT_OK;
+}
+
+salt_status salt_linear_attention(const salt_linear_attention_args* args, void* workspace, size_t workspace_bytes,
+                        void* stream) {
+  const Checks c = check(args);
+  if (!c.ok()) return c.status();
+  const salt_status s = room(c.who, workspace, workspace_bytes, linear_attention_bytes(*args));
+  if (s) return s;
+  int n = 0;
+  const cudaError_t e = linear_attention_launch(*args, workspace, (cudaStream_t)stream, &n);
+  return launched(e, n, c.who);
+}
+
+salt_status salt_linear_attention_step(const salt_linear_attention_step_args* args, void* stream) {
+  const Checks c = check(args);
+  if (!c.ok()) return c.status();
+  int n = 0;
+  const cudaError_t e = linear_attention_step_launch(*args, (cudaStream_t)stream, &n);
+  return launched(e, n, c.who);
+}
+
+salt_status salt_linear_attention_backward_workspace_size(const salt_linear_attention_backward_args* args, size_t* bytes) {
+  const Checks c = check(args);
+  if (!c.ok()) return c.status();
+  if (!bytes) return host_fail(SALT_BAD_ARG, "bytes is NULL");
+  *bytes = linear_attention_backward_bytes(*args);
+  return SALT_OK;
+}
+
+salt_status salt_linear_attention_backward(const salt_linear_attention_backward_args* args, void* workspace, size_t workspace_bytes,
+                        void* stream) {
+  const Checks c = check(args);
+  if (!c.ok()) return c.status();
+  const salt_status s = room(c.who, workspace, workspace_bytes, linear_attention_backward_bytes(*args));
+  if (s) return s;
+  int n = 0;
+  const cudaError_t e = linear_attention_backward_launch(*args, workspace, (cudaStream_t)stream, &n);
+  return launched(e, n, c.who);
+}
+
+salt_status salt_quantize_q8(const salt_quantize_q8_args* args, void* stream) {
+  const Checks c = check(args);
+  if (!c.ok()) return c.status();
+  int n = 0;
+  const cudaError_t e = quantize_q8_launch(*args, (cudaStream_t)stream, &n);
+  return launched(e, n, c.who);
+}
+
+salt_status salt_matmul_q8_workspace_size(const salt_matmul_q8_args* args, size_t* bytes) {
+  const Checks c = check(args);
+  if (!c.ok()) return c.status();
+  if (!bytes) return host_fail(SALT_BAD_ARG, "bytes is NULL");
+  *bytes = matmul_q8_bytes(*args);
+  return SALT_OK;
+}
+
+salt_status salt_matmul_q8(const salt_matmul_q8_args* args, void* workspace, size_t workspace_bytes,
+                        void* stream) {
+  const Checks c = check(args);
+  if (!c.ok()) return c.status();
+  const salt_status s = room(c.who, workspace, workspace_bytes, matmul_q8_bytes(*args));
+  if (s) return s;
+  int n = 0;
+  const cudaError_t e = matmul_q8_launch(*args, workspace, (cudaStream_t)stream, &n);
   return launched(e, n, c.who);
 }
 

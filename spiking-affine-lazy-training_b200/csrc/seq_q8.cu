@@ -1,0 +1,248 @@
+// Quantisation to 8 bits with a scale for every 128 values, and the product of such matrices.
+#include "seq_q8.cuh"
+#include "sequence.cuh"
+
+namespace salt {
+namespace {
+
+constexpr int kGroup = SALT_Q8_GROUP;
+
+template <int H>
+__device__ __forceinline__ void to_e4m3(uint16_t (&q)[H], const f32x2 (&v)[H]) {
+#pragma unroll
+  for (int k = 0; k < H; ++k)
+    q[k] = __nv_cvt_float2_to_fp8x2(halves(v[k]), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ void store8(uint8_t* p, const uint16_t (&q)[4], int n, bool vec) {
+  if (vec && n >= 8) {
+    *reinterpret_cast<uint2*>(p) =
+        make_uint2(q[0] | (uint32_t)q[1] << 16, q[2] | (uint32_t)q[3] << 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) p[i] = (uint8_t)(q[i / 2] >> (i % 2 * 8));
+  }
+}
+
+// Rows by groups of 128: half a warp a group, 8 elements a lane.  Bound by memory: type + 1 bytes
+// an element.
+template <typename T>
+__global__ void __launch_bounds__(256) quantize_rows_kernel(salt_quantize_q8_args a, int groups,
+                                                            bool vec_in, bool vec_out) {
+  const int64_t n = (int64_t)a.rows * groups;
+  const int lane = threadIdx.x & 15;
+  const int64_t step = (int64_t)gridDim.x * 16;
+  // all lanes of a warp take the same number of turns
+  for (int64_t first = blockIdx.x * 16ll + (threadIdx.x >> 5) * 2; first < n; first += step) {
+    const int64_t i = first + (threadIdx.x >> 4 & 1);
+    const bool live = i < n;
+    const int64_t row = live ? i / groups : 0;
+    const int g = live ? (int)(i - row * groups) : 0, at = g * kGroup + lane * 8;
+    const int m = live ? a.dim - at : 0;
+    const Pack<T, 8> p =
+        load_pack<T, 8>(static_cast<const T*>(a.x) + row * a.x_stride + at, m, vec_in);
+    f32x2 v[4];
+    float most = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      v[k] = pair_of(p, 2 * k);
+      const float2 h = halves(v[k]);
+      most = fmaxf(most, fmaxf(fabsf(h.x), fabsf(h.y)));
+    }
+#pragma unroll
+    for (int o = 8; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    const E4m3Scale by(most);
+    if (live && lane == 0) a.scale[i] = by.scale;
+    by.divide(v);
+    uint16_t q[4];
+    to_e4m3(q, v);
+    if (m > 0) store8(static_cast<uint8_t*>(a.out) + row * a.out_stride + at, q, m, vec_out);
+  }
+}
+
+// Tiles of 128 x 128 for scales of whole blocks, for transposed outputs, or both.  A thread holds 8
+// neighbouring rows of 8 columns; a transposed tile goes through shared memory, where 8 values of a
+// column lie together and their place in the column's 16 is turned by the column's pack, so that
+// a half-warp's writes spread over all banks.
+template <typename T, bool BLOCKS, bool TRANSPOSED>
+__global__ void __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2)
+quantize_tile_kernel(salt_quantize_q8_args a, int tiles_x, bool vec_in, bool vec_out) {
+  __shared__ float red[8][kGroup];
+  __shared__ uint2 tile[TRANSPOSED ? kGroup * 16 : 1];
+  const int ty = blockIdx.x / tiles_x, tx = blockIdx.x - ty * tiles_x;
+  const int cp = threadIdx.x & 15, rg = threadIdx.x >> 4, warp = threadIdx.x >> 5;
+  const int row0 = ty * kGroup + rg * 8, col0 = tx * kGroup + cp * 8;
+  Pack<T, 8> p[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    p[i] = load_pack<T, 8>(static_cast<const T*>(a.x) + (int64_t)(row0 + i) * a.x_stride + col0,
+                           row0 + i < a.rows ? a.dim - col0 : 0, vec_in);
+  float most[8];  // of each column
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    most[j] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most[j] = fmaxf(most[j], fabsf(to_f32(p[i].v[j])));
+    most[j] = fmaxf(most[j], __shfl_xor_sync(0xffffffffu, most[j], 16));
+  }
+  if (BLOCKS) {
+#pragma unroll
+    for (int j = 1; j < 8; ++j) most[0] = fmaxf(most[0], most[j]);
+#pragma unroll
+    for (int o = 8; o; o >>= 1) most[0] = fmaxf(most[0], __shfl_xor_sync(0xffffffffu, most[0], o));
+    if ((threadIdx.x & 31) == 0) red[0][warp] = most[0];
+    __syncthreads();
+    for (int w = 0; w < 8; ++w) most[0] = fmaxf(most[0], red[0][w]);
+  } else {
+    if ((threadIdx.x & 16) == 0) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) red[warp][cp * 8 + j] = most[j];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      for (int w = 0; w < 8; ++w) most[j] = fmaxf(most[j], red[w][cp * 8 + j]);
+  }
+  const int up = (a.rows + kGroup - 1) / kGroup;
+  if (BLOCKS && threadIdx.x == 0)
+    a.scale[TRANSPOSED ? (int64_t)tx * up + ty : (int64_t)ty * tiles_x + tx] =
+        E4m3Scale(most[0]).scale;
+  if constexpr (!TRANSPOSED) {
+    const E4m3Scale by(most[0]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      f32x2 v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = pair_of(p[i], 2 * k);
+      by.divide(v);
+      uint16_t q[4];
+      to_e4m3(q, v);
+      if (row0 + i < a.rows && col0 < a.dim)
+        store8(static_cast<uint8_t*>(a.out) + (int64_t)(row0 + i) * a.out_stride + col0, q,
+               a.dim - col0, vec_out);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const E4m3Scale by(most[BLOCKS ? 0 : j]);
+      if (!BLOCKS && rg == 0 && col0 + j < a.dim) a.scale[(int64_t)(col0 + j) * up + ty] = by.scale;
+      f32x2 v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        v[k] = pair(to_f32(p[2 * k].v[j]), to_f32(p[2 * k + 1].v[j]));
+      by.divide(v);
+      uint16_t q[4];
+      to_e4m3(q, v);
+      tile[(cp * 8 + j) * 16 + (rg ^ cp)] =
+          make_uint2(q[0] | (uint32_t)q[1] << 16, q[2] | (uint32_t)q[3] << 16);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int c = i * 16 + rg;  // the tile's column, an output row; cp is its 8 values' place
+      const uint2 u = tile[c * 16 + (cp ^ (c >> 3))];
+      const uint16_t q[4] = {(uint16_t)u.x, (uint16_t)(u.x >> 16), (uint16_t)u.y,
+                             (uint16_t)(u.y >> 16)};
+      const int at = ty * kGroup + cp * 8, row = tx * kGroup + c;
+      if (row < a.dim && at < a.rows)
+        store8(static_cast<uint8_t*>(a.out) + (int64_t)row * a.out_stride + at, q, a.rows - at,
+               vec_out);
+    }
+  }
+}
+
+__device__ __forceinline__ float from_e4m3(uint8_t v) {
+  const __half_raw h = __nv_cvt_fp8_to_halfraw(v, __NV_E4M3);
+  return __half2float(__half(h));
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) matmul_q8_simple_kernel(salt_matmul_q8_args a, int tiles_n) {
+  __shared__ float xs[64][33], wsm[64][33];
+  const int64_t tm = blockIdx.x / tiles_n;
+  const int tn = blockIdx.x - tm * tiles_n;
+  const int64_t m0 = tm * 64;
+  const int n0 = tn * 64;
+  const int x = threadIdx.x & 15, y = threadIdx.x >> 4, groups = (a.k + kGroup - 1) / kGroup;
+  float acc[4][4] = {};
+  const uint8_t* px = static_cast<const uint8_t*>(a.x);
+  const uint8_t* pw = static_cast<const uint8_t*>(a.weight);
+  for (int g = 0; g < groups; ++g) {
+    float part[4][4] = {};
+    for (int k0 = g * kGroup; k0 < min((g + 1) * kGroup, a.k); k0 += 32) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < 64 * 32; i += 256) {
+        const int r = i >> 5, c = i & 31;
+        xs[r][c] = m0 + r < a.rows && k0 + c < a.k ? from_e4m3(px[(m0 + r) * a.x_stride + k0 + c]) : 0.f;
+        wsm[r][c] = n0 + r < a.n && k0 + c < a.k ? from_e4m3(pw[(int64_t)(n0 + r) * a.weight_stride + k0 + c]) : 0.f;
+      }
+      __syncthreads();
+      for (int c = 0; c < 32; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) part[i][j] += xs[y + 16 * i][c] * wsm[x + 16 * j][c];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t m = m0 + y + 16 * i;
+        const int n = n0 + x + 16 * j;
+        if (m < a.rows && n < a.n)
+          acc[i][j] += part[i][j] * (a.x_scale[m * groups + g] *
+                                     a.weight_scale[(int64_t)(a.weight_rows ? n : n / kGroup) * groups + g]);
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t m = m0 + y + 16 * i;
+      const int n = n0 + x + 16 * j;
+      if (m >= a.rows || n >= a.n) continue;
+      const float b = a.bias ? weight_at<T>(a.bias, n, a.bias_type == SALT_F32) : 0.f;
+      static_cast<T*>(a.out)[m * a.out_stride + n] = from_f32<T>(acc[i][j] + b);
+    }
+}
+
+}  // namespace
+
+cudaError_t quantize_q8_launch(const salt_quantize_q8_args& a, cudaStream_t st, int* launches) {
+  if (!a.rows) return cudaSuccess;
+  const int groups = (a.dim + kGroup - 1) / kGroup;
+  const size_t size = type_size(a.type);
+  const bool vec_in = pack_rows(a.x, 8, size, a.x_stride);
+  const bool vec_out = packed_rows(a.out, 8, 1, a.out_stride, 0);
+  if (!a.blocks && !a.transposed) {
+    const int64_t blocks = ((int64_t)a.rows * groups + 15) / 16;
+    SALT_WITH_TYPE(a.type, T,
+                   quantize_rows_kernel<T><<<(unsigned)std::min<int64_t>(blocks, 148 * 16), 256, 0,
+                                             st>>>(a, groups, vec_in, vec_out));
+  } else {
+    const int64_t up = (a.rows + (int64_t)kGroup - 1) / kGroup, tiles = up * groups;
+    if (tiles > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    SALT_WITH_TYPE(a.type, T, {
+      const auto kernel = !a.transposed ? quantize_tile_kernel<T, true, false>
+                          : a.blocks    ? quantize_tile_kernel<T, true, true>
+                                        : quantize_tile_kernel<T, false, true>;
+      kernel<<<(unsigned)tiles, 256, 0, st>>>(a, groups, vec_in, vec_out);
+    });
+  }
+  ++*launches;
+  return cudaGetLastError();
+}
+
+size_t matmul_q8_bytes(const salt_matmul_q8_args&) { return 0; }
+
+cudaError_t matmul_q8_launch(const salt_matmul_q8_args& a, void*, cudaStream_t st, int* launches) {
+  if (!a.rows) return cudaSuccess;
+  const int tiles_n = (a.n + 63) / 64;
+  const int64_t tiles = (int64_t)((a.rows + 63) / 64) * tiles_n;
+  if (tiles > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  SALT_WITH_TYPE(a.type, T, matmul_q8_simple_kernel<T><<<(unsigned)tiles, 256, 0, st>>>(a, tiles_n));
+  ++*launches;
+  return cudaGetLastError();
+}
+
+}  // namespace salt

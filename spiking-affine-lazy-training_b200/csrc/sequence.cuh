@@ -225,6 +225,18 @@ cudaError_t selective_scan_step_launch(const salt_selective_scan_step_args& a, c
 size_t selective_scan_backward_bytes(const salt_selective_scan_backward_args& a);
 cudaError_t selective_scan_backward_launch(const salt_selective_scan_backward_args& a, void* ws,
                                            cudaStream_t st, int* launches);
+size_t linear_attention_bytes(const salt_linear_attention_args& a);
+cudaError_t linear_attention_launch(const salt_linear_attention_args& a, void* ws, cudaStream_t st,
+                                    int* launches);
+cudaError_t linear_attention_step_launch(const salt_linear_attention_step_args& a, cudaStream_t st,
+                                         int* launches);
+size_t linear_attention_backward_bytes(const salt_linear_attention_backward_args& a);
+cudaError_t linear_attention_backward_launch(const salt_linear_attention_backward_args& a, void* ws,
+                                             cudaStream_t st, int* launches);
+cudaError_t quantize_q8_launch(const salt_quantize_q8_args& a, cudaStream_t st, int* launches);
+size_t matmul_q8_bytes(const salt_matmul_q8_args& a);
+cudaError_t matmul_q8_launch(const salt_matmul_q8_args& a, void* ws, cudaStream_t st,
+                             int* launches);
 
 // The second stage of every weight gradient: sums `parts` partial arrays of float32, part p at
 // in + p * n, in an order that their number alone decides.  A part holds up to three gradients of

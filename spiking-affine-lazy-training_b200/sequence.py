@@ -1,10 +1,12 @@
-"""Sequence operators: root-mean-square norm, short causal convolution, selective state space scan.
+"""Sequence operators: root-mean-square norm, short causal convolution, selective state space scan,
+linear attention with a decay for each head, and products of matrices in 8 bits.
 
 The dense, trained counterpart of the float layers' affine scan, for sequences of feature vectors
 (binned spike counts, tokens): ``h = exp(s A) h + s x B`` with a step ``s``, an input map ``B`` and
-a readout ``C`` that depend on the token.  Each operator runs over whole rows, for single tokens on
-a pool of states, and backward, as one call of the C ABI (include/salt_b200.h, "sequence operators")
-on the current stream; no CPU fallback.  No reference counterpart.
+a readout ``C`` that depend on the token, or ``S = l S + k^T v`` with a matrix for each head.  Each
+operator runs over whole rows, for single tokens on a pool of states, and backward, as one call of
+the C ABI (include/salt_b200.h, "sequence operators") on the current stream; no CPU fallback.  No
+reference counterpart.
 
 Arrays are `DeviceArray`s or any object of another library with ``data_ptr()``, ``shape``,
 ``dtype`` and ``stride()`` (in elements) that lives on the current device.  Activations are float32,
@@ -34,6 +36,7 @@ from .device import DeviceArray, _tls, bfloat16, empty, float8_e4m3
 
 CHECKPOINT = 16       # tokens between the scan's checkpoints (SALT_SCAN_CHECKPOINT)
 GROUPS_8BIT = (0, 32, 64, 128, 256)
+Q8_GROUP = 128        # values that share a scale in quantize_q8 and matmul_q8 (SALT_Q8_GROUP)
 _F32, _F16, _BF16, _I32, _E4M3 = range(5)
 _NUMPY = {_F32: np.dtype(np.float32), _F16: np.dtype(np.float16), _BF16: bfloat16,
           _I32: np.dtype(np.int32), _E4M3: float8_e4m3}
@@ -82,6 +85,23 @@ class ScanGradients(NamedTuple):
     dz: object = None
     ddelta_bias: object = None
     dinitial: object = None
+
+
+class AttentionOutput(NamedTuple):
+    out: object
+    final_state: object = None
+
+
+class AttentionGradients(NamedTuple):
+    dq: object
+    dk: object
+    dv: object
+    dinitial: object = None
+
+
+class QuantizedOutput(NamedTuple):
+    out: object
+    scale: object
 
 
 # ---------------------------------------------------------------- arguments
@@ -258,6 +278,11 @@ _pack_conv_backward = _packer(_lib.CausalConvBackwardArgs)
 _pack_scan = _packer(_lib.SelectiveScanArgs)
 _pack_scan_step = _packer(_lib.SelectiveScanStepArgs)
 _pack_scan_backward = _packer(_lib.SelectiveScanBackwardArgs)
+_pack_attention = _packer(_lib.LinearAttentionArgs)
+_pack_attention_step = _packer(_lib.LinearAttentionStepArgs)
+_pack_attention_backward = _packer(_lib.LinearAttentionBackwardArgs)
+_pack_quantize = _packer(_lib.QuantizeQ8Args)
+_pack_matmul = _packer(_lib.MatmulQ8Args)
 
 
 def _with_workspace(query, call, args: bytes) -> None:
@@ -553,3 +578,167 @@ def selective_scan_backward(dy, x, delta, A, B, C, *, checkpoints, D=None, z=Non
     _with_workspace(lib.salt_selective_scan_backward_workspace_size,
                     lib.salt_selective_scan_backward, args)
     return ScanGradients(dx, ddelta, dA, dB, dC, dD, dz, ddelta_bias, dinitial)
+
+
+# ---------------------------------------------------------------- linear attention
+
+def _heads(q, k, v, n: int) -> tuple:
+    """(type, q's shape, kv heads, dim_v) of arrays whose last two of n axes are (heads, dim)."""
+    t = _activation(q, "q")
+    shape = _axes(q, "q", n)
+    return t, shape, _axes(k, "k", n)[-2], _axes(v, "v", n)[-1]
+
+
+def linear_attention(q, k, v, log_decay, *, scale: float = 1.0, n_real=None, initial_state=None,
+                     out=None, final_state=None) -> AttentionOutput:
+    """With one decay ``l = exp(log_decay[h])`` for each head and a matrix as its state:
+
+        S[t] = l S[t-1] + k[t]^T v[t];   out[t] = scale q[t] S[t]
+
+    q: (batch, len, heads, dim_k), k: (batch, len, kv heads, dim_k), v: (batch, len, kv heads,
+    dim_v), head h reading key head ``h // (heads / kv heads)``; dim_k and dim_v 1 to 128, (heads,
+    dim) contiguous, any token and batch strides.  log_decay (heads) float32, at most 0.  n_real
+    (batch, int32) ends each row early.  initial_state and final_state: (batch, heads, dim_k,
+    dim_v) float32, may be one array."""
+    here = _here()
+    t, shape, kv, dim_v = _heads(q, k, v, 4)
+    batch, n, heads, dim_k = shape
+    keys, rows, ends = (batch, n, kv, dim_k), (batch, n, heads, dim_v), (batch, heads, dim_k, dim_v)
+    out, final_state = _made(out, rows, t), _wanted(final_state, ends, _F32)
+    pq, sq = _rows(here, q, "q", shape, t, 2)
+    pk, sk = _rows(here, k, "k", keys, t, 2)
+    pv, sv = _rows(here, v, "v", (batch, n, kv, dim_v), t, 2)
+    po, so = _rows(here, out, "out", rows, t, 2)
+    args = _pack_attention(
+        batch, n, heads, kv, dim_k, dim_v, t, scale, *sq, *sk, *sv, *so, pq, pk, pv,
+        _whole(here, log_decay, "log_decay", (heads,), _F32),
+        _whole(here, n_real, "n_real", (batch,), _I32),
+        _whole(here, initial_state, "initial_state", ends, _F32), po,
+        _whole(here, final_state, "final_state", ends, _F32))
+    lib = _lib.lib()
+    _with_workspace(lib.salt_linear_attention_workspace_size, lib.salt_linear_attention, args)
+    return AttentionOutput(out, final_state)
+
+
+def linear_attention_step(pool, q, k, v, log_decay, *, scale: float = 1.0, slots=None, out=None
+                          ) -> AttentionOutput:
+    """One token of `linear_attention` for each row, q (batch, heads, dim_k) and k, v (batch, kv
+    heads, dim_k or dim_v), on pool[slots[b]] of float32 states (n_slots, heads, dim_k, dim_v), in
+    place; slots as in `causal_conv_step`."""
+    here = _here()
+    t, shape, kv, dim_v = _heads(q, k, v, 3)
+    batch, heads, dim_k = shape
+    n_slots = _axes(pool, "pool", 4)[0]
+    rows = (batch, heads, dim_v)
+    out = _made(out, rows, t)
+    pq, (sq,) = _rows(here, q, "q", shape, t, 2)
+    pk, (sk,) = _rows(here, k, "k", (batch, kv, dim_k), t, 2)
+    pv, (sv,) = _rows(here, v, "v", (batch, kv, dim_v), t, 2)
+    po, (so,) = _rows(here, out, "out", rows, t, 2)
+    args = _pack_attention_step(
+        batch, heads, kv, dim_k, dim_v, n_slots, t, scale, sq, sk, sv, so, pq, pk, pv,
+        _whole(here, log_decay, "log_decay", (heads,), _F32),
+        _whole(here, slots, "slots", (batch,), _I32),
+        _whole(here, pool, "pool", (n_slots, heads, dim_k, dim_v), _F32), po)
+    _lib.check(_lib.lib().salt_linear_attention_step(args, _stream()))
+    return AttentionOutput(out, pool)
+
+
+def linear_attention_backward(dout, q, k, v, log_decay, *, scale: float = 1.0, n_real=None,
+                              initial_state=None, dfinal=None, dq=None, dk=None, dv=None,
+                              dinitial=None) -> AttentionGradients:
+    """Gradients of `linear_attention` for dout, the gradient of its out, and dfinal, that of its
+    final state, from the forward's arguments.  dq, dk and dv hold q's type, dk and dv summed over
+    the heads that share a key head; dinitial is float32 and optional.  The decay is a constant of
+    the head: it gets no gradient."""
+    here = _here()
+    t, shape, kv, dim_v = _heads(q, k, v, 4)
+    batch, n, heads, dim_k = shape
+    keys, values = (batch, n, kv, dim_k), (batch, n, kv, dim_v)
+    rows, ends = (batch, n, heads, dim_v), (batch, heads, dim_k, dim_v)
+    dq, dk, dv = _made(dq, shape, t), _made(dk, keys, t), _made(dv, values, t)
+    dinitial = _wanted(dinitial, ends, _F32)
+    pq, sq = _rows(here, q, "q", shape, t, 2)
+    pk, sk = _rows(here, k, "k", keys, t, 2)
+    pv, sv = _rows(here, v, "v", values, t, 2)
+    pdo, sdo = _rows(here, dout, "dout", rows, t, 2)
+    pdq, sdq = _rows(here, dq, "dq", shape, t, 2)
+    pdk, sdk = _rows(here, dk, "dk", keys, t, 2)
+    pdv, sdv = _rows(here, dv, "dv", values, t, 2)
+    args = _pack_attention_backward(
+        batch, n, heads, kv, dim_k, dim_v, t, scale, *sq, *sk, *sv, *sdo, *sdq, *sdk, *sdv, pq, pk,
+        pv, pdo, _whole(here, log_decay, "log_decay", (heads,), _F32),
+        _whole(here, n_real, "n_real", (batch,), _I32),
+        _whole(here, initial_state, "initial_state", ends, _F32),
+        _whole(here, dfinal, "dfinal", ends, _F32), pdq, pdk, pdv,
+        _whole(here, dinitial, "dinitial", ends, _F32))
+    lib = _lib.lib()
+    _with_workspace(lib.salt_linear_attention_backward_workspace_size,
+                    lib.salt_linear_attention_backward, args)
+    return AttentionGradients(dq, dk, dv, dinitial)
+
+
+# ---------------------------------------------------------------- products in 8 bits
+
+def _groups(n: int) -> int:
+    return -(-n // Q8_GROUP)
+
+
+def quantize_q8(x, *, blocks: bool = False, transposed: bool = False, out=None, scale=None
+                ) -> QuantizedOutput:
+    """x (..., dim), or the transpose of a matrix x, in 8 bits (`device.float8_e4m3`).  Every 128
+    neighbours of an output row share a float32 scale, or with blocks every 128 x 128 of an output
+    matrix do; ``out * scale`` is the value, scale and rounding as in `rms_norm_q8`.  scale is
+    (..., ceil(width / 128)) for rows of `width`, or (ceil(rows / 128), ceil(width / 128)) for
+    blocks.  The operands of `matmul_q8`: activations by rows, a weight by blocks; for its gradients
+    dy by rows with the weight by blocks, transposed (dx), and dy and x by rows, both transposed
+    (dweight)."""
+    here = _here()
+    t = _activation(x, "x")
+    shape = tuple(x.shape)
+    rows, dim = _row_count(shape, "x"), shape[-1]
+    to = shape
+    if blocks or transposed:
+        to = _axes(x, "x", 2)[::-1] if transposed else _axes(x, "x", 2)
+    parts = (_groups(to[0]) if blocks else to[0],) if blocks or transposed else to[:-1]
+    parts += (_groups(to[-1]),)
+    out, scale = _made(out, to, _E4M3), _made(scale, parts, _F32)
+    px, sx = _flat(here, x, "x", shape, t)
+    po, so = _flat(here, out, "out", to, _E4M3)
+    args = _pack_quantize(rows, dim, t, bool(blocks), bool(transposed), 0, sx, so, px, po,
+                          _whole(here, scale, "scale", parts, _F32))
+    _lib.check(_lib.lib().salt_quantize_q8(args, _stream()))
+    return QuantizedOutput(out, scale)
+
+
+def matmul_q8(x, x_scale, weight, weight_scale, *, bias=None, dtype=None, out=None):
+    """``x @ weight.T (+ bias)`` of 8-bit matrices x (..., k), weight (n, k) and their scales: a
+    float32 scale for every 128 values of x's rows, x_scale (..., ceil(k / 128)), as `rms_norm_q8`
+    and `quantize_q8` give them, and for every 128 x 128 block of the weight, weight_scale (ceil(n
+    / 128), ceil(k / 128)), or every 128 values of its rows, (n, ceil(k / 128)).  Returns out (...,
+    n) of out's type, else dtype, else bfloat16; bias (n) holds that type or float32.  Rows whose
+    address or stride is no multiple of 16 bytes cost a copy."""
+    here = _here()
+    for a, name in ((x, "x"), (weight, "weight")):
+        if not hasattr(a, "data_ptr"):
+            raise TypeError(f"{name}: needs a device array, got {type(a).__name__}")
+    shape = tuple(x.shape)
+    rows, depth = _row_count(shape, "x"), shape[-1]
+    n = _axes(weight, "weight", 2)[0]
+    to, groups = shape[:-1] + (n,), _groups(depth)
+    if out is None:
+        out = empty(to, bfloat16 if dtype is None else dtype)
+    t = _activation(out, "out")
+    by_rows = n > 1 and tuple(getattr(weight_scale, "shape", ())) == (n, groups)
+    parts = (n if by_rows else _groups(n), groups)
+    px, sx = _flat(here, x, "x", shape, _E4M3)
+    pw, (sw,) = _rows(here, weight, "weight", (n, depth), _E4M3)
+    po, so = _flat(here, out, "out", to, t)
+    pb, bt = _weight(here, bias, "bias", (n,), t)
+    args = _pack_matmul(
+        rows, n, depth, t, bt, by_rows, sx, sw, so, px,
+        _whole(here, x_scale, "x_scale", shape[:-1] + (groups,), _F32), pw,
+        _whole(here, weight_scale, "weight_scale", parts, _F32), pb, po)
+    lib = _lib.lib()
+    _with_workspace(lib.salt_matmul_q8_workspace_size, lib.salt_matmul_q8, args)
+    return out
