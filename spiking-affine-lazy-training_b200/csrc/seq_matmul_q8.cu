@@ -1,0 +1,451 @@
+// Product of two matrices in 8 bits with a float32 scale for every 128 values of the depth.
+#include <cooperative_groups.h>
+
+#include "sequence.cuh"
+#include "tc.cuh"
+
+namespace salt {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int kGroup = SALT_Q8_GROUP;
+constexpr int kTileA = 128;         // rows of one operand, the accumulators' lanes
+constexpr int kSums = 256;          // threads that scale and add up (8 warps)
+constexpr int kThreads = kSums + 64;  // and a warp each for the copies and the products
+constexpr int kMostSplit = 8;
+
+// Stages of both operands' tiles in flight.
+constexpr int stages(int bn) { return bn == 256 ? 4 : bn == 128 ? 6 : bn == 64 ? 8 : 9; }
+constexpr int stage_bytes(int bn) { return (kTileA + bn) * kGroup; }
+constexpr int shared_bytes(int bn) { return stages(bn) * stage_bytes(bn) + 1024; }
+
+struct Product {
+  int64_t rows_a, rows_b;
+  int tiles_a, tiles_b, groups, split;
+  int shift_a, shift_b;  // rows of a scale, as a power of two
+  const float *scale_a, *scale_b;
+  void* out;
+  int64_t out_stride;
+  const void* bias;
+  bool bias_f32, vec;
+};
+
+// out = sum over groups of scale_a scale_b (the group's product of e4m3 values).
+//
+// The tensor cores add up one group (128 x BN x 128, in 32 bits) into one of two buffers of tensor
+// memory; eight warps take it from there, times both scales, to their running sums in registers,
+// while the next group's product goes to the other buffer.
+//
+// SWAP = false: rows of x are the lanes, weight rows the columns, and a warp's columns share one scale
+// (blocks of 128).  SWAP = true: weight rows are the lanes, rows of x the columns, each with its own
+// scale, which goes through shared memory; a warp's stores are then neighbours in a row of out.
+template <int BN, bool SWAP, typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+matmul_q8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                 const Product p) {
+  constexpr int S = stages(BN), H = BN / 2, PIECE = H < 32 ? H : 32;
+  extern __shared__ uint8_t raw[];
+  uint8_t* tiles = raw + (1024 - tc::shared_at(raw) % 1024) % 1024;
+  __shared__ uint64_t full[S], empty[S], sum_full[2], sum_empty[2];
+  __shared__ uint32_t tmem_at;
+  __shared__ __align__(16) float scales[SWAP ? 2 : 1][SWAP ? BN : 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S; ++i) {
+      tc::barrier_init(&full[i], 1);
+      tc::barrier_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      tc::barrier_init(&sum_full[i], 1);
+      tc::barrier_init(&sum_empty[i], kSums / 32);
+    }
+    tc::barrier_init_fence();
+    tc::prefetch_map(&map_a);
+    tc::prefetch_map(&map_b);
+  }
+  constexpr uint32_t kColumns = 2 * BN < 32 ? 32 : 2 * BN;
+  if (warp == 9) tc::tmem_alloc(&tmem_at, kColumns);
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = tmem_at;
+  const int rank = p.split > 1 ? blockIdx.x % p.split : 0;
+  const int64_t worker = blockIdx.x / p.split, workers = gridDim.x / p.split;
+  const int64_t total = (int64_t)p.tiles_a * p.tiles_b;
+  const int g0 = (int)((int64_t)p.groups * rank / p.split),
+            g1 = (int)((int64_t)p.groups * (rank + 1) / p.split);
+  // bands of 16 tiles of a, so that blocks at work at the same time share both operands in L2
+  auto place = [&](int64_t t, int& ta, int& tb) {
+    const int64_t band = t / (16ll * p.tiles_b);
+    const int64_t in = t - band * 16ll * p.tiles_b;
+    const int high = (int)min((int64_t)16, p.tiles_a - band * 16);
+    tb = (int)(in / high);
+    ta = (int)(band * 16 + in - (int64_t)tb * high);
+  };
+  bool ok = true;
+
+  if (warp == 8) {
+    if (tc::one_lane()) {
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int64_t t = worker; ok && t < total; t += workers) {
+        int ta, tb;
+        place(t, ta, tb);
+        for (int g = g0; g < g1; ++g) {
+          if (!(ok = tc::barrier_wait(&empty[stage], phase ^ 1))) break;
+          uint8_t* a = tiles + stage * stage_bytes(BN);
+          tc::barrier_expect(&full[stage], stage_bytes(BN));
+          tc::load_box(a, &map_a, g * kGroup, ta * kTileA, &full[stage]);
+          tc::load_box(a + kTileA * kGroup, &map_b, g * kGroup, tb * BN, &full[stage]);
+          if (++stage == S) stage = 0, phase ^= 1;
+        }
+      }
+      // all copies have to land before the block may end
+      for (int i = 0; i < S; ++i) {
+        tc::barrier_wait(&empty[stage], phase ^ 1);
+        if (++stage == S) stage = 0, phase ^= 1;
+      }
+    }
+  } else if (warp == 9) {
+    if (tc::one_lane()) {
+      int stage = 0, buffer = 0;
+      uint32_t phase = 0, sum_phase = 0;
+      for (int64_t t = worker; ok && t < total; t += workers) {
+        for (int g = g0; g < g1; ++g) {
+          if (!(ok = tc::barrier_wait(&sum_empty[buffer], sum_phase ^ 1) &&
+                     tc::barrier_wait(&full[stage], phase)))
+            break;
+          tc::fence_after();
+          const uint8_t* at = tiles + stage * stage_bytes(BN);
+          const uint64_t a = tc::operand(at, 1024), b = tc::operand(at + kTileA * kGroup, 1024);
+#pragma unroll
+          for (int k = 0; k < kGroup; k += 32)
+            tc::product_e4m3(tmem + buffer * BN, tc::further(a, k), tc::further(b, k),
+                             tc::shape(kTileA, BN, 0), k > 0);
+          tc::products_done(&empty[stage]);
+          tc::products_done(&sum_full[buffer]);
+          if (++stage == S) stage = 0, phase ^= 1;
+          if (++buffer == 2) buffer = 0, sum_phase ^= 1;
+        }
+      }
+    }
+  } else {
+    const int quarter = warp & 3, half = warp >> 2;
+    const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16) + half * H;
+    int buffer = 0;
+    uint32_t phase = 0;
+    for (int64_t t = worker; ok && t < total; t += workers) {
+      int ta, tb;
+      place(t, ta, tb);
+      const int64_t row = (int64_t)ta * kTileA + quarter * 32 + lane, col0 = (int64_t)tb * BN + half * H;
+      const float* sa = p.scale_a + (min(row, p.rows_a - 1) >> p.shift_a) * p.groups;
+      // of the warp's columns, or (SWAP) of the column that this thread fetches
+      const int64_t of = SWAP ? (int64_t)tb * BN + (int)threadIdx.x % BN : col0;
+      const float* sb = p.scale_b + (min(of, p.rows_b - 1) >> p.shift_b) * p.groups;
+      f32x2 sum[H / 2];
+#pragma unroll
+      for (int i = 0; i < H / 2; ++i) sum[i] = 0;
+      float next_a = g0 < g1 ? sa[g0] : 0.f, next_b = g0 < g1 ? sb[g0] : 0.f;
+      for (int g = g0; g < g1; ++g) {
+        const float now_a = next_a, now_b = next_b;
+        if (g + 1 < g1) next_a = sa[g + 1], next_b = sb[g + 1];
+        if (SWAP) {
+          if (threadIdx.x < BN) scales[g & 1][threadIdx.x] = now_b;
+          tc::named_sync(1, kSums);
+        }
+        if (!(ok = tc::barrier_wait(&sum_full[buffer], phase))) break;
+        tc::fence_after();
+#pragma unroll
+        for (int c = 0; c < H; c += PIECE) {
+          uint32_t r[PIECE];
+          tc::tmem_load<PIECE>(r, mine + buffer * BN + c);
+          tc::loads_done();
+          if (c + PIECE == H) {
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) tc::barrier_arrive(&sum_empty[buffer]);
+          }
+          const f32x2 by = both(SWAP ? now_a : now_a * now_b);
+#pragma unroll
+          for (int i = 0; i < PIECE; i += 4) {
+            f32x2 s0 = by, s1 = by;
+            if (SWAP) {
+              const float4 v = *reinterpret_cast<const float4*>(&scales[g & 1][half * H + c + i]);
+              s0 = mul2(by, pair(v.x, v.y)), s1 = mul2(by, pair(v.z, v.w));
+            }
+            f32x2* to = &sum[(c + i) / 2];
+            to[0] = fma2(pair(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), s0, to[0]);
+            to[1] = fma2(pair(__uint_as_float(r[i + 2]), __uint_as_float(r[i + 3])), s1, to[1]);
+          }
+        }
+        if (++buffer == 2) buffer = 0, phase ^= 1;
+      }
+      if (!ok) {  // a result that nobody can take for one
+#pragma unroll
+        for (int i = 0; i < H / 2; ++i) sum[i] = both(__int_as_float(0x7fffffff));
+      }
+      if (p.split > 1) {
+        // every block's part of the tile, [column][lane], in its own shared memory (all of this
+        // block's copies and products are done: their sums are here)
+        float* part = reinterpret_cast<float*>(tiles);
+#pragma unroll
+        for (int i = 0; i < H / 2; ++i) {
+          const float2 v = halves(sum[i]);
+          part[(half * H + 2 * i) * kTileA + quarter * 32 + lane] = v.x;
+          part[(half * H + 2 * i + 1) * kTileA + quarter * 32 + lane] = v.y;
+        }
+        break;  // joined below
+      }
+      if constexpr (SWAP) {
+        if (row < p.rows_a) {
+          const float b = p.bias ? weight_at<T>(p.bias, row, p.bias_f32) : 0.f;
+          T* out = static_cast<T*>(p.out) + col0 * p.out_stride + row;
+          const int most = (int)min((int64_t)H, p.rows_b - col0);
+#pragma unroll
+          for (int i = 0; i < H / 2; ++i) {
+            const float2 v = halves(sum[i]);
+            if (2 * i < most) out[2 * i * p.out_stride] = from_f32<T>(v.x + b);
+            if (2 * i + 1 < most) out[(2 * i + 1) * p.out_stride] = from_f32<T>(v.y + b);
+          }
+        }
+      } else {
+        if (row < p.rows_a) {
+          T* out = static_cast<T*>(p.out) + row * p.out_stride + col0;
+          const int most = (int)min((int64_t)H, p.rows_b - col0);
+#pragma unroll
+          for (int i = 0; i < H; i += 8) {
+            float f[8];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float2 v = halves(sum[i / 2 + k]);
+              f[2 * k] = v.x, f[2 * k + 1] = v.y;
+            }
+            if (i < most) {
+              if (p.bias) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                  if (i + k < most) f[k] += weight_at<T>(p.bias, col0 + i + k, p.bias_f32);
+              }
+              store_pack<T, 8>(out + i, f, most - i, p.vec);
+            }
+          }
+        }
+      }
+    }
+  }
+  __syncwarp();  // the copies' and the products' warps went apart
+  if (p.split > 1) {
+    // the blocks of a cluster hold parts of one tile: each adds up its share of the columns, in the
+    // blocks' order
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    int ta, tb;
+    place(worker, ta, tb);
+    const int r = threadIdx.x & (kTileA - 1);
+    const int64_t row = (int64_t)ta * kTileA + r;
+    if (threadIdx.x < kSums && row < p.rows_a) {
+      const float* parts[kMostSplit];
+#pragma unroll
+      for (int i = 0; i < kMostSplit; ++i)
+        parts[i] = cluster.map_shared_rank(reinterpret_cast<float*>(tiles), i < p.split ? i : 0);
+      const float b = SWAP && p.bias ? weight_at<T>(p.bias, row, p.bias_f32) : 0.f;
+      for (int c = rank * 2 + (threadIdx.x >> 7); c < BN; c += 2 * p.split) {
+        const int64_t col = (int64_t)tb * BN + c;
+        if (col >= p.rows_b) break;
+        float v[kMostSplit], s = 0.f;
+#pragma unroll
+        for (int i = 0; i < kMostSplit; ++i) v[i] = i < p.split ? parts[i][c * kTileA + r] : 0.f;
+#pragma unroll
+        for (int i = 0; i < kMostSplit; ++i) s += v[i];
+        static_cast<T*>(p.out)[col * p.out_stride + row] = from_f32<T>(s + b);
+      }
+    }
+    cluster.sync();  // the parts are read by others
+  }
+  tc::fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc::fence_after();
+    tc::tmem_free(tmem, kColumns);
+  }
+}
+
+// Rows on boundaries of 16 bytes: what a tensor copy needs, for operands that do not lie so.
+__global__ void __launch_bounds__(256) align_rows_kernel(const uint8_t* from, int64_t stride,
+                                                         int64_t rows, int k, uint4* to, int units) {
+  const int64_t n = rows * units;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+    const int64_t row = i / units;
+    const int at = (int)(i - row * units) * 16;
+    const uint8_t* p = from + row * stride + at;
+    uint32_t w[4] = {};
+    const uintptr_t off = reinterpret_cast<uintptr_t>(p) & 3;
+    if (at >= 4 && at + 20 <= k) {
+      // whole words around the 16 bytes: all of them lie within this row
+      const uint32_t* q = reinterpret_cast<const uint32_t*>(p - off);
+      uint32_t v[5];
+#pragma unroll
+      for (int j = 0; j < 5; ++j) v[j] = q[j];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = __funnelshift_r(v[j], v[j + 1], (unsigned)off * 8);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (at + j < k) w[j / 4] |= (uint32_t)p[j] << (j % 4 * 8);
+    }
+    to[i] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// ---------------------------------------------------------------- host
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                 const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encoder() {
+  static const EncodeTiled f = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault,
+                                         &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<EncodeTiled>(p);
+  }();
+  return f;
+}
+
+// Boxes of 128 bytes x `high` rows; what lies past k or the rows reads as zero.
+bool tile_map(CUtensorMap* map, const void* p, int64_t rows, int64_t k, int64_t stride, int high) {
+  const EncodeTiled f = encoder();
+  if (!f) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)stride};
+  const cuuint32_t box[2] = {kGroup, (cuuint32_t)high}, unit[2] = {1, 1};
+  return f(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dims, strides, box, unit,
+           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+           CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+constexpr int64_t kMostStride = 1ll << 39;  // a tensor map's strides lie under 2^40
+int64_t aligned_stride(int64_t k) { return (k + 15) / 16 * 16; }
+bool tiled(const void* p, int64_t rows, int64_t stride, int64_t k) {
+  return aligned16(p) && (rows == 1 || (stride % 16 == 0 && stride >= k && stride < kMostStride));
+}
+size_t copy_bytes(const void* p, int64_t rows, int64_t stride, int64_t k) {
+  return tiled(p, rows, stride, k) ? 0 : ((size_t)rows * aligned_stride(k) + 255) / 256 * 256;
+}
+
+struct Operand {
+  const void* p;
+  int64_t rows, stride;
+};
+cudaError_t prepare(Operand& o, int64_t k, uint8_t*& ws, cudaStream_t st, int* launches) {
+  if (tiled(o.p, o.rows, o.stride, k)) {
+    if (o.rows == 1) o.stride = aligned_stride(k);
+    return cudaSuccess;
+  }
+  const int units = (int)(aligned_stride(k) / 16);
+  const int64_t blocks = (o.rows * units + 255) / 256;
+  align_rows_kernel<<<(unsigned)std::min<int64_t>(blocks, 148 * 16), 256, 0, st>>>(
+      static_cast<const uint8_t*>(o.p), o.stride, o.rows, (int)k, reinterpret_cast<uint4*>(ws),
+      units);
+  ++*launches;
+  const size_t bytes = copy_bytes(o.p, o.rows, o.stride, k);
+  o.p = ws;
+  o.stride = aligned_stride(k);
+  ws += bytes;
+  return cudaGetLastError();
+}
+
+template <int BN, bool SWAP, typename T>
+cudaError_t launch(Operand a, Operand b, int64_t k, Product p, cudaStream_t st, int* launches) {
+  p.tiles_a = (int)((p.rows_a + kTileA - 1) / kTileA);
+  p.tiles_b = (int)((p.rows_b + BN - 1) / BN);
+  CUtensorMap map_a, map_b;
+  if (!tile_map(&map_a, a.p, a.rows, k, a.stride, kTileA) ||
+      !tile_map(&map_b, b.p, b.rows, k, b.stride, BN))
+    return cudaErrorInvalidValue;
+  const auto kernel = matmul_q8_kernel<BN, SWAP, T>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       shared_bytes(BN));
+  if (e != cudaSuccess) return e;
+  const int64_t total = (int64_t)p.tiles_a * p.tiles_b;
+  cudaLaunchConfig_t c = {};
+  c.gridDim = dim3((unsigned)(p.split > 1 ? total * p.split : std::min<int64_t>(total, 148)));
+  c.blockDim = dim3(kThreads);
+  c.dynamicSmemBytes = shared_bytes(BN);
+  c.stream = st;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = p.split;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  c.attrs = &attr;
+  c.numAttrs = p.split > 1;
+  ++*launches;
+  return cudaLaunchKernelEx(&c, kernel, map_a, map_b, (const Product)p);
+}
+
+template <typename T>
+cudaError_t run(const salt_matmul_q8_args& a, const Operand& x, const Operand& w, cudaStream_t st,
+                int* launches) {
+  Product p = {};
+  p.groups = (a.k + kGroup - 1) / kGroup;
+  p.split = 1;
+  p.out = a.out;
+  p.out_stride = a.out_stride;
+  p.bias = a.bias;
+  p.bias_f32 = a.bias_type == SALT_F32;
+  const int shift_w = a.weight_rows ? 0 : 7;
+  const int64_t tiles_w = (a.n + kTileA - 1) / kTileA;
+  if (!a.weight_rows && a.rows > 128) {
+    p.rows_a = a.rows, p.rows_b = a.n;
+    p.scale_a = a.x_scale, p.scale_b = a.weight_scale;
+    p.shift_a = 0, p.shift_b = shift_w;
+    p.vec = pack_rows(a.out, 8, sizeof(T), a.out_stride);
+    const int64_t wide = ((a.rows + 127ll) / 128) * ((a.n + 255ll) / 256);
+    if (wide >= 148) return launch<256, false, T>(x, w, a.k, p, st, launches);
+    return launch<128, false, T>(x, w, a.k, p, st, launches);
+  }
+  p.rows_a = a.n, p.rows_b = a.rows;
+  p.scale_a = a.weight_scale, p.scale_b = a.x_scale;
+  p.shift_a = shift_w, p.shift_b = 0;
+  // few tiles: blocks share the depth of each
+  auto split = [&](int bn) {
+    const int64_t tiles = tiles_w * ((a.rows + bn - 1) / bn);
+    int s = 1;
+    while (s < kMostSplit && tiles * s * 2 <= 148 && p.groups >= s * 4) s *= 2;
+    return s;
+  };
+  if (a.rows <= 16) return p.split = split(16), launch<16, true, T>(w, x, a.k, p, st, launches);
+  if (a.rows <= 32) return p.split = split(32), launch<32, true, T>(w, x, a.k, p, st, launches);
+  if (a.rows <= 64) return p.split = split(64), launch<64, true, T>(w, x, a.k, p, st, launches);
+  if (tiles_w * ((a.rows + 255ll) / 256) < 148)
+    return p.split = split(128), launch<128, true, T>(w, x, a.k, p, st, launches);
+  return launch<256, true, T>(w, x, a.k, p, st, launches);
+}
+
+}  // namespace
+
+size_t matmul_q8_bytes(const salt_matmul_q8_args& a) {
+  if (!a.rows) return 0;
+  return copy_bytes(a.x, a.rows, a.x_stride, a.k) + copy_bytes(a.weight, a.n, a.weight_stride, a.k);
+}
+
+cudaError_t matmul_q8_launch(const salt_matmul_q8_args& a, void* ws, cudaStream_t st,
+                             int* launches) {
+  if (!a.rows) return cudaSuccess;
+  uint8_t* room = static_cast<uint8_t*>(ws);
+  Operand x{a.x, a.rows, a.x_stride}, w{a.weight, a.n, a.weight_stride};
+  cudaError_t e = prepare(x, a.k, room, st, launches);
+  if (e == cudaSuccess) e = prepare(w, a.k, room, st, launches);
+  if (e != cudaSuccess) return e;
+  SALT_WITH_TYPE(a.type, T, e = run<T>(a, x, w, st, launches));
+  return e;
+}
+
+}  // namespace salt

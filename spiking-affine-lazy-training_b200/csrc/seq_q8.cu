@@ -1,4 +1,4 @@
-// Quantisation to 8 bits with a scale for every 128 values, and the product of such matrices.
+// Quantisation to 8 bits with a scale for every 128 values.
 #include "seq_q8.cuh"
 #include "sequence.cuh"
 
@@ -151,61 +151,6 @@ quantize_tile_kernel(salt_quantize_q8_args a, int tiles_x, bool vec_in, bool vec
   }
 }
 
-__device__ __forceinline__ float from_e4m3(uint8_t v) {
-  const __half_raw h = __nv_cvt_fp8_to_halfraw(v, __NV_E4M3);
-  return __half2float(__half(h));
-}
-
-template <typename T>
-__global__ void __launch_bounds__(256) matmul_q8_simple_kernel(salt_matmul_q8_args a, int tiles_n) {
-  __shared__ float xs[64][33], wsm[64][33];
-  const int64_t tm = blockIdx.x / tiles_n;
-  const int tn = blockIdx.x - tm * tiles_n;
-  const int64_t m0 = tm * 64;
-  const int n0 = tn * 64;
-  const int x = threadIdx.x & 15, y = threadIdx.x >> 4, groups = (a.k + kGroup - 1) / kGroup;
-  float acc[4][4] = {};
-  const uint8_t* px = static_cast<const uint8_t*>(a.x);
-  const uint8_t* pw = static_cast<const uint8_t*>(a.weight);
-  for (int g = 0; g < groups; ++g) {
-    float part[4][4] = {};
-    for (int k0 = g * kGroup; k0 < min((g + 1) * kGroup, a.k); k0 += 32) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < 64 * 32; i += 256) {
-        const int r = i >> 5, c = i & 31;
-        xs[r][c] = m0 + r < a.rows && k0 + c < a.k ? from_e4m3(px[(m0 + r) * a.x_stride + k0 + c]) : 0.f;
-        wsm[r][c] = n0 + r < a.n && k0 + c < a.k ? from_e4m3(pw[(int64_t)(n0 + r) * a.weight_stride + k0 + c]) : 0.f;
-      }
-      __syncthreads();
-      for (int c = 0; c < 32; ++c)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) part[i][j] += xs[y + 16 * i][c] * wsm[x + 16 * j][c];
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t m = m0 + y + 16 * i;
-        const int n = n0 + x + 16 * j;
-        if (m < a.rows && n < a.n)
-          acc[i][j] += part[i][j] * (a.x_scale[m * groups + g] *
-                                     a.weight_scale[(int64_t)(a.weight_rows ? n : n / kGroup) * groups + g]);
-      }
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t m = m0 + y + 16 * i;
-      const int n = n0 + x + 16 * j;
-      if (m >= a.rows || n >= a.n) continue;
-      const float b = a.bias ? weight_at<T>(a.bias, n, a.bias_type == SALT_F32) : 0.f;
-      static_cast<T*>(a.out)[m * a.out_stride + n] = from_f32<T>(acc[i][j] + b);
-    }
-}
-
 }  // namespace
 
 cudaError_t quantize_q8_launch(const salt_quantize_q8_args& a, cudaStream_t st, int* launches) {
@@ -229,18 +174,6 @@ cudaError_t quantize_q8_launch(const salt_quantize_q8_args& a, cudaStream_t st, 
       kernel<<<(unsigned)tiles, 256, 0, st>>>(a, groups, vec_in, vec_out);
     });
   }
-  ++*launches;
-  return cudaGetLastError();
-}
-
-size_t matmul_q8_bytes(const salt_matmul_q8_args&) { return 0; }
-
-cudaError_t matmul_q8_launch(const salt_matmul_q8_args& a, void*, cudaStream_t st, int* launches) {
-  if (!a.rows) return cudaSuccess;
-  const int tiles_n = (a.n + 63) / 64;
-  const int64_t tiles = (int64_t)((a.rows + 63) / 64) * tiles_n;
-  if (tiles > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  SALT_WITH_TYPE(a.type, T, matmul_q8_simple_kernel<T><<<(unsigned)tiles, 256, 0, st>>>(a, tiles_n));
   ++*launches;
   return cudaGetLastError();
 }

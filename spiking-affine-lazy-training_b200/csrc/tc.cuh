@@ -1,0 +1,178 @@
+// Tensor cores of sm_100a (tcgen05, accumulators in tensor memory), tensor copies (TMA) and the
+// barriers between them, as the sequence operators' products use them.
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace salt::tc {
+
+__device__ __forceinline__ uint32_t shared_at(const void* p) {
+  return (uint32_t)__cvta_generic_to_shared(p);
+}
+
+// ---------------------------------------------------------------- barriers in shared memory
+
+__device__ __forceinline__ void barrier_init(uint64_t* b, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(shared_at(b)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void barrier_init_fence() {
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+}
+__device__ __forceinline__ void barrier_arrive(uint64_t* b) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(shared_at(b)) : "memory");
+}
+__device__ __forceinline__ void barrier_expect(uint64_t* b, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(shared_at(b)),
+               "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ bool barrier_try(uint64_t* b, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(done)
+      : "r"(shared_at(b)), "r"(parity)
+      : "memory");
+  return done;
+}
+// Waits for the barrier's phase of that parity to end; gives up (false) after some seconds, which
+// only a fault elsewhere can bring about.
+constexpr long long kWaitCycles = 4ll << 30;
+__device__ __forceinline__ bool barrier_wait(uint64_t* b, uint32_t parity) {
+  if (barrier_try(b, parity)) return true;
+  const long long since = clock64();
+  while (!barrier_try(b, parity))
+    if (clock64() - since > kWaitCycles) return false;
+  return true;
+}
+// Threads of part of a block.
+__device__ __forceinline__ void named_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+// ---------------------------------------------------------------- tensor copies
+
+// Box (inner, outer) from column x (in elements; its bytes a multiple of 16) and row y.
+__device__ __forceinline__ void load_box(void* to, const CUtensorMap* map, int x, int y,
+                                         uint64_t* barrier) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+      "%3}], [%4];" ::"r"(shared_at(to)),
+      "l"(map), "r"(x), "r"(y), "r"(shared_at(barrier))
+      : "memory");
+}
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+
+// ---------------------------------------------------------------- tensor memory
+
+// By one whole warp; `columns` a power of two, 32 to 512.
+__device__ __forceinline__ void tmem_alloc(uint32_t* at, uint32_t columns) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                   shared_at(at)),
+               "r"(columns)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+__device__ __forceinline__ void tmem_free(uint32_t at, uint32_t columns) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(columns));
+}
+__device__ __forceinline__ void fence_before() {
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void fence_after() {
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+// Shared memory that threads wrote, for the tensor cores to read.
+__device__ __forceinline__ void fence_shared() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+__device__ __forceinline__ void loads_done() {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+// N columns of the warp's 32 rows: a register each.
+template <int N>
+__device__ __forceinline__ void tmem_load(uint32_t (&r)[N], uint32_t at) {
+  static_assert(N == 8 || N == 16 || N == 32, "columns of one load");
+  if constexpr (N == 8) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
+                   "=r"(r[6]), "=r"(r[7])
+                 : "r"(at));
+  } else if constexpr (N == 16) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15])
+        : "r"(at));
+  } else {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
+        "%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+          "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+          "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(at));
+  }
+}
+
+// ---------------------------------------------------------------- products
+
+// An operand in shared memory in rows of 128 bytes, swizzled by 128 bytes (the 16-byte unit of row r
+// at place unit ^ (r & 7)), 1024-byte aligned.  Along its depth (`step` bytes between groups of 8
+// rows, of the operand's other axis), or, for 16-bit types, across it (rows are the depth, `step`
+// between groups of 8, `panel` bytes between panels of 64 elements of the other axis).
+__device__ __forceinline__ uint64_t operand(const void* p, uint32_t step, uint32_t panel = 16) {
+  return (uint64_t)((shared_at(p) & 0x3ffff) >> 4) | (uint64_t)(panel >> 4) << 16 |
+         (uint64_t)(step >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// The descriptor of an operand `bytes` further on.
+__device__ __forceinline__ uint64_t further(uint64_t d, uint32_t bytes) { return d + (bytes >> 4); }
+
+// Shape and types of a product with 32-bit sums: M x N; formats 0 e4m3 or float16, 1 bfloat16;
+// `across` for operands whose rows are the depth.
+__host__ __device__ constexpr uint32_t shape(int m, int n, int format, bool a_across = false,
+                                             bool b_across = false) {
+  return 1u << 4 | (uint32_t)format << 7 | (uint32_t)format << 10 | (uint32_t)a_across << 15 |
+         (uint32_t)b_across << 16 | (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24;
+}
+// d (+)= a b over a depth of 32 bytes, by one thread.
+__device__ __forceinline__ void product_e4m3(uint32_t d, uint64_t a, uint64_t b, uint32_t shape,
+                                             bool add) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+      "l"(a), "l"(b), "r"(shape), "r"((uint32_t)add)
+      : "memory");
+}
+__device__ __forceinline__ void product_16(uint32_t d, uint64_t a, uint64_t b, uint32_t shape,
+                                           bool add) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+      "l"(a), "l"(b), "r"(shape), "r"((uint32_t)add)
+      : "memory");
+}
+// The barrier's arrival once all products that this thread issued are done.
+__device__ __forceinline__ void products_done(uint64_t* barrier) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                   shared_at(barrier))
+               : "memory");
+}
+__device__ __forceinline__ bool one_lane() {
+  uint32_t is;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}"
+               : "=r"(is));
+  return is;
+}
+
+}  // namespace salt::tc
