@@ -380,6 +380,9 @@ Checks check(const salt_matmul_q8_args* a) {
   c.need(a->rows >= 0, "rows is negative");
   c.need(a->n >= 1 && a->n <= kMostDim, "n must lie in [1, 2^24]");
   c.need(a->k >= 1 && a->k <= kMostDim, "k must lie in [1, 2^24]");
+  // tiles are counted in 32 bits
+  c.need(((int64_t)a->rows / 128 + 1) * (a->n / 128 + 1) <= 1 << 30,
+         "rows * n is too large for one launch");
   const bool used = a->rows > 0;
   c.input(a->x, used, "x is NULL");
   c.input(a->x_scale, used, "x_scale is NULL");

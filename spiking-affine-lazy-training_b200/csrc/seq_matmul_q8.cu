@@ -10,15 +10,21 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kGroup = SALT_Q8_GROUP;
-constexpr int kTileA = 128;         // rows of one operand, the accumulators' lanes
-constexpr int kSums = 256;          // threads that scale and add up (8 warps)
-constexpr int kThreads = kSums + 64;  // and a warp each for the copies and the products
+constexpr int kTileA = 128;           // rows of one operand in a block, the accumulators' lanes
+constexpr int kSums = 256;             // threads that scale and add up: 8 warps
+constexpr int kThreads = kSums + 128;  // behind them a warp for the copies, one for the products and two
+                                       // for the scales
 constexpr int kMostSplit = 8;
+constexpr int kRing = 8;  // groups whose scales are in flight
 
 // Stages of both operands' tiles in flight.
-constexpr int stages(int bn) { return bn == 256 ? 4 : bn == 128 ? 6 : bn == 64 ? 8 : 9; }
+constexpr int stages(int bn, bool swap) {
+  return bn == 256 ? (swap ? 4 : 3) : bn == 128 ? (swap ? 6 : 5) : bn == 64 ? 8 : 9;
+}
 constexpr int stage_bytes(int bn) { return (kTileA + bn) * kGroup; }
-constexpr int shared_bytes(int bn) { return stages(bn) * stage_bytes(bn) + 1024; }
+constexpr int shared_bytes(int bn, bool swap) {
+  return stages(bn, swap) * stage_bytes(bn) + (swap ? 0 : kSums / 32 * 4096) + 1024;
+}
 
 struct Product {
   int64_t rows_a, rows_b;
@@ -43,13 +49,18 @@ struct Product {
 template <int BN, bool SWAP, typename T>
 __global__ void __launch_bounds__(kThreads, 1)
 matmul_q8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                 const Product p) {
-  constexpr int S = stages(BN), H = BN / 2, PIECE = H < 32 ? H : 32;
+                 const __grid_constant__ CUtensorMap map_out, const Product p) {
+  constexpr int S = stages(BN, SWAP);
+  constexpr int H = BN / 2, PIECE = H < 16 ? H : 16;  // a warp's columns, and those of a load
+  constexpr int kCopies = kSums / 32, kProducts = kCopies + 1, kScales = kCopies + 2;  // warps
   extern __shared__ uint8_t raw[];
   uint8_t* tiles = raw + (1024 - tc::shared_at(raw) % 1024) % 1024;
+  uint8_t* staged = tiles + S * stage_bytes(BN);  // SWAP = false: 4 KB a warp for rows of out
   __shared__ uint64_t full[S], empty[S], sum_full[2], sum_empty[2];
   __shared__ uint32_t tmem_at;
-  __shared__ __align__(16) float scales[SWAP ? 2 : 1][SWAP ? BN : 1];
+  constexpr int kScalesB = SWAP ? BN : 4;  // of each column, or of each block of columns
+  __shared__ __align__(16) float scales_a[kRing][kTileA], scales_b[kRing][kScalesB];
+  __shared__ uint64_t scales_full[kRing], scales_empty[kRing];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) {
@@ -60,40 +71,47 @@ matmul_q8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       tc::barrier_init(&sum_full[i], 1);
       tc::barrier_init(&sum_empty[i], kSums / 32);
     }
+    for (int i = 0; i < kRing; ++i) {
+      tc::barrier_init(&scales_full[i], 64);
+      tc::barrier_init(&scales_empty[i], kSums / 32);
+    }
     tc::barrier_init_fence();
     tc::prefetch_map(&map_a);
     tc::prefetch_map(&map_b);
   }
   constexpr uint32_t kColumns = 2 * BN < 32 ? 32 : 2 * BN;
-  if (warp == 9) tc::tmem_alloc(&tmem_at, kColumns);
+  if (warp == kProducts) tc::tmem_alloc(&tmem_at, kColumns);
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
   const uint32_t tmem = tmem_at;
-  const int rank = p.split > 1 ? blockIdx.x % p.split : 0;
-  const int64_t worker = blockIdx.x / p.split, workers = gridDim.x / p.split;
-  const int64_t total = (int64_t)p.tiles_a * p.tiles_b;
+  // a worker is one block, or those that share the depth of a tile
+  const int rank = blockIdx.x % p.split;
+  const int worker = blockIdx.x / p.split, workers = gridDim.x / p.split;
+  const int total = p.tiles_a * p.tiles_b;
   const int g0 = (int)((int64_t)p.groups * rank / p.split),
             g1 = (int)((int64_t)p.groups * (rank + 1) / p.split);
   // bands of 16 tiles of a, so that blocks at work at the same time share both operands in L2
-  auto place = [&](int64_t t, int& ta, int& tb) {
-    const int64_t band = t / (16ll * p.tiles_b);
-    const int64_t in = t - band * 16ll * p.tiles_b;
-    const int high = (int)min((int64_t)16, p.tiles_a - band * 16);
-    tb = (int)(in / high);
-    ta = (int)(band * 16 + in - (int64_t)tb * high);
+  constexpr int kBand = 16;
+  auto place = [&](int t, int& ta, int& tb) {
+    const int band = t / (kBand * p.tiles_b), in = t - band * kBand * p.tiles_b;
+    const int high = min(kBand, p.tiles_a - band * kBand);
+    tb = in / high;
+    ta = band * kBand + in - tb * high;
   };
-  bool ok = true;
+  uint32_t tries = tc::kTries;
 
-  if (warp == 8) {
+  if (warp >= kCopies) tc::registers_down<64>();
+  if (warp == kCopies) {
     if (tc::one_lane()) {
       int stage = 0;
       uint32_t phase = 0;
-      for (int64_t t = worker; ok && t < total; t += workers) {
+      for (int t = worker; tries && t < total; t += workers) {
         int ta, tb;
         place(t, ta, tb);
         for (int g = g0; g < g1; ++g) {
-          if (!(ok = tc::barrier_wait(&empty[stage], phase ^ 1))) break;
+          tc::barrier_wait(&empty[stage], phase ^ 1, tries);
+          if (!tries) break;
           uint8_t* a = tiles + stage * stage_bytes(BN);
           tc::barrier_expect(&full[stage], stage_bytes(BN));
           tc::load_box(a, &map_a, g * kGroup, ta * kTileA, &full[stage]);
@@ -103,19 +121,19 @@ matmul_q8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       }
       // all copies have to land before the block may end
       for (int i = 0; i < S; ++i) {
-        tc::barrier_wait(&empty[stage], phase ^ 1);
+        tc::barrier_wait(&empty[stage], phase ^ 1, tries);
         if (++stage == S) stage = 0, phase ^= 1;
       }
     }
-  } else if (warp == 9) {
+  } else if (warp == kProducts) {
     if (tc::one_lane()) {
       int stage = 0, buffer = 0;
       uint32_t phase = 0, sum_phase = 0;
-      for (int64_t t = worker; ok && t < total; t += workers) {
+      for (int t = worker; tries && t < total; t += workers) {
         for (int g = g0; g < g1; ++g) {
-          if (!(ok = tc::barrier_wait(&sum_empty[buffer], sum_phase ^ 1) &&
-                     tc::barrier_wait(&full[stage], phase)))
-            break;
+          tc::barrier_wait(&sum_empty[buffer], sum_phase ^ 1, tries);
+          tc::barrier_wait(&full[stage], phase, tries);
+          if (!tries) break;
           tc::fence_after();
           const uint8_t* at = tiles + stage * stage_bytes(BN);
           const uint64_t a = tc::operand(at, 1024), b = tc::operand(at + kTileA * kGroup, 1024);
@@ -123,117 +141,172 @@ matmul_q8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
           for (int k = 0; k < kGroup; k += 32)
             tc::product_e4m3(tmem + buffer * BN, tc::further(a, k), tc::further(b, k),
                              tc::shape(kTileA, BN, 0), k > 0);
-          tc::products_done(&empty[stage]);
           tc::products_done(&sum_full[buffer]);
+          tc::products_done(&empty[stage]);
           if (++stage == S) stage = 0, phase ^= 1;
           if (++buffer == 2) buffer = 0, sum_phase ^= 1;
         }
       }
     }
-  } else {
-    const int quarter = warp & 3, half = warp >> 2;
-    const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16) + half * H;
-    int buffer = 0;
+  } else if (warp >= kScales) {
+    // a warp for the lanes' scales and one for the columns': a row's scales lie together, so that
+    // every load takes as many lines as lanes, and here nobody waits for them
+    const bool lanes = warp == kScales;
+    const int n = lanes ? kTileA : kScalesB;
+    int slot = 0;
     uint32_t phase = 0;
-    for (int64_t t = worker; ok && t < total; t += workers) {
+    for (int t = worker; tries && t < total; t += workers) {
       int ta, tb;
       place(t, ta, tb);
-      const int64_t row = (int64_t)ta * kTileA + quarter * 32 + lane, col0 = (int64_t)tb * BN + half * H;
-      const float* sa = p.scale_a + (min(row, p.rows_a - 1) >> p.shift_a) * p.groups;
-      // of the warp's columns, or (SWAP) of the column that this thread fetches
-      const int64_t of = SWAP ? (int64_t)tb * BN + (int)threadIdx.x % BN : col0;
-      const float* sb = p.scale_b + (min(of, p.rows_b - 1) >> p.shift_b) * p.groups;
-      f32x2 sum[H / 2];
+      const float* from[kTileA / 32 > kScalesB / 32 ? kTileA / 32 : kScalesB / 32];
 #pragma unroll
-      for (int i = 0; i < H / 2; ++i) sum[i] = 0;
-      float next_a = g0 < g1 ? sa[g0] : 0.f, next_b = g0 < g1 ? sb[g0] : 0.f;
+      for (int i = 0; i < (int)(sizeof(from) / sizeof(from[0])); ++i) {
+        const int at = i * 32 + lane;
+        const int64_t row = lanes  ? (int64_t)ta * kTileA + at
+                            : SWAP ? (int64_t)tb * BN + at
+                                   : (int64_t)tb * BN + at * kGroup;
+        from[i] = lanes ? p.scale_a + (min(row, p.rows_a - 1) >> p.shift_a) * p.groups
+                        : p.scale_b + (min(row, p.rows_b - 1) >> p.shift_b) * p.groups;
+      }
       for (int g = g0; g < g1; ++g) {
-        const float now_a = next_a, now_b = next_b;
-        if (g + 1 < g1) next_a = sa[g + 1], next_b = sb[g + 1];
-        if (SWAP) {
-          if (threadIdx.x < BN) scales[g & 1][threadIdx.x] = now_b;
-          tc::named_sync(1, kSums);
-        }
-        if (!(ok = tc::barrier_wait(&sum_full[buffer], phase))) break;
+        tc::barrier_wait_warp(&scales_empty[slot], phase ^ 1, tries);
+        if (!tries) break;
+        float* to = (lanes ? scales_a[slot] : scales_b[slot]) + lane;
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(from) / sizeof(from[0])); ++i)
+          if (i * 32 + lane < n) tc::copy4(to + i * 32, from[i] + g);
+        tc::copies_arrive(&scales_full[slot]);
+        if (++slot == kRing) slot = 0, phase ^= 1;
+      }
+    }
+    tc::copies_done();
+  } else {
+    tc::registers_up<216>();
+    const int quarter = warp & 3, half = warp >> 2;
+    const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16) + half * H;
+    int buffer = 0, slot = 0;
+    uint32_t phase = 0, slot_phase = 0;
+#pragma unroll 1
+    for (int t = worker; tries && t < total; t += workers) {
+      float sum[H];
+#pragma unroll
+      for (int i = 0; i < H; ++i) sum[i] = 0.f;
+      // (unrolled, or with a way out in its middle, the loop copies the sums in every turn)
+#pragma unroll 1
+      for (int g = g0; g < g1; ++g) {
+        tc::barrier_wait_warp(&scales_full[slot], slot_phase, tries);
+        const float* sb = scales_b[slot];
+        const float of_lane = scales_a[slot][quarter * 32 + lane];
+        const float by = SWAP ? of_lane : of_lane * sb[half * H / kGroup];
+        tc::barrier_wait_warp(&sum_full[buffer], phase, tries);
         tc::fence_after();
+        uint32_t r[2][PIECE];
+        tc::tmem_load<PIECE>(r[0], mine + buffer * BN);
 #pragma unroll
         for (int c = 0; c < H; c += PIECE) {
-          uint32_t r[PIECE];
-          tc::tmem_load<PIECE>(r, mine + buffer * BN + c);
           tc::loads_done();
-          if (c + PIECE == H) {
+          if (c + PIECE < H) {  // on its way while this piece is added
+            tc::tmem_load<PIECE>(r[(c / PIECE + 1) % 2], mine + buffer * BN + c + PIECE);
+          } else {
             tc::fence_before();
             __syncwarp();
-            if (lane == 0) tc::barrier_arrive(&sum_empty[buffer]);
+            tc::barrier_arrive_if_zero(&sum_empty[buffer], lane);
           }
-          const f32x2 by = both(SWAP ? now_a : now_a * now_b);
+          const uint32_t(&now)[PIECE] = r[c / PIECE % 2];
 #pragma unroll
           for (int i = 0; i < PIECE; i += 4) {
-            f32x2 s0 = by, s1 = by;
+            float4 v = make_float4(by, by, by, by);
             if (SWAP) {
-              const float4 v = *reinterpret_cast<const float4*>(&scales[g & 1][half * H + c + i]);
-              s0 = mul2(by, pair(v.x, v.y)), s1 = mul2(by, pair(v.z, v.w));
+              v = *reinterpret_cast<const float4*>(sb + half * H + c + i);
+              v.x *= by, v.y *= by, v.z *= by, v.w *= by;
             }
-            f32x2* to = &sum[(c + i) / 2];
-            to[0] = fma2(pair(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), s0, to[0]);
-            to[1] = fma2(pair(__uint_as_float(r[i + 2]), __uint_as_float(r[i + 3])), s1, to[1]);
+            sum[c + i] = fmaf(__uint_as_float(now[i]), v.x, sum[c + i]);
+            sum[c + i + 1] = fmaf(__uint_as_float(now[i + 1]), v.y, sum[c + i + 1]);
+            sum[c + i + 2] = fmaf(__uint_as_float(now[i + 2]), v.z, sum[c + i + 2]);
+            sum[c + i + 3] = fmaf(__uint_as_float(now[i + 3]), v.w, sum[c + i + 3]);
           }
         }
+        __syncwarp();
+        tc::barrier_arrive_if_zero(&scales_empty[slot], lane);
+        if (++slot == kRing) slot = 0, slot_phase ^= 1;
         if (++buffer == 2) buffer = 0, phase ^= 1;
       }
-      if (!ok) {  // a result that nobody can take for one
+      if (!tries) {  // a result that nobody can take for one
 #pragma unroll
-        for (int i = 0; i < H / 2; ++i) sum[i] = both(__int_as_float(0x7fffffff));
+        for (int i = 0; i < H; ++i) sum[i] = __int_as_float(0x7fffffff);
       }
       if (p.split > 1) {
         // every block's part of the tile, [column][lane], in its own shared memory (all of this
         // block's copies and products are done: their sums are here)
-        float* part = reinterpret_cast<float*>(tiles);
+        float* to = reinterpret_cast<float*>(tiles) + quarter * 32 + lane;
 #pragma unroll
-        for (int i = 0; i < H / 2; ++i) {
-          const float2 v = halves(sum[i]);
-          part[(half * H + 2 * i) * kTileA + quarter * 32 + lane] = v.x;
-          part[(half * H + 2 * i + 1) * kTileA + quarter * 32 + lane] = v.y;
-        }
+        for (int i = 0; i < H; ++i) to[(half * H + i) * kTileA] = sum[i];
         break;  // joined below
       }
+      int ta, tb;
+      place(t, ta, tb);
+      const int64_t row = (int64_t)ta * kTileA + quarter * 32 + lane;
+      const int64_t col0 = (int64_t)tb * BN + half * H;
+      const int most = (int)min((int64_t)H, p.rows_b - col0);
       if constexpr (SWAP) {
-        if (row < p.rows_a) {
-          const float b = p.bias ? weight_at<T>(p.bias, row, p.bias_f32) : 0.f;
-          T* out = static_cast<T*>(p.out) + col0 * p.out_stride + row;
-          const int most = (int)min((int64_t)H, p.rows_b - col0);
+        if (row >= p.rows_a) continue;
+        const float b = p.bias ? weight_at<T>(p.bias, row, p.bias_f32) : 0.f;
+        T* out = static_cast<T*>(p.out) + col0 * p.out_stride + row;
 #pragma unroll
-          for (int i = 0; i < H / 2; ++i) {
-            const float2 v = halves(sum[i]);
-            if (2 * i < most) out[2 * i * p.out_stride] = from_f32<T>(v.x + b);
-            if (2 * i + 1 < most) out[(2 * i + 1) * p.out_stride] = from_f32<T>(v.y + b);
-          }
+        for (int i = 0; i < H; ++i) {
+          if (i < most) *out = from_f32<T>(sum[i] + b);
+          out += p.out_stride;
         }
       } else {
-        if (row < p.rows_a) {
-          T* out = static_cast<T*>(p.out) + row * p.out_stride + col0;
-          const int most = (int)min((int64_t)H, p.rows_b - col0);
+        // Through shared memory: 128 bytes of each of the warp's rows at a time, in 16-byte units at
+        // place unit ^ (row & 7), as a tensor copy takes them (or 8 lanes a row, side by side).
+        constexpr int W = 128 / sizeof(T), U = 16 / sizeof(T);
+        uint8_t* at = staged + warp * 4096;
+        const int64_t row0 = row - lane;
 #pragma unroll
-          for (int i = 0; i < H; i += 8) {
-            float f[8];
+        for (int c = 0; c < H; c += W) {
+          if (c >= most) break;
+          if (p.vec && lane == 0) tc::stores_read();
+          __syncwarp();
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float2 v = halves(sum[i / 2 + k]);
-              f[2 * k] = v.x, f[2 * k + 1] = v.y;
+          for (int u = 0; u < 8; ++u) {
+            float f[U];
+#pragma unroll
+            for (int k = 0; k < U; ++k) f[k] = sum[c + u * U + k];
+            if (p.bias) {
+#pragma unroll
+              for (int k = 0; k < U; ++k)
+                if (c + u * U + k < most)
+                  f[k] += weight_at<T>(p.bias, col0 + c + u * U + k, p.bias_f32);
             }
-            if (i < most) {
-              if (p.bias) {
+            store_pack<T, U>(reinterpret_cast<T*>(at + lane * 128 + (u ^ (lane & 7)) * 16), f, U,
+                             true);
+          }
+          if (p.vec) {  // what lies past the edges is left out
+            tc::fence_shared();
+            __syncwarp();
+            if (lane == 0 && row0 < p.rows_a)
+              tc::store_box(&map_out, at, (int)col0 + c, (int)row0);
+            continue;
+          }
+          __syncwarp();
+          const int u = lane & 7, n = most - c - u * U;
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
-                  if (i + k < most) f[k] += weight_at<T>(p.bias, col0 + i + k, p.bias_f32);
-              }
-              store_pack<T, 8>(out + i, f, most - i, p.vec);
-            }
+          for (int i = 0; i < 8; ++i) {
+            const int r = i * 4 + (lane >> 3);
+            if (row0 + r >= p.rows_a || n <= 0) continue;
+            const Pack<T, U> v =
+                *reinterpret_cast<const Pack<T, U>*>(at + r * 128 + (u ^ (r & 7)) * 16);
+            T* out = static_cast<T*>(p.out) + (row0 + r) * p.out_stride + col0 + c + u * U;
+#pragma unroll
+            for (int k = 0; k < U; ++k)
+              if (k < n) out[k] = v.v[k];
           }
         }
       }
     }
   }
+  if (!SWAP && lane == 0) tc::stores_done();
   __syncwarp();  // the copies' and the products' warps went apart
   if (p.split > 1) {
     // the blocks of a cluster hold parts of one tile: each adds up its share of the columns, in the
@@ -265,7 +338,7 @@ matmul_q8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
   }
   tc::fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kProducts) {
     tc::fence_after();
     tc::tmem_free(tmem, kColumns);
   }
@@ -318,6 +391,8 @@ EncodeTiled encoder() {
   return f;
 }
 
+constexpr int64_t kMostStride = 1ll << 39;  // a tensor map's strides lie under 2^40
+
 // Boxes of 128 bytes x `high` rows; what lies past k or the rows reads as zero.
 bool tile_map(CUtensorMap* map, const void* p, int64_t rows, int64_t k, int64_t stride, int high) {
   const EncodeTiled f = encoder();
@@ -331,7 +406,21 @@ bool tile_map(CUtensorMap* map, const void* p, int64_t rows, int64_t k, int64_t 
            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-constexpr int64_t kMostStride = 1ll << 39;  // a tensor map's strides lie under 2^40
+// Boxes of 128 bytes x 32 rows of the output.
+template <typename T>
+bool out_map(CUtensorMap* map, void* p, int64_t rows, int64_t n, int64_t stride) {
+  const EncodeTiled f = encoder();
+  if (!f || stride * (int64_t)sizeof(T) >= kMostStride) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)n, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)stride * sizeof(T)};
+  const cuuint32_t box[2] = {128 / sizeof(T), 32}, unit[2] = {1, 1};
+  const CUtensorMapDataType type = sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                                  : CU_TENSOR_MAP_DATA_TYPE_UINT16;
+  return f(map, type, 2, p, dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
+           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 int64_t aligned_stride(int64_t k) { return (k + 15) / 16 * 16; }
 bool tiled(const void* p, int64_t rows, int64_t stride, int64_t k) {
   return aligned16(p) && (rows == 1 || (stride % 16 == 0 && stride >= k && stride < kMostStride));
@@ -366,19 +455,20 @@ template <int BN, bool SWAP, typename T>
 cudaError_t launch(Operand a, Operand b, int64_t k, Product p, cudaStream_t st, int* launches) {
   p.tiles_a = (int)((p.rows_a + kTileA - 1) / kTileA);
   p.tiles_b = (int)((p.rows_b + BN - 1) / BN);
-  CUtensorMap map_a, map_b;
+  CUtensorMap map_a, map_b, map_out = {};
   if (!tile_map(&map_a, a.p, a.rows, k, a.stride, kTileA) ||
       !tile_map(&map_b, b.p, b.rows, k, b.stride, BN))
     return cudaErrorInvalidValue;
+  if (!SWAP && p.vec && !out_map<T>(&map_out, p.out, p.rows_a, p.rows_b, p.out_stride)) p.vec = false;
   const auto kernel = matmul_q8_kernel<BN, SWAP, T>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       shared_bytes(BN));
+                                       shared_bytes(BN, SWAP));
   if (e != cudaSuccess) return e;
   const int64_t total = (int64_t)p.tiles_a * p.tiles_b;
   cudaLaunchConfig_t c = {};
   c.gridDim = dim3((unsigned)(p.split > 1 ? total * p.split : std::min<int64_t>(total, 148)));
   c.blockDim = dim3(kThreads);
-  c.dynamicSmemBytes = shared_bytes(BN);
+  c.dynamicSmemBytes = shared_bytes(BN, SWAP);
   c.stream = st;
   cudaLaunchAttribute attr = {};
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -387,7 +477,7 @@ cudaError_t launch(Operand a, Operand b, int64_t k, Product p, cudaStream_t st, 
   c.attrs = &attr;
   c.numAttrs = p.split > 1;
   ++*launches;
-  return cudaLaunchKernelEx(&c, kernel, map_a, map_b, (const Product)p);
+  return cudaLaunchKernelEx(&c, kernel, map_a, map_b, map_out, (const Product)p);
 }
 
 template <typename T>
@@ -406,7 +496,7 @@ cudaError_t run(const salt_matmul_q8_args& a, const Operand& x, const Operand& w
     p.rows_a = a.rows, p.rows_b = a.n;
     p.scale_a = a.x_scale, p.scale_b = a.weight_scale;
     p.shift_a = 0, p.shift_b = shift_w;
-    p.vec = pack_rows(a.out, 8, sizeof(T), a.out_stride);
+    p.vec = packed_rows(a.out, 16, sizeof(T), a.out_stride, 0);
     const int64_t wide = ((a.rows + 127ll) / 128) * ((a.n + 255ll) / 256);
     if (wide >= 148) return launch<256, false, T>(x, w, a.k, p, st, launches);
     return launch<128, false, T>(x, w, a.k, p, st, launches);

@@ -38,19 +38,41 @@ __device__ __forceinline__ bool barrier_try(uint64_t* b, uint32_t parity) {
       : "memory");
   return done;
 }
-// Waits for the barrier's phase of that parity to end; gives up (false) after some seconds, which
-// only a fault elsewhere can bring about.
-constexpr long long kWaitCycles = 4ll << 30;
-__device__ __forceinline__ bool barrier_wait(uint64_t* b, uint32_t parity) {
-  if (barrier_try(b, parity)) return true;
-  const long long since = clock64();
-  while (!barrier_try(b, parity))
-    if (clock64() - since > kWaitCycles) return false;
-  return true;
+// Waits for the barrier's phase of that parity to end.  Gives up after `tries` looks, which only a
+// fault elsewhere can bring about (a look that finds nothing takes some 4 us: about a second in
+// all), and leaves tries = 0 behind: later waits then look once.
+constexpr uint32_t kTries = 1u << 18;
+__device__ __forceinline__ void barrier_wait(uint64_t* b, uint32_t parity, uint32_t& tries) {
+  for (uint32_t i = tries; !barrier_try(b, parity); --i)
+    if (i == 0) {
+      tries = 0;
+      break;
+    }
 }
-// Threads of part of a block.
-__device__ __forceinline__ void named_sync(int id, int threads) {
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+// The same by a whole warp, whose lanes stay together.
+__device__ __forceinline__ void barrier_wait_warp(uint64_t* b, uint32_t parity, uint32_t& tries) {
+  for (uint32_t i = tries; !__all_sync(0xffffffffu, barrier_try(b, parity)); --i)
+    if (i == 0) {
+      tries = 0;
+      break;
+    }
+}
+// An arrival of the lanes that hold 0, without a branch.
+__device__ __forceinline__ void barrier_arrive_if_zero(uint64_t* b, int lane) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.eq.s32 p, %1, 0;\n @p mbarrier.arrive.shared::cta.b64 _, [%0];\n}" ::"r"(
+          shared_at(b)),
+      "r"(lane)
+      : "memory");
+}
+// A warpgroup's share of the registers that the block was launched with.
+template <int N>
+__device__ __forceinline__ void registers_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void registers_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 // ---------------------------------------------------------------- tensor copies
@@ -64,9 +86,34 @@ __device__ __forceinline__ void load_box(void* to, const CUtensorMap* map, int x
       "l"(map), "r"(x), "r"(y), "r"(shared_at(barrier))
       : "memory");
 }
+// A box of shared memory to column x and row y, what lies past the array's edges left out.  The memory
+// may be written again after stores_read, and given up after stores_done, by the same thread.
+__device__ __forceinline__ void store_box(const CUtensorMap* map, const void* from, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];\n"
+      "cp.async.bulk.commit_group;" ::"l"(map),
+      "r"(x), "r"(y), "r"(shared_at(from))
+      : "memory");
+}
+__device__ __forceinline__ void stores_read() {
+  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+__device__ __forceinline__ void stores_done() {
+  asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+}
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
+
+// 4 bytes by the calling thread; the barrier counts the thread once all its copies so far are there.
+__device__ __forceinline__ void copy4(void* to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(shared_at(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_arrive(uint64_t* barrier) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(shared_at(barrier))
+               : "memory");
+}
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // ---------------------------------------------------------------- tensor memory
 
