@@ -4,7 +4,10 @@
 // order, dk and dv over (v, dout, q) and (k, q, dout) against it.  One pass computes
 //   forward:  S = l S + k v^T;  out = scale * q S
 //   reverse:  D = C + beta * k v^T;  out = q D;  C = l D   (from the row's end; C starts as given)
+#include <type_traits>
+
 #include "sequence.cuh"
+#include "tc.cuh"
 
 namespace salt {
 namespace {
@@ -26,6 +29,10 @@ struct Pass {
   void* out;
   int64_t out_batch, out_token;
   float* final;
+  // set by the launch
+  int segments, seg_chunks;  // segments of a row that run side by side, chunks of each
+  float* seg_states;         // (batch, heads, segments, dk, dv): what each adds to the state
+  bool vec, vec_out;
 };
 
 __device__ __forceinline__ float decay_of(const float* g, int h) {
@@ -38,56 +45,478 @@ __device__ __forceinline__ const T* row_of(const Rows& r, int b, int64_t t, int 
   return static_cast<const T*>(r.p) + b * r.batch + t * r.token + (int64_t)(h / r.share) * dim;
 }
 
-template <typename T, typename O>
-__global__ void __launch_bounds__(256) attention_simple_kernel(Pass a) {
-  __shared__ float red[8][33];
-  const int tiles = (a.dv + 31) / 32;
-  const int tile = blockIdx.x % tiles, bh = blockIdx.x / tiles, b = bh / a.heads, h = bh % a.heads;
-  const int x = threadIdx.x & 31, y = threadIdx.x >> 5, col = tile * 32 + x;
-  const int n = row_tokens(a.n_real, b, a.len);
-  const float l = expf(decay_of(a.log_decay, h));
-  float s[16];
-  for (int i = 0; i < 16; ++i) {
-    const int r = y + 8 * i;
-    const int64_t base = (int64_t)bh * a.dk * a.dv;
-    s[i] = a.initial && r < a.dk && col < a.dv
-               ? a.initial[base + (a.initial_t ? (int64_t)col * a.dk + r : (int64_t)r * a.dv + col)]
-               : 0.f;
-  }
-  for (int i = 0; i < n; ++i) {
-    const int t = a.reverse ? n - 1 - i : i;
-    const T* q = row_of<T>(a.q, b, t, h, a.dk);
-    const T* k = row_of<T>(a.k, b, t, h, a.dk);
-    const float v = col < a.dv ? to_f32(row_of<T>(a.v, b, t, h, a.dv)[col]) : 0.f;
-    float acc = 0.f;
+constexpr int kTile = 64;      // columns of v that a block takes
+constexpr int kThreads = 256;  // 8 warps: two for each 32 rows of tensor memory
+constexpr int kWeighted = 3;   // parts of a weighted v
+
+// A type's values in parts of bfloat16, 8 bits each: what the tensor cores multiply.
+template <typename T>
+constexpr int parts_of() { return sizeof(T) == 4 ? 3 : std::is_same<T, __half>::value ? 2 : 1; }
+// Tokens of a chunk, and parts of the states and of the weights within a chunk.
+template <typename T>
+constexpr int chunk_of() { return parts_of<T>() == 1 ? 128 : 64; }
+template <typename T>
+constexpr int state_parts() { return sizeof(T) == 4 ? 3 : 2; }
+
+// Shared memory, all operands in rows of 128 bytes (tc::operand): q and k in panels of 64 columns,
+// part after part; k and v twice where copies run ahead.
+template <typename T, int PANELS, bool AHEAD>
+struct Layout {
+  static constexpr int P = parts_of<T>(), C = chunk_of<T>(), B = AHEAD ? 2 : 1;
+  static constexpr int kPanel = C * 128, kKeys = P * PANELS * kPanel, kValues = P * kPanel;
+  static constexpr int q = 0, k = q + kKeys, v = k + B * kKeys, weighted = v + B * kValues,
+                       state = weighted + kWeighted * kPanel,
+                       kState = PANELS * 64 * 128,  // a part of the state
+      bytes = state + state_parts<T>() * kState + 1024;
+};
+
+// A value's parts: each the nearest bfloat16 of what the ones before it leave.
+template <int N>
+__device__ __forceinline__ void split2(uint32_t (&to)[N], float x, float y) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const int r = y + 8 * j;
-      if (r >= a.dk) continue;
-      const float kv = to_f32(k[r]) * v;
-      s[j] = a.reverse ? s[j] + a.scale * kv : l * s[j] + kv;
-      acc += to_f32(q[r]) * s[j];
-      if (a.reverse) s[j] *= l;
-    }
-    red[y][x] = acc;
-    __syncthreads();
-    if (y == 0 && col < a.dv) {
-      float o = 0.f;
-      for (int j = 0; j < 8; ++j) o += red[j][x];
-      static_cast<O*>(a.out)[b * a.out_batch + t * a.out_token + (int64_t)h * a.dv + col] =
-          from_f32<O>(a.reverse ? o : a.scale * o);
-    }
-    __syncthreads();
+  for (int i = 0; i < N; ++i) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    to[i] = *reinterpret_cast<const uint32_t*>(&h);
+    x -= __uint_as_float(to[i] << 16);
+    y -= __uint_as_float(to[i] & 0xffff0000u);
   }
-  if (y == 0 && col < a.dv)
-    for (int t = n; t < a.len; ++t)
-      static_cast<O*>(a.out)[b * a.out_batch + t * a.out_token + (int64_t)h * a.dv + col] =
-          from_f32<O>(0.f);
-  if (a.final && col < a.dv)
-    for (int j = 0; j < 16; ++j) {
-      const int r = y + 8 * j;
-      if (r < a.dk) a.final[(int64_t)bh * a.dk * a.dv + (int64_t)r * a.dv + col] = s[j];
+}
+
+// Rows of `dim` values at p (token t at p + t * stride; `count` of them, the rest zero) to `parts` of
+// panels of 64 columns from column `from`.
+template <typename T, int PANELS, int C>
+__device__ __forceinline__ void load_rows(uint8_t* to, const T* p, int64_t stride, int count, int from,
+                                          int dim, bool vec) {
+  constexpr int P = parts_of<T>(), U = PANELS * 8;
+  for (int i = threadIdx.x; i < C * U; i += kThreads) {
+    const int row = i / U, u = i % U, at = from + u * 8;
+    const Pack<T, 8> x = load_pack<T, 8>(p + row * stride + at, row < count ? dim - at : 0, vec);
+    uint32_t parts[4][P];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) split2<P>(parts[k], to_f32(x.v[2 * k]), to_f32(x.v[2 * k + 1]));
+    uint8_t* place = to + (u >> 3) * C * 128 + row * 128 + (((u & 7) ^ (row & 7)) << 4);
+#pragma unroll
+    for (int j = 0; j < P; ++j)
+      *reinterpret_cast<uint4*>(place + j * PANELS * C * 128) =
+          make_uint4(parts[0][j], parts[1][j], parts[2][j], parts[3][j]);
+  }
+}
+
+// One pass over chunks of C tokens (natural order; from the last one where `reverse`):
+//   out = row weight * (q S) + (q k^T under a triangle of decays) v;
+//   S = l^tokens S + k^T (weights * v)
+// as four products of the tensor cores.  Per chunk and head, with c = C tokens: 2 c^2 dk + 2 c^2 dv +
+// 4 c dk dv operations, against the 5 dk dv a token of the recurrence itself.
+//
+// What is rounded: every operand is bfloat16, in parts of 8 bits.  Inputs are exact (bfloat16 in one
+// part, float16 in two, float32 in three, the last rounded); weighted values have three parts, so
+// that states are good to 2^-24; states and the triangle's values, as operands for out, have three
+// parts for float32 and two (2^-16) for outputs of 16 bits.  Sums and states are float32; the state
+// is carried in registers.
+template <typename T, typename O, int PANELS, bool AHEAD, bool STATE>
+__global__ void __launch_bounds__(kThreads, 1)
+attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                 const __grid_constant__ CUtensorMap map_v, const Pass a) {
+  using L = Layout<T, PANELS, AHEAD>;
+  constexpr int C = L::C, P = L::P, SP = state_parts<T>(), DK = PANELS * 64;
+  constexpr int kPanel = L::kPanel;
+  extern __shared__ uint8_t raw[];
+  uint8_t* sm = raw + (1024 - tc::shared_at(raw) % 1024) % 1024;
+  __shared__ uint64_t loaded_q, loaded_k[2], loaded_v[2], done_q, done_scores, done_state, done_out;
+  __shared__ uint32_t tmem_at;
+  __shared__ float power[C + 1];               // l^i
+  __shared__ __align__(16) float column[32];   // of a column within its 32
+  __shared__ int bad[3][kTile];                // the outermost token whose v is not finite
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane;
+
+  const int tiles = (a.dv + kTile - 1) / kTile;
+  int id = blockIdx.x;
+  const int tile = id % tiles;
+  id /= tiles;
+  const int seg = id % a.segments, bh = id / a.segments, b = bh / a.heads, h = bh - b * a.heads;
+  const int n = row_tokens(a.n_real, b, a.len), chunks = (n + C - 1) / C;
+  const int c0 = min(seg * a.seg_chunks, chunks);
+  // (nobody needs what the last segment alone adds to the state)
+  const bool needed = !STATE || seg != (a.reverse ? 0 : a.segments - 1);
+  const int c1 = needed ? min(c0 + a.seg_chunks, chunks) : c0;
+  const int col0 = tile * kTile, cols = min(kTile, a.dv - col0);
+  const float g = decay_of(a.log_decay, h) * kLog2e;
+  const int64_t state_at = (int64_t)bh * a.dk * a.dv;
+
+  if (threadIdx.x == 0) {
+    uint64_t* all[] = {&loaded_q, &loaded_k[0], &loaded_k[1], &loaded_v[0], &loaded_v[1],
+                       &done_q,   &done_scores, &done_state,  &done_out};
+    for (uint64_t* x : all) tc::barrier_init(x, 1);
+    tc::barrier_init_fence();
+  }
+  if (warp == 0) tc::tmem_alloc(&tmem_at, 512);
+  for (int i = threadIdx.x; i <= C; i += kThreads) power[i] = i == 0 ? 1.f : exp2f(g * (float)i);
+  if (threadIdx.x < 32) {
+    const int i = a.reverse ? threadIdx.x : 31 - threadIdx.x;
+    column[threadIdx.x] = i == 0 ? 1.f : exp2f(g * (float)i);
+  }
+  for (int i = threadIdx.x; i < 3 * kTile; i += kThreads) bad[i / kTile][i % kTile] = -1;
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = tmem_at, mine = tmem + ((uint32_t)(quarter * 32) << 16);
+  // columns of tensor memory
+  constexpr int kScores = 0, kTriangle = 128, kFromState = 256, kOut = 384, kAdded = 448;
+
+  // this thread's part of the state: row `row`, 32 columns
+  float s[32];
+  const int sc0 = col0 + half * 32;
+#pragma unroll
+  for (int j = 0; j < 32; ++j)
+    s[j] = a.initial && row < a.dk && sc0 + j < a.dv
+               ? a.initial[state_at + (a.initial_t ? (int64_t)(sc0 + j) * a.dk + row
+                                                   : (int64_t)row * a.dv + sc0 + j)]
+               : 0.f;
+  if (a.segments > 1 && !STATE) {
+    // the states that the segments in front left behind, each from zero
+    const int before = a.reverse ? a.segments - 1 - seg : seg;
+    for (int i = 0; i < before; ++i) {
+      const int at = a.reverse ? a.segments - 1 - i : i;
+      const int first = at * a.seg_chunks * C, count = min(first + a.seg_chunks * C, n) - first;
+      if (count <= 0) continue;
+      const float l = exp2f(g * (float)count);
+      const float* from = a.seg_states + ((int64_t)bh * a.segments + at) * a.dk * a.dv;
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (row < a.dk && sc0 + j < a.dv)
+          s[j] = fmaf(s[j], l, from[(int64_t)row * a.dv + sc0 + j]);
     }
+  }
+  const auto store_state = [&](int x) {  // as an operand
+    if (row >= DK) return;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      uint32_t parts[4][SP];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) split2<SP>(parts[k], s[8 * u + 2 * k], s[8 * u + 2 * k + 1]);
+#pragma unroll
+      for (int j = 0; j < SP; ++j)
+        *reinterpret_cast<uint4*>(sm + L::state + j * L::kState + row * 128 +
+                                  (((half * 4 + u) ^ (row & 7)) << 4)) =
+            make_uint4(parts[0][j], parts[1][j], parts[2][j], parts[3][j]);
+    }
+  };
+  const int steps = c1 - c0;
+  uint32_t tries = tc::kTries;
+  const auto chunk = [&](int i) { return a.reverse ? c1 - 1 - i : c0 + i; };
+  const auto tokens = [&](int c) { return min(C, n - c * C); };
+  // copies ahead, by thread 0
+  const auto fetch_q = [&](int i) {
+    tc::barrier_expect(&loaded_q, L::kKeys);
+    for (int x = 0; x < PANELS; ++x)
+      tc::load_box4(sm + L::q + x * kPanel, &map_q, x * 64, h / a.q.share, chunk(i) * C, b, &loaded_q);
+  };
+  const auto fetch_k = [&](int i) {
+    tc::barrier_expect(&loaded_k[i & 1], L::kKeys);
+    for (int x = 0; x < PANELS; ++x)
+      tc::load_box4(sm + L::k + (i & 1) * L::kKeys + x * kPanel, &map_k, x * 64, h / a.k.share,
+                    chunk(i) * C, b, &loaded_k[i & 1]);
+  };
+  const auto fetch_v = [&](int i) {
+    tc::barrier_expect(&loaded_v[i & 1], L::kValues);
+    tc::load_box4(sm + L::v + (i & 1) * L::kValues, &map_v, col0, h / a.v.share, chunk(i) * C, b,
+                  &loaded_v[i & 1]);
+  };
+  if (AHEAD && threadIdx.x == 0 && steps > 0) {
+    if (!STATE) fetch_q(0);
+    fetch_k(0);
+    fetch_v(0);
+    if (steps > 1) {
+      fetch_k(1);
+      fetch_v(1);
+    }
+  }
+  if (!STATE && steps > 0) store_state(0);
+
+  // Chunk i's operands: brought in where nobody copied ahead, rows past the end made zero, values
+  // weighted; then its products that need no others' results.
+  const auto begin = [&](int i) {
+    const int c = chunk(i), count = tokens(c), at = AHEAD ? i & 1 : 0;
+    uint8_t* k = sm + L::k + at * L::kKeys;
+    uint8_t* v = sm + L::v + at * L::kValues;
+    if (AHEAD) {
+      tc::barrier_wait_warp(&loaded_v[at], i >> 1 & 1, tries);
+      tc::barrier_wait_warp(&loaded_k[at], i >> 1 & 1, tries);
+      if (!STATE) tc::barrier_wait_warp(&loaded_q, i & 1, tries);
+      if (count < C) {
+        for (int x = threadIdx.x; x < (C - count) * PANELS * 8; x += kThreads) {
+          const int r = count + x / (PANELS * 8), u = x % (PANELS * 8);
+          *reinterpret_cast<uint4*>(k + (u >> 3) * kPanel + r * 128 + ((u & 7) << 4)) =
+              make_uint4(0, 0, 0, 0);
+        }
+      }
+    } else {
+      const int64_t t = (int64_t)c * C;
+      if (!STATE)
+        load_rows<T, PANELS, C>(sm + L::q, row_of<T>(a.q, b, t, h, a.dk), a.q.token, count, 0, a.dk,
+                                a.vec);
+      load_rows<T, PANELS, C>(k, row_of<T>(a.k, b, t, h, a.dk), a.k.token, count, 0, a.dk, a.vec);
+      load_rows<T, 1, C>(v, row_of<T>(a.v, b, t, h, a.dv), a.v.token, count, col0, a.dv, a.vec);
+      __syncthreads();
+    }
+    for (int x = threadIdx.x; x < C * 8; x += kThreads) {
+      const int r = x >> 3, u = x & 7;
+      uint8_t* place = v + r * 128 + ((u ^ (r & 7)) << 4);
+      const float w = r >= count ? 0.f : power[a.reverse ? r + 1 : count - 1 - r];
+      uint32_t in[P][4], out[4][kWeighted];
+      bool fine = true;
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        const uint4 y = *reinterpret_cast<const uint4*>(place + j * kPanel);
+        in[j][0] = y.x, in[j][1] = y.y, in[j][2] = y.z, in[j][3] = y.w;
+      }
+      if (r >= count) {
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+          in[j][0] = in[j][1] = in[j][2] = in[j][3] = 0;
+          *reinterpret_cast<uint4*>(place + j * kPanel) = make_uint4(0, 0, 0, 0);
+        }
+      }
+      // A value that is not finite would reach the tokens on the triangle's other side, as 0 * it:
+      // it becomes zero here, and its column NaN from its token on.
+#pragma unroll
+      for (int m = 0; m < 4; ++m)
+        fine &= (in[0][m] & 0x7f80u) != 0x7f80u && (in[0][m] & 0x7f800000u) != 0x7f800000u;
+      if (!fine) {
+#pragma unroll
+        for (int m = 0; m < 8; ++m) {
+          const uint32_t mask = 0xffffu << (m & 1) * 16, exponent = 0x7f80u << (m & 1) * 16;
+          if ((in[0][m / 2] & exponent) != exponent) continue;
+          if (a.reverse)
+            atomicMax(&bad[i % 3][u * 8 + m], r);
+          else
+            atomicMax(&bad[i % 3][u * 8 + m], C - 1 - r);
+#pragma unroll
+          for (int j = 0; j < P; ++j) in[j][m / 2] &= ~mask;
+        }
+#pragma unroll
+        for (int j = 0; j < P; ++j)
+          *reinterpret_cast<uint4*>(place + j * kPanel) =
+              make_uint4(in[j][0], in[j][1], in[j][2], in[j][3]);
+      }
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        float lo = __uint_as_float(in[0][m] << 16), hi = __uint_as_float(in[0][m] & 0xffff0000u);
+#pragma unroll
+        for (int j = 1; j < P; ++j) {
+          lo += __uint_as_float(in[j][m] << 16);
+          hi += __uint_as_float(in[j][m] & 0xffff0000u);
+        }
+        split2<kWeighted>(out[m], w * lo, w * hi);
+      }
+      uint8_t* to = sm + L::weighted + (place - v);
+#pragma unroll
+      for (int j = 0; j < kWeighted; ++j)
+        *reinterpret_cast<uint4*>(to + j * kPanel) =
+            make_uint4(out[0][j], out[1][j], out[2][j], out[3][j]);
+    }
+    if (threadIdx.x < kTile) bad[(i + 1) % 3][threadIdx.x] = -1;
+    tc::fence_shared();
+    tc::fence_before();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      tc::fence_after();
+      const int depth = (a.dk + 15) / 16;
+      if (!STATE) {
+        bool add = false;
+        for (int x = 0; x < P; ++x)
+          for (int y = 0; y < P && x + y < 3; ++y)
+            for (int d = 0; d < depth; ++d) {
+              const int off = (d >> 2) * kPanel + (d & 3) * 32;
+              tc::product_16(tmem + kScores,
+                             tc::operand(sm + L::q + x * PANELS * kPanel + off, 1024),
+                             tc::operand(k + y * PANELS * kPanel + off, 1024),
+                             tc::shape(128, C, 1), add);
+              add = true;
+            }
+        tc::products_done(&done_scores);
+        add = false;
+        for (int x = 0; x < P; ++x)
+          for (int y = 0; y < SP && x + y < 3; ++y)
+            for (int d = 0; d < depth; ++d) {
+              tc::product_16(tmem + kFromState + (i & 1) * kTile,
+                             tc::operand(sm + L::q + x * PANELS * kPanel + (d >> 2) * kPanel +
+                                             (d & 3) * 32,
+                                         1024),
+                             tc::operand(sm + L::state + y * L::kState + d * 2048, 1024),
+                             tc::shape(128, kTile, 1, false, true), add);
+              add = true;
+            }
+        tc::products_done(&done_q);
+      }
+      bool add = false;
+      for (int x = 0; x < P; ++x)
+        for (int y = 0; y < kWeighted && x + y < 3; ++y)
+          for (int d = 0; d < C / 16; ++d) {
+            tc::product_16(tmem + kAdded,
+                           tc::operand(k + x * PANELS * kPanel + d * 2048, 1024, kPanel),
+                           tc::operand(sm + L::weighted + y * kPanel + d * 2048, 1024),
+                           tc::shape(128, kTile, 1, true, true), add);
+            add = true;
+          }
+      tc::products_done(&done_state);
+    }
+    __syncwarp();
+  };
+  // Chunk i's output, once its products are there.
+  const auto finish = [&](int i) {
+    const int c = chunk(i), count = tokens(c);
+    tc::barrier_wait_warp(&done_out, i & 1, tries);
+    tc::fence_after();
+    uint32_t x[32], y[32];
+    tc::tmem_load<32>(x, mine + kFromState + (i & 1) * kTile + half * 32);
+    tc::tmem_load<32>(y, mine + kOut + half * 32);
+    tc::loads_done();
+    if (row >= count) return;
+    const float by = a.reverse ? power[count - 1 - row] : a.scale * power[row + 1];
+    float f[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      f[j] = fmaf(__uint_as_float(x[j]), by, a.scale * __uint_as_float(y[j]));
+      const int first = bad[i % 3][half * 32 + j];
+      if (first >= 0 && (a.reverse ? row <= first : row >= C - 1 - first) || !tries)
+        f[j] = __int_as_float(0x7fffffff);
+    }
+    O* out = static_cast<O*>(a.out) + b * a.out_batch + ((int64_t)c * C + row) * a.out_token +
+             (int64_t)h * a.dv + sc0;
+#pragma unroll
+    for (int j = 0; j < 32; j += 8)
+      if (sc0 + j < a.dv) store_pack<O, 8>(out + j, f + j, a.dv - sc0 - j, a.vec_out);
+  };
+
+  if (steps > 0) begin(0);
+#pragma unroll 1
+  for (int i = 0; i < steps; ++i) {
+    const int c = chunk(i), count = tokens(c), at = AHEAD ? i & 1 : 0;
+    if (!STATE) {
+      if (AHEAD && i > 0) {
+        finish(i - 1);
+        if (threadIdx.x == 0 && i + 1 < steps) fetch_v(i + 1);  // the last product with that place is done
+        __syncwarp();
+      }
+      // the triangle's weights
+      tc::barrier_wait_warp(&done_scores, i & 1, tries);
+      tc::fence_after();
+#pragma unroll
+      for (int x = 0; x < C / 64; ++x) {
+        const int block = half * (C / 64) + x;
+        if (quarter * 32 >= C) break;
+        uint32_t r[32], parts[16][SP];
+        tc::tmem_load<32>(r, mine + kScores + block * 32);
+        tc::loads_done();
+        const bool none = a.reverse ? block < quarter : block > quarter;
+        if (none) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+#pragma unroll
+            for (int k = 0; k < SP; ++k) parts[j][k] = 0;
+        } else if (block == quarter) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            const int d0 = a.reverse ? j - lane : lane - j, d1 = a.reverse ? d0 + 1 : d0 - 1;
+            split2<SP>(parts[j / 2], d0 >= 0 ? __uint_as_float(r[j]) * power[max(d0, 0)] : 0.f,
+                       d1 >= 0 ? __uint_as_float(r[j + 1]) * power[max(d1, 0)] : 0.f);
+          }
+        } else {
+          const float f = power[a.reverse ? block * 32 - row : row - block * 32 - 31];
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const float4 w = *reinterpret_cast<const float4*>(column + j);
+            split2<SP>(parts[j / 2], __uint_as_float(r[j]) * (f * w.x),
+                       __uint_as_float(r[j + 1]) * (f * w.y));
+            split2<SP>(parts[j / 2 + 1], __uint_as_float(r[j + 2]) * (f * w.z),
+                       __uint_as_float(r[j + 3]) * (f * w.w));
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < SP; ++k) {
+          uint32_t o[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) o[j] = parts[j][k];
+          tc::tmem_store(mine + kTriangle + k * (C / 2) + block * 16, o);
+        }
+      }
+      tc::stores_to_tmem_done();
+      tc::fence_before();
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        tc::fence_after();
+        const uint8_t* v = sm + L::v + at * L::kValues;
+        bool add = false;
+        for (int x = 0; x < SP; ++x)
+          for (int y = 0; y < P && x + y < 3; ++y)
+            for (int d = 0; d < C / 16; ++d) {
+              tc::product_16_from_tmem(tmem + kOut, tmem + kTriangle + x * (C / 2) + d * 8,
+                                       tc::operand(v + y * kPanel + d * 2048, 1024),
+                                       tc::shape(128, kTile, 1, false, true), add);
+              add = true;
+            }
+        tc::products_done(&done_out);
+        if (AHEAD && i + 1 < steps) {
+          tc::barrier_wait(&done_q, i & 1, tries);
+          fetch_q(i + 1);
+        }
+      }
+      tries = __all_sync(0xffffffffu, tries != 0) ? tries : 0;
+    }
+    // the state behind the chunk
+    tc::barrier_wait_warp(&done_state, i & 1, tries);
+    tc::fence_after();
+    uint32_t x[32];
+    tc::tmem_load<32>(x, mine + kAdded + half * 32);
+    tc::loads_done();
+    tc::fence_before();
+    if (AHEAD && threadIdx.x == 0 && i + 2 < steps) {
+      fetch_k(i + 2);
+      if (STATE) fetch_v(i + 2);
+    }
+    __syncwarp();
+    const float l = power[count], by = a.reverse ? a.scale : 1.f;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      s[j] = fmaf(s[j], l, by * __uint_as_float(x[j]));
+      if (bad[i % 3][half * 32 + j] >= 0) s[j] = __int_as_float(0x7fffffff);
+    }
+    if (!STATE && !AHEAD) finish(i);
+    if (i + 1 < steps) {
+      if (!STATE) {
+        tc::barrier_wait_warp(&done_q, i & 1, tries);
+        store_state(0);
+      }
+      begin(i + 1);
+    }
+  }
+  if (!STATE && AHEAD && steps > 0) finish(steps - 1);
+
+  const bool last = a.reverse ? seg == 0 : (c1 == chunks && (c0 < chunks || seg == 0));
+  float* to = STATE ? a.seg_states + ((int64_t)bh * a.segments + seg) * a.dk * a.dv
+                    : last && a.final ? a.final + state_at : nullptr;
+  if (to && row < a.dk) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (sc0 + j < a.dv)
+        to[(int64_t)row * a.dv + sc0 + j] = tries ? s[j] : __int_as_float(0x7fffffff);
+  }
+  if (!STATE) {
+    // tokens behind the row's end
+    const int end = min(a.len, (seg + 1) * a.seg_chunks * C);
+    for (int64_t t = max(n, seg * a.seg_chunks * C) + warp; t < end; t += kThreads / 32)
+      for (int j = lane; j < cols; j += 32)
+        static_cast<O*>(a.out)[b * a.out_batch + t * a.out_token + (int64_t)h * a.dv + col0 + j] =
+            from_f32<O>(0.f);
+  }
+  tc::fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc::fence_after();
+    tc::tmem_free(tmem, 512);
+  }
 }
 
 // Adds up what the heads that share a key head gave: (batch, len, kv, share, dim) of float32 to
@@ -108,13 +537,101 @@ __global__ void __launch_bounds__(256) sum_heads_kernel(const float* from, T* to
   }
 }
 
-template <typename T, typename O>
-cudaError_t run_pass(const Pass& p, cudaStream_t st, int* launches) {
-  const int64_t blocks = (int64_t)p.batch * p.heads * ((p.dv + 31) / 32);
-  if (!blocks) return cudaSuccess;
-  attention_simple_kernel<T, O><<<(unsigned)blocks, 256, 0, st>>>(p);
+// Boxes of `high` tokens x 64 columns of one head.
+bool head_map(CUtensorMap* map, const Rows& r, int dim, int heads, int len, int batch, int high) {
+  const tc::EncodeTiled f = tc::encoder();
+  if (!f || !aligned16(r.p) || dim % 8) return false;
+  const int64_t token = len > 1 ? r.token * 2 : 16, row = batch > 1 ? r.batch * 2 : 16;
+  if (token % 16 || row % 16 || token < 16 || row < 16 || token >= tc::kMostStride ||
+      row >= tc::kMostStride)
+    return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)dim, (cuuint64_t)(heads / r.share), (cuuint64_t)len,
+                              (cuuint64_t)batch};
+  const cuuint64_t strides[3] = {(cuuint64_t)dim * 2, (cuuint64_t)token, (cuuint64_t)row};
+  const cuuint32_t box[4] = {64, 1, (cuuint32_t)high, 1}, unit[4] = {1, 1, 1, 1};
+  return f(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(r.p), dims, strides, box, unit,
+           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+           CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, typename O, int PANELS, bool AHEAD, bool STATE>
+cudaError_t start(const CUtensorMap (&maps)[3], const Pass& p, int64_t blocks, cudaStream_t st,
+                  int* launches) {
+  const auto kernel = attention_kernel<T, O, PANELS, AHEAD, STATE>;
+  constexpr int bytes = Layout<T, PANELS, AHEAD>::bytes;
+  const cudaError_t e =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return e;
+  kernel<<<(unsigned)blocks, kThreads, bytes, st>>>(maps[0], maps[1], maps[2], p);
   ++*launches;
   return cudaGetLastError();
+}
+
+// Segments of a row: the number that needs the least time in rounds of resident blocks (one an SM),
+// counted in chunks; a first pass over all but the last segment costs about half a chunk's time.
+int segments_of(int64_t blocks, int chunks) {
+  int best = 1;
+  double least = 1e300;
+  for (int s = 1; s <= 64 && s <= chunks; ++s) {
+    const int each = (chunks + s - 1) / s;
+    if (s > 1 && (chunks + each - 1) / each != s) continue;
+    const double rounds = (double)((blocks * s + 147) / 148) * each;
+    const double first = s == 1 ? 0 : (double)((blocks * s + 147) / 148) * each * 0.5 + 2;
+    if (rounds + first < least) least = rounds + first, best = s;
+  }
+  return best;
+}
+template <typename T>
+int pass_segments(int batch, int heads, int dv, int len) {
+  const int64_t blocks = (int64_t)batch * heads * ((dv + kTile - 1) / kTile);
+  return blocks ? segments_of(blocks, (len + chunk_of<T>() - 1) / chunk_of<T>()) : 1;
+}
+size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+size_t segment_bytes(int type, int batch, int heads, int dk, int dv, int len) {
+  int s = 1;
+  SALT_WITH_TYPE(type, T, s = pass_segments<T>(batch, heads, dv, len));
+  return s == 1 ? 0 : align256(sizeof(float) * batch * heads * s * dk * dv);
+}
+
+template <typename T, typename O, int PANELS, bool AHEAD>
+cudaError_t run_ahead(const CUtensorMap (&maps)[3], const Pass& p, int64_t blocks, cudaStream_t st,
+                      int* launches) {
+  if (p.segments > 1) {
+    Pass first = p;
+    first.initial = nullptr;
+    const cudaError_t e =
+        start<T, O, PANELS, AHEAD, true>(maps, first, blocks * p.segments, st, launches);
+    if (e != cudaSuccess) return e;
+  }
+  return start<T, O, PANELS, AHEAD, false>(maps, p, blocks * p.segments, st, launches);
+}
+
+// `ws` holds segment_bytes.
+template <typename T, typename O>
+cudaError_t run_pass(Pass p, void* ws, cudaStream_t st, int* launches) {
+  constexpr int C = chunk_of<T>();
+  const int64_t blocks = (int64_t)p.batch * p.heads * ((p.dv + kTile - 1) / kTile);
+  if (!blocks) return cudaSuccess;
+  const int chunks = (p.len + C - 1) / C;
+  p.segments = pass_segments<T>(p.batch, p.heads, p.dv, p.len);
+  p.seg_chunks = std::max(1, (chunks + p.segments - 1) / p.segments);
+  p.seg_states = static_cast<float*>(ws);
+  const auto packed = [&](const Rows& r, int dim) {
+    return pack_rows(r.p, 8, sizeof(T), r.batch, r.token) && dim * sizeof(T) % 16 == 0;
+  };
+  p.vec = packed(p.q, p.dk) && packed(p.k, p.dk) && packed(p.v, p.dv);
+  p.vec_out = packed_rows(p.out, 16, sizeof(O), p.out_batch, p.out_token) &&
+              p.dv * sizeof(O) % 16 == 0;
+  CUtensorMap maps[3] = {};
+  if constexpr (parts_of<T>() == 1) {
+    if (p.len > 0 && head_map(&maps[0], p.q, p.dk, p.heads, p.len, p.batch, C) &&
+        head_map(&maps[1], p.k, p.dk, p.heads, p.len, p.batch, C) &&
+        head_map(&maps[2], p.v, p.dv, p.heads, p.len, p.batch, C))
+      return p.dk <= 64 ? run_ahead<T, O, 1, true>(maps, p, blocks, st, launches)
+                        : run_ahead<T, O, 2, true>(maps, p, blocks, st, launches);
+  }
+  return p.dk <= 64 ? run_ahead<T, O, 1, false>(maps, p, blocks, st, launches)
+                    : run_ahead<T, O, 2, false>(maps, p, blocks, st, launches);
 }
 
 template <typename T>
@@ -142,13 +659,13 @@ __global__ void __launch_bounds__(128) attention_step_kernel(salt_linear_attenti
   out[col] = from_f32<T>(a.scale * acc);
 }
 
-size_t align256(size_t n) { return (n + 255) / 256 * 256; }
-
 }  // namespace
 
-size_t linear_attention_bytes(const salt_linear_attention_args&) { return 0; }
+size_t linear_attention_bytes(const salt_linear_attention_args& a) {
+  return segment_bytes(a.type, a.batch, a.heads, a.dim_k, a.dim_v, a.len);
+}
 
-cudaError_t linear_attention_launch(const salt_linear_attention_args& a, void*, cudaStream_t st,
+cudaError_t linear_attention_launch(const salt_linear_attention_args& a, void* ws, cudaStream_t st,
                                     int* launches) {
   const int share = a.heads / a.kv_heads;
   Pass p{{a.q, a.q_batch_stride, a.q_stride, 1},
@@ -157,7 +674,7 @@ cudaError_t linear_attention_launch(const salt_linear_attention_args& a, void*, 
          a.dim_k, a.dim_v, a.heads, a.len, a.batch, a.scale, false, a.log_decay, a.n_real,
          a.initial_state, false, a.out, a.out_batch_stride, a.out_stride, a.final_state};
   cudaError_t e = cudaSuccess;
-  SALT_WITH_TYPE(a.type, T, e = (run_pass<T, T>(p, st, launches)));
+  SALT_WITH_TYPE(a.type, T, e = (run_pass<T, T>(p, ws, st, launches)));
   return e;
 }
 
@@ -170,8 +687,11 @@ cudaError_t linear_attention_step_launch(const salt_linear_attention_step_args& 
 }
 
 size_t linear_attention_backward_bytes(const salt_linear_attention_backward_args& a) {
-  if (a.heads == a.kv_heads) return 0;
-  return align256(4ull * a.batch * a.len * a.heads * std::max(a.dim_k, a.dim_v));
+  // segments' states of one pass after the other, and parts of dk, then of dv
+  const size_t states = std::max(segment_bytes(a.type, a.batch, a.heads, a.dim_v, a.dim_k, a.len),
+                                 segment_bytes(a.type, a.batch, a.heads, a.dim_k, a.dim_v, a.len));
+  if (a.heads == a.kv_heads) return states;
+  return states + align256(sizeof(float) * a.batch * a.len * a.heads * std::max(a.dim_k, a.dim_v));
 }
 
 cudaError_t linear_attention_backward_launch(const salt_linear_attention_backward_args& a, void* ws,
@@ -185,25 +705,29 @@ cudaError_t linear_attention_backward_launch(const salt_linear_attention_backwar
           a.dfinal, true, a.dk, a.dk_batch_stride, a.dk_stride, nullptr};
   Pass dv{k, q, d, a.dim_k, a.dim_v, a.heads, a.len, a.batch, a.scale, true, a.log_decay, a.n_real,
           a.dfinal, false, a.dv, a.dv_batch_stride, a.dv_stride, a.dinitial};
+  float* parts = reinterpret_cast<float*>(
+      static_cast<uint8_t*>(ws) +
+      std::max(segment_bytes(a.type, a.batch, a.heads, a.dim_v, a.dim_k, a.len),
+               segment_bytes(a.type, a.batch, a.heads, a.dim_k, a.dim_v, a.len)));
   cudaError_t e = cudaSuccess;
   SALT_WITH_TYPE(a.type, T, {
-    e = run_pass<T, T>(dq, st, launches);
+    e = run_pass<T, T>(dq, ws, st, launches);
     for (Pass* p : {&dk, &dv}) {
       if (e != cudaSuccess) return e;
       if (share == 1) {
-        e = run_pass<T, T>(*p, st, launches);
+        e = run_pass<T, T>(*p, ws, st, launches);
         continue;
       }
       T* to = static_cast<T*>(p->out);
       const int64_t to_batch = p->out_batch, to_token = p->out_token;
-      p->out = ws;
+      p->out = parts;
       p->out_token = (int64_t)a.heads * p->dv;
       p->out_batch = p->out_token * a.len;
-      e = run_pass<T, float>(*p, st, launches);
+      e = run_pass<T, float>(*p, ws, st, launches);
       const int64_t n = (int64_t)a.batch * a.len * a.kv_heads * p->dv;
       if (e != cudaSuccess || !n) continue;
       sum_heads_kernel<T><<<(unsigned)std::min<int64_t>((n + 255) / 256, 148 * 8), 256, 0, st>>>(
-          static_cast<const float*>(ws), to, (int64_t)a.batch * a.len, a.len, a.kv_heads, share,
+          parts, to, (int64_t)a.batch * a.len, a.len, a.kv_heads, share,
           p->dv, to_batch, to_token);
       ++*launches;
       e = cudaGetLastError();

@@ -373,25 +373,9 @@ __global__ void __launch_bounds__(256) align_rows_kernel(const uint8_t* from, in
 
 // ---------------------------------------------------------------- host
 
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                 const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiled encoder() {
-  static const EncodeTiled f = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult found;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault,
-                                         &found) != cudaSuccess ||
-        found != cudaDriverEntryPointSuccess)
-      p = nullptr;
-    return reinterpret_cast<EncodeTiled>(p);
-  }();
-  return f;
-}
-
-constexpr int64_t kMostStride = 1ll << 39;  // a tensor map's strides lie under 2^40
+using tc::encoder;
+using tc::EncodeTiled;
+using tc::kMostStride;
 
 // Boxes of 128 bytes x `high` rows; what lies past k or the rows reads as zero.
 bool tile_map(CUtensorMap* map, const void* p, int64_t rows, int64_t k, int64_t stride, int high) {

@@ -101,6 +101,15 @@ __device__ __forceinline__ void stores_read() {
 __device__ __forceinline__ void stores_done() {
   asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
+// The same of an array of four axes: box (inner, 1, rows, 1) from (x, y, z, w).
+__device__ __forceinline__ void load_box4(void* to, const CUtensorMap* map, int x, int y, int z, int w,
+                                          uint64_t* barrier) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+      "%3, %4, %5}], [%6];" ::"r"(shared_at(to)),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(shared_at(barrier))
+      : "memory");
+}
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
@@ -172,6 +181,19 @@ __device__ __forceinline__ void tmem_load(uint32_t (&r)[N], uint32_t at) {
   }
 }
 
+__device__ __forceinline__ void stores_to_tmem_done() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+// 16 columns of the warp's 32 rows from registers.
+__device__ __forceinline__ void tmem_store(uint32_t at, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
 // ---------------------------------------------------------------- products
 
 // An operand in shared memory in rows of 128 bytes, swizzled by 128 bytes (the 16-byte unit of row r
@@ -209,6 +231,15 @@ __device__ __forceinline__ void product_16(uint32_t d, uint64_t a, uint64_t b, u
       "l"(a), "l"(b), "r"(shape), "r"((uint32_t)add)
       : "memory");
 }
+// The same with a in tensor memory: a row a lane, two 16-bit values a column.
+__device__ __forceinline__ void product_16_from_tmem(uint32_t d, uint32_t a, uint64_t b,
+                                                     uint32_t shape, bool add) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+      "r"(a), "l"(b), "r"(shape), "r"((uint32_t)add)
+      : "memory");
+}
 // The barrier's arrival once all products that this thread issued are done.
 __device__ __forceinline__ void products_done(uint64_t* barrier) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
@@ -221,5 +252,27 @@ __device__ __forceinline__ bool one_lane() {
                : "=r"(is));
   return is;
 }
+
+// ---------------------------------------------------------------- host
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                 const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// The driver's encoder of tensor maps; NULL where it has none.
+inline EncodeTiled encoder() {
+  static const EncodeTiled f = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault,
+                                         &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<EncodeTiled>(p);
+  }();
+  return f;
+}
+constexpr int64_t kMostStride = 1ll << 39;  // bytes: a tensor map's strides lie under 2^40
 
 }  // namespace salt::tc
