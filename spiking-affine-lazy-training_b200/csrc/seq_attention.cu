@@ -46,7 +46,8 @@ __device__ __forceinline__ const T* row_of(const Rows& r, int b, int64_t t, int 
 }
 
 constexpr int kTile = 64;      // columns of v that a block takes
-constexpr int kThreads = 256;  // 8 warps: two for each 32 rows of tensor memory
+constexpr int kWorkers = 512;  // 16 warps: four for each 32 rows of tensor memory
+constexpr int kThreads = kWorkers + 32;  // and one for the copies and the products
 constexpr int kWeighted = 3;   // parts of a weighted v
 
 // A type's values in parts of bfloat16, 8 bits each: what the tensor cores multiply.
@@ -88,7 +89,7 @@ template <typename T, int PANELS, int C>
 __device__ __forceinline__ void load_rows(uint8_t* to, const T* p, int64_t stride, int count, int from,
                                           int dim, bool vec) {
   constexpr int P = parts_of<T>(), U = PANELS * 8;
-  for (int i = threadIdx.x; i < C * U; i += kThreads) {
+  for (int i = threadIdx.x; i < C * U; i += kWorkers) {
     const int row = i / U, u = i % U, at = from + u * 8;
     const Pack<T, 8> x = load_pack<T, 8>(p + row * stride + at, row < count ? dim - at : 0, vec);
     uint32_t parts[4][P];
@@ -122,13 +123,15 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   constexpr int kPanel = L::kPanel;
   extern __shared__ uint8_t raw[];
   uint8_t* sm = raw + (1024 - tc::shared_at(raw) % 1024) % 1024;
-  __shared__ uint64_t loaded_q, loaded_k[2], loaded_v[2], done_q, done_scores, done_state, done_out;
+  __shared__ uint64_t loaded_q, loaded_k[2], loaded_v[2];  // copies
+  __shared__ uint64_t done_scores, done_q, done_state, done_out;  // products
+  __shared__ uint64_t ready_chunk, ready_triangle;  // operands that threads wrote
   __shared__ uint32_t tmem_at;
-  __shared__ float power[C + 1];               // l^i
-  __shared__ __align__(16) float column[32];   // of a column within its 32
-  __shared__ int bad[3][kTile];                // the outermost token whose v is not finite
+  __shared__ float power[C + 1];              // l^i
+  __shared__ __align__(16) float column[32];  // of a column within its 32
+  __shared__ int bad[3][kTile];               // the outermost token whose v is not finite
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane;
+  const int quarter = warp & 3, part = warp >> 2, row = quarter * 32 + lane;
 
   const int tiles = (a.dv + kTile - 1) / kTile;
   int id = blockIdx.x;
@@ -139,15 +142,19 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   const int c0 = min(seg * a.seg_chunks, chunks);
   // (nobody needs what the last segment alone adds to the state)
   const bool needed = !STATE || seg != (a.reverse ? 0 : a.segments - 1);
-  const int c1 = needed ? min(c0 + a.seg_chunks, chunks) : c0;
+  const int c1 = needed ? min(c0 + a.seg_chunks, chunks) : c0, steps = c1 - c0;
   const int col0 = tile * kTile, cols = min(kTile, a.dv - col0);
   const float g = decay_of(a.log_decay, h) * kLog2e;
   const int64_t state_at = (int64_t)bh * a.dk * a.dv;
+  const auto chunk = [&](int i) { return a.reverse ? c1 - 1 - i : c0 + i; };
+  const auto tokens = [&](int c) { return min(C, n - c * C); };
 
   if (threadIdx.x == 0) {
-    uint64_t* all[] = {&loaded_q, &loaded_k[0], &loaded_k[1], &loaded_v[0], &loaded_v[1],
-                       &done_q,   &done_scores, &done_state,  &done_out};
-    for (uint64_t* x : all) tc::barrier_init(x, 1);
+    uint64_t* ones[] = {&loaded_q, &loaded_k[0], &loaded_k[1], &loaded_v[0], &loaded_v[1],
+                        &done_q,   &done_scores, &done_state,  &done_out};
+    for (uint64_t* x : ones) tc::barrier_init(x, 1);
+    tc::barrier_init(&ready_chunk, kWorkers / 32);
+    tc::barrier_init(&ready_triangle, kWorkers / 32);
     tc::barrier_init_fence();
   }
   if (warp == 0) tc::tmem_alloc(&tmem_at, 512);
@@ -163,353 +170,383 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   const uint32_t tmem = tmem_at, mine = tmem + ((uint32_t)(quarter * 32) << 16);
   // columns of tensor memory
   constexpr int kScores = 0, kTriangle = 128, kFromState = 256, kOut = 384, kAdded = 448;
-
-  // this thread's part of the state: row `row`, 32 columns
-  float s[32];
-  const int sc0 = col0 + half * 32;
-#pragma unroll
-  for (int j = 0; j < 32; ++j)
-    s[j] = a.initial && row < a.dk && sc0 + j < a.dv
-               ? a.initial[state_at + (a.initial_t ? (int64_t)(sc0 + j) * a.dk + row
-                                                   : (int64_t)row * a.dv + sc0 + j)]
-               : 0.f;
-  if (a.segments > 1 && !STATE) {
-    // the states that the segments in front left behind, each from zero
-    const int before = a.reverse ? a.segments - 1 - seg : seg;
-    for (int i = 0; i < before; ++i) {
-      const int at = a.reverse ? a.segments - 1 - i : i;
-      const int first = at * a.seg_chunks * C, count = min(first + a.seg_chunks * C, n) - first;
-      if (count <= 0) continue;
-      const float l = exp2f(g * (float)count);
-      const float* from = a.seg_states + ((int64_t)bh * a.segments + at) * a.dk * a.dv;
-#pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (row < a.dk && sc0 + j < a.dv)
-          s[j] = fmaf(s[j], l, from[(int64_t)row * a.dv + sc0 + j]);
-    }
-  }
-  const auto store_state = [&](int x) {  // as an operand
-    if (row >= DK) return;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      uint32_t parts[4][SP];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) split2<SP>(parts[k], s[8 * u + 2 * k], s[8 * u + 2 * k + 1]);
-#pragma unroll
-      for (int j = 0; j < SP; ++j)
-        *reinterpret_cast<uint4*>(sm + L::state + j * L::kState + row * 128 +
-                                  (((half * 4 + u) ^ (row & 7)) << 4)) =
-            make_uint4(parts[0][j], parts[1][j], parts[2][j], parts[3][j]);
-    }
-  };
-  const int steps = c1 - c0;
   uint32_t tries = tc::kTries;
-  const auto chunk = [&](int i) { return a.reverse ? c1 - 1 - i : c0 + i; };
-  const auto tokens = [&](int c) { return min(C, n - c * C); };
-  // copies ahead, by thread 0
-  const auto fetch_q = [&](int i) {
-    tc::barrier_expect(&loaded_q, L::kKeys);
-    for (int x = 0; x < PANELS; ++x)
-      tc::load_box4(sm + L::q + x * kPanel, &map_q, x * 64, h / a.q.share, chunk(i) * C, b, &loaded_q);
-  };
-  const auto fetch_k = [&](int i) {
-    tc::barrier_expect(&loaded_k[i & 1], L::kKeys);
-    for (int x = 0; x < PANELS; ++x)
-      tc::load_box4(sm + L::k + (i & 1) * L::kKeys + x * kPanel, &map_k, x * 64, h / a.k.share,
-                    chunk(i) * C, b, &loaded_k[i & 1]);
-  };
-  const auto fetch_v = [&](int i) {
-    tc::barrier_expect(&loaded_v[i & 1], L::kValues);
-    tc::load_box4(sm + L::v + (i & 1) * L::kValues, &map_v, col0, h / a.v.share, chunk(i) * C, b,
-                  &loaded_v[i & 1]);
-  };
-  if (AHEAD && threadIdx.x == 0 && steps > 0) {
-    if (!STATE) fetch_q(0);
-    fetch_k(0);
-    fetch_v(0);
-    if (steps > 1) {
-      fetch_k(1);
-      fetch_v(1);
-    }
-  }
-  if (!STATE && steps > 0) store_state(0);
 
-  // Chunk i's operands: brought in where nobody copied ahead, rows past the end made zero, values
-  // weighted; then its products that need no others' results.
-  const auto begin = [&](int i) {
-    const int c = chunk(i), count = tokens(c), at = AHEAD ? i & 1 : 0;
-    uint8_t* k = sm + L::k + at * L::kKeys;
-    uint8_t* v = sm + L::v + at * L::kValues;
-    if (AHEAD) {
-      tc::barrier_wait_warp(&loaded_v[at], i >> 1 & 1, tries);
-      tc::barrier_wait_warp(&loaded_k[at], i >> 1 & 1, tries);
-      if (!STATE) tc::barrier_wait_warp(&loaded_q, i & 1, tries);
-      if (count < C) {
-        for (int x = threadIdx.x; x < (C - count) * PANELS * 8; x += kThreads) {
-          const int r = count + x / (PANELS * 8), u = x % (PANELS * 8);
-          *reinterpret_cast<uint4*>(k + (u >> 3) * kPanel + r * 128 + ((u & 7) << 4)) =
-              make_uint4(0, 0, 0, 0);
-        }
-      }
-    } else {
-      const int64_t t = (int64_t)c * C;
-      if (!STATE)
-        load_rows<T, PANELS, C>(sm + L::q, row_of<T>(a.q, b, t, h, a.dk), a.q.token, count, 0, a.dk,
-                                a.vec);
-      load_rows<T, PANELS, C>(k, row_of<T>(a.k, b, t, h, a.dk), a.k.token, count, 0, a.dk, a.vec);
-      load_rows<T, 1, C>(v, row_of<T>(a.v, b, t, h, a.dv), a.v.token, count, col0, a.dv, a.vec);
-      __syncthreads();
-    }
-    for (int x = threadIdx.x; x < C * 8; x += kThreads) {
-      const int r = x >> 3, u = x & 7;
-      uint8_t* place = v + r * 128 + ((u ^ (r & 7)) << 4);
-      const float w = r >= count ? 0.f : power[a.reverse ? r + 1 : count - 1 - r];
-      uint32_t in[P][4], out[4][kWeighted];
-      bool fine = true;
-#pragma unroll
-      for (int j = 0; j < P; ++j) {
-        const uint4 y = *reinterpret_cast<const uint4*>(place + j * kPanel);
-        in[j][0] = y.x, in[j][1] = y.y, in[j][2] = y.z, in[j][3] = y.w;
-      }
-      if (r >= count) {
-#pragma unroll
-        for (int j = 0; j < P; ++j) {
-          in[j][0] = in[j][1] = in[j][2] = in[j][3] = 0;
-          *reinterpret_cast<uint4*>(place + j * kPanel) = make_uint4(0, 0, 0, 0);
-        }
-      }
-      // A value that is not finite would reach the tokens on the triangle's other side, as 0 * it:
-      // it becomes zero here, and its column NaN from its token on.
-#pragma unroll
-      for (int m = 0; m < 4; ++m)
-        fine &= (in[0][m] & 0x7f80u) != 0x7f80u && (in[0][m] & 0x7f800000u) != 0x7f800000u;
-      if (!fine) {
-#pragma unroll
-        for (int m = 0; m < 8; ++m) {
-          const uint32_t mask = 0xffffu << (m & 1) * 16, exponent = 0x7f80u << (m & 1) * 16;
-          if ((in[0][m / 2] & exponent) != exponent) continue;
-          if (a.reverse)
-            atomicMax(&bad[i % 3][u * 8 + m], r);
-          else
-            atomicMax(&bad[i % 3][u * 8 + m], C - 1 - r);
-#pragma unroll
-          for (int j = 0; j < P; ++j) in[j][m / 2] &= ~mask;
-        }
-#pragma unroll
-        for (int j = 0; j < P; ++j)
-          *reinterpret_cast<uint4*>(place + j * kPanel) =
-              make_uint4(in[j][0], in[j][1], in[j][2], in[j][3]);
-      }
-#pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        float lo = __uint_as_float(in[0][m] << 16), hi = __uint_as_float(in[0][m] & 0xffff0000u);
-#pragma unroll
-        for (int j = 1; j < P; ++j) {
-          lo += __uint_as_float(in[j][m] << 16);
-          hi += __uint_as_float(in[j][m] & 0xffff0000u);
-        }
-        split2<kWeighted>(out[m], w * lo, w * hi);
-      }
-      uint8_t* to = sm + L::weighted + (place - v);
-#pragma unroll
-      for (int j = 0; j < kWeighted; ++j)
-        *reinterpret_cast<uint4*>(to + j * kPanel) =
-            make_uint4(out[0][j], out[1][j], out[2][j], out[3][j]);
-    }
-    if (threadIdx.x < kTile) bad[(i + 1) % 3][threadIdx.x] = -1;
-    tc::fence_shared();
-    tc::fence_before();
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      tc::fence_after();
+  if (warp == kWorkers / 32) {
+    if (tc::one_lane() && steps > 0) {
+      const auto fetch_q = [&](int i) {
+        if (i >= steps) return;
+        tc::barrier_expect(&loaded_q, L::kKeys);
+        for (int x = 0; x < PANELS; ++x)
+          tc::load_box4(sm + L::q + x * kPanel, &map_q, x * 64, h / a.q.share, chunk(i) * C, b,
+                        &loaded_q);
+      };
+      const auto fetch_k = [&](int i) {
+        if (i >= steps) return;
+        tc::barrier_expect(&loaded_k[i & 1], L::kKeys);
+        for (int x = 0; x < PANELS; ++x)
+          tc::load_box4(sm + L::k + (i & 1) * L::kKeys + x * kPanel, &map_k, x * 64,
+                        h / a.k.share, chunk(i) * C, b, &loaded_k[i & 1]);
+      };
+      const auto fetch_v = [&](int i) {
+        if (i >= steps) return;
+        tc::barrier_expect(&loaded_v[i & 1], L::kValues);
+        tc::load_box4(sm + L::v + (i & 1) * L::kValues, &map_v, col0, h / a.v.share, chunk(i) * C, b,
+                      &loaded_v[i & 1]);
+      };
       const int depth = (a.dk + 15) / 16;
-      if (!STATE) {
+      const uint64_t q = tc::operand(sm + L::q, 1024), state = tc::operand(sm + L::state, 1024),
+                     weighted = tc::operand(sm + L::weighted, 1024);
+      const auto scores = [&](int i) {
+        const uint64_t k = tc::operand(sm + L::k + (AHEAD ? i & 1 : 0) * L::kKeys, 1024);
         bool add = false;
+#pragma unroll
         for (int x = 0; x < P; ++x)
+#pragma unroll
           for (int y = 0; y < P && x + y < 3; ++y)
             for (int d = 0; d < depth; ++d) {
-              const int off = (d >> 2) * kPanel + (d & 3) * 32;
-              tc::product_16(tmem + kScores,
-                             tc::operand(sm + L::q + x * PANELS * kPanel + off, 1024),
-                             tc::operand(k + y * PANELS * kPanel + off, 1024),
-                             tc::shape(128, C, 1), add);
+              const uint32_t off = (d >> 2) * kPanel + (d & 3) * 32;
+              tc::product_16(tmem + kScores, tc::further(q, x * PANELS * kPanel + off),
+                             tc::further(k, y * PANELS * kPanel + off), tc::shape(128, C, 1), add);
               add = true;
             }
         tc::products_done(&done_scores);
-        add = false;
-        for (int x = 0; x < P; ++x)
-          for (int y = 0; y < SP && x + y < 3; ++y)
-            for (int d = 0; d < depth; ++d) {
-              tc::product_16(tmem + kFromState + (i & 1) * kTile,
-                             tc::operand(sm + L::q + x * PANELS * kPanel + (d >> 2) * kPanel +
-                                             (d & 3) * 32,
-                                         1024),
-                             tc::operand(sm + L::state + y * L::kState + d * 2048, 1024),
-                             tc::shape(128, kTile, 1, false, true), add);
-              add = true;
-            }
-        tc::products_done(&done_q);
+      };
+      if (AHEAD) {
+        fetch_v(0);
+        fetch_k(0);
+        if (!STATE) fetch_q(0);
+        fetch_v(1);
+        fetch_k(1);
+        tc::barrier_wait(&loaded_k[0], 0, tries);
+        if (!STATE) {
+          tc::barrier_wait(&loaded_q, 0, tries);
+          scores(0);
+        }
       }
-      bool add = false;
-      for (int x = 0; x < P; ++x)
-        for (int y = 0; y < kWeighted && x + y < 3; ++y)
-          for (int d = 0; d < C / 16; ++d) {
-            tc::product_16(tmem + kAdded,
-                           tc::operand(k + x * PANELS * kPanel + d * 2048, 1024, kPanel),
-                           tc::operand(sm + L::weighted + y * kPanel + d * 2048, 1024),
-                           tc::shape(128, kTile, 1, true, true), add);
-            add = true;
-          }
-      tc::products_done(&done_state);
-    }
-    __syncwarp();
-  };
-  // Chunk i's output, once its products are there.
-  const auto finish = [&](int i) {
-    const int c = chunk(i), count = tokens(c);
-    tc::barrier_wait_warp(&done_out, i & 1, tries);
-    tc::fence_after();
-    uint32_t x[32], y[32];
-    tc::tmem_load<32>(x, mine + kFromState + (i & 1) * kTile + half * 32);
-    tc::tmem_load<32>(y, mine + kOut + half * 32);
-    tc::loads_done();
-    if (row >= count) return;
-    const float by = a.reverse ? power[count - 1 - row] : a.scale * power[row + 1];
-    float f[32];
-#pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      f[j] = fmaf(__uint_as_float(x[j]), by, a.scale * __uint_as_float(y[j]));
-      const int first = bad[i % 3][half * 32 + j];
-      if (first >= 0 && (a.reverse ? row <= first : row >= C - 1 - first) || !tries)
-        f[j] = __int_as_float(0x7fffffff);
-    }
-    O* out = static_cast<O*>(a.out) + b * a.out_batch + ((int64_t)c * C + row) * a.out_token +
-             (int64_t)h * a.dv + sc0;
-#pragma unroll
-    for (int j = 0; j < 32; j += 8)
-      if (sc0 + j < a.dv) store_pack<O, 8>(out + j, f + j, a.dv - sc0 - j, a.vec_out);
-  };
-
-  if (steps > 0) begin(0);
 #pragma unroll 1
-  for (int i = 0; i < steps; ++i) {
-    const int c = chunk(i), count = tokens(c), at = AHEAD ? i & 1 : 0;
-    if (!STATE) {
-      if (AHEAD && i > 0) {
-        finish(i - 1);
-        if (threadIdx.x == 0 && i + 1 < steps) fetch_v(i + 1);  // the last product with that place is done
-        __syncwarp();
-      }
-      // the triangle's weights
-      tc::barrier_wait_warp(&done_scores, i & 1, tries);
-      tc::fence_after();
-#pragma unroll
-      for (int x = 0; x < C / 64; ++x) {
-        const int block = half * (C / 64) + x;
-        if (quarter * 32 >= C) break;
-        uint32_t r[32], parts[16][SP];
-        tc::tmem_load<32>(r, mine + kScores + block * 32);
-        tc::loads_done();
-        const bool none = a.reverse ? block < quarter : block > quarter;
-        if (none) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-#pragma unroll
-            for (int k = 0; k < SP; ++k) parts[j][k] = 0;
-        } else if (block == quarter) {
-#pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            const int d0 = a.reverse ? j - lane : lane - j, d1 = a.reverse ? d0 + 1 : d0 - 1;
-            split2<SP>(parts[j / 2], d0 >= 0 ? __uint_as_float(r[j]) * power[max(d0, 0)] : 0.f,
-                       d1 >= 0 ? __uint_as_float(r[j + 1]) * power[max(d1, 0)] : 0.f);
-          }
-        } else {
-          const float f = power[a.reverse ? block * 32 - row : row - block * 32 - 31];
-#pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            const float4 w = *reinterpret_cast<const float4*>(column + j);
-            split2<SP>(parts[j / 2], __uint_as_float(r[j]) * (f * w.x),
-                       __uint_as_float(r[j + 1]) * (f * w.y));
-            split2<SP>(parts[j / 2 + 1], __uint_as_float(r[j + 2]) * (f * w.z),
-                       __uint_as_float(r[j + 3]) * (f * w.w));
-          }
-        }
-#pragma unroll
-        for (int k = 0; k < SP; ++k) {
-          uint32_t o[16];
-#pragma unroll
-          for (int j = 0; j < 16; ++j) o[j] = parts[j][k];
-          tc::tmem_store(mine + kTriangle + k * (C / 2) + block * 16, o);
-        }
-      }
-      tc::stores_to_tmem_done();
-      tc::fence_before();
-      __syncthreads();
-      if (threadIdx.x == 0) {
+      for (int i = 0; i < steps; ++i) {
+        const int at = AHEAD ? i & 1 : 0;
+        tc::barrier_wait(&ready_chunk, i & 1, tries);
         tc::fence_after();
-        const uint8_t* v = sm + L::v + at * L::kValues;
-        bool add = false;
-        for (int x = 0; x < SP; ++x)
-          for (int y = 0; y < P && x + y < 3; ++y)
-            for (int d = 0; d < C / 16; ++d) {
-              tc::product_16_from_tmem(tmem + kOut, tmem + kTriangle + x * (C / 2) + d * 8,
-                                       tc::operand(v + y * kPanel + d * 2048, 1024),
-                                       tc::shape(128, kTile, 1, false, true), add);
-              add = true;
-            }
-        tc::products_done(&done_out);
+        if (!STATE) {
+          if (!AHEAD) scores(i);
+          bool add = false;
+#pragma unroll
+          for (int x = 0; x < P; ++x)
+#pragma unroll
+            for (int y = 0; y < SP && x + y < 3; ++y)
+              for (int d = 0; d < depth; ++d) {
+                const uint32_t off = (d >> 2) * kPanel + (d & 3) * 32;
+                tc::product_16(tmem + kFromState + (i & 1) * kTile,
+                               tc::further(q, x * PANELS * kPanel + off),
+                               tc::further(state, y * L::kState + d * 2048),
+                               tc::shape(128, kTile, 1, false, true), add);
+                add = true;
+              }
+          tc::products_done(&done_q);
+        }
+        {
+          const uint64_t k = tc::operand(sm + L::k + at * L::kKeys, 1024, kPanel);
+          bool add = false;
+#pragma unroll
+          for (int x = 0; x < P; ++x)
+#pragma unroll
+            for (int y = 0; y < kWeighted && x + y < 3; ++y)
+#pragma unroll
+              for (int d = 0; d < C / 16; ++d) {
+                tc::product_16(tmem + kAdded, tc::further(k, x * PANELS * kPanel + d * 2048),
+                               tc::further(weighted, y * kPanel + d * 2048),
+                               tc::shape(128, kTile, 1, true, true), add);
+                add = true;
+              }
+          tc::products_done(&done_state);
+        }
+        if (!STATE) {
+          if (AHEAD) {
+            tc::barrier_wait(&done_q, i & 1, tries);
+            fetch_q(i + 1);
+          }
+          tc::barrier_wait(&ready_triangle, i & 1, tries);
+          tc::fence_after();
+          const uint64_t v = tc::operand(sm + L::v + at * L::kValues, 1024);
+          bool add = false;
+#pragma unroll
+          for (int x = 0; x < SP; ++x)
+#pragma unroll
+            for (int y = 0; y < P && x + y < 3; ++y)
+#pragma unroll
+              for (int d = 0; d < C / 16; ++d) {
+                tc::product_16_from_tmem(tmem + kOut, tmem + kTriangle + x * (C / 2) + d * 8,
+                                         tc::further(v, y * kPanel + d * 2048),
+                                         tc::shape(128, kTile, 1, false, true), add);
+                add = true;
+              }
+          tc::products_done(&done_out);
+        }
         if (AHEAD && i + 1 < steps) {
-          tc::barrier_wait(&done_q, i & 1, tries);
-          fetch_q(i + 1);
+          tc::barrier_wait(&loaded_k[(i + 1) & 1], (i + 1) >> 1 & 1, tries);
+          if (!STATE) {
+            tc::barrier_wait(&loaded_q, (i + 1) & 1, tries);
+            scores(i + 1);
+          }
+          tc::barrier_wait(&done_state, i & 1, tries);
+          fetch_k(i + 2);
+          if (!STATE) tc::barrier_wait(&done_out, i & 1, tries);
+          fetch_v(i + 2);
         }
       }
-      tries = __all_sync(0xffffffffu, tries != 0) ? tries : 0;
-    }
-    // the state behind the chunk
-    tc::barrier_wait_warp(&done_state, i & 1, tries);
-    tc::fence_after();
-    uint32_t x[32];
-    tc::tmem_load<32>(x, mine + kAdded + half * 32);
-    tc::loads_done();
-    tc::fence_before();
-    if (AHEAD && threadIdx.x == 0 && i + 2 < steps) {
-      fetch_k(i + 2);
-      if (STATE) fetch_v(i + 2);
     }
     __syncwarp();
-    const float l = power[count], by = a.reverse ? a.scale : 1.f;
+  } else {
+    // this thread's part of the state: row `row`, 16 columns
+    float s[16];
+    const int sc0 = col0 + part * 16;
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      s[j] = fmaf(s[j], l, by * __uint_as_float(x[j]));
-      if (bad[i % 3][half * 32 + j] >= 0) s[j] = __int_as_float(0x7fffffff);
-    }
-    if (!STATE && !AHEAD) finish(i);
-    if (i + 1 < steps) {
-      if (!STATE) {
-        tc::barrier_wait_warp(&done_q, i & 1, tries);
-        store_state(0);
+    for (int j = 0; j < 16; ++j)
+      s[j] = a.initial && row < a.dk && sc0 + j < a.dv
+                 ? a.initial[state_at + (a.initial_t ? (int64_t)(sc0 + j) * a.dk + row
+                                                     : (int64_t)row * a.dv + sc0 + j)]
+                 : 0.f;
+    if (a.segments > 1 && !STATE) {
+      // the states that the segments in front left behind, each from zero
+      const int before = a.reverse ? a.segments - 1 - seg : seg;
+      for (int i = 0; i < before; ++i) {
+        const int at = a.reverse ? a.segments - 1 - i : i;
+        const int first = at * a.seg_chunks * C, count = min(first + a.seg_chunks * C, n) - first;
+        if (count <= 0) continue;
+        const float l = exp2f(g * (float)count);
+        const float* from = a.seg_states + ((int64_t)bh * a.segments + at) * a.dk * a.dv;
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (row < a.dk && sc0 + j < a.dv)
+            s[j] = fmaf(s[j], l, from[(int64_t)row * a.dv + sc0 + j]);
       }
-      begin(i + 1);
     }
-  }
-  if (!STATE && AHEAD && steps > 0) finish(steps - 1);
-
-  const bool last = a.reverse ? seg == 0 : (c1 == chunks && (c0 < chunks || seg == 0));
-  float* to = STATE ? a.seg_states + ((int64_t)bh * a.segments + seg) * a.dk * a.dv
-                    : last && a.final ? a.final + state_at : nullptr;
-  if (to && row < a.dk) {
+    const auto store_state = [&] {  // as an operand
+      if (row >= DK) return;
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (sc0 + j < a.dv)
-        to[(int64_t)row * a.dv + sc0 + j] = tries ? s[j] : __int_as_float(0x7fffffff);
-  }
-  if (!STATE) {
-    // tokens behind the row's end
-    const int end = min(a.len, (seg + 1) * a.seg_chunks * C);
-    for (int64_t t = max(n, seg * a.seg_chunks * C) + warp; t < end; t += kThreads / 32)
-      for (int j = lane; j < cols; j += 32)
-        static_cast<O*>(a.out)[b * a.out_batch + t * a.out_token + (int64_t)h * a.dv + col0 + j] =
-            from_f32<O>(0.f);
+      for (int u = 0; u < 2; ++u) {
+        uint32_t x[4][SP];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) split2<SP>(x[k], s[8 * u + 2 * k], s[8 * u + 2 * k + 1]);
+#pragma unroll
+        for (int j = 0; j < SP; ++j)
+          *reinterpret_cast<uint4*>(sm + L::state + j * L::kState + row * 128 +
+                                    (((part * 2 + u) ^ (row & 7)) << 4)) =
+              make_uint4(x[0][j], x[1][j], x[2][j], x[3][j]);
+      }
+    };
+    if (!STATE && steps > 0) store_state();
+
+    // Chunk i's operands: brought in where nobody copied ahead, rows past the end made zero, values
+    // weighted.
+    const auto begin = [&](int i) {
+      const int c = chunk(i), count = tokens(c), at = AHEAD ? i & 1 : 0;
+      uint8_t* k = sm + L::k + at * L::kKeys;
+      uint8_t* v = sm + L::v + at * L::kValues;
+      if (AHEAD) {
+        tc::barrier_wait_warp(&loaded_v[at], i >> 1 & 1, tries);
+        if (count < C) {
+          tc::barrier_wait_warp(&loaded_k[at], i >> 1 & 1, tries);
+          for (int x = threadIdx.x; x < (C - count) * PANELS * 8; x += kWorkers) {
+            const int r = count + x / (PANELS * 8), u = x % (PANELS * 8);
+            *reinterpret_cast<uint4*>(k + (u >> 3) * kPanel + r * 128 + ((u & 7) << 4)) =
+                make_uint4(0, 0, 0, 0);
+          }
+        }
+      } else {
+        const int64_t t = (int64_t)c * C;
+        if (!STATE)
+          load_rows<T, PANELS, C>(sm + L::q, row_of<T>(a.q, b, t, h, a.dk), a.q.token, count, 0, a.dk,
+                                  a.vec);
+        load_rows<T, PANELS, C>(k, row_of<T>(a.k, b, t, h, a.dk), a.k.token, count, 0, a.dk, a.vec);
+        load_rows<T, 1, C>(v, row_of<T>(a.v, b, t, h, a.dv), a.v.token, count, col0, a.dv, a.vec);
+        tc::named_sync(1, kWorkers);
+      }
+#pragma unroll
+      for (int x = threadIdx.x; x < C * 8; x += kWorkers) {
+        const int r = x >> 3, u = x & 7;
+        uint8_t* place = v + r * 128 + ((u ^ (r & 7)) << 4);
+        const float w = r >= count ? 0.f : power[a.reverse ? r + 1 : count - 1 - r];
+        uint32_t in[P][4], out[4][kWeighted];
+        bool fine = true;
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+          const uint4 y = *reinterpret_cast<const uint4*>(place + j * kPanel);
+          in[j][0] = y.x, in[j][1] = y.y, in[j][2] = y.z, in[j][3] = y.w;
+        }
+        if (r >= count) {
+#pragma unroll
+          for (int j = 0; j < P; ++j) {
+            in[j][0] = in[j][1] = in[j][2] = in[j][3] = 0;
+            *reinterpret_cast<uint4*>(place + j * kPanel) = make_uint4(0, 0, 0, 0);
+          }
+        }
+        // A value that is not finite would reach the tokens on the triangle's other side, as 0 * it:
+        // it becomes zero here, and its column NaN from its token on.
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+          fine &= (in[0][m] & 0x7f80u) != 0x7f80u && (in[0][m] & 0x7f800000u) != 0x7f800000u;
+        if (!fine) {
+#pragma unroll
+          for (int m = 0; m < 8; ++m) {
+            const uint32_t mask = 0xffffu << (m & 1) * 16, exponent = 0x7f80u << (m & 1) * 16;
+            if ((in[0][m / 2] & exponent) != exponent) continue;
+            atomicMax(&bad[i % 3][u * 8 + m], a.reverse ? r : C - 1 - r);
+#pragma unroll
+            for (int j = 0; j < P; ++j) in[j][m / 2] &= ~mask;
+          }
+#pragma unroll
+          for (int j = 0; j < P; ++j)
+            *reinterpret_cast<uint4*>(place + j * kPanel) =
+                make_uint4(in[j][0], in[j][1], in[j][2], in[j][3]);
+        }
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          float lo = __uint_as_float(in[0][m] << 16), hi = __uint_as_float(in[0][m] & 0xffff0000u);
+#pragma unroll
+          for (int j = 1; j < P; ++j) {
+            lo += __uint_as_float(in[j][m] << 16);
+            hi += __uint_as_float(in[j][m] & 0xffff0000u);
+          }
+          split2<kWeighted>(out[m], w * lo, w * hi);
+        }
+        uint8_t* to = sm + L::weighted + (place - v);
+#pragma unroll
+        for (int j = 0; j < kWeighted; ++j)
+          *reinterpret_cast<uint4*>(to + j * kPanel) =
+              make_uint4(out[0][j], out[1][j], out[2][j], out[3][j]);
+      }
+      tc::fence_shared();
+      tc::fence_before();
+      __syncwarp();
+      tc::barrier_arrive_if_zero(&ready_chunk, lane);
+    };
+    // Chunk i's output, once its products are there.
+    const auto finish = [&](int i) {
+      const int c = chunk(i), count = tokens(c);
+      tc::barrier_wait_warp(&done_out, i & 1, tries);
+      tc::fence_after();
+      uint32_t x[16], y[16];
+      tc::tmem_load<16>(x, mine + kFromState + (i & 1) * kTile + part * 16);
+      tc::tmem_load<16>(y, mine + kOut + part * 16);
+      tc::loads_done();
+      if (row >= count) return;
+      const float by = a.reverse ? power[count - 1 - row] : a.scale * power[row + 1];
+      float f[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        f[j] = fmaf(__uint_as_float(x[j]), by, a.scale * __uint_as_float(y[j]));
+        const int first = bad[i % 3][part * 16 + j];
+        if ((first >= 0 && (a.reverse ? row <= first : row >= C - 1 - first)) || !tries)
+          f[j] = __int_as_float(0x7fffffff);
+      }
+      O* out = static_cast<O*>(a.out) + b * a.out_batch + ((int64_t)c * C + row) * a.out_token +
+               (int64_t)h * a.dv + sc0;
+#pragma unroll
+      for (int j = 0; j < 16; j += 8)
+        if (sc0 + j < a.dv) store_pack<O, 8>(out + j, f + j, a.dv - sc0 - j, a.vec_out);
+    };
+
+#pragma unroll 1
+    for (int i = 0; i < steps; ++i) {
+      const int count = tokens(chunk(i));
+      begin(i);
+      if (!STATE) {
+        if (AHEAD && i > 0) finish(i - 1);
+        // the triangle's weights
+        tc::barrier_wait_warp(&done_scores, i & 1, tries);
+        tc::fence_after();
+        if (part < C / 32 && quarter < C / 32) {
+          uint32_t r[32], x[16][SP];
+          tc::tmem_load<32>(r, mine + kScores + part * 32);
+          tc::loads_done();
+          const bool none = a.reverse ? part < quarter || part * 32 >= count : part > quarter;
+          if (none) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+#pragma unroll
+              for (int k = 0; k < SP; ++k) x[j][k] = 0;
+          } else if (part == quarter || (a.reverse && part * 32 + 32 > count)) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              // (against time, columns past the end lie on the triangle's side)
+              const int at = part * 32 + j;
+              const int d0 = a.reverse ? at - row : row - at, d1 = a.reverse ? d0 + 1 : d0 - 1;
+              const bool in0 = d0 >= 0 && !(a.reverse && at >= count),
+                         in1 = d1 >= 0 && !(a.reverse && at + 1 >= count);
+              split2<SP>(x[j / 2], in0 ? __uint_as_float(r[j]) * power[d0] : 0.f,
+                         in1 ? __uint_as_float(r[j + 1]) * power[d1] : 0.f);
+            }
+          } else {
+            const float f = power[a.reverse ? part * 32 - row : row - part * 32 - 31];
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+              const float4 w = *reinterpret_cast<const float4*>(column + j);
+              split2<SP>(x[j / 2], __uint_as_float(r[j]) * (f * w.x),
+                         __uint_as_float(r[j + 1]) * (f * w.y));
+              split2<SP>(x[j / 2 + 1], __uint_as_float(r[j + 2]) * (f * w.z),
+                         __uint_as_float(r[j + 3]) * (f * w.w));
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < SP; ++k) {
+            uint32_t o[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) o[j] = x[j][k];
+            tc::tmem_store(mine + kTriangle + k * (C / 2) + part * 16, o);
+          }
+          tc::stores_to_tmem_done();
+        }
+        tc::fence_before();
+        __syncwarp();
+        tc::barrier_arrive_if_zero(&ready_triangle, lane);
+      }
+      // the state behind the chunk
+      tc::barrier_wait_warp(&done_state, i & 1, tries);
+      tc::fence_after();
+      uint32_t x[16];
+      tc::tmem_load<16>(x, mine + kAdded + part * 16);
+      tc::loads_done();
+      tc::fence_before();
+      const float l = power[count], by = a.reverse ? a.scale : 1.f;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        s[j] = fmaf(s[j], l, by * __uint_as_float(x[j]));
+        if (bad[i % 3][part * 16 + j] >= 0) s[j] = __int_as_float(0x7fffffff);
+      }
+      if (!STATE && !AHEAD) finish(i);
+      if (i + 1 < steps) {
+        if (!STATE) {
+          tc::barrier_wait_warp(&done_q, i & 1, tries);
+          store_state();
+        }
+        // every warp is past the chunk before: its marks are free, and (where nobody copies ahead)
+        // every operand
+        tc::named_sync(1, kWorkers);
+        if (threadIdx.x < kTile) bad[(i + 2) % 3][threadIdx.x] = -1;
+      }
+    }
+    if (!STATE && AHEAD && steps > 0) finish(steps - 1);
+
+    const bool last = a.reverse ? seg == 0 : (c1 == chunks && (c0 < chunks || seg == 0));
+    float* to = STATE ? a.seg_states + ((int64_t)bh * a.segments + seg) * a.dk * a.dv
+                      : last && a.final ? a.final + state_at : nullptr;
+    if (to && row < a.dk) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (sc0 + j < a.dv)
+          to[(int64_t)row * a.dv + sc0 + j] = tries ? s[j] : __int_as_float(0x7fffffff);
+    }
+    if (!STATE) {
+      // tokens behind the row's end
+      const int end = min(a.len, (seg + 1) * a.seg_chunks * C);
+      for (int64_t t = max(n, seg * a.seg_chunks * C) + warp; t < end; t += kWorkers / 32)
+        for (int j = lane; j < cols; j += 32)
+          static_cast<O*>(a.out)[b * a.out_batch + t * a.out_token + (int64_t)h * a.dv + col0 + j] =
+              from_f32<O>(0.f);
+    }
   }
   tc::fence_before();
   __syncthreads();

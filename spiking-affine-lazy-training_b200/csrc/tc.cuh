@@ -65,6 +65,10 @@ __device__ __forceinline__ void barrier_arrive_if_zero(uint64_t* b, int lane) {
       "r"(lane)
       : "memory");
 }
+// Threads of part of a block.
+__device__ __forceinline__ void named_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
 // A warpgroup's share of the registers that the block was launched with.
 template <int N>
 __device__ __forceinline__ void registers_up() {
