@@ -32,7 +32,7 @@ struct Pass {
   // set by the launch
   int segments, seg_chunks;  // segments of a row that run side by side, chunks of each
   float* seg_states;         // (batch, heads, segments, dk, dv): what each adds to the state
-  bool vec, vec_out;
+  bool vec, vec_out, copies_out;
 };
 
 __device__ __forceinline__ float decay_of(const float* g, int h) {
@@ -67,8 +67,10 @@ struct Layout {
   static constexpr int kPanel = C * 128, kKeys = P * PANELS * kPanel, kValues = P * kPanel;
   static constexpr int q = 0, k = q + kKeys, v = k + B * kKeys, weighted = v + B * kValues,
                        state = weighted + kWeighted * kPanel,
-                       kState = PANELS * 64 * 128,  // a part of the state
-      bytes = state + state_parts<T>() * kState + 1024;
+                       kState = PANELS * 64 * 128;  // a part of the state
+  static constexpr int
+      out = state + state_parts<T>() * kState,  // 1 KB a warp
+      bytes = out + (AHEAD ? 16 * 1024 : 0) + 1024;
 };
 
 // A value's parts: each the nearest bfloat16 of what the ones before it leave.
@@ -117,7 +119,8 @@ __device__ __forceinline__ void load_rows(uint8_t* to, const T* p, int64_t strid
 template <typename T, typename O, int PANELS, bool AHEAD, bool STATE>
 __global__ void __launch_bounds__(kThreads, 1)
 attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                 const __grid_constant__ CUtensorMap map_v, const Pass a) {
+                 const __grid_constant__ CUtensorMap map_v,
+                 const __grid_constant__ CUtensorMap map_out, const Pass a) {
   using L = Layout<T, PANELS, AHEAD>;
   constexpr int C = L::C, P = L::P, SP = state_parts<T>(), DK = PANELS * 64;
   constexpr int kPanel = L::kPanel;
@@ -130,6 +133,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   __shared__ float power[C + 1];              // l^i
   __shared__ __align__(16) float column[32];  // of a column within its 32
   __shared__ int bad[3][kTile];               // the outermost token whose v is not finite
+  __shared__ int any_bad[3];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int quarter = warp & 3, part = warp >> 2, row = quarter * 32 + lane;
 
@@ -164,6 +168,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     column[threadIdx.x] = i == 0 ? 1.f : exp2f(g * (float)i);
   }
   for (int i = threadIdx.x; i < 3 * kTile; i += kThreads) bad[i / kTile][i % kTile] = -1;
+  if (threadIdx.x < 3) any_bad[threadIdx.x] = 0;
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
@@ -302,27 +307,16 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     // this thread's part of the state: row `row`, 16 columns
     float s[16];
     const int sc0 = col0 + part * 16;
+    const bool joined = a.segments > 1 && !STATE;
+    const float* from =
+        joined ? a.seg_states + ((int64_t)bh * a.segments + seg) * a.dk * a.dv
+               : a.initial ? a.initial + state_at : nullptr;
+    const bool across = a.initial_t && !joined;
 #pragma unroll
     for (int j = 0; j < 16; ++j)
-      s[j] = a.initial && row < a.dk && sc0 + j < a.dv
-                 ? a.initial[state_at + (a.initial_t ? (int64_t)(sc0 + j) * a.dk + row
-                                                     : (int64_t)row * a.dv + sc0 + j)]
+      s[j] = from && row < a.dk && sc0 + j < a.dv
+                 ? from[across ? (int64_t)(sc0 + j) * a.dk + row : (int64_t)row * a.dv + sc0 + j]
                  : 0.f;
-    if (a.segments > 1 && !STATE) {
-      // the states that the segments in front left behind, each from zero
-      const int before = a.reverse ? a.segments - 1 - seg : seg;
-      for (int i = 0; i < before; ++i) {
-        const int at = a.reverse ? a.segments - 1 - i : i;
-        const int first = at * a.seg_chunks * C, count = min(first + a.seg_chunks * C, n) - first;
-        if (count <= 0) continue;
-        const float l = exp2f(g * (float)count);
-        const float* from = a.seg_states + ((int64_t)bh * a.segments + at) * a.dk * a.dv;
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (row < a.dk && sc0 + j < a.dv)
-            s[j] = fmaf(s[j], l, from[(int64_t)row * a.dv + sc0 + j]);
-      }
-    }
     const auto store_state = [&] {  // as an operand
       if (row >= DK) return;
 #pragma unroll
@@ -389,6 +383,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         for (int m = 0; m < 4; ++m)
           fine &= (in[0][m] & 0x7f80u) != 0x7f80u && (in[0][m] & 0x7f800000u) != 0x7f800000u;
         if (!fine) {
+          any_bad[i % 3] = 1;
 #pragma unroll
           for (int m = 0; m < 8; ++m) {
             const uint32_t mask = 0xffffu << (m & 1) * 16, exponent = 0x7f80u << (m & 1) * 16;
@@ -432,16 +427,37 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       tc::tmem_load<16>(x, mine + kFromState + (i & 1) * kTile + part * 16);
       tc::tmem_load<16>(y, mine + kOut + part * 16);
       tc::loads_done();
-      if (row >= count) return;
-      const float by = a.reverse ? power[count - 1 - row] : a.scale * power[row + 1];
+      const bool live = row < count;
+      const float by = !live ? 0.f : a.reverse ? power[count - 1 - row] : a.scale * power[row + 1];
       float f[16];
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        f[j] = fmaf(__uint_as_float(x[j]), by, a.scale * __uint_as_float(y[j]));
-        const int first = bad[i % 3][part * 16 + j];
-        if ((first >= 0 && (a.reverse ? row <= first : row >= C - 1 - first)) || !tries)
-          f[j] = __int_as_float(0x7fffffff);
+      for (int j = 0; j < 16; ++j)
+        f[j] = live ? fmaf(__uint_as_float(x[j]), by, a.scale * __uint_as_float(y[j])) : 0.f;
+      if (any_bad[i % 3] || !tries) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int first = bad[i % 3][part * 16 + j];
+          if (live && ((first >= 0 && (a.reverse ? row <= first : row >= C - 1 - first)) || !tries))
+            f[j] = __int_as_float(0x7fffffff);
+        }
       }
+      if constexpr (AHEAD && sizeof(O) == 2) {
+        if (a.copies_out) {
+          // 32 bytes a row, through shared memory: as stores from here every 16 bytes would be a line
+          // of their own.  Rows past the end are zero anyway; those past `len` are left out.
+          uint8_t* to = sm + L::out + warp * 1024;
+          if (lane == 0) tc::stores_read();
+          __syncwarp();
+          store_pack<O, 8>(reinterpret_cast<O*>(to + lane * 32), f, 8, true);
+          store_pack<O, 8>(reinterpret_cast<O*>(to + lane * 32 + 16), f + 8, 8, true);
+          tc::fence_shared();
+          __syncwarp();
+          if (lane == 0 && quarter * 32 < a.len - c * C && sc0 < a.dv)
+            tc::store_box4(&map_out, to, sc0, h, c * C + quarter * 32, b);
+          return;
+        }
+      }
+      if (!live) return;
       O* out = static_cast<O*>(a.out) + b * a.out_batch + ((int64_t)c * C + row) * a.out_token +
                (int64_t)h * a.dv + sc0;
 #pragma unroll
@@ -476,8 +492,9 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
               const int d0 = a.reverse ? at - row : row - at, d1 = a.reverse ? d0 + 1 : d0 - 1;
               const bool in0 = d0 >= 0 && !(a.reverse && at >= count),
                          in1 = d1 >= 0 && !(a.reverse && at + 1 >= count);
-              split2<SP>(x[j / 2], in0 ? __uint_as_float(r[j]) * power[d0] : 0.f,
-                         in1 ? __uint_as_float(r[j + 1]) * power[d1] : 0.f);
+              const float w0 = power[max(d0, 0)], w1 = power[max(d1, 0)];  // (no branches)
+              split2<SP>(x[j / 2], in0 ? __uint_as_float(r[j]) * w0 : 0.f,
+                         in1 ? __uint_as_float(r[j + 1]) * w1 : 0.f);
             }
           } else {
             const float f = power[a.reverse ? part * 32 - row : row - part * 32 - 31];
@@ -512,9 +529,11 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       tc::fence_before();
       const float l = power[count], by = a.reverse ? a.scale : 1.f;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        s[j] = fmaf(s[j], l, by * __uint_as_float(x[j]));
-        if (bad[i % 3][part * 16 + j] >= 0) s[j] = __int_as_float(0x7fffffff);
+      for (int j = 0; j < 16; ++j) s[j] = fmaf(s[j], l, by * __uint_as_float(x[j]));
+      if (any_bad[i % 3]) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (bad[i % 3][part * 16 + j] >= 0) s[j] = __int_as_float(0x7fffffff);
       }
       if (!STATE && !AHEAD) finish(i);
       if (i + 1 < steps) {
@@ -526,9 +545,12 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         // every operand
         tc::named_sync(1, kWorkers);
         if (threadIdx.x < kTile) bad[(i + 2) % 3][threadIdx.x] = -1;
+        if (threadIdx.x == 0) any_bad[(i + 2) % 3] = 0;
       }
     }
     if (!STATE && AHEAD && steps > 0) finish(steps - 1);
+    if (AHEAD && lane == 0) tc::stores_done();
+    __syncwarp();
 
     const bool last = a.reverse ? seg == 0 : (c1 == chunks && (c0 < chunks || seg == 0));
     float* to = STATE ? a.seg_states + ((int64_t)bh * a.segments + seg) * a.dk * a.dv
@@ -542,7 +564,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     if (!STATE) {
       // tokens behind the row's end
       const int end = min(a.len, (seg + 1) * a.seg_chunks * C);
-      for (int64_t t = max(n, seg * a.seg_chunks * C) + warp; t < end; t += kWorkers / 32)
+      for (int64_t t = max(a.copies_out ? chunks * C : n, seg * a.seg_chunks * C) + warp; t < end; t += kWorkers / 32)
         for (int j = lane; j < cols; j += 32)
           static_cast<O*>(a.out)[b * a.out_batch + t * a.out_token + (int64_t)h * a.dv + col0 + j] =
               from_f32<O>(0.f);
@@ -553,6 +575,25 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   if (warp == 0) {
     tc::fence_after();
     tc::tmem_free(tmem, 512);
+  }
+}
+
+// The states in front of a row's segments, in place of what each adds from zero: one value a thread,
+// from segment to segment (against time from the last one).
+__global__ void __launch_bounds__(256) join_segments_kernel(const Pass a, int chunk) {
+  const int each = a.dk * a.dv, i = blockIdx.x * 256 + threadIdx.x, bh = blockIdx.y;
+  if (i >= each) return;
+  const int b = bh / a.heads, n = row_tokens(a.n_real, b, a.len);
+  const float g = decay_of(a.log_decay, bh - b * a.heads) * kLog2e;
+  const int row = i / a.dv, col = i - row * a.dv;
+  float s = a.initial ? a.initial[(int64_t)bh * each + (a.initial_t ? col * a.dk + row : i)] : 0.f;
+  float* at = a.seg_states + (int64_t)bh * a.segments * each + i;
+  for (int x = 0; x < a.segments; ++x) {
+    const int seg = a.reverse ? a.segments - 1 - x : x;
+    const int first = seg * a.seg_chunks * chunk, count = min(first + a.seg_chunks * chunk, n) - first;
+    const float added = x + 1 < a.segments ? at[(int64_t)seg * each] : 0.f;
+    at[(int64_t)seg * each] = s;
+    if (count > 0) s = fmaf(s, exp2f(g * (float)count), added);
   }
 }
 
@@ -574,8 +615,9 @@ __global__ void __launch_bounds__(256) sum_heads_kernel(const float* from, T* to
   }
 }
 
-// Boxes of `high` tokens x 64 columns of one head.
-bool head_map(CUtensorMap* map, const Rows& r, int dim, int heads, int len, int batch, int high) {
+// Boxes of `high` tokens x 64 columns of one head; for outputs x 16 columns, as they lie.
+bool head_map(CUtensorMap* map, const Rows& r, int dim, int heads, int len, int batch, int high,
+              bool out = false) {
   const tc::EncodeTiled f = tc::encoder();
   if (!f || !aligned16(r.p) || dim % 8) return false;
   const int64_t token = len > 1 ? r.token * 2 : 16, row = batch > 1 ? r.batch * 2 : 16;
@@ -585,36 +627,38 @@ bool head_map(CUtensorMap* map, const Rows& r, int dim, int heads, int len, int 
   const cuuint64_t dims[4] = {(cuuint64_t)dim, (cuuint64_t)(heads / r.share), (cuuint64_t)len,
                               (cuuint64_t)batch};
   const cuuint64_t strides[3] = {(cuuint64_t)dim * 2, (cuuint64_t)token, (cuuint64_t)row};
-  const cuuint32_t box[4] = {64, 1, (cuuint32_t)high, 1}, unit[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {out ? 16u : 64u, 1, (cuuint32_t)high, 1}, unit[4] = {1, 1, 1, 1};
   return f(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(r.p), dims, strides, box, unit,
-           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+           CU_TENSOR_MAP_INTERLEAVE_NONE,
+           out ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
            CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <typename T, typename O, int PANELS, bool AHEAD, bool STATE>
-cudaError_t start(const CUtensorMap (&maps)[3], const Pass& p, int64_t blocks, cudaStream_t st,
+cudaError_t start(const CUtensorMap (&maps)[4], const Pass& p, int64_t blocks, cudaStream_t st,
                   int* launches) {
   const auto kernel = attention_kernel<T, O, PANELS, AHEAD, STATE>;
   constexpr int bytes = Layout<T, PANELS, AHEAD>::bytes;
   const cudaError_t e =
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return e;
-  kernel<<<(unsigned)blocks, kThreads, bytes, st>>>(maps[0], maps[1], maps[2], p);
+  kernel<<<(unsigned)blocks, kThreads, bytes, st>>>(maps[0], maps[1], maps[2], maps[3], p);
   ++*launches;
   return cudaGetLastError();
 }
 
 // Segments of a row: the number that needs the least time in rounds of resident blocks (one an SM),
-// counted in chunks; a first pass over all but the last segment costs about half a chunk's time.
+// counted in chunks of the main pass.  A block takes about as long as a chunk to begin and end; the
+// first pass, over all but the last segment, takes two fifths of a chunk's time for each, and with the
+// joining of its states two more.
 int segments_of(int64_t blocks, int chunks) {
   int best = 1;
   double least = 1e300;
-  for (int s = 1; s <= 64 && s <= chunks; ++s) {
+  for (int s = 1; s <= 64 && s <= chunks && blocks * s <= 148 * 8; ++s) {
     const int each = (chunks + s - 1) / s;
-    if (s > 1 && (chunks + each - 1) / each != s) continue;
-    const double rounds = (double)((blocks * s + 147) / 148) * each;
-    const double first = s == 1 ? 0 : (double)((blocks * s + 147) / 148) * each * 0.5 + 2;
-    if (rounds + first < least) least = rounds + first, best = s;
+    const double rounds = (double)((blocks * s + 147) / 148);
+    const double time = rounds * (each + 1) + (s > 1 ? rounds * (0.4 * each + 1) + 2 : 0);
+    if (time < least) least = time, best = s;
   }
   return best;
 }
@@ -631,13 +675,18 @@ size_t segment_bytes(int type, int batch, int heads, int dk, int dv, int len) {
 }
 
 template <typename T, typename O, int PANELS, bool AHEAD>
-cudaError_t run_ahead(const CUtensorMap (&maps)[3], const Pass& p, int64_t blocks, cudaStream_t st,
+cudaError_t run_ahead(const CUtensorMap (&maps)[4], const Pass& p, int64_t blocks, cudaStream_t st,
                       int* launches) {
   if (p.segments > 1) {
     Pass first = p;
     first.initial = nullptr;
-    const cudaError_t e =
-        start<T, O, PANELS, AHEAD, true>(maps, first, blocks * p.segments, st, launches);
+    cudaError_t e = start<T, O, PANELS, AHEAD, true>(maps, first, blocks * p.segments, st, launches);
+    if (e != cudaSuccess) return e;
+    // (rows and heads: at most 2^24, and where segments are used less than twice the SMs)
+    join_segments_kernel<<<dim3((p.dk * p.dv + 255) / 256, p.batch * p.heads), 256, 0, st>>>(
+        p, chunk_of<T>());
+    ++*launches;
+    e = cudaGetLastError();
     if (e != cudaSuccess) return e;
   }
   return start<T, O, PANELS, AHEAD, false>(maps, p, blocks * p.segments, st, launches);
@@ -656,16 +705,20 @@ cudaError_t run_pass(Pass p, void* ws, cudaStream_t st, int* launches) {
   const auto packed = [&](const Rows& r, int dim) {
     return pack_rows(r.p, 8, sizeof(T), r.batch, r.token) && dim * sizeof(T) % 16 == 0;
   };
+  p.copies_out = false;
   p.vec = packed(p.q, p.dk) && packed(p.k, p.dk) && packed(p.v, p.dv);
   p.vec_out = packed_rows(p.out, 16, sizeof(O), p.out_batch, p.out_token) &&
               p.dv * sizeof(O) % 16 == 0;
-  CUtensorMap maps[3] = {};
+  CUtensorMap maps[4] = {};
   if constexpr (parts_of<T>() == 1) {
     if (p.len > 0 && head_map(&maps[0], p.q, p.dk, p.heads, p.len, p.batch, C) &&
         head_map(&maps[1], p.k, p.dk, p.heads, p.len, p.batch, C) &&
-        head_map(&maps[2], p.v, p.dv, p.heads, p.len, p.batch, C))
+        head_map(&maps[2], p.v, p.dv, p.heads, p.len, p.batch, C)) {
+      p.copies_out = sizeof(O) == 2 && head_map(&maps[3], {p.out, p.out_batch, p.out_token, 1}, p.dv,
+                                                p.heads, p.len, p.batch, 32, true);
       return p.dk <= 64 ? run_ahead<T, O, 1, true>(maps, p, blocks, st, launches)
                         : run_ahead<T, O, 2, true>(maps, p, blocks, st, launches);
+    }
   }
   return p.dk <= 64 ? run_ahead<T, O, 1, false>(maps, p, blocks, st, launches)
                     : run_ahead<T, O, 2, false>(maps, p, blocks, st, launches);

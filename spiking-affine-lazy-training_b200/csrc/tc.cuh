@@ -99,6 +99,14 @@ __device__ __forceinline__ void store_box(const CUtensorMap* map, const void* fr
       "r"(x), "r"(y), "r"(shared_at(from))
       : "memory");
 }
+__device__ __forceinline__ void store_box4(const CUtensorMap* map, const void* from, int x, int y, int z,
+                                           int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3, %4}], [%5];\n"
+      "cp.async.bulk.commit_group;" ::"l"(map),
+      "r"(x), "r"(y), "r"(z), "r"(w), "r"(shared_at(from))
+      : "memory");
+}
 __device__ __forceinline__ void stores_read() {
   asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
 }
