@@ -475,44 +475,49 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         tc::barrier_wait_warp(&done_scores, i & 1, tries);
         tc::fence_after();
         if (part < C / 32 && quarter < C / 32) {
-          uint32_t r[32], x[16][SP];
-          tc::tmem_load<32>(r, mine + kScores + part * 32);
-          tc::loads_done();
           const bool none = a.reverse ? part < quarter || part * 32 >= count : part > quarter;
-          if (none) {
+          const bool edge = part == quarter || (a.reverse && part * 32 + 32 > count);
+          const float f = none || edge ? 0.f
+                                       : power[a.reverse ? part * 32 - row : row - part * 32 - 31];
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
+          for (int y = 0; y < 32; y += 16) {
+            uint32_t r[16], x[8][SP];
+            tc::tmem_load<16>(r, mine + kScores + part * 32 + y);
+            tc::loads_done();
+            if (none) {
 #pragma unroll
-              for (int k = 0; k < SP; ++k) x[j][k] = 0;
-          } else if (part == quarter || (a.reverse && part * 32 + 32 > count)) {
+              for (int j = 0; j < 8; ++j)
 #pragma unroll
-            for (int j = 0; j < 32; j += 2) {
-              // (against time, columns past the end lie on the triangle's side)
-              const int at = part * 32 + j;
-              const int d0 = a.reverse ? at - row : row - at, d1 = a.reverse ? d0 + 1 : d0 - 1;
-              const bool in0 = d0 >= 0 && !(a.reverse && at >= count),
-                         in1 = d1 >= 0 && !(a.reverse && at + 1 >= count);
-              const float w0 = power[max(d0, 0)], w1 = power[max(d1, 0)];  // (no branches)
-              split2<SP>(x[j / 2], in0 ? __uint_as_float(r[j]) * w0 : 0.f,
-                         in1 ? __uint_as_float(r[j + 1]) * w1 : 0.f);
+                for (int k = 0; k < SP; ++k) x[j][k] = 0;
+            } else if (edge) {
+#pragma unroll
+              for (int j = 0; j < 16; j += 2) {
+                // (against time, columns past the end lie on the triangle's side)
+                const int at = part * 32 + y + j;
+                const int d0 = a.reverse ? at - row : row - at, d1 = a.reverse ? d0 + 1 : d0 - 1;
+                const bool in0 = d0 >= 0 && !(a.reverse && at >= count),
+                           in1 = d1 >= 0 && !(a.reverse && at + 1 >= count);
+                const float w0 = power[max(d0, 0)], w1 = power[max(d1, 0)];  // (no branches)
+                split2<SP>(x[j / 2], in0 ? __uint_as_float(r[j]) * w0 : 0.f,
+                           in1 ? __uint_as_float(r[j + 1]) * w1 : 0.f);
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 16; j += 4) {
+                const float4 w = *reinterpret_cast<const float4*>(column + y + j);
+                split2<SP>(x[j / 2], __uint_as_float(r[j]) * (f * w.x),
+                           __uint_as_float(r[j + 1]) * (f * w.y));
+                split2<SP>(x[j / 2 + 1], __uint_as_float(r[j + 2]) * (f * w.z),
+                           __uint_as_float(r[j + 3]) * (f * w.w));
+              }
             }
-          } else {
-            const float f = power[a.reverse ? part * 32 - row : row - part * 32 - 31];
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-              const float4 w = *reinterpret_cast<const float4*>(column + j);
-              split2<SP>(x[j / 2], __uint_as_float(r[j]) * (f * w.x),
-                         __uint_as_float(r[j + 1]) * (f * w.y));
-              split2<SP>(x[j / 2 + 1], __uint_as_float(r[j + 2]) * (f * w.z),
-                         __uint_as_float(r[j + 3]) * (f * w.w));
+            for (int k = 0; k < SP; ++k) {
+              uint32_t o[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) o[j] = x[j][k];
+              tc::tmem_store(mine + kTriangle + k * (C / 2) + part * 16 + y / 2, o);
             }
-          }
-#pragma unroll
-          for (int k = 0; k < SP; ++k) {
-            uint32_t o[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) o[j] = x[j][k];
-            tc::tmem_store(mine + kTriangle + k * (C / 2) + part * 16, o);
           }
           tc::stores_to_tmem_done();
         }

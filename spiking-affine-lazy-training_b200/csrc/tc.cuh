@@ -196,14 +196,11 @@ __device__ __forceinline__ void tmem_load(uint32_t (&r)[N], uint32_t at) {
 __device__ __forceinline__ void stores_to_tmem_done() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
-// 16 columns of the warp's 32 rows from registers.
-__device__ __forceinline__ void tmem_store(uint32_t at, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
+// 8 columns of the warp's 32 rows from registers.
+__device__ __forceinline__ void tmem_store(uint32_t at, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(at),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 
 // ---------------------------------------------------------------- products
