@@ -359,6 +359,9 @@ Checks check(const salt_quantize_q8_args* a) {
   c.type(a->type);
   c.need(a->rows >= 0, "rows is negative");
   c.need(a->dim >= 1 && a->dim <= kMostDim, "dim must lie in [1, 2^24]");
+  // a block has 32 groups of a row at least, or a tile of 128 x 128
+  c.need((int64_t)a->rows * ((a->dim + 127) / 128) <= (int64_t)INT32_MAX * 32,
+         "rows * dim is too large for one launch");
   const bool used = a->rows > 0;
   c.input(a->x, used, "x is NULL");
   c.input(a->out, used, "out is NULL");

@@ -73,15 +73,20 @@ struct Layout {
       bytes = out + (AHEAD ? 16 * 1024 : 0) + 1024;
 };
 
-// A value's parts: each the nearest bfloat16 of what the ones before it leave.
+// Two values in parts of bfloat16: the upper 8 bits of what is left, time and again; the last of two
+// parts is rounded to the nearest (2^-16 of the value in all), three hold all 24 bits.
 template <int N>
 __device__ __forceinline__ void split2(uint32_t (&to)[N], float x, float y) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-    to[i] = *reinterpret_cast<const uint32_t*>(&h);
-    x -= __uint_as_float(to[i] << 16);
-    y -= __uint_as_float(to[i] & 0xffff0000u);
+    if (i == N - 1 && N < 3) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+      to[i] = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      to[i] = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
+      x -= __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+      y -= __uint_as_float(__float_as_uint(y) & 0xffff0000u);
+    }
   }
 }
 
@@ -130,10 +135,11 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   __shared__ uint64_t done_scores, done_q, done_state, done_out;  // products
   __shared__ uint64_t ready_chunk, ready_triangle;  // operands that threads wrote
   __shared__ uint32_t tmem_at;
-  __shared__ float power[C + 1];              // l^i
+  __shared__ float powers[32 + C + 1];        // l^i from place 32 on
   __shared__ __align__(16) float column[32];  // of a column within its 32
   __shared__ int bad[3][kTile];               // the outermost token whose v is not finite
   __shared__ int any_bad[3];
+  float* power = powers + 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int quarter = warp & 3, part = warp >> 2, row = quarter * 32 + lane;
 
@@ -162,7 +168,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     tc::barrier_init_fence();
   }
   if (warp == 0) tc::tmem_alloc(&tmem_at, 512);
-  for (int i = threadIdx.x; i <= C; i += kThreads) power[i] = i == 0 ? 1.f : exp2f(g * (float)i);
+  for (int i = (int)threadIdx.x - 32; i <= C; i += kThreads)
+    power[i] = i <= 0 ? 1.f : exp2f(g * (float)i);  // (in front of place 0: any number)
   if (threadIdx.x < 32) {
     const int i = a.reverse ? threadIdx.x : 31 - threadIdx.x;
     column[threadIdx.x] = i == 0 ? 1.f : exp2f(g * (float)i);
@@ -476,9 +483,12 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         tc::fence_after();
         if (part < C / 32 && quarter < C / 32) {
           const bool none = a.reverse ? part < quarter || part * 32 >= count : part > quarter;
-          const bool edge = part == quarter || (a.reverse && part * 32 + 32 > count);
-          const float f = none || edge ? 0.f
-                                       : power[a.reverse ? part * 32 - row : row - part * 32 - 31];
+          const bool diagonal = part == quarter;
+          // against time, columns past the end lie on the triangle's side
+          const bool cut = a.reverse && part * 32 + 32 > count;
+          const float f = none || diagonal || cut
+                              ? 0.f
+                              : power[a.reverse ? part * 32 - row : row - part * 32 - 31];
 #pragma unroll
           for (int y = 0; y < 32; y += 16) {
             uint32_t r[16], x[8][SP];
@@ -489,17 +499,24 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
               for (int j = 0; j < 8; ++j)
 #pragma unroll
                 for (int k = 0; k < SP; ++k) x[j][k] = 0;
-            } else if (edge) {
+            } else if (cut) {
 #pragma unroll
               for (int j = 0; j < 16; j += 2) {
-                // (against time, columns past the end lie on the triangle's side)
-                const int at = part * 32 + y + j;
-                const int d0 = a.reverse ? at - row : row - at, d1 = a.reverse ? d0 + 1 : d0 - 1;
-                const bool in0 = d0 >= 0 && !(a.reverse && at >= count),
-                           in1 = d1 >= 0 && !(a.reverse && at + 1 >= count);
-                const float w0 = power[max(d0, 0)], w1 = power[max(d1, 0)];  // (no branches)
-                split2<SP>(x[j / 2], in0 ? __uint_as_float(r[j]) * w0 : 0.f,
-                           in1 ? __uint_as_float(r[j + 1]) * w1 : 0.f);
+                const int at = part * 32 + y + j, d = at - row;
+                const float w0 = power[max(d, 0)], w1 = power[max(d + 1, 0)];
+                split2<SP>(x[j / 2], d >= 0 && at < count ? __uint_as_float(r[j]) * w0 : 0.f,
+                           d >= -1 && at + 1 < count ? __uint_as_float(r[j + 1]) * w1 : 0.f);
+              }
+            } else if (diagonal) {
+              // (weights of the other side are loaded and left: a branch a value would cost more)
+              const float* w = a.reverse ? power - lane + y : power + lane - y;
+#pragma unroll
+              for (int j = 0; j < 16; j += 2) {
+                const int c0 = y + j, c1 = c0 + 1;
+                const float p0 = __uint_as_float(r[j]) * w[a.reverse ? j : -j],
+                            p1 = __uint_as_float(r[j + 1]) * w[a.reverse ? j + 1 : -j - 1];
+                split2<SP>(x[j / 2], (a.reverse ? c0 >= lane : c0 <= lane) ? p0 : 0.f,
+                           (a.reverse ? c1 >= lane : c1 <= lane) ? p1 : 0.f);
               }
             } else {
 #pragma unroll
@@ -729,29 +746,72 @@ cudaError_t run_pass(Pass p, void* ws, cudaStream_t st, int* launches) {
                     : run_ahead<T, O, 2, false>(maps, p, blocks, st, launches);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(128) attention_step_kernel(salt_linear_attention_step_args a) {
-  const int bh = blockIdx.x, b = bh / a.heads, h = bh % a.heads, share = a.heads / a.kv_heads;
+// One token of a row's head: S = l S + k v^T; out = scale * q S.  A block has a head; its 8 warps take
+// every eighth row of the state, a lane four columns (side by side with VEC, 32 apart without), and all
+// of a thread's loads go out before its first store, which the compiler may not put behind loads of the
+// same array.  Bound by memory, 8 bytes a value of the state.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256, 2) attention_step_kernel(salt_linear_attention_step_args a) {
+  __shared__ __align__(16) float parts[8][128];
+  const int bh = blockIdx.x, b = bh / a.heads, h = bh - b * a.heads, share = a.heads / a.kv_heads;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int slot = a.slots ? a.slots[b] : b;
   T* out = static_cast<T*>(a.out) + b * a.out_stride + (int64_t)h * a.dim_v;
-  const int col = threadIdx.x;
-  if (col >= a.dim_v) return;
-  if (slot < 0 || slot >= a.n_slots) {
-    out[col] = from_f32<T>(0.f);
+  if (slot < 0 || slot >= a.n_slots) {  // the whole block
+    if (threadIdx.x < a.dim_v) out[threadIdx.x] = from_f32<T>(0.f);
     return;
   }
   const T* q = static_cast<const T*>(a.q) + b * a.q_stride + (int64_t)h * a.dim_k;
   const T* k = static_cast<const T*>(a.k) + b * a.k_stride + (int64_t)(h / share) * a.dim_k;
   const T* v = static_cast<const T*>(a.v) + b * a.v_stride + (int64_t)(h / share) * a.dim_v;
   float* s = a.pool + ((int64_t)slot * a.heads + h) * a.dim_k * a.dim_v;
-  const float l = expf(decay_of(a.log_decay, h)), vc = to_f32(v[col]);
-  float acc = 0.f;
-  for (int r = 0; r < a.dim_k; ++r) {
-    const float x = l * s[r * a.dim_v + col] + to_f32(k[r]) * vc;
-    s[r * a.dim_v + col] = x;
-    acc += to_f32(q[r]) * x;
+  const auto column = [&](int j) { return VEC ? lane * 4 + j : lane + 32 * j; };
+  float x[16][4];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int row = warp + 8 * i;
+    if (VEC) {
+      if (row < a.dim_k && lane * 4 < a.dim_v)
+        *reinterpret_cast<float4*>(x[i]) =
+            *reinterpret_cast<const float4*>(s + row * a.dim_v + lane * 4);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (row < a.dim_k && column(j) < a.dim_v) x[i][j] = s[row * a.dim_v + column(j)];
+    }
   }
-  out[col] = from_f32<T>(a.scale * acc);
+  const float l = expf(decay_of(a.log_decay, h));
+  float w[4], sum[4] = {};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w[j] = column(j) < a.dim_v ? to_f32(v[column(j)]) : 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int row = warp + 8 * i;
+    if (row >= a.dim_k) break;
+    const float kr = to_f32(k[row]), qr = to_f32(q[row]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x[i][j] = fmaf(l, x[i][j], kr * w[j]);
+      sum[j] = fmaf(qr, x[i][j], sum[j]);
+    }
+    if (VEC) {
+      if (lane * 4 < a.dim_v)
+        *reinterpret_cast<float4*>(s + row * a.dim_v + lane * 4) = *reinterpret_cast<float4*>(x[i]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (column(j) < a.dim_v) s[row * a.dim_v + column(j)] = x[i][j];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) parts[warp][column(j)] = sum[j];
+  __syncthreads();
+  if (threadIdx.x < a.dim_v) {
+    float o = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o += parts[i][threadIdx.x];
+    out[threadIdx.x] = from_f32<T>(a.scale * o);
+  }
 }
 
 }  // namespace
@@ -776,7 +836,11 @@ cudaError_t linear_attention_launch(const salt_linear_attention_args& a, void* w
 cudaError_t linear_attention_step_launch(const salt_linear_attention_step_args& a, cudaStream_t st,
                                          int* launches) {
   if (!a.batch) return cudaSuccess;
-  SALT_WITH_TYPE(a.type, T, attention_step_kernel<T><<<a.batch * a.heads, 128, 0, st>>>(a));
+  const bool vec = aligned16(a.pool) && a.dim_v % 4 == 0;
+  SALT_WITH_TYPE(a.type, T, {
+    const auto kernel = vec ? attention_step_kernel<T, true> : attention_step_kernel<T, false>;
+    kernel<<<a.batch * a.heads, 256, 0, st>>>(a);
+  });
   ++*launches;
   return cudaGetLastError();
 }

@@ -24,54 +24,65 @@ __device__ __forceinline__ void store8(uint8_t* p, const uint16_t (&q)[4], int n
   }
 }
 
-// Rows by groups of 128: half a warp a group, 8 elements a lane.  Bound by memory: type + 1 bytes
-// an element.
+// Rows by groups of 128: half a warp a group, 8 elements a lane, four groups' loads on their way at a
+// time.  Bound by memory: type + 1 bytes an element.
 template <typename T>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(salt_quantize_q8_args a, int groups,
+__global__ void __launch_bounds__(256) quantize_rows_kernel(salt_quantize_q8_args a, unsigned groups,
                                                             bool vec_in, bool vec_out) {
+  constexpr int N = sizeof(T) == 4 ? 2 : 4;
   const int64_t n = (int64_t)a.rows * groups;
   const int lane = threadIdx.x & 15;
-  const int64_t step = (int64_t)gridDim.x * 16;
-  // all lanes of a warp take the same number of turns
-  for (int64_t first = blockIdx.x * 16ll + (threadIdx.x >> 5) * 2; first < n; first += step) {
-    const int64_t i = first + (threadIdx.x >> 4 & 1);
-    const bool live = i < n;
-    const int64_t row = live ? i / groups : 0;
-    const int g = live ? (int)(i - row * groups) : 0, at = g * kGroup + lane * 8;
-    const int m = live ? a.dim - at : 0;
-    const Pack<T, 8> p =
-        load_pack<T, 8>(static_cast<const T*>(a.x) + row * a.x_stride + at, m, vec_in);
+  const int64_t first = ((int64_t)blockIdx.x * N * 16) + (threadIdx.x >> 4);
+  // (a product of 32 bits where the rows allow it: a division of 64 would cost as much as the rest)
+  Pack<T, 8> p[N];
+  int64_t row[N];
+  int at[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int64_t g = first + i * 16;
+    row[i] = g >> 32 ? g / groups : (unsigned)g / groups;
+    at[i] = (int)(g - row[i] * groups) * kGroup + lane * 8;
+    p[i] = load_pack<T, 8>(static_cast<const T*>(a.x) + row[i] * a.x_stride + at[i],
+                           g < n ? a.dim - at[i] : 0, vec_in);
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int64_t g = first + i * 16;
     f32x2 v[4];
     float most = 0.f;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      v[k] = pair_of(p, 2 * k);
+      v[k] = pair_of(p[i], 2 * k);
       const float2 h = halves(v[k]);
       most = fmaxf(most, fmaxf(fabsf(h.x), fabsf(h.y)));
     }
 #pragma unroll
     for (int o = 8; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
     const E4m3Scale by(most);
-    if (live && lane == 0) a.scale[i] = by.scale;
+    if (g < n && lane == 0) a.scale[g] = by.scale;
     by.divide(v);
     uint16_t q[4];
     to_e4m3(q, v);
-    if (m > 0) store8(static_cast<uint8_t*>(a.out) + row * a.out_stride + at, q, m, vec_out);
+    if (g < n && at[i] < a.dim)
+      store8(static_cast<uint8_t*>(a.out) + row[i] * a.out_stride + at[i], q, a.dim - at[i], vec_out);
   }
 }
 
 // Tiles of 128 x 128 for scales of whole blocks, for transposed outputs, or both.  A thread holds 8
 // neighbouring rows of 8 columns; a transposed tile goes through shared memory, where 8 values of a
 // column lie together and their place in the column's 16 is turned by the column's pack, so that
-// a half-warp's writes spread over all banks.
+// a half-warp's writes spread over all banks.  Scales are made once a column (or tile) and read from
+// shared memory.  Bound by memory: type + 1 bytes an element.
 template <typename T, bool BLOCKS, bool TRANSPOSED>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2)
 quantize_tile_kernel(salt_quantize_q8_args a, int tiles_x, bool vec_in, bool vec_out) {
   __shared__ float red[8][kGroup];
+  __shared__ E4m3Scale scales[BLOCKS ? 1 : kGroup];
   __shared__ uint2 tile[TRANSPOSED ? kGroup * 16 : 1];
   const int ty = blockIdx.x / tiles_x, tx = blockIdx.x - ty * tiles_x;
   const int cp = threadIdx.x & 15, rg = threadIdx.x >> 4, warp = threadIdx.x >> 5;
   const int row0 = ty * kGroup + rg * 8, col0 = tx * kGroup + cp * 8;
+  const int up = (a.rows + kGroup - 1) / kGroup;
   Pack<T, 8> p[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i)
@@ -83,32 +94,38 @@ quantize_tile_kernel(salt_quantize_q8_args a, int tiles_x, bool vec_in, bool vec
     most[j] = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) most[j] = fmaxf(most[j], fabsf(to_f32(p[i].v[j])));
-    most[j] = fmaxf(most[j], __shfl_xor_sync(0xffffffffu, most[j], 16));
   }
   if (BLOCKS) {
 #pragma unroll
     for (int j = 1; j < 8; ++j) most[0] = fmaxf(most[0], most[j]);
 #pragma unroll
-    for (int o = 8; o; o >>= 1) most[0] = fmaxf(most[0], __shfl_xor_sync(0xffffffffu, most[0], o));
+    for (int o = 16; o; o >>= 1) most[0] = fmaxf(most[0], __shfl_xor_sync(0xffffffffu, most[0], o));
     if ((threadIdx.x & 31) == 0) red[0][warp] = most[0];
     __syncthreads();
-    for (int w = 0; w < 8; ++w) most[0] = fmaxf(most[0], red[0][w]);
+    if (threadIdx.x == 0) {
+      float m = 0.f;
+      for (int w = 0; w < 8; ++w) m = fmaxf(m, red[0][w]);
+      scales[0] = E4m3Scale(m);
+      a.scale[TRANSPOSED ? (int64_t)tx * up + ty : (int64_t)ty * tiles_x + tx] = scales[0].scale;
+    }
   } else {
-    if ((threadIdx.x & 16) == 0) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) red[warp][cp * 8 + j] = most[j];
+    for (int j = 0; j < 8; ++j) {
+      most[j] = fmaxf(most[j], __shfl_xor_sync(0xffffffffu, most[j], 16));
+      if ((threadIdx.x & 16) == 0) red[warp][cp * 8 + j] = most[j];
     }
     __syncthreads();
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      for (int w = 0; w < 8; ++w) most[j] = fmaxf(most[j], red[w][cp * 8 + j]);
+    if (threadIdx.x < kGroup) {
+      float m = 0.f;
+      for (int w = 0; w < 8; ++w) m = fmaxf(m, red[w][threadIdx.x]);
+      scales[threadIdx.x] = E4m3Scale(m);
+      const int col = tx * kGroup + threadIdx.x;
+      if (col < a.dim) a.scale[(int64_t)col * up + ty] = scales[threadIdx.x].scale;
+    }
   }
-  const int up = (a.rows + kGroup - 1) / kGroup;
-  if (BLOCKS && threadIdx.x == 0)
-    a.scale[TRANSPOSED ? (int64_t)tx * up + ty : (int64_t)ty * tiles_x + tx] =
-        E4m3Scale(most[0]).scale;
+  __syncthreads();
   if constexpr (!TRANSPOSED) {
-    const E4m3Scale by(most[0]);
+    const E4m3Scale by = scales[0];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       f32x2 v[4];
@@ -124,8 +141,7 @@ quantize_tile_kernel(salt_quantize_q8_args a, int tiles_x, bool vec_in, bool vec
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const E4m3Scale by(most[BLOCKS ? 0 : j]);
-      if (!BLOCKS && rg == 0 && col0 + j < a.dim) a.scale[(int64_t)(col0 + j) * up + ty] = by.scale;
+      const E4m3Scale by = scales[BLOCKS ? 0 : cp * 8 + j];
       f32x2 v[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k)
@@ -160,10 +176,11 @@ cudaError_t quantize_q8_launch(const salt_quantize_q8_args& a, cudaStream_t st, 
   const bool vec_in = pack_rows(a.x, 8, size, a.x_stride);
   const bool vec_out = packed_rows(a.out, 8, 1, a.out_stride, 0);
   if (!a.blocks && !a.transposed) {
-    const int64_t blocks = ((int64_t)a.rows * groups + 15) / 16;
-    SALT_WITH_TYPE(a.type, T,
-                   quantize_rows_kernel<T><<<(unsigned)std::min<int64_t>(blocks, 148 * 16), 256, 0,
-                                             st>>>(a, groups, vec_in, vec_out));
+    const int each = 16 * (a.type == SALT_F32 ? 2 : 4);  // groups of a block
+    const int64_t blocks = ((int64_t)a.rows * groups + each - 1) / each;
+    if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    SALT_WITH_TYPE(a.type, T, quantize_rows_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(
+                                  a, groups, vec_in, vec_out));
   } else {
     const int64_t up = (a.rows + (int64_t)kGroup - 1) / kGroup, tiles = up * groups;
     if (tiles > 0x7fffffff) return cudaErrorInvalidConfiguration;

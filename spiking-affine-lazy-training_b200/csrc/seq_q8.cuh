@@ -24,6 +24,7 @@ constexpr float kE4m3Max = 448.f;
 struct E4m3Scale {
   float scale, lift;
   f32x2 high, low;
+  E4m3Scale() = default;
   __device__ __forceinline__ explicit E4m3Scale(float m) : lift(1.f) {
     float divisor;
     if (m >= 0x1p-60f && m < 0x1p60f) {
