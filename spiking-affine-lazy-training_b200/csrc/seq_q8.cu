@@ -1,4 +1,6 @@
 // Quantisation to 8 bits with a scale for every 128 values.
+#include <type_traits>
+
 #include "seq_q8.cuh"
 #include "sequence.cuh"
 
@@ -24,46 +26,89 @@ __device__ __forceinline__ void store8(uint8_t* p, const uint16_t (&q)[4], int n
   }
 }
 
+// The largest magnitudes of a pack, NaNs left out.
+__device__ __forceinline__ float largest(const Pack<float, 8>& p) {
+  float m = fabsf(p.v[0]);
+#pragma unroll
+  for (int i = 1; i < 8; ++i) m = fmaxf(m, fabsf(p.v[i]));
+  return fmaxf(m, 0.f);
+}
+template <typename T>
+__device__ __forceinline__ float largest(const Pack<T, 8>& p) {
+  using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
+  const T2* q = reinterpret_cast<const T2*>(&p);
+  const T2 m = __hmax2(__hmax2(__habs2(q[0]), __habs2(q[1])), __hmax2(__habs2(q[2]), __habs2(q[3])));
+  return fmaxf(fmaxf(to_f32(m.x), to_f32(m.y)), 0.f);
+}
+// The same of each column of 8 packs.
+__device__ __forceinline__ void column_largest(float (&m)[8], const Pack<float, 8> (&p)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    m[j] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m[j] = fmaxf(m[j], fabsf(p[i].v[j]));
+  }
+}
+template <typename T>
+__device__ __forceinline__ void column_largest(float (&m)[8], const Pack<T, 8> (&p)[8]) {
+  using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    T2 x = __habs2(reinterpret_cast<const T2*>(&p[0])[j]);
+#pragma unroll
+    for (int i = 1; i < 8; ++i) x = __hmax2(x, __habs2(reinterpret_cast<const T2*>(&p[i])[j]));
+    m[2 * j] = fmaxf(to_f32(x.x), 0.f), m[2 * j + 1] = fmaxf(to_f32(x.y), 0.f);
+  }
+}
+// A pack of a row, zeros where `live` is not: whole ones go out before anything depends on them.
+template <typename T, bool VEC>
+__device__ __forceinline__ Pack<T, 8> fetch(const T* row, int at, int dim, bool live) {
+  if (!VEC) return load_pack<T, 8>(row + at, live ? dim - at : 0, false);
+  return load_whole<T, 8>(row, live ? at : dim, dim);
+}
+template <typename T>
+__device__ __forceinline__ void clear(Pack<T, 8>& p) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) p.v[i] = from_f32<T>(0.f);
+}
+
 // Rows by groups of 128: half a warp a group, 8 elements a lane, four groups' loads on their way at a
 // time.  Bound by memory: type + 1 bytes an element.
-template <typename T>
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(salt_quantize_q8_args a, unsigned groups,
-                                                            bool vec_in, bool vec_out) {
+                                                            bool vec_out) {
   constexpr int N = sizeof(T) == 4 ? 2 : 4;
   const int64_t n = (int64_t)a.rows * groups;
   const int lane = threadIdx.x & 15;
   const int64_t first = ((int64_t)blockIdx.x * N * 16) + (threadIdx.x >> 4);
-  // (a product of 32 bits where the rows allow it: a division of 64 would cost as much as the rest)
+  // (a division of 32 bits where the rows allow it: one of 64 would cost as much as the rest)
   Pack<T, 8> p[N];
   int64_t row[N];
   int at[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int64_t g = first + i * 16;
-    row[i] = g >> 32 ? g / groups : (unsigned)g / groups;
+    row[i] = n >> 32 ? g / groups : (unsigned)g / groups;
     at[i] = (int)(g - row[i] * groups) * kGroup + lane * 8;
-    p[i] = load_pack<T, 8>(static_cast<const T*>(a.x) + row[i] * a.x_stride + at[i],
-                           g < n ? a.dim - at[i] : 0, vec_in);
+    p[i] = fetch<T, VEC>(static_cast<const T*>(a.x) + (g < n ? row[i] : 0) * a.x_stride, at[i], a.dim,
+                         g < n);
   }
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int64_t g = first + i * 16;
-    f32x2 v[4];
-    float most = 0.f;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      v[k] = pair_of(p[i], 2 * k);
-      const float2 h = halves(v[k]);
-      most = fmaxf(most, fmaxf(fabsf(h.x), fabsf(h.y)));
-    }
+    const bool live = g < n && at[i] < a.dim;
+    float most = VEC && !live ? 0.f : largest(p[i]);
 #pragma unroll
     for (int o = 8; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
     const E4m3Scale by(most);
     if (g < n && lane == 0) a.scale[g] = by.scale;
+    f32x2 v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = pair_of(p[i], 2 * k);
     by.divide(v);
     uint16_t q[4];
     to_e4m3(q, v);
-    if (g < n && at[i] < a.dim)
+    if (live)
       store8(static_cast<uint8_t*>(a.out) + row[i] * a.out_stride + at[i], q, a.dim - at[i], vec_out);
   }
 }
@@ -73,9 +118,9 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(salt_quantize_q8_arg
 // column lie together and their place in the column's 16 is turned by the column's pack, so that
 // a half-warp's writes spread over all banks.  Scales are made once a column (or tile) and read from
 // shared memory.  Bound by memory: type + 1 bytes an element.
-template <typename T, bool BLOCKS, bool TRANSPOSED>
+template <typename T, bool VEC, bool BLOCKS, bool TRANSPOSED>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2)
-quantize_tile_kernel(salt_quantize_q8_args a, int tiles_x, bool vec_in, bool vec_out) {
+quantize_tile_kernel(salt_quantize_q8_args a, int tiles_x, bool vec_out) {
   __shared__ float red[8][kGroup];
   __shared__ E4m3Scale scales[BLOCKS ? 1 : kGroup];
   __shared__ uint2 tile[TRANSPOSED ? kGroup * 16 : 1];
@@ -86,14 +131,19 @@ quantize_tile_kernel(salt_quantize_q8_args a, int tiles_x, bool vec_in, bool vec
   Pack<T, 8> p[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i)
-    p[i] = load_pack<T, 8>(static_cast<const T*>(a.x) + (int64_t)(row0 + i) * a.x_stride + col0,
-                           row0 + i < a.rows ? a.dim - col0 : 0, vec_in);
-  float most[8];  // of each column
+    p[i] = fetch<T, VEC>(static_cast<const T*>(a.x) + (int64_t)min(row0 + i, a.rows - 1) * a.x_stride,
+                         col0, a.dim, row0 + i < a.rows);
+  if (VEC && (row0 + 8 > a.rows || col0 >= a.dim)) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    most[j] = 0.f;
+    for (int i = 0; i < 8; ++i)
+      if (row0 + i >= a.rows || col0 >= a.dim) clear(p[i]);
+  }
+  float most[8];  // of each column, or (blocks) of each row
+  if (BLOCKS) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) most[j] = fmaxf(most[j], fabsf(to_f32(p[i].v[j])));
+    for (int j = 0; j < 8; ++j) most[j] = largest(p[j]);
+  } else {
+    column_largest(most, p);
   }
   if (BLOCKS) {
 #pragma unroll
@@ -173,22 +223,28 @@ cudaError_t quantize_q8_launch(const salt_quantize_q8_args& a, cudaStream_t st, 
   if (!a.rows) return cudaSuccess;
   const int groups = (a.dim + kGroup - 1) / kGroup;
   const size_t size = type_size(a.type);
-  const bool vec_in = pack_rows(a.x, 8, size, a.x_stride);
+  const bool vec_in = a.dim % 8 == 0 && pack_rows(a.x, 8, size, a.x_stride);
   const bool vec_out = packed_rows(a.out, 8, 1, a.out_stride, 0);
   if (!a.blocks && !a.transposed) {
     const int each = 16 * (a.type == SALT_F32 ? 2 : 4);  // groups of a block
     const int64_t blocks = ((int64_t)a.rows * groups + each - 1) / each;
     if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    SALT_WITH_TYPE(a.type, T, quantize_rows_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(
-                                  a, groups, vec_in, vec_out));
+    SALT_WITH_TYPE(a.type, T, {
+      const auto kernel = vec_in ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>;
+      kernel<<<(unsigned)blocks, 256, 0, st>>>(a, groups, vec_out);
+    });
   } else {
     const int64_t up = (a.rows + (int64_t)kGroup - 1) / kGroup, tiles = up * groups;
     if (tiles > 0x7fffffff) return cudaErrorInvalidConfiguration;
     SALT_WITH_TYPE(a.type, T, {
-      const auto kernel = !a.transposed ? quantize_tile_kernel<T, true, false>
-                          : a.blocks    ? quantize_tile_kernel<T, true, true>
-                                        : quantize_tile_kernel<T, false, true>;
-      kernel<<<(unsigned)tiles, 256, 0, st>>>(a, groups, vec_in, vec_out);
+      const auto kernel =
+          vec_in ? (!a.transposed ? quantize_tile_kernel<T, true, true, false>
+                    : a.blocks    ? quantize_tile_kernel<T, true, true, true>
+                                  : quantize_tile_kernel<T, true, false, true>)
+                 : (!a.transposed ? quantize_tile_kernel<T, false, true, false>
+                    : a.blocks    ? quantize_tile_kernel<T, false, true, true>
+                                  : quantize_tile_kernel<T, false, false, true>);
+      kernel<<<(unsigned)tiles, 256, 0, st>>>(a, groups, vec_out);
     });
   }
   ++*launches;
