@@ -21,6 +21,8 @@ constexpr int kRing = 8;  // groups whose scales are in flight
 constexpr int stages(int bn, bool swap) {
   return bn == 256 ? (swap ? 4 : 3) : bn == 128 ? (swap ? 6 : 5) : bn == 64 ? 8 : 9;
 }
+// Buffers of tensor memory for groups' products.
+constexpr int buffers(int bn) { return bn >= 64 ? 512 / bn : 8; }
 constexpr int stage_bytes(int bn) { return (kTileA + bn) * kGroup; }
 constexpr int shared_bytes(int bn, bool swap) {
   return stages(bn, swap) * stage_bytes(bn) + (swap ? 0 : kSums / 32 * 4096) + 1024;
@@ -50,13 +52,13 @@ template <int BN, bool SWAP, typename T>
 __global__ void __launch_bounds__(kThreads, 1)
 matmul_q8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                  const __grid_constant__ CUtensorMap map_out, const Product p) {
-  constexpr int S = stages(BN, SWAP);
+  constexpr int S = stages(BN, SWAP), B = buffers(BN);
   constexpr int H = BN / 2, PIECE = H < 16 ? H : 16;  // a warp's columns, and those of a load
   constexpr int kCopies = kSums / 32, kProducts = kCopies + 1, kScales = kCopies + 2;  // warps
   extern __shared__ uint8_t raw[];
   uint8_t* tiles = raw + (1024 - tc::shared_at(raw) % 1024) % 1024;
   uint8_t* staged = tiles + S * stage_bytes(BN);  // SWAP = false: 4 KB a warp for rows of out
-  __shared__ uint64_t full[S], empty[S], sum_full[2], sum_empty[2];
+  __shared__ uint64_t full[S], empty[S], sum_full[B], sum_empty[B];
   __shared__ uint32_t tmem_at;
   constexpr int kScalesB = SWAP ? BN : 4;  // of each column, or of each block of columns
   __shared__ __align__(16) float scales_a[kRing][kTileA], scales_b[kRing][kScalesB];
@@ -67,7 +69,7 @@ matmul_q8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       tc::barrier_init(&full[i], 1);
       tc::barrier_init(&empty[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < B; ++i) {
       tc::barrier_init(&sum_full[i], 1);
       tc::barrier_init(&sum_empty[i], kSums / 32);
     }
@@ -79,7 +81,7 @@ matmul_q8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     tc::prefetch_map(&map_a);
     tc::prefetch_map(&map_b);
   }
-  constexpr uint32_t kColumns = 2 * BN < 32 ? 32 : 2 * BN;
+  constexpr uint32_t kColumns = B * BN;
   if (warp == kProducts) tc::tmem_alloc(&tmem_at, kColumns);
   tc::fence_before();
   __syncthreads();
@@ -144,7 +146,7 @@ matmul_q8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
           tc::products_done(&sum_full[buffer]);
           tc::products_done(&empty[stage]);
           if (++stage == S) stage = 0, phase ^= 1;
-          if (++buffer == 2) buffer = 0, sum_phase ^= 1;
+          if (++buffer == B) buffer = 0, sum_phase ^= 1;
         }
       }
     }
@@ -229,7 +231,7 @@ matmul_q8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         __syncwarp();
         tc::barrier_arrive_if_zero(&scales_empty[slot], lane);
         if (++slot == kRing) slot = 0, slot_phase ^= 1;
-        if (++buffer == 2) buffer = 0, phase ^= 1;
+        if (++buffer == B) buffer = 0, phase ^= 1;
       }
       if (!tries) {  // a result that nobody can take for one
 #pragma unroll
@@ -349,7 +351,7 @@ __global__ void __launch_bounds__(256) align_rows_kernel(const uint8_t* from, in
                                                          int64_t rows, int k, uint4* to, int units) {
   const int64_t n = rows * units;
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
-    const int64_t row = i / units;
+    const int64_t row = n >> 32 ? i / units : (unsigned)i / (unsigned)units;
     const int at = (int)(i - row * units) * 16;
     const uint8_t* p = from + row * stride + at;
     uint32_t w[4] = {};
@@ -475,32 +477,54 @@ cudaError_t run(const salt_matmul_q8_args& a, const Operand& x, const Operand& w
   p.bias = a.bias;
   p.bias_f32 = a.bias_type == SALT_F32;
   const int shift_w = a.weight_rows ? 0 : 7;
-  const int64_t tiles_w = (a.n + kTileA - 1) / kTileA;
-  if (!a.weight_rows && a.rows > 128) {
-    p.rows_a = a.rows, p.rows_b = a.n;
-    p.scale_a = a.x_scale, p.scale_b = a.weight_scale;
-    p.shift_a = 0, p.shift_b = shift_w;
-    p.vec = packed_rows(a.out, 16, sizeof(T), a.out_stride, 0);
-    const int64_t wide = ((a.rows + 127ll) / 128) * ((a.n + 255ll) / 256);
-    if (wide >= 148) return launch<256, false, T>(x, w, a.k, p, st, launches);
-    return launch<128, false, T>(x, w, a.k, p, st, launches);
+  // Time in rounds of resident blocks (one an SM), counted in groups of a tile.  `each` is what a group
+  // of a tile takes, in us: measured with K = 2048 to 8192 at full rounds.
+  const auto time = [&](int64_t tiles, double each, int split) {
+    return (double)((tiles * split + 147) / 148) * (each * ((p.groups + split - 1) / split) + 1) +
+           (split > 1 ? 2 : 0);
+  };
+  const auto tiles = [&](int64_t lanes, int64_t columns, int bn) {
+    return ((lanes + kTileA - 1) / kTileA) * ((columns + bn - 1) / bn);
+  };
+  // few tiles: blocks share the depth of each
+  const auto split_of = [&](int bn) {
+    const int64_t n = tiles(a.n, a.rows, bn);
+    int s = 1;
+    while (s < kMostSplit && n * s * 2 <= 148 && p.groups >= s * 4) s *= 2;
+    return s;
+  };
+  const auto by_columns = [&](int bn, double each) {
+    return time(tiles(a.n, a.rows, bn), each, split_of(bn));
+  };
+  const double least = std::min(by_columns(128, 0.5), by_columns(256, 1.0) + (split_of(256) > 1 ? 1e9 : 0));
+  if (!a.weight_rows && a.rows > 64) {
+    const double wide = time(tiles(a.rows, a.n, 256), 0.63, 1),
+                 narrow = time(tiles(a.rows, a.n, 128), 0.5, 1);
+    if (std::min(wide, narrow) <= least) {
+      p.rows_a = a.rows, p.rows_b = a.n;
+      p.scale_a = a.x_scale, p.scale_b = a.weight_scale;
+      p.shift_a = 0, p.shift_b = shift_w;
+      p.vec = packed_rows(a.out, 16, sizeof(T), a.out_stride, 0);
+      return wide <= narrow ? launch<256, false, T>(x, w, a.k, p, st, launches)
+                            : launch<128, false, T>(x, w, a.k, p, st, launches);
+    }
   }
   p.rows_a = a.n, p.rows_b = a.rows;
   p.scale_a = a.weight_scale, p.scale_b = a.x_scale;
   p.shift_a = shift_w, p.shift_b = 0;
-  // few tiles: blocks share the depth of each
-  auto split = [&](int bn) {
-    const int64_t tiles = tiles_w * ((a.rows + bn - 1) / bn);
-    int s = 1;
-    while (s < kMostSplit && tiles * s * 2 <= 148 && p.groups >= s * 4) s *= 2;
-    return s;
-  };
-  if (a.rows <= 16) return p.split = split(16), launch<16, true, T>(w, x, a.k, p, st, launches);
-  if (a.rows <= 32) return p.split = split(32), launch<32, true, T>(w, x, a.k, p, st, launches);
-  if (a.rows <= 64) return p.split = split(64), launch<64, true, T>(w, x, a.k, p, st, launches);
-  if (tiles_w * ((a.rows + 255ll) / 256) < 148)
-    return p.split = split(128), launch<128, true, T>(w, x, a.k, p, st, launches);
-  return launch<256, true, T>(w, x, a.k, p, st, launches);
+  const int bn = a.rows <= 16   ? 16
+                 : a.rows <= 32 ? 32
+                 : a.rows <= 64 ? 64
+                 : by_columns(128, 0.5) <= least ? 128
+                                                 : 256;
+  p.split = bn == 256 ? 1 : split_of(bn);
+  switch (bn) {
+    case 16: return launch<16, true, T>(w, x, a.k, p, st, launches);
+    case 32: return launch<32, true, T>(w, x, a.k, p, st, launches);
+    case 64: return launch<64, true, T>(w, x, a.k, p, st, launches);
+    case 128: return launch<128, true, T>(w, x, a.k, p, st, launches);
+    default: return launch<256, true, T>(w, x, a.k, p, st, launches);
+  }
 }
 
 }  // namespace
