@@ -32,7 +32,8 @@ struct Pass {
   // set by the launch
   int segments, seg_chunks;  // segments of a row that run side by side, chunks of each
   float* seg_states;         // (batch, heads, segments, dk, dv): what each adds to the state
-  bool vec, vec_out, copies_out;
+  int width_q, width_k, width_v;  // values of one load of the rows
+  bool vec_out, copies_out;
 };
 
 __device__ __forceinline__ float decay_of(const float* g, int h) {
@@ -90,25 +91,55 @@ __device__ __forceinline__ void split2(uint32_t (&to)[N], float x, float y) {
   }
 }
 
-// Rows of `dim` values at p (token t at p + t * stride; `count` of them, the rest zero) to `parts` of
-// panels of 64 columns from column `from`.
+// Rows of `dim` values at p (token t at p + t * stride; `count` of them, the rest zero) from column
+// `from` on: a thread's packs of 8, then their parts in panels of 64 columns.
 template <typename T, int PANELS, int C>
-__device__ __forceinline__ void load_rows(uint8_t* to, const T* p, int64_t stride, int count, int from,
-                                          int dim, bool vec) {
-  constexpr int P = parts_of<T>(), U = PANELS * 8;
-  for (int i = threadIdx.x; i < C * U; i += kWorkers) {
-    const int row = i / U, u = i % U, at = from + u * 8;
-    const Pack<T, 8> x = load_pack<T, 8>(p + row * stride + at, row < count ? dim - at : 0, vec);
-    uint32_t parts[4][P];
+struct ByThreads {
+  static constexpr int U = PANELS * 8, N = C * U / kWorkers;
+  Pack<T, 8> p[N];
+  // `width`: values of a load that every row's start and length allow, 8, 4 or 1
+  __device__ __forceinline__ void fetch(const T* from_p, int64_t stride, int count, int from, int dim,
+                                        int width) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) split2<P>(parts[k], to_f32(x.v[2 * k]), to_f32(x.v[2 * k + 1]));
-    uint8_t* place = to + (u >> 3) * C * 128 + row * 128 + (((u & 7) ^ (row & 7)) << 4);
+    for (int i = 0; i < N; ++i) {
+      const int x = threadIdx.x + i * kWorkers, row = x / U, at = from + x % U * 8;
+      const T* r = from_p + (row < count ? row : 0) * stride;
+      if (width == 8) {
+        p[i] = load_whole<T, 8>(r, at, dim);
+      } else if (width == 4) {
+        const Pack<T, 4> lo = load_whole<T, 4>(r, at, dim), hi = load_whole<T, 4>(r, at + 4, dim);
 #pragma unroll
-    for (int j = 0; j < P; ++j)
-      *reinterpret_cast<uint4*>(place + j * PANELS * C * 128) =
-          make_uint4(parts[0][j], parts[1][j], parts[2][j], parts[3][j]);
+        for (int k = 0; k < 4; ++k) {
+          p[i].v[k] = lo.v[k];
+          p[i].v[k + 4] = at + 4 < dim ? hi.v[k] : from_f32<T>(0.f);
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) p[i].v[k] = at + k < dim ? r[at + k] : from_f32<T>(0.f);
+      }
+      if (row >= count || at >= dim) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) p[i].v[k] = from_f32<T>(0.f);
+      }
+    }
   }
-}
+  __device__ __forceinline__ void store(uint8_t* to) const {
+    constexpr int P = parts_of<T>();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int x = threadIdx.x + i * kWorkers, row = x / U, u = x % U;
+      uint32_t parts[4][P];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        split2<P>(parts[k], to_f32(p[i].v[2 * k]), to_f32(p[i].v[2 * k + 1]));
+      uint8_t* place = to + (u >> 3) * C * 128 + row * 128 + (((u & 7) ^ (row & 7)) << 4);
+#pragma unroll
+      for (int j = 0; j < P; ++j)
+        *reinterpret_cast<uint4*>(place + j * PANELS * C * 128) =
+            make_uint4(parts[0][j], parts[1][j], parts[2][j], parts[3][j]);
+    }
+  }
+};
 
 // One pass over chunks of C tokens (natural order; from the last one where `reverse`):
 //   out = row weight * (q S) + (q k^T under a triangle of decays) v;
@@ -358,11 +389,15 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         }
       } else {
         const int64_t t = (int64_t)c * C;
+        ByThreads<T, PANELS, C> from_q, from_k;
+        ByThreads<T, 1, C> from_v;
+        from_v.fetch(row_of<T>(a.v, b, t, h, a.dv), a.v.token, count, col0, a.dv, a.width_v);
+        from_k.fetch(row_of<T>(a.k, b, t, h, a.dk), a.k.token, count, 0, a.dk, a.width_k);
         if (!STATE)
-          load_rows<T, PANELS, C>(sm + L::q, row_of<T>(a.q, b, t, h, a.dk), a.q.token, count, 0, a.dk,
-                                  a.vec);
-        load_rows<T, PANELS, C>(k, row_of<T>(a.k, b, t, h, a.dk), a.k.token, count, 0, a.dk, a.vec);
-        load_rows<T, 1, C>(v, row_of<T>(a.v, b, t, h, a.dv), a.v.token, count, col0, a.dv, a.vec);
+          from_q.fetch(row_of<T>(a.q, b, t, h, a.dk), a.q.token, count, 0, a.dk, a.width_q);
+        from_v.store(v);
+        from_k.store(k);
+        if (!STATE) from_q.store(sm + L::q);
         tc::named_sync(1, kWorkers);
       }
 #pragma unroll
@@ -610,12 +645,20 @@ __global__ void __launch_bounds__(256) join_segments_kernel(const Pass a, int ch
   const int row = i / a.dv, col = i - row * a.dv;
   float s = a.initial ? a.initial[(int64_t)bh * each + (a.initial_t ? col * a.dk + row : i)] : 0.f;
   float* at = a.seg_states + (int64_t)bh * a.segments * each + i;
-  for (int x = 0; x < a.segments; ++x) {
-    const int seg = a.reverse ? a.segments - 1 - x : x;
-    const int first = seg * a.seg_chunks * chunk, count = min(first + a.seg_chunks * chunk, n) - first;
-    const float added = x + 1 < a.segments ? at[(int64_t)seg * each] : 0.f;
-    at[(int64_t)seg * each] = s;
-    if (count > 0) s = fmaf(s, exp2f(g * (float)count), added);
+  const auto place = [&](int x) { return at + (int64_t)(a.reverse ? a.segments - 1 - x : x) * each; };
+  for (int x0 = 0; x0 < a.segments; x0 += 8) {
+    float added[8];  // (loaded before the first store, which the compiler would keep in front of them)
+#pragma unroll
+    for (int x = 0; x < 8; ++x) added[x] = x0 + x + 1 < a.segments ? *place(x0 + x) : 0.f;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      if (x0 + x >= a.segments) break;
+      const int seg = a.reverse ? a.segments - 1 - x0 - x : x0 + x;
+      const int first = seg * a.seg_chunks * chunk,
+                count = min(first + a.seg_chunks * chunk, n) - first;
+      *place(x0 + x) = s;
+      if (count > 0) s = fmaf(s, exp2f(g * (float)count), added[x]);
+    }
   }
 }
 
@@ -671,7 +714,7 @@ cudaError_t start(const CUtensorMap (&maps)[4], const Pass& p, int64_t blocks, c
 
 // Segments of a row: the number that needs the least time in rounds of resident blocks (one an SM),
 // counted in chunks of the main pass.  A block takes about as long as a chunk to begin and end; the
-// first pass, over all but the last segment, takes two fifths of a chunk's time for each, and with the
+// first pass, over all but the last segment, takes about half of a chunk's time for each, and with the
 // joining of its states two more.
 int segments_of(int64_t blocks, int chunks) {
   int best = 1;
@@ -679,7 +722,7 @@ int segments_of(int64_t blocks, int chunks) {
   for (int s = 1; s <= 64 && s <= chunks && blocks * s <= 148 * 8; ++s) {
     const int each = (chunks + s - 1) / s;
     const double rounds = (double)((blocks * s + 147) / 148);
-    const double time = rounds * (each + 1) + (s > 1 ? rounds * (0.4 * each + 1) + 2 : 0);
+    const double time = rounds * (each + 1) + (s > 1 ? rounds * (0.55 * each + 1) + 2 : 0);
     if (time < least) least = time, best = s;
   }
   return best;
@@ -724,11 +767,13 @@ cudaError_t run_pass(Pass p, void* ws, cudaStream_t st, int* launches) {
   p.segments = pass_segments<T>(p.batch, p.heads, p.dv, p.len);
   p.seg_chunks = std::max(1, (chunks + p.segments - 1) / p.segments);
   p.seg_states = static_cast<float*>(ws);
-  const auto packed = [&](const Rows& r, int dim) {
-    return pack_rows(r.p, 8, sizeof(T), r.batch, r.token) && dim * sizeof(T) % 16 == 0;
+  const auto width = [&](const Rows& r, int dim) {
+    return dim % 8 == 0 && pack_rows(r.p, 8, sizeof(T), r.batch, r.token)   ? 8
+           : dim % 4 == 0 && pack_rows(r.p, 4, sizeof(T), r.batch, r.token) ? 4
+                                                                            : 1;
   };
   p.copies_out = false;
-  p.vec = packed(p.q, p.dk) && packed(p.k, p.dk) && packed(p.v, p.dv);
+  p.width_q = width(p.q, p.dk), p.width_k = width(p.k, p.dk), p.width_v = width(p.v, p.dv);
   p.vec_out = packed_rows(p.out, 16, sizeof(O), p.out_batch, p.out_token) &&
               p.dv * sizeof(O) % 16 == 0;
   CUtensorMap maps[4] = {};
