@@ -12,13 +12,8 @@
 namespace salt {
 namespace {
 
-struct Rows {
-  const void* p;
-  int64_t batch, token;
-  int share;  // heads that read one head of this array
-};
 struct Pass {
-  Rows q, k, v;
+  int q_share, k_share, v_share;  // heads that read one head of an array
   int dk, dv, heads, len, batch;
   float scale;
   bool reverse;
@@ -32,18 +27,12 @@ struct Pass {
   // set by the launch
   int segments, seg_chunks;  // segments of a row that run side by side, chunks of each
   float* seg_states;         // (batch, heads, segments, dk, dv): what each adds to the state
-  int width_q, width_k, width_v;  // values of one load of the rows
   bool vec_out, copies_out;
 };
 
 __device__ __forceinline__ float decay_of(const float* g, int h) {
   const float v = g[h];
   return v > 0.f ? 0.f : v < -200.f ? -200.f : v;  // a NaN stays one
-}
-
-template <typename T>
-__device__ __forceinline__ const T* row_of(const Rows& r, int b, int64_t t, int h, int dim) {
-  return static_cast<const T*>(r.p) + b * r.batch + t * r.token + (int64_t)(h / r.share) * dim;
 }
 
 constexpr int kTile = 64;      // columns of v that a block takes
@@ -55,23 +44,21 @@ constexpr int kWeighted = 3;   // parts of a weighted v
 template <typename T>
 constexpr int parts_of() { return sizeof(T) == 4 ? 3 : std::is_same<T, __half>::value ? 2 : 1; }
 // Tokens of a chunk, and parts of the states and of the weights within a chunk.
-template <typename T>
-constexpr int chunk_of() { return parts_of<T>() == 1 ? 128 : 64; }
-template <typename T>
-constexpr int state_parts() { return sizeof(T) == 4 ? 3 : 2; }
+constexpr int chunk_of(int parts) { return parts == 1 ? 128 : 64; }
+constexpr int state_parts(int parts) { return parts == 3 ? 3 : 2; }
 
 // Shared memory, all operands in rows of 128 bytes (tc::operand): q and k in panels of 64 columns,
-// part after part; k and v twice where copies run ahead.
-template <typename T, int PANELS, bool AHEAD>
+// part after part; k and v twice, for copies a chunk further ahead, where there is room.
+template <int P, int PANELS, typename O>
 struct Layout {
-  static constexpr int P = parts_of<T>(), C = chunk_of<T>(), B = AHEAD ? 2 : 1;
+  static constexpr int C = chunk_of(P), B = P == 3 ? 1 : 2;
   static constexpr int kPanel = C * 128, kKeys = P * PANELS * kPanel, kValues = P * kPanel;
+  static constexpr int kState = PANELS * 64 * 128;  // a part of the state
+  // rows of out, 16 columns of 32 rows a warp; without room for them out is stored from registers
+  static constexpr int kStaged = P == 1 && sizeof(O) == 4 ? 0 : 32 * 16 * sizeof(O);
   static constexpr int q = 0, k = q + kKeys, v = k + B * kKeys, weighted = v + B * kValues,
-                       state = weighted + kWeighted * kPanel,
-                       kState = PANELS * 64 * 128;  // a part of the state
-  static constexpr int
-      out = state + state_parts<T>() * kState,  // 1 KB a warp
-      bytes = out + (AHEAD ? 16 * 1024 : 0) + 1024;
+                       state = weighted + kWeighted * kPanel, out = state + state_parts(P) * kState,
+                       bytes = out + kWorkers / 32 * kStaged + 1024;
 };
 
 // Two values in parts of bfloat16: the upper 8 bits of what is left, time and again; the last of two
@@ -91,55 +78,32 @@ __device__ __forceinline__ void split2(uint32_t (&to)[N], float x, float y) {
   }
 }
 
-// Rows of `dim` values at p (token t at p + t * stride; `count` of them, the rest zero) from column
-// `from` on: a thread's packs of 8, then their parts in panels of 64 columns.
-template <typename T, int PANELS, int C>
-struct ByThreads {
-  static constexpr int U = PANELS * 8, N = C * U / kWorkers;
-  Pack<T, 8> p[N];
-  // `width`: values of a load that every row's start and length allow, 8, 4 or 1
-  __device__ __forceinline__ void fetch(const T* from_p, int64_t stride, int count, int from, int dim,
-                                        int width) {
+// An array (batch, len, heads, dim) of T in planes of bfloat16 parts (part, batch, len, heads, dim
+// rounded up to 8), zero past the rows' ends: what tensor copies can take of every type, alignment and
+// size.  Bound by memory.
+template <typename T>
+__global__ void __launch_bounds__(256) planes_kernel(const T* from, int64_t batch_stride, int64_t stride,
+                                                     int batch, int len, int heads, int dim,
+                                                     const int32_t* n_real, uint4* to, bool vec) {
+  constexpr int P = parts_of<T>();
+  const int units = (dim + 7) / 8, each = heads * units;
+  const int64_t n = (int64_t)batch * len * each;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+    const int64_t token = n >> 32 ? i / each : (unsigned)i / (unsigned)each;
+    const int in = (int)(i - token * each), h = in / units, at = (in - h * units) * 8;
+    const int b = (int)(n >> 32 ? token / len : (unsigned)token / (unsigned)len);
+    const int t = (int)(token - (int64_t)b * len);
+    const Pack<T, 8> p =
+        load_pack<T, 8>(from + b * batch_stride + t * stride + (int64_t)h * dim + at,
+                        t < row_tokens(n_real, b, len) ? dim - at : 0, vec);
+    uint32_t parts[4][P];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int x = threadIdx.x + i * kWorkers, row = x / U, at = from + x % U * 8;
-      const T* r = from_p + (row < count ? row : 0) * stride;
-      if (width == 8) {
-        p[i] = load_whole<T, 8>(r, at, dim);
-      } else if (width == 4) {
-        const Pack<T, 4> lo = load_whole<T, 4>(r, at, dim), hi = load_whole<T, 4>(r, at + 4, dim);
+    for (int k = 0; k < 4; ++k) split2<P>(parts[k], to_f32(p.v[2 * k]), to_f32(p.v[2 * k + 1]));
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          p[i].v[k] = lo.v[k];
-          p[i].v[k + 4] = at + 4 < dim ? hi.v[k] : from_f32<T>(0.f);
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) p[i].v[k] = at + k < dim ? r[at + k] : from_f32<T>(0.f);
-      }
-      if (row >= count || at >= dim) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) p[i].v[k] = from_f32<T>(0.f);
-      }
-    }
+    for (int j = 0; j < P; ++j)
+      to[j * n + i] = make_uint4(parts[0][j], parts[1][j], parts[2][j], parts[3][j]);
   }
-  __device__ __forceinline__ void store(uint8_t* to) const {
-    constexpr int P = parts_of<T>();
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int x = threadIdx.x + i * kWorkers, row = x / U, u = x % U;
-      uint32_t parts[4][P];
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        split2<P>(parts[k], to_f32(p[i].v[2 * k]), to_f32(p[i].v[2 * k + 1]));
-      uint8_t* place = to + (u >> 3) * C * 128 + row * 128 + (((u & 7) ^ (row & 7)) << 4);
-#pragma unroll
-      for (int j = 0; j < P; ++j)
-        *reinterpret_cast<uint4*>(place + j * PANELS * C * 128) =
-            make_uint4(parts[0][j], parts[1][j], parts[2][j], parts[3][j]);
-    }
-  }
-};
+}
 
 // One pass over chunks of C tokens (natural order; from the last one where `reverse`):
 //   out = row weight * (q S) + (q k^T under a triangle of decays) v;
@@ -152,17 +116,17 @@ struct ByThreads {
 // that states are good to 2^-24; states and the triangle's values, as operands for out, have three
 // parts for float32 and two (2^-16) for outputs of 16 bits.  Sums and states are float32; the state
 // is carried in registers.
-template <typename T, typename O, int PANELS, bool AHEAD, bool STATE>
+template <int P, typename O, int PANELS, bool STATE>
 __global__ void __launch_bounds__(kThreads, 1)
 attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                  const __grid_constant__ CUtensorMap map_v,
                  const __grid_constant__ CUtensorMap map_out, const Pass a) {
-  using L = Layout<T, PANELS, AHEAD>;
-  constexpr int C = L::C, P = L::P, SP = state_parts<T>(), DK = PANELS * 64;
+  using L = Layout<P, PANELS, O>;
+  constexpr int C = L::C, B = L::B, SP = state_parts(P), DK = PANELS * 64;
   constexpr int kPanel = L::kPanel;
   extern __shared__ uint8_t raw[];
   uint8_t* sm = raw + (1024 - tc::shared_at(raw) % 1024) % 1024;
-  __shared__ uint64_t loaded_q, loaded_k[2], loaded_v[2];  // copies
+  __shared__ uint64_t loaded_q, loaded_k[B], loaded_v[B];  // copies
   __shared__ uint64_t done_scores, done_q, done_state, done_out;  // products
   __shared__ uint64_t ready_chunk, ready_triangle;  // operands that threads wrote
   __shared__ uint32_t tmem_at;
@@ -191,9 +155,12 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   const auto tokens = [&](int c) { return min(C, n - c * C); };
 
   if (threadIdx.x == 0) {
-    uint64_t* ones[] = {&loaded_q, &loaded_k[0], &loaded_k[1], &loaded_v[0], &loaded_v[1],
-                        &done_q,   &done_scores, &done_state,  &done_out};
-    for (uint64_t* x : ones) tc::barrier_init(x, 1);
+    for (int i = 0; i < B; ++i) {
+      tc::barrier_init(&loaded_k[i], 1);
+      tc::barrier_init(&loaded_v[i], 1);
+    }
+    for (uint64_t* x : {&loaded_q, &done_q, &done_scores, &done_state, &done_out})
+      tc::barrier_init(x, 1);
     tc::barrier_init(&ready_chunk, kWorkers / 32);
     tc::barrier_init(&ready_triangle, kWorkers / 32);
     tc::barrier_init_fence();
@@ -217,31 +184,29 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 
   if (warp == kWorkers / 32) {
     if (tc::one_lane() && steps > 0) {
+      const auto fetch = [&](int to, const CUtensorMap* map, int panels, int col, int head, int i,
+                             uint64_t* barrier) {
+        tc::barrier_expect(barrier, P * panels * kPanel);
+        for (int x = 0; x < P * panels; ++x)
+          tc::load_box4(sm + to + x * kPanel, map, col + x % panels * 64, head, chunk(i) * C,
+                        x / panels * a.batch + b, barrier);
+      };
       const auto fetch_q = [&](int i) {
-        if (i >= steps) return;
-        tc::barrier_expect(&loaded_q, L::kKeys);
-        for (int x = 0; x < PANELS; ++x)
-          tc::load_box4(sm + L::q + x * kPanel, &map_q, x * 64, h / a.q.share, chunk(i) * C, b,
-                        &loaded_q);
+        if (i < steps) fetch(L::q, &map_q, PANELS, 0, h / a.q_share, i, &loaded_q);
       };
       const auto fetch_k = [&](int i) {
-        if (i >= steps) return;
-        tc::barrier_expect(&loaded_k[i & 1], L::kKeys);
-        for (int x = 0; x < PANELS; ++x)
-          tc::load_box4(sm + L::k + (i & 1) * L::kKeys + x * kPanel, &map_k, x * 64,
-                        h / a.k.share, chunk(i) * C, b, &loaded_k[i & 1]);
+        if (i < steps)
+          fetch(L::k + i % B * L::kKeys, &map_k, PANELS, 0, h / a.k_share, i, &loaded_k[i % B]);
       };
       const auto fetch_v = [&](int i) {
-        if (i >= steps) return;
-        tc::barrier_expect(&loaded_v[i & 1], L::kValues);
-        tc::load_box4(sm + L::v + (i & 1) * L::kValues, &map_v, col0, h / a.v.share, chunk(i) * C, b,
-                      &loaded_v[i & 1]);
+        if (i < steps)
+          fetch(L::v + i % B * L::kValues, &map_v, 1, col0, h / a.v_share, i, &loaded_v[i % B]);
       };
       const int depth = (a.dk + 15) / 16;
       const uint64_t q = tc::operand(sm + L::q, 1024), state = tc::operand(sm + L::state, 1024),
                      weighted = tc::operand(sm + L::weighted, 1024);
       const auto scores = [&](int i) {
-        const uint64_t k = tc::operand(sm + L::k + (AHEAD ? i & 1 : 0) * L::kKeys, 1024);
+        const uint64_t k = tc::operand(sm + L::k + i % B * L::kKeys, 1024);
         bool add = false;
 #pragma unroll
         for (int x = 0; x < P; ++x)
@@ -255,25 +220,21 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             }
         tc::products_done(&done_scores);
       };
-      if (AHEAD) {
-        fetch_v(0);
-        fetch_k(0);
-        if (!STATE) fetch_q(0);
-        fetch_v(1);
-        fetch_k(1);
-        tc::barrier_wait(&loaded_k[0], 0, tries);
-        if (!STATE) {
-          tc::barrier_wait(&loaded_q, 0, tries);
-          scores(0);
-        }
+      for (int i = 0; i < B; ++i) {
+        fetch_v(i);
+        fetch_k(i);
+        if (!STATE && i == 0) fetch_q(0);
+      }
+      tc::barrier_wait(&loaded_k[0], 0, tries);
+      if (!STATE) {
+        tc::barrier_wait(&loaded_q, 0, tries);
+        scores(0);
       }
 #pragma unroll 1
       for (int i = 0; i < steps; ++i) {
-        const int at = AHEAD ? i & 1 : 0;
         tc::barrier_wait(&ready_chunk, i & 1, tries);
         tc::fence_after();
         if (!STATE) {
-          if (!AHEAD) scores(i);
           bool add = false;
 #pragma unroll
           for (int x = 0; x < P; ++x)
@@ -290,7 +251,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           tc::products_done(&done_q);
         }
         {
-          const uint64_t k = tc::operand(sm + L::k + at * L::kKeys, 1024, kPanel);
+          const uint64_t k = tc::operand(sm + L::k + i % B * L::kKeys, 1024, kPanel);
           bool add = false;
 #pragma unroll
           for (int x = 0; x < P; ++x)
@@ -306,13 +267,11 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           tc::products_done(&done_state);
         }
         if (!STATE) {
-          if (AHEAD) {
-            tc::barrier_wait(&done_q, i & 1, tries);
-            fetch_q(i + 1);
-          }
+          tc::barrier_wait(&done_q, i & 1, tries);
+          fetch_q(i + 1);
           tc::barrier_wait(&ready_triangle, i & 1, tries);
           tc::fence_after();
-          const uint64_t v = tc::operand(sm + L::v + at * L::kValues, 1024);
+          const uint64_t v = tc::operand(sm + L::v + i % B * L::kValues, 1024);
           bool add = false;
 #pragma unroll
           for (int x = 0; x < SP; ++x)
@@ -327,17 +286,19 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
               }
           tc::products_done(&done_out);
         }
-        if (AHEAD && i + 1 < steps) {
-          tc::barrier_wait(&loaded_k[(i + 1) & 1], (i + 1) >> 1 & 1, tries);
-          if (!STATE) {
-            tc::barrier_wait(&loaded_q, (i + 1) & 1, tries);
-            scores(i + 1);
-          }
-          tc::barrier_wait(&done_state, i & 1, tries);
-          fetch_k(i + 2);
-          if (!STATE) tc::barrier_wait(&done_out, i & 1, tries);
-          fetch_v(i + 2);
-        }
+        if (i + 1 == steps) break;
+        const auto next = [&] {
+          tc::barrier_wait(&loaded_k[(i + 1) % B], (i + 1) / B & 1, tries);
+          if (STATE) return;
+          tc::barrier_wait(&loaded_q, (i + 1) & 1, tries);
+          scores(i + 1);
+        };
+        if (B == 2) next();
+        tc::barrier_wait(&done_state, i & 1, tries);
+        fetch_k(i + B);
+        if (!STATE) tc::barrier_wait(&done_out, i & 1, tries);
+        fetch_v(i + B);
+        if (B == 1) next();
       }
     }
     __syncwarp();
@@ -371,34 +332,19 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     };
     if (!STATE && steps > 0) store_state();
 
-    // Chunk i's operands: brought in where nobody copied ahead, rows past the end made zero, values
-    // weighted.
+    // Chunk i's operands: rows past the end made zero, values weighted.
     const auto begin = [&](int i) {
-      const int c = chunk(i), count = tokens(c), at = AHEAD ? i & 1 : 0;
-      uint8_t* k = sm + L::k + at * L::kKeys;
-      uint8_t* v = sm + L::v + at * L::kValues;
-      if (AHEAD) {
-        tc::barrier_wait_warp(&loaded_v[at], i >> 1 & 1, tries);
-        if (count < C) {
-          tc::barrier_wait_warp(&loaded_k[at], i >> 1 & 1, tries);
-          for (int x = threadIdx.x; x < (C - count) * PANELS * 8; x += kWorkers) {
-            const int r = count + x / (PANELS * 8), u = x % (PANELS * 8);
-            *reinterpret_cast<uint4*>(k + (u >> 3) * kPanel + r * 128 + ((u & 7) << 4)) =
-                make_uint4(0, 0, 0, 0);
-          }
+      const int count = tokens(chunk(i));
+      uint8_t* k = sm + L::k + i % B * L::kKeys;
+      uint8_t* v = sm + L::v + i % B * L::kValues;
+      tc::barrier_wait_warp(&loaded_v[i % B], i / B & 1, tries);
+      if (P == 1 && count < C) {  // (planes of several parts hold zeros there)
+        tc::barrier_wait_warp(&loaded_k[i % B], i / B & 1, tries);
+        for (int x = threadIdx.x; x < (C - count) * PANELS * 8; x += kWorkers) {
+          const int r = count + x / (PANELS * 8), u = x % (PANELS * 8);
+          *reinterpret_cast<uint4*>(k + (u >> 3) * kPanel + r * 128 + ((u & 7) << 4)) =
+              make_uint4(0, 0, 0, 0);
         }
-      } else {
-        const int64_t t = (int64_t)c * C;
-        ByThreads<T, PANELS, C> from_q, from_k;
-        ByThreads<T, 1, C> from_v;
-        from_v.fetch(row_of<T>(a.v, b, t, h, a.dv), a.v.token, count, col0, a.dv, a.width_v);
-        from_k.fetch(row_of<T>(a.k, b, t, h, a.dk), a.k.token, count, 0, a.dk, a.width_k);
-        if (!STATE)
-          from_q.fetch(row_of<T>(a.q, b, t, h, a.dk), a.q.token, count, 0, a.dk, a.width_q);
-        from_v.store(v);
-        from_k.store(k);
-        if (!STATE) from_q.store(sm + L::q);
-        tc::named_sync(1, kWorkers);
       }
 #pragma unroll
       for (int x = threadIdx.x; x < C * 8; x += kWorkers) {
@@ -483,18 +429,18 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             f[j] = __int_as_float(0x7fffffff);
         }
       }
-      if constexpr (AHEAD && sizeof(O) == 2) {
+      if constexpr (L::kStaged > 0) {
         if (a.copies_out) {
-          // 32 bytes a row, through shared memory: as stores from here every 16 bytes would be a line
+          // 16 columns a row, through shared memory: as stores from here every 16 bytes would be a line
           // of their own.  Rows past the end are zero anyway; those past `len` are left out.
-          uint8_t* to = sm + L::out + warp * 1024;
+          uint8_t* to = sm + L::out + warp * L::kStaged;
           if (lane == 0) tc::stores_read();
           __syncwarp();
-          store_pack<O, 8>(reinterpret_cast<O*>(to + lane * 32), f, 8, true);
-          store_pack<O, 8>(reinterpret_cast<O*>(to + lane * 32 + 16), f + 8, 8, true);
+          store_pack<O, 8>(reinterpret_cast<O*>(to) + lane * 16, f, 8, true);
+          store_pack<O, 8>(reinterpret_cast<O*>(to) + lane * 16 + 8, f + 8, 8, true);
           tc::fence_shared();
           __syncwarp();
-          if (lane == 0 && quarter * 32 < a.len - c * C && sc0 < a.dv)
+          if (lane == 0 && quarter * 32 < min(C, a.len - c * C) && sc0 < a.dv)
             tc::store_box4(&map_out, to, sc0, h, c * C + quarter * 32, b);
           return;
         }
@@ -512,7 +458,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       const int count = tokens(chunk(i));
       begin(i);
       if (!STATE) {
-        if (AHEAD && i > 0) finish(i - 1);
+        if (i > 0) finish(i - 1);
         // the triangle's weights
         tc::barrier_wait_warp(&done_scores, i & 1, tries);
         tc::fence_after();
@@ -592,21 +538,19 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         for (int j = 0; j < 16; ++j)
           if (bad[i % 3][part * 16 + j] >= 0) s[j] = __int_as_float(0x7fffffff);
       }
-      if (!STATE && !AHEAD) finish(i);
       if (i + 1 < steps) {
         if (!STATE) {
           tc::barrier_wait_warp(&done_q, i & 1, tries);
           store_state();
         }
-        // every warp is past the chunk before: its marks are free, and (where nobody copies ahead)
-        // every operand
+        // every warp is past the chunk before: its marks are free
         tc::named_sync(1, kWorkers);
         if (threadIdx.x < kTile) bad[(i + 2) % 3][threadIdx.x] = -1;
         if (threadIdx.x == 0) any_bad[(i + 2) % 3] = 0;
       }
     }
-    if (!STATE && AHEAD && steps > 0) finish(steps - 1);
-    if (AHEAD && lane == 0) tc::stores_done();
+    if (!STATE && steps > 0) finish(steps - 1);
+    if (!STATE && lane == 0) tc::stores_done();
     __syncwarp();
 
     const bool last = a.reverse ? seg == 0 : (c1 == chunks && (c0 < chunks || seg == 0));
@@ -680,30 +624,71 @@ __global__ void __launch_bounds__(256) sum_heads_kernel(const float* from, T* to
   }
 }
 
-// Boxes of `high` tokens x 64 columns of one head; for outputs x 16 columns, as they lie.
-bool head_map(CUtensorMap* map, const Rows& r, int dim, int heads, int len, int batch, int high,
-              bool out = false) {
+size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+
+// An array (batch, len, heads, dim) of the call, or its planes.
+struct Array {
+  const void* p;
+  int64_t batch_stride, stride;  // in elements
+  int heads, dim;
+};
+
+// Boxes of `high` tokens x `columns` of one head of an array of elements of `size` bytes, if tensor
+// copies can take it.
+bool head_map(CUtensorMap* map, const Array& x, size_t size, int len, int batch, int high, int columns,
+              bool swizzled) {
   const tc::EncodeTiled f = tc::encoder();
-  if (!f || !aligned16(r.p) || dim % 8) return false;
-  const int64_t token = len > 1 ? r.token * 2 : 16, row = batch > 1 ? r.batch * 2 : 16;
-  if (token % 16 || row % 16 || token < 16 || row < 16 || token >= tc::kMostStride ||
-      row >= tc::kMostStride)
+  const int64_t token = len > 1 ? x.stride * (int64_t)size : 16,
+                row = batch > 1 ? x.batch_stride * (int64_t)size : 16;
+  if (!f || !aligned16(x.p) || x.dim * size % 16 || token % 16 || row % 16 || token < 16 || row < 16 ||
+      token >= tc::kMostStride || row >= tc::kMostStride)
     return false;
-  const cuuint64_t dims[4] = {(cuuint64_t)dim, (cuuint64_t)(heads / r.share), (cuuint64_t)len,
+  const cuuint64_t dims[4] = {(cuuint64_t)x.dim, (cuuint64_t)x.heads, (cuuint64_t)len,
                               (cuuint64_t)batch};
-  const cuuint64_t strides[3] = {(cuuint64_t)dim * 2, (cuuint64_t)token, (cuuint64_t)row};
-  const cuuint32_t box[4] = {out ? 16u : 64u, 1, (cuuint32_t)high, 1}, unit[4] = {1, 1, 1, 1};
-  return f(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(r.p), dims, strides, box, unit,
-           CU_TENSOR_MAP_INTERLEAVE_NONE,
-           out ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
+  const cuuint64_t strides[3] = {(cuuint64_t)(x.dim * size), (cuuint64_t)token, (cuuint64_t)row};
+  const cuuint32_t box[4] = {(cuuint32_t)columns, 1, (cuuint32_t)high, 1}, unit[4] = {1, 1, 1, 1};
+  return f(map, size == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 4,
+           const_cast<void*>(x.p), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
+           swizzled ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
            CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, typename O, int PANELS, bool AHEAD, bool STATE>
+// The call's arrays as the pass takes them: bfloat16 as it lies where tensor copies can, else planes.
+template <typename T>
+bool as_it_lies(const Array& x, int len, int batch) {
+  CUtensorMap map;
+  return parts_of<T>() == 1 && head_map(&map, x, 2, len, batch, 128, 64, true);
+}
+template <typename T>
+size_t planes_bytes(const Array& x, int len, int batch) {
+  if (!len || !batch || as_it_lies<T>(x, len, batch)) return 0;
+  return align256((size_t)parts_of<T>() * batch * len * x.heads * ((x.dim + 7) / 8) * 16);
+}
+template <typename T>
+cudaError_t take(Array& x, int len, int batch, const int32_t* n_real, uint8_t*& ws, cudaStream_t st,
+                 int* launches) {
+  if (!len || !batch || as_it_lies<T>(x, len, batch)) return cudaSuccess;
+  const size_t bytes = planes_bytes<T>(x, len, batch);
+  const int units = (x.dim + 7) / 8;
+  const int64_t n = (int64_t)batch * len * x.heads * units;
+  planes_kernel<T><<<(unsigned)std::min<int64_t>((n + 255) / 256, 148 * 16), 256, 0, st>>>(
+      static_cast<const T*>(x.p), x.batch_stride, x.stride, batch, len, x.heads, x.dim, n_real,
+      reinterpret_cast<uint4*>(ws),
+      x.dim % 8 == 0 && pack_rows(x.p, 8, sizeof(T), x.batch_stride, x.stride));
+  ++*launches;
+  x.p = ws;
+  x.dim = units * 8;
+  x.stride = (int64_t)x.heads * x.dim;
+  x.batch_stride = x.stride * len;
+  ws += bytes;
+  return cudaGetLastError();
+}
+
+template <int P, typename O, int PANELS, bool STATE>
 cudaError_t start(const CUtensorMap (&maps)[4], const Pass& p, int64_t blocks, cudaStream_t st,
                   int* launches) {
-  const auto kernel = attention_kernel<T, O, PANELS, AHEAD, STATE>;
-  constexpr int bytes = Layout<T, PANELS, AHEAD>::bytes;
+  const auto kernel = attention_kernel<P, O, PANELS, STATE>;
+  constexpr int bytes = Layout<P, PANELS, O>::bytes;
   const cudaError_t e =
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return e;
@@ -729,66 +714,62 @@ int segments_of(int64_t blocks, int chunks) {
 }
 template <typename T>
 int pass_segments(int batch, int heads, int dv, int len) {
+  constexpr int C = chunk_of(parts_of<T>());
   const int64_t blocks = (int64_t)batch * heads * ((dv + kTile - 1) / kTile);
-  return blocks ? segments_of(blocks, (len + chunk_of<T>() - 1) / chunk_of<T>()) : 1;
+  return blocks ? segments_of(blocks, (len + C - 1) / C) : 1;
 }
-size_t align256(size_t n) { return (n + 255) / 256 * 256; }
-size_t segment_bytes(int type, int batch, int heads, int dk, int dv, int len) {
-  int s = 1;
-  SALT_WITH_TYPE(type, T, s = pass_segments<T>(batch, heads, dv, len));
+template <typename T>
+size_t segment_bytes(int batch, int heads, int dk, int dv, int len) {
+  const int s = pass_segments<T>(batch, heads, dv, len);
   return s == 1 ? 0 : align256(sizeof(float) * batch * heads * s * dk * dv);
 }
 
-template <typename T, typename O, int PANELS, bool AHEAD>
-cudaError_t run_ahead(const CUtensorMap (&maps)[4], const Pass& p, int64_t blocks, cudaStream_t st,
-                      int* launches) {
+template <int P, typename O, int PANELS>
+cudaError_t run_panels(const CUtensorMap (&maps)[4], const Pass& p, int64_t blocks, cudaStream_t st,
+                       int* launches) {
   if (p.segments > 1) {
     Pass first = p;
     first.initial = nullptr;
-    cudaError_t e = start<T, O, PANELS, AHEAD, true>(maps, first, blocks * p.segments, st, launches);
+    // (nothing of out is touched: its type is any)
+    cudaError_t e = start<P, float, PANELS, true>(maps, first, blocks * p.segments, st, launches);
     if (e != cudaSuccess) return e;
-    // (rows and heads: at most 2^24, and where segments are used less than twice the SMs)
+    // (rows and heads: at most 2^24, and where segments are used few)
     join_segments_kernel<<<dim3((p.dk * p.dv + 255) / 256, p.batch * p.heads), 256, 0, st>>>(
-        p, chunk_of<T>());
+        p, chunk_of(P));
     ++*launches;
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
   }
-  return start<T, O, PANELS, AHEAD, false>(maps, p, blocks * p.segments, st, launches);
+  return start<P, O, PANELS, false>(maps, p, blocks * p.segments, st, launches);
 }
 
-// `ws` holds segment_bytes.
+// One pass over arrays that `take` brought into shape; `ws` holds segment_bytes.
 template <typename T, typename O>
-cudaError_t run_pass(Pass p, void* ws, cudaStream_t st, int* launches) {
-  constexpr int C = chunk_of<T>();
+cudaError_t run_pass(Pass p, const Array& q, const Array& k, const Array& v, void* ws, cudaStream_t st,
+                     int* launches) {
+  constexpr int P = parts_of<T>(), C = chunk_of(P);
   const int64_t blocks = (int64_t)p.batch * p.heads * ((p.dv + kTile - 1) / kTile);
   if (!blocks) return cudaSuccess;
+  p.q_share = p.heads / q.heads, p.k_share = p.heads / k.heads, p.v_share = p.heads / v.heads;
   const int chunks = (p.len + C - 1) / C;
   p.segments = pass_segments<T>(p.batch, p.heads, p.dv, p.len);
   p.seg_chunks = std::max(1, (chunks + p.segments - 1) / p.segments);
   p.seg_states = static_cast<float*>(ws);
-  const auto width = [&](const Rows& r, int dim) {
-    return dim % 8 == 0 && pack_rows(r.p, 8, sizeof(T), r.batch, r.token)   ? 8
-           : dim % 4 == 0 && pack_rows(r.p, 4, sizeof(T), r.batch, r.token) ? 4
-                                                                            : 1;
-  };
-  p.copies_out = false;
-  p.width_q = width(p.q, p.dk), p.width_k = width(p.k, p.dk), p.width_v = width(p.v, p.dv);
   p.vec_out = packed_rows(p.out, 16, sizeof(O), p.out_batch, p.out_token) &&
               p.dv * sizeof(O) % 16 == 0;
   CUtensorMap maps[4] = {};
-  if constexpr (parts_of<T>() == 1) {
-    if (p.len > 0 && head_map(&maps[0], p.q, p.dk, p.heads, p.len, p.batch, C) &&
-        head_map(&maps[1], p.k, p.dk, p.heads, p.len, p.batch, C) &&
-        head_map(&maps[2], p.v, p.dv, p.heads, p.len, p.batch, C)) {
-      p.copies_out = sizeof(O) == 2 && head_map(&maps[3], {p.out, p.out_batch, p.out_token, 1}, p.dv,
-                                                p.heads, p.len, p.batch, 32, true);
-      return p.dk <= 64 ? run_ahead<T, O, 1, true>(maps, p, blocks, st, launches)
-                        : run_ahead<T, O, 2, true>(maps, p, blocks, st, launches);
-    }
+  p.copies_out = false;
+  if (p.len > 0) {
+    if (!head_map(&maps[0], q, 2, p.len, p.batch * P, C, 64, true) ||
+        !head_map(&maps[1], k, 2, p.len, p.batch * P, C, 64, true) ||
+        !head_map(&maps[2], v, 2, p.len, p.batch * P, C, 64, true))
+      return cudaErrorInvalidValue;
+    p.copies_out = Layout<P, 1, O>::kStaged > 0 &&
+                   head_map(&maps[3], {p.out, p.out_batch, p.out_token, p.heads, p.dv}, sizeof(O),
+                            p.len, p.batch, 32, 16, false);
   }
-  return p.dk <= 64 ? run_ahead<T, O, 1, false>(maps, p, blocks, st, launches)
-                    : run_ahead<T, O, 2, false>(maps, p, blocks, st, launches);
+  return p.dk <= 64 ? run_panels<P, O, 1>(maps, p, blocks, st, launches)
+                    : run_panels<P, O, 2>(maps, p, blocks, st, launches);
 }
 
 // One token of a row's head: S = l S + k v^T; out = scale * q S.  A block has a head; its 8 warps take
@@ -859,22 +840,110 @@ __global__ void __launch_bounds__(256, 2) attention_step_kernel(salt_linear_atte
   }
 }
 
+struct Arrays {
+  Array q, k, v, d;
+};
+template <class A>
+Arrays arrays_of(const A& a) {
+  return {{a.q, a.q_batch_stride, a.q_stride, a.heads, a.dim_k},
+          {a.k, a.k_batch_stride, a.k_stride, a.kv_heads, a.dim_k},
+          {a.v, a.v_batch_stride, a.v_stride, a.kv_heads, a.dim_v},
+          {}};
+}
+Arrays arrays_of_backward(const salt_linear_attention_backward_args& a) {
+  Arrays x = arrays_of(a);
+  x.d = {a.dout, a.dout_batch_stride, a.dout_stride, a.heads, a.dim_v};
+  return x;
+}
+template <typename T>
+size_t forward_bytes(const salt_linear_attention_args& a) {
+  const Arrays x = arrays_of(a);
+  return planes_bytes<T>(x.q, a.len, a.batch) + planes_bytes<T>(x.k, a.len, a.batch) +
+         planes_bytes<T>(x.v, a.len, a.batch) +
+         segment_bytes<T>(a.batch, a.heads, a.dim_k, a.dim_v, a.len);
+}
+// Backward: planes, segments' states of one pass after the other, and what the heads that share a key
+// head give to dk, then to dv.
+template <typename T>
+size_t backward_states(const salt_linear_attention_backward_args& a) {
+  return std::max(segment_bytes<T>(a.batch, a.heads, a.dim_v, a.dim_k, a.len),
+                  segment_bytes<T>(a.batch, a.heads, a.dim_k, a.dim_v, a.len));
+}
+template <typename T>
+size_t backward_bytes(const salt_linear_attention_backward_args& a) {
+  const Arrays x = arrays_of_backward(a);
+  size_t n = backward_states<T>(a);
+  for (const Array* y : {&x.q, &x.k, &x.v, &x.d}) n += planes_bytes<T>(*y, a.len, a.batch);
+  if (a.heads != a.kv_heads)
+    n += align256(sizeof(float) * a.batch * a.len * a.heads * std::max(a.dim_k, a.dim_v));
+  return n;
+}
+
+template <typename T>
+cudaError_t forward(const salt_linear_attention_args& a, uint8_t* ws, cudaStream_t st, int* launches) {
+  Arrays x = arrays_of(a);
+  for (Array* y : {&x.q, &x.k, &x.v}) {
+    const cudaError_t e = take<T>(*y, a.len, a.batch, a.n_real, ws, st, launches);
+    if (e != cudaSuccess) return e;
+  }
+  const Pass p{0, 0, 0, a.dim_k, a.dim_v, a.heads, a.len, a.batch, a.scale, false, a.log_decay,
+               a.n_real, a.initial_state, false, a.out, a.out_batch_stride, a.out_stride,
+               a.final_state};
+  return run_pass<T, T>(p, x.q, x.k, x.v, ws, st, launches);
+}
+
+template <typename T>
+cudaError_t backward(const salt_linear_attention_backward_args& a, uint8_t* ws, cudaStream_t st,
+                     int* launches) {
+  Arrays x = arrays_of_backward(a);
+  cudaError_t e = cudaSuccess;
+  for (Array* y : {&x.q, &x.k, &x.v, &x.d}) {
+    e = take<T>(*y, a.len, a.batch, a.n_real, ws, st, launches);
+    if (e != cudaSuccess) return e;
+  }
+  float* parts = reinterpret_cast<float*>(ws + backward_states<T>(a));
+  const Pass dq{0, 0, 0, a.dim_v, a.dim_k, a.heads, a.len, a.batch, a.scale, false, a.log_decay,
+                a.n_real, a.initial_state, true, a.dq, a.dq_batch_stride, a.dq_stride, nullptr};
+  Pass dk{0, 0, 0, a.dim_v, a.dim_k, a.heads, a.len, a.batch, a.scale, true, a.log_decay, a.n_real,
+          a.dfinal, true, a.dk, a.dk_batch_stride, a.dk_stride, nullptr};
+  Pass dv{0, 0, 0, a.dim_k, a.dim_v, a.heads, a.len, a.batch, a.scale, true, a.log_decay, a.n_real,
+          a.dfinal, false, a.dv, a.dv_batch_stride, a.dv_stride, a.dinitial};
+  e = run_pass<T, T>(dq, x.d, x.v, x.k, ws, st, launches);
+  const int share = a.heads / a.kv_heads;
+  for (Pass* p : {&dk, &dv}) {
+    if (e != cudaSuccess) return e;
+    T* to = static_cast<T*>(p->out);
+    const int64_t to_batch = p->out_batch, to_token = p->out_token;
+    if (share > 1) {
+      p->out = parts;
+      p->out_token = (int64_t)a.heads * p->dv;
+      p->out_batch = p->out_token * a.len;
+    }
+    const Array &q = p == &dk ? x.v : x.k, &k = p == &dk ? x.d : x.q, &v = p == &dk ? x.q : x.d;
+    e = share > 1 ? run_pass<T, float>(*p, q, k, v, ws, st, launches)
+                  : run_pass<T, T>(*p, q, k, v, ws, st, launches);
+    const int64_t n = (int64_t)a.batch * a.len * a.kv_heads * p->dv;
+    if (e != cudaSuccess || share == 1 || !n) continue;
+    sum_heads_kernel<T><<<(unsigned)std::min<int64_t>((n + 255) / 256, 148 * 8), 256, 0, st>>>(
+        parts, to, (int64_t)a.batch * a.len, a.len, a.kv_heads, share, p->dv, to_batch, to_token);
+    ++*launches;
+    e = cudaGetLastError();
+  }
+  return e;
+}
+
 }  // namespace
 
 size_t linear_attention_bytes(const salt_linear_attention_args& a) {
-  return segment_bytes(a.type, a.batch, a.heads, a.dim_k, a.dim_v, a.len);
+  size_t n = 0;
+  SALT_WITH_TYPE(a.type, T, n = forward_bytes<T>(a));
+  return n;
 }
 
 cudaError_t linear_attention_launch(const salt_linear_attention_args& a, void* ws, cudaStream_t st,
                                     int* launches) {
-  const int share = a.heads / a.kv_heads;
-  Pass p{{a.q, a.q_batch_stride, a.q_stride, 1},
-         {a.k, a.k_batch_stride, a.k_stride, share},
-         {a.v, a.v_batch_stride, a.v_stride, share},
-         a.dim_k, a.dim_v, a.heads, a.len, a.batch, a.scale, false, a.log_decay, a.n_real,
-         a.initial_state, false, a.out, a.out_batch_stride, a.out_stride, a.final_state};
   cudaError_t e = cudaSuccess;
-  SALT_WITH_TYPE(a.type, T, e = (run_pass<T, T>(p, ws, st, launches)));
+  SALT_WITH_TYPE(a.type, T, e = forward<T>(a, static_cast<uint8_t*>(ws), st, launches));
   return e;
 }
 
@@ -891,52 +960,15 @@ cudaError_t linear_attention_step_launch(const salt_linear_attention_step_args& 
 }
 
 size_t linear_attention_backward_bytes(const salt_linear_attention_backward_args& a) {
-  // segments' states of one pass after the other, and parts of dk, then of dv
-  const size_t states = std::max(segment_bytes(a.type, a.batch, a.heads, a.dim_v, a.dim_k, a.len),
-                                 segment_bytes(a.type, a.batch, a.heads, a.dim_k, a.dim_v, a.len));
-  if (a.heads == a.kv_heads) return states;
-  return states + align256(sizeof(float) * a.batch * a.len * a.heads * std::max(a.dim_k, a.dim_v));
+  size_t n = 0;
+  SALT_WITH_TYPE(a.type, T, n = backward_bytes<T>(a));
+  return n;
 }
 
 cudaError_t linear_attention_backward_launch(const salt_linear_attention_backward_args& a, void* ws,
                                              cudaStream_t st, int* launches) {
-  const int share = a.heads / a.kv_heads;
-  const Rows q{a.q, a.q_batch_stride, a.q_stride, 1}, k{a.k, a.k_batch_stride, a.k_stride, share},
-      v{a.v, a.v_batch_stride, a.v_stride, share}, d{a.dout, a.dout_batch_stride, a.dout_stride, 1};
-  const Pass dq{d, v, k, a.dim_v, a.dim_k, a.heads, a.len, a.batch, a.scale, false, a.log_decay,
-                a.n_real, a.initial_state, true, a.dq, a.dq_batch_stride, a.dq_stride, nullptr};
-  Pass dk{v, d, q, a.dim_v, a.dim_k, a.heads, a.len, a.batch, a.scale, true, a.log_decay, a.n_real,
-          a.dfinal, true, a.dk, a.dk_batch_stride, a.dk_stride, nullptr};
-  Pass dv{k, q, d, a.dim_k, a.dim_v, a.heads, a.len, a.batch, a.scale, true, a.log_decay, a.n_real,
-          a.dfinal, false, a.dv, a.dv_batch_stride, a.dv_stride, a.dinitial};
-  float* parts = reinterpret_cast<float*>(
-      static_cast<uint8_t*>(ws) +
-      std::max(segment_bytes(a.type, a.batch, a.heads, a.dim_v, a.dim_k, a.len),
-               segment_bytes(a.type, a.batch, a.heads, a.dim_k, a.dim_v, a.len)));
   cudaError_t e = cudaSuccess;
-  SALT_WITH_TYPE(a.type, T, {
-    e = run_pass<T, T>(dq, ws, st, launches);
-    for (Pass* p : {&dk, &dv}) {
-      if (e != cudaSuccess) return e;
-      if (share == 1) {
-        e = run_pass<T, T>(*p, ws, st, launches);
-        continue;
-      }
-      T* to = static_cast<T*>(p->out);
-      const int64_t to_batch = p->out_batch, to_token = p->out_token;
-      p->out = parts;
-      p->out_token = (int64_t)a.heads * p->dv;
-      p->out_batch = p->out_token * a.len;
-      e = run_pass<T, float>(*p, ws, st, launches);
-      const int64_t n = (int64_t)a.batch * a.len * a.kv_heads * p->dv;
-      if (e != cudaSuccess || !n) continue;
-      sum_heads_kernel<T><<<(unsigned)std::min<int64_t>((n + 255) / 256, 148 * 8), 256, 0, st>>>(
-          parts, to, (int64_t)a.batch * a.len, a.len, a.kv_heads, share,
-          p->dv, to_batch, to_token);
-      ++*launches;
-      e = cudaGetLastError();
-    }
-  });
+  SALT_WITH_TYPE(a.type, T, e = backward<T>(a, static_cast<uint8_t*>(ws), st, launches));
   return e;
 }
 
