@@ -430,20 +430,29 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         }
       }
       if constexpr (L::kStaged > 0) {
+        // 16 columns a row, through shared memory: as stores from here every 16 bytes would be a line
+        // of their own
+        O* to = reinterpret_cast<O*>(sm + L::out + warp * L::kStaged);
+        if (a.copies_out && lane == 0) tc::stores_read();
+        __syncwarp();
+        store_pack<O, 8>(to + lane * 16, f, 8, true);
+        store_pack<O, 8>(to + lane * 16 + 8, f + 8, 8, true);
         if (a.copies_out) {
-          // 16 columns a row, through shared memory: as stores from here every 16 bytes would be a line
-          // of their own.  Rows past the end are zero anyway; those past `len` are left out.
-          uint8_t* to = sm + L::out + warp * L::kStaged;
-          if (lane == 0) tc::stores_read();
-          __syncwarp();
-          store_pack<O, 8>(reinterpret_cast<O*>(to) + lane * 16, f, 8, true);
-          store_pack<O, 8>(reinterpret_cast<O*>(to) + lane * 16 + 8, f + 8, 8, true);
+          // rows past the end are zero anyway; those past `len` are left out
           tc::fence_shared();
           __syncwarp();
           if (lane == 0 && quarter * 32 < min(C, a.len - c * C) && sc0 < a.dv)
             tc::store_box4(&map_out, to, sc0, h, c * C + quarter * 32, b);
           return;
         }
+        __syncwarp();
+        const int col = lane & 15;
+        O* out = static_cast<O*>(a.out) + b * a.out_batch + (int64_t)h * a.dv + sc0 + col;
+        if (sc0 + col < a.dv) {
+          for (int r = lane >> 4; r < min(32, count - quarter * 32); r += 2)
+            out[((int64_t)c * C + quarter * 32 + r) * a.out_token] = to[r * 16 + col];
+        }
+        return;
       }
       if (!live) return;
       O* out = static_cast<O*>(a.out) + b * a.out_batch + ((int64_t)c * C + row) * a.out_token +
