@@ -64,18 +64,24 @@ struct Layout {
 // Two values in parts of bfloat16: the upper 8 bits of what is left, time and again; the last of two
 // parts is rounded to the nearest (2^-16 of the value in all), three hold all 24 bits.
 template <int N>
-__device__ __forceinline__ void split2(uint32_t (&to)[N], float x, float y) {
+__device__ __forceinline__ void split2(uint32_t (&to)[N], f32x2 v) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
+    const float2 x = halves(v);
     if (i == N - 1 && N < 3) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+      const __nv_bfloat162 h = __floats2bfloat162_rn(x.x, x.y);
       to[i] = *reinterpret_cast<const uint32_t*>(&h);
     } else {
-      to[i] = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
-      x -= __uint_as_float(__float_as_uint(x) & 0xffff0000u);
-      y -= __uint_as_float(__float_as_uint(y) & 0xffff0000u);
+      to[i] = __byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x7632);
+      if (i < N - 1)  // the sign goes over with the upper bits
+        v = add2(v, pair(__uint_as_float((__float_as_uint(x.x) & 0xffff0000u) ^ 0x80000000u),
+                         __uint_as_float((__float_as_uint(x.y) & 0xffff0000u) ^ 0x80000000u)));
     }
   }
+}
+template <int N>
+__device__ __forceinline__ void split2(uint32_t (&to)[N], float x, float y) {
+  split2<N>(to, pair(x, y));
 }
 
 // An array (batch, len, heads, dim) of T in planes of bfloat16 parts (part, batch, len, heads, dim
@@ -304,7 +310,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     __syncwarp();
   } else {
     // this thread's part of the state: row `row`, 16 columns
-    float s[16];
+    f32x2 s[8];
     const int sc0 = col0 + part * 16;
     const bool joined = a.segments > 1 && !STATE;
     const float* from =
@@ -312,17 +318,21 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                : a.initial ? a.initial + state_at : nullptr;
     const bool across = a.initial_t && !joined;
 #pragma unroll
-    for (int j = 0; j < 16; ++j)
-      s[j] = from && row < a.dk && sc0 + j < a.dv
-                 ? from[across ? (int64_t)(sc0 + j) * a.dk + row : (int64_t)row * a.dv + sc0 + j]
-                 : 0.f;
+    for (int j = 0; j < 16; j += 2) {
+      const auto load = [&](int c) {
+        return from && row < a.dk && c < a.dv
+                   ? from[across ? (int64_t)c * a.dk + row : (int64_t)row * a.dv + c]
+                   : 0.f;
+      };
+      s[j / 2] = pair(load(sc0 + j), load(sc0 + j + 1));
+    }
     const auto store_state = [&] {  // as an operand
       if (row >= DK) return;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         uint32_t x[4][SP];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) split2<SP>(x[k], s[8 * u + 2 * k], s[8 * u + 2 * k + 1]);
+        for (int k = 0; k < 4; ++k) split2<SP>(x[k], s[4 * u + k]);
 #pragma unroll
         for (int j = 0; j < SP; ++j)
           *reinterpret_cast<uint4*>(sm + L::state + j * L::kState + row * 128 +
@@ -352,7 +362,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         uint8_t* place = v + r * 128 + ((u ^ (r & 7)) << 4);
         const float w = r >= count ? 0.f : power[a.reverse ? r + 1 : count - 1 - r];
         uint32_t in[P][4], out[4][kWeighted];
-        bool fine = true;
+        uint32_t carry = 0;  // from an exponent of all ones
 #pragma unroll
         for (int j = 0; j < P; ++j) {
           const uint4 y = *reinterpret_cast<const uint4*>(place + j * kPanel);
@@ -368,9 +378,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         // A value that is not finite would reach the tokens on the triangle's other side, as 0 * it:
         // it becomes zero here, and its column NaN from its token on.
 #pragma unroll
-        for (int m = 0; m < 4; ++m)
-          fine &= (in[0][m] & 0x7f80u) != 0x7f80u && (in[0][m] & 0x7f800000u) != 0x7f800000u;
-        if (!fine) {
+        for (int m = 0; m < 4; ++m) carry |= (in[0][m] & 0x7f807f80u) + 0x00800080u;
+        if (carry & 0x80008000u) {
           any_bad[i % 3] = 1;
 #pragma unroll
           for (int m = 0; m < 8; ++m) {
@@ -387,13 +396,14 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         }
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-          float lo = __uint_as_float(in[0][m] << 16), hi = __uint_as_float(in[0][m] & 0xffff0000u);
+          f32x2 y = 0;
 #pragma unroll
-          for (int j = 1; j < P; ++j) {
-            lo += __uint_as_float(in[j][m] << 16);
-            hi += __uint_as_float(in[j][m] & 0xffff0000u);
+          for (int j = 0; j < P; ++j) {
+            const f32x2 part = pair(__uint_as_float(in[j][m] << 16),
+                                    __uint_as_float(in[j][m] & 0xffff0000u));
+            y = j == 0 ? part : add2(y, part);
           }
-          split2<kWeighted>(out[m], w * lo, w * hi);
+          split2<kWeighted>(out[m], mul2(y, both(w)));
         }
         uint8_t* to = sm + L::weighted + (place - v);
 #pragma unroll
@@ -419,8 +429,12 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       const float by = !live ? 0.f : a.reverse ? power[count - 1 - row] : a.scale * power[row + 1];
       float f[16];
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
-        f[j] = live ? fmaf(__uint_as_float(x[j]), by, a.scale * __uint_as_float(y[j])) : 0.f;
+      for (int j = 0; j < 16; j += 2) {
+        const float2 o =
+            halves(fma2(pair(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), both(by),
+                        mul2(pair(__uint_as_float(y[j]), __uint_as_float(y[j + 1])), both(a.scale))));
+        f[j] = live ? o.x : 0.f, f[j + 1] = live ? o.y : 0.f;
+      }
       if (any_bad[i % 3] || !tries) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
@@ -512,10 +526,11 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 #pragma unroll
               for (int j = 0; j < 16; j += 4) {
                 const float4 w = *reinterpret_cast<const float4*>(column + y + j);
-                split2<SP>(x[j / 2], __uint_as_float(r[j]) * (f * w.x),
-                           __uint_as_float(r[j + 1]) * (f * w.y));
-                split2<SP>(x[j / 2 + 1], __uint_as_float(r[j + 2]) * (f * w.z),
-                           __uint_as_float(r[j + 3]) * (f * w.w));
+                split2<SP>(x[j / 2], mul2(pair(__uint_as_float(r[j]), __uint_as_float(r[j + 1])),
+                                          mul2(pair(w.x, w.y), both(f))));
+                split2<SP>(x[j / 2 + 1],
+                           mul2(pair(__uint_as_float(r[j + 2]), __uint_as_float(r[j + 3])),
+                                mul2(pair(w.z, w.w), both(f))));
               }
             }
 #pragma unroll
@@ -541,11 +556,16 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       tc::fence_before();
       const float l = power[count], by = a.reverse ? a.scale : 1.f;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) s[j] = fmaf(s[j], l, by * __uint_as_float(x[j]));
+      for (int j = 0; j < 8; ++j)
+        s[j] = fma2(s[j], both(l),
+                    mul2(pair(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), both(by)));
       if (any_bad[i % 3]) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (bad[i % 3][part * 16 + j] >= 0) s[j] = __int_as_float(0x7fffffff);
+        for (int j = 0; j < 16; ++j) {
+          if (bad[i % 3][part * 16 + j] < 0) continue;
+          const float2 y = halves(s[j / 2]);
+          s[j / 2] = j % 2 ? pair(y.x, __int_as_float(0x7fffffff)) : pair(__int_as_float(0x7fffffff), y.y);
+        }
       }
       if (i + 1 < steps) {
         if (!STATE) {
@@ -568,8 +588,10 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     if (to && row < a.dk) {
 #pragma unroll
       for (int j = 0; j < 16; ++j)
-        if (sc0 + j < a.dv)
-          to[(int64_t)row * a.dv + sc0 + j] = tries ? s[j] : __int_as_float(0x7fffffff);
+        if (sc0 + j < a.dv) {
+          const float2 y = halves(s[j / 2]);
+          to[(int64_t)row * a.dv + sc0 + j] = !tries ? __int_as_float(0x7fffffff) : j % 2 ? y.y : y.x;
+        }
     }
     if (!STATE) {
       // tokens behind the row's end
