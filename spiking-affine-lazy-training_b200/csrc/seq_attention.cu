@@ -121,7 +121,8 @@ __global__ void __launch_bounds__(256) planes_kernel(const T* from, int64_t batc
 // part, float16 in two, float32 in three, the last rounded); weighted values have three parts, so
 // that states are good to 2^-24; states and the triangle's values, as operands for out, have three
 // parts for float32 and two (2^-16) for outputs of 16 bits.  Sums and states are float32; the state
-// is carried in registers.
+// is carried in registers.  The tensor cores cut their sums off after every instruction, so the parts'
+// products go from the smallest to the largest: in the other order float32's outputs were off by 2.5e-6.
 template <int P, typename O, int PANELS, bool STATE>
 __global__ void __launch_bounds__(kThreads, 1)
 attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -215,15 +216,18 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         const uint64_t k = tc::operand(sm + L::k + i % B * L::kKeys, 1024);
         bool add = false;
 #pragma unroll
-        for (int x = 0; x < P; ++x)
+        for (int o = 2; o >= 0; --o)
 #pragma unroll
-          for (int y = 0; y < P && x + y < 3; ++y)
+          for (int x = 0; x < P; ++x) {
+            const int y = o - x;
+            if (y < 0 || y >= P) continue;
             for (int d = 0; d < depth; ++d) {
               const uint32_t off = (d >> 2) * kPanel + (d & 3) * 32;
               tc::product_16(tmem + kScores, tc::further(q, x * PANELS * kPanel + off),
                              tc::further(k, y * PANELS * kPanel + off), tc::shape(128, C, 1), add);
               add = true;
             }
+          }
         tc::products_done(&done_scores);
       };
       for (int i = 0; i < B; ++i) {
@@ -243,9 +247,11 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         if (!STATE) {
           bool add = false;
 #pragma unroll
-          for (int x = 0; x < P; ++x)
+          for (int o = 2; o >= 0; --o)
 #pragma unroll
-            for (int y = 0; y < SP && x + y < 3; ++y)
+            for (int x = 0; x < P; ++x) {
+              const int y = o - x;
+              if (y < 0 || y >= SP) continue;
               for (int d = 0; d < depth; ++d) {
                 const uint32_t off = (d >> 2) * kPanel + (d & 3) * 32;
                 tc::product_16(tmem + kFromState + (i & 1) * kTile,
@@ -254,15 +260,18 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                                tc::shape(128, kTile, 1, false, true), add);
                 add = true;
               }
+            }
           tc::products_done(&done_q);
         }
         {
           const uint64_t k = tc::operand(sm + L::k + i % B * L::kKeys, 1024, kPanel);
           bool add = false;
 #pragma unroll
-          for (int x = 0; x < P; ++x)
+          for (int o = 2; o >= 0; --o)
 #pragma unroll
-            for (int y = 0; y < kWeighted && x + y < 3; ++y)
+            for (int x = 0; x < P; ++x) {
+              const int y = o - x;
+              if (y < 0 || y >= kWeighted) continue;
 #pragma unroll
               for (int d = 0; d < C / 16; ++d) {
                 tc::product_16(tmem + kAdded, tc::further(k, x * PANELS * kPanel + d * 2048),
@@ -270,6 +279,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                                tc::shape(128, kTile, 1, true, true), add);
                 add = true;
               }
+            }
           tc::products_done(&done_state);
         }
         if (!STATE) {
@@ -280,9 +290,11 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           const uint64_t v = tc::operand(sm + L::v + i % B * L::kValues, 1024);
           bool add = false;
 #pragma unroll
-          for (int x = 0; x < SP; ++x)
+          for (int o = 2; o >= 0; --o)
 #pragma unroll
-            for (int y = 0; y < P && x + y < 3; ++y)
+            for (int x = 0; x < SP; ++x) {
+              const int y = o - x;
+              if (y < 0 || y >= P) continue;
 #pragma unroll
               for (int d = 0; d < C / 16; ++d) {
                 tc::product_16_from_tmem(tmem + kOut, tmem + kTriangle + x * (C / 2) + d * 8,
@@ -290,6 +302,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                                          tc::shape(128, kTile, 1, false, true), add);
                 add = true;
               }
+            }
           tc::products_done(&done_out);
         }
         if (i + 1 == steps) break;
