@@ -44,18 +44,19 @@ constexpr int kWeighted = 3;   // parts of a weighted v
 template <typename T>
 constexpr int parts_of() { return sizeof(T) == 4 ? 3 : std::is_same<T, __half>::value ? 2 : 1; }
 // Tokens of a chunk, and parts of the states and of the weights within a chunk.
-constexpr int chunk_of(int parts) { return parts == 1 ? 128 : 64; }
+// (64 where 128 do not fit into shared memory)
+constexpr int chunk_of(int parts, int panels) { return parts == 1 || (parts == 2 && panels == 1) ? 128 : 64; }
 constexpr int state_parts(int parts) { return parts == 3 ? 3 : 2; }
 
 // Shared memory, all operands in rows of 128 bytes (tc::operand): q and k in panels of 64 columns,
 // part after part; k and v twice, for copies a chunk further ahead, where there is room.
 template <int P, int PANELS, typename O>
 struct Layout {
-  static constexpr int C = chunk_of(P), B = P == 3 ? 1 : 2;
+  static constexpr int C = chunk_of(P, PANELS), B = P == 3 || (P == 2 && C == 128) ? 1 : 2;
   static constexpr int kPanel = C * 128, kKeys = P * PANELS * kPanel, kValues = P * kPanel;
   static constexpr int kState = PANELS * 64 * 128;  // a part of the state
   // rows of out, 16 columns of 32 rows a warp; without room for them out is stored from registers
-  static constexpr int kStaged = P == 1 && sizeof(O) == 4 ? 0 : 32 * 16 * sizeof(O);
+  static constexpr int kStaged = C == 128 && sizeof(O) == 4 ? 0 : 32 * 16 * sizeof(O);
   static constexpr int q = 0, k = q + kKeys, v = k + B * kKeys, weighted = v + B * kValues,
                        state = weighted + kWeighted * kPanel, out = state + state_parts(P) * kState,
                        bytes = out + kWorkers / 32 * kStaged + 1024;
@@ -84,30 +85,40 @@ __device__ __forceinline__ void split2(uint32_t (&to)[N], float x, float y) {
   split2<N>(to, pair(x, y));
 }
 
-// An array (batch, len, heads, dim) of T in planes of bfloat16 parts (part, batch, len, heads, dim
-// rounded up to 8), zero past the rows' ends: what tensor copies can take of every type, alignment and
-// size.  Bound by memory.
+// Arrays (batch, len, heads, dim) of T in planes of bfloat16 parts (part, batch, len, heads, dim rounded
+// up to 8), zero past the rows' ends: what tensor copies can take of every type, alignment and size.
+// blockIdx.y is the array.  Bound by memory.
+struct ToPlanes {
+  const void* from;
+  int64_t batch_stride, stride;
+  uint4* to;
+  int heads, dim;
+  bool vec;
+};
+struct AllToPlanes {
+  ToPlanes a[4];
+};
 template <typename T>
-__global__ void __launch_bounds__(256) planes_kernel(const T* from, int64_t batch_stride, int64_t stride,
-                                                     int batch, int len, int heads, int dim,
-                                                     const int32_t* n_real, uint4* to, bool vec) {
+__global__ void __launch_bounds__(256) planes_kernel(const AllToPlanes all, int batch, int len,
+                                                     const int32_t* n_real) {
   constexpr int P = parts_of<T>();
-  const int units = (dim + 7) / 8, each = heads * units;
+  const ToPlanes x = all.a[blockIdx.y];
+  const int units = (x.dim + 7) / 8, each = x.heads * units;
   const int64_t n = (int64_t)batch * len * each;
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
     const int64_t token = n >> 32 ? i / each : (unsigned)i / (unsigned)each;
     const int in = (int)(i - token * each), h = in / units, at = (in - h * units) * 8;
     const int b = (int)(n >> 32 ? token / len : (unsigned)token / (unsigned)len);
     const int t = (int)(token - (int64_t)b * len);
-    const Pack<T, 8> p =
-        load_pack<T, 8>(from + b * batch_stride + t * stride + (int64_t)h * dim + at,
-                        t < row_tokens(n_real, b, len) ? dim - at : 0, vec);
+    const Pack<T, 8> p = load_pack<T, 8>(
+        static_cast<const T*>(x.from) + b * x.batch_stride + t * x.stride + (int64_t)h * x.dim + at,
+        t < row_tokens(n_real, b, len) ? x.dim - at : 0, x.vec);
     uint32_t parts[4][P];
 #pragma unroll
     for (int k = 0; k < 4; ++k) split2<P>(parts[k], to_f32(p.v[2 * k]), to_f32(p.v[2 * k + 1]));
 #pragma unroll
     for (int j = 0; j < P; ++j)
-      to[j * n + i] = make_uint4(parts[0][j], parts[1][j], parts[2][j], parts[3][j]);
+      x.to[j * n + i] = make_uint4(parts[0][j], parts[1][j], parts[2][j], parts[3][j]);
   }
 }
 
@@ -361,7 +372,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       uint8_t* k = sm + L::k + i % B * L::kKeys;
       uint8_t* v = sm + L::v + i % B * L::kValues;
       tc::barrier_wait_warp(&loaded_v[i % B], i / B & 1, tries);
-      if (P == 1 && count < C) {  // (planes of several parts hold zeros there)
+      if (P == 1 && count < C) {  // (planes hold zeros there)
         tc::barrier_wait_warp(&loaded_k[i % B], i / B & 1, tries);
         for (int x = threadIdx.x; x < (C - count) * PANELS * 8; x += kWorkers) {
           const int r = count + x / (PANELS * 8), u = x % (PANELS * 8);
@@ -708,23 +719,29 @@ size_t planes_bytes(const Array& x, int len, int batch) {
   if (!len || !batch || as_it_lies<T>(x, len, batch)) return 0;
   return align256((size_t)parts_of<T>() * batch * len * x.heads * ((x.dim + 7) / 8) * 16);
 }
-template <typename T>
-cudaError_t take(Array& x, int len, int batch, const int32_t* n_real, uint8_t*& ws, cudaStream_t st,
-                 int* launches) {
-  if (!len || !batch || as_it_lies<T>(x, len, batch)) return cudaSuccess;
-  const size_t bytes = planes_bytes<T>(x, len, batch);
-  const int units = (x.dim + 7) / 8;
-  const int64_t n = (int64_t)batch * len * x.heads * units;
-  planes_kernel<T><<<(unsigned)std::min<int64_t>((n + 255) / 256, 148 * 16), 256, 0, st>>>(
-      static_cast<const T*>(x.p), x.batch_stride, x.stride, batch, len, x.heads, x.dim, n_real,
-      reinterpret_cast<uint4*>(ws),
-      x.dim % 8 == 0 && pack_rows(x.p, 8, sizeof(T), x.batch_stride, x.stride));
+template <typename T, int N>
+cudaError_t take(Array* const (&all)[N], int len, int batch, const int32_t* n_real, uint8_t*& ws,
+                 cudaStream_t st, int* launches) {
+  AllToPlanes to = {};
+  int count = 0;
+  int64_t most = 0;
+  for (Array* x : all) {
+    if (!len || !batch || as_it_lies<T>(*x, len, batch)) continue;
+    const size_t bytes = planes_bytes<T>(*x, len, batch);
+    const int units = (x->dim + 7) / 8;
+    to.a[count++] = {x->p, x->batch_stride, x->stride, reinterpret_cast<uint4*>(ws), x->heads, x->dim,
+                     x->dim % 8 == 0 && pack_rows(x->p, 8, sizeof(T), x->batch_stride, x->stride)};
+    most = std::max(most, (int64_t)batch * len * x->heads * units);
+    x->p = ws;
+    x->dim = units * 8;
+    x->stride = (int64_t)x->heads * x->dim;
+    x->batch_stride = x->stride * len;
+    ws += bytes;
+  }
+  if (!count) return cudaSuccess;
+  planes_kernel<T><<<dim3((unsigned)std::min<int64_t>((most + 255) / 256, 148 * 8), count), 256, 0,
+                     st>>>(to, batch, len, n_real);
   ++*launches;
-  x.p = ws;
-  x.dim = units * 8;
-  x.stride = (int64_t)x.heads * x.dim;
-  x.batch_stride = x.stride * len;
-  ws += bytes;
   return cudaGetLastError();
 }
 
@@ -757,14 +774,14 @@ int segments_of(int64_t blocks, int chunks) {
   return best;
 }
 template <typename T>
-int pass_segments(int batch, int heads, int dv, int len) {
-  constexpr int C = chunk_of(parts_of<T>());
+int pass_segments(int batch, int heads, int dk, int dv, int len) {
+  const int C = chunk_of(parts_of<T>(), dk <= 64 ? 1 : 2);
   const int64_t blocks = (int64_t)batch * heads * ((dv + kTile - 1) / kTile);
   return blocks ? segments_of(blocks, (len + C - 1) / C) : 1;
 }
 template <typename T>
 size_t segment_bytes(int batch, int heads, int dk, int dv, int len) {
-  const int s = pass_segments<T>(batch, heads, dv, len);
+  const int s = pass_segments<T>(batch, heads, dk, dv, len);
   return s == 1 ? 0 : align256(sizeof(float) * batch * heads * s * dk * dv);
 }
 
@@ -779,7 +796,7 @@ cudaError_t run_panels(const CUtensorMap (&maps)[4], const Pass& p, int64_t bloc
     if (e != cudaSuccess) return e;
     // (rows and heads: at most 2^24, and where segments are used few)
     join_segments_kernel<<<dim3((p.dk * p.dv + 255) / 256, p.batch * p.heads), 256, 0, st>>>(
-        p, chunk_of(P));
+        p, chunk_of(P, PANELS));
     ++*launches;
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
@@ -791,12 +808,13 @@ cudaError_t run_panels(const CUtensorMap (&maps)[4], const Pass& p, int64_t bloc
 template <typename T, typename O>
 cudaError_t run_pass(Pass p, const Array& q, const Array& k, const Array& v, void* ws, cudaStream_t st,
                      int* launches) {
-  constexpr int P = parts_of<T>(), C = chunk_of(P);
+  constexpr int P = parts_of<T>();
+  const int C = chunk_of(P, p.dk <= 64 ? 1 : 2);
   const int64_t blocks = (int64_t)p.batch * p.heads * ((p.dv + kTile - 1) / kTile);
   if (!blocks) return cudaSuccess;
   p.q_share = p.heads / q.heads, p.k_share = p.heads / k.heads, p.v_share = p.heads / v.heads;
   const int chunks = (p.len + C - 1) / C;
-  p.segments = pass_segments<T>(p.batch, p.heads, p.dv, p.len);
+  p.segments = pass_segments<T>(p.batch, p.heads, p.dk, p.dv, p.len);
   p.seg_chunks = std::max(1, (chunks + p.segments - 1) / p.segments);
   p.seg_states = static_cast<float*>(ws);
   p.vec_out = packed_rows(p.out, 16, sizeof(O), p.out_batch, p.out_token) &&
@@ -808,7 +826,7 @@ cudaError_t run_pass(Pass p, const Array& q, const Array& k, const Array& v, voi
         !head_map(&maps[1], k, 2, p.len, p.batch * P, C, 64, true) ||
         !head_map(&maps[2], v, 2, p.len, p.batch * P, C, 64, true))
       return cudaErrorInvalidValue;
-    p.copies_out = Layout<P, 1, O>::kStaged > 0 &&
+    p.copies_out = (p.dk <= 64 ? Layout<P, 1, O>::kStaged : Layout<P, 2, O>::kStaged) > 0 &&
                    head_map(&maps[3], {p.out, p.out_batch, p.out_token, p.heads, p.dv}, sizeof(O),
                             p.len, p.batch, 32, 16, false);
   }
@@ -926,10 +944,8 @@ size_t backward_bytes(const salt_linear_attention_backward_args& a) {
 template <typename T>
 cudaError_t forward(const salt_linear_attention_args& a, uint8_t* ws, cudaStream_t st, int* launches) {
   Arrays x = arrays_of(a);
-  for (Array* y : {&x.q, &x.k, &x.v}) {
-    const cudaError_t e = take<T>(*y, a.len, a.batch, a.n_real, ws, st, launches);
-    if (e != cudaSuccess) return e;
-  }
+  const cudaError_t e = take<T, 3>({&x.q, &x.k, &x.v}, a.len, a.batch, a.n_real, ws, st, launches);
+  if (e != cudaSuccess) return e;
   const Pass p{0, 0, 0, a.dim_k, a.dim_v, a.heads, a.len, a.batch, a.scale, false, a.log_decay,
                a.n_real, a.initial_state, false, a.out, a.out_batch_stride, a.out_stride,
                a.final_state};
@@ -940,11 +956,9 @@ template <typename T>
 cudaError_t backward(const salt_linear_attention_backward_args& a, uint8_t* ws, cudaStream_t st,
                      int* launches) {
   Arrays x = arrays_of_backward(a);
-  cudaError_t e = cudaSuccess;
-  for (Array* y : {&x.q, &x.k, &x.v, &x.d}) {
-    e = take<T>(*y, a.len, a.batch, a.n_real, ws, st, launches);
-    if (e != cudaSuccess) return e;
-  }
+  cudaError_t e =
+      take<T, 4>({&x.q, &x.k, &x.v, &x.d}, a.len, a.batch, a.n_real, ws, st, launches);
+  if (e != cudaSuccess) return e;
   float* parts = reinterpret_cast<float*>(ws + backward_states<T>(a));
   const Pass dq{0, 0, 0, a.dim_v, a.dim_k, a.heads, a.len, a.batch, a.scale, false, a.log_decay,
                 a.n_real, a.initial_state, true, a.dq, a.dq_batch_stride, a.dq_stride, nullptr};

@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import math
 import threading
 import weakref
 from typing import NamedTuple
@@ -253,8 +254,7 @@ class DeviceArray:
     @staticmethod
     def empty(shape, dtype) -> "DeviceArray":
         shape = (int(shape),) if np.isscalar(shape) else tuple(int(v) for v in shape)
-        nbytes = int(np.prod(shape, dtype=np.int64)) * np.dtype(dtype).itemsize
-        a = _Allocation(nbytes)
+        a = _Allocation(math.prod(shape) * np.dtype(dtype).itemsize)
         return DeviceArray(a.ptr, shape, dtype, a)
 
     @staticmethod
