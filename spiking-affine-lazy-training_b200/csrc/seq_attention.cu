@@ -27,7 +27,7 @@ struct Pass {
   // set by the launch
   int segments, seg_chunks;  // segments of a row that run side by side, chunks of each
   float* seg_states;         // (batch, heads, segments, dk, dv): what each adds to the state
-  bool vec_out, copies_out;
+  bool copies_out;
 };
 
 __device__ __forceinline__ float decay_of(const float* g, int h) {
@@ -55,8 +55,8 @@ struct Layout {
   static constexpr int C = chunk_of(P, PANELS), B = P == 3 || (P == 2 && C == 128) ? 1 : 2;
   static constexpr int kPanel = C * 128, kKeys = P * PANELS * kPanel, kValues = P * kPanel;
   static constexpr int kState = PANELS * 64 * 128;  // a part of the state
-  // rows of out, 16 columns of 32 rows a warp; without room for them out is stored from registers
-  static constexpr int kStaged = C == 128 && sizeof(O) == 4 ? 0 : 32 * 16 * sizeof(O);
+  // a warp's 32 rows of out, 32 bytes each at a time
+  static constexpr int kStaged = 1024, kOutColumns = 32 / sizeof(O);
   static constexpr int q = 0, k = q + kKeys, v = k + B * kKeys, weighted = v + B * kValues,
                        state = weighted + kWeighted * kPanel, out = state + state_parts(P) * kState,
                        bytes = out + kWorkers / 32 * kStaged + 1024;
@@ -467,37 +467,32 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             f[j] = __int_as_float(0x7fffffff);
         }
       }
-      if constexpr (L::kStaged > 0) {
-        // 16 columns a row, through shared memory: as stores from here every 16 bytes would be a line
-        // of their own
-        O* to = reinterpret_cast<O*>(sm + L::out + warp * L::kStaged);
+      // 32 bytes a row, through shared memory: as stores from here every 16 bytes would be a line of
+      // their own
+      constexpr int W = L::kOutColumns;
+      O* to = reinterpret_cast<O*>(sm + L::out + warp * L::kStaged);
+#pragma unroll
+      for (int y = 0; y < 16; y += W) {
         if (a.copies_out && lane == 0) tc::stores_read();
         __syncwarp();
-        store_pack<O, 8>(to + lane * 16, f, 8, true);
-        store_pack<O, 8>(to + lane * 16 + 8, f + 8, 8, true);
+#pragma unroll
+        for (int j = 0; j < W; j += 8) store_pack<O, 8>(to + lane * W + j, f + y + j, 8, true);
         if (a.copies_out) {
           // rows past the end are zero anyway; those past `len` are left out
           tc::fence_shared();
           __syncwarp();
-          if (lane == 0 && quarter * 32 < min(C, a.len - c * C) && sc0 < a.dv)
-            tc::store_box4(&map_out, to, sc0, h, c * C + quarter * 32, b);
-          return;
+          if (lane == 0 && quarter * 32 < min(C, a.len - c * C) && sc0 + y < a.dv)
+            tc::store_box4(&map_out, to, sc0 + y, h, c * C + quarter * 32, b);
+        } else {
+          __syncwarp();
+          const int col = lane % W;
+          O* out = static_cast<O*>(a.out) + b * a.out_batch + (int64_t)h * a.dv + sc0 + y + col;
+          if (sc0 + y + col < a.dv) {
+            for (int r = lane / W; r < min(32, count - quarter * 32); r += 32 / W)
+              out[((int64_t)c * C + quarter * 32 + r) * a.out_token] = to[r * W + col];
+          }
         }
-        __syncwarp();
-        const int col = lane & 15;
-        O* out = static_cast<O*>(a.out) + b * a.out_batch + (int64_t)h * a.dv + sc0 + col;
-        if (sc0 + col < a.dv) {
-          for (int r = lane >> 4; r < min(32, count - quarter * 32); r += 2)
-            out[((int64_t)c * C + quarter * 32 + r) * a.out_token] = to[r * 16 + col];
-        }
-        return;
       }
-      if (!live) return;
-      O* out = static_cast<O*>(a.out) + b * a.out_batch + ((int64_t)c * C + row) * a.out_token +
-               (int64_t)h * a.dv + sc0;
-#pragma unroll
-      for (int j = 0; j < 16; j += 8)
-        if (sc0 + j < a.dv) store_pack<O, 8>(out + j, f + j, a.dv - sc0 - j, a.vec_out);
     };
 
 #pragma unroll 1
@@ -817,8 +812,6 @@ cudaError_t run_pass(Pass p, const Array& q, const Array& k, const Array& v, voi
   p.segments = pass_segments<T>(p.batch, p.heads, p.dk, p.dv, p.len);
   p.seg_chunks = std::max(1, (chunks + p.segments - 1) / p.segments);
   p.seg_states = static_cast<float*>(ws);
-  p.vec_out = packed_rows(p.out, 16, sizeof(O), p.out_batch, p.out_token) &&
-              p.dv * sizeof(O) % 16 == 0;
   CUtensorMap maps[4] = {};
   p.copies_out = false;
   if (p.len > 0) {
@@ -826,9 +819,8 @@ cudaError_t run_pass(Pass p, const Array& q, const Array& k, const Array& v, voi
         !head_map(&maps[1], k, 2, p.len, p.batch * P, C, 64, true) ||
         !head_map(&maps[2], v, 2, p.len, p.batch * P, C, 64, true))
       return cudaErrorInvalidValue;
-    p.copies_out = (p.dk <= 64 ? Layout<P, 1, O>::kStaged : Layout<P, 2, O>::kStaged) > 0 &&
-                   head_map(&maps[3], {p.out, p.out_batch, p.out_token, p.heads, p.dv}, sizeof(O),
-                            p.len, p.batch, 32, 16, false);
+    p.copies_out = head_map(&maps[3], {p.out, p.out_batch, p.out_token, p.heads, p.dv}, sizeof(O),
+                            p.len, p.batch, 32, 32 / sizeof(O), false);
   }
   return p.dk <= 64 ? run_panels<P, O, 1>(maps, p, blocks, st, launches)
                     : run_panels<P, O, 2>(maps, p, blocks, st, launches);
