@@ -10,6 +10,7 @@ namespace {
 constexpr int32_t kMostLen = 1 << 30;
 constexpr int32_t kMostDim = 1 << 24;
 constexpr int32_t kMostHeads = 1 << 16;
+constexpr int32_t kMostRows = INT32_MAX - 256;  // a tile's last row is counted in 32 bits
 
 // Whether no two of rows * len runs of `dim` elements, at b * batch + t * token, share an element.
 bool apart(int64_t batch, int64_t token, int32_t rows, int32_t len, int32_t dim) {
@@ -357,7 +358,7 @@ Checks check(const salt_quantize_q8_args* a) {
   c.need(a, "args is NULL");
   if (!c.ok()) return c;
   c.type(a->type);
-  c.need(a->rows >= 0, "rows is negative");
+  c.need(a->rows >= 0 && a->rows <= kMostRows, "rows must lie in [0, 2^31 - 257]");
   c.need(a->dim >= 1 && a->dim <= kMostDim, "dim must lie in [1, 2^24]");
   // a block has 32 groups of a row at least, or a tile of 128 x 128
   c.need((int64_t)a->rows * ((a->dim + 127) / 128) <= (int64_t)INT32_MAX * 32,
@@ -380,7 +381,7 @@ Checks check(const salt_matmul_q8_args* a) {
   if (!c.ok()) return c;
   c.type(a->type);
   c.wide(a->bias_type, a->type, "bias_type must be type or SALT_F32");
-  c.need(a->rows >= 0, "rows is negative");
+  c.need(a->rows >= 0 && a->rows <= kMostRows, "rows must lie in [0, 2^31 - 257]");
   c.need(a->n >= 1 && a->n <= kMostDim, "n must lie in [1, 2^24]");
   c.need(a->k >= 1 && a->k <= kMostDim, "k must lie in [1, 2^24]");
   // tiles are counted in 32 bits

@@ -180,12 +180,20 @@ def test_c_entries_refuse_null_sizes_and_small_workspaces():
     m = _lib.MatmulQ8Args(4, 300, 200, 0, 0, 0, 200, 200, 300, at, at, at, at, None, at)
     size = lib.salt_matmul_q8_workspace_size
     assert size(ctypes.byref(m), ctypes.byref(n)) == 0
-    for field, bad in (("type", 4), ("bias_type", 1), ("rows", -1), ("n", 0), ("k", 0),
+    for field, bad in (("type", 4), ("bias_type", 1), ("rows", -1), ("rows", 2 ** 31 - 1), ("n", 0), ("k", 0),
                        ("k", 2 ** 24 + 1), ("x_stride", -1), ("out_stride", 299), ("x", None),
                        ("weight_scale", None), ("out", None)):
         old = getattr(m, field)
         setattr(m, field, bad)
         assert size(ctypes.byref(m), ctypes.byref(n)) == _lib.SALT_BAD_ARG, field
         setattr(m, field, old)
+    q = _lib.QuantizeQ8Args(4, 200, 0, 0, 0, 0, 200, 200, at, at, at)
+    for field, bad in (("type", 4), ("rows", -1), ("rows", 2 ** 31 - 1), ("dim", 0),
+                       ("dim", 2 ** 24 + 1), ("x_stride", -1), ("out_stride", 199), ("x", None),
+                       ("scale", None)):
+        old = getattr(q, field)
+        setattr(q, field, bad)
+        assert lib.salt_quantize_q8(ctypes.byref(q), None) == _lib.SALT_BAD_ARG, field
+        setattr(q, field, old)
     m.type, m.bias_type, m.rows = 2, 1, 0  # without rows, too, and with a bias of neither type
     assert size(ctypes.byref(m), ctypes.byref(n)) == _lib.SALT_BAD_ARG
