@@ -60,6 +60,8 @@ struct Layout {
   static constexpr int q = 0, k = q + kKeys, v = k + B * kKeys, weighted = v + B * kValues,
                        state = weighted + kWeighted * kPanel, out = state + state_parts(P) * kState,
                        bytes = out + kWorkers / 32 * kStaged + 1024;
+  // the pass that wants the states alone has weighted values of two chunks instead
+  static constexpr int state_bytes = weighted + 2 * kWeighted * kPanel + 1024;
 };
 
 // Two values in parts of bfloat16: the upper 8 bits of what is left, time and again; the last of two
@@ -198,6 +200,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   const uint32_t tmem = tmem_at, mine = tmem + ((uint32_t)(quarter * 32) << 16);
   // columns of tensor memory
   constexpr int kScores = 0, kTriangle = 128, kFromState = 256, kOut = 384, kAdded = 448;
+  const auto added = [&](int i) { return STATE ? (i & 1) * kTile : kAdded; };
+  const auto values = [&](int i) { return STATE ? (i & 1) * kWeighted * kPanel : 0; };
   uint32_t tries = tc::kTries;
 
   if (warp == kWorkers / 32) {
@@ -285,8 +289,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
               if (y < 0 || y >= kWeighted) continue;
 #pragma unroll
               for (int d = 0; d < C / 16; ++d) {
-                tc::product_16(tmem + kAdded, tc::further(k, x * PANELS * kPanel + d * 2048),
-                               tc::further(weighted, y * kPanel + d * 2048),
+                tc::product_16(tmem + added(i), tc::further(k, x * PANELS * kPanel + d * 2048),
+                               tc::further(weighted, values(i) + y * kPanel + d * 2048),
                                tc::shape(128, kTile, 1, true, true), add);
                 add = true;
               }
@@ -429,7 +433,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           }
           split2<kWeighted>(out[m], mul2(y, both(w)));
         }
-        uint8_t* to = sm + L::weighted + (place - v);
+        uint8_t* to = sm + L::weighted + values(i) + (place - v);
 #pragma unroll
         for (int j = 0; j < kWeighted; ++j)
           *reinterpret_cast<uint4*>(to + j * kPanel) =
@@ -495,10 +499,14 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       }
     };
 
+    if (STATE && steps > 0) begin(0);
 #pragma unroll 1
     for (int i = 0; i < steps; ++i) {
       const int count = tokens(chunk(i));
-      begin(i);
+      if (!STATE)
+        begin(i);
+      else if (i + 1 < steps)
+        begin(i + 1);  // while this chunk's product runs
       if (!STATE) {
         if (i > 0) finish(i - 1);
         // the triangle's weights
@@ -570,7 +578,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       tc::barrier_wait_warp(&done_state, i & 1, tries);
       tc::fence_after();
       uint32_t x[16];
-      tc::tmem_load<16>(x, mine + kAdded + part * 16);
+      tc::tmem_load<16>(x, mine + added(i) + part * 16);
       tc::loads_done();
       tc::fence_before();
       const float l = power[count], by = a.reverse ? a.scale : 1.f;
@@ -591,10 +599,11 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           tc::barrier_wait_warp(&done_q, i & 1, tries);
           store_state();
         }
-        // every warp is past the chunk before: its marks are free
+        // every warp is past the chunk before (STATE: past this one): its marks are free
         tc::named_sync(1, kWorkers);
-        if (threadIdx.x < kTile) bad[(i + 2) % 3][threadIdx.x] = -1;
-        if (threadIdx.x == 0) any_bad[(i + 2) % 3] = 0;
+        constexpr int kFree = STATE ? 0 : 2;
+        if (threadIdx.x < kTile) bad[(i + kFree) % 3][threadIdx.x] = -1;
+        if (threadIdx.x == 0) any_bad[(i + kFree) % 3] = 0;
       }
     }
     if (!STATE && steps > 0) finish(steps - 1);
@@ -744,7 +753,7 @@ template <int P, typename O, int PANELS, bool STATE>
 cudaError_t start(const CUtensorMap (&maps)[4], const Pass& p, int64_t blocks, cudaStream_t st,
                   int* launches) {
   const auto kernel = attention_kernel<P, O, PANELS, STATE>;
-  constexpr int bytes = Layout<P, PANELS, O>::bytes;
+  constexpr int bytes = STATE ? Layout<P, PANELS, O>::state_bytes : Layout<P, PANELS, O>::bytes;
   const cudaError_t e =
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return e;
