@@ -143,12 +143,16 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                  const __grid_constant__ CUtensorMap map_out, const Pass a) {
   using L = Layout<P, PANELS, O>;
   constexpr int C = L::C, B = L::B, SP = state_parts(P), DK = PANELS * 64;
+  constexpr int VB = STATE ? B + PANELS : B;  // places for values, also where q is not needed
   constexpr int kPanel = L::kPanel;
   extern __shared__ uint8_t raw[];
   uint8_t* sm = raw + (1024 - tc::shared_at(raw) % 1024) % 1024;
-  __shared__ uint64_t loaded_q, loaded_k[B], loaded_v[B];  // copies
-  __shared__ uint64_t done_scores, done_q, done_state, done_out;  // products
-  __shared__ uint64_t ready_chunk, ready_triangle;  // operands that threads wrote
+  __shared__ uint64_t loaded_q, loaded_k[B], loaded_v[VB];  // copies
+  // Products, and operands that threads wrote.  (Who waits at a barrier has to see every phase of it: the
+  // next one ends only after all of them went on.  STATE runs a chunk ahead of its products, and takes
+  // two barriers in turn.)
+  constexpr int R = STATE ? 2 : 1;
+  __shared__ uint64_t done_scores, done_q, done_state[R], done_out, ready_chunk[R], ready_triangle;
   __shared__ uint32_t tmem_at;
   __shared__ float powers[32 + C + 1];        // l^i from place 32 on
   __shared__ __align__(16) float column[32];  // of a column within its 32
@@ -175,13 +179,13 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   const auto tokens = [&](int c) { return min(C, n - c * C); };
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < B; ++i) {
-      tc::barrier_init(&loaded_k[i], 1);
-      tc::barrier_init(&loaded_v[i], 1);
+    for (int i = 0; i < B; ++i) tc::barrier_init(&loaded_k[i], 1);
+    for (int i = 0; i < VB; ++i) tc::barrier_init(&loaded_v[i], 1);
+    for (uint64_t* x : {&loaded_q, &done_q, &done_scores, &done_out}) tc::barrier_init(x, 1);
+    for (int i = 0; i < R; ++i) {
+      tc::barrier_init(&done_state[i], 1);
+      tc::barrier_init(&ready_chunk[i], kWorkers / 32);
     }
-    for (uint64_t* x : {&loaded_q, &done_q, &done_scores, &done_state, &done_out})
-      tc::barrier_init(x, 1);
-    tc::barrier_init(&ready_chunk, kWorkers / 32);
     tc::barrier_init(&ready_triangle, kWorkers / 32);
     tc::barrier_init_fence();
   }
@@ -201,6 +205,9 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   // columns of tensor memory
   constexpr int kScores = 0, kTriangle = 128, kFromState = 256, kOut = 384, kAdded = 448;
   const auto added = [&](int i) { return STATE ? (i & 1) * kTile : kAdded; };
+  const auto value_place = [&](int i) {
+    return i % VB < B ? L::v + i % VB * L::kValues : L::q + (i % VB - B) * L::kValues;
+  };
   const auto values = [&](int i) { return STATE ? (i & 1) * kWeighted * kPanel : 0; };
   uint32_t tries = tc::kTries;
 
@@ -222,7 +229,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       };
       const auto fetch_v = [&](int i) {
         if (i < steps)
-          fetch(L::v + i % B * L::kValues, &map_v, 1, col0, h / a.v_share, i, &loaded_v[i % B]);
+          fetch(value_place(i), &map_v, 1, col0, h / a.v_share, i, &loaded_v[i % VB]);
       };
       const int depth = (a.dk + 15) / 16;
       const uint64_t q = tc::operand(sm + L::q, 1024), state = tc::operand(sm + L::state, 1024),
@@ -245,9 +252,9 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           }
         tc::products_done(&done_scores);
       };
-      for (int i = 0; i < B; ++i) {
+      for (int i = 0; i < VB; ++i) {
         fetch_v(i);
-        fetch_k(i);
+        if (i < B) fetch_k(i);
         if (!STATE && i == 0) fetch_q(0);
       }
       tc::barrier_wait(&loaded_k[0], 0, tries);
@@ -257,8 +264,9 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       }
 #pragma unroll 1
       for (int i = 0; i < steps; ++i) {
-        tc::barrier_wait(&ready_chunk, i & 1, tries);
+        tc::barrier_wait(&ready_chunk[i % R], i / R & 1, tries);
         tc::fence_after();
+        if (STATE) fetch_v(i + VB);
         if (!STATE) {
           bool add = false;
 #pragma unroll
@@ -295,7 +303,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 add = true;
               }
             }
-          tc::products_done(&done_state);
+          tc::products_done(&done_state[i % R]);
         }
         if (!STATE) {
           tc::barrier_wait(&done_q, i & 1, tries);
@@ -328,10 +336,12 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           scores(i + 1);
         };
         if (B == 2) next();
-        tc::barrier_wait(&done_state, i & 1, tries);
+        tc::barrier_wait(&done_state[i % R], i / R & 1, tries);
         fetch_k(i + B);
-        if (!STATE) tc::barrier_wait(&done_out, i & 1, tries);
-        fetch_v(i + B);
+        if (!STATE) {
+          tc::barrier_wait(&done_out, i & 1, tries);
+          fetch_v(i + B);
+        }
         if (B == 1) next();
       }
     }
@@ -374,8 +384,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     const auto begin = [&](int i) {
       const int count = tokens(chunk(i));
       uint8_t* k = sm + L::k + i % B * L::kKeys;
-      uint8_t* v = sm + L::v + i % B * L::kValues;
-      tc::barrier_wait_warp(&loaded_v[i % B], i / B & 1, tries);
+      uint8_t* v = sm + value_place(i);
+      tc::barrier_wait_warp(&loaded_v[i % VB], i / VB & 1, tries);
       if (P == 1 && count < C) {  // (planes hold zeros there)
         tc::barrier_wait_warp(&loaded_k[i % B], i / B & 1, tries);
         for (int x = threadIdx.x; x < (C - count) * PANELS * 8; x += kWorkers) {
@@ -442,7 +452,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       tc::fence_shared();
       tc::fence_before();
       __syncwarp();
-      tc::barrier_arrive_if_zero(&ready_chunk, lane);
+      tc::barrier_arrive_if_zero(&ready_chunk[i % R], lane);
     };
     // Chunk i's output, once its products are there.
     const auto finish = [&](int i) {
@@ -575,7 +585,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         tc::barrier_arrive_if_zero(&ready_triangle, lane);
       }
       // the state behind the chunk
-      tc::barrier_wait_warp(&done_state, i & 1, tries);
+      tc::barrier_wait_warp(&done_state[i % R], i / R & 1, tries);
       tc::fence_after();
       uint32_t x[16];
       tc::tmem_load<16>(x, mine + added(i) + part * 16);

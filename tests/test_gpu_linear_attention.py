@@ -190,6 +190,32 @@ def test_long_rows_of_few_heads(kind, n, dk, dv):
         c.check_backward()
 
 
+@pytest.mark.parametrize("kind, dk", (("bfloat16", 128), ("bfloat16", 32), ("float16", 128),
+                                      ("float16", 64), ("float32", 64)))
+def test_segments_of_many_chunks(kind, dk):
+    """More heads than a few, so that each segment of a row has tens of chunks: both passes go around
+    all their buffers again and again.  The definition in chunks here: 64 bits, 50 tokens at a time."""
+    heads, n, dv = 16, 9000, 64
+    c = Case(kind, 1, n, heads, heads, dk, dv, 11, log_decay=np.log1p(-(2.0 ** -np.linspace(3, 11, heads))))
+    q, k, v = (c.host[x][0].transpose(1, 0, 2) for x in "qkv")
+    lam = A.decays(c.log_decay)[:, None, None]
+    at = np.arange(50)
+    inner = np.where(at[:, None] >= at, lam ** np.maximum(at[:, None] - at, 0), 0)
+    s, m = np.zeros((2, heads, dk, dv))
+    want, mag = np.zeros((2, heads, n, dv))
+    for t in range(0, n, 50):
+        cut = slice(t, t + 50)
+        for w, size, f in ((want, s, lambda a: a), (mag, m, np.abs)):
+            qc, kc, vc = (f(a[:, cut]) for a in (q, k, v))
+            w[:, cut] = (qc * lam ** (at[:, None] + 1)) @ size + ((qc @ kc.swapaxes(1, 2)) * inner) @ vc
+            size *= lam ** 50
+            size += (kc * lam ** (49 - at[:, None])).swapaxes(1, 2) @ vc
+    out, final = c.forward()
+    R.assert_close(out.values()[0].transpose(1, 0, 2), c.scale * want, c.scale * mag,
+                   steps(n, kind), kind, "out")
+    R.assert_close(R.values(final)[0], s, m, steps(n), "float32", "state")
+
+
 def test_many_rows_and_heads():
     """More heads than blocks that fit at once."""
     c = Case("bfloat16", 40, 70, 16, 4, 32, 32, 1, n_real=list(range(0, 80, 2)))
