@@ -764,8 +764,8 @@ cudaError_t start(const CUtensorMap (&maps)[4], const Pass& p, int64_t blocks, c
                   int* launches) {
   const auto kernel = attention_kernel<P, O, PANELS, STATE>;
   constexpr int bytes = STATE ? Layout<P, PANELS, O>::state_bytes : Layout<P, PANELS, O>::bytes;
-  const cudaError_t e =
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  static std::atomic<uint64_t> allowed{0};
+  const cudaError_t e = tc::allow_shared(reinterpret_cast<const void*>(kernel), bytes, allowed);
   if (e != cudaSuccess) return e;
   kernel<<<(unsigned)blocks, kThreads, bytes, st>>>(maps[0], maps[1], maps[2], maps[3], p);
   ++*launches;

@@ -447,8 +447,9 @@ cudaError_t launch(Operand a, Operand b, int64_t k, Product p, cudaStream_t st, 
     return cudaErrorInvalidValue;
   if (!SWAP && p.vec && !out_map<T>(&map_out, p.out, p.rows_a, p.rows_b, p.out_stride)) p.vec = false;
   const auto kernel = matmul_q8_kernel<BN, SWAP, T>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       shared_bytes(BN, SWAP));
+  static std::atomic<uint64_t> allowed{0};
+  const cudaError_t e = tc::allow_shared(reinterpret_cast<const void*>(kernel),
+                                         shared_bytes(BN, SWAP), allowed);
   if (e != cudaSuccess) return e;
   const int64_t total = (int64_t)p.tiles_a * p.tiles_b;
   cudaLaunchConfig_t c = {};

@@ -4,6 +4,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 namespace salt::tc {
@@ -281,6 +282,18 @@ inline EncodeTiled encoder() {
     return reinterpret_cast<EncodeTiled>(p);
   }();
   return f;
+}
+// Lets a kernel have that much dynamic shared memory: asked of the runtime once a device (`done` is the
+// kernel's own, a bit a device).
+inline cudaError_t allow_shared(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
 }
 constexpr int64_t kMostStride = 1ll << 39;  // bytes: a tensor map's strides lie under 2^40
 
