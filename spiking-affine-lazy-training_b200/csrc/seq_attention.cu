@@ -45,7 +45,9 @@ template <typename T>
 constexpr int parts_of() { return sizeof(T) == 4 ? 3 : std::is_same<T, __half>::value ? 2 : 1; }
 // Tokens of a chunk, and parts of the states and of the weights within a chunk.
 // (64 where 128 do not fit into shared memory)
-constexpr int chunk_of(int parts, int panels) { return parts == 1 || (parts == 2 && panels == 1) ? 128 : 64; }
+constexpr int chunk_of(int parts, int panels) {
+  return parts == 1 || (parts == 2 && panels == 1) ? 128 : 64;
+}
 constexpr int state_parts(int parts) { return parts == 3 ? 3 : 2; }
 
 // Shared memory, all operands in rows of 128 bytes (tc::operand): q and k in panels of 64 columns,
@@ -130,12 +132,29 @@ __global__ void __launch_bounds__(256) planes_kernel(const AllToPlanes all, int 
 // as four products of the tensor cores.  Per chunk and head, with c = C tokens: 2 c^2 dk + 2 c^2 dv +
 // 4 c dk dv operations, against the 5 dk dv a token of the recurrence itself.
 //
+// A block has a row's head and 64 columns of v.  Sixteen warps write operands and take results, one warp
+// copies and multiplies:
+//   values' weights -> [q S, k^T (weights v)] -> the state -> the next chunk's values' weights
+//   [q k^T] -> triangle -> [its product with v] -> out, a chunk behind
+//
 // What is rounded: every operand is bfloat16, in parts of 8 bits.  Inputs are exact (bfloat16 in one
-// part, float16 in two, float32 in three, the last rounded); weighted values have three parts, so
-// that states are good to 2^-24; states and the triangle's values, as operands for out, have three
+// part, float16 in two, float32 in three); weighted values have three parts, so that states are good to
+// 2^-24; states and the triangle's values, as operands for out, have three
 // parts for float32 and two (2^-16) for outputs of 16 bits.  Sums and states are float32; the state
 // is carried in registers.  The tensor cores cut their sums off after every instruction, so the parts'
-// products go from the smallest to the largest: in the other order float32's outputs were off by 2.5e-6.
+// products go from the smallest to the largest: in the other order float32's outputs were off by 2.5e-6
+// instead of 3.5e-7.
+//
+// What bounds it: the threads' work on operands.  8 rows of 2048 x 16 heads of 128 in bfloat16 take 133
+// us, 2.1 TB/s, 3.2 times their bytes' time: 256 blocks are two rounds of 16 chunks of some 7000 cycles,
+// of which the tensor cores work 2900 (an instruction of 128 x 64 x 16 takes 48 cycles, 30 with an
+// operand in tensor memory), the warps wait 1200 at barriers, and an instruction issues in every other
+// cycle.  One row of 32768 takes 334 us: 9 segments, 105 of it the states' pass.  float16 heads of 128
+// and float32 have chunks of 64 tokens, since shared memory holds no more of their parts: the long row
+// in float16 takes 850 us.
+// Measured and left: eight warps (269 us), all products' warps in step with the others (189 us; this
+// is 133), roles for the warps, eight for triangle and out, four for the state and four for the values
+// (180 us: four warps wait too long for their own instructions).
 template <int P, typename O, int PANELS, bool STATE>
 __global__ void __launch_bounds__(kThreads, 1)
 attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -148,9 +167,9 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   extern __shared__ uint8_t raw[];
   uint8_t* sm = raw + (1024 - tc::shared_at(raw) % 1024) % 1024;
   __shared__ uint64_t loaded_q, loaded_k[B], loaded_v[VB];  // copies
-  // Products, and operands that threads wrote.  (Who waits at a barrier has to see every phase of it: the
-  // next one ends only after all of them went on.  STATE runs a chunk ahead of its products, and takes
-  // two barriers in turn.)
+  // Products, and operands that threads wrote.  (Who waits at a barrier has to see every phase of it:
+  // the next one ends only after all of them went on.  STATE runs a chunk ahead of its products, and
+  // takes two barriers in turn.)
   constexpr int R = STATE ? 2 : 1;
   __shared__ uint64_t done_scores, done_q, done_state[R], done_out, ready_chunk[R], ready_triangle;
   __shared__ uint32_t tmem_at;
@@ -601,7 +620,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         for (int j = 0; j < 16; ++j) {
           if (bad[i % 3][part * 16 + j] < 0) continue;
           const float2 y = halves(s[j / 2]);
-          s[j / 2] = j % 2 ? pair(y.x, __int_as_float(0x7fffffff)) : pair(__int_as_float(0x7fffffff), y.y);
+          const float nan = __int_as_float(0x7fffffff);
+          s[j / 2] = j % 2 ? pair(y.x, nan) : pair(nan, y.y);
         }
       }
       if (i + 1 < steps) {
@@ -634,7 +654,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     if (!STATE) {
       // tokens behind the row's end
       const int end = min(a.len, (seg + 1) * a.seg_chunks * C);
-      for (int64_t t = max(a.copies_out ? chunks * C : n, seg * a.seg_chunks * C) + warp; t < end; t += kWorkers / 32)
+      for (int64_t t = max(a.copies_out ? chunks * C : n, seg * a.seg_chunks * C) + warp; t < end;
+           t += kWorkers / 32)
         for (int j = lane; j < cols; j += 32)
           static_cast<O*>(a.out)[b * a.out_batch + t * a.out_token + (int64_t)h * a.dv + col0 + j] =
               from_f32<O>(0.f);

@@ -41,13 +41,25 @@ struct Product {
 
 // out = sum over groups of scale_a scale_b (the group's product of e4m3 values).
 //
-// The tensor cores add up one group (128 x BN x 128, in 32 bits) into one of two buffers of tensor
-// memory; eight warps take it from there, times both scales, to their running sums in registers,
-// while the next group's product goes to the other buffer.
+// The tensor cores add up one group (128 x BN x 128, in 32 bits) into one of two to eight buffers of
+// tensor memory; eight warps take it from there, times both scales, to their running sums in registers,
+// while the next groups' products go to the other buffers.
 //
 // SWAP = false: rows of x are the lanes, weight rows the columns, and a warp's columns share one scale
 // (blocks of 128).  SWAP = true: weight rows are the lanes, rows of x the columns, each with its own
 // scale, which goes through shared memory; a warp's stores are then neighbours in a row of out.
+//
+// What bounds it: a scale for every 128 of the depth makes the sums a multiplication and an addition of
+// every value for each group.  At BN = 256 a group's products take 512 cycles and its sums 360 of every
+// scheduler's, next to some 250 of waiting at barriers and taking the values out of tensor memory:
+// 16384 x 5120 x 5120 takes 426 us in bfloat16, 2.02 PFLOP/s (350 us without sums and outputs, 268 us
+// the library's product with one scale a tensor).  Columns with a scale each take two multiplications a
+// value: 2048 x 4096 x 8192 with both operands' scales by rows, to float32, 141 us, 0.97 PFLOP/s.  Few
+// rows are bound by what a block waits for: 64 rows of 8192 x 8192 take 26 us, 2.6 TB/s; 16 rows of 2048
+// x 4096 9 us, most of it the start, the first copies and the joining.
+// Measured and left: two blocks on a tile of 256 x 256 (440 us then, as much as one), sixteen warps of
+// sums (455), packed arithmetic for the sums (447), two sets of warps on every other group of narrow
+// tiles (24.4 us for 64 rows).
 template <int BN, bool SWAP, typename T>
 __global__ void __launch_bounds__(kThreads, 1)
 matmul_q8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
@@ -347,13 +359,22 @@ matmul_q8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
 }
 
 // Rows on boundaries of 16 bytes: what a tensor copy needs, for operands that do not lie so.
-__global__ void __launch_bounds__(256) align_rows_kernel(const uint8_t* from, int64_t stride,
-                                                         int64_t rows, int k, uint4* to, int units) {
-  const int64_t n = rows * units;
+// blockIdx.y is the operand.
+struct Rows {
+  const uint8_t* from;
+  int64_t stride, rows;
+  uint4* to;
+};
+struct BothRows {
+  Rows r[2];
+};
+__global__ void __launch_bounds__(256) align_rows_kernel(const BothRows both, int k, int units) {
+  const Rows x = both.r[blockIdx.y];
+  const int64_t n = x.rows * units;
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
     const int64_t row = n >> 32 ? i / units : (unsigned)i / (unsigned)units;
     const int at = (int)(i - row * units) * 16;
-    const uint8_t* p = from + row * stride + at;
+    const uint8_t* p = x.from + row * x.stride + at;
     uint32_t w[4] = {};
     const uintptr_t off = reinterpret_cast<uintptr_t>(p) & 3;
     if (at >= 4 && at + 20 <= k) {
@@ -369,7 +390,7 @@ __global__ void __launch_bounds__(256) align_rows_kernel(const uint8_t* from, in
       for (int j = 0; j < 16; ++j)
         if (at + j < k) w[j / 4] |= (uint32_t)p[j] << (j % 4 * 8);
     }
-    to[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    x.to[i] = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
@@ -419,21 +440,29 @@ struct Operand {
   const void* p;
   int64_t rows, stride;
 };
-cudaError_t prepare(Operand& o, int64_t k, uint8_t*& ws, cudaStream_t st, int* launches) {
-  if (tiled(o.p, o.rows, o.stride, k)) {
-    if (o.rows == 1) o.stride = aligned_stride(k);
-    return cudaSuccess;
-  }
+// Both operands as tensor copies can take them, copied to the workspace where they are not.
+cudaError_t prepare(Operand* const (&all)[2], int64_t k, uint8_t* ws, cudaStream_t st, int* launches) {
+  BothRows to = {};
+  int count = 0;
+  int64_t most = 0;
   const int units = (int)(aligned_stride(k) / 16);
-  const int64_t blocks = (o.rows * units + 255) / 256;
-  align_rows_kernel<<<(unsigned)std::min<int64_t>(blocks, 148 * 16), 256, 0, st>>>(
-      static_cast<const uint8_t*>(o.p), o.stride, o.rows, (int)k, reinterpret_cast<uint4*>(ws),
-      units);
+  for (Operand* o : all) {
+    if (tiled(o->p, o->rows, o->stride, k)) {
+      if (o->rows == 1) o->stride = aligned_stride(k);
+      continue;
+    }
+    to.r[count++] = {static_cast<const uint8_t*>(o->p), o->stride, o->rows,
+                     reinterpret_cast<uint4*>(ws)};
+    most = std::max(most, o->rows * units);
+    const size_t bytes = copy_bytes(o->p, o->rows, o->stride, k);
+    o->p = ws;
+    o->stride = aligned_stride(k);
+    ws += bytes;
+  }
+  if (!count) return cudaSuccess;
+  align_rows_kernel<<<dim3((unsigned)std::min<int64_t>((most + 255) / 256, 148 * 8), count), 256, 0,
+                      st>>>(to, (int)k, units);
   ++*launches;
-  const size_t bytes = copy_bytes(o.p, o.rows, o.stride, k);
-  o.p = ws;
-  o.stride = aligned_stride(k);
-  ws += bytes;
   return cudaGetLastError();
 }
 
@@ -478,8 +507,9 @@ cudaError_t run(const salt_matmul_q8_args& a, const Operand& x, const Operand& w
   p.bias = a.bias;
   p.bias_f32 = a.bias_type == SALT_F32;
   const int shift_w = a.weight_rows ? 0 : 7;
-  // Time in rounds of resident blocks (one an SM), counted in groups of a tile.  `each` is what a group
-  // of a tile takes, in us: measured with K = 2048 to 8192 at full rounds.
+  // Time in us by rounds of resident blocks (one an SM); `each` is what a group of a tile takes,
+  // measured at full rounds with a depth of 2048 to 8192.  (1024 x 4096 x 4096: 128 tiles of 128 x 256
+  // take 28 us, 256 tiles of 128 x 128 37 us.)
   const auto time = [&](int64_t tiles, double each, int split) {
     return (double)((tiles * split + 147) / 148) * (each * ((p.groups + split - 1) / split) + 1) +
            (split > 1 ? 2 : 0);
@@ -497,7 +527,7 @@ cudaError_t run(const salt_matmul_q8_args& a, const Operand& x, const Operand& w
   const auto by_columns = [&](int bn, double each) {
     return time(tiles(a.n, a.rows, bn), each, split_of(bn));
   };
-  const double least = std::min(by_columns(128, 0.5), by_columns(256, 1.0) + (split_of(256) > 1 ? 1e9 : 0));
+  const double least = std::min(by_columns(128, 0.5), time(tiles(a.n, a.rows, 256), 1.0, 1));
   if (!a.weight_rows && a.rows > 64) {
     const double wide = time(tiles(a.rows, a.n, 256), 0.63, 1),
                  narrow = time(tiles(a.rows, a.n, 128), 0.5, 1);
@@ -538,10 +568,8 @@ size_t matmul_q8_bytes(const salt_matmul_q8_args& a) {
 cudaError_t matmul_q8_launch(const salt_matmul_q8_args& a, void* ws, cudaStream_t st,
                              int* launches) {
   if (!a.rows) return cudaSuccess;
-  uint8_t* room = static_cast<uint8_t*>(ws);
   Operand x{a.x, a.rows, a.x_stride}, w{a.weight, a.n, a.weight_stride};
-  cudaError_t e = prepare(x, a.k, room, st, launches);
-  if (e == cudaSuccess) e = prepare(w, a.k, room, st, launches);
+  cudaError_t e = prepare({&x, &w}, a.k, static_cast<uint8_t*>(ws), st, launches);
   if (e != cudaSuccess) return e;
   SALT_WITH_TYPE(a.type, T, e = run<T>(a, x, w, st, launches));
   return e;

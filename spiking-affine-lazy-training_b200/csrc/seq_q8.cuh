@@ -24,7 +24,12 @@ constexpr float kE4m3Max = 448.f;
 struct E4m3Scale {
   float scale, lift;
   f32x2 high, low;
-  E4m3Scale() = default;
+  // the four numbers of one, to be kept in shared memory
+  __device__ __forceinline__ float4 packed() const {
+    return make_float4(scale, lift, halves(high).x, halves(low).x);
+  }
+  __device__ __forceinline__ explicit E4m3Scale(const float4& p)
+      : scale(p.x), lift(p.y), high(both(p.z)), low(both(p.w)) {}
   __device__ __forceinline__ explicit E4m3Scale(float m) : lift(1.f) {
     float divisor;
     if (m >= 0x1p-60f && m < 0x1p60f) {
