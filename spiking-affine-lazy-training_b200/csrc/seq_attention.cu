@@ -413,56 +413,73 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
               make_uint4(0, 0, 0, 0);
         }
       }
+      // A thread has the same 8 columns of N rows; all of its loads go out before its first store.
+      constexpr int N = C * 8 / kWorkers, kApart = kWorkers / 8;
+      const int r0 = threadIdx.x >> 3, u = threadIdx.x & 7;
+      uint8_t* place = v + r0 * 128 + ((u ^ (r0 & 7)) << 4);  // kApart is a multiple of 8
+      uint32_t in[N][P][4], carry = 0;  // (carry: from an exponent of all ones)
 #pragma unroll
-      for (int x = threadIdx.x; x < C * 8; x += kWorkers) {
-        const int r = x >> 3, u = x & 7;
-        uint8_t* place = v + r * 128 + ((u ^ (r & 7)) << 4);
-        const float w = r >= count ? 0.f : power[a.reverse ? r + 1 : count - 1 - r];
-        uint32_t in[P][4], out[4][kWeighted];
-        uint32_t carry = 0;  // from an exponent of all ones
+      for (int x = 0; x < N; ++x)
 #pragma unroll
         for (int j = 0; j < P; ++j) {
-          const uint4 y = *reinterpret_cast<const uint4*>(place + j * kPanel);
-          in[j][0] = y.x, in[j][1] = y.y, in[j][2] = y.z, in[j][3] = y.w;
+          const uint4 y = *reinterpret_cast<const uint4*>(place + x * kApart * 128 + j * kPanel);
+          in[x][j][0] = y.x, in[x][j][1] = y.y, in[x][j][2] = y.z, in[x][j][3] = y.w;
         }
-        if (r >= count) {
+      if (count < C) {
+#pragma unroll
+        for (int x = 0; x < N; ++x) {
+          if (r0 + x * kApart < count) continue;
 #pragma unroll
           for (int j = 0; j < P; ++j) {
-            in[j][0] = in[j][1] = in[j][2] = in[j][3] = 0;
-            *reinterpret_cast<uint4*>(place + j * kPanel) = make_uint4(0, 0, 0, 0);
+            in[x][j][0] = in[x][j][1] = in[x][j][2] = in[x][j][3] = 0;
+            *reinterpret_cast<uint4*>(place + x * kApart * 128 + j * kPanel) =
+                make_uint4(0, 0, 0, 0);
           }
         }
+      }
+#pragma unroll
+      for (int x = 0; x < N; ++x)
+#pragma unroll
+        for (int m = 0; m < 4; ++m) carry |= (in[x][0][m] & 0x7f807f80u) + 0x00800080u;
+      if (carry & 0x80008000u) {
         // A value that is not finite would reach the tokens on the triangle's other side, as 0 * it:
         // it becomes zero here, and its column NaN from its token on.
+        any_bad[i % 3] = 1;
 #pragma unroll
-        for (int m = 0; m < 4; ++m) carry |= (in[0][m] & 0x7f807f80u) + 0x00800080u;
-        if (carry & 0x80008000u) {
-          any_bad[i % 3] = 1;
+        for (int x = 0; x < N; ++x) {
+          const int r = r0 + x * kApart;
 #pragma unroll
           for (int m = 0; m < 8; ++m) {
             const uint32_t mask = 0xffffu << (m & 1) * 16, exponent = 0x7f80u << (m & 1) * 16;
-            if ((in[0][m / 2] & exponent) != exponent) continue;
+            if ((in[x][0][m / 2] & exponent) != exponent) continue;
             atomicMax(&bad[i % 3][u * 8 + m], a.reverse ? r : C - 1 - r);
 #pragma unroll
-            for (int j = 0; j < P; ++j) in[j][m / 2] &= ~mask;
+            for (int j = 0; j < P; ++j) in[x][j][m / 2] &= ~mask;
           }
 #pragma unroll
           for (int j = 0; j < P; ++j)
-            *reinterpret_cast<uint4*>(place + j * kPanel) =
-                make_uint4(in[j][0], in[j][1], in[j][2], in[j][3]);
+            *reinterpret_cast<uint4*>(place + x * kApart * 128 + j * kPanel) =
+                make_uint4(in[x][j][0], in[x][j][1], in[x][j][2], in[x][j][3]);
         }
+      }
+#pragma unroll
+      for (int x = 0; x < N; ++x) {
+        const int r = r0 + x * kApart;
+        // (rows past the end are zero, whatever their weight; power has 32 places in front)
+        const float w = power[a.reverse ? r + 1 : max(count - 1 - r, 0)];
+        uint32_t out[4][kWeighted];
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
           f32x2 y = 0;
 #pragma unroll
           for (int j = 0; j < P; ++j) {
-            const f32x2 part = pair(__uint_as_float(in[j][m] << 16),
-                                    __uint_as_float(in[j][m] & 0xffff0000u));
-            y = j == 0 ? part : add2(y, part);
+            const f32x2 one = pair(__uint_as_float(in[x][j][m] << 16),
+                                   __uint_as_float(in[x][j][m] & 0xffff0000u));
+            y = j == 0 ? one : add2(y, one);
           }
           split2<kWeighted>(out[m], mul2(y, both(w)));
         }
-        uint8_t* to = sm + L::weighted + values(i) + (place - v);
+        uint8_t* to = sm + L::weighted + values(i) + (place - v) + x * kApart * 128;
 #pragma unroll
         for (int j = 0; j < kWeighted; ++j)
           *reinterpret_cast<uint4*>(to + j * kPanel) =
@@ -541,8 +558,10 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         // the triangle's weights
         tc::barrier_wait_warp(&done_scores, i & 1, tries);
         tc::fence_after();
-        if (part < C / 32 && quarter < C / 32) {
-          const bool none = a.reverse ? part < quarter || part * 32 >= count : part > quarter;
+        // blocks on the other side hold the zeros that the first chunk left there
+        const bool beside = a.reverse ? part < quarter : part > quarter;
+        if (part < C / 32 && quarter < C / 32 && !(beside && i > 0)) {
+          const bool none = beside || (a.reverse && part * 32 >= count);
           const bool diagonal = part == quarter;
           // against time, columns past the end lie on the triangle's side
           const bool cut = a.reverse && part * 32 + 32 > count;
