@@ -655,21 +655,32 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         if (threadIdx.x == 0) any_bad[(i + kFree) % 3] = 0;
       }
     }
-    if (!STATE && steps > 0) finish(steps - 1);
-    if (!STATE && lane == 0) tc::stores_done();
-    __syncwarp();
-
+    // the state goes out while the last outputs' product runs
     const bool last = a.reverse ? seg == 0 : (c1 == chunks && (c0 < chunks || seg == 0));
     float* to = STATE ? a.seg_states + ((int64_t)bh * a.segments + seg) * a.dk * a.dv
                       : last && a.final ? a.final + state_at : nullptr;
     if (to && row < a.dk) {
+      const float nan = __int_as_float(0x7fffffff);
+      to += (int64_t)row * a.dv + sc0;
+      if (sc0 + 16 <= a.dv && a.dv % 4 == 0 && reinterpret_cast<uintptr_t>(to) % 16 == 0) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (sc0 + j < a.dv) {
-          const float2 y = halves(s[j / 2]);
-          to[(int64_t)row * a.dv + sc0 + j] = !tries ? __int_as_float(0x7fffffff) : j % 2 ? y.y : y.x;
+        for (int j = 0; j < 8; j += 2) {
+          const float2 x = halves(s[j]), y = halves(s[j + 1]);
+          reinterpret_cast<float4*>(to)[j / 2] =
+              tries ? make_float4(x.x, x.y, y.x, y.y) : make_float4(nan, nan, nan, nan);
         }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (sc0 + j < a.dv) {
+            const float2 y = halves(s[j / 2]);
+            to[j] = !tries ? nan : j % 2 ? y.y : y.x;
+          }
+      }
     }
+    if (!STATE && steps > 0) finish(steps - 1);
+    if (!STATE && lane == 0) tc::stores_done();
+    __syncwarp();
     if (!STATE) {
       // tokens behind the row's end
       const int end = min(a.len, (seg + 1) * a.seg_chunks * C);
