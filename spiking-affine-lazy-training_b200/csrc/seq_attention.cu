@@ -145,16 +145,17 @@ __global__ void __launch_bounds__(256) planes_kernel(const AllToPlanes all, int 
 // products go from the smallest to the largest: in the other order float32's outputs were off by 2.5e-6
 // instead of 3.5e-7.
 //
-// What bounds it: the threads' work on operands.  8 rows of 2048 x 16 heads of 128 in bfloat16 take 133
-// us, 2.1 TB/s, 3.2 times their bytes' time: 256 blocks are two rounds of 16 chunks of some 7000 cycles,
+// What bounds it: the threads' work on operands.  8 rows of 2048 x 16 heads of 128 in bfloat16 take 122
+// us, 2.3 TB/s, 2.9 times their bytes' time: 256 blocks are two rounds of 16 chunks of some 7000 cycles,
 // of which the tensor cores work 2900 (an instruction of 128 x 64 x 16 takes 48 cycles, 30 with an
 // operand in tensor memory), the warps wait 1200 at barriers, and an instruction issues in every other
-// cycle.  One row of 32768 takes 334 us: 9 segments, 105 of it the states' pass.  float16 heads of 128
+// cycle.  One row of 32768 takes 324 us: 9 segments, 105 of it the states' pass.  float16 heads of 128
 // and float32 have chunks of 64 tokens, since shared memory holds no more of their parts: the long row
-// in float16 takes 850 us.
+// in float16 takes 840 us.
 // Measured and left: eight warps (269 us), all products' warps in step with the others (189 us; this
-// is 133), roles for the warps, eight for triangle and out, four for the state and four for the values
-// (180 us: four warps wait too long for their own instructions).
+// was 133), roles for the warps, eight for triangle and out, four for the state and four for the values
+// (180 us: four warps wait too long for their own instructions), the direction as a template
+// parameter (heads of 100 x 77: 117 us to 111; heads of 128: backward 360 us to 364).
 template <int P, typename O, int PANELS, bool STATE>
 __global__ void __launch_bounds__(kThreads, 1)
 attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,

@@ -343,3 +343,21 @@ def test_step_of_many_rows():
     y, m, s, sm = A.attention(*(c.host[x] for x in "qkv"), c.log_decay, c.scale, init=c.init)
     R.assert_close(R.values(out), y[:, 0], m[:, 0], 84, "bfloat16", "out")
     R.assert_close(R.values(state), s, sm, 12, "float32", "state")
+
+
+@pytest.mark.parametrize("dk, dv", ((64, 64), (75, 52), (128, 100)))
+@pytest.mark.parametrize("n", (1, 100, 700))
+def test_a_state_at_any_address(n, dk, dv):
+    """States whose memory starts a float behind a multiple of 16 bytes: the same bits, and nothing
+    beside them is written."""
+    c = Case("bfloat16", 2, n, 2, 1, dk, dv, 4, init=True)
+    out, final = c.forward()
+    size = c.init.size
+    around = R.to_device(np.concatenate([[7.0], c.init.ravel(), [7.0]]))
+    state = D.DeviceArray(around.ptr + 4, c.init.shape, np.float32, around)
+    moved = S.linear_attention(c.dev["q"], c.dev["k"], c.dev["v"], c.decay, scale=c.scale,
+                               initial_state=state, final_state=state)
+    np.testing.assert_array_equal(R.values(moved.out), out.values())
+    got = R.values(around)
+    np.testing.assert_array_equal(got[1:-1], R.values(final).ravel())
+    assert got[0] == 7.0 and got[size + 1] == 7.0
