@@ -242,6 +242,17 @@ __device__ __forceinline__ void products_done(uint64_t* barrier) {
                    shared_at(barrier))
                : "memory");
 }
+// Kernels of one call that follow one another on a stream (`follow` below): the next may set itself up
+// once every block of this one runs, and every thread waits for the whole kernel in front, and all that
+// it wrote, before it touches memory that kernels of the call write or have written.  (Every kernel of
+// the call waits, so the one in front ends after all those before it.)
+__device__ __forceinline__ void let_next_begin() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void wait_for_earlier() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 __device__ __forceinline__ bool one_lane() {
   uint32_t is;
   asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}"
@@ -250,6 +261,25 @@ __device__ __forceinline__ bool one_lane() {
 }
 
 // ---------------------------------------------------------------- host
+
+// Launches a kernel that calls `wait_for_earlier`; the call's first one (`follows` false) starts behind
+// all that the stream holds.
+template <typename... Params, typename... Args>
+cudaError_t follow(bool follows, void (*kernel)(Params...), dim3 grid, int threads, size_t shared,
+                   cudaStream_t st, const Args&... args) {
+  cudaLaunchConfig_t c = {};
+  c.gridDim = grid;
+  c.blockDim = dim3(threads);
+  c.dynamicSmemBytes = shared;
+  c.stream = st;
+  cudaLaunchAttribute overlap = {};
+  overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  overlap.val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = &overlap;
+  c.numAttrs = follows ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&c, kernel, static_cast<Params>(args)...);
+  return e == cudaSuccess ? e : cudaGetLastError();
+}
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
