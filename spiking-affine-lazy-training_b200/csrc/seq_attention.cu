@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(256) planes_kernel(const AllToPlanes all, int 
 // us, 2.3 TB/s, 2.9 times their bytes' time: 256 blocks are two rounds of 16 chunks of some 7000 cycles,
 // of which the tensor cores work 2900 (an instruction of 128 x 64 x 16 takes 48 cycles, 30 with an
 // operand in tensor memory), the warps wait 1200 at barriers, and an instruction issues in every other
-// cycle.  One row of 32768 takes 324 us: 9 segments, 105 of it the states' pass.  float16 heads of 128
+// cycle.  One row of 32768 takes 320 us: 9 segments, 105 of it the states' pass.  float16 heads of 128
 // and float32 have chunks of 64 tokens, since shared memory holds no more of their parts: the long row
 // in float16 takes 840 us.
 // A call's kernels set themselves up while the one in front ends (tc::follow): a backward pass of 14
