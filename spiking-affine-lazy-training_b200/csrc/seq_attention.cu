@@ -38,57 +38,55 @@ __device__ __forceinline__ float decay_of(const float* g, int h) {
 constexpr int kTile = 64;      // columns of v that a block takes
 constexpr int kWorkers = 512;  // 16 warps: four for each 32 rows of tensor memory
 constexpr int kThreads = kWorkers + 32;  // and one for the copies and the products
-constexpr int kWeighted = 3;   // parts of a weighted v
+constexpr int kParts = 3;      // of what is computed in 32 bits: a weighted v, a state, a weight in a chunk
 
 // A type's values in parts of bfloat16, 8 bits each: what the tensor cores multiply.
 template <typename T>
 constexpr int parts_of() { return sizeof(T) == 4 ? 3 : std::is_same<T, __half>::value ? 2 : 1; }
-// Tokens of a chunk, and parts of the states and of the weights within a chunk.
-// (64 where 128 do not fit into shared memory)
+// Tokens of a chunk: 64 where 128 do not fit into shared memory.
 constexpr int chunk_of(int parts, int panels) {
   return parts == 1 || (parts == 2 && panels == 1) ? 128 : 64;
 }
-constexpr int state_parts(int parts) { return parts == 3 ? 3 : 2; }
 
 // Shared memory, all operands in rows of 128 bytes (tc::operand): q and k in panels of 64 columns,
-// part after part; k and v twice, for copies a chunk further ahead, where there is room.
+// part after part; k and v twice, for copies a chunk further ahead, where there is room.  A chunk's
+// outputs leave through memory of their own, or, where that does not fit (bfloat16 heads over 64), through
+// the chunk's values, which no product reads any more.
 template <int P, int PANELS, typename O>
 struct Layout {
   static constexpr int C = chunk_of(P, PANELS), B = P == 3 || (P == 2 && C == 128) ? 1 : 2;
   static constexpr int kPanel = C * 128, kKeys = P * PANELS * kPanel, kValues = P * kPanel;
   static constexpr int kState = PANELS * 64 * 128;  // a part of the state
   // a warp's 32 rows of out, 32 bytes each at a time
-  static constexpr int kStaged = 1024, kOutColumns = 32 / sizeof(O);
+  static constexpr int kStaged = 1024, kOutColumns = 32 / sizeof(O), kOut = kWorkers / 32 * kStaged;
+  static constexpr bool out_in_values = P == 1 && PANELS == 2;
+  static_assert(!out_in_values || (B == 2 && kValues == kOut), "outputs through the values' place");
   static constexpr int q = 0, k = q + kKeys, v = k + B * kKeys, weighted = v + B * kValues,
-                       state = weighted + kWeighted * kPanel, out = state + state_parts(P) * kState,
-                       bytes = out + kWorkers / 32 * kStaged + 1024;
+                       state = weighted + kParts * kPanel, out = state + kParts * kState,
+                       bytes = out + (out_in_values ? 0 : kOut) + 1024;
   // the pass that wants the states alone has weighted values of two chunks instead
-  static constexpr int state_bytes = weighted + 2 * kWeighted * kPanel + 1024;
+  static constexpr int state_bytes = weighted + 2 * kParts * kPanel + 1024;
+  static_assert(bytes <= 225 * 1024 && state_bytes <= 225 * 1024, "2 KB are the kernel's own");
 };
 
-// Two values in parts of bfloat16: the upper 8 bits of what is left, time and again; the last of two
-// parts is rounded to the nearest (2^-16 of the value in all), three hold all 24 bits.
+// The next part of two values, their upper 8 bits each, taken out of them.  (The sign goes over with the
+// upper bits.)
+__device__ __forceinline__ uint32_t next_part(f32x2& v) {
+  const float2 x = halves(v);
+  v = add2(v, pair(__uint_as_float((__float_as_uint(x.x) & 0xffff0000u) ^ 0x80000000u),
+                   __uint_as_float((__float_as_uint(x.y) & 0xffff0000u) ^ 0x80000000u)));
+  return __byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x7632);
+}
+// Two values in parts of bfloat16: one holds bfloat16's 8 bits, two float16's 11, three all 24.
 template <int N>
 __device__ __forceinline__ void split2(uint32_t (&to)[N], f32x2 v) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float2 x = halves(v);
-    if (i == N - 1 && N < 3) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(x.x, x.y);
-      to[i] = *reinterpret_cast<const uint32_t*>(&h);
-    } else {
-      to[i] = __byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x7632);
-      if (i < N - 1)  // the sign goes over with the upper bits
-        v = add2(v, pair(__uint_as_float((__float_as_uint(x.x) & 0xffff0000u) ^ 0x80000000u),
-                         __uint_as_float((__float_as_uint(x.y) & 0xffff0000u) ^ 0x80000000u)));
-    }
-  }
+  for (int i = 0; i < N; ++i) to[i] = next_part(v);
 }
 template <int N>
 __device__ __forceinline__ void split2(uint32_t (&to)[N], float x, float y) {
   split2<N>(to, pair(x, y));
 }
-
 // Arrays (batch, len, heads, dim) of T in planes of bfloat16 parts (part, batch, len, heads, dim rounded
 // up to 8), zero past the rows' ends: what tensor copies can take of every type, alignment and size.
 // blockIdx.y is the array.  Bound by memory.
@@ -140,20 +138,20 @@ __global__ void __launch_bounds__(256) planes_kernel(const AllToPlanes all, int 
 //   [q k^T] -> triangle -> [its product with v] -> out, a chunk behind
 //
 // What is rounded: every operand is bfloat16, in parts of 8 bits.  Inputs are exact (bfloat16 in one
-// part, float16 in two, float32 in three); weighted values have three parts, so that states are good to
-// 2^-24; states and the triangle's values, as operands for out, have three
-// parts for float32 and two (2^-16) for outputs of 16 bits.  Sums and states are float32; the state
-// is carried in registers.  The tensor cores cut their sums off after every instruction, so the parts'
+// part, float16 in two, float32 in three); what is computed in 32 bits, the weighted values, states and
+// the triangle, has three parts, which hold its 24 bits, whatever the outputs' type (two for outputs of
+// 16 bits took 125 us instead of 141 below, and lost what is left where an output's terms cancel).  Sums
+// and states are float32; the state is carried in registers.  The tensor cores cut their sums off after
+// every instruction, so the parts'
 // products go from the smallest to the largest: in the other order float32's outputs were off by 2.5e-6
 // instead of 3.5e-7.
 //
-// What bounds it: the threads' work on operands.  8 rows of 2048 x 16 heads of 128 in bfloat16 take 122
-// us, 2.3 TB/s, 2.9 times their bytes' time: 256 blocks are two rounds of 16 chunks of some 7000 cycles,
-// of which the tensor cores work 2900 (an instruction of 128 x 64 x 16 takes 48 cycles, 30 with an
-// operand in tensor memory), the warps wait 1200 at barriers, and an instruction issues in every other
-// cycle.  One row of 32768 takes 320 us: 9 segments, 105 of it the states' pass.  float16 heads of 128
-// and float32 have chunks of 64 tokens, since shared memory holds no more of their parts: the long row
-// in float16 takes 840 us.
+// What bounds it: the threads' work on operands.  8 rows of 2048 x 16 heads of 128 in bfloat16 take 141
+// us, 2.0 TB/s, 3.3 times their bytes' time: 256 blocks are two rounds of 16 chunks of some 8000 cycles,
+// of which the tensor cores work 3500 (an instruction of 128 x 64 x 16 takes 48 cycles, 30 with an
+// operand in tensor memory).  One row of 32768 takes 347 us: 9 segments, 105 of it the states' pass.
+// float16 heads of 128 and float32 have chunks of 64 tokens, since shared memory holds no more of their
+// parts: the long row in float16 takes 896 us, in float32 1290 us.
 // A call's kernels set themselves up while the one in front ends (tc::follow): a backward pass of 14
 // small launches (3 x 1021 x 12 heads of 64 x 100, 4 key heads, float16) went from 181 us to 161.
 // Measured and left: eight warps (269 us), all products' warps in step with the others (189 us; this
@@ -166,7 +164,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                  const __grid_constant__ CUtensorMap map_v,
                  const __grid_constant__ CUtensorMap map_out, const Pass a) {
   using L = Layout<P, PANELS, O>;
-  constexpr int C = L::C, B = L::B, SP = state_parts(P), DK = PANELS * 64;
+  constexpr int C = L::C, B = L::B, DK = PANELS * 64;
   constexpr int VB = STATE ? B + PANELS : B;  // places for values, also where q is not needed
   constexpr int kPanel = L::kPanel;
   extern __shared__ uint8_t raw[];
@@ -177,6 +175,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   // takes two barriers in turn.)
   constexpr int R = STATE ? 2 : 1;
   __shared__ uint64_t done_scores, done_q, done_state[R], done_out, ready_chunk[R], ready_triangle;
+  __shared__ uint64_t out_gone;  // out_in_values: the outputs of the chunk in front left the values' place
   __shared__ uint32_t tmem_at;
   __shared__ float powers[32 + C + 1];        // l^i from place 32 on
   __shared__ __align__(16) float column[32];  // of a column within its 32
@@ -211,6 +210,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       tc::barrier_init(&ready_chunk[i], kWorkers / 32);
     }
     tc::barrier_init(&ready_triangle, kWorkers / 32);
+    tc::barrier_init(&out_gone, kWorkers / 32);
     tc::barrier_init_fence();
   }
   if (warp == 0) tc::tmem_alloc(&tmem_at, 512);
@@ -231,10 +231,16 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   // columns of tensor memory
   constexpr int kScores = 0, kTriangle = 128, kFromState = 256, kOut = 384, kAdded = 448;
   const auto added = [&](int i) { return STATE ? (i & 1) * kTile : kAdded; };
+  // Parts of chunk i's triangle.  With 128 tokens the third lies where the outputs from the state of the
+  // chunk in front were: each warp has read its columns of them before it writes the same ones.
+  constexpr bool kAway = C == 128;
+  const auto triangle = [&](int i, int x) {
+    return kAway && x == 2 ? kFromState + (~i & 1) * kTile : kTriangle + x * (C / 2);
+  };
   const auto value_place = [&](int i) {
     return i % VB < B ? L::v + i % VB * L::kValues : L::q + (i % VB - B) * L::kValues;
   };
-  const auto values = [&](int i) { return STATE ? (i & 1) * kWeighted * kPanel : 0; };
+  const auto values = [&](int i) { return STATE ? (i & 1) * kParts * kPanel : 0; };
   uint32_t tries = tc::kTries;
 
   if (warp == kWorkers / 32) {
@@ -300,7 +306,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 #pragma unroll
             for (int x = 0; x < P; ++x) {
               const int y = o - x;
-              if (y < 0 || y >= SP) continue;
+              if (y < 0 || y >= kParts) continue;
               for (int d = 0; d < depth; ++d) {
                 const uint32_t off = (d >> 2) * kPanel + (d & 3) * 32;
                 tc::product_16(tmem + kFromState + (i & 1) * kTile,
@@ -320,7 +326,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 #pragma unroll
             for (int x = 0; x < P; ++x) {
               const int y = o - x;
-              if (y < 0 || y >= kWeighted) continue;
+              if (y < 0 || y >= kParts) continue;
 #pragma unroll
               for (int d = 0; d < C / 16; ++d) {
                 tc::product_16(tmem + added(i), tc::further(k, x * PANELS * kPanel + d * 2048),
@@ -334,6 +340,10 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         if (!STATE) {
           tc::barrier_wait(&done_q, i & 1, tries);
           fetch_q(i + 1);
+          if (L::out_in_values && i > 0) {
+            tc::barrier_wait(&out_gone, (i - 1) & 1, tries);
+            fetch_v(i + 1);
+          }
           tc::barrier_wait(&ready_triangle, i & 1, tries);
           tc::fence_after();
           const uint64_t v = tc::operand(sm + L::v + i % B * L::kValues, 1024);
@@ -341,12 +351,12 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 #pragma unroll
           for (int o = 2; o >= 0; --o)
 #pragma unroll
-            for (int x = 0; x < SP; ++x) {
+            for (int x = 0; x < kParts; ++x) {
               const int y = o - x;
               if (y < 0 || y >= P) continue;
 #pragma unroll
               for (int d = 0; d < C / 16; ++d) {
-                tc::product_16_from_tmem(tmem + kOut, tmem + kTriangle + x * (C / 2) + d * 8,
+                tc::product_16_from_tmem(tmem + kOut, tmem + triangle(i, x) + d * 8,
                                          tc::further(v, y * kPanel + d * 2048),
                                          tc::shape(128, kTile, 1, false, true), add);
                 add = true;
@@ -366,7 +376,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         fetch_k(i + B);
         if (!STATE) {
           tc::barrier_wait(&done_out, i & 1, tries);
-          fetch_v(i + B);
+          if (!L::out_in_values) fetch_v(i + B);
         }
         if (B == 1) next();
       }
@@ -394,11 +404,11 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       if (row >= DK) return;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        uint32_t x[4][SP];
+        uint32_t x[4][kParts];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) split2<SP>(x[k], s[4 * u + k]);
+        for (int k = 0; k < 4; ++k) split2<kParts>(x[k], s[4 * u + k]);
 #pragma unroll
-        for (int j = 0; j < SP; ++j)
+        for (int j = 0; j < kParts; ++j)
           *reinterpret_cast<uint4*>(sm + L::state + j * L::kState + row * 128 +
                                     (((part * 2 + u) ^ (row & 7)) << 4)) =
               make_uint4(x[0][j], x[1][j], x[2][j], x[3][j]);
@@ -474,7 +484,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         const int r = r0 + x * kApart;
         // (rows past the end are zero, whatever their weight; power has 32 places in front)
         const float w = power[a.reverse ? r + 1 : max(count - 1 - r, 0)];
-        uint32_t out[4][kWeighted];
+        uint32_t out[4][kParts];
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
           f32x2 y = 0;
@@ -484,11 +494,11 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                                    __uint_as_float(in[x][j][m] & 0xffff0000u));
             y = j == 0 ? one : add2(y, one);
           }
-          split2<kWeighted>(out[m], mul2(y, both(w)));
+          split2<kParts>(out[m], mul2(y, both(w)));
         }
         uint8_t* to = sm + L::weighted + values(i) + (place - v) + x * kApart * 128;
 #pragma unroll
-        for (int j = 0; j < kWeighted; ++j)
+        for (int j = 0; j < kParts; ++j)
           *reinterpret_cast<uint4*>(to + j * kPanel) =
               make_uint4(out[0][j], out[1][j], out[2][j], out[3][j]);
       }
@@ -527,7 +537,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       // 32 bytes a row, through shared memory: as stores from here every 16 bytes would be a line of
       // their own
       constexpr int W = L::kOutColumns;
-      O* to = reinterpret_cast<O*>(sm + L::out + warp * L::kStaged);
+      O* to = reinterpret_cast<O*>(sm + (L::out_in_values ? value_place(i) : L::out) +
+                                   warp * L::kStaged);
 #pragma unroll
       for (int y = 0; y < 16; y += W) {
         if (a.copies_out && lane == 0) tc::stores_read();
@@ -552,6 +563,18 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       }
     };
 
+    // The chunk in front's outputs are on their way out of the values' place.
+    const auto leave_values = [&] {
+      if (!L::out_in_values) return;
+      if (a.copies_out) {
+        if (lane == 0) tc::stores_read();
+      } else {
+        tc::fence_shared();
+      }
+      __syncwarp();
+      tc::barrier_arrive_if_zero(&out_gone, lane);
+    };
+
     if (STATE && steps > 0) begin(0);
 #pragma unroll 1
     for (int i = 0; i < steps; ++i) {
@@ -565,9 +588,9 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         // the triangle's weights
         tc::barrier_wait_warp(&done_scores, i & 1, tries);
         tc::fence_after();
-        // blocks on the other side hold the zeros that the first chunk left there
+        // blocks on the other side hold the zeros that the first chunk left there (but a part away)
         const bool beside = a.reverse ? part < quarter : part > quarter;
-        if (part < C / 32 && quarter < C / 32 && !(beside && i > 0)) {
+        if (part < C / 32 && quarter < C / 32) {
           const bool none = beside || (a.reverse && part * 32 >= count);
           const bool diagonal = part == quarter;
           // against time, columns past the end lie on the triangle's side
@@ -575,53 +598,56 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           const float f = none || diagonal || cut
                               ? 0.f
                               : power[a.reverse ? part * 32 - row : row - part * 32 - 31];
-#pragma unroll
+          // (as a loop: unrolled, 8 x 2048 x 16 heads of 128 took 145 us instead of 141)
+#pragma unroll 1
           for (int y = 0; y < 32; y += 16) {
-            uint32_t r[16], x[8][SP];
-            tc::tmem_load<16>(r, mine + kScores + part * 32 + y);
-            tc::loads_done();
+            f32x2 x[8];
             if (none) {
 #pragma unroll
-              for (int j = 0; j < 8; ++j)
-#pragma unroll
-                for (int k = 0; k < SP; ++k) x[j][k] = 0;
-            } else if (cut) {
-#pragma unroll
-              for (int j = 0; j < 16; j += 2) {
-                const int at = part * 32 + y + j, d = at - row;
-                const float w0 = power[max(d, 0)], w1 = power[max(d + 1, 0)];
-                split2<SP>(x[j / 2], d >= 0 && at < count ? __uint_as_float(r[j]) * w0 : 0.f,
-                           d >= -1 && at + 1 < count ? __uint_as_float(r[j + 1]) * w1 : 0.f);
-              }
-            } else if (diagonal) {
-              // (weights of the other side are loaded and left: a branch a value would cost more)
-              const float* w = a.reverse ? power - lane + y : power + lane - y;
-#pragma unroll
-              for (int j = 0; j < 16; j += 2) {
-                const int c0 = y + j, c1 = c0 + 1;
-                const float p0 = __uint_as_float(r[j]) * w[a.reverse ? j : -j],
-                            p1 = __uint_as_float(r[j + 1]) * w[a.reverse ? j + 1 : -j - 1];
-                split2<SP>(x[j / 2], (a.reverse ? c0 >= lane : c0 <= lane) ? p0 : 0.f,
-                           (a.reverse ? c1 >= lane : c1 <= lane) ? p1 : 0.f);
-              }
+              for (int j = 0; j < 8; ++j) x[j] = 0;
             } else {
+              uint32_t r[16];
+              tc::tmem_load<16>(r, mine + kScores + part * 32 + y);
+              tc::loads_done();
+              if (cut) {
 #pragma unroll
-              for (int j = 0; j < 16; j += 4) {
-                const float4 w = *reinterpret_cast<const float4*>(column + y + j);
-                split2<SP>(x[j / 2], mul2(pair(__uint_as_float(r[j]), __uint_as_float(r[j + 1])),
-                                          mul2(pair(w.x, w.y), both(f))));
-                split2<SP>(x[j / 2 + 1],
-                           mul2(pair(__uint_as_float(r[j + 2]), __uint_as_float(r[j + 3])),
-                                mul2(pair(w.z, w.w), both(f))));
+                for (int j = 0; j < 16; j += 2) {
+                  const int at = part * 32 + y + j, d = at - row;
+                  const float w0 = power[max(d, 0)], w1 = power[max(d + 1, 0)];
+                  x[j / 2] = pair(d >= 0 && at < count ? __uint_as_float(r[j]) * w0 : 0.f,
+                                  d >= -1 && at + 1 < count ? __uint_as_float(r[j + 1]) * w1 : 0.f);
+                }
+              } else if (diagonal) {
+                // (weights of the other side are loaded and left: a branch a value would cost more)
+                const float* w = a.reverse ? power - lane + y : power + lane - y;
+#pragma unroll
+                for (int j = 0; j < 16; j += 2) {
+                  const int c0 = y + j, c1 = c0 + 1;
+                  const float p0 = __uint_as_float(r[j]) * w[a.reverse ? j : -j],
+                              p1 = __uint_as_float(r[j + 1]) * w[a.reverse ? j + 1 : -j - 1];
+                  x[j / 2] = pair((a.reverse ? c0 >= lane : c0 <= lane) ? p0 : 0.f,
+                                  (a.reverse ? c1 >= lane : c1 <= lane) ? p1 : 0.f);
+                }
+              } else {
+#pragma unroll
+                for (int j = 0; j < 16; j += 4) {
+                  const float4 w = *reinterpret_cast<const float4*>(column + y + j);
+                  x[j / 2] = mul2(pair(__uint_as_float(r[j]), __uint_as_float(r[j + 1])),
+                                  mul2(pair(w.x, w.y), both(f)));
+                  x[j / 2 + 1] = mul2(pair(__uint_as_float(r[j + 2]), __uint_as_float(r[j + 3])),
+                                      mul2(pair(w.z, w.w), both(f)));
+                }
               }
             }
 #pragma unroll
-            for (int k = 0; k < SP; ++k) {
+            for (int k = 0; k < kParts; ++k) {
+              if (beside && i > 0 && !(kAway && k == 2)) continue;
               uint32_t o[8];
 #pragma unroll
-              for (int j = 0; j < 8; ++j) o[j] = x[j][k];
-              tc::tmem_store(mine + kTriangle + k * (C / 2) + part * 16 + y / 2, o);
+              for (int j = 0; j < 8; ++j) o[j] = next_part(x[j]);
+              tc::tmem_store(mine + triangle(i, k) + part * 16 + y / 2, o);
             }
+            if (y == 0 && i > 0) leave_values();
           }
           tc::stores_to_tmem_done();
         }
