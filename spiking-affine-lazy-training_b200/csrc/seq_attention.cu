@@ -176,7 +176,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   constexpr int R = STATE ? 2 : 1;
   __shared__ uint64_t done_scores, done_q, done_state[R], done_out, ready_chunk[R], ready_triangle;
   __shared__ uint64_t out_gone;  // out_in_values: the outputs of the chunk in front left the values' place
-  __shared__ uint32_t tmem_at;
+  __shared__ uint64_t drained;  // every product issued
+  __shared__ uint32_t tmem_at, gave_up;
   __shared__ float powers[32 + C + 1];        // l^i from place 32 on
   __shared__ __align__(16) float column[32];  // of a column within its 32
   __shared__ int bad[3][kTile];               // the outermost token whose v is not finite
@@ -204,13 +205,15 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   if (threadIdx.x == 0) {
     for (int i = 0; i < B; ++i) tc::barrier_init(&loaded_k[i], 1);
     for (int i = 0; i < VB; ++i) tc::barrier_init(&loaded_v[i], 1);
-    for (uint64_t* x : {&loaded_q, &done_q, &done_scores, &done_out}) tc::barrier_init(x, 1);
+    for (uint64_t* x : {&loaded_q, &done_q, &done_scores, &done_out, &drained})
+      tc::barrier_init(x, 1);
     for (int i = 0; i < R; ++i) {
       tc::barrier_init(&done_state[i], 1);
       tc::barrier_init(&ready_chunk[i], kWorkers / 32);
     }
     tc::barrier_init(&ready_triangle, kWorkers / 32);
     tc::barrier_init(&out_gone, kWorkers / 32);
+    gave_up = 0;
     tc::barrier_init_fence();
   }
   if (warp == 0) tc::tmem_alloc(&tmem_at, 512);
@@ -252,16 +255,22 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           tc::load_box4(sm + to + x * kPanel, map, col + x % panels * 64, head, chunk(i) * C,
                         x / panels * a.batch + b, barrier);
       };
+      int asked_q = 0, asked_k = 0, asked_v = 0;  // chunks so far
       const auto fetch_q = [&](int i) {
-        if (i < steps) fetch(L::q, &map_q, PANELS, 0, h / a.q_share, i, &loaded_q);
+        if (i < steps) fetch(L::q, &map_q, PANELS, 0, h / a.q_share, i, &loaded_q), ++asked_q;
       };
       const auto fetch_k = [&](int i) {
         if (i < steps)
-          fetch(L::k + i % B * L::kKeys, &map_k, PANELS, 0, h / a.k_share, i, &loaded_k[i % B]);
+          fetch(L::k + i % B * L::kKeys, &map_k, PANELS, 0, h / a.k_share, i, &loaded_k[i % B]),
+              ++asked_k;
       };
       const auto fetch_v = [&](int i) {
         if (i < steps)
-          fetch(value_place(i), &map_v, 1, col0, h / a.v_share, i, &loaded_v[i % VB]);
+          fetch(value_place(i), &map_v, 1, col0, h / a.v_share, i, &loaded_v[i % VB]), ++asked_v;
+      };
+      const auto wait = [&](uint64_t* barrier, uint32_t parity) {
+        tc::barrier_wait(barrier, parity, tries, &gave_up);
+        return tries > 0;
       };
       const int depth = (a.dk + 15) / 16;
       const uint64_t q = tc::operand(sm + L::q, 1024), state = tc::operand(sm + L::state, 1024),
@@ -284,101 +293,116 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           }
         tc::products_done(&done_scores);
       };
-      for (int i = 0; i < VB; ++i) {
-        fetch_v(i);
-        if (i < B) fetch_k(i);
-        if (!STATE && i == 0) fetch_q(0);
-      }
-      tc::barrier_wait(&loaded_k[0], 0, tries);
-      if (!STATE) {
-        tc::barrier_wait(&loaded_q, 0, tries);
-        scores(0);
-      }
+      const auto work = [&] {  // until a wait is given up
+        for (int i = 0; i < VB; ++i) {
+          fetch_v(i);
+          if (i < B) fetch_k(i);
+          if (!STATE && i == 0) fetch_q(0);
+        }
+        if (!wait(&loaded_k[0], 0)) return;
+        if (!STATE) {
+          if (!wait(&loaded_q, 0)) return;
+          scores(0);
+        }
 #pragma unroll 1
-      for (int i = 0; i < steps; ++i) {
-        tc::barrier_wait(&ready_chunk[i % R], i / R & 1, tries);
-        tc::fence_after();
-        if (STATE) fetch_v(i + VB);
-        if (!STATE) {
-          bool add = false;
-#pragma unroll
-          for (int o = 2; o >= 0; --o)
-#pragma unroll
-            for (int x = 0; x < P; ++x) {
-              const int y = o - x;
-              if (y < 0 || y >= kParts) continue;
-              for (int d = 0; d < depth; ++d) {
-                const uint32_t off = (d >> 2) * kPanel + (d & 3) * 32;
-                tc::product_16(tmem + kFromState + (i & 1) * kTile,
-                               tc::further(q, x * PANELS * kPanel + off),
-                               tc::further(state, y * L::kState + d * 2048),
-                               tc::shape(128, kTile, 1, false, true), add);
-                add = true;
-              }
-            }
-          tc::products_done(&done_q);
-        }
-        {
-          const uint64_t k = tc::operand(sm + L::k + i % B * L::kKeys, 1024, kPanel);
-          bool add = false;
-#pragma unroll
-          for (int o = 2; o >= 0; --o)
-#pragma unroll
-            for (int x = 0; x < P; ++x) {
-              const int y = o - x;
-              if (y < 0 || y >= kParts) continue;
-#pragma unroll
-              for (int d = 0; d < C / 16; ++d) {
-                tc::product_16(tmem + added(i), tc::further(k, x * PANELS * kPanel + d * 2048),
-                               tc::further(weighted, values(i) + y * kPanel + d * 2048),
-                               tc::shape(128, kTile, 1, true, true), add);
-                add = true;
-              }
-            }
-          tc::products_done(&done_state[i % R]);
-        }
-        if (!STATE) {
-          tc::barrier_wait(&done_q, i & 1, tries);
-          fetch_q(i + 1);
-          if (L::out_in_values && i > 0) {
-            tc::barrier_wait(&out_gone, (i - 1) & 1, tries);
-            fetch_v(i + 1);
-          }
-          tc::barrier_wait(&ready_triangle, i & 1, tries);
+        for (int i = 0; i < steps; ++i) {
+          if (!wait(&ready_chunk[i % R], i / R & 1)) return;
           tc::fence_after();
-          const uint64_t v = tc::operand(sm + L::v + i % B * L::kValues, 1024);
-          bool add = false;
+          if (STATE) fetch_v(i + VB);
+          if (!STATE) {
+            bool add = false;
 #pragma unroll
-          for (int o = 2; o >= 0; --o)
+            for (int o = 2; o >= 0; --o)
 #pragma unroll
-            for (int x = 0; x < kParts; ++x) {
-              const int y = o - x;
-              if (y < 0 || y >= P) continue;
-#pragma unroll
-              for (int d = 0; d < C / 16; ++d) {
-                tc::product_16_from_tmem(tmem + kOut, tmem + triangle(i, x) + d * 8,
-                                         tc::further(v, y * kPanel + d * 2048),
-                                         tc::shape(128, kTile, 1, false, true), add);
-                add = true;
+              for (int x = 0; x < P; ++x) {
+                const int y = o - x;
+                if (y < 0 || y >= kParts) continue;
+                for (int d = 0; d < depth; ++d) {
+                  const uint32_t off = (d >> 2) * kPanel + (d & 3) * 32;
+                  tc::product_16(tmem + kFromState + (i & 1) * kTile,
+                                 tc::further(q, x * PANELS * kPanel + off),
+                                 tc::further(state, y * L::kState + d * 2048),
+                                 tc::shape(128, kTile, 1, false, true), add);
+                  add = true;
+                }
               }
+            tc::products_done(&done_q);
+          }
+          {
+            const uint64_t k = tc::operand(sm + L::k + i % B * L::kKeys, 1024, kPanel);
+            bool add = false;
+#pragma unroll
+            for (int o = 2; o >= 0; --o)
+#pragma unroll
+              for (int x = 0; x < P; ++x) {
+                const int y = o - x;
+                if (y < 0 || y >= kParts) continue;
+#pragma unroll
+                for (int d = 0; d < C / 16; ++d) {
+                  tc::product_16(tmem + added(i), tc::further(k, x * PANELS * kPanel + d * 2048),
+                                 tc::further(weighted, values(i) + y * kPanel + d * 2048),
+                                 tc::shape(128, kTile, 1, true, true), add);
+                  add = true;
+                }
+              }
+            tc::products_done(&done_state[i % R]);
+          }
+          if (!STATE) {
+            if (!wait(&done_q, i & 1)) return;
+            fetch_q(i + 1);
+            if (L::out_in_values && i > 0) {
+              if (!wait(&out_gone, (i - 1) & 1)) return;
+              fetch_v(i + 1);
             }
-          tc::products_done(&done_out);
+            if (!wait(&ready_triangle, i & 1)) return;
+            tc::fence_after();
+            const uint64_t v = tc::operand(sm + L::v + i % B * L::kValues, 1024);
+            bool add = false;
+#pragma unroll
+            for (int o = 2; o >= 0; --o)
+#pragma unroll
+              for (int x = 0; x < kParts; ++x) {
+                const int y = o - x;
+                if (y < 0 || y >= P) continue;
+#pragma unroll
+                for (int d = 0; d < C / 16; ++d) {
+                  tc::product_16_from_tmem(tmem + kOut, tmem + triangle(i, x) + d * 8,
+                                           tc::further(v, y * kPanel + d * 2048),
+                                           tc::shape(128, kTile, 1, false, true), add);
+                  add = true;
+                }
+              }
+            tc::products_done(&done_out);
+          }
+          if (i + 1 == steps) break;
+          const auto next = [&] {
+            if (!wait(&loaded_k[(i + 1) % B], (i + 1) / B & 1)) return false;
+            if (STATE) return true;
+            if (!wait(&loaded_q, (i + 1) & 1)) return false;
+            scores(i + 1);
+            return true;
+          };
+          if (B == 2 && !next()) return;
+          if (!wait(&done_state[i % R], i / R & 1)) return;
+          fetch_k(i + B);
+          if (!STATE) {
+            if (!wait(&done_out, i & 1)) return;
+            if (!L::out_in_values) fetch_v(i + B);
+          }
+          if (B == 1 && !next()) return;
         }
-        if (i + 1 == steps) break;
-        const auto next = [&] {
-          tc::barrier_wait(&loaded_k[(i + 1) % B], (i + 1) / B & 1, tries);
-          if (STATE) return;
-          tc::barrier_wait(&loaded_q, (i + 1) & 1, tries);
-          scores(i + 1);
-        };
-        if (B == 2) next();
-        tc::barrier_wait(&done_state[i % R], i / R & 1, tries);
-        fetch_k(i + B);
-        if (!STATE) {
-          tc::barrier_wait(&done_out, i & 1, tries);
-          if (!L::out_in_values) fetch_v(i + B);
-        }
-        if (B == 1) next();
+      };
+      work();
+      // nothing may be under way when the block ends
+      uint32_t more = tc::kTries;
+      tc::products_done(&drained);
+      tc::barrier_wait(&drained, 0, more, &gave_up);
+      if (tc::marked(&gave_up)) {
+        for (int i = max(0, asked_v - VB); i < asked_v; ++i)
+          tc::barrier_wait(&loaded_v[i % VB], i / VB & 1, more, &gave_up);
+        for (int i = max(0, asked_k - B); i < asked_k; ++i)
+          tc::barrier_wait(&loaded_k[i % B], i / B & 1, more, &gave_up);
+        if (asked_q > 0) tc::barrier_wait(&loaded_q, (asked_q - 1) & 1, more, &gave_up);
       }
     }
     __syncwarp();
@@ -421,9 +445,9 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       const int count = tokens(chunk(i));
       uint8_t* k = sm + L::k + i % B * L::kKeys;
       uint8_t* v = sm + value_place(i);
-      tc::barrier_wait_warp(&loaded_v[i % VB], i / VB & 1, tries);
+      tc::barrier_wait_warp(&loaded_v[i % VB], i / VB & 1, tries, &gave_up);
       if (P == 1 && count < C) {  // (planes hold zeros there)
-        tc::barrier_wait_warp(&loaded_k[i % B], i / B & 1, tries);
+        tc::barrier_wait_warp(&loaded_k[i % B], i / B & 1, tries, &gave_up);
         for (int x = threadIdx.x; x < (C - count) * PANELS * 8; x += kWorkers) {
           const int r = count + x / (PANELS * 8), u = x % (PANELS * 8);
           *reinterpret_cast<uint4*>(k + (u >> 3) * kPanel + r * 128 + ((u & 7) << 4)) =
@@ -510,7 +534,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     // Chunk i's output, once its products are there.
     const auto finish = [&](int i) {
       const int c = chunk(i), count = tokens(c);
-      tc::barrier_wait_warp(&done_out, i & 1, tries);
+      tc::barrier_wait_warp(&done_out, i & 1, tries, &gave_up);
       tc::fence_after();
       uint32_t x[16], y[16];
       tc::tmem_load<16>(x, mine + kFromState + (i & 1) * kTile + part * 16);
@@ -526,11 +550,12 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                         mul2(pair(__uint_as_float(y[j]), __uint_as_float(y[j + 1])), both(a.scale))));
         f[j] = live ? o.x : 0.f, f[j + 1] = live ? o.y : 0.f;
       }
-      if (any_bad[i % 3] || !tries) {
+      const bool lost = tc::marked(&gave_up);  // a result that nobody can take for one
+      if (any_bad[i % 3] || lost) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const int first = bad[i % 3][part * 16 + j];
-          if (live && ((first >= 0 && (a.reverse ? row <= first : row >= C - 1 - first)) || !tries))
+          if (live && ((first >= 0 && (a.reverse ? row <= first : row >= C - 1 - first)) || lost))
             f[j] = __int_as_float(0x7fffffff);
         }
       }
@@ -586,7 +611,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       if (!STATE) {
         if (i > 0) finish(i - 1);
         // the triangle's weights
-        tc::barrier_wait_warp(&done_scores, i & 1, tries);
+        tc::barrier_wait_warp(&done_scores, i & 1, tries, &gave_up);
         tc::fence_after();
         // blocks on the other side hold the zeros that the first chunk left there (but a part away)
         const bool beside = a.reverse ? part < quarter : part > quarter;
@@ -656,7 +681,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         tc::barrier_arrive_if_zero(&ready_triangle, lane);
       }
       // the state behind the chunk
-      tc::barrier_wait_warp(&done_state[i % R], i / R & 1, tries);
+      tc::barrier_wait_warp(&done_state[i % R], i / R & 1, tries, &gave_up);
       tc::fence_after();
       uint32_t x[16];
       tc::tmem_load<16>(x, mine + added(i) + part * 16);
@@ -678,7 +703,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       }
       if (i + 1 < steps) {
         if (!STATE) {
-          tc::barrier_wait_warp(&done_q, i & 1, tries);
+          tc::barrier_wait_warp(&done_q, i & 1, tries, &gave_up);
           store_state();
         }
         // every warp is past the chunk before (STATE: past this one): its marks are free
@@ -694,20 +719,21 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                       : last && a.final ? a.final + state_at : nullptr;
     if (to && row < a.dk) {
       const float nan = __int_as_float(0x7fffffff);
+      const bool lost = tc::marked(&gave_up);
       to += (int64_t)row * a.dv + sc0;
       if (sc0 + 16 <= a.dv && a.dv % 4 == 0 && reinterpret_cast<uintptr_t>(to) % 16 == 0) {
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
           const float2 x = halves(s[j]), y = halves(s[j + 1]);
           reinterpret_cast<float4*>(to)[j / 2] =
-              tries ? make_float4(x.x, x.y, y.x, y.y) : make_float4(nan, nan, nan, nan);
+              lost ? make_float4(nan, nan, nan, nan) : make_float4(x.x, x.y, y.x, y.y);
         }
       } else {
 #pragma unroll
         for (int j = 0; j < 16; ++j)
           if (sc0 + j < a.dv) {
             const float2 y = halves(s[j / 2]);
-            to[j] = !tries ? nan : j % 2 ? y.y : y.x;
+            to[j] = lost ? nan : j % 2 ? y.y : y.x;
           }
       }
     }

@@ -71,7 +71,8 @@ matmul_q8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
   uint8_t* tiles = raw + (1024 - tc::shared_at(raw) % 1024) % 1024;
   uint8_t* staged = tiles + S * stage_bytes(BN);  // SWAP = false: 4 KB a warp for rows of out
   __shared__ uint64_t full[S], empty[S], sum_full[B], sum_empty[B];
-  __shared__ uint32_t tmem_at;
+  __shared__ uint64_t drained;  // every product issued
+  __shared__ uint32_t tmem_at, gave_up;  // (by a warp of sums)
   constexpr int kScalesB = SWAP ? BN : 4;  // of each column, or of each block of columns
   __shared__ __align__(16) float scales_a[kRing][kTileA], scales_b[kRing][kScalesB];
   __shared__ uint64_t scales_full[kRing], scales_empty[kRing];
@@ -89,6 +90,8 @@ matmul_q8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       tc::barrier_init(&scales_full[i], 64);
       tc::barrier_init(&scales_empty[i], kSums / 32);
     }
+    tc::barrier_init(&drained, 1);
+    gave_up = 0;
     tc::barrier_init_fence();
     tc::prefetch_map(&map_a);
     tc::prefetch_map(&map_b);
@@ -134,8 +137,9 @@ matmul_q8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         }
       }
       // all copies have to land before the block may end
+      uint32_t more = tc::kTries;
       for (int i = 0; i < S; ++i) {
-        tc::barrier_wait(&empty[stage], phase ^ 1, tries);
+        tc::barrier_wait(&full[stage], phase ^ 1, more);
         if (++stage == S) stage = 0, phase ^= 1;
       }
     }
@@ -161,6 +165,9 @@ matmul_q8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
           if (++buffer == B) buffer = 0, sum_phase ^= 1;
         }
       }
+      uint32_t more = tc::kTries;  // and all products
+      tc::products_done(&drained);
+      tc::barrier_wait(&drained, 0, more);
     }
   } else if (warp >= kScales) {
     // a warp for the lanes' scales and one for the columns': a row's scales lie together, so that
@@ -200,14 +207,17 @@ matmul_q8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16) + half * H;
     int buffer = 0, slot = 0;
     uint32_t phase = 0, slot_phase = 0;
+    // A wait that is given up leaves NaN in this and all further tiles, and no arrival any more, so that
+    // nothing overwrites what others still read.  (A mark within the waits, as in the attention kernel,
+    // took 16384 x 5120 x 5120 from 422 us to 467.)
 #pragma unroll 1
-    for (int t = worker; tries && t < total; t += workers) {
+    for (int t = worker; t < total; t += workers) {
       float sum[H];
 #pragma unroll
       for (int i = 0; i < H; ++i) sum[i] = 0.f;
       // (unrolled, or with a way out in its middle, the loop copies the sums in every turn)
 #pragma unroll 1
-      for (int g = g0; g < g1; ++g) {
+      for (int g = tries ? g0 : g1; g < g1; ++g) {
         tc::barrier_wait_warp(&scales_full[slot], slot_phase, tries);
         const float* sb = scales_b[slot];
         const float of_lane = scales_a[slot][quarter * 32 + lane];
@@ -224,7 +234,7 @@ matmul_q8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
           } else {
             tc::fence_before();
             __syncwarp();
-            tc::barrier_arrive_if_zero(&sum_empty[buffer], lane);
+            tc::barrier_arrive_if_zero(&sum_empty[buffer], tries ? lane : 1);
           }
           const uint32_t(&now)[PIECE] = r[c / PIECE % 2];
 #pragma unroll
@@ -241,11 +251,12 @@ matmul_q8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
           }
         }
         __syncwarp();
-        tc::barrier_arrive_if_zero(&scales_empty[slot], lane);
+        tc::barrier_arrive_if_zero(&scales_empty[slot], tries ? lane : 1);
         if (++slot == kRing) slot = 0, slot_phase ^= 1;
         if (++buffer == B) buffer = 0, phase ^= 1;
       }
       if (!tries) {  // a result that nobody can take for one
+        gave_up = 1;
 #pragma unroll
         for (int i = 0; i < H; ++i) sum[i] = __int_as_float(0x7fffffff);
       }
@@ -326,6 +337,11 @@ matmul_q8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     // the blocks of a cluster hold parts of one tile: each adds up its share of the columns, in the
     // blocks' order
     cg::cluster_group cluster = cg::this_cluster();
+    __syncthreads();
+    if (tc::marked(&gave_up)) {  // copies that were under way until now may lie over the parts
+      for (int i = threadIdx.x; i < BN * kTileA; i += kThreads)
+        reinterpret_cast<float*>(tiles)[i] = __int_as_float(0x7fffffff);
+    }
     cluster.sync();
     int ta, tb;
     place(worker, ta, tb);

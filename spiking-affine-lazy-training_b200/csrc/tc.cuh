@@ -38,7 +38,8 @@ __device__ __forceinline__ bool barrier_try(uint64_t* b, uint32_t parity) {
 }
 // Waits for the barrier's phase of that parity to end.  Gives up after `tries` looks, which only a
 // fault elsewhere can bring about (a look that finds nothing takes some 4 us: about a second in
-// all), and leaves tries = 0 behind: later waits then look once.
+// all), and leaves tries = 0 behind: later waits then look once.  Others' waits may still end well, so
+// who gave up arrives at no barrier any more, and what waits for it gives up in turn ...
 constexpr uint32_t kTries = 1u << 18;
 __device__ __forceinline__ void barrier_wait(uint64_t* b, uint32_t parity, uint32_t& tries) {
   for (uint32_t i = tries; !barrier_try(b, parity); --i)
@@ -54,6 +55,28 @@ __device__ __forceinline__ void barrier_wait_warp(uint64_t* b, uint32_t parity, 
       tries = 0;
       break;
     }
+}
+// ... or leaves a mark that the block's threads share, at which each looks before it writes results.
+__device__ __forceinline__ void barrier_wait(uint64_t* b, uint32_t parity, uint32_t& tries,
+                                             uint32_t* gave_up) {
+  for (uint32_t i = tries; !barrier_try(b, parity); --i)
+    if (i == 0) {
+      tries = 0;
+      *reinterpret_cast<volatile uint32_t*>(gave_up) = 1;
+      break;
+    }
+}
+__device__ __forceinline__ void barrier_wait_warp(uint64_t* b, uint32_t parity, uint32_t& tries,
+                                                  uint32_t* gave_up) {
+  for (uint32_t i = tries; !__all_sync(0xffffffffu, barrier_try(b, parity)); --i)
+    if (i == 0) {
+      tries = 0;
+      *reinterpret_cast<volatile uint32_t*>(gave_up) = 1;
+      break;
+    }
+}
+__device__ __forceinline__ bool marked(const uint32_t* gave_up) {
+  return *reinterpret_cast<const volatile uint32_t*>(gave_up) != 0;
 }
 // An arrival of the lanes that hold 0, without a branch.
 __device__ __forceinline__ void barrier_arrive_if_zero(uint64_t* b, int lane) {
