@@ -18,6 +18,8 @@ static thread_local int64_t g_launches = 0;
 
 static salt_status fail(salt_status s, const std::string& msg) {
   g_err = msg;
+  // the runtime keeps an error until it is asked for: the next launch would report this one as its own
+  if (s == SALT_CUDA_ERROR) cudaGetLastError();
   return s;
 }
 

@@ -316,8 +316,10 @@ inline EncodeTiled encoder() {
     cudaDriverEntryPointQueryResult found;
     if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault,
                                          &found) != cudaSuccess ||
-        found != cudaDriverEntryPointSuccess)
+        found != cudaDriverEntryPointSuccess) {
+      cudaGetLastError();
       p = nullptr;
+    }
     return reinterpret_cast<EncodeTiled>(p);
   }();
   return f;
