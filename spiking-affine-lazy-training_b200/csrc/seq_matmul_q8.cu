@@ -15,7 +15,8 @@ constexpr int kSums = 256;             // threads that scale and add up: 8 warps
 constexpr int kThreads = kSums + 128;  // behind them a warp for the copies, one for the products and two
                                        // for the scales
 constexpr int kMostSplit = 8;
-constexpr int kRing = 8;  // groups whose scales are in flight
+constexpr int kRing = 8;    // groups whose scales are in flight
+constexpr int kBehind = 4;  // of them, those whose scales nobody has looked at
 
 // Stages of both operands' tiles in flight.
 constexpr int stages(int bn, bool swap) {
@@ -39,6 +40,20 @@ struct Product {
   bool bias_f32, vec;
 };
 
+// In its upper two bits, whether any of four scales lies outside 2^-47 to 2^17, between which two multiply
+// to a normal number.  (Powers that let one instruction look at a scale, on the scale's way from memory.)
+__device__ __forceinline__ uint32_t unusual_bits(float4 v) {
+  constexpr uint32_t low = (127u - 47u) << 24;
+  return ((__float_as_uint(v.x) << 1) - low) | ((__float_as_uint(v.y) << 1) - low) |
+         ((__float_as_uint(v.z) << 1) - low) | ((__float_as_uint(v.w) << 1) - low);
+}
+// a b v where a b may overflow or be subnormal though the whole does not: the larger factor is the
+// last one of a large product, the first one of a small.
+__device__ __forceinline__ float scaled(float v, float a, float b) {
+  const bool a_first = (fabsf(a) < fabsf(b)) == (fabsf(a * b) >= 1.f);
+  return v * (a_first ? a : b) * (a_first ? b : a);
+}
+
 // out = sum over groups of scale_a scale_b (the group's product of e4m3 values).
 //
 // The tensor cores add up one group (128 x BN x 128, in 32 bits) into one of two to eight buffers of
@@ -52,11 +67,17 @@ struct Product {
 // What bounds it: a scale for every 128 of the depth makes the sums a multiplication and an addition of
 // every value for each group.  At BN = 256 a group's products take 512 cycles and its sums 360 of every
 // scheduler's, next to some 250 of waiting at barriers and taking the values out of tensor memory:
-// 16384 x 5120 x 5120 takes 426 us in bfloat16, 2.02 PFLOP/s (350 us without sums and outputs, 268 us
+// 16384 x 5120 x 5120 takes 436 us in bfloat16, 1.97 PFLOP/s (350 us without sums and outputs, 268 us
 // the library's product with one scale a tensor).  Columns with a scale each take two multiplications a
-// value: 2048 x 4096 x 8192 with both operands' scales by rows, to float32, 141 us, 0.97 PFLOP/s.  Few
+// value: 2048 x 4096 x 8192 with both operands' scales by rows, to float32, 147 us, 0.94 PFLOP/s.  Few
 // rows are bound by what a block waits for: 64 rows of 8192 x 8192 take 26 us, 2.6 TB/s; 16 rows of 2048
 // x 4096 9 us, most of it the start, the first copies and the joining.
+// The definition has (x scale) (weight scale), and a product of both scales may overflow or be subnormal
+// where that does not: from the first group of a tile with such scales on, the values meet the scales one
+// after the other.  That loop, with a look at the scales in every group, costs 1 to 3 % (432 -> 436 us
+// above, 143 -> 147 us with scales by rows); as a branch beside every 16 values it cost a third.  With scales
+// by rows the warps that copy them look, since the sums' warps have no instruction to spare: three
+// instructions a scale in there took 162 us.
 // Measured and left: two blocks on a tile of 256 x 256 (440 us then, as much as one), sixteen warps of
 // sums (455), packed arithmetic for the sums (447), two sets of warps on every other group of narrow
 // tiles (24.4 us for 64 rows).
@@ -76,6 +97,7 @@ matmul_q8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
   constexpr int kScalesB = SWAP ? BN : 4;  // of each column, or of each block of columns
   __shared__ __align__(16) float scales_a[kRing][kTileA], scales_b[kRing][kScalesB];
   __shared__ uint64_t scales_full[kRing], scales_empty[kRing];
+  __shared__ uint2 unusual[kRing];  // SWAP: whether any of a group's scales is, of the lanes, of the columns
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) {
@@ -174,8 +196,19 @@ matmul_q8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     // every load takes as many lines as lanes, and here nobody waits for them
     const bool lanes = warp == kScales;
     const int n = lanes ? kTileA : kScalesB;
-    int slot = 0;
+    int slot = 0, ready = 0, behind = 0;
     uint32_t phase = 0;
+    const auto pass_on = [&] {  // the oldest group whose scales are there
+      __syncwarp();
+      const float4* at = reinterpret_cast<const float4*>(lanes ? scales_a[ready] : scales_b[ready]);
+      uint32_t odd = lane * 4 < n ? unusual_bits(at[lane]) : 0;
+      if (kScalesB > 128 && !lanes) odd |= unusual_bits(at[32 + lane]);
+      const bool any = __any_sync(0xffffffffu, odd >> 30);
+      if (lane == 0) (lanes ? unusual[ready].x : unusual[ready].y) = any;
+      tc::barrier_arrive_if_zero(&scales_full[ready], 0);
+      if (++ready == kRing) ready = 0;
+      --behind;
+    };
     for (int t = worker; tries && t < total; t += workers) {
       int ta, tb;
       place(t, ta, tb);
@@ -196,11 +229,20 @@ matmul_q8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
 #pragma unroll
         for (int i = 0; i < (int)(sizeof(from) / sizeof(from[0])); ++i)
           if (i * 32 + lane < n) tc::copy4(to + i * 32, from[i] + g);
-        tc::copies_arrive(&scales_full[slot]);
+        if constexpr (SWAP) {
+          tc::copies_group();
+          if (++behind > kBehind) {
+            tc::copies_wait<kBehind>();
+            pass_on();
+          }
+        } else {
+          tc::copies_arrive(&scales_full[slot]);
+        }
         if (++slot == kRing) slot = 0, phase ^= 1;
       }
     }
     tc::copies_done();
+    while (SWAP && tries && behind > 0) pass_on();
   } else {
     tc::registers_up<216>();
     const int quarter = warp & 3, half = warp >> 2;
@@ -215,9 +257,10 @@ matmul_q8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       float sum[H];
 #pragma unroll
       for (int i = 0; i < H; ++i) sum[i] = 0.f;
-      // (unrolled, or with a way out in its middle, the loop copies the sums in every turn)
+      int g = tries ? g0 : g1;
+      // (unrolled, the loop copies the sums in every turn)
 #pragma unroll 1
-      for (int g = tries ? g0 : g1; g < g1; ++g) {
+      for (; g < g1; ++g) {
         tc::barrier_wait_warp(&scales_full[slot], slot_phase, tries);
         const float* sb = scales_b[slot];
         const float of_lane = scales_a[slot][quarter * 32 + lane];
@@ -226,6 +269,14 @@ matmul_q8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         tc::fence_after();
         uint32_t r[2][PIECE];
         tc::tmem_load<PIECE>(r[0], mine + buffer * BN);
+        bool plain;
+        if constexpr (SWAP) {
+          const uint2 u = unusual[slot];
+          plain = !(u.x | u.y);
+        } else {  // a normal number
+          plain = __all_sync(0xffffffffu, (__float_as_uint(by) << 1) - 0x01000000u < 0xfd000000u);
+        }
+        if (!plain) break;
 #pragma unroll
         for (int c = 0; c < H; c += PIECE) {
           tc::loads_done();
@@ -249,6 +300,36 @@ matmul_q8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             sum[c + i + 2] = fmaf(__uint_as_float(now[i + 2]), v.z, sum[c + i + 2]);
             sum[c + i + 3] = fmaf(__uint_as_float(now[i + 3]), v.w, sum[c + i + 3]);
           }
+        }
+        __syncwarp();
+        tc::barrier_arrive_if_zero(&scales_empty[slot], tries ? lane : 1);
+        if (++slot == kRing) slot = 0, slot_phase ^= 1;
+        if (++buffer == B) buffer = 0, phase ^= 1;
+      }
+#pragma unroll 1
+      for (; g < g1; ++g) {  // near the ends of float32's range
+        tc::barrier_wait_warp(&scales_full[slot], slot_phase, tries);
+        const float* sb = scales_b[slot];
+        const float of_lane = scales_a[slot][quarter * 32 + lane];
+        tc::barrier_wait_warp(&sum_full[buffer], phase, tries);
+        tc::fence_after();
+        uint32_t r[2][PIECE];
+        tc::tmem_load<PIECE>(r[0], mine + buffer * BN);
+#pragma unroll
+        for (int c = 0; c < H; c += PIECE) {
+          tc::loads_done();
+          if (c + PIECE < H) {  // on its way while this piece is added
+            tc::tmem_load<PIECE>(r[(c / PIECE + 1) % 2], mine + buffer * BN + c + PIECE);
+          } else {
+            tc::fence_before();
+            __syncwarp();
+            tc::barrier_arrive_if_zero(&sum_empty[buffer], tries ? lane : 1);
+          }
+          const uint32_t(&now)[PIECE] = r[c / PIECE % 2];
+#pragma unroll
+          for (int i = 0; i < PIECE; ++i)
+            sum[c + i] += scaled(__uint_as_float(now[i]), of_lane,
+                                 sb[SWAP ? half * H + c + i : half * H / kGroup]);
         }
         __syncwarp();
         tc::barrier_arrive_if_zero(&scales_empty[slot], tries ? lane : 1);

@@ -155,6 +155,12 @@ __device__ __forceinline__ void copies_arrive(uint64_t* barrier) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(shared_at(barrier))
                : "memory");
 }
+// The same in groups: all but the thread's last N groups are there.
+__device__ __forceinline__ void copies_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // ---------------------------------------------------------------- tensor memory
