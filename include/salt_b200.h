@@ -559,11 +559,13 @@ salt_status salt_selective_scan_backward(const salt_selective_scan_backward_args
  * (batch, len, kv_heads, dim_k or dim_v), out (batch, len, heads, dim_v), all with contiguous
  * (heads, dim); head h reads key head h / (heads / kv_heads).  dim_k and dim_v are 1 to 128.
  * log_decay (heads) is float32 and at most 0: greater values count as 0, values under -200 as -200
- * (a decay that float32 rounds to 0).  Rows past n_real have to be memory, whatever it holds.  A v that
- * is not finite makes its column of out and of the state NaN from its token on, and reaches no token
- * before it.  Arrays that are not bfloat16 on boundaries of 16 bytes (address, strides, dim) are brought
- * into parts of bfloat16 first, in the workspace: up to 1.5 times their size.  initial_state and
- * final_state (batch, heads, dim_k, dim_v) float32 may be NULL, or be the same array. */
+ * (a decay that float32 rounds to 0).  Rows past n_real have to be memory, whatever it holds.  A NaN
+ * or infinity in any input makes those outputs not finite that the recurrence makes so, and no others
+ * (no token before it, no head that does not read it): a v its column of out and of the state from its
+ * token on.  An infinity, or what overflows float32 on the way, may come out as NaN.  Arrays that are not
+ * bfloat16 on boundaries of 16 bytes (address, strides, dim) are brought into parts of bfloat16 first, in
+ * the workspace: up to 1.5 times their size.  initial_state and final_state (batch, heads, dim_k, dim_v)
+ * float32 may be NULL, or be the same array. */
 typedef struct {
   int32_t batch, len, heads, kv_heads, dim_k, dim_v;
   int32_t type;

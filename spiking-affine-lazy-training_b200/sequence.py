@@ -599,7 +599,9 @@ def linear_attention(q, k, v, log_decay, *, scale: float = 1.0, n_real=None, ini
     dim_v), head h reading key head ``h // (heads / kv heads)``; dim_k and dim_v 1 to 128, (heads,
     dim) contiguous, any token and batch strides.  log_decay (heads) float32, at most 0.  n_real
     (batch, int32) ends each row early.  initial_state and final_state: (batch, heads, dim_k,
-    dim_v) float32, may be one array."""
+    dim_v) float32, may be one array.  States and sums hold 32 bits whatever q's type.  A NaN or
+    infinity reaches the outputs that the recurrence lets it reach, and no others; an infinity may
+    come out as NaN."""
     here = _here()
     t, shape, kv, dim_v = _heads(q, k, v, 4)
     batch, n, heads, dim_k = shape
