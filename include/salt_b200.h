@@ -562,10 +562,15 @@ salt_status salt_selective_scan_backward(const salt_selective_scan_backward_args
  * (a decay that float32 rounds to 0).  Rows past n_real have to be memory, whatever it holds.  A NaN
  * or infinity in any input makes those outputs not finite that the recurrence makes so, and no others
  * (no token before it, no head that does not read it): a v its column of out and of the state from its
- * token on.  An infinity, or what overflows float32 on the way, may come out as NaN.  Arrays that are not
- * bfloat16 on boundaries of 16 bytes (address, strides, dim) are brought into parts of bfloat16 first, in
- * the workspace: up to 1.5 times their size.  initial_state and final_state (batch, heads, dim_k, dim_v)
- * float32 may be NULL, or be the same array. */
+ * token on.  An infinity, or what overflows float32 on the way, may come out as NaN.  initial_state
+ * and final_state (batch, heads, dim_k, dim_v) float32 may be NULL, or be the same array.
+ * The workspace, of which the query gives the size, holds
+ *   - a copy in parts of bfloat16 of each array (in backward of dout, too) that is not bfloat16 on
+ *     boundaries of 16 bytes (address, strides, dim): 2 (bfloat16), 4 (float16) or 6 (float32) bytes
+ *     for each of batch * len * heads * dim values, with dim rounded up to 8 and whole even where a
+ *     stride is 0;
+ *   - where batch * heads is too small to fill the GPU, up to 64 states for each;
+ *   - in backward with shared key heads, 4 * batch * len * heads * max(dim_k, dim_v) bytes. */
 typedef struct {
   int32_t batch, len, heads, kv_heads, dim_k, dim_v;
   int32_t type;
