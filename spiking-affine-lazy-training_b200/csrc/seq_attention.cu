@@ -149,15 +149,18 @@ __global__ void __launch_bounds__(256) planes_kernel(const AllToPlanes all, int 
 // What bounds it: the threads' work on operands.  8 rows of 2048 x 16 heads of 128 in bfloat16 take 141
 // us, 2.0 TB/s, 3.3 times their bytes' time: 256 blocks are two rounds of 16 chunks of some 8000 cycles,
 // of which the tensor cores work 3500 (an instruction of 128 x 64 x 16 takes 48 cycles, 30 with an
-// operand in tensor memory).  One row of 32768 takes 347 us: 9 segments, 105 of it the states' pass.
-// float16 heads of 128 and float32 have chunks of 64 tokens, since shared memory holds no more of their
-// parts: the long row in float16 takes 896 us, in float32 1290 us.
-// A call's kernels set themselves up while the one in front ends (tc::follow): a backward pass of 14
-// small launches (3 x 1021 x 12 heads of 64 x 100, 4 key heads, float16) went from 181 us to 161.
-// Measured and left: eight warps (269 us), all products' warps in step with the others (189 us; this
-// was 133), roles for the warps, eight for triangle and out, four for the state and four for the values
-// (180 us: four warps wait too long for their own instructions), the direction as a template
-// parameter (heads of 100 x 77: 117 us to 111; heads of 128: backward 360 us to 364).
+// operand in tensor memory), and an instruction issues in every other cycle.  One row of 32768 takes 346
+// us: 9 segments, 98 of it the states' pass.  float16 heads of 128 and float32 have chunks of 64 tokens,
+// since shared memory holds no more of their parts: the long row in float16 takes 880 us, in float32 1265.
+// 17 warps leave 96 registers to a thread, and most instances keep some values in local memory: 4 and 24
+// bytes for bfloat16 heads up to 64 and over, 28 for float16 heads over 64, 56 and 104 for float32.
+// A call's kernels set themselves up while the one in front ends (tc::follow): a backward pass of 10
+// small launches (3 x 1021 x 12 heads of 64 x 100, 4 key heads, float16; 166 us) gained 20 us.
+// Measured and left: eight warps (269 us when sixteen took 189), all products' warps in step with the
+// others (189 us when this was 133), roles for the warps, eight for triangle and out, four for the state
+// and four for the values (180 us when this was 139: four warps wait too long for their own
+// instructions), the direction as a template parameter (5 % for heads of 100 x 77, 1 % slower for heads
+// of 128 backward).
 template <int P, typename O, int PANELS, bool STATE>
 __global__ void __launch_bounds__(kThreads, 1)
 attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,

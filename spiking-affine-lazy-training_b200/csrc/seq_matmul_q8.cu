@@ -70,7 +70,7 @@ __device__ __forceinline__ float scaled(float v, float a, float b) {
 // 16384 x 5120 x 5120 takes 436 us in bfloat16, 1.97 PFLOP/s (350 us without sums and outputs, 268 us
 // the library's product with one scale a tensor).  Columns with a scale each take two multiplications a
 // value: 2048 x 4096 x 8192 with both operands' scales by rows, to float32, 147 us, 0.94 PFLOP/s.  Few
-// rows are bound by what a block waits for: 64 rows of 8192 x 8192 take 26 us, 2.6 TB/s; 16 rows of 2048
+// rows are bound by what a block waits for: 64 rows of 8192 x 8192 take 28 us, 2.4 TB/s; 16 rows of 2048
 // x 4096 9 us, most of it the start, the first copies and the joining.
 // The definition has (x scale) (weight scale), and a product of both scales may overflow or be subnormal
 // where that does not: from the first group of a tile with such scales on, the values meet the scales one
